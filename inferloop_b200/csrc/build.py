@@ -48,6 +48,8 @@ MODULES: Dict[str, List[str]] = {
     "recurrent": [],
     "delta": [],
     "mlstm": [],
+    "kv4": [],
+    "attention_kv4": [],
 }
 
 _LOCK = threading.Lock()

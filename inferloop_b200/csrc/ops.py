@@ -1634,6 +1634,84 @@ def tc_row_blocks(ctas_one: int, ctas_two: int, sms: int, behind_cache: bool) ->
     return 2 if ctas_two >= sms else 1
 
 
+# --------------------------------------------------------------------------- 4-bit key/value cache
+KV4_UNIT = 16              # tokens of a unit of the 4-bit cache: page sizes are multiples of it
+KV4_GROUP = 32             # elements of a row that share a scale: head sizes are multiples of it
+KV4_MAX_HEAD = 512
+
+
+def kv4_cache_shape(pages: int, nkv: int, page_size: int, d: int) -> tuple:
+    """Shape of the uint8 tensor that holds a layer's keys and values of head size `d` in 4 bits: 4.5 bits an element with
+    the scales (format: csrc/kv4.cuh)."""
+    if page_size <= 0 or page_size % KV4_UNIT:
+        raise KernelError(f"4-bit cache: page size {page_size} must be a multiple of {KV4_UNIT}")
+    if d <= 0 or d % KV4_GROUP or d > KV4_MAX_HEAD:
+        raise KernelError(f"4-bit cache: head size {d} must be a multiple of {KV4_GROUP} up to {KV4_MAX_HEAD}")
+    return (int(pages), int(nkv), page_size // KV4_UNIT, 18 * d)
+
+
+def _kv4_need(what: str, cache: torch.Tensor, block_table: torch.Tensor, nkv: int, d: int) -> tuple:
+    """(pages, page size) of a 4-bit cache that holds `nkv` heads of `d`."""
+    _need(cache, what + " cache", torch.uint8); _need(block_table, what + " block table", torch.int32)
+    if cache.dim() != 4 or cache.shape[2] == 0 or tuple(cache.shape) != kv4_cache_shape(cache.shape[0], nkv, cache.shape[2] * KV4_UNIT, d):
+        raise KernelError(f"{what}: cache shape {tuple(cache.shape)} is not [pages, {nkv}, page size / {KV4_UNIT}, {18 * d}]")
+    if block_table.dim() != 2:
+        raise KernelError(f"{what}: the block table must be [sequences, blocks]")
+    return cache.shape[0], cache.shape[2] * KV4_UNIT
+
+
+def kv4_write(k: torch.Tensor, v: torch.Tensor, step, block_table: torch.Tensor, cache: torch.Tensor) -> None:
+    """The step's keys and values [T, nkv, d] (tokens and heads of any stride: views of a projection's rows, say) into the
+    4-bit cache, each at its token's position; a token whose page is not held is left out.  32 neighbouring elements share the scale
+    s = bfloat16(max |x| / 7) and are kept as x / s rounded to -7 .. 7, halves away from zero.  A group with an infinity or NaN
+    in it reads back as NaN."""
+    _need(k, "kv4_write keys", contiguous=False); _need(v, "kv4_write values", k.dtype, contiguous=False)
+    if k.dim() != 3 or v.shape != k.shape or (k.numel() and (k.stride(2) != 1 or v.stride(2) != 1)):
+        raise KernelError("kv4_write: keys and values must be [tokens, heads, head size] with a head's elements side by side")
+    T, nkv, d = k.shape
+    num_pages, page_size = _kv4_need("kv4_write", cache, block_table, nkv, d)
+    _need(step.positions, "kv4_write positions", torch.int32); _need(step.seq_of_token, "kv4_write sequence indices", torch.int32)
+    if step.positions.numel() != T or step.seq_of_token.numel() != T:
+        raise KernelError(f"kv4_write: {T} rows for a step of {step.positions.numel()} tokens")
+    ll = ctypes.c_longlong
+    _call("kv4", "ilb_kv4_write", _ptr(k), ll(k.stride(0)), ll(k.stride(1)), _ptr(v), ll(v.stride(0)), ll(v.stride(1)), _i(_code(k)),
+          _ptr(step.positions), _ptr(step.seq_of_token), _ptr(block_table), _i(block_table.shape[1]), _i(page_size), _i(num_pages), _ptr(cache),
+          _i(T), _i(nkv), _i(d), _stream(cache))
+
+
+def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, out_table: torch.Tensor, k_out: torch.Tensor,
+             v_out: torch.Tensor) -> None:
+    """Pages of the 4-bit cache read back into pages [out pages, nkv, page_size, d] of k_out's type: page b of sequence s, if it
+    holds any of the sequence's lengths[s] tokens, goes to page out_table[s, b] (-1: nowhere).  Rows from the length on, and those
+    of a page that is not held, are zeros; other pages of the output are left alone."""
+    _need(k_out, "kv4_read keys"); _need(v_out, "kv4_read values", k_out.dtype)
+    if k_out.dim() != 4 or v_out.shape != k_out.shape:
+        raise KernelError("kv4_read: outputs must be [pages, heads, page size, head size]")
+    out_pages, nkv, ps, d = k_out.shape
+    num_pages, page_size = _kv4_need("kv4_read", cache, block_table, nkv, d)
+    _need(out_table, "kv4_read output table", torch.int32); _need(lengths, "kv4_read lengths", torch.int32)
+    if ps != page_size or out_table.shape != block_table.shape or lengths.numel() != block_table.shape[0]:
+        raise KernelError("kv4_read: output pages, output table or lengths do not match the cache and its block table")
+    _call("kv4", "ilb_kv4_read", _ptr(cache), _ptr(block_table), _ptr(out_table), _i(block_table.shape[1]), _ptr(lengths), _i(block_table.shape[0]),
+          _i(page_size), _i(num_pages), _i(out_pages), _ptr(k_out), _ptr(v_out), _i(_code(k_out)), _i(nkv), _i(d), _stream(cache))
+
+
+def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step, block_table: torch.Tensor, window: int, scale: float,
+                  nq: int, nkv: int, d: int, sink: Optional[torch.Tensor] = None) -> None:
+    """Causal attention of the step's tokens over the 4-bit cache; q and out are [T, nq * d] of one type.  `window` and `sink`
+    as in `attention`; a token that sees no key (its pages are not held) gets zeros."""
+    _need(q, "kv4_attention q"); _need(out, "kv4_attention out", q.dtype); _need(sink, "kv4_attention sink", torch.float32)
+    num_pages, page_size = _kv4_need("kv4_attention", cache, block_table, nkv, d)
+    T = q.shape[0]
+    if nq <= 0 or nq % nkv or tuple(q.shape) != (T, nq * d) or out.shape != q.shape or step.positions.numel() != T or step.cu_q.numel() != block_table.shape[0] + 1:
+        raise KernelError("kv4_attention: queries, output, step and block table do not agree")
+    if sink is not None and sink.numel() != nq:
+        raise KernelError("kv4_attention: one sink logit per query head")
+    _call("attention_kv4", "ilb_kv4_attention_simple", _ptr(q), _ptr(out), _i(_code(q)), _ptr(cache), _ptr(step.positions), _ptr(step.seq_of_token),
+          _ptr(block_table), _i(block_table.shape[1]), _i(page_size), _i(num_pages), _i(window or 0), _f(scale), _i(T), _i(nq), _i(nkv), _i(d),
+          _i(q.shape[1]), _i(out.shape[1]), _ptr(sink), _stream(q))
+
+
 DECODE_FUSED_ENABLED = True     # tests switch it off to run q/k norm + rotation + cache write as a launch of its own
 DECODE_CLUSTER_ENABLED = True   # tests switch it off to reach the ticketed split-KV decode kernel
 FLASH_ENABLED = True       # tests switch it off to exercise the exact kernel in bfloat16
