@@ -3,26 +3,572 @@
 // over the keys j that a token sees: its own position and those before it, in its window or aligned chunk, whose page is held.
 // A token that sees no key gets zeros.
 //
-// One block a (token, query head); a warp takes 32 keys at a time, a lane a key for the scores and 32 elements apart for the values.
-// Scores, the running maximum, exponentials and sums are 32-bit.
+// Few rows against many keys (`rows_kernel`).  A row is a (token, query head of the group); 8 NB rows of a (sequence, kv head) are a block
+// of the launch, whose keys are shared out over `splits` CTAs and there over warps, a unit of 16 keys at a time.  A unit is one piece of
+// 18 D bytes of the cache: a warp keeps kStages of them on their way to its own ring in shared memory by bulk copies.
+//   scores   S^T = K Q^T on m16n8k16, the 16 keys as rows, so that groups of up to 8 query heads fill the 8 columns.  A code c + 8 in the
+//            last bits of a bfloat16's mantissa is the number 128 + c + 8, exactly: one AND-OR a pair.  The sums of a group of 32 elements
+//            start at -136 times the sum of the group's q, which takes the 136 out again, and are then scaled by the group's scale in
+//            32 bits (with 32-bit queries, which go in as three bfloat16 pieces, 136 is subtracted from the operands instead:
+//            the sum's cancellation would cost 7 bits).
+//   softmax  32-bit, base 2.  The reference point of a row's exponentials is not raised before a score exceeds it by 4 (in powers of
+//            two), a vote of the warp: the sums stay far from overflow and the maximum's exchange between lanes is rare.
+//   values   O^T += V^T P^T in fp16: the codes of two neighbouring tokens lie in one word each, so AND-OR (1024 + c + 8) and a
+//            subtraction of 1032 make the operand's column pairs; the scale goes into p, which is rounded once, as p times scale, to
+//            fp16's 11 bits (bfloat16's 8 cost a third more error in the result than its own rounding has).  For its range
+//            the reference point takes in the exponent of the largest scale met: p times scale stays below 2^15 and is normal down to 2^-20
+//            of the largest.  (32-bit queries: p times scale in three bfloat16 pieces.)
+//            The accumulator of S^T is turned into the second operand by movmatrix.
+//   merge    a CTA's warps through shared memory; several CTAs' records through a scratch buffer, by the CTA that takes the last ticket, in
+//            the order of the CTAs (the result does not depend on who is last).
 #include <math.h>
+#include <cuda_fp16.h>
+#include <type_traits>
 #include "kv4.cuh"
+#include "sm100.cuh"
 
 using namespace ilb;
 
 namespace {
 
-constexpr int kWarps = 4, kMaxHead = 512;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ------------------------------------------------------------------ few rows, many keys
+constexpr int kWarps = 4, kStages = 4, kThreads = kWarps * 32;
+constexpr int kMinUnits = 2;                // units a warp should have before another CTA joins
+
+struct Params {
+  const void* q; void* out; const uint8_t* cache; const int* positions; const int* cu_q; const int* block_table; const float* sink;
+  float* scratch; int* tickets; int* error_flag;
+  int max_blocks, page_size, num_pages, window, nq, nkv, q_stride, out_stride, row_blocks, max_tokens, splits;
+  float scale_log2;
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t turned(uint32_t x) {            // an 8 x 8 matrix of 16-bit elements, transposed across the warp
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// 1032 + c of two codes as fp16 numbers less 1032
+__device__ __forceinline__ uint32_t half_pair(uint32_t w, int nibble) {
+  const uint32_t r = ((w >> (4 * nibble)) & 0x000f000fu) | 0x64006400u, c1032 = 0x64086408u;
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&r), *reinterpret_cast<const __half2*>(&c1032));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// c += a b of fp16 numbers
+__device__ __forceinline__ void mma_half(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 136 + c of two codes as bfloat16 numbers, and c
+__device__ __forceinline__ uint32_t raised(uint32_t w, int nibble) { return ((w >> (4 * nibble)) & 0x000f000fu) | 0x43004300u; }
+__device__ __forceinline__ uint32_t plain_pair(uint32_t r) {
+  const uint32_t c136 = 0x43084308u;
+  const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&r), *reinterpret_cast<const __nv_bfloat162*>(&c136));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+// d = a b + c
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+// N consecutive words of shared memory from an address that is a multiple of 4 N bytes (of 4 for odd N)
+template <int N>
+__device__ __forceinline__ void lds(uint32_t addr, uint32_t (&w)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "r"(addr + 4 * i));
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[i]), "=r"(w[i + 1]) : "r"(addr + 4 * i));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(addr + 4 * i));
+  }
+}
+// The bfloat16 scales of a token's groups, as 32-bit numbers
+template <int N>
+__device__ __forceinline__ void lds_scales(uint32_t addr, float (&s)[N]) {
+  if constexpr (N % 2 == 0) {
+    uint32_t w[N / 2];
+    lds(addr, w);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) { s[2 * i] = bf_lo(w[i]); s[2 * i + 1] = bf_hi(w[i]); }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      uint16_t h;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(addr + 2 * i));
+      s[i] = __uint_as_float((uint32_t)h << 16);
+    }
+  }
+}
+// x as the sum of PIECES bfloat16 numbers: element i of the three
+template <int PIECES>
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[PIECES]) {
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    w[i] = pack_bf16(a, b);
+    a -= bf_lo(w[i]);
+    b -= bf_hi(w[i]);
+  }
+}
+
+template <int D, int NB, int PIECES>
+struct Shape {
+  static constexpr int kGroups = D / 32, kUnitBytes = 18 * D, kRows = 8 * NB;
+  static constexpr int kRecRow = D + 4;                                   // of a record in shared memory: no bank is met twice
+  static constexpr int kRing = kWarps * kStages * kUnitBytes;
+  static constexpr int kRecords = kWarps * kRows * kRecRow * 4;
+  static constexpr int kBody = kRing > kRecords ? kRing : kRecords;       // (the records take the ring's place)
+  static constexpr int kQ = PIECES > 1 ? kGroups * 4 * PIECES * 32 * 4 : 0;      // 32-bit queries: their pieces in operand order
+  static constexpr int kStats = 3 * kWarps * kRows * 4 + 2 * kRows * 4;
+  static constexpr int kSmem = kBody + kQ + kStats + kWarps * kStages * 8 + 16;
+};
+
+template <typename T, int D, int NB, int PIECES>
+__global__ void __launch_bounds__(kThreads, NB == 1 && D <= 128 ? 4 : 2) rows_kernel(const Params p) {
+  using Sh = Shape<D, NB, PIECES>;
+  constexpr int NG = Sh::kGroups, U = Sh::kUnitBytes, kRows = Sh::kRows;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float* rec = reinterpret_cast<float*>(smem);
+  float* stat_m = reinterpret_cast<float*>(smem + Sh::kBody + Sh::kQ);    // [warp][row]
+  float* stat_l = stat_m + kWarps * kRows;
+  float* factor = stat_l + kWarps * kRows;                                // [warp][row]
+  float* row_m = factor + kWarps * kRows;                                 // [row], then the sums
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Sh::kBody + Sh::kQ + Sh::kStats);
+  int* flags = reinterpret_cast<int*>(bars + kWarps * kStages);
+  const uint32_t ring = smem_u32(smem) + warp * kStages * U, bar0 = smem_u32(bars + warp * kStages), q_smem = smem_u32(smem) + Sh::kBody;
+
+  pdl_launch_dependents();
+  if (lane == 0) {
+    for (int s = 0; s < kStages; ++s) mbar_init(bar0 + 8 * s, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
+  pdl_wait();
+
+  const int seq = blockIdx.z / p.row_blocks, rb = blockIdx.z % p.row_blocks, head = blockIdx.y, G = p.nq / p.nkv;
+  const int tok0 = p.cu_q[seq], q_len = p.cu_q[seq + 1] - tok0, rows = q_len * G;
+  if (q_len > p.max_tokens || rb * kRows >= rows) return;
+  const int row0 = rb * kRows, n_rows = min(kRows, rows - row0);
+  // keys that the block's tokens see at all, and those that every one of them sees
+  const int pos_a = p.positions[tok0 + row0 / G], pos_b = p.positions[tok0 + (row0 + n_rows - 1) / G];
+  const int lo_a = first_key(pos_a, p.window), lo_b = first_key(pos_b, p.window);
+  const int unit0 = lo_a / kKv4Unit, n_units = pos_b / kKv4Unit + 1 - unit0;
+  int on = (n_units + kWarps * kMinUnits - 1) / (kWarps * kMinUnits);
+  on = on < 1 ? 1 : on > p.splits ? p.splits : on;                        // CTAs that take part
+  if ((int)blockIdx.x >= on) return;
+  const int begin = (int)((long long)n_units * blockIdx.x / on), end = (int)((long long)n_units * (blockIdx.x + 1) / on);
+  const int mine = end - begin > warp ? (end - begin - warp + kWarps - 1) / kWarps : 0;      // units of this warp: begin + warp + i kWarps
+
+  // ---- the stream of units: lane l knows where the l-th of every 32 lies
+  const int upp = p.page_size / kKv4Unit;
+  const int* table = p.block_table + (size_t)seq * p.max_blocks;
+  long long where = -1;                                                   // unit in the cache, or -1: not held
+  auto look_up = [&](int i0) {
+    const int i = i0 + lane;
+    where = -1;
+    if (i < mine) {
+      const int u = unit0 + begin + warp + i * kWarps, blk = u / upp;
+      const int page = blk < p.max_blocks ? __ldg(table + blk) : -1;
+      if (page >= 0 && page < p.num_pages) where = ((long long)page * p.nkv + head) * upp + u % upp;
+    }
+  };
+  uint32_t held = 0;                                                      // bit i: the i-th unit of these 32 is held
+  auto ask = [&](int i) {                                                 // (unit i must be one of the 32 looked up)
+    const long long at = __shfl_sync(0xffffffffu, where, i & 31);
+    if (at >= 0 && lane == 0) {
+      mbar_expect_tx(bar0 + 8 * (i % kStages), U);
+      bulk_load(ring + (i % kStages) * U, p.cache + at * U, U, bar0 + 8 * (i % kStages));
+    }
+    held = (held & ~(1u << (i & 31))) | (at >= 0 ? 1u << (i & 31) : 0u);
+  };
+  if (mine > 0) look_up(0);
+#pragma unroll
+  for (int i = 0; i < kStages; ++i)
+    if (i < mine) ask(i);
+
+  // ---- queries as second operands, rows g of each block of 8; -136 times the sums of their groups
+  constexpr int kQRegs = PIECES == 1 ? NG * 4 : 1;
+  uint32_t qf[NB][kQRegs];
+  float init[NB][PIECES == 1 ? NG : 1][2];
+  float base[NB][2], m[NB][2], l[NB][2];
+  float scale_top = 0.f, scale_exp = 0.f;                                 // fp16: values' scales up to 16 times this need no new exponent; the exponent
+  int row_lo[NB][2], row_hi[NB][2];                                       // of columns 2 t, 2 t + 1
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int r = row0 + nb * 8 + g;
+    const bool there = r < rows;
+    const T* src = reinterpret_cast<const T*>(p.q) + (size_t)(tok0 + (there ? r / G : 0)) * p.q_stride + (size_t)(head * G + (there ? r % G : 0)) * D;
+#pragma unroll
+    for (int G32 = 0; G32 < NG; ++G32) {
+      float x[8];
+      if constexpr (sizeof(T) == 2) {
+        const uint4 w = there ? *reinterpret_cast<const uint4*>(src + G32 * 32 + 8 * t) : make_uint4(0u, 0u, 0u, 0u);
+        x[0] = bf_lo(w.x); x[1] = bf_hi(w.x); x[2] = bf_lo(w.y); x[3] = bf_hi(w.y); x[4] = bf_lo(w.z); x[5] = bf_hi(w.z); x[6] = bf_lo(w.w); x[7] = bf_hi(w.w);
+      } else {
+        const float4 a = there ? *reinterpret_cast<const float4*>(src + G32 * 32 + 8 * t) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 b = there ? *reinterpret_cast<const float4*>(src + G32 * 32 + 8 * t + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+      }
+      // the pairs that the key's words hold: elements i and i + 4 of the lane's eight
+      if constexpr (PIECES == 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qf[nb][G32 * 4 + i] = pack_bf16(x[i], x[i + 4]);
+        float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        init[nb][G32][0] = -136.f * __shfl_sync(0xffffffffu, sum, 8 * t);
+        init[nb][G32][1] = -136.f * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+      } else if (warp == 0) {
+        uint32_t w[4][PIECES];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split_pair<PIECES>(x[i], x[i + 4], w[i]);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(q_smem + ((G32 * PIECES + i) * 32 + lane) * 16), "r"(w[0][i]), "r"(w[1][i]),
+                       "r"(w[2][i]), "r"(w[3][i]) : "memory");
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int rc = row0 + nb * 8 + 2 * t + c;
+      const int pos = rc < rows ? p.positions[tok0 + rc / G] : -1;
+      row_hi[nb][c] = pos + 1;
+      row_lo[nb][c] = rc < rows ? first_key(pos, p.window) : 0;
+      base[nb][c] = 0.f; m[nb][c] = -INFINITY; l[nb][c] = 0.f;
+    }
+  }
+  if constexpr (PIECES > 1) __syncthreads();
+  float o[NG * 2][NB][4];
+#pragma unroll
+  for (int i = 0; i < NG * 2; ++i)
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][nb][e] = 0.f;
+
+  // ---- units
+  uint32_t phases = 0;                                                    // bit s: parity of stage s's next completion
+  bool ok = true;
+  int failed_at = 0;
+  for (int i = 0; i < mine; ++i) {
+    const int s = i % kStages;
+    const bool there = (held >> (i & 31)) & 1u;
+    if (there) {
+      if (!__all_sync(0xffffffffu, mbar_wait(bar0 + 8 * s, (phases >> s) & 1u))) { ok = false; failed_at = i; break; }
+      phases ^= 1u << s;
+      const uint32_t unit = ring + s * U;
+      const int key0 = (unit0 + begin + warp + i * kWarps) * kKv4Unit;
+      float sv[NB][4];
+      {
+        uint32_t ka[NG], kb[NG];                                          // words of tokens g and g + 8
+        lds(unit + g * (D / 2) + t * (D / 8), ka);
+        lds(unit + (g + 8) * (D / 2) + t * (D / 8), kb);
+        float sa[NG], sb[NG];
+        lds_scales(unit + 16 * D + g * (D / 16), sa);
+        lds_scales(unit + 16 * D + (g + 8) * (D / 16), sb);
+#pragma unroll
+        for (int G32 = 0; G32 < NG; ++G32) {
+          uint32_t a[2][4];
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            a[ks][0] = raised(ka[G32], 2 * ks); a[ks][1] = raised(kb[G32], 2 * ks);
+            a[ks][2] = raised(ka[G32], 2 * ks + 1); a[ks][3] = raised(kb[G32], 2 * ks + 1);
+            if constexpr (PIECES > 1) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) a[ks][e] = plain_pair(a[ks][e]);
+            }
+          }
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            float acc[4];
+            if constexpr (PIECES == 1) {
+              const float c[4] = {init[nb][G32][0], init[nb][G32][1], init[nb][G32][0], init[nb][G32][1]};
+              mma(acc, a[0], qf[nb][G32 * 4], qf[nb][G32 * 4 + 1], c);
+              mma(acc, a[1], qf[nb][G32 * 4 + 2], qf[nb][G32 * 4 + 3], acc);
+            } else {
+              acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
+#pragma unroll
+              for (int i3 = PIECES - 1; i3 >= 0; --i3) {                  // the smallest pieces first
+                uint32_t w[4];
+                lds(q_smem + ((G32 * PIECES + i3) * 32 + lane) * 16, w);
+                mma(acc, a[0], w[0], w[1], acc);
+                mma(acc, a[1], w[2], w[3], acc);
+              }
+            }
+            if (G32 == 0) {
+              sv[nb][0] = sa[0] * acc[0]; sv[nb][1] = sa[0] * acc[1]; sv[nb][2] = sb[0] * acc[2]; sv[nb][3] = sb[0] * acc[3];
+            } else {
+              sv[nb][0] = fmaf(sa[G32], acc[0], sv[nb][0]); sv[nb][1] = fmaf(sa[G32], acc[1], sv[nb][1]);
+              sv[nb][2] = fmaf(sb[G32], acc[2], sv[nb][2]); sv[nb][3] = fmaf(sb[G32], acc[3], sv[nb][3]);
+            }
+          }
+        }
+      }
+      const bool whole = key0 >= lo_b && key0 + kKv4Unit <= pos_a + 1;    // every row of the block sees all 16 keys
+      float va_s[NG], vb_s[NG];                                           // values' scales of tokens g and g + 8
+      lds_scales(unit + 17 * D + g * (D / 16), va_s);
+      lds_scales(unit + 17 * D + (g + 8) * (D / 16), vb_s);
+      bool raise = false;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sv[nb][e] *= p.scale_log2;
+      }
+      if (!whole) {
+        bool first = false, second = false;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + g + (e >> 1) * 8;
+            const bool seen = key >= row_lo[nb][e & 1] && key < row_hi[nb][e & 1];
+            if (!seen) sv[nb][e] = -INFINITY;
+            if (e < 2) first |= seen;
+            else second |= seen;
+          }
+        // (a lane knows two rows of each block; what none of a token's four lanes sees is not looked at)
+        const uint32_t quad = 0xfu << (lane & 28);
+        first = (__ballot_sync(0xffffffffu, first) & quad) != 0;
+        second = (__ballot_sync(0xffffffffu, second) & quad) != 0;
+#pragma unroll
+        for (int G32 = 0; G32 < NG; ++G32) { va_s[G32] = first ? va_s[G32] : 0.f; vb_s[G32] = second ? vb_s[G32] : 0.f; }
+      }
+      float most = 0.f;
+      if constexpr (PIECES == 1) {
+#pragma unroll
+        for (int G32 = 0; G32 < NG; ++G32) most = fmaxf(most, fmaxf(va_s[G32], vb_s[G32]));
+        raise = most > 16.f * scale_top;
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+        raise |= fmaxf(sv[nb][0], sv[nb][2]) > m[nb][0] + 4.f || fmaxf(sv[nb][1], sv[nb][3]) > m[nb][1] + 4.f;
+      if (__any_sync(0xffffffffu, raise)) {
+        if constexpr (PIECES == 1) {
+          most = warp_max(most);
+          if (most > scale_top) {
+            scale_top = most;
+            scale_exp = fmaxf((float)((int)(__float_as_uint(most) >> 23) - 127), -100.f) - 6.f;
+          }
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float mx = fmaxf(sv[nb][c], sv[nb][c + 2]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float m_new = fmaxf(m[nb][c], mx), b_new = m_new == -INFINITY ? 0.f : m_new + scale_exp;
+            const float corr = m[nb][c] == -INFINITY ? (l[nb][c] == 0.f ? 0.f : 1.f) : exp2f(base[nb][c] - b_new);
+            base[nb][c] = b_new;
+            m[nb][c] = m_new;
+            l[nb][c] *= corr;
+#pragma unroll
+            for (int d = 0; d < NG * 2; ++d) { o[d][nb][c] *= corr; o[d][nb][c + 2] *= corr; }
+          }
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sv[nb][e] = exp2f(sv[nb][e] - base[nb][e & 1]);
+        l[nb][0] += sv[nb][0] + sv[nb][2];
+        l[nb][1] += sv[nb][1] + sv[nb][3];
+      }
+      auto values = [&](auto masked) {
+        uint32_t va[NG], vb[NG];                                          // tokens 2 t, 2 t + 1 and 2 t + 8, 2 t + 9: half-words of the groups
+        lds(unit + 8 * D + lane * (D / 8), va);
+        lds(unit + 12 * D + lane * (D / 8), vb);
+#pragma unroll
+        for (int G32 = 0; G32 < NG; ++G32) {
+          // half-word i of an array of NG words: the even token's groups come first, then the odd one's
+          constexpr auto half_sel = [](int even, int odd) { return (uint32_t)((even & 1 ? 0x32 : 0x10) | (odd & 1 ? 0x7600 : 0x5400)); };
+          const uint32_t wa = __byte_perm(va[G32 / 2], va[(NG + G32) / 2], half_sel(G32, NG + G32));
+          const uint32_t wb = __byte_perm(vb[G32 / 2], vb[(NG + G32) / 2], half_sel(G32, NG + G32));
+          uint32_t a[2][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if constexpr (PIECES == 1) {
+              a[h][0] = half_pair(wa, 2 * h); a[h][1] = half_pair(wa, 2 * h + 1);
+              a[h][2] = half_pair(wb, 2 * h); a[h][3] = half_pair(wb, 2 * h + 1);
+            } else {
+              a[h][0] = plain_pair(raised(wa, 2 * h)); a[h][1] = plain_pair(raised(wa, 2 * h + 1));
+              a[h][2] = plain_pair(raised(wb, 2 * h)); a[h][3] = plain_pair(raised(wb, 2 * h + 1));
+            }
+          }
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            float w[4] = {sv[nb][0] * va_s[G32], sv[nb][1] * va_s[G32], sv[nb][2] * vb_s[G32], sv[nb][3] * vb_s[G32]};
+            if constexpr (decltype(masked)::value) {                      // what a row does not see adds nothing, whatever its scale is
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[e] = sv[nb][e] == 0.f ? 0.f : w[e];
+            }
+            if constexpr (PIECES == 1) {
+              const uint32_t x0 = turned(pack_half(w[0], w[1])), x1 = turned(pack_half(w[2], w[3]));
+              mma_half(o[2 * G32][nb], a[0], x0, x1);
+              mma_half(o[2 * G32 + 1][nb], a[1], x0, x1);
+            } else {
+              uint32_t b0[PIECES], b1[PIECES];
+              split_pair<PIECES>(w[0], w[1], b0);
+              split_pair<PIECES>(w[2], w[3], b1);
+#pragma unroll
+              for (int i3 = PIECES - 1; i3 >= 0; --i3) {
+                const uint32_t x0 = turned(b0[i3]), x1 = turned(b1[i3]);
+                mma_16816(o[2 * G32][nb], a[0], x0, x1);
+                mma_16816(o[2 * G32 + 1][nb], a[1], x0, x1);
+              }
+            }
+          }
+        }
+      };
+      if (whole) values(std::false_type{});
+      else values(std::true_type{});
+      __syncwarp();                                                       // every lane is done with the stage
+    }
+    if (((i + kStages) & 31) == 0) look_up(i + kStages);
+    if (i + kStages < mine) ask(i + kStages);
+  }
+  if (!ok) {                                                              // the copies still on their way land before the ring is written over
+    for (int i = failed_at + 1; i < mine && i < failed_at + kStages; ++i)
+      if ((held >> (i & 31)) & 1u) mbar_wait(bar0 + 8 * (i % kStages), (phases >> (i % kStages)) & 1u);
+    if (lane == 0 && p.error_flag) *p.error_flag = 1;
+  }
+
+  // ---- merge: warps of the CTA
+  __syncthreads();                                                        // the ring is free
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int r = nb * 8 + 2 * t + c;
+      float sum = l[nb][c];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+      if (g == 0) { stat_m[warp * kRows + r] = m[nb][c] == -INFINITY ? -INFINITY : base[nb][c]; stat_l[warp * kRows + r] = sum; }
+      float* dst = rec + (size_t)(warp * kRows + r) * Sh::kRecRow + 4 * g;
+#pragma unroll
+      for (int G32 = 0; G32 < NG; ++G32)
+        *reinterpret_cast<float4*>(dst + 32 * G32) = make_float4(o[2 * G32][nb][c], o[2 * G32][nb][c + 2], o[2 * G32 + 1][nb][c], o[2 * G32 + 1][nb][c + 2]);
+    }
+  __syncthreads();
+  auto write_row = [&](int r, int d4, float4 v, float total) {
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const int row = row0 + r;
+    T* dst = reinterpret_cast<T*>(p.out) + (size_t)(tok0 + row / G) * p.out_stride + (size_t)(head * G + row % G) * D + 4 * d4;
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+    else *reinterpret_cast<float4*>(dst) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+  };
+  auto sink_of = [&](int r) { return p.sink != nullptr ? p.sink[head * G + (row0 + r) % G] * kLog2e : -INFINITY; };
+  const bool alone = on == 1;
+  if (threadIdx.x < kRows) {
+    const int r = threadIdx.x;
+    const float sink = alone && r < n_rows ? sink_of(r) : -INFINITY;
+    float top = sink;
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stat_m[w * kRows + r]);
+    float total = sink == -INFINITY ? 0.f : exp2f(sink - top);
+    for (int w = 0; w < kWarps; ++w) {
+      const float mw = stat_m[w * kRows + r], f = mw == -INFINITY ? (stat_l[w * kRows + r] == 0.f ? 0.f : 1.f) : exp2f(mw - top);
+      factor[w * kRows + r] = f;
+      total = fmaf(stat_l[w * kRows + r], f, total);
+    }
+    row_m[r] = top;
+    row_m[kRows + r] = total;
+  }
+  __syncthreads();
+  const size_t place = ((size_t)blockIdx.z * p.nkv + head) * p.splits;    // records of this block of rows
+  constexpr int kQuads = D / 4;
+  for (int at = threadIdx.x; at < n_rows * kQuads; at += kThreads) {
+    const int r = at / kQuads, d4 = at % kQuads;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float4 x = *reinterpret_cast<const float4*>(rec + (size_t)(w * kRows + r) * Sh::kRecRow + 4 * d4);
+      const float f = factor[w * kRows + r];
+      v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
+    }
+    if (alone) write_row(r, d4, v, row_m[kRows + r]);
+    else __stcg(reinterpret_cast<float4*>(p.scratch + ((place + blockIdx.x) * kRows + r) * (D + 4) + 4 * d4), v);
+  }
+  if (alone) return;
+  // ---- merge: CTAs
+  if (threadIdx.x < n_rows)
+    __stcg(reinterpret_cast<float2*>(p.scratch + ((place + blockIdx.x) * kRows + threadIdx.x) * (D + 4) + D),
+           make_float2(row_m[threadIdx.x], row_m[kRows + threadIdx.x]));
+  __threadfence();
+  __syncthreads();
+  int* ticket = p.tickets + (size_t)blockIdx.z * p.nkv + head;
+  if (threadIdx.x == 0) {
+    const int n = atomicAdd(ticket, 1);
+    flags[0] = n == on - 1;
+    if (n == on - 1) *ticket = 0;                                         // (zero between launches)
+  }
+  __syncthreads();
+  if (!flags[0]) return;
+  __threadfence();
+  for (int at = threadIdx.x; at < n_rows * kQuads; at += kThreads) {
+    const int r = at / kQuads, d4 = at % kQuads;
+    const float* first = p.scratch + (place * kRows + r) * (D + 4);
+    const size_t step = (size_t)kRows * (D + 4);
+    const float sink = sink_of(r);
+    float top = sink, total = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < on; ++c) {                                        // in the order of the CTAs, whoever came last
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(first + c * step + D));
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(first + c * step + 4 * d4));
+      const float m_new = fmaxf(top, ml.x), b = m_new == -INFINITY ? 0.f : m_new;
+      const float f = exp2f(top - b), e = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2f(ml.x - b);
+      if (c == 0 && sink != -INFINITY) total = 1.f;                       // exp(sink), against itself
+      total = fmaf(total, f, ml.y * e);
+      v.x = fmaf(v.x, f, x.x * e); v.y = fmaf(v.y, f, x.y * e); v.z = fmaf(v.z, f, x.z * e); v.w = fmaf(v.w, f, x.w * e);
+      top = m_new;
+    }
+    write_row(r, d4, v, total);
+  }
+}
+
+template <typename T, int D, int NB, int PIECES>
+int launch_rows(const Params& p, dim3 grid, cudaStream_t stream) {
+  static OncePerDevice once;
+  auto kernel = rows_kernel<T, D, NB, PIECES>;
+  constexpr int smem = Shape<D, NB, PIECES>::kSmem;
+  const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+  if (e != cudaSuccess) return fail("kv4_attention: %s", cudaGetErrorString(e));
+  ilb::launch(kernel, grid, dim3(kThreads), smem, stream, p);
+  return check_launch("kv4_attention");
+}
+
+// ------------------------------------------------------------------ any head size
+// One block a (token, query head); a warp takes 32 keys at a time, a lane a key for the scores and every 32nd element of the values.
+constexpr int kSimpleWarps = 4, kMaxHead = 512;
 
 template <typename T>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kSimpleWarps * 32)
 kv4_attention_simple_kernel(const T* __restrict__ q, T* __restrict__ out, const uint8_t* __restrict__ cache, const int* __restrict__ positions,
                             const int* __restrict__ seq_of_token, const int* __restrict__ block_table, int max_blocks, int page_size, int num_pages,
                             int window, float scale, int nq, int nkv, int d, int q_stride, int out_stride, const float* __restrict__ sink) {
   pdl_launch_dependents();
   pdl_wait();
   __shared__ float qs[kMaxHead];
-  __shared__ float red_m[kWarps], red_l[kWarps], red_o[kWarps][kMaxHead];
+  __shared__ float red_m[kSimpleWarps], red_l[kSimpleWarps], red_o[kSimpleWarps][kMaxHead];
   const int t = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = h / (nq / nkv), per_row = d / kKv4Group;
   const int pos = positions[t], lo = first_key(pos, window);
@@ -39,7 +585,7 @@ kv4_attention_simple_kernel(const T* __restrict__ q, T* __restrict__ out, const 
 #pragma unroll
   for (int i = 0; i < kMaxHead / 32; ++i) o[i] = 0.f;
   float m = -INFINITY, l = 0.f;
-  for (int k0 = lo + warp * 32; k0 <= pos; k0 += kWarps * 32) {
+  for (int k0 = lo + warp * 32; k0 <= pos; k0 += kSimpleWarps * 32) {
     const int key = k0 + lane, j = key % kKv4Unit;
     const uint8_t* unit = key <= pos ? find(key) : nullptr;
     float s = -INFINITY;
@@ -79,22 +625,83 @@ kv4_attention_simple_kernel(const T* __restrict__ q, T* __restrict__ out, const 
   for (int i = 0; i < per_row; ++i) red_o[warp][lane + 32 * i] = o[i];
   __syncthreads();
   float top = sink != nullptr ? sink[h] : -INFINITY;
-  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, red_m[w]);
-  float total = sink != nullptr ? expf(sink[h] - top) : 0.f, f[kWarps];
+  for (int w = 0; w < kSimpleWarps; ++w) top = fmaxf(top, red_m[w]);
+  float total = sink != nullptr ? expf(sink[h] - top) : 0.f, f[kSimpleWarps];
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < kSimpleWarps; ++w) {
     f[w] = red_m[w] == -INFINITY ? 0.f : expf(red_m[w] - top);
     total = fmaf(red_l[w], f[w], total);
   }
   for (int c = threadIdx.x; c < d; c += blockDim.x) {
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) sum = fmaf(red_o[w][c], f[w], sum);
+    for (int w = 0; w < kSimpleWarps; ++w) sum = fmaf(red_o[w][c], f[w], sum);
     out[(size_t)t * out_stride + (size_t)h * d + c] = from_float<T>(total == 0.f ? 0.f : sum / total);
   }
 }
 
 }  // namespace
+
+// Rows that a block of the launch takes: 8 of a group of up to 8 heads' single token or of 32-bit queries, else 16.
+static int rows_per_block(int dtype, int rows) { return dtype == kF32 || rows <= 8 ? 8 : 16; }
+
+// Head sizes that the kernel of few rows takes.
+static bool rows_head(int d) { return d == 32 || d == 64 || d == 96 || d == 128 || d == 256; }
+
+// Blocks of rows of sequences that bring up to `max_tokens` tokens, CTAs that may share a block's keys, and floats of scratch and tickets
+// that the launch needs.
+ILB_EXPORT int ilb_kv4_attention_rows_plan(int dtype, int n_seqs, int max_tokens, int nq, int nkv, int d, int max_blocks, int page_size, int sms,
+                                           int* row_blocks, int* splits, long long* scratch, long long* tickets) {
+  ILB_REQUIRE(n_seqs >= 0 && max_tokens > 0 && nkv > 0 && nq > 0 && nq % nkv == 0 && sms > 0 && rows_head(d), "kv4_attention: bad sizes");
+  const int rows = max_tokens * (nq / nkv), per = rows_per_block(dtype, rows);
+  const long long rb = (rows + per - 1) / per, blocks = rb * n_seqs * nkv;
+  const long long slots = (long long)sms * (per == 8 && d <= 128 ? 4 : 2);       // CTAs at work at once
+  const long long most = ((long long)max_blocks * page_size / kKv4Unit + kWarps * kMinUnits - 1) / (kWarps * kMinUnits);
+  long long s = blocks > 0 ? slots / blocks : 1;
+  s = s < 1 ? 1 : s > most ? most : s;
+  *row_blocks = (int)rb;
+  *splits = (int)s;
+  *scratch = s > 1 ? blocks * s * per * (d + 4) : 0;
+  *tickets = s > 1 ? blocks : 0;
+  return 0;
+}
+
+ILB_EXPORT int ilb_kv4_attention_rows(const void* q, void* out, int dtype, const void* cache, const int* positions, const int* cu_q,
+                                      const int* block_table, int max_blocks, int page_size, int num_pages, int window, float scale, int n_seqs,
+                                      int max_tokens, int nq, int nkv, int d, int q_stride, int out_stride, const float* sink, int sms, float* scratch,
+                                      long long scratch_floats, int* tickets, long long n_tickets, int* error_flag, cudaStream_t stream) {
+  ILB_REQUIRE(page_size > 0 && page_size % kKv4Unit == 0 && num_pages > 0 && max_blocks > 0, "kv4_attention: bad cache geometry");
+  ILB_REQUIRE(dtype == kF32 || dtype == kBF16, "kv4_attention: unknown element type");
+  int row_blocks = 0, splits = 0;
+  long long need = 0, need_tickets = 0;
+  if (int rc = ilb_kv4_attention_rows_plan(dtype, n_seqs, max_tokens, nq, nkv, d, max_blocks, page_size, sms, &row_blocks, &splits, &need, &need_tickets))
+    return rc;
+  ILB_REQUIRE(need <= scratch_floats && need_tickets <= n_tickets, "kv4_attention: the scratch holds %lld floats and %lld tickets, %lld and %lld are needed",
+              scratch_floats, n_tickets, need, need_tickets);
+  ILB_REQUIRE((long long)n_seqs * row_blocks <= 65535 && nkv <= 65535, "kv4_attention: %d sequences of %d blocks of rows are too many for one launch",
+              n_seqs, row_blocks);
+  ILB_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)scratch) % 16 == 0 && q_stride % 8 == 0 && out_stride % 8 == 0,
+              "kv4_attention: queries, output, cache and scratch must start on 16-byte boundaries");
+  if (n_seqs == 0) return 0;
+  Params p = {q, out, (const uint8_t*)cache, positions, cu_q, block_table, sink, scratch, tickets, error_flag, max_blocks, page_size, num_pages, window,
+              nq, nkv, q_stride, out_stride, row_blocks, max_tokens, splits, scale * kLog2e};
+  const dim3 grid((unsigned)splits, (unsigned)nkv, (unsigned)(n_seqs * row_blocks));
+  const bool wide = rows_per_block(dtype, max_tokens * (nq / nkv)) == 16;
+#define ILB_KV4_ROWS(SIZE)                                                                       \
+  case SIZE:                                                                                     \
+    if (dtype == kF32) return launch_rows<float, SIZE, 1, 3>(p, grid, stream);                   \
+    if (wide) return launch_rows<__nv_bfloat16, SIZE, 2, 1>(p, grid, stream);                    \
+    return launch_rows<__nv_bfloat16, SIZE, 1, 1>(p, grid, stream);
+  switch (d) {
+    ILB_KV4_ROWS(32)
+    ILB_KV4_ROWS(64)
+    ILB_KV4_ROWS(96)
+    ILB_KV4_ROWS(128)
+    ILB_KV4_ROWS(256)
+  }
+#undef ILB_KV4_ROWS
+  return fail("kv4_attention: head size %d", d);
+}
 
 ILB_EXPORT int ilb_kv4_attention_simple(const void* q, void* out, int dtype, const void* cache, const int* positions, const int* seq_of_token,
                                         const int* block_table, int max_blocks, int page_size, int num_pages, int window, float scale, int n_tokens,
@@ -106,10 +713,10 @@ ILB_EXPORT int ilb_kv4_attention_simple(const void* q, void* out, int dtype, con
   if (n_tokens == 0) return 0;
   const dim3 grid((unsigned)n_tokens, (unsigned)nq);
   if (dtype == kF32)
-    ilb::launch(kv4_attention_simple_kernel<float>, grid, dim3(kWarps * 32), 0, stream, (const float*)q, (float*)out, (const uint8_t*)cache, positions,
+    ilb::launch(kv4_attention_simple_kernel<float>, grid, dim3(kSimpleWarps * 32), 0, stream, (const float*)q, (float*)out, (const uint8_t*)cache, positions,
                 seq_of_token, block_table, max_blocks, page_size, num_pages, window, scale, nq, nkv, d, q_stride, out_stride, sink);
   else
-    ilb::launch(kv4_attention_simple_kernel<__nv_bfloat16>, grid, dim3(kWarps * 32), 0, stream, (const __nv_bfloat16*)q, (__nv_bfloat16*)out,
+    ilb::launch(kv4_attention_simple_kernel<__nv_bfloat16>, grid, dim3(kSimpleWarps * 32), 0, stream, (const __nv_bfloat16*)q, (__nv_bfloat16*)out,
                 (const uint8_t*)cache, positions, seq_of_token, block_table, max_blocks, page_size, num_pages, window, scale, nq, nkv, d, q_stride,
                 out_stride, sink);
   return check_launch("kv4_attention");

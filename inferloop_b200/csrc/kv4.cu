@@ -66,19 +66,28 @@ kv4_write_kernel(const T* __restrict__ k, long long k_row, long long k_head, con
   if (l == 0) *reinterpret_cast<__nv_bfloat16*>(unit + kv4_scale_at(d, value, j, G)) = scale;
 }
 
-// A block a (sequence, page, head): the page's rows below the sequence's length, zeros from there on.
+// A block a (sequence, page, head): the page's rows below the sequence's length, zeros from there on.  Without an output table
+// page b of sequence s goes to page s max_blocks + b; with positions (the tokens that will attend to what is read), rows that the
+// window of the sequence's first token lies behind are zeros, and pages further behind than any tile of keys reaches are left out.
+constexpr int kReadBehind = 256;
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-kv4_read_kernel(const uint8_t* __restrict__ cache, const int* __restrict__ block_table, const int* __restrict__ out_table, int max_blocks,
-                const int* __restrict__ lengths, int page_size, int num_pages, int out_pages, T* __restrict__ k_out, T* __restrict__ v_out,
-                int nkv, int d) {
+kv4_read_kernel(const uint8_t* __restrict__ cache, const int* __restrict__ block_table, int table_stride, const int* __restrict__ out_table,
+                int max_blocks, const int* __restrict__ lengths, const int* __restrict__ positions, const int* __restrict__ cu_q, int window,
+                int page_size, int num_pages, int out_pages, T* __restrict__ k_out, T* __restrict__ v_out, int nkv, int d) {
   pdl_launch_dependents();
   pdl_wait();
   const int blk = blockIdx.x % max_blocks, seq = blockIdx.x / max_blocks, head = blockIdx.y;
-  const int to = out_table[blockIdx.x];
+  const int to = out_table != nullptr ? out_table[(size_t)seq * max_blocks + blk] : (int)blockIdx.x;
   const int live = min(lengths[seq] - blk * page_size, page_size);
   if (to < 0 || to >= out_pages || live <= 0) return;
-  const int page = block_table[blockIdx.x];
+  int first = 0;                                                          // of the page's rows, the first that is read
+  if (positions != nullptr) {
+    first = first_key(positions[cu_q[seq]], window) - blk * page_size;
+    if (first >= page_size + kReadBehind) return;
+  }
+  const int page = block_table[(size_t)seq * table_stride + blk];
   const bool held = page >= 0 && page < num_pages;
   const uint8_t* src = cache + ((size_t)page * nkv + head) * (page_size / kKv4Unit) * kv4_unit_bytes(d);
   const size_t dst = ((size_t)to * nkv + head) * page_size * d;
@@ -87,7 +96,7 @@ kv4_read_kernel(const uint8_t* __restrict__ cache, const int* __restrict__ block
     const int G = at % per_row, slot = at / per_row, j = slot % kKv4Unit;
     const uint8_t* unit = src + (size_t)(slot / kKv4Unit) * kv4_unit_bytes(d);
     float x[2][4] = {};
-    if (held && slot < live) {
+    if (held && slot < live && slot >= first) {
 #pragma unroll
       for (int value = 0; value < 2; ++value) {
         const uint32_t codes = *reinterpret_cast<const uint16_t*>(unit + (value ? kv4_value_at(d, j, G, l) : kv4_key_at(d, j, G, l)));
@@ -132,21 +141,24 @@ ILB_EXPORT int ilb_kv4_write(const void* k, long long k_row, long long k_head, c
   return check_launch("kv4_write");
 }
 
-// k_out, v_out: [out_pages][nkv][page_size][d]; out_table [n_seqs][max_blocks] names the page that a sequence's page goes to (-1: none).
-ILB_EXPORT int ilb_kv4_read(const void* cache, const int* block_table, const int* out_table, int max_blocks, const int* lengths, int n_seqs,
-                            int page_size, int num_pages, int out_pages, void* k_out, void* v_out, int dtype, int nkv, int d, cudaStream_t stream) {
+// k_out, v_out: [out_pages][nkv][page_size][d]; out_table [n_seqs][max_blocks] names the page that a sequence's page goes to (-1: none);
+// null, and positions with cu_q or null: see the kernel.  Rows of block_table are table_stride apart.
+ILB_EXPORT int ilb_kv4_read(const void* cache, const int* block_table, int table_stride, const int* out_table, int max_blocks, const int* lengths,
+                            const int* positions, const int* cu_q, int window, int n_seqs, int page_size, int num_pages, int out_pages, void* k_out,
+                            void* v_out, int dtype, int nkv, int d, cudaStream_t stream) {
   if (int rc = check_cache("kv4_read", page_size, num_pages, max_blocks, nkv, d)) return rc;
-  ILB_REQUIRE(n_seqs >= 0 && (dtype == kF32 || dtype == kBF16) && out_pages >= 0, "kv4_read: bad sizes or types");
+  ILB_REQUIRE(n_seqs >= 0 && (dtype == kF32 || dtype == kBF16) && out_pages >= 0 && table_stride >= max_blocks, "kv4_read: bad sizes or types");
+  ILB_REQUIRE((positions == nullptr) == (cu_q == nullptr), "kv4_read: positions come with the sequences' offsets");
   ILB_REQUIRE(((uintptr_t)cache | (uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0, "kv4_read: cache and output must start on 16-byte boundaries");
   ILB_REQUIRE((long long)n_seqs * max_blocks <= 0x7fffffffLL && nkv <= 65535, "kv4_read: too many pages for one launch");
   if (n_seqs == 0 || out_pages == 0) return 0;
   const dim3 grid((unsigned)(n_seqs * max_blocks), (unsigned)nkv);
-  if (dtype == kF32)
-    ilb::launch(kv4_read_kernel<float>, grid, dim3(kThreads), 0, stream, (const uint8_t*)cache, block_table, out_table, max_blocks, lengths, page_size,
-                num_pages, out_pages, (float*)k_out, (float*)v_out, nkv, d);
-  else
-    ilb::launch(kv4_read_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, stream, (const uint8_t*)cache, block_table, out_table, max_blocks, lengths,
-                page_size, num_pages, out_pages, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, nkv, d);
+#define ILB_KV4_READ(T)                                                                                                                   \
+  ilb::launch(kv4_read_kernel<T>, grid, dim3(kThreads), 0, stream, (const uint8_t*)cache, block_table, table_stride, out_table, max_blocks, lengths, \
+              positions, cu_q, window, page_size, num_pages, out_pages, (T*)k_out, (T*)v_out, nkv, d)
+  if (dtype == kF32) ILB_KV4_READ(float);
+  else ILB_KV4_READ(__nv_bfloat16);
+#undef ILB_KV4_READ
   return check_launch("kv4_read");
 }
 

@@ -37,6 +37,11 @@ def _stream(t: torch.Tensor) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(t.device.index))
 
 
+def _raw_stream(t: torch.Tensor) -> int:
+    """The same as a plain number, for launchers of `_SIGNATURES`."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
 def _need(t: Optional[torch.Tensor], what: str, dtype: Optional[torch.dtype] = None,
           contiguous: bool = True) -> None:
     if t is None:
@@ -53,6 +58,16 @@ LAUNCHES = 0          # kernels launched through this module since import
 
 
 _FUNCTIONS: dict = {}  # launcher name -> (function, its library)
+
+# Argument kinds of launchers whose calls pass plain numbers (p pointer, i int, q 64-bit int, f float): converted by ctypes at a
+# fraction of what wrapping every argument takes.  The others wrap theirs (`_i`, `_f`, `_ptr`).
+_SIGNATURES = {
+    "ilb_kv4_write": "pqqpqqipppiiipiiip",
+    "ilb_kv4_read": "ppipipppiiiiippiiip",
+    "ilb_kv4_attention_simple": "ppippppiiiifiiiiiipp",
+    "ilb_kv4_attention_rows": "ppippppiiiifiiiiiiipipqpqpp",
+}
+_KINDS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "q": ctypes.c_longlong, "f": ctypes.c_float}
 
 
 SCOPE = "other"       # the op class the next launches belong to (see `scope`)
@@ -74,6 +89,8 @@ def _call(module: str, fn: str, *args) -> None:
         lib = load_module(module)
         f = getattr(lib, fn)
         f.restype = ctypes.c_int
+        if fn in _SIGNATURES:
+            f.argtypes = [_KINDS[k] for k in _SIGNATURES[fn]]
         entry = _FUNCTIONS[fn] = (f, lib)
     timer = TIMER
     begin = timer.node_begin() if timer is not None else None
@@ -1673,10 +1690,9 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, step, block_table: torch.Tensor,
     _need(step.positions, "kv4_write positions", torch.int32); _need(step.seq_of_token, "kv4_write sequence indices", torch.int32)
     if step.positions.numel() != T or step.seq_of_token.numel() != T:
         raise KernelError(f"kv4_write: {T} rows for a step of {step.positions.numel()} tokens")
-    ll = ctypes.c_longlong
-    _call("kv4", "ilb_kv4_write", _ptr(k), ll(k.stride(0)), ll(k.stride(1)), _ptr(v), ll(v.stride(0)), ll(v.stride(1)), _i(_code(k)),
-          _ptr(step.positions), _ptr(step.seq_of_token), _ptr(block_table), _i(block_table.shape[1]), _i(page_size), _i(num_pages), _ptr(cache),
-          _i(T), _i(nkv), _i(d), _stream(cache))
+    _call("kv4", "ilb_kv4_write", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _code(k),
+          step.positions.data_ptr(), step.seq_of_token.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, num_pages,
+          cache.data_ptr(), T, nkv, d, _raw_stream(cache))
 
 
 def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, out_table: torch.Tensor, k_out: torch.Tensor,
@@ -1692,24 +1708,64 @@ def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tens
     _need(out_table, "kv4_read output table", torch.int32); _need(lengths, "kv4_read lengths", torch.int32)
     if ps != page_size or out_table.shape != block_table.shape or lengths.numel() != block_table.shape[0]:
         raise KernelError("kv4_read: output pages, output table or lengths do not match the cache and its block table")
-    _call("kv4", "ilb_kv4_read", _ptr(cache), _ptr(block_table), _ptr(out_table), _i(block_table.shape[1]), _ptr(lengths), _i(block_table.shape[0]),
-          _i(page_size), _i(num_pages), _i(out_pages), _ptr(k_out), _ptr(v_out), _i(_code(k_out)), _i(nkv), _i(d), _stream(cache))
+    S, max_blocks = block_table.shape
+    _call("kv4", "ilb_kv4_read", cache.data_ptr(), block_table.data_ptr(), max_blocks, out_table.data_ptr(), max_blocks, lengths.data_ptr(), None, None,
+          0, S, page_size, num_pages, out_pages, k_out.data_ptr(), v_out.data_ptr(), _code(k_out), nkv, d, _raw_stream(cache))
+
+
+KV4_ROWS_HEADS = (32, 64, 96, 128, 256)     # head sizes of the kernel of few rows (others: the simple kernel)
+_KV4_WORKSPACE: dict = {}
+_KV4_PLANS: dict = {}      # sizes of a launch -> (floats of scratch, tickets) that it needs
+
+
+def _kv4_workspace(device: torch.device):
+    """The scratch of callers that bring no workspace of their own: one per device."""
+    ws = _KV4_WORKSPACE.get(device)
+    if ws is None:
+        from ..parts.base import Workspace
+        ws = _KV4_WORKSPACE[device] = Workspace(device)
+    return ws
 
 
 def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step, block_table: torch.Tensor, window: int, scale: float,
-                  nq: int, nkv: int, d: int, sink: Optional[torch.Tensor] = None) -> None:
+                  nq: int, nkv: int, d: int, sink: Optional[torch.Tensor] = None, workspace=None) -> None:
     """Causal attention of the step's tokens over the 4-bit cache; q and out are [T, nq * d] of one type.  `window` and `sink`
-    as in `attention`; a token that sees no key (its pages are not held) gets zeros."""
-    _need(q, "kv4_attention q"); _need(out, "kv4_attention out", q.dtype); _need(sink, "kv4_attention sink", torch.float32)
+    as in `attention`; a token that sees no key (its pages are not held) gets zeros.  Keys of a sequence that are shared out
+    over several CTAs meet in `workspace` (None: one of the device's own)."""
+    _need(q, "kv4_attention q"); _need(out, "kv4_attention out", q.dtype)
     num_pages, page_size = _kv4_need("kv4_attention", cache, block_table, nkv, d)
-    T = q.shape[0]
-    if nq <= 0 or nq % nkv or tuple(q.shape) != (T, nq * d) or out.shape != q.shape or step.positions.numel() != T or step.cu_q.numel() != block_table.shape[0] + 1:
+    T, S = q.shape[0], block_table.shape[0]
+    if nq <= 0 or nq % nkv or q.shape[1] != nq * d or out.shape != q.shape or step.positions.numel() != T or step.cu_q.numel() != S + 1:
         raise KernelError("kv4_attention: queries, output, step and block table do not agree")
-    if sink is not None and sink.numel() != nq:
-        raise KernelError("kv4_attention: one sink logit per query head")
-    _call("attention_kv4", "ilb_kv4_attention_simple", _ptr(q), _ptr(out), _i(_code(q)), _ptr(cache), _ptr(step.positions), _ptr(step.seq_of_token),
-          _ptr(block_table), _i(block_table.shape[1]), _i(page_size), _i(num_pages), _i(window or 0), _f(scale), _i(T), _i(nq), _i(nkv), _i(d),
-          _i(q.shape[1]), _i(out.shape[1]), _ptr(sink), _stream(q))
+    _need(step.positions, "kv4_attention positions", torch.int32); _need(step.cu_q, "kv4_attention offsets", torch.int32)
+    if sink is not None:
+        _need(sink, "kv4_attention sink", torch.float32)
+        if sink.numel() != nq:
+            raise KernelError("kv4_attention: one sink logit per query head")
+    if T == 0:
+        return
+    window, max_blocks, device, code = window or 0, block_table.shape[1], q.device, _code(q)
+    at, to, held = q.data_ptr(), out.data_ptr(), cache.data_ptr()
+    sinks = None if sink is None else sink.data_ptr()
+    if d not in KV4_ROWS_HEADS or (at | to | held) % 16:
+        _need(step.seq_of_token, "kv4_attention sequence indices", torch.int32)
+        _call("attention_kv4", "ilb_kv4_attention_simple", at, to, code, held, step.positions.data_ptr(), step.seq_of_token.data_ptr(),
+              block_table.data_ptr(), max_blocks, page_size, num_pages, window, scale, T, nq, nkv, d, nq * d, nq * d, sinks, _raw_stream(q))
+        return
+    ws = _kv4_workspace(device) if workspace is None else workspace
+    most, sms = 1 if step.decode_only else max(step.h_q_len), _sm_count(device)
+    key = (code, S, most, nq, nkv, d, max_blocks, page_size, sms)
+    plan = _KV4_PLANS.get(key)
+    if plan is None:
+        lib, found = load_module("attention_kv4"), (ctypes.c_int(), ctypes.c_int(), ctypes.c_longlong(), ctypes.c_longlong())
+        if lib.ilb_kv4_attention_rows_plan(*map(_i, key), *map(ctypes.byref, found)) != 0:
+            raise KernelError(lib.ilb_last_error().decode())
+        plan = _KV4_PLANS[key] = (found[2].value, found[3].value)
+    scratch = ws.buffer("kv4.records", (plan[0],), torch.float32)
+    tickets = ws.zeroed("kv4.tickets", (max(plan[1], 4096),), torch.int32)
+    _call("attention_kv4", "ilb_kv4_attention_rows", at, to, code, held, step.positions.data_ptr(), step.cu_q.data_ptr(), block_table.data_ptr(),
+          max_blocks, page_size, num_pages, window, scale, S, most, nq, nkv, d, nq * d, nq * d, sinks, sms, scratch.data_ptr(), scratch.numel(),
+          tickets.data_ptr(), tickets.numel(), _tc_state(device).error.data_ptr(), _raw_stream(q))
 
 
 DECODE_FUSED_ENABLED = True     # tests switch it off to run q/k norm + rotation + cache write as a launch of its own
