@@ -6,11 +6,13 @@
 // Few rows against many keys (`rows_kernel`).  A row is a (token, query head of the group); 8 NB rows of a (sequence, kv head) are a block
 // of the launch, whose keys are shared out over `splits` CTAs and there over warps, a unit of 16 keys at a time.  A unit is one piece of
 // 18 D bytes of the cache: a warp keeps kStages of them on their way to its own ring in shared memory by bulk copies.
-//   scores   S^T = K Q^T on m16n8k16, the 16 keys as rows, so that groups of up to 8 query heads fill the 8 columns.  A code c + 8 in the
-//            last bits of a bfloat16's mantissa is the number 128 + c + 8, exactly: one AND-OR a pair.  The sums of a group of 32 elements
-//            start at -136 times the sum of the group's q, which takes the 136 out again, and are then scaled by the group's scale in
-//            32 bits (with 32-bit queries, which go in as three bfloat16 pieces, 136 is subtracted from the operands instead:
-//            the sum's cancellation would cost 7 bits).
+//   scores   S^T = K Q^T on m16n8k16, the 16 keys as rows, so that groups of up to 8 query heads fill the 8 columns.  In fp16, where one
+//            AND-OR in place makes an exact number of a code c + 8: 1024 + c + 8 from the last bits of the mantissa, 64 + c + 8 from the
+//            four before them.  The sums of a group of 32 elements start at minus what the offsets 1032 and 72 will add (a bare subtraction
+//            per operand would cost as much as making it), and are then scaled by the group's scale in 32 bits.  A bfloat16 query is exact
+//            in fp16 once its row is brought to [1, 2) by a power of two (what is 2^-16 of the row's largest loses bits that the
+//            sum does not hold).  32-bit queries go in as three bfloat16 pieces, and there the operands are c itself: the
+//            offsets' cancellation would cost 10 of the sum's 24 bits.
 //   softmax  32-bit, base 2.  The reference point of a row's exponentials is not raised before a score exceeds it by 4 (in powers of
 //            two), a vote of the warp: the sums stay far from overflow and the maximum's exchange between lanes is rare.
 //   values   O^T += V^T P^T in fp16: the codes of two neighbouring tokens lie in one word each, so AND-OR (1024 + c + 8) and a
@@ -34,8 +36,9 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ------------------------------------------------------------------ few rows, many keys
-constexpr int kWarps = 4, kStages = 4, kThreads = kWarps * 32;
+constexpr int kStages = 4;
 constexpr int kMinUnits = 2;                // units a warp should have before another CTA joins
+constexpr int kMaxSplits = 148;             // CTAs that share a block's keys at most
 
 struct Params {
   const void* q; void* out; const uint8_t* cache; const int* positions; const int* cu_q; const int* block_table; const float* sink;
@@ -53,11 +56,23 @@ __device__ __forceinline__ uint32_t turned(uint32_t x) {            // an 8 x 8 
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// 1032 + c of two codes as fp16 numbers less 1032
-__device__ __forceinline__ uint32_t half_pair(uint32_t w, int nibble) {
-  const uint32_t r = ((w >> (4 * nibble)) & 0x000f000fu) | 0x64006400u, c1032 = 0x64086408u;
-  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&r), *reinterpret_cast<const __half2*>(&c1032));
+// Codes of nibbles 0 .. 3 of both halves of w (`w8` = w >> 8) as fp16 numbers: 1024 + code from nibbles 0 and 2, 64 + code from 1 and 3;
+// less 1032 and 72 the codes' c.
+template <int I>
+__device__ __forceinline__ uint32_t offset_pair(uint32_t w, uint32_t w8) {
+  const uint32_t x = I < 2 ? w : w8;
+  return I % 2 == 0 ? (x & 0x000f000fu) | 0x64006400u : (x & 0x00f000f0u) | 0x54005400u;
+}
+template <int I>
+__device__ __forceinline__ uint32_t half_pair(uint32_t w, uint32_t w8) {
+  const uint32_t r = offset_pair<I>(w, w8), off = I % 2 == 0 ? 0x64086408u : 0x54805480u;
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&r), *reinterpret_cast<const __half2*>(&off));
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float ex2(float x) {                      // 2 ulp; below 2^-126 zero
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
@@ -79,10 +94,10 @@ __device__ __forceinline__ uint32_t plain_pair(uint32_t r) {
 }
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-// d = a b + c
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+// d = a b + c of fp16 numbers
+__device__ __forceinline__ void mma_half(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
@@ -129,21 +144,26 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[PIECE
   }
 }
 
-template <int D, int NB, int PIECES>
+template <int D, int NB, int PIECES, int kWarps>
 struct Shape {
   static constexpr int kGroups = D / 32, kUnitBytes = 18 * D, kRows = 8 * NB;
   static constexpr int kRecRow = D + 4;                                   // of a record in shared memory: no bank is met twice
   static constexpr int kRing = kWarps * kStages * kUnitBytes;
   static constexpr int kRecords = kWarps * kRows * kRecRow * 4;
-  static constexpr int kBody = kRing > kRecords ? kRing : kRecords;       // (the records take the ring's place)
+  static constexpr int kShares = 2 * kMaxSplits * kRows * 4;              // maxima and sums of the records of other CTAs
+  static constexpr int kBody = kRing > kRecords ? (kRing > kShares ? kRing : kShares) : (kRecords > kShares ? kRecords : kShares);      // one after the other
   static constexpr int kQ = PIECES > 1 ? kGroups * 4 * PIECES * 32 * 4 : 0;      // 32-bit queries: their pieces in operand order
   static constexpr int kStats = 3 * kWarps * kRows * 4 + 2 * kRows * 4;
   static constexpr int kSmem = kBody + kQ + kStats + kWarps * kStages * 8 + 16;
 };
 
-template <typename T, int D, int NB, int PIECES>
-__global__ void __launch_bounds__(kThreads, NB == 1 && D <= 128 ? 4 : 2) rows_kernel(const Params p) {
-  using Sh = Shape<D, NB, PIECES>;
+// Warps that an SM has registers for, and CTAs of so many: few rows' worth of state in NB = 1 up to D = 128, twice that otherwise.
+template <int D, int NB> constexpr int kSmWarps = NB == 1 && D <= 128 ? 16 : 8;
+
+template <typename T, int D, int NB, int PIECES, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_kernel(const Params p) {
+  using Sh = Shape<D, NB, PIECES, kWarps>;
+  constexpr int kThreads = kWarps * 32;
   constexpr int NG = Sh::kGroups, U = Sh::kUnitBytes, kRows = Sh::kRows;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -181,22 +201,22 @@ __global__ void __launch_bounds__(kThreads, NB == 1 && D <= 128 ? 4 : 2) rows_ke
   // ---- the stream of units: lane l knows where the l-th of every 32 lies
   const int upp = p.page_size / kKv4Unit;
   const int* table = p.block_table + (size_t)seq * p.max_blocks;
-  long long where = -1;                                                   // unit in the cache, or -1: not held
+  int where = -1;                                                         // unit in the cache, or -1: not held
   auto look_up = [&](int i0) {
     const int i = i0 + lane;
     where = -1;
     if (i < mine) {
       const int u = unit0 + begin + warp + i * kWarps, blk = u / upp;
       const int page = blk < p.max_blocks ? __ldg(table + blk) : -1;
-      if (page >= 0 && page < p.num_pages) where = ((long long)page * p.nkv + head) * upp + u % upp;
+      if (page >= 0 && page < p.num_pages) where = (page * p.nkv + head) * upp + u % upp;
     }
   };
   uint32_t held = 0;                                                      // bit i: the i-th unit of these 32 is held
   auto ask = [&](int i) {                                                 // (unit i must be one of the 32 looked up)
-    const long long at = __shfl_sync(0xffffffffu, where, i & 31);
+    const int at = __shfl_sync(0xffffffffu, where, i & 31);
     if (at >= 0 && lane == 0) {
       mbar_expect_tx(bar0 + 8 * (i % kStages), U);
-      bulk_load(ring + (i % kStages) * U, p.cache + at * U, U, bar0 + 8 * (i % kStages));
+      bulk_load(ring + (i % kStages) * U, p.cache + (size_t)at * U, U, bar0 + 8 * (i % kStages));
     }
     held = (held & ~(1u << (i & 31))) | (at >= 0 ? 1u << (i & 31) : 0u);
   };
@@ -205,42 +225,69 @@ __global__ void __launch_bounds__(kThreads, NB == 1 && D <= 128 ? 4 : 2) rows_ke
   for (int i = 0; i < kStages; ++i)
     if (i < mine) ask(i);
 
-  // ---- queries as second operands, rows g of each block of 8; -136 times the sums of their groups
+  // ---- queries as second operands, rows g of each block of 8; what the offsets of the keys' operands add to the groups' sums
   constexpr int kQRegs = PIECES == 1 ? NG * 4 : 1;
   uint32_t qf[NB][kQRegs];
   float init[NB][PIECES == 1 ? NG : 1][2];
-  float base[NB][2], m[NB][2], l[NB][2];
+  float base[NB][2], m[NB][2], l[NB][2], mult[NB][2];                     // of columns 2 t, 2 t + 1; mult: what makes a logit in base 2 of a sum
   float scale_top = 0.f, scale_exp = 0.f;                                 // fp16: values' scales up to 16 times this need no new exponent; the exponent
-  int row_lo[NB][2], row_hi[NB][2];                                       // of columns 2 t, 2 t + 1
+  int row_lo[NB][2], row_hi[NB][2];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const int r = row0 + nb * 8 + g;
     const bool there = r < rows;
-    const T* src = reinterpret_cast<const T*>(p.q) + (size_t)(tok0 + (there ? r / G : 0)) * p.q_stride + (size_t)(head * G + (there ? r % G : 0)) * D;
+    const T* src = reinterpret_cast<const T*>(p.q) + (size_t)(tok0 + (there ? r / G : 0)) * p.q_stride + (size_t)(head * G + (there ? r % G : 0)) * D + 8 * t;
+    if constexpr (PIECES == 1) {
+      uint4 raw[NG];
+      uint32_t top = 0;
 #pragma unroll
-    for (int G32 = 0; G32 < NG; ++G32) {
-      float x[8];
-      if constexpr (sizeof(T) == 2) {
-        const uint4 w = there ? *reinterpret_cast<const uint4*>(src + G32 * 32 + 8 * t) : make_uint4(0u, 0u, 0u, 0u);
-        x[0] = bf_lo(w.x); x[1] = bf_hi(w.x); x[2] = bf_lo(w.y); x[3] = bf_hi(w.y); x[4] = bf_lo(w.z); x[5] = bf_hi(w.z); x[6] = bf_lo(w.w); x[7] = bf_hi(w.w);
-      } else {
-        const float4 a = there ? *reinterpret_cast<const float4*>(src + G32 * 32 + 8 * t) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 b = there ? *reinterpret_cast<const float4*>(src + G32 * 32 + 8 * t + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-      }
-      // the pairs that the key's words hold: elements i and i + 4 of the lane's eight
-      if constexpr (PIECES == 1) {
+      for (int G32 = 0; G32 < NG; ++G32) raw[G32] = there ? *reinterpret_cast<const uint4*>(src + G32 * 32) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) qf[nb][G32 * 4 + i] = pack_bf16(x[i], x[i + 4]);
-        float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+      for (int G32 = 0; G32 < NG; ++G32)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w = (&raw[G32].x)[i];
+          top = max(top, max((w & 0x7fffu) << 16, w & 0x7fff0000u));
+        }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^-e of the row's largest element's exponent (an infinity or NaN stays one)
+      const int e = (int)(top >> 23), up = min(max(254 - e, 1), 253);
+      const float bring = e == 255 ? 1.f : __uint_as_float((uint32_t)up << 23), back = e == 255 ? 1.f : __uint_as_float((uint32_t)(254 - up) << 23);
+#pragma unroll
+      for (int G32 = 0; G32 < NG; ++G32) {
+        const uint4 w = raw[G32];
+        const float x[8] = {bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y), bf_lo(w.z), bf_hi(w.z), bf_lo(w.w), bf_hi(w.w)};
+        // the pairs that the key's words hold: elements i and i + 4 of the lane's eight
+        float even = 0.f, odd = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t pair = pack_half(x[i] * bring, x[i + 4] * bring);
+          qf[nb][G32 * 4 + i] = pair;
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+          if (i % 2 == 0) even += f.x + f.y;
+          else odd += f.x + f.y;
+        }
+        float sum = fmaf(even, -1032.f, odd * -72.f);
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        init[nb][G32][0] = -136.f * __shfl_sync(0xffffffffu, sum, 8 * t);
-        init[nb][G32][1] = -136.f * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
-      } else if (warp == 0) {
-        uint32_t w[4][PIECES];
+        init[nb][G32][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+        init[nb][G32][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+      }
+      mult[nb][0] = __shfl_sync(0xffffffffu, back, 8 * t) * p.scale_log2;
+      mult[nb][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4) * p.scale_log2;
+    } else {
+      mult[nb][0] = mult[nb][1] = p.scale_log2;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split_pair<PIECES>(x[i], x[i + 4], w[i]);
+      for (int G32 = 0; G32 < NG; ++G32) {
+        if (warp != 0) break;
+        const float4 a = there ? *reinterpret_cast<const float4*>(src + G32 * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 b = there ? *reinterpret_cast<const float4*>(src + G32 * 32 + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+        uint32_t w[4][PIECES];
+        split_pair<PIECES>(a.x, b.x, w[0]);
+        split_pair<PIECES>(a.y, b.y, w[1]);
+        split_pair<PIECES>(a.z, b.z, w[2]);
+        split_pair<PIECES>(a.w, b.w, w[3]);
 #pragma unroll
         for (int i = 0; i < PIECES; ++i)
           asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(q_smem + ((G32 * PIECES + i) * 32 + lane) * 16), "r"(w[0][i]), "r"(w[1][i]),
@@ -288,13 +335,17 @@ __global__ void __launch_bounds__(kThreads, NB == 1 && D <= 128 ? 4 : 2) rows_ke
 #pragma unroll
         for (int G32 = 0; G32 < NG; ++G32) {
           uint32_t a[2][4];
+          if constexpr (PIECES == 1) {
+            const uint32_t ka8 = ka[G32] >> 8, kb8 = kb[G32] >> 8;
+            a[0][0] = offset_pair<0>(ka[G32], ka8); a[0][1] = offset_pair<0>(kb[G32], kb8);
+            a[0][2] = offset_pair<1>(ka[G32], ka8); a[0][3] = offset_pair<1>(kb[G32], kb8);
+            a[1][0] = offset_pair<2>(ka[G32], ka8); a[1][1] = offset_pair<2>(kb[G32], kb8);
+            a[1][2] = offset_pair<3>(ka[G32], ka8); a[1][3] = offset_pair<3>(kb[G32], kb8);
+          } else {
 #pragma unroll
-          for (int ks = 0; ks < 2; ++ks) {
-            a[ks][0] = raised(ka[G32], 2 * ks); a[ks][1] = raised(kb[G32], 2 * ks);
-            a[ks][2] = raised(ka[G32], 2 * ks + 1); a[ks][3] = raised(kb[G32], 2 * ks + 1);
-            if constexpr (PIECES > 1) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) a[ks][e] = plain_pair(a[ks][e]);
+            for (int ks = 0; ks < 2; ++ks) {
+              a[ks][0] = plain_pair(raised(ka[G32], 2 * ks)); a[ks][1] = plain_pair(raised(kb[G32], 2 * ks));
+              a[ks][2] = plain_pair(raised(ka[G32], 2 * ks + 1)); a[ks][3] = plain_pair(raised(kb[G32], 2 * ks + 1));
             }
           }
 #pragma unroll
@@ -302,16 +353,16 @@ __global__ void __launch_bounds__(kThreads, NB == 1 && D <= 128 ? 4 : 2) rows_ke
             float acc[4];
             if constexpr (PIECES == 1) {
               const float c[4] = {init[nb][G32][0], init[nb][G32][1], init[nb][G32][0], init[nb][G32][1]};
-              mma(acc, a[0], qf[nb][G32 * 4], qf[nb][G32 * 4 + 1], c);
-              mma(acc, a[1], qf[nb][G32 * 4 + 2], qf[nb][G32 * 4 + 3], acc);
+              mma_half(acc, a[0], qf[nb][G32 * 4], qf[nb][G32 * 4 + 1], c);
+              mma_half(acc, a[1], qf[nb][G32 * 4 + 2], qf[nb][G32 * 4 + 3], acc);
             } else {
               acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
 #pragma unroll
               for (int i3 = PIECES - 1; i3 >= 0; --i3) {                  // the smallest pieces first
                 uint32_t w[4];
                 lds(q_smem + ((G32 * PIECES + i3) * 32 + lane) * 16, w);
-                mma(acc, a[0], w[0], w[1], acc);
-                mma(acc, a[1], w[2], w[3], acc);
+                mma_16816(acc, a[0], w[0], w[1]);
+                mma_16816(acc, a[1], w[2], w[3]);
               }
             }
             if (G32 == 0) {
@@ -331,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, NB == 1 && D <= 128 ? 4 : 2) rows_ke
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sv[nb][e] *= p.scale_log2;
+        for (int e = 0; e < 4; ++e) sv[nb][e] *= mult[nb][e & 1];
       }
       if (!whole) {
         bool first = false, second = false;
@@ -389,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, NB == 1 && D <= 128 ? 4 : 2) rows_ke
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sv[nb][e] = exp2f(sv[nb][e] - base[nb][e & 1]);
+        for (int e = 0; e < 4; ++e) sv[nb][e] = ex2(sv[nb][e] - base[nb][e & 1]);
         l[nb][0] += sv[nb][0] + sv[nb][2];
         l[nb][1] += sv[nb][1] + sv[nb][3];
       }
@@ -404,12 +455,13 @@ __global__ void __launch_bounds__(kThreads, NB == 1 && D <= 128 ? 4 : 2) rows_ke
           const uint32_t wa = __byte_perm(va[G32 / 2], va[(NG + G32) / 2], half_sel(G32, NG + G32));
           const uint32_t wb = __byte_perm(vb[G32 / 2], vb[(NG + G32) / 2], half_sel(G32, NG + G32));
           uint32_t a[2][4];
+          if constexpr (PIECES == 1) {
+            const uint32_t wa8 = wa >> 8, wb8 = wb >> 8;
+            a[0][0] = half_pair<0>(wa, wa8); a[0][1] = half_pair<1>(wa, wa8); a[0][2] = half_pair<0>(wb, wb8); a[0][3] = half_pair<1>(wb, wb8);
+            a[1][0] = half_pair<2>(wa, wa8); a[1][1] = half_pair<3>(wa, wa8); a[1][2] = half_pair<2>(wb, wb8); a[1][3] = half_pair<3>(wb, wb8);
+          } else {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if constexpr (PIECES == 1) {
-              a[h][0] = half_pair(wa, 2 * h); a[h][1] = half_pair(wa, 2 * h + 1);
-              a[h][2] = half_pair(wb, 2 * h); a[h][3] = half_pair(wb, 2 * h + 1);
-            } else {
+            for (int h = 0; h < 2; ++h) {
               a[h][0] = plain_pair(raised(wa, 2 * h)); a[h][1] = plain_pair(raised(wa, 2 * h + 1));
               a[h][2] = plain_pair(raised(wb, 2 * h)); a[h][3] = plain_pair(raised(wb, 2 * h + 1));
             }
@@ -524,36 +576,59 @@ __global__ void __launch_bounds__(kThreads, NB == 1 && D <= 128 ? 4 : 2) rows_ke
   __syncthreads();
   if (!flags[0]) return;
   __threadfence();
+  // (factors of all records first, side by side; the records then come many loads at a time)
+  const float* first = p.scratch + place * kRows * (D + 4);
+  constexpr size_t kStep = (size_t)kRows * (D + 4);
+  float* shares = rec;                                                    // [record][row]
+  for (int at = threadIdx.x; at < on * kRows; at += kThreads) {
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(first + (size_t)at * (D + 4) + D));
+    shares[2 * at] = ml.x;
+    shares[2 * at + 1] = ml.y;
+  }
+  __syncthreads();
+  if (threadIdx.x < n_rows) {
+    const int r = threadIdx.x;
+    const float sink = sink_of(r);
+    float top = sink;
+    for (int c = 0; c < on; ++c) top = fmaxf(top, shares[2 * (c * kRows + r)]);
+    float total = sink == -INFINITY ? 0.f : exp2f(sink - top);
+    for (int c = 0; c < on; ++c) {                                        // in the order of the CTAs, whoever came last
+      const float mc = shares[2 * (c * kRows + r)], lc = shares[2 * (c * kRows + r) + 1];
+      const float f = mc == -INFINITY ? (lc == 0.f ? 0.f : 1.f) : exp2f(mc - top);
+      shares[2 * (c * kRows + r)] = f;
+      total = fmaf(lc, f, total);
+    }
+    row_m[kRows + r] = total;
+  }
+  __syncthreads();
   for (int at = threadIdx.x; at < n_rows * kQuads; at += kThreads) {
     const int r = at / kQuads, d4 = at % kQuads;
-    const float* first = p.scratch + (place * kRows + r) * (D + 4);
-    const size_t step = (size_t)kRows * (D + 4);
-    const float sink = sink_of(r);
-    float top = sink, total = 0.f;
+    const float* src = first + (size_t)r * (D + 4) + 4 * d4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = 0; c < on; ++c) {                                        // in the order of the CTAs, whoever came last
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(first + c * step + D));
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(first + c * step + 4 * d4));
-      const float m_new = fmaxf(top, ml.x), b = m_new == -INFINITY ? 0.f : m_new;
-      const float f = exp2f(top - b), e = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2f(ml.x - b);
-      if (c == 0 && sink != -INFINITY) total = 1.f;                       // exp(sink), against itself
-      total = fmaf(total, f, ml.y * e);
-      v.x = fmaf(v.x, f, x.x * e); v.y = fmaf(v.y, f, x.y * e); v.z = fmaf(v.z, f, x.z * e); v.w = fmaf(v.w, f, x.w * e);
-      top = m_new;
+#pragma unroll 8
+    for (int c = 0; c < on; ++c) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(src + c * kStep));
+      const float f = shares[2 * (c * kRows + r)];
+      v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
     }
-    write_row(r, d4, v, total);
+    write_row(r, d4, v, row_m[kRows + r]);
   }
 }
 
-template <typename T, int D, int NB, int PIECES>
-int launch_rows(const Params& p, dim3 grid, cudaStream_t stream) {
+template <typename T, int D, int NB, int PIECES, int kWarps>
+int launch_as(const Params& p, dim3 grid, cudaStream_t stream) {
   static OncePerDevice once;
-  auto kernel = rows_kernel<T, D, NB, PIECES>;
-  constexpr int smem = Shape<D, NB, PIECES>::kSmem;
+  auto kernel = rows_kernel<T, D, NB, PIECES, kWarps>;
+  constexpr int smem = Shape<D, NB, PIECES, kWarps>::kSmem;
+  static_assert(kSmWarps<D, NB> / kWarps * (smem + 1024) <= 228 * 1024, "the CTAs of an SM do not fit its shared memory");
   const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
   if (e != cudaSuccess) return fail("kv4_attention: %s", cudaGetErrorString(e));
-  ilb::launch(kernel, grid, dim3(kThreads), smem, stream, p);
+  ilb::launch(kernel, grid, dim3(kWarps * 32), smem, stream, p);
   return check_launch("kv4_attention");
+}
+template <typename T, int D, int NB, int PIECES>
+int launch_rows(const Params& p, dim3 grid, int warps, cudaStream_t stream) {
+  return warps == 4 ? launch_as<T, D, NB, PIECES, 4>(p, grid, stream) : launch_as<T, D, NB, PIECES, kSmWarps<D, NB>>(p, grid, stream);
 }
 
 // ------------------------------------------------------------------ any head size
@@ -642,25 +717,33 @@ kv4_attention_simple_kernel(const T* __restrict__ q, T* __restrict__ out, const 
 
 }  // namespace
 
-// Rows that a block of the launch takes: 8 of a group of up to 8 heads' single token or of 32-bit queries, else 16.
-static int rows_per_block(int dtype, int rows) { return dtype == kF32 || rows <= 8 ? 8 : 16; }
+// Rows that a block of the launch takes: 8 of a group of up to 8 heads' single token, of 32-bit queries or of heads of 256 (whose state of
+// 16 rows no thread's registers hold), else 16.
+static int rows_per_block(int dtype, int rows, int d) { return dtype == kF32 || rows <= 8 || d > 128 ? 8 : 16; }
 
 // Head sizes that the kernel of few rows takes.
 static bool rows_head(int d) { return d == 32 || d == 64 || d == 96 || d == 128 || d == 256; }
 
+// Warps of a CTA: blocks that fill the device by themselves get small CTAs, several to an SM; fewer blocks are shared out over CTAs of
+// a whole SM each, so that fewer records have to meet.
+static int warps_per_cta(int sm_warps, long long blocks, int sms) { return blocks > sms ? 4 : sm_warps; }
+
 // Blocks of rows of sequences that bring up to `max_tokens` tokens, CTAs that may share a block's keys, and floats of scratch and tickets
 // that the launch needs.
 ILB_EXPORT int ilb_kv4_attention_rows_plan(int dtype, int n_seqs, int max_tokens, int nq, int nkv, int d, int max_blocks, int page_size, int sms,
-                                           int* row_blocks, int* splits, long long* scratch, long long* tickets) {
+                                           int* row_blocks, int* splits, int* warps, long long* scratch, long long* tickets) {
   ILB_REQUIRE(n_seqs >= 0 && max_tokens > 0 && nkv > 0 && nq > 0 && nq % nkv == 0 && sms > 0 && rows_head(d), "kv4_attention: bad sizes");
-  const int rows = max_tokens * (nq / nkv), per = rows_per_block(dtype, rows);
+  const int rows = max_tokens * (nq / nkv), per = rows_per_block(dtype, rows, d);
   const long long rb = (rows + per - 1) / per, blocks = rb * n_seqs * nkv;
-  const long long slots = (long long)sms * (per == 8 && d <= 128 ? 4 : 2);       // CTAs at work at once
-  const long long most = ((long long)max_blocks * page_size / kKv4Unit + kWarps * kMinUnits - 1) / (kWarps * kMinUnits);
+  const int sm_warps = per == 8 && d <= 128 ? 16 : 8, w = warps_per_cta(sm_warps, blocks, sms);
+  const long long slots = (long long)sms * (sm_warps / w);                        // CTAs at work at once
+  const long long most = ((long long)max_blocks * page_size / kKv4Unit + w * kMinUnits - 1) / (w * kMinUnits);
   long long s = blocks > 0 ? slots / blocks : 1;
   s = s < 1 ? 1 : s > most ? most : s;
+  s = s > kMaxSplits ? kMaxSplits : s;
   *row_blocks = (int)rb;
   *splits = (int)s;
+  *warps = w;
   *scratch = s > 1 ? blocks * s * per * (d + 4) : 0;
   *tickets = s > 1 ? blocks : 0;
   return 0;
@@ -672,9 +755,10 @@ ILB_EXPORT int ilb_kv4_attention_rows(const void* q, void* out, int dtype, const
                                       long long scratch_floats, int* tickets, long long n_tickets, int* error_flag, cudaStream_t stream) {
   ILB_REQUIRE(page_size > 0 && page_size % kKv4Unit == 0 && num_pages > 0 && max_blocks > 0, "kv4_attention: bad cache geometry");
   ILB_REQUIRE(dtype == kF32 || dtype == kBF16, "kv4_attention: unknown element type");
-  int row_blocks = 0, splits = 0;
+  int row_blocks = 0, splits = 0, warps = 0;
   long long need = 0, need_tickets = 0;
-  if (int rc = ilb_kv4_attention_rows_plan(dtype, n_seqs, max_tokens, nq, nkv, d, max_blocks, page_size, sms, &row_blocks, &splits, &need, &need_tickets))
+  if (int rc = ilb_kv4_attention_rows_plan(dtype, n_seqs, max_tokens, nq, nkv, d, max_blocks, page_size, sms, &row_blocks, &splits, &warps, &need,
+                                           &need_tickets))
     return rc;
   ILB_REQUIRE(need <= scratch_floats && need_tickets <= n_tickets, "kv4_attention: the scratch holds %lld floats and %lld tickets, %lld and %lld are needed",
               scratch_floats, n_tickets, need, need_tickets);
@@ -686,12 +770,12 @@ ILB_EXPORT int ilb_kv4_attention_rows(const void* q, void* out, int dtype, const
   Params p = {q, out, (const uint8_t*)cache, positions, cu_q, block_table, sink, scratch, tickets, error_flag, max_blocks, page_size, num_pages, window,
               nq, nkv, q_stride, out_stride, row_blocks, max_tokens, splits, scale * kLog2e};
   const dim3 grid((unsigned)splits, (unsigned)nkv, (unsigned)(n_seqs * row_blocks));
-  const bool wide = rows_per_block(dtype, max_tokens * (nq / nkv)) == 16;
+  const bool wide = rows_per_block(dtype, max_tokens * (nq / nkv), d) == 16;
 #define ILB_KV4_ROWS(SIZE)                                                                       \
   case SIZE:                                                                                     \
-    if (dtype == kF32) return launch_rows<float, SIZE, 1, 3>(p, grid, stream);                   \
-    if (wide) return launch_rows<__nv_bfloat16, SIZE, 2, 1>(p, grid, stream);                    \
-    return launch_rows<__nv_bfloat16, SIZE, 1, 1>(p, grid, stream);
+    if (dtype == kF32) return launch_rows<float, SIZE, 1, 3>(p, grid, warps, stream);            \
+    if (wide) return launch_rows<__nv_bfloat16, SIZE, 2, 1>(p, grid, warps, stream); \
+    return launch_rows<__nv_bfloat16, SIZE, 1, 1>(p, grid, warps, stream);
   switch (d) {
     ILB_KV4_ROWS(32)
     ILB_KV4_ROWS(64)

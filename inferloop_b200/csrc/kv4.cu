@@ -66,48 +66,80 @@ kv4_write_kernel(const T* __restrict__ k, long long k_row, long long k_head, con
   if (l == 0) *reinterpret_cast<__nv_bfloat16*>(unit + kv4_scale_at(d, value, j, G)) = scale;
 }
 
-// A block a (sequence, page, head): the page's rows below the sequence's length, zeros from there on.  Without an output table
-// page b of sequence s goes to page s max_blocks + b; with positions (the tokens that will attend to what is read), rows that the
-// window of the sequence's first token lies behind are zeros, and pages further behind than any tile of keys reaches are left out.
-constexpr int kReadBehind = 256;
+// Eight codes of a word times their scale, in order (a product of two bfloat16 numbers, rounded once).
+__device__ __forceinline__ void spread(uint32_t w, uint32_t scale, __nv_bfloat16* dst) {
+  uint32_t pair[4];                                                       // elements i and i + 4
+  const uint32_t s2 = scale | scale << 16, c136 = 0x43084308u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t r = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;      // 128 + code
+    const __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&r), *reinterpret_cast<const __nv_bfloat162*>(&c136)),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&s2));
+    pair[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  *reinterpret_cast<uint4*>(dst) = make_uint4(__byte_perm(pair[0], pair[1], 0x5410), __byte_perm(pair[2], pair[3], 0x5410),
+                                              __byte_perm(pair[0], pair[1], 0x7632), __byte_perm(pair[2], pair[3], 0x7632));
+}
+__device__ __forceinline__ void spread(uint32_t w, uint32_t scale, float* dst) {
+  const float s = __uint_as_float(scale << 16);
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = (float)((int)((w >> (4 * i)) & 15u) - 8) * s;
+  reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+  reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
+// A block takes `entries` places of the block table and one head, finds the pages among them that are wanted and deals their rows out to its
+// threads, eight elements of keys and of values each: a step that wants one page of each of many long sequences costs a look at
+// the tables and no more.  Rows from the sequence's length on are zeros.
+constexpr int kReadThreads = 256, kMaxEntries = 32;
+
+template <typename T, int DIM>
+__global__ void __launch_bounds__(kReadThreads)
 kv4_read_kernel(const uint8_t* __restrict__ cache, const int* __restrict__ block_table, int table_stride, const int* __restrict__ out_table,
-                int max_blocks, const int* __restrict__ lengths, const int* __restrict__ positions, const int* __restrict__ cu_q, int window,
-                int page_size, int num_pages, int out_pages, T* __restrict__ k_out, T* __restrict__ v_out, int nkv, int d) {
+                int n_seqs, int max_blocks, int entries, const int* __restrict__ lengths, int page_size, int num_pages, int out_pages,
+                T* __restrict__ k_out, T* __restrict__ v_out, int nkv, int d_any) {
   pdl_launch_dependents();
   pdl_wait();
-  const int blk = blockIdx.x % max_blocks, seq = blockIdx.x / max_blocks, head = blockIdx.y;
-  const int to = out_table != nullptr ? out_table[(size_t)seq * max_blocks + blk] : (int)blockIdx.x;
-  const int live = min(lengths[seq] - blk * page_size, page_size);
-  if (to < 0 || to >= out_pages || live <= 0) return;
-  int first = 0;                                                          // of the page's rows, the first that is read
-  if (positions != nullptr) {
-    first = first_key(positions[cu_q[seq]], window) - blk * page_size;
-    if (first >= page_size + kReadBehind) return;
-  }
-  const int page = block_table[(size_t)seq * table_stride + blk];
-  const bool held = page >= 0 && page < num_pages;
-  const uint8_t* src = cache + ((size_t)page * nkv + head) * (page_size / kKv4Unit) * kv4_unit_bytes(d);
-  const size_t dst = ((size_t)to * nkv + head) * page_size * d;
-  const int per_row = d / kKv4Group, l = threadIdx.x & 7;
-  for (int at = threadIdx.x >> 3; at < page_size * per_row; at += kThreads / 8) {
-    const int G = at % per_row, slot = at / per_row, j = slot % kKv4Unit;
-    const uint8_t* unit = src + (size_t)(slot / kKv4Unit) * kv4_unit_bytes(d);
-    float x[2][4] = {};
-    if (held && slot < live && slot >= first) {
-#pragma unroll
-      for (int value = 0; value < 2; ++value) {
-        const uint32_t codes = *reinterpret_cast<const uint16_t*>(unit + (value ? kv4_value_at(d, j, G, l) : kv4_key_at(d, j, G, l)));
-        const float s = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(unit + kv4_scale_at(d, value, j, G)));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[value][i] = (float)((int)((codes >> (4 * i)) & 15u) - 8) * s;
-      }
+  __shared__ int from[kMaxEntries], to[kMaxEntries], rows[kMaxEntries];
+  __shared__ int wanted;
+  const int d = DIM > 0 ? DIM : d_any, head = blockIdx.y;
+  if (threadIdx.x < 32) {
+    const long long at = (long long)blockIdx.x * entries + threadIdx.x;
+    int page = -1, out = -1, live = 0;
+    if ((int)threadIdx.x < entries && at < (long long)n_seqs * max_blocks) {
+      const int seq = (int)(at / max_blocks), blk = (int)(at % max_blocks);
+      out = out_table[at];
+      live = min(lengths[seq] - blk * page_size, page_size);
+      page = block_table[(size_t)seq * table_stride + blk];
     }
-    const size_t o = dst + (size_t)slot * d + G * kKv4Group + 4 * l;
-    store4(k_out + o, x[0]);
-    store4(v_out + o, x[1]);
+    const bool want = out >= 0 && out < out_pages && live > 0;
+    const uint32_t all = __ballot_sync(0xffffffffu, want);
+    if (want) {
+      const int i = __popc(all & ((1u << threadIdx.x) - 1u));
+      from[i] = page >= 0 && page < num_pages ? page : -1;
+      to[i] = out;
+      rows[i] = live;
+    }
+    if (threadIdx.x == 0) wanted = __popc(all);
+  }
+  __syncthreads();
+  const int per_row = d / 8, per_page = page_size * per_row, n = wanted * per_page;
+#pragma unroll 2
+  for (int x = threadIdx.x; x < n; x += kReadThreads) {
+    const int i = x / per_page, at = x - i * per_page, slot = at / per_row, e8 = at - slot * per_row, j = slot % kKv4Unit, G = e8 >> 2, l = 2 * (e8 & 3);
+    uint32_t k = 0x88888888u, v = 0x88888888u, ks = 0, vs = 0;            // zeros
+    if (from[i] >= 0 && slot < rows[i]) {
+      const uint8_t* unit = cache + (((size_t)from[i] * nkv + head) * (page_size / kKv4Unit) + slot / kKv4Unit) * kv4_unit_bytes(d);
+      k = *reinterpret_cast<const uint32_t*>(unit + kv4_key_at(d, j, G, l));
+      v = (uint32_t)*reinterpret_cast<const uint16_t*>(unit + kv4_value_at(d, j, G, l)) |
+          (uint32_t)*reinterpret_cast<const uint16_t*>(unit + kv4_value_at(d, j, G, l + 1)) << 16;
+      ks = *reinterpret_cast<const uint16_t*>(unit + kv4_scale_at(d, false, j, G));
+      vs = *reinterpret_cast<const uint16_t*>(unit + kv4_scale_at(d, true, j, G));
+    }
+    const size_t o = (((size_t)to[i] * nkv + head) * page_size + slot) * d + 8 * e8;
+    spread(k, ks, k_out + o);
+    spread(v, vs, v_out + o);
   }
 }
 
@@ -141,23 +173,33 @@ ILB_EXPORT int ilb_kv4_write(const void* k, long long k_row, long long k_head, c
   return check_launch("kv4_write");
 }
 
-// k_out, v_out: [out_pages][nkv][page_size][d]; out_table [n_seqs][max_blocks] names the page that a sequence's page goes to (-1: none);
-// null, and positions with cu_q or null: see the kernel.  Rows of block_table are table_stride apart.
+// k_out, v_out: [out_pages][nkv][page_size][d]; out_table [n_seqs][max_blocks] names the page that a sequence's page goes to (-1: none).
+// Rows of block_table are table_stride apart.
 ILB_EXPORT int ilb_kv4_read(const void* cache, const int* block_table, int table_stride, const int* out_table, int max_blocks, const int* lengths,
-                            const int* positions, const int* cu_q, int window, int n_seqs, int page_size, int num_pages, int out_pages, void* k_out,
-                            void* v_out, int dtype, int nkv, int d, cudaStream_t stream) {
+                            int n_seqs, int page_size, int num_pages, int out_pages, void* k_out, void* v_out, int dtype, int nkv, int d,
+                            cudaStream_t stream) {
   if (int rc = check_cache("kv4_read", page_size, num_pages, max_blocks, nkv, d)) return rc;
   ILB_REQUIRE(n_seqs >= 0 && (dtype == kF32 || dtype == kBF16) && out_pages >= 0 && table_stride >= max_blocks, "kv4_read: bad sizes or types");
-  ILB_REQUIRE((positions == nullptr) == (cu_q == nullptr), "kv4_read: positions come with the sequences' offsets");
   ILB_REQUIRE(((uintptr_t)cache | (uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0, "kv4_read: cache and output must start on 16-byte boundaries");
-  ILB_REQUIRE((long long)n_seqs * max_blocks <= 0x7fffffffLL && nkv <= 65535, "kv4_read: too many pages for one launch");
+  const long long places = (long long)n_seqs * max_blocks;
+  ILB_REQUIRE(places <= 0x7fffffffLL && nkv <= 65535 && page_size <= (1 << 16), "kv4_read: too many pages for one launch");
   if (n_seqs == 0 || out_pages == 0) return 0;
-  const dim3 grid((unsigned)(n_seqs * max_blocks), (unsigned)nkv);
-#define ILB_KV4_READ(T)                                                                                                                   \
-  ilb::launch(kv4_read_kernel<T>, grid, dim3(kThreads), 0, stream, (const uint8_t*)cache, block_table, table_stride, out_table, max_blocks, lengths, \
-              positions, cu_q, window, page_size, num_pages, out_pages, (T*)k_out, (T*)v_out, nkv, d)
-  if (dtype == kF32) ILB_KV4_READ(float);
-  else ILB_KV4_READ(__nv_bfloat16);
+  // as many places a block as leave two rounds of blocks (eight to an SM of 148)
+  long long entries = places * nkv / (2 * 8 * 148);
+  entries = entries < 1 ? 1 : entries > kMaxEntries ? kMaxEntries : entries;
+  const dim3 grid((unsigned)((places + entries - 1) / entries), (unsigned)nkv);
+#define ILB_KV4_READ(T, DIM)                                                                                                                  \
+  ilb::launch(kv4_read_kernel<T, DIM>, grid, dim3(kReadThreads), 0, stream, (const uint8_t*)cache, block_table, table_stride, out_table, n_seqs, \
+              max_blocks, (int)entries, lengths, page_size, num_pages, out_pages, (T*)k_out, (T*)v_out, nkv, d)
+  if (dtype == kF32) {
+    if (d == 64) ILB_KV4_READ(float, 64);
+    else if (d == 128) ILB_KV4_READ(float, 128);
+    else ILB_KV4_READ(float, 0);
+  } else {
+    if (d == 64) ILB_KV4_READ(__nv_bfloat16, 64);
+    else if (d == 128) ILB_KV4_READ(__nv_bfloat16, 128);
+    else ILB_KV4_READ(__nv_bfloat16, 0);
+  }
 #undef ILB_KV4_READ
   return check_launch("kv4_read");
 }

@@ -63,7 +63,7 @@ _FUNCTIONS: dict = {}  # launcher name -> (function, its library)
 # fraction of what wrapping every argument takes.  The others wrap theirs (`_i`, `_f`, `_ptr`).
 _SIGNATURES = {
     "ilb_kv4_write": "pqqpqqipppiiipiiip",
-    "ilb_kv4_read": "ppipipppiiiiippiiip",
+    "ilb_kv4_read": "ppipipiiiippiiip",
     "ilb_kv4_attention_simple": "ppippppiiiifiiiiiipp",
     "ilb_kv4_attention_rows": "ppippppiiiifiiiiiiipipqpqpp",
 }
@@ -1669,12 +1669,21 @@ def kv4_cache_shape(pages: int, nkv: int, page_size: int, d: int) -> tuple:
 
 def _kv4_need(what: str, cache: torch.Tensor, block_table: torch.Tensor, nkv: int, d: int) -> tuple:
     """(pages, page size) of a 4-bit cache that holds `nkv` heads of `d`."""
-    _need(cache, what + " cache", torch.uint8); _need(block_table, what + " block table", torch.int32)
-    if cache.dim() != 4 or cache.shape[2] == 0 or tuple(cache.shape) != kv4_cache_shape(cache.shape[0], nkv, cache.shape[2] * KV4_UNIT, d):
-        raise KernelError(f"{what}: cache shape {tuple(cache.shape)} is not [pages, {nkv}, page size / {KV4_UNIT}, {18 * d}]")
+    if cache.dtype is not torch.uint8 or block_table.dtype is not torch.int32 or not (cache.is_contiguous() and block_table.is_contiguous()
+                                                                                     and cache.is_cuda and block_table.is_cuda):
+        _need(cache, what + " cache", torch.uint8); _need(block_table, what + " block table", torch.int32)
+    shape = cache.shape
+    if len(shape) != 4 or shape[1] != nkv or shape[3] != 18 * d or shape[2] == 0 or d % KV4_GROUP or not 0 < d <= KV4_MAX_HEAD:
+        raise KernelError(f"{what}: cache shape {tuple(shape)} is not [pages, {nkv}, page size / {KV4_UNIT}, {18 * d}]")
     if block_table.dim() != 2:
         raise KernelError(f"{what}: the block table must be [sequences, blocks]")
-    return cache.shape[0], cache.shape[2] * KV4_UNIT
+    return shape[0], shape[2] * KV4_UNIT
+
+
+def _kv4_ints(what: str, *tensors: torch.Tensor) -> None:
+    for t in tensors:
+        if t.dtype is not torch.int32 or not (t.is_cuda and t.is_contiguous()):
+            _need(t, what, torch.int32)
 
 
 def kv4_write(k: torch.Tensor, v: torch.Tensor, step, block_table: torch.Tensor, cache: torch.Tensor) -> None:
@@ -1687,12 +1696,13 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, step, block_table: torch.Tensor,
         raise KernelError("kv4_write: keys and values must be [tokens, heads, head size] with a head's elements side by side")
     T, nkv, d = k.shape
     num_pages, page_size = _kv4_need("kv4_write", cache, block_table, nkv, d)
-    _need(step.positions, "kv4_write positions", torch.int32); _need(step.seq_of_token, "kv4_write sequence indices", torch.int32)
-    if step.positions.numel() != T or step.seq_of_token.numel() != T:
-        raise KernelError(f"kv4_write: {T} rows for a step of {step.positions.numel()} tokens")
+    positions, seqs = step.positions, step.seq_of_token
+    _kv4_ints("kv4_write positions and sequence indices", positions, seqs)
+    if positions.numel() != T or seqs.numel() != T:
+        raise KernelError(f"kv4_write: {T} rows for a step of {positions.numel()} tokens")
     _call("kv4", "ilb_kv4_write", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _code(k),
-          step.positions.data_ptr(), step.seq_of_token.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, num_pages,
-          cache.data_ptr(), T, nkv, d, _raw_stream(cache))
+          positions.data_ptr(), seqs.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, num_pages, cache.data_ptr(), T, nkv, d,
+          _raw_stream(cache))
 
 
 def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, out_table: torch.Tensor, k_out: torch.Tensor,
@@ -1705,12 +1715,12 @@ def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tens
         raise KernelError("kv4_read: outputs must be [pages, heads, page size, head size]")
     out_pages, nkv, ps, d = k_out.shape
     num_pages, page_size = _kv4_need("kv4_read", cache, block_table, nkv, d)
-    _need(out_table, "kv4_read output table", torch.int32); _need(lengths, "kv4_read lengths", torch.int32)
+    _kv4_ints("kv4_read output table and lengths", out_table, lengths)
     if ps != page_size or out_table.shape != block_table.shape or lengths.numel() != block_table.shape[0]:
         raise KernelError("kv4_read: output pages, output table or lengths do not match the cache and its block table")
     S, max_blocks = block_table.shape
-    _call("kv4", "ilb_kv4_read", cache.data_ptr(), block_table.data_ptr(), max_blocks, out_table.data_ptr(), max_blocks, lengths.data_ptr(), None, None,
-          0, S, page_size, num_pages, out_pages, k_out.data_ptr(), v_out.data_ptr(), _code(k_out), nkv, d, _raw_stream(cache))
+    _call("kv4", "ilb_kv4_read", cache.data_ptr(), block_table.data_ptr(), max_blocks, out_table.data_ptr(), max_blocks, lengths.data_ptr(), S, page_size, num_pages,
+          out_pages, k_out.data_ptr(), v_out.data_ptr(), _code(k_out), nkv, d, _raw_stream(cache))
 
 
 KV4_ROWS_HEADS = (32, 64, 96, 128, 256)     # head sizes of the kernel of few rows (others: the simple kernel)
@@ -1734,38 +1744,41 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
     over several CTAs meet in `workspace` (None: one of the device's own)."""
     _need(q, "kv4_attention q"); _need(out, "kv4_attention out", q.dtype)
     num_pages, page_size = _kv4_need("kv4_attention", cache, block_table, nkv, d)
-    T, S = q.shape[0], block_table.shape[0]
-    if nq <= 0 or nq % nkv or q.shape[1] != nq * d or out.shape != q.shape or step.positions.numel() != T or step.cu_q.numel() != S + 1:
+    (T, width), (S, max_blocks) = q.shape, block_table.shape
+    positions, cu_q = step.positions, step.cu_q
+    if nq <= 0 or nq % nkv or width != nq * d or out.shape != q.shape or positions.numel() != T or cu_q.numel() != S + 1:
         raise KernelError("kv4_attention: queries, output, step and block table do not agree")
-    _need(step.positions, "kv4_attention positions", torch.int32); _need(step.cu_q, "kv4_attention offsets", torch.int32)
+    _kv4_ints("kv4_attention positions and offsets", positions, cu_q)
     if sink is not None:
         _need(sink, "kv4_attention sink", torch.float32)
         if sink.numel() != nq:
             raise KernelError("kv4_attention: one sink logit per query head")
     if T == 0:
         return
-    window, max_blocks, device, code = window or 0, block_table.shape[1], q.device, _code(q)
+    window, device, code = window or 0, q.device, _code(q)
     at, to, held = q.data_ptr(), out.data_ptr(), cache.data_ptr()
     sinks = None if sink is None else sink.data_ptr()
     if d not in KV4_ROWS_HEADS or (at | to | held) % 16:
         _need(step.seq_of_token, "kv4_attention sequence indices", torch.int32)
-        _call("attention_kv4", "ilb_kv4_attention_simple", at, to, code, held, step.positions.data_ptr(), step.seq_of_token.data_ptr(),
-              block_table.data_ptr(), max_blocks, page_size, num_pages, window, scale, T, nq, nkv, d, nq * d, nq * d, sinks, _raw_stream(q))
+        _call("attention_kv4", "ilb_kv4_attention_simple", at, to, code, held, positions.data_ptr(), step.seq_of_token.data_ptr(),
+              block_table.data_ptr(), max_blocks, page_size, num_pages, window, scale, T, nq, nkv, d, width, width, sinks, _raw_stream(q))
         return
     ws = _kv4_workspace(device) if workspace is None else workspace
     most, sms = 1 if step.decode_only else max(step.h_q_len), _sm_count(device)
     key = (code, S, most, nq, nkv, d, max_blocks, page_size, sms)
     plan = _KV4_PLANS.get(key)
     if plan is None:
-        lib, found = load_module("attention_kv4"), (ctypes.c_int(), ctypes.c_int(), ctypes.c_longlong(), ctypes.c_longlong())
+        lib, found = load_module("attention_kv4"), (ctypes.c_int(), ctypes.c_int(), ctypes.c_int(), ctypes.c_longlong(), ctypes.c_longlong())
         if lib.ilb_kv4_attention_rows_plan(*map(_i, key), *map(ctypes.byref, found)) != 0:
             raise KernelError(lib.ilb_last_error().decode())
-        plan = _KV4_PLANS[key] = (found[2].value, found[3].value)
-    scratch = ws.buffer("kv4.records", (plan[0],), torch.float32)
-    tickets = ws.zeroed("kv4.tickets", (max(plan[1], 4096),), torch.int32)
-    _call("attention_kv4", "ilb_kv4_attention_rows", at, to, code, held, step.positions.data_ptr(), step.cu_q.data_ptr(), block_table.data_ptr(),
-          max_blocks, page_size, num_pages, window, scale, S, most, nq, nkv, d, nq * d, nq * d, sinks, sms, scratch.data_ptr(), scratch.numel(),
-          tickets.data_ptr(), tickets.numel(), _tc_state(device).error.data_ptr(), _raw_stream(q))
+        plan = _KV4_PLANS[key] = (found[3].value, found[4].value)
+    scratch = tickets = None
+    if plan[0]:
+        scratch = ws.buffer("kv4.records", (plan[0],), torch.float32).data_ptr()
+        tickets = ws.zeroed("kv4.tickets", (max(plan[1], 4096),), torch.int32).data_ptr()
+    _call("attention_kv4", "ilb_kv4_attention_rows", at, to, code, held, positions.data_ptr(), cu_q.data_ptr(), block_table.data_ptr(),
+          max_blocks, page_size, num_pages, window, scale, S, most, nq, nkv, d, width, width, sinks, sms, scratch, plan[0], tickets, plan[1],
+          _tc_state(device).error.data_ptr(), _raw_stream(q))
 
 
 DECODE_FUSED_ENABLED = True     # tests switch it off to run q/k norm + rotation + cache write as a launch of its own
