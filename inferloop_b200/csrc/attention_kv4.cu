@@ -4,8 +4,9 @@
 // A token that sees no key gets zeros.
 //
 // Few rows against many keys (`rows_kernel`).  A row is a (token, query head of the group); 8 NB rows of a (sequence, kv head) are a block
-// of the launch, whose keys are shared out over `splits` CTAs and there over warps, a unit of 16 keys at a time.  A unit is one piece of
-// 18 D bytes of the cache: a warp keeps kStages of them on their way to its own ring in shared memory by bulk copies.
+// of the launch, whose keys are shared out over `splits` CTAs and there over warps, two units of 16 keys at a time (one at a time took a
+// quarter more instructions a key).  A unit is one piece of 18 D bytes of the cache: a warp keeps kStages pairs of them on their way to its
+// own ring in shared memory by bulk copies, so nothing but the merge at the end crosses from warp to warp.
 //   scores   S^T = K Q^T on m16n8k16, the 16 keys as rows, so that groups of up to 8 query heads fill the 8 columns.  In fp16, where one
 //            AND-OR in place makes an exact number of a code c + 8: 1024 + c + 8 from the last bits of the mantissa, 64 + c + 8 from the
 //            four before them.  The sums of a group of 32 elements start at minus what the offsets 1032 and 72 will add (a bare subtraction
@@ -36,8 +37,8 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ------------------------------------------------------------------ few rows, many keys
-constexpr int kStages = 4;
-constexpr int kMinUnits = 2;                // units a warp should have before another CTA joins
+constexpr int kStages = 2;                  // pairs of units in a warp's ring
+constexpr int kMinPairs = 1;                // pairs a warp should have before another CTA joins
 constexpr int kMaxSplits = 148;             // CTAs that share a block's keys at most
 
 struct Params {
@@ -58,10 +59,15 @@ __device__ __forceinline__ uint32_t turned(uint32_t x) {            // an 8 x 8 
 }
 // Codes of nibbles 0 .. 3 of both halves of w (`w8` = w >> 8) as fp16 numbers: 1024 + code from nibbles 0 and 2, 64 + code from 1 and 3;
 // less 1032 and 72 the codes' c.
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {      // (x & mask) | bits, in one instruction
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+  return y;
+}
 template <int I>
 __device__ __forceinline__ uint32_t offset_pair(uint32_t w, uint32_t w8) {
   const uint32_t x = I < 2 ? w : w8;
-  return I % 2 == 0 ? (x & 0x000f000fu) | 0x64006400u : (x & 0x00f000f0u) | 0x54005400u;
+  return I % 2 == 0 ? and_or(x, 0x000f000fu, 0x64006400u) : and_or(x, 0x00f000f0u, 0x54005400u);
 }
 template <int I>
 __device__ __forceinline__ uint32_t half_pair(uint32_t w, uint32_t w8) {
@@ -78,15 +84,8 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// c += a b of fp16 numbers
-__device__ __forceinline__ void mma_half(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 // 136 + c of two codes as bfloat16 numbers, and c
-__device__ __forceinline__ uint32_t raised(uint32_t w, int nibble) { return ((w >> (4 * nibble)) & 0x000f000fu) | 0x43004300u; }
+__device__ __forceinline__ uint32_t raised(uint32_t w, int nibble) { return and_or(w >> (4 * nibble), 0x000f000fu, 0x43004300u); }
 __device__ __forceinline__ uint32_t plain_pair(uint32_t r) {
   const uint32_t c136 = 0x43084308u;
   const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&r), *reinterpret_cast<const __nv_bfloat162*>(&c136));
@@ -94,44 +93,77 @@ __device__ __forceinline__ uint32_t plain_pair(uint32_t r) {
 }
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-// d = a b + c of fp16 numbers
-__device__ __forceinline__ void mma_half(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+// c += a b of fp16 numbers; d = a b of fp16 or bfloat16 numbers; d = a b + c
+#define ILB_KV4_MMA "mma.sync.aligned.m16n8k16.row.col.f32."
+__device__ __forceinline__ void mma_half(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(ILB_KV4_MMA "f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// N consecutive words of shared memory from an address that is a multiple of 4 N bytes (of 4 for odd N)
-template <int N>
+__device__ __forceinline__ void mma_half_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(ILB_KV4_MMA "f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_half_onto(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1) {
+  asm volatile(ILB_KV4_MMA "f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1) {
+  asm volatile(ILB_KV4_MMA "bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %4, %5}, {%6, %7}, {%8, %8, %8, %8};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_bf16_more(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1) {
+  asm volatile(ILB_KV4_MMA "bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %4, %5}, {%6, %7}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(b0), "r"(b1));
+}
+// N consecutive words of shared memory from addr + OFF, which is a multiple of 4 N bytes (of 4 for odd N)
+template <int N, int OFF = 0>
 __device__ __forceinline__ void lds(uint32_t addr, uint32_t (&w)[N]) {
-  if constexpr (N % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < N; i += 4)
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "r"(addr + 4 * i));
-  } else if constexpr (N % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < N; i += 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[i]), "=r"(w[i + 1]) : "r"(addr + 4 * i));
+  if constexpr (N == 8) {
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr), "n"(OFF));
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "r"(addr), "n"(OFF + 16));
+  } else if constexpr (N == 4) {
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr), "n"(OFF));
+  } else if constexpr (N == 2) {
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2 + %3];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr), "n"(OFF));
+  } else if constexpr (N == 3) {
+    asm volatile("ld.shared.u32 %0, [%1 + %2];" : "=r"(w[0]) : "r"(addr), "n"(OFF));
+    asm volatile("ld.shared.u32 %0, [%1 + %2];" : "=r"(w[1]) : "r"(addr), "n"(OFF + 4));
+    asm volatile("ld.shared.u32 %0, [%1 + %2];" : "=r"(w[2]) : "r"(addr), "n"(OFF + 8));
   } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(addr + 4 * i));
+    static_assert(N == 1, "words of a lane");
+    asm volatile("ld.shared.u32 %0, [%1 + %2];" : "=r"(w[0]) : "r"(addr), "n"(OFF));
   }
 }
-// The bfloat16 scales of a token's groups, as 32-bit numbers
+// The bfloat16 scales of a token's N groups: pairs as they lie, a last odd one in the upper half of a word.
 template <int N>
-__device__ __forceinline__ void lds_scales(uint32_t addr, float (&s)[N]) {
-  if constexpr (N % 2 == 0) {
-    uint32_t w[N / 2];
-    lds(addr, w);
+struct Scales {
+  uint32_t w[(N + 1) / 2];
+  template <int OFF>
+  __device__ __forceinline__ void load(uint32_t addr) {
+    if constexpr (N % 2 == 0) lds<N / 2, OFF>(addr, w);
+    else {
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) { s[2 * i] = bf_lo(w[i]); s[2 * i + 1] = bf_hi(w[i]); }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      uint16_t h;
-      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(addr + 2 * i));
-      s[i] = __uint_as_float((uint32_t)h << 16);
+      for (int i = 0; i < (N + 1) / 2; ++i) {
+        uint16_t a = 0, b = 0;
+        asm volatile("ld.shared.u16 %0, [%1 + %2];" : "=h"(a) : "r"(addr + 4 * i), "n"(OFF));
+        if (2 * i + 1 < N) asm volatile("ld.shared.u16 %0, [%1 + %2];" : "=h"(b) : "r"(addr + 4 * i), "n"(OFF + 2));
+        w[i] = (uint32_t)a | (uint32_t)b << 16;
+      }
     }
   }
+  __device__ __forceinline__ float operator[](int i) const { return i & 1 ? bf_hi(w[i / 2]) : bf_lo(w[i / 2]); }
+  __device__ __forceinline__ void drop() {
+#pragma unroll
+    for (int i = 0; i < (N + 1) / 2; ++i) w[i] = 0u;
+  }
+};
+// The larger of two pairs of bfloat16 numbers, pair by pair (what is no number loses)
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 v = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 // x as the sum of PIECES bfloat16 numbers: element i of the three
 template <int PIECES>
@@ -148,12 +180,12 @@ template <int D, int NB, int PIECES, int kWarps>
 struct Shape {
   static constexpr int kGroups = D / 32, kUnitBytes = 18 * D, kRows = 8 * NB;
   static constexpr int kRecRow = D + 4;                                   // of a record in shared memory: no bank is met twice
-  static constexpr int kRing = kWarps * kStages * kUnitBytes;
+  static constexpr int kRing = kWarps * kStages * 2 * kUnitBytes;
   static constexpr int kRecords = kWarps * kRows * kRecRow * 4;
   static constexpr int kShares = 2 * kMaxSplits * kRows * 4;              // maxima and sums of the records of other CTAs
   static constexpr int kBody = kRing > kRecords ? (kRing > kShares ? kRing : kShares) : (kRecords > kShares ? kRecords : kShares);      // one after the other
   static constexpr int kQ = PIECES > 1 ? kGroups * 4 * PIECES * 32 * 4 : 0;      // 32-bit queries: their pieces in operand order
-  static constexpr int kStats = 3 * kWarps * kRows * 4 + 2 * kRows * 4;
+  static constexpr int kStats = 3 * kWarps * kRows * 4 + 4 * kRows * 4;
   static constexpr int kSmem = kBody + kQ + kStats + kWarps * kStages * 8 + 16;
 };
 
@@ -172,9 +204,10 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
   float* stat_l = stat_m + kWarps * kRows;
   float* factor = stat_l + kWarps * kRows;                                // [warp][row]
   float* row_m = factor + kWarps * kRows;                                 // [row], then the sums
+  int* row_sees = reinterpret_cast<int*>(row_m + 2 * kRows);              // [row]: the first key and, kRows further, the one behind the last
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Sh::kBody + Sh::kQ + Sh::kStats);
   int* flags = reinterpret_cast<int*>(bars + kWarps * kStages);
-  const uint32_t ring = smem_u32(smem) + warp * kStages * U, bar0 = smem_u32(bars + warp * kStages), q_smem = smem_u32(smem) + Sh::kBody;
+  const uint32_t ring = smem_u32(smem) + warp * kStages * 2 * U, bar0 = smem_u32(bars + warp * kStages), q_smem = smem_u32(smem) + Sh::kBody;
 
   pdl_launch_dependents();
   if (lane == 0) {
@@ -192,46 +225,56 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
   const int pos_a = p.positions[tok0 + row0 / G], pos_b = p.positions[tok0 + (row0 + n_rows - 1) / G];
   const int lo_a = first_key(pos_a, p.window), lo_b = first_key(pos_b, p.window);
   const int unit0 = lo_a / kKv4Unit, n_units = pos_b / kKv4Unit + 1 - unit0;
-  int on = (n_units + kWarps * kMinUnits - 1) / (kWarps * kMinUnits);
+  const int n_pairs = (n_units + 1) / 2;
+  int on = (n_pairs + kWarps * kMinPairs - 1) / (kWarps * kMinPairs);
   on = on < 1 ? 1 : on > p.splits ? p.splits : on;                        // CTAs that take part
   if ((int)blockIdx.x >= on) return;
-  const int begin = (int)((long long)n_units * blockIdx.x / on), end = (int)((long long)n_units * (blockIdx.x + 1) / on);
-  const int mine = end - begin > warp ? (end - begin - warp + kWarps - 1) / kWarps : 0;      // units of this warp: begin + warp + i kWarps
+  const int begin = (int)((long long)n_pairs * blockIdx.x / on), end = (int)((long long)n_pairs * (blockIdx.x + 1) / on);
+  const int mine = end - begin > warp ? (end - begin - warp + kWarps - 1) / kWarps : 0;      // pairs of this warp: begin + warp + i kWarps
 
-  // ---- the stream of units: lane l knows where the l-th of every 32 lies
+  // ---- the stream of units: lane 2 i + h knows where unit h of the i-th of every 16 pairs lies
   const int upp = p.page_size / kKv4Unit;
   const int* table = p.block_table + (size_t)seq * p.max_blocks;
-  int where = -1;                                                         // unit in the cache, or -1: not held
+  const uint8_t* src_unit = nullptr;                                      // null: not held
+  uint32_t there_now = 0;                                                 // bit 2 i + h: it is held
   auto look_up = [&](int i0) {
-    const int i = i0 + lane;
-    where = -1;
-    if (i < mine) {
-      const int u = unit0 + begin + warp + i * kWarps, blk = u / upp;
-      const int page = blk < p.max_blocks ? __ldg(table + blk) : -1;
-      if (page >= 0 && page < p.num_pages) where = (page * p.nkv + head) * upp + u % upp;
+    const int i = i0 + (lane >> 1), u = 2 * (begin + warp + i * kWarps) + (lane & 1);
+    src_unit = nullptr;
+    if (i < mine && u < n_units) {
+      const int blk = (unit0 + u) / upp, page = blk < p.max_blocks ? table[blk] : -1;
+      if (page >= 0 && page < p.num_pages) src_unit = p.cache + (((size_t)page * p.nkv + head) * upp + (unit0 + u) % upp) * U;
+    }
+    there_now = __ballot_sync(0xffffffffu, src_unit != nullptr);
+  };
+  uint32_t asked = 0;                                                     // two bits a pair on its way: which of its units come
+  auto ask = [&](int i, int s, int behind) {                              // pair i, one of the 16 looked up, into stage s, behind so many others
+    const uint32_t both = (there_now >> (2 * i & 31)) & 3u;
+    asked |= both << (2 * behind);
+    if ((lane >> 1) == (i & 15)) {                                        // the lanes that know where
+      const uint32_t bar = bar0 + 8 * s;
+      if ((lane & 1) == 0) mbar_expect_tx(bar, ((both & 1u) + (both >> 1)) * U);
+      if (src_unit != nullptr) bulk_load(ring + (2 * s + (lane & 1)) * U, src_unit, U, bar);
     }
   };
-  uint32_t held = 0;                                                      // bit i: the i-th unit of these 32 is held
-  auto ask = [&](int i) {                                                 // (unit i must be one of the 32 looked up)
-    const int at = __shfl_sync(0xffffffffu, where, i & 31);
-    if (at >= 0 && lane == 0) {
-      mbar_expect_tx(bar0 + 8 * (i % kStages), U);
-      bulk_load(ring + (i % kStages) * U, p.cache + (size_t)at * U, U, bar0 + 8 * (i % kStages));
-    }
-    held = (held & ~(1u << (i & 31))) | (at >= 0 ? 1u << (i & 31) : 0u);
-  };
-  if (mine > 0) look_up(0);
+  if (mine > 0) {
+    look_up(0);
 #pragma unroll
-  for (int i = 0; i < kStages; ++i)
-    if (i < mine) ask(i);
+    for (int i = 0; i < kStages; ++i)
+      if (i < mine) ask(i, i, i);
+  }
 
   // ---- queries as second operands, rows g of each block of 8; what the offsets of the keys' operands add to the groups' sums
   constexpr int kQRegs = PIECES == 1 ? NG * 4 : 1;
   uint32_t qf[NB][kQRegs];
-  float init[NB][PIECES == 1 ? NG : 1][2];
-  float base[NB][2], m[NB][2], l[NB][2], mult[NB][2];                     // of columns 2 t, 2 t + 1; mult: what makes a logit in base 2 of a sum
+  constexpr bool kByProduct = PIECES == 1 && NG % 2 == 0;                 // the offsets' share comes as a product with the scales
+  constexpr int kOffMmas = (3 * NG + 15) / 16;                            // slot k of it: piece k / NG of group k % NG
+  uint32_t off[NB][kByProduct ? kOffMmas : 1][2];
+  float init[NB][PIECES == 1 && !kByProduct ? NG : 1][2];
+  // Of columns 2 t, 2 t + 1.  mult: what makes a logit in base 2 of a score; top: a score above it moves the reference point `base`
+  // (`step` above the one that the point was last set by); l: the sum
+  float base[NB][2], top_score[NB][2], step[NB][2], l[NB][2], mult[NB][2];
+  const float sign = p.scale_log2 < 0.f ? -1.f : 1.f;                     // (a negative scale turns the query around, mult stays positive)
   float scale_top = 0.f, scale_exp = 0.f;                                 // fp16: values' scales up to 16 times this need no new exponent; the exponent
-  int row_lo[NB][2], row_hi[NB][2];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const int r = row0 + nb * 8 + g;
@@ -239,6 +282,7 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
     const T* src = reinterpret_cast<const T*>(p.q) + (size_t)(tok0 + (there ? r / G : 0)) * p.q_stride + (size_t)(head * G + (there ? r % G : 0)) * D + 8 * t;
     if constexpr (PIECES == 1) {
       uint4 raw[NG];
+      [[maybe_unused]] float sums[NG];
       uint32_t top = 0;
 #pragma unroll
       for (int G32 = 0; G32 < NG; ++G32) raw[G32] = there ? *reinterpret_cast<const uint4*>(src + G32 * 32) : make_uint4(0u, 0u, 0u, 0u);
@@ -253,7 +297,7 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^-e of the row's largest element's exponent (an infinity or NaN stays one)
       const int e = (int)(top >> 23), up = min(max(254 - e, 1), 253);
-      const float bring = e == 255 ? 1.f : __uint_as_float((uint32_t)up << 23), back = e == 255 ? 1.f : __uint_as_float((uint32_t)(254 - up) << 23);
+      const float bring = sign * (e == 255 ? 1.f : __uint_as_float((uint32_t)up << 23)), back = e == 255 ? 1.f : __uint_as_float((uint32_t)(254 - up) << 23);
 #pragma unroll
       for (int G32 = 0; G32 < NG; ++G32) {
         const uint4 w = raw[G32];
@@ -271,23 +315,40 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
         float sum = fmaf(even, -1032.f, odd * -72.f);
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        init[nb][G32][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
-        init[nb][G32][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+        if constexpr (kByProduct) sums[G32] = sum;
+        else {
+          init[nb][G32][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+          init[nb][G32][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+        }
       }
-      mult[nb][0] = __shfl_sync(0xffffffffu, back, 8 * t) * p.scale_log2;
-      mult[nb][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4) * p.scale_log2;
+      if constexpr (kByProduct) {
+#pragma unroll
+        for (int j = 0; j < kOffMmas; ++j) off[nb][j][0] = off[nb][j][1] = 0u;
+#pragma unroll
+        for (int G32 = 0; G32 < NG; G32 += 2) {
+          uint32_t w[3];
+          split_pair<3>(sums[G32], sums[G32 + 1], w);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {                                   // slots k, k + 1: lane t = k % 8 / 2 of this row holds them
+            const int k = i * NG + G32;
+            if (t == k % 8 / 2) off[nb][k / 16][k % 16 / 8] = w[i];
+          }
+        }
+      }
+      mult[nb][0] = __shfl_sync(0xffffffffu, back, 8 * t) * fabsf(p.scale_log2);
+      mult[nb][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4) * fabsf(p.scale_log2);
     } else {
-      mult[nb][0] = mult[nb][1] = p.scale_log2;
+      mult[nb][0] = mult[nb][1] = fabsf(p.scale_log2);
 #pragma unroll
       for (int G32 = 0; G32 < NG; ++G32) {
         if (warp != 0) break;
         const float4 a = there ? *reinterpret_cast<const float4*>(src + G32 * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
         const float4 b = there ? *reinterpret_cast<const float4*>(src + G32 * 32 + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
         uint32_t w[4][PIECES];
-        split_pair<PIECES>(a.x, b.x, w[0]);
-        split_pair<PIECES>(a.y, b.y, w[1]);
-        split_pair<PIECES>(a.z, b.z, w[2]);
-        split_pair<PIECES>(a.w, b.w, w[3]);
+        split_pair<PIECES>(sign * a.x, sign * b.x, w[0]);
+        split_pair<PIECES>(sign * a.y, sign * b.y, w[1]);
+        split_pair<PIECES>(sign * a.z, sign * b.z, w[2]);
+        split_pair<PIECES>(sign * a.w, sign * b.w, w[3]);
 #pragma unroll
         for (int i = 0; i < PIECES; ++i)
           asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(q_smem + ((G32 * PIECES + i) * 32 + lane) * 16), "r"(w[0][i]), "r"(w[1][i]),
@@ -296,14 +357,17 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const int rc = row0 + nb * 8 + 2 * t + c;
-      const int pos = rc < rows ? p.positions[tok0 + rc / G] : -1;
-      row_hi[nb][c] = pos + 1;
-      row_lo[nb][c] = rc < rows ? first_key(pos, p.window) : 0;
-      base[nb][c] = 0.f; m[nb][c] = -INFINITY; l[nb][c] = 0.f;
+      mult[nb][c] = fmaxf(mult[nb][c], 1e-30f);                           // (a scale of zero: no score is told from another)
+      step[nb][c] = 4.f / mult[nb][c];
+      base[nb][c] = 0.f; top_score[nb][c] = -INFINITY; l[nb][c] = 0.f;
     }
   }
-  if constexpr (PIECES > 1) __syncthreads();
+  if (threadIdx.x < kRows) {
+    const int r = row0 + threadIdx.x, pos = r < rows ? p.positions[tok0 + r / G] : -1;
+    row_sees[threadIdx.x] = r < rows ? first_key(pos, p.window) : 0;
+    row_sees[kRows + threadIdx.x] = pos + 1;
+  }
+  __syncthreads();
   float o[NG * 2][NB][4];
 #pragma unroll
   for (int i = 0; i < NG * 2; ++i)
@@ -312,195 +376,232 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][nb][e] = 0.f;
 
-  // ---- units
-  uint32_t phases = 0;                                                    // bit s: parity of stage s's next completion
+  // ---- pairs of units
   bool ok = true;
-  int failed_at = 0;
+  int stage = 0, failed_at = 0;
+  uint32_t parity = 0;
   for (int i = 0; i < mine; ++i) {
-    const int s = i % kStages;
-    const bool there = (held >> (i & 31)) & 1u;
-    if (there) {
-      if (!__all_sync(0xffffffffu, mbar_wait(bar0 + 8 * s, (phases >> s) & 1u))) { ok = false; failed_at = i; break; }
-      phases ^= 1u << s;
-      const uint32_t unit = ring + s * U;
-      const int key0 = (unit0 + begin + warp + i * kWarps) * kKv4Unit;
-      float sv[NB][4];
-      {
-        uint32_t ka[NG], kb[NG];                                          // words of tokens g and g + 8
-        lds(unit + g * (D / 2) + t * (D / 8), ka);
-        lds(unit + (g + 8) * (D / 2) + t * (D / 8), kb);
-        float sa[NG], sb[NG];
-        lds_scales(unit + 16 * D + g * (D / 16), sa);
-        lds_scales(unit + 16 * D + (g + 8) * (D / 16), sb);
+    if (!__all_sync(0xffffffffu, mbar_try_wait(bar0 + 8 * stage, parity)) && !__all_sync(0xffffffffu, mbar_wait(bar0 + 8 * stage, parity))) {
+      ok = false;
+      failed_at = i;
+      break;
+    }
+    const uint32_t both = asked & 3u;
+    asked >>= 2;
+    const uint32_t at = ring + stage * 2 * U, codes = at + lane * (D / 8), scales = at + g * (D / 16);
+    const int key0 = (unit0 + 2 * (begin + warp + i * kWarps)) * kKv4Unit;
+    // every row of the block sees all 32 keys
+    const bool whole = both == 3u && key0 >= lo_b && key0 + 2 * kKv4Unit <= pos_a + 1;
+    float sv[2][NB][4];
+    auto scores = [&](auto unit) {
+      constexpr int H = decltype(unit)::value, BASE = H * U;
+      uint32_t ka[NG], kb[NG];                                            // words of tokens g and g + 8
+      Scales<NG> sa, sb;
+      lds<NG, BASE>(codes, ka);
+      lds<NG, BASE + 4 * D>(codes, kb);
+      sa.template load<BASE + 16 * D>(scales);
+      sb.template load<BASE + 16 * D + D / 2>(scales);
+      if constexpr (kByProduct) {
+        uint32_t wa[1], wb[1];
+        lds<1, BASE + 16 * D>(scales + 4 * (t % (NG / 2)), wa);
+        lds<1, BASE + 16 * D + D / 2>(scales + 4 * (t % (NG / 2)), wb);
 #pragma unroll
-        for (int G32 = 0; G32 < NG; ++G32) {
-          uint32_t a[2][4];
+        for (int nb = 0; nb < NB; ++nb) {
+          mma_bf16_first(sv[H][nb], wa[0], wb[0], off[nb][0][0], off[nb][0][1]);
+#pragma unroll
+          for (int j = 1; j < kOffMmas; ++j) mma_bf16_more(sv[H][nb], wa[0], wb[0], off[nb][j][0], off[nb][j][1]);
+        }
+      }
+#pragma unroll
+      for (int G32 = 0; G32 < NG; ++G32) {
+        uint32_t a[2][4];
+        if constexpr (PIECES == 1) {
+          const uint32_t ka8 = ka[G32] >> 8, kb8 = kb[G32] >> 8;
+          a[0][0] = offset_pair<0>(ka[G32], ka8); a[0][1] = offset_pair<0>(kb[G32], kb8);
+          a[0][2] = offset_pair<1>(ka[G32], ka8); a[0][3] = offset_pair<1>(kb[G32], kb8);
+          a[1][0] = offset_pair<2>(ka[G32], ka8); a[1][1] = offset_pair<2>(kb[G32], kb8);
+          a[1][2] = offset_pair<3>(ka[G32], ka8); a[1][3] = offset_pair<3>(kb[G32], kb8);
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            a[ks][0] = plain_pair(raised(ka[G32], 2 * ks)); a[ks][1] = plain_pair(raised(kb[G32], 2 * ks));
+            a[ks][2] = plain_pair(raised(ka[G32], 2 * ks + 1)); a[ks][3] = plain_pair(raised(kb[G32], 2 * ks + 1));
+          }
+        }
+        const float fa = sa[G32], fb = sb[G32];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          float acc[4];
           if constexpr (PIECES == 1) {
-            const uint32_t ka8 = ka[G32] >> 8, kb8 = kb[G32] >> 8;
-            a[0][0] = offset_pair<0>(ka[G32], ka8); a[0][1] = offset_pair<0>(kb[G32], kb8);
-            a[0][2] = offset_pair<1>(ka[G32], ka8); a[0][3] = offset_pair<1>(kb[G32], kb8);
-            a[1][0] = offset_pair<2>(ka[G32], ka8); a[1][1] = offset_pair<2>(kb[G32], kb8);
-            a[1][2] = offset_pair<3>(ka[G32], ka8); a[1][3] = offset_pair<3>(kb[G32], kb8);
+            if constexpr (kByProduct) mma_half_first(acc, a[0], qf[nb][G32 * 4], qf[nb][G32 * 4 + 1]);
+            else mma_half_onto(acc, a[0], qf[nb][G32 * 4], qf[nb][G32 * 4 + 1], init[nb][G32][0], init[nb][G32][1]);
+            mma_half(acc, a[1], qf[nb][G32 * 4 + 2], qf[nb][G32 * 4 + 3]);
           } else {
+            acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-              a[ks][0] = plain_pair(raised(ka[G32], 2 * ks)); a[ks][1] = plain_pair(raised(kb[G32], 2 * ks));
-              a[ks][2] = plain_pair(raised(ka[G32], 2 * ks + 1)); a[ks][3] = plain_pair(raised(kb[G32], 2 * ks + 1));
+            for (int i3 = PIECES - 1; i3 >= 0; --i3) {                    // the smallest pieces first
+              uint32_t w[4];
+              lds<4>(q_smem + ((G32 * PIECES + i3) * 32 + lane) * 16, w);
+              mma_16816(acc, a[0], w[0], w[1]);
+              mma_16816(acc, a[1], w[2], w[3]);
             }
           }
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            float acc[4];
-            if constexpr (PIECES == 1) {
-              const float c[4] = {init[nb][G32][0], init[nb][G32][1], init[nb][G32][0], init[nb][G32][1]};
-              mma_half(acc, a[0], qf[nb][G32 * 4], qf[nb][G32 * 4 + 1], c);
-              mma_half(acc, a[1], qf[nb][G32 * 4 + 2], qf[nb][G32 * 4 + 3], acc);
-            } else {
-              acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
-#pragma unroll
-              for (int i3 = PIECES - 1; i3 >= 0; --i3) {                  // the smallest pieces first
-                uint32_t w[4];
-                lds(q_smem + ((G32 * PIECES + i3) * 32 + lane) * 16, w);
-                mma_16816(acc, a[0], w[0], w[1]);
-                mma_16816(acc, a[1], w[2], w[3]);
-              }
-            }
-            if (G32 == 0) {
-              sv[nb][0] = sa[0] * acc[0]; sv[nb][1] = sa[0] * acc[1]; sv[nb][2] = sb[0] * acc[2]; sv[nb][3] = sb[0] * acc[3];
-            } else {
-              sv[nb][0] = fmaf(sa[G32], acc[0], sv[nb][0]); sv[nb][1] = fmaf(sa[G32], acc[1], sv[nb][1]);
-              sv[nb][2] = fmaf(sb[G32], acc[2], sv[nb][2]); sv[nb][3] = fmaf(sb[G32], acc[3], sv[nb][3]);
-            }
+          float* x = sv[H][nb];
+          if (G32 == 0 && !kByProduct) {
+            x[0] = fa * acc[0]; x[1] = fa * acc[1]; x[2] = fb * acc[2]; x[3] = fb * acc[3];
+          } else {
+            x[0] = fmaf(fa, acc[0], x[0]); x[1] = fmaf(fa, acc[1], x[1]);
+            x[2] = fmaf(fb, acc[2], x[2]); x[3] = fmaf(fb, acc[3], x[3]);
           }
         }
       }
-      const bool whole = key0 >= lo_b && key0 + kKv4Unit <= pos_a + 1;    // every row of the block sees all 16 keys
-      float va_s[NG], vb_s[NG];                                           // values' scales of tokens g and g + 8
-      lds_scales(unit + 17 * D + g * (D / 16), va_s);
-      lds_scales(unit + 17 * D + (g + 8) * (D / 16), vb_s);
-      bool raise = false;
+    };
+    scores(std::integral_constant<int, 0>{});
+    scores(std::integral_constant<int, 1>{});
+    Scales<NG> vs[2][2];                                                  // values' scales of tokens g and g + 8 of each unit
+    vs[0][0].template load<17 * D>(scales);
+    vs[0][1].template load<17 * D + D / 2>(scales);
+    vs[1][0].template load<U + 17 * D>(scales);
+    vs[1][1].template load<U + 17 * D + D / 2>(scales);
+    if (!whole) {
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sv[nb][e] *= mult[nb][e & 1];
-      }
-      if (!whole) {
-        bool first = false, second = false;
+        for (int half = 0; half < 2; ++half) {
+          const int key = key0 + h * kKv4Unit + half * 8 + g;
+          bool any = false;
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+          for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = key0 + g + (e >> 1) * 8;
-            const bool seen = key >= row_lo[nb][e & 1] && key < row_hi[nb][e & 1];
-            if (!seen) sv[nb][e] = -INFINITY;
-            if (e < 2) first |= seen;
-            else second |= seen;
-          }
-        // (a lane knows two rows of each block; what none of a token's four lanes sees is not looked at)
-        const uint32_t quad = 0xfu << (lane & 28);
-        first = (__ballot_sync(0xffffffffu, first) & quad) != 0;
-        second = (__ballot_sync(0xffffffffu, second) & quad) != 0;
+            for (int c = 0; c < 2; ++c) {
+              const int r = nb * 8 + 2 * t + c;
+              const bool seen = ((both >> h) & 1u) && key >= row_sees[r] && key < row_sees[kRows + r];
+              if (!seen) sv[h][nb][2 * half + c] = -INFINITY;
+              any |= seen;
+            }
+          // (a lane knows two rows of each block; what none of a token's four lanes sees is not looked at)
+          if ((__ballot_sync(0xffffffffu, any) & (0xfu << (lane & 28))) == 0u) vs[h][half].drop();
+        }
+    }
+    bool raise = false;
+    float most = 0.f;
+    if constexpr (PIECES == 1) {
+      uint32_t top = 0u;
 #pragma unroll
-        for (int G32 = 0; G32 < NG; ++G32) { va_s[G32] = first ? va_s[G32] : 0.f; vb_s[G32] = second ? vb_s[G32] : 0.f; }
-      }
-      float most = 0.f;
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int j = 0; j < (NG + 1) / 2; ++j) top = larger(top, vs[h][half].w[j]);
+      most = fmaxf(bf_lo(top), bf_hi(top));
+      raise = most > 16.f * scale_top;
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        raise |= fmaxf(fmaxf(sv[0][nb][c], sv[0][nb][c + 2]), fmaxf(sv[1][nb][c], sv[1][nb][c + 2])) > top_score[nb][c];
+    if (__any_sync(0xffffffffu, raise)) {
       if constexpr (PIECES == 1) {
-#pragma unroll
-        for (int G32 = 0; G32 < NG; ++G32) most = fmaxf(most, fmaxf(va_s[G32], vb_s[G32]));
-        raise = most > 16.f * scale_top;
+        most = warp_max(most);
+        if (most > scale_top) {
+          scale_top = most;
+          scale_exp = fmaxf((float)((int)(__float_as_uint(most) >> 23) - 127), -100.f) - 6.f;
+        }
       }
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
-        raise |= fmaxf(sv[nb][0], sv[nb][2]) > m[nb][0] + 4.f || fmaxf(sv[nb][1], sv[nb][3]) > m[nb][1] + 4.f;
-      if (__any_sync(0xffffffffu, raise)) {
-        if constexpr (PIECES == 1) {
-          most = warp_max(most);
-          if (most > scale_top) {
-            scale_top = most;
-            scale_exp = fmaxf((float)((int)(__float_as_uint(most) >> 23) - 127), -100.f) - 6.f;
-          }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float mx = fmaxf(fmaxf(sv[0][nb][c], sv[0][nb][c + 2]), fmaxf(sv[1][nb][c], sv[1][nb][c + 2]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float m_old = top_score[nb][c] - step[nb][c], m_new = fmaxf(m_old, mx), b_new = m_new == -INFINITY ? 0.f : fmaf(m_new, mult[nb][c], scale_exp);
+          const float corr = m_old == -INFINITY ? (l[nb][c] == 0.f ? 0.f : 1.f) : exp2f(base[nb][c] - b_new);
+          base[nb][c] = b_new;
+          top_score[nb][c] = m_new + step[nb][c];
+          l[nb][c] *= corr;
+#pragma unroll
+          for (int d = 0; d < NG * 2; ++d) { o[d][nb][c] *= corr; o[d][nb][c + 2] *= corr; }
         }
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float mx = fmaxf(sv[nb][c], sv[nb][c + 2]);
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            const float m_new = fmaxf(m[nb][c], mx), b_new = m_new == -INFINITY ? 0.f : m_new + scale_exp;
-            const float corr = m[nb][c] == -INFINITY ? (l[nb][c] == 0.f ? 0.f : 1.f) : exp2f(base[nb][c] - b_new);
-            base[nb][c] = b_new;
-            m[nb][c] = m_new;
-            l[nb][c] *= corr;
-#pragma unroll
-            for (int d = 0; d < NG * 2; ++d) { o[d][nb][c] *= corr; o[d][nb][c + 2] *= corr; }
-          }
-      }
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sv[nb][e] = ex2(sv[nb][e] - base[nb][e & 1]);
-        l[nb][0] += sv[nb][0] + sv[nb][2];
-        l[nb][1] += sv[nb][1] + sv[nb][3];
-      }
-      auto values = [&](auto masked) {
-        uint32_t va[NG], vb[NG];                                          // tokens 2 t, 2 t + 1 and 2 t + 8, 2 t + 9: half-words of the groups
-        lds(unit + 8 * D + lane * (D / 8), va);
-        lds(unit + 12 * D + lane * (D / 8), vb);
-#pragma unroll
-        for (int G32 = 0; G32 < NG; ++G32) {
-          // half-word i of an array of NG words: the even token's groups come first, then the odd one's
-          constexpr auto half_sel = [](int even, int odd) { return (uint32_t)((even & 1 ? 0x32 : 0x10) | (odd & 1 ? 0x7600 : 0x5400)); };
-          const uint32_t wa = __byte_perm(va[G32 / 2], va[(NG + G32) / 2], half_sel(G32, NG + G32));
-          const uint32_t wb = __byte_perm(vb[G32 / 2], vb[(NG + G32) / 2], half_sel(G32, NG + G32));
-          uint32_t a[2][4];
-          if constexpr (PIECES == 1) {
-            const uint32_t wa8 = wa >> 8, wb8 = wb >> 8;
-            a[0][0] = half_pair<0>(wa, wa8); a[0][1] = half_pair<1>(wa, wa8); a[0][2] = half_pair<0>(wb, wb8); a[0][3] = half_pair<1>(wb, wb8);
-            a[1][0] = half_pair<2>(wa, wa8); a[1][1] = half_pair<3>(wa, wa8); a[1][2] = half_pair<2>(wb, wb8); a[1][3] = half_pair<3>(wb, wb8);
-          } else {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              a[h][0] = plain_pair(raised(wa, 2 * h)); a[h][1] = plain_pair(raised(wa, 2 * h + 1));
-              a[h][2] = plain_pair(raised(wb, 2 * h)); a[h][3] = plain_pair(raised(wb, 2 * h + 1));
-            }
-          }
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            float w[4] = {sv[nb][0] * va_s[G32], sv[nb][1] * va_s[G32], sv[nb][2] * vb_s[G32], sv[nb][3] * vb_s[G32]};
-            if constexpr (decltype(masked)::value) {                      // what a row does not see adds nothing, whatever its scale is
-#pragma unroll
-              for (int e = 0; e < 4; ++e) w[e] = sv[nb][e] == 0.f ? 0.f : w[e];
-            }
-            if constexpr (PIECES == 1) {
-              const uint32_t x0 = turned(pack_half(w[0], w[1])), x1 = turned(pack_half(w[2], w[3]));
-              mma_half(o[2 * G32][nb], a[0], x0, x1);
-              mma_half(o[2 * G32 + 1][nb], a[1], x0, x1);
-            } else {
-              uint32_t b0[PIECES], b1[PIECES];
-              split_pair<PIECES>(w[0], w[1], b0);
-              split_pair<PIECES>(w[2], w[3], b1);
-#pragma unroll
-              for (int i3 = PIECES - 1; i3 >= 0; --i3) {
-                const uint32_t x0 = turned(b0[i3]), x1 = turned(b1[i3]);
-                mma_16816(o[2 * G32][nb], a[0], x0, x1);
-                mma_16816(o[2 * G32 + 1][nb], a[1], x0, x1);
-              }
-            }
-          }
-        }
-      };
-      if (whole) values(std::false_type{});
-      else values(std::true_type{});
-      __syncwarp();                                                       // every lane is done with the stage
     }
-    if (((i + kStages) & 31) == 0) look_up(i + kStages);
-    if (i + kStages < mine) ask(i + kStages);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sv[h][nb][e] = ex2(fmaf(sv[h][nb][e], mult[nb][e & 1], -base[nb][e & 1]));
+#pragma unroll
+      for (int c = 0; c < 2; ++c) l[nb][c] += (sv[0][nb][c] + sv[0][nb][c + 2]) + (sv[1][nb][c] + sv[1][nb][c + 2]);
+    }
+    auto values = [&](auto unit, auto masked) {
+      constexpr int H = decltype(unit)::value, BASE = H * U;
+      uint32_t va[NG], vb[NG];                                            // tokens 2 t, 2 t + 1 and 2 t + 8, 2 t + 9: half-words of the groups
+      lds<NG, BASE + 8 * D>(codes, va);
+      lds<NG, BASE + 12 * D>(codes, vb);
+#pragma unroll
+      for (int G32 = 0; G32 < NG; ++G32) {
+        // half-word i of an array of NG words: the even token's groups come first, then the odd one's
+        constexpr auto half_sel = [](int even, int odd) { return (uint32_t)((even & 1 ? 0x32 : 0x10) | (odd & 1 ? 0x7600 : 0x5400)); };
+        const uint32_t wa = __byte_perm(va[G32 / 2], va[(NG + G32) / 2], half_sel(G32, NG + G32));
+        const uint32_t wb = __byte_perm(vb[G32 / 2], vb[(NG + G32) / 2], half_sel(G32, NG + G32));
+        uint32_t a[2][4];
+        if constexpr (PIECES == 1) {
+          const uint32_t wa8 = wa >> 8, wb8 = wb >> 8;
+          a[0][0] = half_pair<0>(wa, wa8); a[0][1] = half_pair<1>(wa, wa8); a[0][2] = half_pair<0>(wb, wb8); a[0][3] = half_pair<1>(wb, wb8);
+          a[1][0] = half_pair<2>(wa, wa8); a[1][1] = half_pair<3>(wa, wa8); a[1][2] = half_pair<2>(wb, wb8); a[1][3] = half_pair<3>(wb, wb8);
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            a[h][0] = plain_pair(raised(wa, 2 * h)); a[h][1] = plain_pair(raised(wa, 2 * h + 1));
+            a[h][2] = plain_pair(raised(wb, 2 * h)); a[h][3] = plain_pair(raised(wb, 2 * h + 1));
+          }
+        }
+        const float fa = vs[H][0][G32], fb = vs[H][1][G32];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const float* x = sv[H][nb];
+          float w[4] = {x[0] * fa, x[1] * fa, x[2] * fb, x[3] * fb};
+          if constexpr (decltype(masked)::value) {                        // what a row does not see adds nothing, whatever its scale is
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = x[e] == 0.f ? 0.f : w[e];
+          }
+          if constexpr (PIECES == 1) {
+            const uint32_t x0 = turned(pack_half(w[0], w[1])), x1 = turned(pack_half(w[2], w[3]));
+            mma_half(o[2 * G32][nb], a[0], x0, x1);
+            mma_half(o[2 * G32 + 1][nb], a[1], x0, x1);
+          } else {
+            uint32_t b0[PIECES], b1[PIECES];
+            split_pair<PIECES>(w[0], w[1], b0);
+            split_pair<PIECES>(w[2], w[3], b1);
+#pragma unroll
+            for (int i3 = PIECES - 1; i3 >= 0; --i3) {
+              const uint32_t x0 = turned(b0[i3]), x1 = turned(b1[i3]);
+              mma_16816(o[2 * G32][nb], a[0], x0, x1);
+              mma_16816(o[2 * G32 + 1][nb], a[1], x0, x1);
+            }
+          }
+        }
+      }
+    };
+    if (whole) {
+      values(std::integral_constant<int, 0>{}, std::false_type{});
+      values(std::integral_constant<int, 1>{}, std::false_type{});
+    } else {
+      values(std::integral_constant<int, 0>{}, std::true_type{});
+      values(std::integral_constant<int, 1>{}, std::true_type{});
+    }
+    __syncwarp();                                                         // every lane is done with the stage
+    if (((i + kStages) & 15) == 0) look_up(i + kStages);
+    if (i + kStages < mine) ask(i + kStages, stage, kStages - 1);
+    if (++stage == kStages) { stage = 0; parity ^= 1u; }
   }
   if (!ok) {                                                              // the copies still on their way land before the ring is written over
-    for (int i = failed_at + 1; i < mine && i < failed_at + kStages; ++i)
-      if ((held >> (i & 31)) & 1u) mbar_wait(bar0 + 8 * (i % kStages), (phases >> (i % kStages)) & 1u);
+    for (int i = failed_at + 1; i < mine && i < failed_at + kStages; ++i) {
+      if (++stage == kStages) { stage = 0; parity ^= 1u; }
+      mbar_wait(bar0 + 8 * stage, parity);
+    }
     if (lane == 0 && p.error_flag) *p.error_flag = 1;
   }
 
@@ -515,7 +616,7 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
       sum += __shfl_xor_sync(0xffffffffu, sum, 4);
       sum += __shfl_xor_sync(0xffffffffu, sum, 8);
       sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-      if (g == 0) { stat_m[warp * kRows + r] = m[nb][c] == -INFINITY ? -INFINITY : base[nb][c]; stat_l[warp * kRows + r] = sum; }
+      if (g == 0) { stat_m[warp * kRows + r] = top_score[nb][c] == -INFINITY ? -INFINITY : base[nb][c]; stat_l[warp * kRows + r] = sum; }
       float* dst = rec + (size_t)(warp * kRows + r) * Sh::kRecRow + 4 * g;
 #pragma unroll
       for (int G32 = 0; G32 < NG; ++G32)
@@ -631,6 +732,15 @@ int launch_rows(const Params& p, dim3 grid, int warps, cudaStream_t stream) {
   return warps == 4 ? launch_as<T, D, NB, PIECES, 4>(p, grid, stream) : launch_as<T, D, NB, PIECES, kSmWarps<D, NB>>(p, grid, stream);
 }
 
+template <int D>
+int launch_head(const Params& p, int dtype, bool wide, dim3 grid, int warps, cudaStream_t stream) {
+  if (dtype == kF32) return launch_rows<float, D, 1, 3>(p, grid, warps, stream);
+  if constexpr (D <= 128) {
+    if (wide) return launch_rows<__nv_bfloat16, D, 2, 1>(p, grid, warps, stream);
+  }
+  return launch_rows<__nv_bfloat16, D, 1, 1>(p, grid, warps, stream);
+}
+
 // ------------------------------------------------------------------ any head size
 // One block a (token, query head); a warp takes 32 keys at a time, a lane a key for the scores and every 32nd element of the values.
 constexpr int kSimpleWarps = 4, kMaxHead = 512;
@@ -737,7 +847,7 @@ ILB_EXPORT int ilb_kv4_attention_rows_plan(int dtype, int n_seqs, int max_tokens
   const long long rb = (rows + per - 1) / per, blocks = rb * n_seqs * nkv;
   const int sm_warps = per == 8 && d <= 128 ? 16 : 8, w = warps_per_cta(sm_warps, blocks, sms);
   const long long slots = (long long)sms * (sm_warps / w);                        // CTAs at work at once
-  const long long most = ((long long)max_blocks * page_size / kKv4Unit + w * kMinUnits - 1) / (w * kMinUnits);
+  const long long most = ((long long)max_blocks * page_size / kKv4Unit / 2 + w * kMinPairs) / (w * kMinPairs);
   long long s = blocks > 0 ? slots / blocks : 1;
   s = s < 1 ? 1 : s > most ? most : s;
   s = s > kMaxSplits ? kMaxSplits : s;
@@ -771,19 +881,13 @@ ILB_EXPORT int ilb_kv4_attention_rows(const void* q, void* out, int dtype, const
               nq, nkv, q_stride, out_stride, row_blocks, max_tokens, splits, scale * kLog2e};
   const dim3 grid((unsigned)splits, (unsigned)nkv, (unsigned)(n_seqs * row_blocks));
   const bool wide = rows_per_block(dtype, max_tokens * (nq / nkv), d) == 16;
-#define ILB_KV4_ROWS(SIZE)                                                                       \
-  case SIZE:                                                                                     \
-    if (dtype == kF32) return launch_rows<float, SIZE, 1, 3>(p, grid, warps, stream);            \
-    if (wide) return launch_rows<__nv_bfloat16, SIZE, 2, 1>(p, grid, warps, stream); \
-    return launch_rows<__nv_bfloat16, SIZE, 1, 1>(p, grid, warps, stream);
   switch (d) {
-    ILB_KV4_ROWS(32)
-    ILB_KV4_ROWS(64)
-    ILB_KV4_ROWS(96)
-    ILB_KV4_ROWS(128)
-    ILB_KV4_ROWS(256)
+    case 32: return launch_head<32>(p, dtype, wide, grid, warps, stream);
+    case 64: return launch_head<64>(p, dtype, wide, grid, warps, stream);
+    case 96: return launch_head<96>(p, dtype, wide, grid, warps, stream);
+    case 128: return launch_head<128>(p, dtype, wide, grid, warps, stream);
+    case 256: return launch_head<256>(p, dtype, wide, grid, warps, stream);
   }
-#undef ILB_KV4_ROWS
   return fail("kv4_attention: head size %d", d);
 }
 

@@ -5,6 +5,8 @@ using namespace ilb;
 
 namespace {
 
+// (The pointers are not __restrict__: what an earlier launch may write is read by loads that stay behind the dependency wait.)
+
 template <typename T> __device__ __forceinline__ void load4(const T* p, bool wide, float (&x)[4]);
 template <> __device__ __forceinline__ void load4(const __nv_bfloat16* p, bool wide, float (&x)[4]) {
   if (wide) {
@@ -36,9 +38,9 @@ constexpr int kThreads = 128;
 // Eight lanes a group of 32 elements: maximum over them, four codes each, 16 bits of V or (two lanes together) a word of K.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-kv4_write_kernel(const T* __restrict__ k, long long k_row, long long k_head, const T* __restrict__ v, long long v_row, long long v_head,
-                 bool wide, const int* __restrict__ positions, const int* __restrict__ seq_of_token, const int* __restrict__ block_table,
-                 int max_blocks, int page_size, int num_pages, uint8_t* __restrict__ cache, int n_tokens, int nkv, int d) {
+kv4_write_kernel(const T* k, long long k_row, long long k_head, const T* v, long long v_row, long long v_head,
+                 bool wide, const int* positions, const int* seq_of_token, const int* block_table,
+                 int max_blocks, int page_size, int num_pages, uint8_t* cache, int n_tokens, int nkv, int d) {
   pdl_launch_dependents();
   pdl_wait();
   const int per_row = d / kKv4Group;
@@ -96,9 +98,9 @@ constexpr int kReadThreads = 256, kMaxEntries = 32;
 
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kReadThreads)
-kv4_read_kernel(const uint8_t* __restrict__ cache, const int* __restrict__ block_table, int table_stride, const int* __restrict__ out_table,
-                int n_seqs, int max_blocks, int entries, const int* __restrict__ lengths, int page_size, int num_pages, int out_pages,
-                T* __restrict__ k_out, T* __restrict__ v_out, int nkv, int d_any) {
+kv4_read_kernel(const uint8_t* cache, const int* block_table, int table_stride, const int* out_table,
+                int n_seqs, int max_blocks, int entries, const int* lengths, int page_size, int num_pages, int out_pages,
+                T* k_out, T* v_out, int nkv, int d_any) {
   pdl_launch_dependents();
   pdl_wait();
   __shared__ int from[kMaxEntries], to[kMaxEntries], rows[kMaxEntries];
