@@ -4,9 +4,11 @@
 // A token that sees no key gets zeros.
 //
 // Few rows against many keys (`rows_kernel`).  A row is a (token, query head of the group); 8 NB rows of a (sequence, kv head) are a block
-// of the launch, whose keys are shared out over `splits` CTAs and there over warps, two units of 16 keys at a time (one at a time took a
-// quarter more instructions a key).  A unit is one piece of 18 D bytes of the cache: a warp keeps kStages pairs of them on their way to its
-// own ring in shared memory by bulk copies, so nothing but the merge at the end crosses from warp to warp.
+// of work.  A block's keys are cut into equal runs, one a CTA, none longer than the device's share (`longest_run`): a few blocks fill it, and
+// one long sequence among short ones does not hold the launch up; the CTAs find their runs from the lengths, which the device
+// knows.  In a run a warp takes two units of 16 keys at a time (one at a time took a quarter more instructions a key).  A unit
+// is one piece of 18 D bytes of the cache: a warp keeps kStages pairs of them on their way to its own ring in shared memory by bulk
+// copies, so nothing but the merge at the end crosses from warp to warp.
 //   scores   S^T = K Q^T on m16n8k16, the 16 keys as rows, so that groups of up to 8 query heads fill the 8 columns.  In fp16, where one
 //            AND-OR in place makes an exact number of a code c + 8: 1024 + c + 8 from the last bits of the mantissa, 64 + c + 8 from the
 //            four before them.  The sums of a group of 32 elements start at minus what the offsets 1032 and 72 will add (a bare subtraction
@@ -39,12 +41,16 @@ constexpr float kLog2e = 1.4426950408889634f;
 // ------------------------------------------------------------------ few rows, many keys
 constexpr int kStages = 2;                  // pairs of units in a warp's ring
 constexpr int kMinPairs = 1;                // pairs a warp should have before another CTA joins
-constexpr int kMaxSplits = 148;             // CTAs that share a block's keys at most
+constexpr int kSms = 148;
+constexpr int kMaxCut = 1024;               // (sequence, block of rows) pairs whose keys are cut: so many and more even out by themselves
+constexpr int kFewRecords = 8;              // records that a thread asks for all at once
 
 struct Params {
   const void* q; void* out; const uint8_t* cache; const int* positions; const int* cu_q; const int* block_table; const float* sink;
   float* scratch; int* tickets; int* error_flag;
-  int max_blocks, page_size, num_pages, window, nq, nkv, q_stride, out_stride, row_blocks, max_tokens, splits;
+  int max_blocks, page_size, num_pages, window, nq, nkv, q_stride, out_stride, row_blocks, max_tokens;
+  int single;                              // every sequence brings one token
+  int n_z, slots;                          // (sequence, block of rows) pairs; CTAs at work at once, or 0: a CTA a block
   float scale_log2;
 };
 
@@ -176,21 +182,37 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[PIECE
   }
 }
 
+// Pairs that a run has at most.  Fewer blocks than `slots`: so many that no more CTAs than slots come out, however the lengths lie.  More,
+// or nearly as many: half as much again as the slots' average, so that blocks of about one length stay whole (64 x 1,030 keys in 512 blocks:
+// 25 us, cut in two 33).  At least a pair a warp.
+__device__ __forceinline__ int longest_run(int pairs, int blocks, int slots, int warps) {
+  const int by_average = pairs / 2 >= slots ? (pairs / 2 * 3 + slots - 1) / slots : (pairs * 3 / 2 + slots - 1) / slots;
+  const int by_count = blocks < slots ? (pairs + slots - blocks - 1) / (slots - blocks) : by_average;
+  return max(min(by_average, by_count), kMinPairs * warps);
+}
+// The CTAs that come out at most.
+inline long long most_ctas(long long blocks, long long slots) {
+  const long long by_average = blocks + (2 * slots + 2) / 3;
+  return blocks < slots && slots < by_average ? by_average : blocks < slots ? slots : by_average;
+}
+
+// Warps that an SM has registers for: those of few rows' state (NB = 1 up to D = 128), half as many otherwise.
+template <int D, int NB> constexpr int kSmWarps = NB == 1 && D <= 128 ? 16 : 8;
+
 template <int D, int NB, int PIECES, int kWarps>
 struct Shape {
   static constexpr int kGroups = D / 32, kUnitBytes = 18 * D, kRows = 8 * NB;
   static constexpr int kRecRow = D + 4;                                   // of a record in shared memory: no bank is met twice
   static constexpr int kRing = kWarps * kStages * 2 * kUnitBytes;
   static constexpr int kRecords = kWarps * kRows * kRecRow * 4;
-  static constexpr int kShares = 2 * kMaxSplits * kRows * 4;              // maxima and sums of the records of other CTAs
-  static constexpr int kBody = kRing > kRecords ? (kRing > kShares ? kRing : kShares) : (kRecords > kShares ? kRecords : kShares);      // one after the other
-  static constexpr int kQ = PIECES > 1 ? kGroups * 4 * PIECES * 32 * 4 : 0;      // 32-bit queries: their pieces in operand order
-  static constexpr int kStats = 3 * kWarps * kRows * 4 + 4 * kRows * 4;
+  static constexpr int kSlots = kSms * kSmWarps<D, NB> / kWarps;          // no run is shorter than a slot's share: a block has no more of them
+  static constexpr int kShares = 2 * kSlots * kRows * 4;              // maxima and sums of the records of other CTAs
+  static constexpr int kMerge = kRecords > kShares ? kRecords : kShares, kBody = kRing > kMerge ? kRing : kMerge;      // one after the other
+  // queries in operand order: fp16, with the sums of their offsets and 2^e a row, or 32-bit numbers' pieces
+  static constexpr int kQ = PIECES == 1 ? NB * kGroups * 512 + kRows * (kGroups + 1) * 4 : kGroups * PIECES * 512;
+  static constexpr int kStats = 2 * kWarps * kRows * 4 + 4 * kRows * 4;
   static constexpr int kSmem = kBody + kQ + kStats + kWarps * kStages * 8 + 16;
 };
-
-// Warps that an SM has registers for, and CTAs of so many: few rows' worth of state in NB = 1 up to D = 128, twice that otherwise.
-template <int D, int NB> constexpr int kSmWarps = NB == 1 && D <= 128 ? 16 : 8;
 
 template <typename T, int D, int NB, int PIECES, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_kernel(const Params p) {
@@ -200,10 +222,10 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float* rec = reinterpret_cast<float*>(smem);
-  float* stat_m = reinterpret_cast<float*>(smem + Sh::kBody + Sh::kQ);    // [warp][row]
-  float* stat_l = stat_m + kWarps * kRows;
-  float* factor = stat_l + kWarps * kRows;                                // [warp][row]
-  float* row_m = factor + kWarps * kRows;                                 // [row], then the sums
+  float* q_sums = reinterpret_cast<float*>(smem + Sh::kBody + NB * NG * 512);      // [row][group], then 2^e of the rows
+  float* factor = reinterpret_cast<float*>(smem + Sh::kBody + Sh::kQ);       // [warp][row]: maximum, then factor
+  float* stat_l = factor + kWarps * kRows;
+  float* row_m = stat_l + kWarps * kRows;                                 // [row], then the sums
   int* row_sees = reinterpret_cast<int*>(row_m + 2 * kRows);              // [row]: the first key and, kRows further, the one behind the last
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Sh::kBody + Sh::kQ + Sh::kStats);
   int* flags = reinterpret_cast<int*>(bars + kWarps * kStages);
@@ -217,34 +239,91 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
   __syncwarp();
   pdl_wait();
 
-  const int seq = blockIdx.z / p.row_blocks, rb = blockIdx.z % p.row_blocks, head = blockIdx.y, G = p.nq / p.nkv;
-  const int tok0 = p.cu_q[seq], q_len = p.cu_q[seq + 1] - tok0, rows = q_len * G;
-  if (q_len > p.max_tokens || rb * kRows >= rows) return;
-  const int row0 = rb * kRows, n_rows = min(kRows, rows - row0);
+  const int G = p.nq / p.nkv, upp = p.page_size / kKv4Unit;
+  // A block: its sequence's first token and their number, positions of the first and the last token that has rows in it
+  auto block_of = [&](int z) {
+    const int seq = z / p.row_blocks, row0 = z % p.row_blocks * kRows;
+    if (p.single && p.row_blocks == 1) {                                  // (a step of single tokens: sequence s brings token s)
+      const int pos = p.positions[seq];
+      return make_int4(seq, 1, pos, pos);
+    }
+    int4 b = make_int4(p.cu_q[seq], 0, -1, -1);
+    b.y = p.cu_q[seq + 1] - b.x;
+    if (b.y > p.max_tokens || row0 >= b.y * G) b.y = 0;                   // (not this launch's, or no rows)
+    if (b.y > 0) {
+      b.z = p.positions[b.x + row0 / G];
+      b.w = p.positions[b.x + (min(row0 + kRows, b.y * G) - 1) / G];
+    }
+    return b;
+  };
+  auto pairs_of = [&](int4 b) { return b.y > 0 ? (b.w / kKv4Unit + 2 - first_key(b.z, p.window) / kKv4Unit) / 2 : 0; };
+  // Which block and which run of it: every warp finds out by itself, a lane a block of every 32
+  int z = blockIdx.z, head = blockIdx.y, run = 0, runs = 1, place = 0;    // place: of the block's first record
+  int4 mine4;
+  if (p.slots == 0) mine4 = block_of(z);
+  else if (p.n_z == 1) {
+    mine4 = block_of(z = 0);
+    const int n = pairs_of(mine4);
+    if (n == 0) return;
+    runs = (n + longest_run(n * p.nkv, p.nkv, p.slots, kWarps) - 1) / longest_run(n * p.nkv, p.nkv, p.slots, kWarps);
+    head = blockIdx.x / runs;
+    run = blockIdx.x % runs;
+    place = head * runs;
+    if (head >= p.nkv) return;
+  } else {
+    int total = 0;
+    for (int z0 = lane; z0 < p.n_z; z0 += 32) total += pairs_of(block_of(z0));
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (total == 0) return;
+    const int longest = longest_run(total * p.nkv, p.n_z * p.nkv, p.slots, kWarps);
+    int before = 0;
+    z = -1;
+    for (int z0 = 0; z0 < p.n_z && z < 0; z0 += 32) {
+      const int4 b = z0 + lane < p.n_z ? block_of(z0 + lane) : make_int4(0, 0, -1, -1);
+      const int cuts = (pairs_of(b) + longest - 1) / longest;             // CTAs a head
+      int upto = cuts * p.nkv;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const uint32_t reached = __ballot_sync(0xffffffffu, (int)blockIdx.x < before + upto);
+      if (reached != 0u) {
+        const int at = __ffs(reached) - 1;
+        z = z0 + at;
+        runs = __shfl_sync(0xffffffffu, cuts, at);
+        const int local = (int)blockIdx.x - before - __shfl_sync(0xffffffffu, upto, at) + runs * p.nkv;
+        mine4 = make_int4(__shfl_sync(0xffffffffu, b.x, at), __shfl_sync(0xffffffffu, b.y, at), __shfl_sync(0xffffffffu, b.z, at), __shfl_sync(0xffffffffu, b.w, at));
+        head = local / runs;
+        run = local % runs;
+        place = (int)blockIdx.x - run;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (z < 0) return;
+  }
+  const int n_pairs = pairs_of(mine4), begin = (int)((unsigned)n_pairs * run / runs), end = (int)((unsigned)n_pairs * (run + 1) / runs);
+  if (n_pairs == 0) return;
+  const int seq = z / p.row_blocks, row0 = z % p.row_blocks * kRows, tok0 = mine4.x, rows = mine4.y * G, n_rows = min(kRows, rows - row0);
   // keys that the block's tokens see at all, and those that every one of them sees
-  const int pos_a = p.positions[tok0 + row0 / G], pos_b = p.positions[tok0 + (row0 + n_rows - 1) / G];
-  const int lo_a = first_key(pos_a, p.window), lo_b = first_key(pos_b, p.window);
-  const int unit0 = lo_a / kKv4Unit, n_units = pos_b / kKv4Unit + 1 - unit0;
-  const int n_pairs = (n_units + 1) / 2;
-  int on = (n_pairs + kWarps * kMinPairs - 1) / (kWarps * kMinPairs);
-  on = on < 1 ? 1 : on > p.splits ? p.splits : on;                        // CTAs that take part
-  if ((int)blockIdx.x >= on) return;
-  const int begin = (int)((long long)n_pairs * blockIdx.x / on), end = (int)((long long)n_pairs * (blockIdx.x + 1) / on);
+  const int pos_a = mine4.z, pos_b = mine4.w, lo_b = first_key(pos_b, p.window);
+  const int unit0 = first_key(pos_a, p.window) / kKv4Unit, n_units = pos_b / kKv4Unit + 1 - unit0;
   const int mine = end - begin > warp ? (end - begin - warp + kWarps - 1) / kWarps : 0;      // pairs of this warp: begin + warp + i kWarps
 
   // ---- the stream of units: lane 2 i + h knows where unit h of the i-th of every 16 pairs lies
-  const int upp = p.page_size / kKv4Unit;
   const int* table = p.block_table + (size_t)seq * p.max_blocks;
   const uint8_t* src_unit = nullptr;                                      // null: not held
   uint32_t there_now = 0;                                                 // bit 2 i + h: it is held
-  auto look_up = [&](int i0) {
-    const int i = i0 + (lane >> 1), u = 2 * (begin + warp + i * kWarps) + (lane & 1);
-    src_unit = nullptr;
-    if (i < mine && u < n_units) {
-      const int blk = (unit0 + u) / upp, page = blk < p.max_blocks ? table[blk] : -1;
-      if (page >= 0 && page < p.num_pages) src_unit = p.cache + (((size_t)page * p.nkv + head) * upp + (unit0 + u) % upp) * U;
-    }
-    there_now = __ballot_sync(0xffffffffu, src_unit != nullptr);
+  auto unit_of = [&](int i0) { return 2 * (begin + warp + (i0 + (lane >> 1)) * kWarps) + (lane & 1); };
+  auto page_of = [&](int i0) {                                            // (its load may be waited for later)
+    const int u = unit_of(i0), blk = (unit0 + u) / upp;
+    return i0 + (lane >> 1) < mine && u < n_units && blk < p.max_blocks ? table[blk] : -1;
+  };
+  auto look_up = [&](int i0, int page) {
+    const bool is_held = page >= 0 && page < p.num_pages;
+    src_unit = is_held ? p.cache + (((size_t)page * p.nkv + head) * upp + (unit0 + unit_of(i0)) % upp) * U : nullptr;
+    there_now = __ballot_sync(0xffffffffu, is_held);
   };
   uint32_t asked = 0;                                                     // two bits a pair on its way: which of its units come
   auto ask = [&](int i, int s, int behind) {                              // pair i, one of the 16 looked up, into stage s, behind so many others
@@ -256,118 +335,138 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
       if (src_unit != nullptr) bulk_load(ring + (2 * s + (lane & 1)) * U, src_unit, U, bar);
     }
   };
+  const int first_page = page_of(0);
+
+  // ---- queries as second operands, rows g of each block of 8, made once a CTA (a warp a group of 32 elements) and shared; with them what the
+  // offsets of the keys' operands add to the groups' sums
+  constexpr bool kByProduct = PIECES == 1 && NG % 2 == 0;                 // the offsets' share comes as a product with the scales
+  constexpr int kOffMmas = (3 * NG + 15) / 16;                            // slot k of it: piece k / NG of group k % NG
+  const float sign = p.scale_log2 < 0.f ? -1.f : 1.f;                     // (a negative scale turns the query around, mult stays positive)
+  auto row_at = [&](int nb) {
+    const int r = row0 + nb * 8 + g;
+    return r < rows ? reinterpret_cast<const T*>(p.q) + (size_t)(tok0 + r / G) * p.q_stride + (size_t)(head * G + r % G) * D + 8 * t : nullptr;
+  };
+  constexpr int kItems = (NB * NG + kWarps - 1) / kWarps;
+  uint4 raw[PIECES == 1 ? NG : 1], own[PIECES == 1 ? kItems : 1];
+  if constexpr (PIECES == 1) {
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+      const int item = warp + j * kWarps, nb = item / NG;
+      const T* src = item < NB * NG ? row_at(nb) : nullptr;
+      own[j] = src != nullptr ? *reinterpret_cast<const uint4*>(src + item % NG * 32) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
   if (mine > 0) {
-    look_up(0);
+    look_up(0, first_page);
 #pragma unroll
     for (int i = 0; i < kStages; ++i)
       if (i < mine) ask(i, i, i);
   }
-
-  // ---- queries as second operands, rows g of each block of 8; what the offsets of the keys' operands add to the groups' sums
-  constexpr int kQRegs = PIECES == 1 ? NG * 4 : 1;
-  uint32_t qf[NB][kQRegs];
-  constexpr bool kByProduct = PIECES == 1 && NG % 2 == 0;                 // the offsets' share comes as a product with the scales
-  constexpr int kOffMmas = (3 * NG + 15) / 16;                            // slot k of it: piece k / NG of group k % NG
-  uint32_t off[NB][kByProduct ? kOffMmas : 1][2];
-  float init[NB][PIECES == 1 && !kByProduct ? NG : 1][2];
-  // Of columns 2 t, 2 t + 1.  mult: what makes a logit in base 2 of a score; top: a score above it moves the reference point `base`
-  // (`step` above the one that the point was last set by); l: the sum
-  float base[NB][2], top_score[NB][2], step[NB][2], l[NB][2], mult[NB][2];
-  const float sign = p.scale_log2 < 0.f ? -1.f : 1.f;                     // (a negative scale turns the query around, mult stays positive)
-  float scale_top = 0.f, scale_exp = 0.f;                                 // fp16: values' scales up to 16 times this need no new exponent; the exponent
+  if constexpr (PIECES == 1) {
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int r = row0 + nb * 8 + g;
-    const bool there = r < rows;
-    const T* src = reinterpret_cast<const T*>(p.q) + (size_t)(tok0 + (there ? r / G : 0)) * p.q_stride + (size_t)(head * G + (there ? r % G : 0)) * D + 8 * t;
-    if constexpr (PIECES == 1) {
-      uint4 raw[NG];
-      [[maybe_unused]] float sums[NG];
+    for (int j = 0; j < kItems; ++j) {
+      const int item = warp + j * kWarps, nb = item / NG;
+      if (item >= NB * NG) break;
+      const T* src = row_at(nb);
       uint32_t top = 0;
 #pragma unroll
-      for (int G32 = 0; G32 < NG; ++G32) raw[G32] = there ? *reinterpret_cast<const uint4*>(src + G32 * 32) : make_uint4(0u, 0u, 0u, 0u);
+      for (int G32 = 0; G32 < NG; ++G32) raw[G32] = src != nullptr ? *reinterpret_cast<const uint4*>(src + G32 * 32) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-      for (int G32 = 0; G32 < NG; ++G32)
+      for (int G32 = 0; G32 < NG; ++G32) {
+        const uint32_t w[4] = {raw[G32].x, raw[G32].y, raw[G32].z, raw[G32].w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t w = (&raw[G32].x)[i];
-          top = max(top, max((w & 0x7fffu) << 16, w & 0x7fff0000u));
-        }
+        for (int i = 0; i < 4; ++i) top = max(top, max((w[i] & 0x7fffu) << 16, w[i] & 0x7fff0000u));
+      }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^-e of the row's largest element's exponent (an infinity or NaN stays one)
       const int e = (int)(top >> 23), up = min(max(254 - e, 1), 253);
       const float bring = sign * (e == 255 ? 1.f : __uint_as_float((uint32_t)up << 23)), back = e == 255 ? 1.f : __uint_as_float((uint32_t)(254 - up) << 23);
+      const uint4 w = own[j];
+      const float x[8] = {bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y), bf_lo(w.z), bf_hi(w.z), bf_lo(w.w), bf_hi(w.w)};
+      // the pairs that the key's words hold: elements i and i + 4 of the lane's eight
+      uint32_t pair[4];
+      float even = 0.f, odd = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        pair[i] = pack_half(x[i] * bring, x[i + 4] * bring);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair[i]));
+        if (i % 2 == 0) even += f.x + f.y;
+        else odd += f.x + f.y;
+      }
+      float sum = fmaf(even, -1032.f, odd * -72.f);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(q_smem + (item * 32 + lane) * 16), "r"(pair[0]), "r"(pair[1]), "r"(pair[2]), "r"(pair[3])
+                   : "memory");
+      if (t == 0) {
+        q_sums[(nb * 8 + g) * NG + item % NG] = sum;
+        if (item % NG == 0) q_sums[kRows * NG + nb * 8 + g] = back;
+      }
+    }
+  } else {
+    for (int G32 = warp; G32 < NG; G32 += kWarps) {
+      const T* src = row_at(0);
+      const float4 a = src != nullptr ? *reinterpret_cast<const float4*>(src + G32 * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 b = src != nullptr ? *reinterpret_cast<const float4*>(src + G32 * 32 + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      uint32_t w[4][PIECES];
+      split_pair<PIECES>(sign * a.x, sign * b.x, w[0]);
+      split_pair<PIECES>(sign * a.y, sign * b.y, w[1]);
+      split_pair<PIECES>(sign * a.z, sign * b.z, w[2]);
+      split_pair<PIECES>(sign * a.w, sign * b.w, w[3]);
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(q_smem + ((G32 * PIECES + i) * 32 + lane) * 16), "r"(w[0][i]), "r"(w[1][i]),
+                     "r"(w[2][i]), "r"(w[3][i]) : "memory");
+    }
+  }
+  if (threadIdx.x < kRows) {                                              // (a sequence's tokens follow one another)
+    const int r = row0 + threadIdx.x, pos = r < rows ? pos_a + r / G - row0 / G : -1;
+    row_sees[threadIdx.x] = r < rows ? first_key(pos, p.window) : 0;
+    row_sees[kRows + threadIdx.x] = pos + 1;
+  }
+  __syncthreads();
+  uint32_t qf[NB][PIECES == 1 ? NG * 4 : 1], off[NB][kByProduct ? kOffMmas : 1][2];
+  float init[NB][PIECES == 1 && !kByProduct ? NG : 1][2];
+  // Of columns 2 t, 2 t + 1.  mult: what makes a logit in base 2 of a score; top: a score above it moves the reference point `base`
+  // (`step` above the one that the point was last set by); l: the sum
+  float base[NB][2], top_score[NB][2], step[NB][2], l[NB][2], mult[NB][2];
+  float scale_top = 0.f, scale_exp = 0.f;                                 // fp16: values' scales up to 16 times this need no new exponent; the exponent
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    if constexpr (PIECES == 1) {
 #pragma unroll
       for (int G32 = 0; G32 < NG; ++G32) {
-        const uint4 w = raw[G32];
-        const float x[8] = {bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y), bf_lo(w.z), bf_hi(w.z), bf_lo(w.w), bf_hi(w.w)};
-        // the pairs that the key's words hold: elements i and i + 4 of the lane's eight
-        float even = 0.f, odd = 0.f;
+        uint32_t w[4];
+        lds<4>(q_smem + ((nb * NG + G32) * 32 + lane) * 16, w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t pair = pack_half(x[i] * bring, x[i + 4] * bring);
-          qf[nb][G32 * 4 + i] = pair;
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
-          if (i % 2 == 0) even += f.x + f.y;
-          else odd += f.x + f.y;
-        }
-        float sum = fmaf(even, -1032.f, odd * -72.f);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if constexpr (kByProduct) sums[G32] = sum;
-        else {
-          init[nb][G32][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
-          init[nb][G32][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+        for (int i = 0; i < 4; ++i) qf[nb][G32 * 4 + i] = w[i];
+        if constexpr (!kByProduct) {
+          init[nb][G32][0] = q_sums[(nb * 8 + 2 * t) * NG + G32];
+          init[nb][G32][1] = q_sums[(nb * 8 + 2 * t + 1) * NG + G32];
         }
       }
-      if constexpr (kByProduct) {
+      if constexpr (kByProduct) {                                         // slots k = 2 t + 8 h + 16 j and the next: groups 2 t % NG and the next
+        const float* sums = q_sums + (nb * 8 + g) * NG + 2 * t % NG;
+        uint32_t w[3];
+        split_pair<3>(sums[0], sums[1], w);
 #pragma unroll
-        for (int j = 0; j < kOffMmas; ++j) off[nb][j][0] = off[nb][j][1] = 0u;
+        for (int j = 0; j < kOffMmas; ++j)
 #pragma unroll
-        for (int G32 = 0; G32 < NG; G32 += 2) {
-          uint32_t w[3];
-          split_pair<3>(sums[G32], sums[G32 + 1], w);
-#pragma unroll
-          for (int i = 0; i < 3; ++i) {                                   // slots k, k + 1: lane t = k % 8 / 2 of this row holds them
-            const int k = i * NG + G32;
-            if (t == k % 8 / 2) off[nb][k / 16][k % 16 / 8] = w[i];
+          for (int h = 0; h < 2; ++h) {
+            const int piece = (2 * t + 8 * h + 16 * j) / NG;
+            off[nb][j][h] = piece == 0 ? w[0] : piece == 1 ? w[1] : piece == 2 ? w[2] : 0u;
           }
-        }
-      }
-      mult[nb][0] = __shfl_sync(0xffffffffu, back, 8 * t) * fabsf(p.scale_log2);
-      mult[nb][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4) * fabsf(p.scale_log2);
-    } else {
-      mult[nb][0] = mult[nb][1] = fabsf(p.scale_log2);
-#pragma unroll
-      for (int G32 = 0; G32 < NG; ++G32) {
-        if (warp != 0) break;
-        const float4 a = there ? *reinterpret_cast<const float4*>(src + G32 * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 b = there ? *reinterpret_cast<const float4*>(src + G32 * 32 + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-        uint32_t w[4][PIECES];
-        split_pair<PIECES>(sign * a.x, sign * b.x, w[0]);
-        split_pair<PIECES>(sign * a.y, sign * b.y, w[1]);
-        split_pair<PIECES>(sign * a.z, sign * b.z, w[2]);
-        split_pair<PIECES>(sign * a.w, sign * b.w, w[3]);
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i)
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(q_smem + ((G32 * PIECES + i) * 32 + lane) * 16), "r"(w[0][i]), "r"(w[1][i]),
-                       "r"(w[2][i]), "r"(w[3][i]) : "memory");
       }
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
+      mult[nb][c] = fabsf(p.scale_log2) * (PIECES == 1 ? q_sums[kRows * NG + nb * 8 + 2 * t + c] : 1.f);
       mult[nb][c] = fmaxf(mult[nb][c], 1e-30f);                           // (a scale of zero: no score is told from another)
       step[nb][c] = 4.f / mult[nb][c];
       base[nb][c] = 0.f; top_score[nb][c] = -INFINITY; l[nb][c] = 0.f;
     }
   }
-  if (threadIdx.x < kRows) {
-    const int r = row0 + threadIdx.x, pos = r < rows ? p.positions[tok0 + r / G] : -1;
-    row_sees[threadIdx.x] = r < rows ? first_key(pos, p.window) : 0;
-    row_sees[kRows + threadIdx.x] = pos + 1;
-  }
-  __syncthreads();
   float o[NG * 2][NB][4];
 #pragma unroll
   for (int i = 0; i < NG * 2; ++i)
@@ -593,7 +692,7 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
       values(std::integral_constant<int, 1>{}, std::true_type{});
     }
     __syncwarp();                                                         // every lane is done with the stage
-    if (((i + kStages) & 15) == 0) look_up(i + kStages);
+    if (((i + kStages) & 15) == 0) look_up(i + kStages, page_of(i + kStages));
     if (i + kStages < mine) ask(i + kStages, stage, kStages - 1);
     if (++stage == kStages) { stage = 0; parity ^= 1u; }
   }
@@ -616,7 +715,7 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
       sum += __shfl_xor_sync(0xffffffffu, sum, 4);
       sum += __shfl_xor_sync(0xffffffffu, sum, 8);
       sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-      if (g == 0) { stat_m[warp * kRows + r] = top_score[nb][c] == -INFINITY ? -INFINITY : base[nb][c]; stat_l[warp * kRows + r] = sum; }
+      if (g == 0) { factor[warp * kRows + r] = top_score[nb][c] == -INFINITY ? -INFINITY : base[nb][c]; stat_l[warp * kRows + r] = sum; }
       float* dst = rec + (size_t)(warp * kRows + r) * Sh::kRecRow + 4 * g;
 #pragma unroll
       for (int G32 = 0; G32 < NG; ++G32)
@@ -631,23 +730,28 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
     else *reinterpret_cast<float4*>(dst) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
   };
   auto sink_of = [&](int r) { return p.sink != nullptr ? p.sink[head * G + (row0 + r) % G] * kLog2e : -INFINITY; };
-  const bool alone = on == 1;
-  if (threadIdx.x < kRows) {
-    const int r = threadIdx.x;
-    const float sink = alone && r < n_rows ? sink_of(r) : -INFINITY;
-    float top = sink;
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stat_m[w * kRows + r]);
-    float total = sink == -INFINITY ? 0.f : exp2f(sink - top);
-    for (int w = 0; w < kWarps; ++w) {
-      const float mw = stat_m[w * kRows + r], f = mw == -INFINITY ? (stat_l[w * kRows + r] == 0.f ? 0.f : 1.f) : exp2f(mw - top);
-      factor[w * kRows + r] = f;
-      total = fmaf(stat_l[w * kRows + r], f, total);
+  const bool alone = runs == 1;
+  // (kWarps lanes a row: the maximum, the factors and the sum by exchange)
+  if (threadIdx.x < kRows * kWarps) {
+    const int r = threadIdx.x / kWarps, w = threadIdx.x % kWarps;
+    const float mw = factor[w * kRows + r], lw = stat_l[w * kRows + r], sink = alone && r < n_rows ? sink_of(r) : -INFINITY;
+    float top = fmaxf(sink, mw);
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float f = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : exp2f(mw - top);
+    float sum = lw * f;
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    factor[w * kRows + r] = f;
+    if (w == 0) {
+      row_m[r] = top;
+      row_m[kRows + r] = sum + (sink == -INFINITY ? 0.f : exp2f(sink - top));
     }
-    row_m[r] = top;
-    row_m[kRows + r] = total;
   }
   __syncthreads();
-  const size_t place = ((size_t)blockIdx.z * p.nkv + head) * p.splits;    // records of this block of rows
+  constexpr size_t kRecord = (size_t)kRows * (D + 4);
+  float* first_record = p.scratch + (size_t)place * kRecord;              // of the block's runs, one behind the other
+  float* record = first_record + (size_t)run * kRecord;
   constexpr int kQuads = D / 4;
   for (int at = threadIdx.x; at < n_rows * kQuads; at += kThreads) {
     const int r = at / kQuads, d4 = at % kQuads;
@@ -659,57 +763,83 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
       v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
     }
     if (alone) write_row(r, d4, v, row_m[kRows + r]);
-    else __stcg(reinterpret_cast<float4*>(p.scratch + ((place + blockIdx.x) * kRows + r) * (D + 4) + 4 * d4), v);
+    else __stcg(reinterpret_cast<float4*>(record + (size_t)r * (D + 4) + 4 * d4), v);
   }
   if (alone) return;
   // ---- merge: CTAs
   if (threadIdx.x < n_rows)
-    __stcg(reinterpret_cast<float2*>(p.scratch + ((place + blockIdx.x) * kRows + threadIdx.x) * (D + 4) + D),
-           make_float2(row_m[threadIdx.x], row_m[kRows + threadIdx.x]));
-  __threadfence();
+    __stcg(reinterpret_cast<float2*>(record + (size_t)threadIdx.x * (D + 4) + D), make_float2(row_m[threadIdx.x], row_m[kRows + threadIdx.x]));
   __syncthreads();
-  int* ticket = p.tickets + (size_t)blockIdx.z * p.nkv + head;
   if (threadIdx.x == 0) {
+    __threadfence();                                                      // (for all of the CTA's writes, which the barrier put before it)
+    int* ticket = p.tickets + (size_t)z * p.nkv + head;
     const int n = atomicAdd(ticket, 1);
-    flags[0] = n == on - 1;
-    if (n == on - 1) *ticket = 0;                                         // (zero between launches)
+    flags[0] = n == runs - 1;
+    if (n == runs - 1) *ticket = 0;                                       // (zero between launches)
+    __threadfence();
   }
   __syncthreads();
   if (!flags[0]) return;
-  __threadfence();
-  // (factors of all records first, side by side; the records then come many loads at a time)
-  const float* first = p.scratch + place * kRows * (D + 4);
-  constexpr size_t kStep = (size_t)kRows * (D + 4);
-  float* shares = rec;                                                    // [record][row]
-  for (int at = threadIdx.x; at < on * kRows; at += kThreads) {
-    const float2 ml = __ldcg(reinterpret_cast<const float2*>(first + (size_t)at * (D + 4) + D));
-    shares[2 * at] = ml.x;
-    shares[2 * at + 1] = ml.y;
+  auto share_of = [&](float2 ml, float top) { return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2f(ml.x - top); };
+  if (runs <= kFewRecords) {                                              // one wait for everything, in the order of the runs
+    for (int at = threadIdx.x; at < n_rows * kQuads; at += kThreads) {
+      const int r = at / kQuads, d4 = at % kQuads;
+      const float* src = first_record + (size_t)r * (D + 4);
+      float2 ml[kFewRecords];
+      float4 x[kFewRecords];
+#pragma unroll
+      for (int c = 0; c < kFewRecords; ++c) {
+        const bool there = c < runs;
+        ml[c] = there ? __ldcg(reinterpret_cast<const float2*>(src + c * kRecord + D)) : make_float2(-INFINITY, 0.f);
+        x[c] = there ? __ldcg(reinterpret_cast<const float4*>(src + c * kRecord + 4 * d4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      const float sink = sink_of(r);
+      float top = sink;
+#pragma unroll
+      for (int c = 0; c < kFewRecords; ++c) top = fmaxf(top, ml[c].x);
+      float sum = sink == -INFINITY ? 0.f : exp2f(sink - top);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < kFewRecords; ++c) {
+        const float f = share_of(ml[c], top);
+        sum = fmaf(ml[c].y, f, sum);
+        v.x = fmaf(x[c].x, f, v.x); v.y = fmaf(x[c].y, f, v.y); v.z = fmaf(x[c].z, f, v.z); v.w = fmaf(x[c].w, f, v.w);
+      }
+      write_row(r, d4, v, sum);
+    }
+    return;
   }
-  __syncthreads();
-  if (threadIdx.x < n_rows) {
-    const int r = threadIdx.x;
+  // (more of them: a row's shares by a warp first, then the records many loads at a time)
+  float* shares = rec;                                                    // [row][record]
+  for (int r = warp; r < n_rows; r += kWarps) {
     const float sink = sink_of(r);
     float top = sink;
-    for (int c = 0; c < on; ++c) top = fmaxf(top, shares[2 * (c * kRows + r)]);
-    float total = sink == -INFINITY ? 0.f : exp2f(sink - top);
-    for (int c = 0; c < on; ++c) {                                        // in the order of the CTAs, whoever came last
-      const float mc = shares[2 * (c * kRows + r)], lc = shares[2 * (c * kRows + r) + 1];
-      const float f = mc == -INFINITY ? (lc == 0.f ? 0.f : 1.f) : exp2f(mc - top);
-      shares[2 * (c * kRows + r)] = f;
-      total = fmaf(lc, f, total);
+    for (int c = lane; c < runs; c += 32) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(first_record + c * kRecord + (size_t)r * (D + 4) + D));
+      shares[2 * (r * runs + c)] = ml.x;
+      shares[2 * (r * runs + c) + 1] = ml.y;
+      top = fmaxf(top, ml.x);
     }
-    row_m[kRows + r] = total;
+    top = warp_max(top);
+    float sum = 0.f;
+    for (int c = lane; c < runs; c += 32) {
+      const float2 ml = make_float2(shares[2 * (r * runs + c)], shares[2 * (r * runs + c) + 1]);
+      const float f = share_of(ml, top);
+      shares[2 * (r * runs + c)] = f;
+      sum = fmaf(ml.y, f, sum);
+    }
+    sum = warp_sum(sum);                                                  // (an order that depends on the runs' number alone)
+    if (lane == 0) row_m[kRows + r] = sum + (sink == -INFINITY ? 0.f : exp2f(sink - top));
   }
   __syncthreads();
   for (int at = threadIdx.x; at < n_rows * kQuads; at += kThreads) {
     const int r = at / kQuads, d4 = at % kQuads;
-    const float* src = first + (size_t)r * (D + 4) + 4 * d4;
+    const float* src = first_record + (size_t)r * (D + 4) + 4 * d4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-    for (int c = 0; c < on; ++c) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(src + c * kStep));
-      const float f = shares[2 * (c * kRows + r)];
+    for (int c = 0; c < runs; ++c) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(src + c * kRecord));
+      const float f = shares[2 * (r * runs + c)];
       v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
     }
     write_row(r, d4, v, row_m[kRows + r]);
@@ -721,7 +851,7 @@ int launch_as(const Params& p, dim3 grid, cudaStream_t stream) {
   static OncePerDevice once;
   auto kernel = rows_kernel<T, D, NB, PIECES, kWarps>;
   constexpr int smem = Shape<D, NB, PIECES, kWarps>::kSmem;
-  static_assert(kSmWarps<D, NB> / kWarps * (smem + 1024) <= 228 * 1024, "the CTAs of an SM do not fit its shared memory");
+  static_assert(kSmWarps<D, NB> / kWarps * (smem + 1024) <= 228 * 1024 && smem <= 227 * 1024, "the CTAs of an SM do not fit its shared memory");
   const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
   if (e != cudaSuccess) return fail("kv4_attention: %s", cudaGetErrorString(e));
   ilb::launch(kernel, grid, dim3(kWarps * 32), smem, stream, p);
@@ -834,59 +964,61 @@ static int rows_per_block(int dtype, int rows, int d) { return dtype == kF32 || 
 // Head sizes that the kernel of few rows takes.
 static bool rows_head(int d) { return d == 32 || d == 64 || d == 96 || d == 128 || d == 256; }
 
-// Warps of a CTA: blocks that fill the device by themselves get small CTAs, several to an SM; fewer blocks are shared out over CTAs of
-// a whole SM each, so that fewer records have to meet.
-static int warps_per_cta(int sm_warps, long long blocks, int sms) { return blocks > sms ? 4 : sm_warps; }
+struct Plan { int row_blocks, n_z, warps, slots, ctas; long long scratch, tickets; };
 
-// Blocks of rows of sequences that bring up to `max_tokens` tokens, CTAs that may share a block's keys, and floats of scratch and tickets
-// that the launch needs.
-ILB_EXPORT int ilb_kv4_attention_rows_plan(int dtype, int n_seqs, int max_tokens, int nq, int nkv, int d, int max_blocks, int page_size, int sms,
-                                           int* row_blocks, int* splits, int* warps, long long* scratch, long long* tickets) {
+// Blocks that fill the device by themselves get CTAs of four warps, several to an SM; fewer blocks, whose keys more CTAs share, CTAs of a
+// whole SM each, so that fewer records have to meet (2 x 16,000 keys: 31 us with four warps, 21 with 16).
+static int make_plan(Plan* pl, int dtype, int n_seqs, int max_tokens, int nq, int nkv, int d, int sms) {
   ILB_REQUIRE(n_seqs >= 0 && max_tokens > 0 && nkv > 0 && nq > 0 && nq % nkv == 0 && sms > 0 && rows_head(d), "kv4_attention: bad sizes");
   const int rows = max_tokens * (nq / nkv), per = rows_per_block(dtype, rows, d);
-  const long long rb = (rows + per - 1) / per, blocks = rb * n_seqs * nkv;
-  const int sm_warps = per == 8 && d <= 128 ? 16 : 8, w = warps_per_cta(sm_warps, blocks, sms);
-  const long long slots = (long long)sms * (sm_warps / w);                        // CTAs at work at once
-  const long long most = ((long long)max_blocks * page_size / kKv4Unit / 2 + w * kMinPairs) / (w * kMinPairs);
-  long long s = blocks > 0 ? slots / blocks : 1;
-  s = s < 1 ? 1 : s > most ? most : s;
-  s = s > kMaxSplits ? kMaxSplits : s;
-  *row_blocks = (int)rb;
-  *splits = (int)s;
-  *warps = w;
-  *scratch = s > 1 ? blocks * s * per * (d + 4) : 0;
-  *tickets = s > 1 ? blocks : 0;
+  const long long rb = (rows + per - 1) / per, n_z = rb * n_seqs;
+  ILB_REQUIRE(n_z <= 65535 && nkv <= 65535, "kv4_attention: %d sequences of %lld blocks of rows are too many for one launch", n_seqs, rb);
+  const int sm_warps = per == 8 && d <= 128 ? 16 : 8;
+  pl->row_blocks = (int)rb;
+  pl->n_z = (int)n_z;
+  pl->warps = n_z * nkv > sms ? 4 : sm_warps;
+  pl->slots = (sms < kSms ? sms : kSms) * (sm_warps / pl->warps);
+  if (n_z >= kMaxCut || (rb > 1 && n_z * nkv >= 2 * pl->slots)) pl->slots = 0;      // (blocks of rows of one portion are of about one length)
+  pl->ctas = (int)most_ctas(n_z * nkv, pl->slots);
+  pl->scratch = pl->slots > 0 ? (long long)pl->ctas * per * (d + 4) : 0;
+  pl->tickets = pl->slots > 0 ? n_z * nkv : 0;
+  return 0;
+}
+
+// Floats of scratch and tickets (zero between launches) that a launch over sequences of up to `max_tokens` tokens needs.
+ILB_EXPORT int ilb_kv4_attention_rows_plan(int dtype, int n_seqs, int max_tokens, int nq, int nkv, int d, int sms, long long* scratch,
+                                           long long* tickets) {
+  Plan pl;
+  if (int rc = make_plan(&pl, dtype, n_seqs, max_tokens, nq, nkv, d, sms)) return rc;
+  *scratch = pl.scratch;
+  *tickets = pl.tickets;
   return 0;
 }
 
 ILB_EXPORT int ilb_kv4_attention_rows(const void* q, void* out, int dtype, const void* cache, const int* positions, const int* cu_q,
                                       const int* block_table, int max_blocks, int page_size, int num_pages, int window, float scale, int n_seqs,
-                                      int max_tokens, int nq, int nkv, int d, int q_stride, int out_stride, const float* sink, int sms, float* scratch,
+                                      int max_tokens, int single, int nq, int nkv, int d, int q_stride, int out_stride, const float* sink, int sms, float* scratch,
                                       long long scratch_floats, int* tickets, long long n_tickets, int* error_flag, cudaStream_t stream) {
   ILB_REQUIRE(page_size > 0 && page_size % kKv4Unit == 0 && num_pages > 0 && max_blocks > 0, "kv4_attention: bad cache geometry");
   ILB_REQUIRE(dtype == kF32 || dtype == kBF16, "kv4_attention: unknown element type");
-  int row_blocks = 0, splits = 0, warps = 0;
-  long long need = 0, need_tickets = 0;
-  if (int rc = ilb_kv4_attention_rows_plan(dtype, n_seqs, max_tokens, nq, nkv, d, max_blocks, page_size, sms, &row_blocks, &splits, &warps, &need,
-                                           &need_tickets))
-    return rc;
-  ILB_REQUIRE(need <= scratch_floats && need_tickets <= n_tickets, "kv4_attention: the scratch holds %lld floats and %lld tickets, %lld and %lld are needed",
-              scratch_floats, n_tickets, need, need_tickets);
-  ILB_REQUIRE((long long)n_seqs * row_blocks <= 65535 && nkv <= 65535, "kv4_attention: %d sequences of %d blocks of rows are too many for one launch",
-              n_seqs, row_blocks);
+  Plan pl;
+  if (int rc = make_plan(&pl, dtype, n_seqs, max_tokens, nq, nkv, d, sms)) return rc;
+  ILB_REQUIRE(!single || max_tokens == 1, "kv4_attention: a step of single tokens brings one each");
+  ILB_REQUIRE(pl.scratch <= scratch_floats && pl.tickets <= n_tickets, "kv4_attention: the scratch holds %lld floats and %lld tickets, %lld and %lld are needed",
+              scratch_floats, n_tickets, pl.scratch, pl.tickets);
   ILB_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)scratch) % 16 == 0 && q_stride % 8 == 0 && out_stride % 8 == 0,
               "kv4_attention: queries, output, cache and scratch must start on 16-byte boundaries");
   if (n_seqs == 0) return 0;
   Params p = {q, out, (const uint8_t*)cache, positions, cu_q, block_table, sink, scratch, tickets, error_flag, max_blocks, page_size, num_pages, window,
-              nq, nkv, q_stride, out_stride, row_blocks, max_tokens, splits, scale * kLog2e};
-  const dim3 grid((unsigned)splits, (unsigned)nkv, (unsigned)(n_seqs * row_blocks));
+              nq, nkv, q_stride, out_stride, pl.row_blocks, max_tokens, single, pl.n_z, pl.slots, scale * kLog2e};
+  const dim3 grid = pl.slots > 0 ? dim3((unsigned)pl.ctas) : dim3(1, (unsigned)nkv, (unsigned)pl.n_z);
   const bool wide = rows_per_block(dtype, max_tokens * (nq / nkv), d) == 16;
   switch (d) {
-    case 32: return launch_head<32>(p, dtype, wide, grid, warps, stream);
-    case 64: return launch_head<64>(p, dtype, wide, grid, warps, stream);
-    case 96: return launch_head<96>(p, dtype, wide, grid, warps, stream);
-    case 128: return launch_head<128>(p, dtype, wide, grid, warps, stream);
-    case 256: return launch_head<256>(p, dtype, wide, grid, warps, stream);
+    case 32: return launch_head<32>(p, dtype, wide, grid, pl.warps, stream);
+    case 64: return launch_head<64>(p, dtype, wide, grid, pl.warps, stream);
+    case 96: return launch_head<96>(p, dtype, wide, grid, pl.warps, stream);
+    case 128: return launch_head<128>(p, dtype, wide, grid, pl.warps, stream);
+    case 256: return launch_head<256>(p, dtype, wide, grid, pl.warps, stream);
   }
   return fail("kv4_attention: head size %d", d);
 }

@@ -65,7 +65,7 @@ _SIGNATURES = {
     "ilb_kv4_write": "pqqpqqipppiiipiiip",
     "ilb_kv4_read": "ppipipiiiippiiip",
     "ilb_kv4_attention_simple": "ppippppiiiifiiiiiipp",
-    "ilb_kv4_attention_rows": "ppippppiiiifiiiiiiipipqpqpp",
+    "ilb_kv4_attention_rows": "ppippppiiiifiiiiiiiipipqpqpp",
 }
 _KINDS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "q": ctypes.c_longlong, "f": ctypes.c_float}
 
@@ -1691,16 +1691,18 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, step, block_table: torch.Tensor,
     4-bit cache, each at its token's position; a token whose page is not held is left out.  32 neighbouring elements share the scale
     s = bfloat16(max |x| / 7) and are kept as x / s rounded to -7 .. 7, halves away from zero.  A group with an infinity or NaN
     in it reads back as NaN."""
-    _need(k, "kv4_write keys", contiguous=False); _need(v, "kv4_write values", k.dtype, contiguous=False)
-    if k.dim() != 3 or v.shape != k.shape or (k.numel() and (k.stride(2) != 1 or v.stride(2) != 1)):
+    if v.dtype is not k.dtype or not (k.is_cuda and v.is_cuda):
+        _need(k, "kv4_write keys", contiguous=False); _need(v, "kv4_write values", k.dtype, contiguous=False)
+    shape, ks, vs = k.shape, k.stride(), v.stride()
+    if len(shape) != 3 or v.shape != shape or (k.numel() and (ks[2] != 1 or vs[2] != 1)):
         raise KernelError("kv4_write: keys and values must be [tokens, heads, head size] with a head's elements side by side")
-    T, nkv, d = k.shape
+    T, nkv, d = shape
     num_pages, page_size = _kv4_need("kv4_write", cache, block_table, nkv, d)
     positions, seqs = step.positions, step.seq_of_token
     _kv4_ints("kv4_write positions and sequence indices", positions, seqs)
     if positions.numel() != T or seqs.numel() != T:
         raise KernelError(f"kv4_write: {T} rows for a step of {positions.numel()} tokens")
-    _call("kv4", "ilb_kv4_write", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _code(k),
+    _call("kv4", "ilb_kv4_write", k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _code(k),
           positions.data_ptr(), seqs.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, num_pages, cache.data_ptr(), T, nkv, d,
           _raw_stream(cache))
 
@@ -1710,10 +1712,12 @@ def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tens
     """Pages of the 4-bit cache read back into pages [out pages, nkv, page_size, d] of k_out's type: page b of sequence s, if it
     holds any of the sequence's lengths[s] tokens, goes to page out_table[s, b] (-1: nowhere).  Rows from the length on, and those
     of a page that is not held, are zeros; other pages of the output are left alone."""
-    _need(k_out, "kv4_read keys"); _need(v_out, "kv4_read values", k_out.dtype)
-    if k_out.dim() != 4 or v_out.shape != k_out.shape:
+    if v_out.dtype is not k_out.dtype or not (k_out.is_cuda and v_out.is_cuda and k_out.is_contiguous() and v_out.is_contiguous()):
+        _need(k_out, "kv4_read keys"); _need(v_out, "kv4_read values", k_out.dtype)
+    shape = k_out.shape
+    if len(shape) != 4 or v_out.shape != shape:
         raise KernelError("kv4_read: outputs must be [pages, heads, page size, head size]")
-    out_pages, nkv, ps, d = k_out.shape
+    out_pages, nkv, ps, d = shape
     num_pages, page_size = _kv4_need("kv4_read", cache, block_table, nkv, d)
     _kv4_ints("kv4_read output table and lengths", out_table, lengths)
     if ps != page_size or out_table.shape != block_table.shape or lengths.numel() != block_table.shape[0]:
@@ -1742,11 +1746,14 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
     """Causal attention of the step's tokens over the 4-bit cache; q and out are [T, nq * d] of one type.  `window` and `sink`
     as in `attention`; a token that sees no key (its pages are not held) gets zeros.  Keys of a sequence that are shared out
     over several CTAs meet in `workspace` (None: one of the device's own)."""
-    _need(q, "kv4_attention q"); _need(out, "kv4_attention out", q.dtype)
+    dtype = q.dtype
+    if out.dtype is not dtype or not (q.is_cuda and out.is_cuda and q.is_contiguous() and out.is_contiguous()):
+        _need(q, "kv4_attention q"); _need(out, "kv4_attention out", dtype)
     num_pages, page_size = _kv4_need("kv4_attention", cache, block_table, nkv, d)
-    (T, width), (S, max_blocks) = q.shape, block_table.shape
+    shape, (S, max_blocks) = q.shape, block_table.shape
+    T, width = shape if len(shape) == 2 else (-1, -1)
     positions, cu_q = step.positions, step.cu_q
-    if nq <= 0 or nq % nkv or width != nq * d or out.shape != q.shape or positions.numel() != T or cu_q.numel() != S + 1:
+    if nq <= 0 or nq % nkv or width != nq * d or out.shape != shape or positions.numel() != T or cu_q.numel() != S + 1:
         raise KernelError("kv4_attention: queries, output, step and block table do not agree")
     _kv4_ints("kv4_attention positions and offsets", positions, cu_q)
     if sink is not None:
@@ -1755,7 +1762,7 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
             raise KernelError("kv4_attention: one sink logit per query head")
     if T == 0:
         return
-    window, device, code = window or 0, q.device, _code(q)
+    window, device, code = window or 0, q.device, F32 if dtype is torch.float32 else _code(q)
     at, to, held = q.data_ptr(), out.data_ptr(), cache.data_ptr()
     sinks = None if sink is None else sink.data_ptr()
     if d not in KV4_ROWS_HEADS or (at | to | held) % 16:
@@ -1765,19 +1772,19 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
         return
     ws = _kv4_workspace(device) if workspace is None else workspace
     most, sms = 1 if step.decode_only else max(step.h_q_len), _sm_count(device)
-    key = (code, S, most, nq, nkv, d, max_blocks, page_size, sms)
+    key = (code, S, most, nq, nkv, d, sms)
     plan = _KV4_PLANS.get(key)
     if plan is None:
-        lib, found = load_module("attention_kv4"), (ctypes.c_int(), ctypes.c_int(), ctypes.c_int(), ctypes.c_longlong(), ctypes.c_longlong())
+        lib, found = load_module("attention_kv4"), (ctypes.c_longlong(), ctypes.c_longlong())
         if lib.ilb_kv4_attention_rows_plan(*map(_i, key), *map(ctypes.byref, found)) != 0:
             raise KernelError(lib.ilb_last_error().decode())
-        plan = _KV4_PLANS[key] = (found[3].value, found[4].value)
+        plan = _KV4_PLANS[key] = (found[0].value, found[1].value)
     scratch = tickets = None
     if plan[0]:
-        scratch = ws.buffer("kv4.records", (plan[0],), torch.float32).data_ptr()
-        tickets = ws.zeroed("kv4.tickets", (max(plan[1], 4096),), torch.int32).data_ptr()
+        scratch = ws.address("kv4.records", plan[0], torch.float32)
+        tickets = ws.address("kv4.tickets", max(plan[1], 4096), torch.int32, True)
     _call("attention_kv4", "ilb_kv4_attention_rows", at, to, code, held, positions.data_ptr(), cu_q.data_ptr(), block_table.data_ptr(),
-          max_blocks, page_size, num_pages, window, scale, S, most, nq, nkv, d, width, width, sinks, sms, scratch, plan[0], tickets, plan[1],
+          max_blocks, page_size, num_pages, window, scale, S, most, 1 if step.decode_only else 0, nq, nkv, d, width, width, sinks, sms, scratch, plan[0], tickets, plan[1],
           _tc_state(device).error.data_ptr(), _raw_stream(q))
 
 
