@@ -35,12 +35,17 @@
 // head size (DV) than keys, and with `turn` every head's output is turned back in pairs
 // (i, i + DV / 2) by its position's angle as it is written.
 //
+// HALF: operands in fp16 that were brought into its range by powers of two (a 4-bit cache read back exactly, kv4.cu): queries a row,
+// keys and values a tile of 128 keys.  A row's scores get its and the tile's powers back with the scale; the values' power joins the
+// exponents, so that P V comes out in one unit, and leaves the row sum again.  Keys whose page is not held are not seen.
+//
 // Reference counterparts: the query-tile prefill kernel on MMAs
 // (crates/backend/cuda-kernels/src/tile/attention/resident_attention_prefill_kernels.rs:378-469)
 // and the CuTe-generated sm_100a artifact that the reference ships for another geometry only
 // (crates/backend/cuda/kernels/fa4-attention/README.md:30-34).  Formula:
 // crates/testing/cpu/reference-ops/src/kernels.rs:251-297.
 #include <cuda.h>
+#include <cuda_fp16.h>
 #include <math.h>
 #include <mutex>
 #include <unordered_map>
@@ -72,9 +77,9 @@ __device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, uint32_t mn_gro
   return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)((mn_group_bytes >> 4) & 0x3FFF) << 16) |
          ((uint64_t)((k_group_bytes >> 4) & 0x3FFF) << 32) | (1ull << 46) | (2ull << 61);
 }
-// D 32-bit, A bfloat16 K-major, B bfloat16 K-major or MN-major.
-__host__ __device__ constexpr uint32_t instr_desc(int mma_m, int mma_n, int b_mn_major) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(mma_n >> 3) << 17) |
+// D 32-bit, A bfloat16 (or, both, fp16) K-major, B K-major or MN-major.
+__host__ __device__ constexpr uint32_t instr_desc(int mma_m, int mma_n, int b_mn_major, bool half = false) {
+  return (1u << 4) | (half ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(mma_n >> 3) << 17) |
          ((uint32_t)(mma_m >> 4) << 24);
 }
 __device__ __forceinline__ void tmem_store_32(uint32_t addr, const float (&v)[32]) {
@@ -149,6 +154,8 @@ struct Params {
   const float2* turn;                             // POOL: [tokens][DV / 2] (cos, sin), or null
   int skip_single;       // sequences that bring one token are somebody else's (the decode kernel's)
   const float* sink;     // [nq] or null: a logit per query head that joins the softmax's denominator unscaled, without a value
+  // HALF: [sequence][tile][kv head] 2^e of the keys, e of the values, 2^-e of the values, a bit for every 16 keys that are held; [token][nq] 2^e of the queries
+  const float4* tile_info; const float* q_power;
 };
 
 // QB = row blocks of a CTA.  Measured on this part (one thread issuing, operands in place): a
@@ -162,7 +169,7 @@ struct Params {
 //   every K and V tile that comes in; tensor memory holds one S buffer and O per block (4 x
 //   128 columns), scores are issued one tile ahead, and while one block's warps work on a
 //   tile the tensor core works for the other block.
-template <int D, int DV, int QB, bool POOL>
+template <int D, int DV, int QB, bool POOL, bool HALF>
 __global__ void __launch_bounds__(64 + 256 * QB)
 prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_k_run,
@@ -364,8 +371,8 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     // (One lane issues.  Having the whole warp walk this loop with lane 0 predicated, so that
     // the operands could stay in uniform registers, was measured and was slower.)
     if (lane == 0) {
-      constexpr uint32_t idesc_s = instr_desc(kRows, KS, 0);
-      constexpr uint32_t idesc_o = instr_desc(kRows, DV, 1);
+      constexpr uint32_t idesc_s = instr_desc(kRows, KS, 0, HALF);
+      constexpr uint32_t idesc_o = instr_desc(kRows, DV, 1, HALF);
       bool ok = mbar_wait(q_full, 0);
       // scores of (block q, score tile u) = Q_q K^T over the tile's KS keys, into their S buffer
       auto issue_s = [&](int q, int u) {
@@ -456,6 +463,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const int row_pooled = POOL ? lo / p.pool : 0;     // pooled rows this row sees
     constexpr int kOCols = DV / 2;                     // columns of O this thread owns
     float m_used = -1e30f, l = 0.f;
+    const float row_scale = HALF && live ? p.scale_log2 * p.q_power[(size_t)(tok0 + tl) * p.nq + head] : p.scale_log2;
     bool ok = true;
     auto block_sync = [&]() {                           // the 256 threads of this row block
       if (q == 0) asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -467,6 +475,15 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const int see_lo = in_pool ? 0 : lo, see_hi = in_pool ? row_pooled - 1 : pos;      // what this row sees of the tile's set of keys
       const int t = s_buf(q, u);
       const uint32_t s_t = s_cols(q, u) + lane_addr;     // this row of the S buffer
+      float scale = row_scale, v_exp = 0.f, v_back = 1.f;
+      uint32_t held = 0xfu;                               // this thread's 64 keys
+      if constexpr (HALF) {
+        const float4 info = p.tile_info[((size_t)seq * p.max_blocks + first_tile + u) * p.nkv + kvh];
+        scale = row_scale * info.x;
+        v_exp = info.y;
+        v_back = info.z;
+        held = (__float_as_uint(info.w) >> (4 * half)) & 0xfu;
+      }
       // `ok` only ever changes through waits that all 256 threads of the block share, so they
       // leave the loop together and nobody is left alone at the named barrier below
       if (!mbar_wait(s_full + 8 * t, s_use(u) & 1)) ok = false;
@@ -479,12 +496,12 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       // raw scores stay in v (the scale is positive and folds into the exponent's multiply-add);
       // keys this row may not see become -inf; the maximum is taken in log2 units, in four
       // chains so that no instruction waits for the one before it
-      const bool all_visible = key0 + E - 1 <= see_hi && key0 >= see_lo;
+      const bool all_visible = key0 + E - 1 <= see_hi && key0 >= see_lo && (!HALF || held == 0xfu);
       if (!all_visible) {
 #pragma unroll
         for (int c = 0; c < E; ++c) {
           const int key = key0 + c;
-          v[c] = (key <= see_hi && key >= see_lo) ? v[c] : -INFINITY;
+          v[c] = (key <= see_hi && key >= see_lo && (!HALF || ((held >> (c / 16)) & 1u))) ? v[c] : -INFINITY;
         }
       }
       float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -493,7 +510,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 #pragma unroll
         for (int i = 0; i < 4; ++i) m4[i] = fmaxf(m4[i], v[c + i]);
       }
-      float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
+      float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale + v_exp;
       xmax[(u & 1) * 256 + half * 128 + row] = mx;
       // (this barrier also separates every thread's reads of S from the other half's writes of P below)
       block_sync();
@@ -505,11 +522,16 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       uint32_t packed[E / 2];
 #pragma unroll
       for (int e = 0; e < E / 2; ++e) {
-        const float e0 = ex2(fmaf(v[2 * e], p.scale_log2, -m_new));
-        const float e1 = ex2(fmaf(v[2 * e + 1], p.scale_log2, -m_new));
+        const float e0 = ex2(fmaf(v[2 * e], scale, v_exp - m_new));
+        const float e1 = ex2(fmaf(v[2 * e + 1], scale, v_exp - m_new));
         sum0 += e0; sum1 += e1;
-        __nv_bfloat162 hh = __floats2bfloat162_rn(e0, e1);
-        packed[e] = *reinterpret_cast<uint32_t*>(&hh);
+        if constexpr (HALF) {
+          __half2 hh = __floats2half2_rn(e0, e1);
+          packed[e] = *reinterpret_cast<uint32_t*>(&hh);
+        } else {
+          __nv_bfloat162 hh = __floats2bfloat162_rn(e0, e1);
+          packed[e] = *reinterpret_cast<uint32_t*>(&hh);
+        }
       }
       // O is at rest once the block's previous P V has run (it ran while the exponentials above
       // were taken; waiting for it every tile also keeps this thread's count of the barrier's phases exact)
@@ -531,7 +553,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         l *= corr;
         m_used = m_new;
       }
-      l += sum0 + sum1;
+      l += HALF ? (sum0 + sum1) * v_back : sum0 + sum1;
       // P takes the first KS / 2 columns of the S buffer its scores came from: this thread's
       // keys are columns (E / 2) half .. (E / 2) half + E / 2 - 1
       tmem_store_32u(s_t + half * (E / 2), packed);
@@ -606,16 +628,54 @@ int encode(CUtensorMap* out, const void* ptr, int rank, const cuuint64_t* dims, 
 
 struct Maps { CUtensorMap q, k, v, k_run, v_run, pk, pv; };
 
-template <int D, int DV, int QB, bool POOL>
+// The cache [page][kv head][key][d] as (64 of d, key in its group of 8, slice of the head,
+// group in the page, page x kv head): a box is the whole page of one head and lands as
+// [group][slice][8 keys][64], the operand layout with its groups 1 or 2 KB apart.
+// (The strides are not ascending: the encoder takes that; the coordinates are all zero
+// but the last, so every copy starts on a 16-byte boundary.)
+int page_map(CUtensorMap* out_map, const void* ptr, int hd, int pages, int nkv, int page_size, const char* what) {
+  const cuuint64_t slices = (cuuint64_t)hd / 64, groups = (cuuint64_t)page_size / 8;
+  const cuuint64_t dims[5] = {64, 8, slices, groups, (cuuint64_t)pages * nkv};
+  const cuuint64_t strides[4] = {(cuuint64_t)hd * 2, 128, (cuuint64_t)hd * 2 * 8, (cuuint64_t)hd * 2 * page_size};
+  const cuuint32_t box[5] = {64, 8, (cuuint32_t)slices, (cuuint32_t)groups, 1};
+  return encode(out_map, ptr, 5, dims, strides, box, what);
+}
+// the same with (group in the page, kv head) as one dimension and the page as the last: a
+// box spans half the pages of a 128-key tile when their numbers follow one another
+int run_map(CUtensorMap* out_map, const void* ptr, int hd, int pages, int nkv, int page_size, const char* what) {
+  const cuuint64_t slices = (cuuint64_t)hd / 64, groups = (cuuint64_t)page_size / 8;
+  const cuuint64_t rdims[5] = {64, 8, slices, groups * nkv, (cuuint64_t)pages};
+  const cuuint64_t rstrides[4] = {(cuuint64_t)hd * 2, 128, (cuuint64_t)hd * 2 * 8, (cuuint64_t)hd * 2 * page_size * nkv};
+  const int pages_per_tile = kKeys / page_size;
+  const cuuint32_t run[5] = {64, 8, (cuuint32_t)slices, (cuuint32_t)groups, (cuuint32_t)(pages_per_tile > 1 ? pages_per_tile / 2 : 1)};
+  return encode(out_map, ptr, 5, rdims, rstrides, run, what);
+}
+int make_maps(Maps* m, const void* q, const void* k_cache, const void* v_cache, int n_tokens, int q_stride, int nq, int nkv, int d, int dv, int page_size,
+              int num_pages) {
+  const int G = nq / nkv;
+  {   // q as (d, heads, tokens); a box is 64 x G x floor(128/G) = the rows of a tile, one slice of the head
+    const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)nq, (cuuint64_t)n_tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)q_stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(kRows / G)};
+    if (encode(&m->q, q, 3, dims, strides, box, "q")) return -1;
+  }
+  if (page_map(&m->k, k_cache, d, num_pages, nkv, page_size, "k cache") || page_map(&m->v, v_cache, dv, num_pages, nkv, page_size, "v cache") ||
+      run_map(&m->k_run, k_cache, d, num_pages, nkv, page_size, "k cache (page run)") ||
+      run_map(&m->v_run, v_cache, dv, num_pages, nkv, page_size, "v cache (page run)")) return -1;
+  m->pk = m->k; m->pv = m->v;
+  return 0;
+}
+
+template <int D, int DV, int QB, bool POOL, bool HALF = false>
 int launch(const Maps& m, const Params& p, int n_tiles, cudaStream_t stream) {
   constexpr int kStagesK = stages_k(D, QB), kStagesV = stages_v(D, QB);
   constexpr size_t smem = (size_t)kRows * 128 * (D / 64 * (QB + kStagesK) + DV / 64 * kStagesV) + 1024 +
                           (1 + 2 * kStagesK + 2 * kStagesV + 10 + 2) * 8 + (size_t)QB * 768 * 4;
   static_assert(smem <= 227 * 1024, "tiles do not fit shared memory");
   static OncePerDevice once;
-  if (once.run([&] { return cudaFuncSetAttribute(prefill_tc_kernel<D, DV, QB, POOL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }) != cudaSuccess)
+  if (once.run([&] { return cudaFuncSetAttribute(prefill_tc_kernel<D, DV, QB, POOL, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); }) != cudaSuccess)
     return fail("attention (tensor cores): cannot reserve %zu bytes of shared memory", smem);
-  ilb::launch(prefill_tc_kernel<D, DV, QB, POOL>, dim3(p.nkv, n_tiles), dim3(64 + 256 * QB), smem, stream, m.q, m.k, m.v, m.k_run, m.v_run,
+  ilb::launch(prefill_tc_kernel<D, DV, QB, POOL, HALF>, dim3(p.nkv, n_tiles), dim3(64 + 256 * QB), smem, stream, m.q, m.k, m.v, m.k_run, m.v_run,
               m.pk, m.pv, p);
   return check_launch("attention prefill (tensor cores)");
 }
@@ -650,46 +710,15 @@ ILB_EXPORT int ilb_attention_prefill_tc(const void* q, void* out, const void* k_
               "attention (tensor cores): bad sizes");
   ILB_REQUIRE(q_stride % 8 == 0 && out_stride % 8 == 0 && ((uintptr_t)q % 16 == 0) && ((uintptr_t)out % 16 == 0) &&
               ((uintptr_t)k_cache % 16 == 0) && ((uintptr_t)v_cache % 16 == 0), "attention (tensor cores): misaligned operands");
-  const int G = nq / nkv;
   Maps m;
-  {   // q as (d, heads, tokens); a box is 64 x G x floor(128/G) = the rows of a tile, one slice of the head
-    const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)nq, (cuuint64_t)n_tokens};
-    const cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)q_stride * 2};
-    const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(kRows / G)};
-    if (encode(&m.q, q, 3, dims, strides, box, "q")) return -1;
-  }
-  // The cache [page][kv head][key][d] as (64 of d, key in its group of 8, slice of the head,
-  // group in the page, page x kv head): a box is the whole page of one head and lands as
-  // [group][slice][8 keys][64], the operand layout with its groups 1 or 2 KB apart.
-  // (The strides are not ascending: the encoder takes that; the coordinates are all zero
-  // but the last, so every copy starts on a 16-byte boundary.)
-  auto page_map = [&](CUtensorMap* out_map, const void* ptr, int hd, int pages, const char* what) {
-    const cuuint64_t slices = (cuuint64_t)hd / 64, groups = (cuuint64_t)page_size / 8;
-    const cuuint64_t dims[5] = {64, 8, slices, groups, (cuuint64_t)pages * nkv};
-    const cuuint64_t strides[4] = {(cuuint64_t)hd * 2, 128, (cuuint64_t)hd * 2 * 8, (cuuint64_t)hd * 2 * page_size};
-    const cuuint32_t box[5] = {64, 8, (cuuint32_t)slices, (cuuint32_t)groups, 1};
-    return encode(out_map, ptr, 5, dims, strides, box, what);
-  };
-  // the same with (group in the page, kv head) as one dimension and the page as the last: a
-  // box spans half the pages of a 128-key tile when their numbers follow one another
-  auto run_map = [&](CUtensorMap* out_map, const void* ptr, int hd, const char* what) {
-    const cuuint64_t slices = (cuuint64_t)hd / 64, groups = (cuuint64_t)page_size / 8;
-    const cuuint64_t rdims[5] = {64, 8, slices, groups * nkv, (cuuint64_t)num_pages};
-    const cuuint64_t rstrides[4] = {(cuuint64_t)hd * 2, 128, (cuuint64_t)hd * 2 * 8, (cuuint64_t)hd * 2 * page_size * nkv};
-    const int pages_per_tile = kKeys / page_size;
-    const cuuint32_t run[5] = {64, 8, (cuuint32_t)slices, (cuuint32_t)groups, (cuuint32_t)(pages_per_tile > 1 ? pages_per_tile / 2 : 1)};
-    return encode(out_map, ptr, 5, rdims, rstrides, run, what);
-  };
-  if (page_map(&m.k, k_cache, d, num_pages, "k cache") || page_map(&m.v, v_cache, dv, num_pages, "v cache") ||
-      run_map(&m.k_run, k_cache, d, "k cache (page run)") || run_map(&m.v_run, v_cache, dv, "v cache (page run)")) return -1;
-  m.pk = m.k; m.pv = m.v;
+  if (make_maps(&m, q, k_cache, v_cache, n_tokens, q_stride, nq, nkv, d, dv, page_size, num_pages)) return -1;
   Params p{(__nv_bfloat16*)out, positions, cu_q, block_table, error_flag, max_blocks, n_seqs, nq, nkv, window,
-           out_stride, page_size, num_pages, scale * kLog2e, p_table, p_num_pages, pool, (const float2*)turn, skip_single ? 1 : 0, sink};
+           out_stride, page_size, num_pages, scale * kLog2e, p_table, p_num_pages, pool, (const float2*)turn, skip_single ? 1 : 0, sink, nullptr, nullptr};
   if (pool > 0) {
     ILB_REQUIRE(window > 0 && sink == nullptr && pk_cache != nullptr && pv_cache != nullptr && p_table != nullptr && p_num_pages > 0 &&
                 ((uintptr_t)pk_cache % 16 == 0) && ((uintptr_t)pv_cache % 16 == 0) && ((uintptr_t)turn % 16 == 0),
                 "attention (tensor cores): pooled blocks need a window, no sink, and aligned pages of their own");
-    if (page_map(&m.pk, pk_cache, d, p_num_pages, "pooled keys") || page_map(&m.pv, pv_cache, dv, p_num_pages, "pooled values")) return -1;
+    if (page_map(&m.pk, pk_cache, d, p_num_pages, nkv, page_size, "pooled keys") || page_map(&m.pv, pv_cache, dv, p_num_pages, nkv, page_size, "pooled values")) return -1;
 #define ILB_POOLED(D, DV) \
     if (d == D && dv == DV) return row_blocks == 2 ? launch<D, DV, 2, true>(m, p, n_tiles, stream) : launch<D, DV, 1, true>(m, p, n_tiles, stream)
     ILB_POOLED(64, 64);
@@ -702,6 +731,27 @@ ILB_EXPORT int ilb_attention_prefill_tc(const void* q, void* out, const void* k_
   if (row_blocks == 2)
     return d == 64 ? launch<64, 64, 2, false>(m, p, n_tiles, stream) : launch<128, 128, 2, false>(m, p, n_tiles, stream);
   return d == 64 ? launch<64, 64, 1, false>(m, p, n_tiles, stream) : launch<128, 128, 1, false>(m, p, n_tiles, stream);
+}
+
+// The same over fp16 keys and values in pages of a tile (128 keys) each, page `tile` of sequence s at s * max_tiles + tile, as
+// ilb_kv4_unpack leaves them with `tile_info` [n_seqs][max_tiles][nkv][4], `q_power` [tokens][nq] and the queries q [tokens][nq d]:
+// portions of more than one token, scale > 0.
+ILB_EXPORT int ilb_attention_prefill_half(const void* q, void* out, const void* k, const void* v, const void* tile_info, const float* q_power,
+                                          const int* positions, const int* cu_q, const int* page_order, int max_tiles, int window, float scale,
+                                          int n_tokens, int n_seqs, int n_tiles, int row_blocks, int nq, int nkv, int d, const float* sink,
+                                          int* error_flag, cudaStream_t stream) {
+  ILB_REQUIRE(row_blocks == 1 || row_blocks == 2, "attention (tensor cores): %d row blocks per CTA (1 or 2)", row_blocks);
+  ILB_REQUIRE(ilb_attention_tc_supported(nq, nkv, d, kKeys) && scale > 0.f, "attention (tensor cores): heads %d/%d, head size %d, scale %g are not built",
+              nq, nkv, d, (double)scale);
+  ILB_REQUIRE(n_tokens > 0 && n_seqs > 0 && n_tiles > 0 && n_tiles <= 65535 && max_tiles > 0, "attention (tensor cores): bad sizes");
+  ILB_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)tile_info) % 16) == 0, "attention (tensor cores): misaligned operands");
+  Maps m;
+  if (make_maps(&m, q, k, v, n_tokens, nq * d, nq, nkv, d, d, kKeys, n_seqs * max_tiles)) return -1;
+  Params p{(__nv_bfloat16*)out, positions, cu_q, page_order, error_flag, max_tiles, n_seqs, nq, nkv, window, nq * d, kKeys, n_seqs * max_tiles,
+           scale * kLog2e, nullptr, 0, 0, nullptr, 0, sink, (const float4*)tile_info, q_power};
+  if (row_blocks == 2)
+    return d == 64 ? launch<64, 64, 2, false, true>(m, p, n_tiles, stream) : launch<128, 128, 2, false, true>(m, p, n_tiles, stream);
+  return d == 64 ? launch<64, 64, 1, false, true>(m, p, n_tiles, stream) : launch<128, 128, 1, false, true>(m, p, n_tiles, stream);
 }
 
 ILB_DEFINE_LAST_ERROR()

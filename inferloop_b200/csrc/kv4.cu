@@ -1,4 +1,5 @@
 // Rows into the 4-bit key/value cache and back (format: kv4.cuh).
+#include <cuda_fp16.h>
 #include "kv4.cuh"
 
 using namespace ilb;
@@ -145,6 +146,134 @@ kv4_read_kernel(const uint8_t* cache, const int* block_table, int table_stride, 
   }
 }
 
+// ------------------------------------------------------------------ operands of the prefill attention
+// A portion's keys and values in fp16 for tensor cores that multiply one type: code times scale has 11 significant bits, fp16's, so
+// they are exact once a tile of 128 keys is brought to fp16's range by one power of two for its keys and one for its values (what is
+// 2^-24 of the tile's largest loses bits).  Queries, a row each, likewise: bfloat16's 8 bits are exact.
+// Blocks of kUnpackThreads: first a tile of a head each, then rows of queries, a warp a row.
+constexpr int kTile = 128, kUnpackThreads = 512;
+
+__device__ __forceinline__ uint32_t half_times(uint32_t code_pair, __half2 s) {        // (codes + 1024 as fp16 numbers) -> (code - 8) s
+  const uint32_t c1032 = 0x64086408u;
+  const __half2 v = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&code_pair), *reinterpret_cast<const __half2*>(&c1032)), s);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint4 spread_half(uint32_t w, __half2 s) {
+  uint32_t pair[4];                                                       // elements i and i + 4
+#pragma unroll
+  for (int i = 0; i < 4; ++i) pair[i] = half_times(((w >> (4 * i)) & 0x000f000fu) | 0x64006400u, s);
+  return make_uint4(__byte_perm(pair[0], pair[1], 0x5410), __byte_perm(pair[2], pair[3], 0x5410), __byte_perm(pair[0], pair[1], 0x7632),
+                    __byte_perm(pair[2], pair[3], 0x7632));
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)min(max(e + 127, 1), 254) << 23); }
+
+template <int D>
+__global__ void __launch_bounds__(kUnpackThreads)
+kv4_unpack_kernel(const uint8_t* cache, const int* block_table, int table_stride, const int* lengths, const int* positions, const int* cu_q, int window,
+                  int page_size, int num_pages, int n_seqs, int max_tiles, int nkv, __half* k_out, __half* v_out, float4* info, const __nv_bfloat16* q,
+                  __half* q_out, float* q_power, int nq, int tile_blocks) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int kUnits = kTile / kKv4Unit, NG = D / kKv4Group, U = kv4_unit_bytes(D);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if ((int)blockIdx.x >= tile_blocks) {                                   // ---- queries
+    const int tok0 = cu_q[0], rows = (cu_q[n_seqs] - tok0) * nq;
+    const int row = ((int)blockIdx.x - tile_blocks) * (kUnpackThreads / 32) + warp;
+    if (row >= rows) return;
+    const size_t at = ((size_t)tok0 * nq + row) * D;
+    constexpr int E = D / 32;                                             // elements a lane
+    float x[E];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(q + at + lane * E + i);
+      x[i] = __uint_as_float(w << 16);
+      x[i + 1] = __uint_as_float(w & 0xffff0000u);
+      top = max(top, max((w & 0x7fffu) << 16, w & 0x7fff0000u));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int e = top >= 0x7f800000u ? 0 : max((int)(top >> 23) - 127, -126);
+    const float bring = power_of_two(-e);
+#pragma unroll
+    for (int i = 0; i < E; i += 2) *reinterpret_cast<__half2*>(q_out + at + lane * E + i) = __floats2half2_rn(x[i] * bring, x[i + 1] * bring);
+    if (lane == 0) q_power[(size_t)tok0 * nq + row] = power_of_two(e);
+    return;
+  }
+  // ---- a tile of a head
+  __shared__ int unit_at[kUnits];                                         // in the cache, or -1
+  __shared__ uint32_t top[2][kUnpackThreads / 32];
+  const int head = blockIdx.x % nkv, tile = blockIdx.x / nkv % max_tiles, seq = blockIdx.x / nkv / max_tiles;
+  const int length = lengths[seq], key0 = tile * kTile, first = first_key(positions[cu_q[seq]], window);
+  if (key0 >= length || first >= key0 + kTile) return;                    // (no token of the portion comes near this tile)
+  if (threadIdx.x < 32) {
+    const int key = key0 + (int)threadIdx.x * kKv4Unit;
+    int at = -1;
+    if (threadIdx.x < kUnits && key < length) {
+      const int page = block_table[(size_t)seq * table_stride + key / page_size];
+      if (page >= 0 && page < num_pages) at = (page * nkv + head) * (page_size / kKv4Unit) + key % page_size / kKv4Unit;
+    }
+    if (threadIdx.x < kUnits) unit_at[threadIdx.x] = at;
+  }
+  __syncthreads();
+  const int lo = max(first - key0, 0), hi = min(length - key0, kTile);    // rows that some token sees
+  uint32_t most[2] = {0u, 0u};
+  for (int i = threadIdx.x; i < kTile * NG; i += kUnpackThreads) {
+    const int row = i / NG, at = unit_at[row / kKv4Unit];
+    if (at < 0 || row < lo || row >= hi) continue;
+    const uint8_t* unit = cache + (size_t)at * U;
+#pragma unroll
+    for (int value = 0; value < 2; ++value) {
+      const uint32_t s = *reinterpret_cast<const uint16_t*>(unit + kv4_scale_at(D, value, row % kKv4Unit, i % NG));
+      if (s < 0x7f80u) most[value] = max(most[value], s);
+    }
+  }
+#pragma unroll
+  for (int value = 0; value < 2; ++value) {
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) most[value] = max(most[value], __shfl_xor_sync(0xffffffffu, most[value], o));
+    if (lane == 0) top[value][warp] = most[value];
+  }
+  __syncthreads();
+  int e[2];
+  for (int value = 0; value < 2; ++value) {
+    uint32_t m = 0;
+    for (int w = 0; w < kUnpackThreads / 32; ++w) m = max(m, top[value][w]);
+    e[value] = m == 0u ? 0 : max((int)(m >> 7) - 127, -100) - 10;         // the largest scale comes to 2^10, seven times it below 2^14
+  }
+  const size_t page = (size_t)seq * max_tiles + tile;
+  if (threadIdx.x == 0) {
+    uint32_t held = 0;
+    for (int u = 0; u < kUnits; ++u) held |= unit_at[u] >= 0 ? 1u << u : 0u;
+    info[page * nkv + head] = make_float4(power_of_two(e[0]), (float)e[1], power_of_two(-e[1]), __uint_as_float(held));
+  }
+  const float bring_k = power_of_two(-e[0]), bring_v = power_of_two(-e[1]);
+  const size_t out = (page * nkv + head) * kTile * D;
+  constexpr int kPerRow = D / 8, kItems = kTile * kPerRow / kUnpackThreads;
+  static_assert(kItems * kUnpackThreads == kTile * kPerRow, "eight elements a thread at a time");
+  uint32_t k[kItems], v[kItems], ks[kItems], vs[kItems];
+#pragma unroll
+  for (int n = 0; n < kItems; ++n) {
+    const int i = threadIdx.x + n * kUnpackThreads, row = i / kPerRow, e8 = i % kPerRow, j = row % kKv4Unit, G = e8 >> 2, l = 2 * (e8 & 3), at = unit_at[row / kKv4Unit];
+    k[n] = v[n] = 0x88888888u;
+    ks[n] = vs[n] = 0u;
+    if (at >= 0 && row >= lo && row < hi) {
+      const uint8_t* unit = cache + (size_t)at * U;
+      k[n] = *reinterpret_cast<const uint32_t*>(unit + kv4_key_at(D, j, G, l));
+      v[n] = (uint32_t)*reinterpret_cast<const uint16_t*>(unit + kv4_value_at(D, j, G, l)) |
+             (uint32_t)*reinterpret_cast<const uint16_t*>(unit + kv4_value_at(D, j, G, l + 1)) << 16;
+      ks[n] = *reinterpret_cast<const uint16_t*>(unit + kv4_scale_at(D, false, j, G));
+      vs[n] = *reinterpret_cast<const uint16_t*>(unit + kv4_scale_at(D, true, j, G));
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < kItems; ++n) {
+    const size_t o = out + (size_t)(threadIdx.x + n * kUnpackThreads) * 8;
+    *reinterpret_cast<uint4*>(k_out + o) = spread_half(k[n], __float2half2_rn(__uint_as_float(ks[n] << 16) * bring_k));
+    *reinterpret_cast<uint4*>(v_out + o) = spread_half(v[n], __float2half2_rn(__uint_as_float(vs[n] << 16) * bring_v));
+  }
+}
+
 int check_cache(const char* what, int page_size, int num_pages, int max_blocks, int nkv, int d) {
   ILB_REQUIRE(nkv > 0 && d > 0 && d % kKv4Group == 0 && d <= 512, "%s: head size %d must be a multiple of 32 up to 512, and there must be heads", what, d);
   ILB_REQUIRE(page_size > 0 && page_size % kKv4Unit == 0, "%s: page size %d must be a multiple of 16", what, page_size);
@@ -204,6 +333,28 @@ ILB_EXPORT int ilb_kv4_read(const void* cache, const int* block_table, int table
   }
 #undef ILB_KV4_READ
   return check_launch("kv4_read");
+}
+
+// What ilb_attention_prefill_half reads, for n_seqs sequences (rows of block_table, table_stride apart; lengths [n_seqs]; positions of all
+// tokens; cu_q [n_seqs + 1]): keys and values k, v [n_seqs max_tiles][nkv][128][d], info [n_seqs][max_tiles][nkv][4], and of the queries
+// [tokens][nq d] in bfloat16 those tokens' rows of q_out and q_power [tokens][nq].  n_rows: rows of queries, for the launch.
+ILB_EXPORT int ilb_kv4_unpack(const void* cache, const int* block_table, int table_stride, const int* lengths, const int* positions, const int* cu_q,
+                              int window, int page_size, int num_pages, int n_seqs, int max_tiles, int nkv, int d, void* k, void* v, void* info,
+                              const void* q, void* q_out, float* q_power, int nq, long long n_rows, cudaStream_t stream) {
+  if (int rc = check_cache("kv4_unpack", page_size, num_pages, table_stride, nkv, d)) return rc;
+  ILB_REQUIRE((d == 64 || d == 128) && n_seqs > 0 && max_tiles > 0 && nq > 0 && n_rows >= 0, "kv4_unpack: bad sizes");
+  ILB_REQUIRE((((uintptr_t)cache | (uintptr_t)k | (uintptr_t)v | (uintptr_t)info | (uintptr_t)q | (uintptr_t)q_out) % 16) == 0,
+              "kv4_unpack: operands must start on 16-byte boundaries");
+  const long long tiles = (long long)n_seqs * max_tiles * nkv, blocks = tiles + (n_rows + kUnpackThreads / 32 - 1) / (kUnpackThreads / 32);
+  ILB_REQUIRE(blocks <= 0x7fffffffLL, "kv4_unpack: too much for one launch");
+#define ILB_KV4_UNPACK(DIM)                                                                                                                \
+  ilb::launch(kv4_unpack_kernel<DIM>, dim3((unsigned)blocks), dim3(kUnpackThreads), 0, stream, (const uint8_t*)cache, block_table, table_stride, lengths, \
+              positions, cu_q, window, page_size, num_pages, n_seqs, max_tiles, nkv, (__half*)k, (__half*)v, (float4*)info, (const __nv_bfloat16*)q,      \
+              (__half*)q_out, q_power, nq, (int)tiles)
+  if (d == 64) ILB_KV4_UNPACK(64);
+  else ILB_KV4_UNPACK(128);
+#undef ILB_KV4_UNPACK
+  return check_launch("kv4_unpack");
 }
 
 ILB_DEFINE_LAST_ERROR()

@@ -64,6 +64,8 @@ _FUNCTIONS: dict = {}  # launcher name -> (function, its library)
 _SIGNATURES = {
     "ilb_kv4_write": "pqqpqqipppiiipiiip",
     "ilb_kv4_read": "ppipipiiiippiiip",
+    "ilb_kv4_unpack": "ppippp" + "iiiiiii" + "pppppp" + "iqp",
+    "ilb_attention_prefill_half": "ppppppppp" + "iifiiiiiii" + "ppp",
     "ilb_kv4_attention_simple": "ppippppiiiifiiiiiipp",
     "ilb_kv4_attention_rows": "ppippppiiiifiiiiiiiipipqpqpp",
 }
@@ -1728,6 +1730,10 @@ def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tens
 
 
 KV4_ROWS_HEADS = (32, 64, 96, 128, 256)     # head sizes of the kernel of few rows (others: the simple kernel)
+KV4_PORTION_ROWS = 128      # rows (tokens x query heads of a group) from which a portion's keys and values are unpacked once for the prefill kernel
+KV4_UNPACK_TOKENS = 1 << 16 # tokens whose keys and values are unpacked at a time (more of them: one group of sequences after another)
+KV4_TILE = 128              # keys of a tile of the prefill kernel
+_KV4_ORDER: dict = {}       # 0, 1, 2, .. on each device
 _KV4_WORKSPACE: dict = {}
 _KV4_PLANS: dict = {}      # sizes of a launch -> (floats of scratch, tickets) that it needs
 
@@ -1744,8 +1750,10 @@ def _kv4_workspace(device: torch.device):
 def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step, block_table: torch.Tensor, window: int, scale: float,
                   nq: int, nkv: int, d: int, sink: Optional[torch.Tensor] = None, workspace=None) -> None:
     """Causal attention of the step's tokens over the 4-bit cache; q and out are [T, nq * d] of one type.  `window` and `sink`
-    as in `attention`; a token that sees no key (its pages are not held) gets zeros.  Keys of a sequence that are shared out
-    over several CTAs meet in `workspace` (None: one of the device's own)."""
+    as in `attention`; a token that sees no key (its pages are not held) gets zeros.  Sequences that bring few tokens read the
+    codes themselves; longer portions' keys and values (bfloat16 queries, heads of 64 and 128) are unpacked into `workspace` (None:
+    one of the device's own) for the tensor cores' prefill kernel.  There a value that was kept as NaN reaches every token of its
+    portion that lies in the same tile of 128 keys, as it does with a bfloat16 cache."""
     dtype = q.dtype
     if out.dtype is not dtype or not (q.is_cuda and out.is_cuda and q.is_contiguous() and out.is_contiguous()):
         _need(q, "kv4_attention q"); _need(out, "kv4_attention out", dtype)
@@ -1755,7 +1763,7 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
     positions, cu_q = step.positions, step.cu_q
     if nq <= 0 or nq % nkv or width != nq * d or out.shape != shape or positions.numel() != T or cu_q.numel() != S + 1:
         raise KernelError("kv4_attention: queries, output, step and block table do not agree")
-    _kv4_ints("kv4_attention positions and offsets", positions, cu_q)
+    _kv4_ints("kv4_attention positions, offsets and lengths", positions, cu_q, step.kv_len)
     if sink is not None:
         _need(sink, "kv4_attention sink", torch.float32)
         if sink.numel() != nq:
@@ -1771,7 +1779,28 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
               block_table.data_ptr(), max_blocks, page_size, num_pages, window, scale, T, nq, nkv, d, width, width, sinks, _raw_stream(q))
         return
     ws = _kv4_workspace(device) if workspace is None else workspace
-    most, sms = 1 if step.decode_only else max(step.h_q_len), _sm_count(device)
+    most, sms = 1, _sm_count(device)
+    if not step.decode_only:
+        lens = step.h_q_len
+        most = longest = max(lens)
+        short = max(KV4_PORTION_ROWS // (nq // nkv), 1)
+        if longest > short and dtype is torch.bfloat16 and scale > 0 and attention_tc_supported(nq, nkv, d, KV4_TILE):
+            a = 0
+            while a < S:                                 # runs of neighbouring sequences with long portions, as many as the scratch takes
+                if lens[a] <= short:
+                    a += 1
+                    continue
+                b, tiles = a, 0
+                while b < S and lens[b] > short:
+                    n = max(tiles, -(-step.h_kv_len[b] // KV4_TILE))
+                    if b > a and n * KV4_TILE * (b + 1 - a) > KV4_UNPACK_TOKENS:
+                        break
+                    b, tiles = b + 1, n
+                _kv4_portions(q, out, cache, step, block_table, a, b, tiles, window, scale, nq, nkv, d, sink, ws)
+                a = b
+            most = max((n for n in lens if n <= short), default=0)
+        if most == 0:
+            return
     key = (code, S, most, nq, nkv, d, sms)
     plan = _KV4_PLANS.get(key)
     if plan is None:
@@ -1786,6 +1815,28 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
     _call("attention_kv4", "ilb_kv4_attention_rows", at, to, code, held, positions.data_ptr(), cu_q.data_ptr(), block_table.data_ptr(),
           max_blocks, page_size, num_pages, window, scale, S, most, 1 if step.decode_only else 0, nq, nkv, d, width, width, sinks, sms, scratch, plan[0], tickets, plan[1],
           _tc_state(device).error.data_ptr(), _raw_stream(q))
+
+
+def _kv4_portions(q, out, cache, step, block_table, a: int, b: int, tiles: int, window: int, scale: float, nq: int, nkv: int, d: int, sink, ws) -> None:
+    """Sequences a .. b - 1 of the step on the prefill kernel: what they see is unpacked, `tiles` tiles of 128 keys a sequence."""
+    n, device, lens = b - a, q.device, step.h_q_len[a:b]
+    half = torch.float16
+    k, v = (ws.address("kv4." + w, n * tiles * nkv * KV4_TILE * d, half) for w in ("keys", "values"))
+    info = ws.address("kv4.tiles", n * tiles * nkv * 4, torch.float32)
+    q_half, q_power = ws.address("kv4.queries", q.numel(), half), ws.address("kv4.query_powers", q.shape[0] * nq, torch.float32)
+    order = _KV4_ORDER.get(device)
+    if order is None or order.numel() < n * tiles:       # page s * tiles + t holds tile t of sequence s
+        order = _KV4_ORDER[device] = torch.arange(max(n * tiles, 1 << 14), dtype=torch.int32, device=device)
+    positions, cu_q, stream = step.positions.data_ptr(), step.cu_q.data_ptr() + 4 * a, _raw_stream(q)
+    sinks = None if sink is None else sink.data_ptr()
+    _call("kv4", "ilb_kv4_unpack", cache.data_ptr(), block_table.data_ptr() + 4 * a * block_table.shape[1], block_table.shape[1],
+          step.kv_len.data_ptr() + 4 * a, positions, cu_q, window, cache.shape[2] * KV4_UNIT, cache.shape[0], n, tiles, nkv, d, k, v, info,
+          q.data_ptr(), q_half, q_power, nq, sum(lens) * nq, stream)
+    per_block = 128 // (nq // nkv)
+    one, two = sum(-(-x // per_block) for x in lens), sum(-(-x // (2 * per_block)) for x in lens)
+    blocks = TC_ATTENTION_ROW_BLOCKS or tc_row_blocks(one * nkv, two * nkv, _sm_count(device), all(kv >= 2 * x for x, kv in zip(lens, step.h_kv_len[a:b])))
+    _call("attention_tc", "ilb_attention_prefill_half", q_half, out.data_ptr(), k, v, info, q_power, positions, cu_q, order.data_ptr(), tiles, window,
+          scale, q.shape[0], n, two if blocks == 2 else one, blocks, nq, nkv, d, sinks, _tc_state(device).error.data_ptr(), stream)
 
 
 DECODE_FUSED_ENABLED = True     # tests switch it off to run q/k norm + rotation + cache write as a launch of its own
