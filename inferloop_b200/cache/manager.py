@@ -6,6 +6,7 @@ size, window).  A group has its own pool, its own block tables and one device te
 `[layers_in_group, 2, pages, kv_heads, page_size, head_dim]`; layer l's keys are
 `storage[l, 0]`, its values `storage[l, 1]` (a group whose values have another head size
 than its keys keeps them in a tensor of their own, `[layers, pages, kv_heads, page_size, v_head_dim]`).
+A group in 4 bits (`PagedKVNeed.bits`) has bytes instead, `[layers_in_group, pages, kv_heads, page_size / 16, 18 head_dim]`.
 A layer may have a second set of pages beside its tokens' (`CacheNeeds.pooled`), in a group whose rows stand
 for `stride` tokens each: such a group needs a page per `page_size * stride` tokens.  Pages are taken when the step that first
 touches them is prepared, all groups or none (the reference grows pages per step,
@@ -51,6 +52,7 @@ class LayerCache:
     state: Dict[str, torch.Tensor] = field(default_factory=dict)
     instance: int = 0          # which run of a layer that runs several times (RunEntry.instance)
     pooled: Optional["LayerCache"] = None      # the layer's second set of pages, whose rows stand for several tokens each
+    kv4: Optional[torch.Tensor] = None         # keys and values in 4 bits (k and v are None then)
 
 
 @dataclass
@@ -65,6 +67,8 @@ class PageGroup:
     storage_v: Optional[torch.Tensor] = None      # the values, when their head size is not the keys'
 
     def page_bytes(self, element_size: int) -> int:
+        if self.need.bits == 4:
+            return len(self.layers) * self.need.kv_heads * self.page_size // 16 * 18 * self.need.head_dim
         return (len(self.layers) * self.need.kv_heads * self.page_size
                 * (self.need.head_dim + self.need.value_dim) * element_size)
 
@@ -131,8 +135,17 @@ class CacheManager:
         for gi, (need, layers) in enumerate(found):
             pool = PagePool(pages_of[gi], _handle=self._lib.ilb_ledger_pool(self._h, gi), _ids=self._ids)
             self.groups.append(PageGroup(gi, need, layers, pool, self.page_size))
+        for g in self.groups:
+            if g.need.bits not in (None, 4) or (g.need.bits == 4 and (self.page_size % 16 or g.need.head_dim % 32 or g.need.head_dim > 512
+                                                                      or g.need.value_dim != g.need.head_dim or g.need.stride != 1)):
+                raise ValueError(f"a cache in 4 bits takes pages of a multiple of 16 tokens and equal key and value heads of a multiple of 32 "
+                                 f"up to 512, found pages of {self.page_size} and {g.need}")
         if device is not None:
             for g in self.groups:
+                if g.need.bits == 4:
+                    g.storage = torch.zeros((len(g.layers), g.pool.num_pages, g.need.kv_heads, self.page_size // 16, 18 * g.need.head_dim),
+                                            dtype=torch.uint8, device=device)
+                    continue
                 both = g.need.value_dim == g.need.head_dim
                 g.storage = torch.zeros(
                     (len(g.layers), 2 if both else 1, g.pool.num_pages, g.need.kv_heads, self.page_size, g.need.head_dim),
@@ -287,7 +300,7 @@ class CacheManager:
 
         def pages(key):
             gi, k, v = self._group_of_layer.get(key), None, None
-            if gi is not None and self.groups[gi].storage is not None:
+            if gi is not None and self.groups[gi].storage is not None and self.groups[gi].need.bits is None:
                 g = self.groups[gi]
                 s = g.storage[self._index_in_group[key]]
                 k = s[0]
@@ -298,13 +311,16 @@ class CacheManager:
             return gi, k, v
 
         gi, k, v = pages(owner)
+        kv4 = None
+        if gi is not None and self.groups[gi].need.bits == 4 and self.groups[gi].storage is not None:
+            kv4 = self.groups[gi].storage[self._index_in_group[owner]]
         pooled = None
         if owner + ("pooled",) in self._group_of_layer:
             pg, pk, pv = pages(owner + ("pooled",))
             pooled = LayerCache(entry.cache_of, pg, self.page_size, pk, pv, entry.writes_cache, {}, entry.instance)
         state = {need.name: self._slot_state[(owner, need.name)]
                  for need in self._slot_needs.get(owner, ()) if (owner, need.name) in self._slot_state}
-        return LayerCache(entry.cache_of, gi, self.page_size, k, v, entry.writes_cache, state, entry.instance, pooled)
+        return LayerCache(entry.cache_of, gi, self.page_size, k, v, entry.writes_cache, state, entry.instance, pooled, kv4)
 
     def model_state(self) -> Dict[str, torch.Tensor]:
         """The state per request that belongs to no layer: name -> [slots, *shape]."""
@@ -330,6 +346,7 @@ class CacheManager:
             "groups": [{
                 "index": g.index, "layers": list(g.layers), "kv_heads": g.need.kv_heads,
                 "head_dim": g.need.head_dim, "v_head_dim": g.need.value_dim, "window": g.need.window, "stride": g.need.stride,
+                "bits": g.need.bits,
                 "total": g.pool.num_pages, "free": g.pool.num_free,
                 "active": g.pool.num_pages - g.pool.num_free,
                 "allocations": g.pool.allocations, "reuses": g.pool.reuses,

@@ -36,6 +36,7 @@ def _add_engine_options(p: argparse.ArgumentParser) -> None:
     p.add_argument("--device-timing", choices=["off", "graph", "node"], default="off",
                    help="device time per step (graph) or per kernel and op class (node), reported under runtime")
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    p.add_argument("--kv-cache", choices=["auto", "int4"], default="auto", help="keys and values in the dtype, or in 4 bits")
     p.add_argument("--random-weights", type=int, default=None, metavar="SEED",
                    help="ignore model.safetensors; make weights from config.json and this seed")
 
@@ -85,7 +86,7 @@ def _engine(args, folder: str):
                   max_num_batched_tokens=args.max_num_batched_tokens, max_model_len=args.max_model_len,
                   max_output_tokens=args.max_output_tokens, max_num_seqs=args.max_num_seqs,
                   gpu_memory_utilization=args.gpu_memory_utilization,
-                  random_weights_seed=args.random_weights, device_timing=args.device_timing)
+                  random_weights_seed=args.random_weights, device_timing=args.device_timing, kv_cache=args.kv_cache)
 
 
 def _sampling(engine, d: Dict[str, Any]):

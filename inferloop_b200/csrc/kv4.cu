@@ -34,7 +34,7 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&x)[4]) {
 }
 __device__ __forceinline__ void store4(float* p, const float (&x)[4]) { *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]); }
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 128, kMaxHeadDim = 512;
 
 // Eight lanes a group of 32 elements: maximum over them, four codes each, 16 bits of V or (two lanes together) a word of K.
 template <typename T>
@@ -143,6 +143,106 @@ kv4_read_kernel(const uint8_t* cache, const int* block_table, int table_stride, 
     const size_t o = (((size_t)to[i] * nkv + head) * page_size + slot) * d + 8 * e8;
     spread(k, ks, k_out + o);
     spread(v, vs, v_out + o);
+  }
+}
+
+// The input stage of a layer whose cache is held in 4 bits: per-head norm and rotation of queries and keys as in qk_norm_rope.cu (its modes),
+// in 32 bits, queries out, keys and values into the cache.  A warp a (token, head), four elements a lane and 128 of them; rotation
+// partners through shared memory.  Keys are quantised from their 32-bit values, values (bfloat16 ones exactly) as they come.
+constexpr int kInputWarps = 8;
+constexpr int kPairsInterleaved = 1, kNormAfterRotation = 2, kNormUnweighted = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(kInputWarps * 32)
+qk_norm_rope_kv4_kernel(const T* qkv, int qkv_stride, T* q_out, int q_stride, bool wide, const float* q_weight, const float* k_weight, float eps, const float2* rope,
+                        int rotary_dim, int mode, const int* positions, const int* seq_of_token, const int* block_table, int max_blocks, int page_size,
+                        int num_pages, uint8_t* cache, int n_tokens, int nq, int nkv, int d) {
+  pdl_launch_dependents();
+  pdl_wait();
+  __shared__ float rows[kInputWarps][kMaxHeadDim];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int heads = nq + 2 * nkv;
+  const long long item = (long long)blockIdx.x * kInputWarps + warp;
+  const int t = (int)(item / heads), head = (int)(item % heads);
+  if (t >= n_tokens) return;
+  const bool is_q = head < nq, is_v = head >= nq + nkv;
+  const int h = is_q ? head : is_v ? head - nq - nkv : head - nq;
+  constexpr int kChunks = kMaxHeadDim / 128;
+  float x[kChunks][4];
+#pragma unroll
+  for (int c = 0; c < kChunks; ++c) {
+    x[c][0] = x[c][1] = x[c][2] = x[c][3] = 0.f;
+    const int e = 128 * c + 4 * lane;
+    if (e < d) load4(qkv + (size_t)t * qkv_stride + (size_t)head * d + e, wide, x[c]);
+  }
+  if (!is_v) {
+    const float* weight = is_q ? q_weight : k_weight;
+    auto norm = [&] {
+      float ss = 0.f;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ss = fmaf(x[c][i], x[c][i], ss);
+      ss = warp_sum(ss);
+      const float inv = 1.0f / sqrtf(ss / (float)d + eps);
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int e = 128 * c + 4 * lane + i;
+          if (e < d) x[c][i] = weight != nullptr ? x[c][i] * inv * weight[e] : x[c][i] * inv;
+        }
+    };
+    const bool normed = weight != nullptr || (mode & kNormUnweighted);
+    if (normed && !(mode & kNormAfterRotation)) norm();
+    if (rope != nullptr) {
+      float* row = rows[warp];
+      const float2* cs = rope + (size_t)t * (rotary_dim / 2);
+      const int half = rotary_dim / 2;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+        if (128 * c + 4 * lane < d) *reinterpret_cast<float4*>(row + 128 * c + 4 * lane) = make_float4(x[c][0], x[c][1], x[c][2], x[c][3]);
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int e = 128 * c + 4 * lane + i;
+          if (e >= rotary_dim) continue;
+          const bool inter = mode & kPairsInterleaved, second = inter ? (e & 1) != 0 : e >= half;
+          const int pair = inter ? e / 2 : second ? e - half : e;
+          const float2 w = cs[pair];
+          const float other = row[inter ? e ^ 1 : second ? e - half : e + half];
+          // products and sums rounded separately, as in the layers with a wider cache
+          x[c][i] = second ? __fadd_rn(__fmul_rn(other, w.y), __fmul_rn(x[c][i], w.x)) : __fsub_rn(__fmul_rn(x[c][i], w.x), __fmul_rn(other, w.y));
+        }
+      __syncwarp();
+    }
+    if (normed && (mode & kNormAfterRotation)) norm();
+  }
+  if (is_q) {
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c)
+      if (128 * c + 4 * lane < d) store4(q_out + (size_t)t * q_stride + (size_t)head * d + 128 * c + 4 * lane, x[c]);
+    return;
+  }
+  if (cache == nullptr) return;
+  const int pos = positions[t], blk = pos / page_size;
+  const int page = blk >= 0 && blk < max_blocks ? block_table[(size_t)seq_of_token[t] * max_blocks + blk] : -1;
+  if (page < 0 || page >= num_pages) return;                              // never write outside the pool
+  const int slot = pos % page_size, j = slot % kKv4Unit, l = lane & 7;
+  uint8_t* unit = cache + (((size_t)page * nkv + h) * (page_size / kKv4Unit) + slot / kKv4Unit) * kv4_unit_bytes(d);
+#pragma unroll
+  for (int c = 0; c < kChunks; ++c) {
+    if (128 * c >= d) break;
+    const int G = 4 * c + (lane >> 3);
+    __nv_bfloat16 scale;
+    const uint32_t codes = is_v && sizeof(T) == 2 ? kv4_quantise<true>(x[c], scale) : kv4_quantise<false>(x[c], scale);
+    const uint32_t pair = codes | (__shfl_down_sync(0xffffffffu, codes, 1) << 16);
+    if (G * kKv4Group >= d) continue;
+    if (is_v) *reinterpret_cast<uint16_t*>(unit + kv4_value_at(d, j, G, l)) = (uint16_t)codes;
+    else if ((l & 1) == 0) *reinterpret_cast<uint32_t*>(unit + kv4_key_at(d, j, G, l)) = pair;
+    if (l == 0) *reinterpret_cast<__nv_bfloat16*>(unit + kv4_scale_at(d, is_v, j, G)) = scale;
   }
 }
 
@@ -275,7 +375,7 @@ kv4_unpack_kernel(const uint8_t* cache, const int* block_table, int table_stride
 }
 
 int check_cache(const char* what, int page_size, int num_pages, int max_blocks, int nkv, int d) {
-  ILB_REQUIRE(nkv > 0 && d > 0 && d % kKv4Group == 0 && d <= 512, "%s: head size %d must be a multiple of 32 up to 512, and there must be heads", what, d);
+  ILB_REQUIRE(nkv > 0 && d > 0 && d % kKv4Group == 0 && d <= kMaxHeadDim, "%s: head size %d must be a multiple of 32 up to 512, and there must be heads", what, d);
   ILB_REQUIRE(page_size > 0 && page_size % kKv4Unit == 0, "%s: page size %d must be a multiple of 16", what, page_size);
   ILB_REQUIRE(num_pages > 0 && max_blocks > 0, "%s: bad cache geometry", what);
   return 0;
@@ -333,6 +433,32 @@ ILB_EXPORT int ilb_kv4_read(const void* cache, const int* block_table, int table
   }
 #undef ILB_KV4_READ
   return check_launch("kv4_read");
+}
+
+// qkv: rows q | k | v of n_tokens tokens, qkv_stride apart; weights, rope [n_tokens][rotary_dim / 2][2] and cache may be null (no norm, no
+// rotation, nothing kept); mode as in ilb_qk_norm_rope_cache.
+ILB_EXPORT int ilb_qk_norm_rope_kv4(const void* qkv, int qkv_stride, void* q_out, int q_stride, int dtype, const float* q_weight, const float* k_weight,
+                                    float eps, const float* rope, int rotary_dim, int mode, const int* positions, const int* seq_of_token,
+                                    const int* block_table, int max_blocks, int page_size, int num_pages, void* cache, int n_tokens, int nq, int nkv,
+                                    int d, cudaStream_t stream) {
+  if (int rc = check_cache("qk_norm_rope_kv4", page_size, num_pages, max_blocks, nkv, d)) return rc;
+  ILB_REQUIRE(n_tokens >= 0 && nq > 0 && (dtype == kF32 || dtype == kBF16), "qk_norm_rope_kv4: bad sizes or types");
+  ILB_REQUIRE(rope == nullptr || (rotary_dim > 0 && rotary_dim % 2 == 0 && rotary_dim <= d), "qk_norm_rope_kv4: rotary dimension %d must be even and at most %d",
+              rotary_dim, d);
+  ILB_REQUIRE(mode >= 0 && mode < 8 && qkv_stride >= (nq + 2 * nkv) * d && q_stride >= nq * d && q_stride % 4 == 0, "qk_norm_rope_kv4: unknown mode or rows too short");
+  ILB_REQUIRE((((uintptr_t)cache | (uintptr_t)q_out) % 16) == 0, "qk_norm_rope_kv4: cache and queries must start on 16-byte boundaries");
+  if (n_tokens == 0) return 0;
+  const long long blocks = ((long long)n_tokens * (nq + 2 * nkv) + kInputWarps - 1) / kInputWarps;
+  ILB_REQUIRE(blocks <= 0x7fffffffLL, "qk_norm_rope_kv4: too many tokens for one launch");
+  const bool wide = (uintptr_t)qkv % (dtype == kF32 ? 16 : 8) == 0 && qkv_stride % 4 == 0;
+#define ILB_KV4_INPUT(T)                                                                                                                          \
+  ilb::launch(qk_norm_rope_kv4_kernel<T>, dim3((unsigned)blocks), dim3(kInputWarps * 32), 0, stream, (const T*)qkv, qkv_stride, (T*)q_out, q_stride, wide, \
+              q_weight, k_weight, eps, (const float2*)rope, rope ? rotary_dim : 0, mode, positions, seq_of_token, block_table, max_blocks, page_size,      \
+              num_pages, (uint8_t*)cache, n_tokens, nq, nkv, d)
+  if (dtype == kF32) ILB_KV4_INPUT(float);
+  else ILB_KV4_INPUT(__nv_bfloat16);
+#undef ILB_KV4_INPUT
+  return check_launch("qk_norm_rope_kv4");
 }
 
 // What ilb_attention_prefill_half reads, for n_seqs sequences (rows of block_table, table_stride apart; lengths [n_seqs]; positions of all

@@ -64,6 +64,7 @@ _FUNCTIONS: dict = {}  # launcher name -> (function, its library)
 _SIGNATURES = {
     "ilb_kv4_write": "pqqpqqipppiiipiiip",
     "ilb_kv4_read": "ppipipiiiippiiip",
+    "ilb_qk_norm_rope_kv4": "pipi" + "ippfpii" + "pppiii" + "piiiip",
     "ilb_kv4_unpack": "ppippp" + "iiiiiii" + "pppppp" + "iqp",
     "ilb_attention_prefill_half": "ppppppppp" + "iifiiiiiii" + "ppp",
     "ilb_kv4_attention_simple": "ppippppiiiifiiiiiipp",
@@ -1669,6 +1670,13 @@ def kv4_cache_shape(pages: int, nkv: int, page_size: int, d: int) -> tuple:
     return (int(pages), int(nkv), page_size // KV4_UNIT, 18 * d)
 
 
+def kv4_scratch_bytes(tokens: int, nq: int, nkv: int, d: int) -> int:
+    """Workspace that `kv4_attention` asks for at most in steps of so many tokens: the unpacked keys and values of a group of
+    portions, their queries, the records of shared keys."""
+    unpacked = KV4_UNPACK_TOKENS * nkv * d * 4 if attention_tc_supported(nq, nkv, d, KV4_TILE) else 0
+    return unpacked + tokens * nq * (2 * d + 4) + (512 * nkv + 4 * 148) * 8 * (d + 4) * 4
+
+
 def _kv4_need(what: str, cache: torch.Tensor, block_table: torch.Tensor, nkv: int, d: int) -> tuple:
     """(pages, page size) of a 4-bit cache that holds `nkv` heads of `d`."""
     if cache.dtype is not torch.uint8 or block_table.dtype is not torch.int32 or not (cache.is_contiguous() and block_table.is_contiguous()
@@ -1709,6 +1717,26 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, step, block_table: torch.Tensor,
           _raw_stream(cache))
 
 
+def qk_norm_rope_kv4(qkv: torch.Tensor, q_out: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float,
+                     rope: Optional[torch.Tensor], rotary_dim: int, step, block_table: torch.Tensor, cache: torch.Tensor, write: bool, nq: int, nkv: int,
+                     d: int, mode: int = 0) -> None:
+    """`qk_norm_rope_cache` for a 4-bit cache, in one launch: per-head q/k RMSNorm and rotation of the projection's rows q | k | v,
+    q -> q_out, keys (quantised from their 32-bit values) and values -> the cache as `kv4_write` keeps them (`write` False: nowhere)."""
+    _need(qkv, "qkv", contiguous=False); _need(q_out, "q_out", qkv.dtype); _need(q_weight, "q_norm weight", torch.float32)
+    _need(k_weight, "k_norm weight", torch.float32); _need(rope, "rope table", torch.float32)
+    T = qkv.shape[0]
+    num_pages, page_size = _kv4_need("qk_norm_rope_kv4", cache, block_table, nkv, d)
+    _kv4_ints("qk_norm_rope_kv4 positions and sequence indices", step.positions, step.seq_of_token)
+    if qkv.stride(1) != 1 or qkv.shape[1] < (nq + 2 * nkv) * d or tuple(q_out.shape) != (T, nq * d) or step.positions.numel() != T \
+            or step.seq_of_token.numel() != T or (rope is not None and tuple(rope.shape) != (T, rotary_dim // 2, 2)) \
+            or any(w is not None and w.numel() != d for w in (q_weight, k_weight)):
+        raise KernelError("qk_norm_rope_kv4: projection, queries, weights, angles and step do not agree")
+    _call("kv4", "ilb_qk_norm_rope_kv4", qkv.data_ptr(), qkv.stride(0), q_out.data_ptr(), nq * d, _code(qkv),
+          None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps,
+          None if rope is None else rope.data_ptr(), rotary_dim, mode, step.positions.data_ptr(), step.seq_of_token.data_ptr(), block_table.data_ptr(),
+          block_table.shape[1], page_size, num_pages, cache.data_ptr() if write else None, T, nq, nkv, d, _raw_stream(cache))
+
+
 def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, out_table: torch.Tensor, k_out: torch.Tensor,
              v_out: torch.Tensor) -> None:
     """Pages of the 4-bit cache read back into pages [out pages, nkv, page_size, d] of k_out's type: page b of sequence s, if it
@@ -1731,7 +1759,7 @@ def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tens
 
 KV4_ROWS_HEADS = (32, 64, 96, 128, 256)     # head sizes of the kernel of few rows (others: the simple kernel)
 KV4_PORTION_ROWS = 128      # rows (tokens x query heads of a group) from which a portion's keys and values are unpacked once for the prefill kernel
-KV4_UNPACK_TOKENS = 1 << 16 # tokens whose keys and values are unpacked at a time (more of them: one group of sequences after another)
+KV4_UNPACK_TOKENS = 1 << 17 # tokens whose keys and values are unpacked at a time: sequences in groups; one with more keys reads the codes
 KV4_TILE = 128              # keys of a tile of the prefill kernel
 _KV4_ORDER: dict = {}       # 0, 1, 2, .. on each device
 _KV4_WORKSPACE: dict = {}
@@ -1785,20 +1813,22 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
         most = longest = max(lens)
         short = max(KV4_PORTION_ROWS // (nq // nkv), 1)
         if longest > short and dtype is torch.bfloat16 and scale > 0 and attention_tc_supported(nq, nkv, d, KV4_TILE):
-            a = 0
-            while a < S:                                 # runs of neighbouring sequences with long portions, as many as the scratch takes
-                if lens[a] <= short:
-                    a += 1
-                    continue
-                b, tiles = a, 0
-                while b < S and lens[b] > short:
-                    n = max(tiles, -(-step.h_kv_len[b] // KV4_TILE))
-                    if b > a and n * KV4_TILE * (b + 1 - a) > KV4_UNPACK_TOKENS:
-                        break
-                    b, tiles = b + 1, n
-                _kv4_portions(q, out, cache, step, block_table, a, b, tiles, window, scale, nq, nkv, d, sink, ws)
-                a = b
-            most = max((n for n in lens if n <= short), default=0)
+            kv, a, most = step.h_kv_len, 0, 0
+            if max(kv) <= KV4_UNPACK_TOKENS:             # (else the rows kernel takes whatever comes: it leaves out by length alone)
+                while a < S:                             # runs of neighbouring sequences with long portions, as many as the scratch takes
+                    if lens[a] <= short:
+                        a, most = a + 1, max(most, lens[a])
+                        continue
+                    b, tiles = a, 0
+                    while b < S and lens[b] > short:
+                        n = max(tiles, -(-kv[b] // KV4_TILE))
+                        if b > a and n * KV4_TILE * (b + 1 - a) > KV4_UNPACK_TOKENS:
+                            break
+                        b, tiles = b + 1, n
+                    _kv4_portions(q, out, cache, step, block_table, a, b, tiles, window, scale, nq, nkv, d, sink, ws)
+                    a = b
+            else:
+                most = longest
         if most == 0:
             return
     key = (code, S, most, nq, nkv, d, sms)

@@ -57,9 +57,11 @@ class Engine:
                  max_output_tokens: Optional[int] = None, max_num_seqs: int = 64,
                  gpu_memory_utilization: float = DEFAULT_GPU_MEMORY_UTILIZATION,
                  prefill_chunk_tokens: int = 512, random_weights_seed: Optional[int] = None,
-                 cuda_graphs: bool = True, device_timing: str = "off", runner=None) -> None:
+                 cuda_graphs: bool = True, device_timing: str = "off", runner=None, kv_cache: str = "auto") -> None:
         """`model`: a folder with config.json and safetensors, or a config mapping
-        together with `random_weights_seed` (weights are then made on the device)."""
+        together with `random_weights_seed` (weights are then made on the device).
+        `kv_cache`: "auto" keeps keys and values in `dtype`, "int4" in 4 bits with a scale for every 32
+        elements (4.5 bits an element; `block_size` a multiple of 16, head sizes multiples of 32)."""
         self.block_size = int(block_size)
         self.max_output_tokens = max_output_tokens
         # what a request without sampling fields gets, and the folder's stop tokens
@@ -80,13 +82,13 @@ class Engine:
             if isinstance(model, (str, os.PathLike)):
                 self.runner = ModelRunner.from_folder(
                     str(model), dtype=dt, device=dev, page_size=self.block_size,
-                    num_pages=first_pages, max_requests=max(max_num_seqs, 1))
+                    num_pages=first_pages, max_requests=max(max_num_seqs, 1), kv_cache=kv_cache)
             else:
                 if random_weights_seed is None:
                     raise ValueError("a config mapping needs random_weights_seed")
                 self.runner = ModelRunner.from_config(
                     model, random_weights_seed, dtype=dt, device=dev, page_size=self.block_size,
-                    num_pages=first_pages, max_requests=max(max_num_seqs, 1))
+                    num_pages=first_pages, max_requests=max(max_num_seqs, 1), kv_cache=kv_cache)
             if pages is None:
                 step_tokens = max_num_batched_tokens or max(prefill_chunk_tokens + max_num_seqs - 1, 1)
                 self.runner.resize_cache(self._pages_from_memory(dev, gpu_memory_utilization, max_num_seqs,

@@ -46,6 +46,14 @@ def parse_dtype(name) -> torch.dtype:
         raise ValueError(f"unknown dtype {name!r}; use bfloat16 or float32") from None
 
 
+def parse_kv_cache(name: str) -> Optional[int]:
+    """Bits that keys and values are kept in: None for "auto" (the compute dtype), 4 for "int4"."""
+    try:
+        return {"auto": None, "int4": 4}[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"unknown kv cache {name!r}; use auto or int4") from None
+
+
 def require_cuda(device) -> torch.device:
     dev = torch.device(device)
     if dev.type != "cuda":
@@ -206,12 +214,17 @@ def prepare_step(cache: CacheManager, stager: StepStager, entries: Sequence[Step
 class ModelRunner:
     def __init__(self, spec: ModelSpec, tensors: Mapping[str, torch.Tensor], dtype: torch.dtype,
                  device: torch.device, page_size: int, num_pages: int, max_requests: int,
-                 cuda_graphs: bool = True) -> None:
+                 cuda_graphs: bool = True, kv_cache: str = "auto") -> None:
         self.spec = spec
         self.dtype = dtype
         self.device = device
-        self.ctx = BuildContext(dtype=dtype, device=device, workspace=Workspace(device))
+        self.kv_cache = kv_cache
+        self.ctx = BuildContext(dtype=dtype, device=device, workspace=Workspace(device), kv_bits=parse_kv_cache(kv_cache))
         self.model = DecoderModel(spec, self.ctx)
+        if self.ctx.kv_bits is not None:
+            wide = sorted({n.paged for n in self.model.cache_needs() if n.paged is not None and n.paged.bits is None}, key=repr)
+            if wide:
+                raise ValueError(f"{spec.architecture}: a {kv_cache} cache is not served for layers that keep {wide[0]}")
         self.model.bind(tensors)
         self.cache = CacheManager(self.model.cache_needs(), page_size, num_pages, max_requests,
                                   dtype=dtype, device=device, run_order=spec.run_order,
@@ -237,9 +250,10 @@ class ModelRunner:
     def from_folder(cls, folder: str, dtype="bfloat16", device="cuda:0", page_size: int = 16,
                     num_pages: int = 256, max_requests: int = 64, registry=None,
                     allow_unexpected: bool = False,
-                    progress: Optional[Callable[[str], None]] = None) -> "ModelRunner":
+                    progress: Optional[Callable[[str], None]] = None, kv_cache: str = "auto") -> "ModelRunner":
         dev = require_cuda(device)
         dt = parse_dtype(dtype)
+        parse_kv_cache(kv_cache)
         path = os.path.join(folder, "config.json")
         if not os.path.exists(path):
             raise FileNotFoundError(f"{folder}: no config.json")
@@ -249,19 +263,19 @@ class ModelRunner:
         decls = DecoderModel(spec, BuildContext(dt, None, Workspace(None))).declare_weights()
         tensors, _ = load_weights(folder, decls, spec.weight_prefixes, spec.embedding_name, dt, dev,
                                   allow_unexpected=allow_unexpected, progress=progress)
-        return cls(spec, tensors, dt, dev, page_size, num_pages, max_requests)
+        return cls(spec, tensors, dt, dev, page_size, num_pages, max_requests, kv_cache=kv_cache)
 
     @classmethod
     def from_config(cls, config: Mapping, seed: int, dtype="bfloat16", device="cuda:0",
                     page_size: int = 16, num_pages: int = 256, max_requests: int = 64,
-                    registry=None) -> "ModelRunner":
+                    registry=None, kv_cache: str = "auto") -> "ModelRunner":
         """Random weights made on the device (no folder is written)."""
         dev = require_cuda(device)
         dt = parse_dtype(dtype)
         _, _, spec = read_model_config(json.dumps(dict(config)), registry)
         decls = DecoderModel(spec, BuildContext(dt, None, Workspace(None))).declare_weights()
         tensors = random_weights(decls, seed, dt, dev)
-        return cls(spec, tensors, dt, dev, page_size, num_pages, max_requests)
+        return cls(spec, tensors, dt, dev, page_size, num_pages, max_requests, kv_cache=kv_cache)
 
     def resize_cache(self, num_pages, max_requests: int) -> None:
         """Replace the cache by one of another size (`num_pages`: one number, or one per page

@@ -45,6 +45,10 @@ last token is cached; the tokens' own pages go when both the window and their bl
 [heads, hidden] whose rows ride behind q|k|v in the one projection; "element": every element of the heads' outputs by its own
 sigmoid, from a matrix [heads * v_head_dim, hidden].  `out_scale`: a constant on the whole mixer's
 output (a mixer that runs beside another one), applied in 32-bit to what the output projection reads and to its bias.
+
+A cache in 4 bits (`BuildContext.kv_bits`): keys and values are quantised as the input stage writes them and attention reads the codes
+(csrc/kv4.cuh), for layers with keys and values of one head size (a multiple of 32), per-head norms or none, a plain softmax, with a
+window, aligned chunks or neither, sinks and gates.
 """
 from __future__ import annotations
 
@@ -144,6 +148,13 @@ class GQAttention(Mixer):
         if (self.taps or self.values_are_keys) and (not self.taps or not self.qk_norm_rows or self.value_position is not None or self.pool or self.bias):
             raise ValueError("attention: convolutions (and values that are keys behind one) are served with norms over whole rows, without biases, "
                              "turned values and pooled blocks")
+        self.kv_bits = ctx.kv_bits
+        if self.kv_bits not in (None, 4):
+            raise ValueError(f"attention: a cache of {self.kv_bits} bits is not served, only one of 4")
+        if self.kv_bits == 4 and (self.shaped or self.value_mix is not None or self.qk_norm_rows or self.dv != self.d or self.d % ops.KV4_GROUP
+                                  or self.d > ops.KV4_MAX_HEAD):
+            raise ValueError("attention: a cache in 4 bits is served for equal key and value heads of a multiple of 32 up to 512, norms per head, a "
+                             "plain softmax and unmixed values")
         if self.values_are_keys and self.dv != self.d:
             raise ValueError(f"attention: values that are keys have the keys' head size, found {self.dv} and {self.d}")
         p = prefix
@@ -229,7 +240,7 @@ class GQAttention(Mixer):
         if not self.pool:
             # (no token looks back beyond its own chunk)
             slots = (SlotStateNeed("conv", (self.taps - 1, (self.nq + self.nkv) * self.d), torch.float32),) if self.taps else ()
-            return CacheNeeds(paged=PagedKVNeed(self.nkv, self.d, self.chunk or self.window, v_dim), slots=slots)
+            return CacheNeeds(paged=PagedKVNeed(self.nkv, self.d, self.chunk or self.window, v_dim, bits=self.kv_bits), slots=slots)
         # a token is read while it is in the window, and until its block is complete
         return CacheNeeds(paged=PagedKVNeed(self.nkv, self.d, max(self.window, self.pool), v_dim),
                           pooled=PagedKVNeed(self.nkv, self.d, None, v_dim, self.pool))
@@ -238,7 +249,8 @@ class GQAttention(Mixer):
         size = torch.empty((), dtype=self.ctx.dtype).element_size()
         width = (self.nq + self.nkv) * self.d + self.v_cols + self.gate_rows
         kept = self.nkv * self.dv if self.value_mix else 0
-        return tokens * ((width + self.nq * (self.d + self.dv) + kept) * size + self.rotary_dim * 4)
+        four = ops.kv4_scratch_bytes(tokens, self.nq, self.nkv, self.d) if self.kv_bits == 4 else 0
+        return four + tokens * ((width + self.nq * (self.d + self.dv) + kept) * size + self.rotary_dim * 4)
 
     # ------------------------------------------------------------------ run
     def input_rows(self):
@@ -277,6 +289,15 @@ class GQAttention(Mixer):
         rope = self.position.table(step)
         if self.qk_norm_rows:
             self._forward_rows(qkv, rope, table, step, cache, gate_col0, residual, out)
+            return
+        if self.kv_bits == 4:
+            q, o = ws.buffer("attn.q", (T, self.nq * self.d), dt), ws.buffer("attn.o", (T, self.nq * self.d), dt)
+            ops.scope("attention.qk_norm_rotation_cache_write")
+            ops.qk_norm_rope_kv4(qkv, q, self.q_norm, self.k_norm, self.qk_norm_eps, rope, self.rotary_dim, step, table, cache.kv4, cache.writable,
+                                 self.nq, self.nkv, self.d, self.mode)
+            ops.scope("attention.attention")
+            ops.kv4_attention(q, o, cache.kv4, step, table, self.seen, self.scale, self.nq, self.nkv, self.d, sink=self.sink, workspace=ws)
+            self._finish(o, qkv, gate_col0, residual, out)
             return
         v_first = None
         if self.value_mix is not None:

@@ -84,6 +84,7 @@ class BuildContext:
     device: Optional[torch.device]           # None while only declaring weights
     workspace: Workspace
     cache_dtype: Optional[torch.dtype] = None
+    kv_bits: Optional[int] = None            # 4: keys and values are kept in 4 bits (csrc/kv4.cuh); None: in the cache's dtype
 
     def __post_init__(self) -> None:
         if self.cache_dtype is None:
@@ -99,6 +100,7 @@ class PagedKVNeed:
     window: Optional[int] = None     # None: all keys are kept; n: only the last n are read
     v_head_dim: Optional[int] = None  # head size of the values when it is not the keys'; 0: the cached vector is all there is
     stride: int = 1                  # tokens that one cached row stands for: n keeps a row per n tokens, once all n are there
+    bits: Optional[int] = None       # 4: rows are kept in 4 bits with their scales, keys and values of a token side by side
 
     @property
     def value_dim(self) -> int:
