@@ -65,11 +65,6 @@ __device__ __forceinline__ uint32_t turned(uint32_t x) {            // an 8 x 8 
 }
 // Codes of nibbles 0 .. 3 of both halves of w (`w8` = w >> 8) as fp16 numbers: 1024 + code from nibbles 0 and 2, 64 + code from 1 and 3;
 // less 1032 and 72 the codes' c.
-__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {      // (x & mask) | bits, in one instruction
-  uint32_t y;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
-  return y;
-}
 template <int I>
 __device__ __forceinline__ uint32_t offset_pair(uint32_t w, uint32_t w8) {
   const uint32_t x = I < 2 ? w : w8;

@@ -36,37 +36,89 @@ __device__ __forceinline__ void store4(float* p, const float (&x)[4]) { *reinter
 
 constexpr int kThreads = 128, kMaxHeadDim = 512;
 
-// Eight lanes a group of 32 elements: maximum over them, four codes each, 16 bits of V or (two lanes together) a word of K.
-template <typename T>
+// Eight lanes a group of 32 elements: maximum over them, four codes each, 16 bits of V or (two lanes together) a word of K.  A thread has
+// one place of the rows (keys or values, head, group, four elements) of TOKENS tokens in a row, all asked for before any is looked
+// at: with one token a thread the chain of loads (position, page, store) was most of the time (2,048 tokens of 8 heads of 128: 9 us, four a
+// thread 5).
+template <typename T, int TOKENS, int DIM>
 __global__ void __launch_bounds__(kThreads)
 kv4_write_kernel(const T* k, long long k_row, long long k_head, const T* v, long long v_row, long long v_head,
                  bool wide, const int* positions, const int* seq_of_token, const int* block_table,
-                 int max_blocks, int page_size, int num_pages, uint8_t* cache, int n_tokens, int nkv, int d) {
+                 int max_blocks, int page_size, int num_pages, uint8_t* cache, int n_tokens, int nkv, int d_any) {
   pdl_launch_dependents();
   pdl_wait();
-  const int per_row = d / kKv4Group;
-  const long long at = ((long long)blockIdx.x * kThreads + threadIdx.x) >> 3;       // group of (token, k | v, head)
-  const int l = threadIdx.x & 7;
-  const int G = (int)(at % per_row);
-  const long long row = at / per_row;
-  const int head = (int)(row % nkv), value = (int)(row / nkv % 2);
-  const long long t = row / (2 * nkv);
-  float x[4] = {0.f, 0.f, 0.f, 0.f};
-  if (t < n_tokens)
-    load4(value ? v + t * v_row + head * v_head + G * kKv4Group + 4 * l : k + t * k_row + head * k_head + G * kKv4Group + 4 * l, wide, x);
-  __nv_bfloat16 scale;
-  const uint32_t codes = kv4_quantise<sizeof(T) == 2>(x, scale);
-  const uint32_t pair = codes | (__shfl_down_sync(0xffffffffu, codes, 1) << 16);
-  if (t >= n_tokens) return;
-  const int pos = positions[t], blk = pos / page_size;
-  if (blk < 0 || blk >= max_blocks) return;
-  const int page = block_table[(size_t)seq_of_token[t] * max_blocks + blk];
-  if (page < 0 || page >= num_pages) return;                                       // never write outside the pool
-  const int slot = pos % page_size, j = slot % kKv4Unit;
-  uint8_t* unit = cache + (((size_t)page * nkv + head) * (page_size / kKv4Unit) + slot / kKv4Unit) * kv4_unit_bytes(d);
-  if (value) *reinterpret_cast<uint16_t*>(unit + kv4_value_at(d, j, G, l)) = (uint16_t)codes;
-  else if ((l & 1) == 0) *reinterpret_cast<uint32_t*>(unit + kv4_key_at(d, j, G, l)) = pair;
-  if (l == 0) *reinterpret_cast<__nv_bfloat16*>(unit + kv4_scale_at(d, value, j, G)) = scale;
+  const int d = DIM > 0 ? DIM : d_any;
+  const int per_row = d / kKv4Group, at = (blockIdx.y * kThreads + threadIdx.x) >> 3;        // group of (k | v, head)
+  const int l = threadIdx.x & 7, G = at % per_row, head = at / per_row % nkv, value = at / per_row / nkv;
+  const long long t0 = (long long)blockIdx.x * TOKENS;
+  const T* src = (value ? v + head * v_head : k + head * k_head) + G * kKv4Group + 4 * l;
+  const long long stride = value ? v_row : k_row;
+  const bool mine = value < 2;
+  float x[TOKENS][4];
+#pragma unroll
+  for (int i = 0; i < TOKENS; ++i) {
+    x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
+    if (mine && t0 + i < n_tokens) load4(src + (t0 + i) * stride, wide, x[i]);
+  }
+  // lane i of a warp finds where token i lies: its unit of head 0 (-1: nowhere), and its place in the unit
+  const int lane = threadIdx.x & 31, upp = page_size / kKv4Unit;
+  long long where = -1;
+  int place = 0;
+  if (lane < TOKENS && t0 + lane < n_tokens) {
+    const int pos = positions[t0 + lane], seq = seq_of_token[t0 + lane], u = pos / kKv4Unit, blk = u / upp;
+    const int page = pos >= 0 && blk < max_blocks ? block_table[(size_t)seq * max_blocks + blk] : -1;
+    if (page >= 0 && page < num_pages) where = (long long)page * nkv * upp + (u - blk * upp);      // never outside the pool
+    place = pos % kKv4Unit;
+  }
+  const size_t unit_bytes = kv4_unit_bytes(d);
+  constexpr bool kTurn = TOKENS == 4 && DIM == 128;
+  uint32_t codes[TOKENS];
+  __nv_bfloat16 scale[TOKENS];
+#pragma unroll
+  for (int i = 0; i < TOKENS; ++i) codes[i] = kv4_quantise<sizeof(T) == 2>(x[i], scale[i]);
+  if constexpr (kTurn) {
+    // A warp holds a row of each of four tokens: lane (G, l) trades its 16 bits of the four tokens for those of the four groups of token G,
+    // eight bytes of values, and of keys after a trade with its neighbour: a store of eight bytes in place of four of two.
+    const int g = lane >> 3;
+    uint32_t mine4[4];                                                    // [group] of token g
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mine4[i] = 0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {                                         // round r: the lane r groups further has this lane's token, and wants that one's
+      const int send = (g - r) & 3;
+      const uint32_t out = send == 0 ? codes[0] : send == 1 ? codes[1] : send == 2 ? codes[2] : codes[3];
+      const uint32_t in = __shfl_sync(0xffffffffu, out, ((g + r) & 3) * 8 + l);
+      const int from = (g + r) & 3;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mine4[i] = from == i ? in : mine4[i];
+    }
+    uint32_t lo = mine4[0] | mine4[1] << 16, hi = mine4[2] | mine4[3] << 16;      // values: the groups' half-words lie side by side
+    if (!value) {                                                         // keys: words of one group, halves of l and l + 1
+      const uint32_t other_lo = __shfl_xor_sync(0xffffffffu, lo, 1), other_hi = __shfl_xor_sync(0xffffffffu, hi, 1);
+      const uint32_t a = l & 1 ? other_hi : lo, b = l & 1 ? hi : other_lo;        // even lanes take groups 0 and 1, odd ones 2 and 3
+      lo = __byte_perm(a, b, 0x5410);
+      hi = __byte_perm(a, b, 0x7632);
+    }
+    const long long at_unit = __shfl_sync(0xffffffffu, where, g);
+    const int j = __shfl_sync(0xffffffffu, place, g);
+    if (at_unit >= 0 && mine) {
+      uint8_t* unit = cache + (size_t)(at_unit + (long long)head * upp) * unit_bytes;
+      *reinterpret_cast<uint2*>(unit + (value ? kv4_value_at(d, j, 0, l) : kv4_key_at(d, j, 0, l & 6) + 8 * (l & 1))) = make_uint2(lo, hi);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TOKENS; ++i) {
+    const long long at_unit = __shfl_sync(0xffffffffu, where, i);
+    const int j = __shfl_sync(0xffffffffu, place, i);
+    const uint32_t pair = kTurn ? 0u : codes[i] | (__shfl_down_sync(0xffffffffu, codes[i], 1) << 16);
+    if (at_unit < 0 || !mine) continue;
+    uint8_t* unit = cache + (size_t)(at_unit + (long long)head * upp) * unit_bytes;
+    if constexpr (!kTurn) {
+      if (value) *reinterpret_cast<uint16_t*>(unit + kv4_value_at(d, j, G, l)) = (uint16_t)codes[i];
+      else if ((l & 1) == 0) *reinterpret_cast<uint32_t*>(unit + kv4_key_at(d, j, G, l)) = pair;
+    }
+    if (l == 0) *reinterpret_cast<__nv_bfloat16*>(unit + kv4_scale_at(d, value, j, G)) = scale[i];
+  }
 }
 
 // Eight codes of a word times their scale, in order (a product of two bfloat16 numbers, rounded once).
@@ -148,26 +200,25 @@ kv4_read_kernel(const uint8_t* cache, const int* block_table, int table_stride, 
 
 // The input stage of a layer whose cache is held in 4 bits: per-head norm and rotation of queries and keys as in qk_norm_rope.cu (its modes),
 // in 32 bits, queries out, keys and values into the cache.  A warp a (token, head), four elements a lane and 128 of them; rotation
-// partners through shared memory.  Keys are quantised from their 32-bit values, values (bfloat16 ones exactly) as they come.
+// partners through shared memory.  Keys are quantised from their 32-bit values (in the
+// bfloat16 engine by the product: a quotient within 2^-20 of a half may go either way), values as kv4_write does.
 constexpr int kInputWarps = 8;
 constexpr int kPairsInterleaved = 1, kNormAfterRotation = 2, kNormUnweighted = 4;
 
-template <typename T>
+template <typename T, int CHUNKS>
 __global__ void __launch_bounds__(kInputWarps * 32)
 qk_norm_rope_kv4_kernel(const T* qkv, int qkv_stride, T* q_out, int q_stride, bool wide, const float* q_weight, const float* k_weight, float eps, const float2* rope,
                         int rotary_dim, int mode, const int* positions, const int* seq_of_token, const int* block_table, int max_blocks, int page_size,
-                        int num_pages, uint8_t* cache, int n_tokens, int nq, int nkv, int d) {
+                        int num_pages, uint8_t* cache, int nq, int nkv, int d, bool quads) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ float rows[kInputWarps][kMaxHeadDim];
+  __shared__ __align__(16) float rows[kInputWarps][128 * CHUNKS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int heads = nq + 2 * nkv;
-  const long long item = (long long)blockIdx.x * kInputWarps + warp;
-  const int t = (int)(item / heads), head = (int)(item % heads);
-  if (t >= n_tokens) return;
+  const int t = blockIdx.x, head = blockIdx.y * kInputWarps + warp;
+  if (head >= nq + 2 * nkv) return;
   const bool is_q = head < nq, is_v = head >= nq + nkv;
   const int h = is_q ? head : is_v ? head - nq - nkv : head - nq;
-  constexpr int kChunks = kMaxHeadDim / 128;
+  constexpr int kChunks = CHUNKS;
   float x[kChunks][4];
 #pragma unroll
   for (int c = 0; c < kChunks; ++c) {
@@ -199,23 +250,50 @@ qk_norm_rope_kv4_kernel(const T* qkv, int qkv_stride, T* q_out, int q_stride, bo
       float* row = rows[warp];
       const float2* cs = rope + (size_t)t * (rotary_dim / 2);
       const int half = rotary_dim / 2;
+      const bool inter = mode & kPairsInterleaved;
+      // products and sums rounded separately, as in the layers with a wider cache
+      auto first = [](float a, float b, float2 w) { return __fsub_rn(__fmul_rn(a, w.x), __fmul_rn(b, w.y)); };
+      auto second = [](float a, float b, float2 w) { return __fadd_rn(__fmul_rn(a, w.y), __fmul_rn(b, w.x)); };
+      if (!inter) {
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c)
-        if (128 * c + 4 * lane < d) *reinterpret_cast<float4*>(row + 128 * c + 4 * lane) = make_float4(x[c][0], x[c][1], x[c][2], x[c][3]);
-      __syncwarp();
+        for (int c = 0; c < kChunks; ++c)
+          if (128 * c + 4 * lane < d) *reinterpret_cast<float4*>(row + 128 * c + 4 * lane) = make_float4(x[c][0], x[c][1], x[c][2], x[c][3]);
+        __syncwarp();
+      }
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int e = 128 * c + 4 * lane + i;
+      for (int c = 0; c < kChunks; ++c) {
+        const int e = 128 * c + 4 * lane;
+        if (quads) {                                                      // four elements have four partners side by side
           if (e >= rotary_dim) continue;
-          const bool inter = mode & kPairsInterleaved, second = inter ? (e & 1) != 0 : e >= half;
-          const int pair = inter ? e / 2 : second ? e - half : e;
-          const float2 w = cs[pair];
-          const float other = row[inter ? e ^ 1 : second ? e - half : e + half];
-          // products and sums rounded separately, as in the layers with a wider cache
-          x[c][i] = second ? __fadd_rn(__fmul_rn(other, w.y), __fmul_rn(x[c][i], w.x)) : __fsub_rn(__fmul_rn(x[c][i], w.x), __fmul_rn(other, w.y));
+          if (inter) {
+            const float4 w = *reinterpret_cast<const float4*>(cs + e / 2);
+            const float a0 = x[c][0], b0 = x[c][1], a1 = x[c][2], b1 = x[c][3];
+            x[c][0] = first(a0, b0, make_float2(w.x, w.y)); x[c][1] = second(a0, b0, make_float2(w.x, w.y));
+            x[c][2] = first(a1, b1, make_float2(w.z, w.w)); x[c][3] = second(a1, b1, make_float2(w.z, w.w));
+          } else {
+            const bool upper = e >= half;
+            const float4* w4 = reinterpret_cast<const float4*>(cs + (upper ? e - half : e));
+            const float4 wa = w4[0], wb = w4[1], o = *reinterpret_cast<const float4*>(row + (upper ? e - half : e + half));
+            const float2 w[4] = {make_float2(wa.x, wa.y), make_float2(wa.z, wa.w), make_float2(wb.x, wb.y), make_float2(wb.z, wb.w)};
+            const float other[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[c][i] = upper ? second(other[i], x[c][i], w[i]) : first(x[c][i], other[i], w[i]);
+          }
+        } else {
+          float y[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            y[i] = x[c][i];
+            if (e + i >= rotary_dim) continue;
+            const bool upper = inter ? (i & 1) != 0 : e + i >= half;
+            const float2 w = cs[inter ? (e + i) / 2 : upper ? e + i - half : e + i];
+            const float other = inter ? x[c][i ^ 1] : row[upper ? e + i - half : e + i + half];
+            y[i] = upper ? second(other, x[c][i], w) : first(x[c][i], other, w);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[c][i] = y[i];
         }
+      }
       __syncwarp();
     }
     if (normed && (mode & kNormAfterRotation)) norm();
@@ -237,7 +315,7 @@ qk_norm_rope_kv4_kernel(const T* qkv, int qkv_stride, T* q_out, int q_stride, bo
     if (128 * c >= d) break;
     const int G = 4 * c + (lane >> 3);
     __nv_bfloat16 scale;
-    const uint32_t codes = is_v && sizeof(T) == 2 ? kv4_quantise<true>(x[c], scale) : kv4_quantise<false>(x[c], scale);
+    const uint32_t codes = sizeof(T) == 2 ? kv4_quantise<true>(x[c], scale) : kv4_quantise<false>(x[c], scale);
     const uint32_t pair = codes | (__shfl_down_sync(0xffffffffu, codes, 1) << 16);
     if (G * kKv4Group >= d) continue;
     if (is_v) *reinterpret_cast<uint16_t*>(unit + kv4_value_at(d, j, G, l)) = (uint16_t)codes;
@@ -391,16 +469,24 @@ ILB_EXPORT int ilb_kv4_write(const void* k, long long k_row, long long k_head, c
   ILB_REQUIRE(n_tokens >= 0 && (dtype == kF32 || dtype == kBF16), "kv4_write: bad sizes or types");
   ILB_REQUIRE((uintptr_t)cache % 16 == 0, "kv4_write: the cache must start on a 16-byte boundary");
   if (n_tokens == 0) return 0;
-  const long long groups = 2LL * n_tokens * nkv * (d / kKv4Group), blocks = (groups * 8 + kThreads - 1) / kThreads;
-  ILB_REQUIRE(blocks <= 0x7fffffffLL, "kv4_write: too many tokens for one launch");
   const bool wide = (((uintptr_t)k | (uintptr_t)v) % (dtype == kF32 ? 16 : 8)) == 0 && ((k_row | k_head | v_row | v_head) & 3) == 0;
-  if (dtype == kF32)
-    ilb::launch(kv4_write_kernel<float>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, (const float*)k, k_row, k_head, (const float*)v, v_row,
-                v_head, wide, positions, seq_of_token, block_table, max_blocks, page_size, num_pages, (uint8_t*)cache, n_tokens, nkv, d);
-  else
-    ilb::launch(kv4_write_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, (const __nv_bfloat16*)k, k_row, k_head,
-                (const __nv_bfloat16*)v, v_row, v_head, wide, positions, seq_of_token, block_table, max_blocks, page_size, num_pages,
-                (uint8_t*)cache, n_tokens, nkv, d);
+  const long long lanes = 2LL * nkv * d / 4, rows = (lanes + kThreads - 1) / kThreads;
+  ILB_REQUIRE(rows <= 65535, "kv4_write: too many heads for one launch");
+  const int tokens = n_tokens >= 256 ? 4 : 1;                             // (fewer tokens do not fill the device four at a time)
+  const dim3 grid((unsigned)((n_tokens + tokens - 1) / tokens), (unsigned)rows);
+#define ILB_KV4_WRITE(T, TOKENS, DIM)                                                                                                            \
+  ilb::launch(kv4_write_kernel<T, TOKENS, DIM>, grid, dim3(kThreads), 0, stream, (const T*)k, k_row, k_head, (const T*)v, v_row, v_head, wide, positions, \
+              seq_of_token, block_table, max_blocks, page_size, num_pages, (uint8_t*)cache, n_tokens, nkv, d)
+  if (dtype == kF32) {
+    if (tokens == 4 && d == 128) ILB_KV4_WRITE(float, 4, 128);
+    else if (tokens == 4) ILB_KV4_WRITE(float, 4, 0);
+    else ILB_KV4_WRITE(float, 1, 0);
+  } else {
+    if (tokens == 4 && d == 128) ILB_KV4_WRITE(__nv_bfloat16, 4, 128);
+    else if (tokens == 4) ILB_KV4_WRITE(__nv_bfloat16, 4, 0);
+    else ILB_KV4_WRITE(__nv_bfloat16, 1, 0);
+  }
+#undef ILB_KV4_WRITE
   return check_launch("kv4_write");
 }
 
@@ -448,15 +534,23 @@ ILB_EXPORT int ilb_qk_norm_rope_kv4(const void* qkv, int qkv_stride, void* q_out
   ILB_REQUIRE(mode >= 0 && mode < 8 && qkv_stride >= (nq + 2 * nkv) * d && q_stride >= nq * d && q_stride % 4 == 0, "qk_norm_rope_kv4: unknown mode or rows too short");
   ILB_REQUIRE((((uintptr_t)cache | (uintptr_t)q_out) % 16) == 0, "qk_norm_rope_kv4: cache and queries must start on 16-byte boundaries");
   if (n_tokens == 0) return 0;
-  const long long blocks = ((long long)n_tokens * (nq + 2 * nkv) + kInputWarps - 1) / kInputWarps;
-  ILB_REQUIRE(blocks <= 0x7fffffffLL, "qk_norm_rope_kv4: too many tokens for one launch");
+  const dim3 grid((unsigned)n_tokens, (unsigned)((nq + 2 * nkv + kInputWarps - 1) / kInputWarps));
+  ILB_REQUIRE(grid.y <= 65535, "qk_norm_rope_kv4: too many heads for one launch");
   const bool wide = (uintptr_t)qkv % (dtype == kF32 ? 16 : 8) == 0 && qkv_stride % 4 == 0;
-#define ILB_KV4_INPUT(T)                                                                                                                          \
-  ilb::launch(qk_norm_rope_kv4_kernel<T>, dim3((unsigned)blocks), dim3(kInputWarps * 32), 0, stream, (const T*)qkv, qkv_stride, (T*)q_out, q_stride, wide, \
-              q_weight, k_weight, eps, (const float2*)rope, rope ? rotary_dim : 0, mode, positions, seq_of_token, block_table, max_blocks, page_size,      \
-              num_pages, (uint8_t*)cache, n_tokens, nq, nkv, d)
-  if (dtype == kF32) ILB_KV4_INPUT(float);
-  else ILB_KV4_INPUT(__nv_bfloat16);
+  const bool quads = rope != nullptr && rotary_dim % 8 == 0 && (uintptr_t)rope % 16 == 0;
+#define ILB_KV4_INPUT(T, CHUNKS)                                                                                                                  \
+  ilb::launch(qk_norm_rope_kv4_kernel<T, CHUNKS>, grid, dim3(kInputWarps * 32), 0, stream, (const T*)qkv, qkv_stride, (T*)q_out, q_stride, wide, q_weight, \
+              k_weight, eps, (const float2*)rope, rope ? rotary_dim : 0, mode, positions, seq_of_token, block_table, max_blocks, page_size, num_pages,     \
+              (uint8_t*)cache, nq, nkv, d, quads)
+  if (dtype == kF32) {
+    if (d <= 128) ILB_KV4_INPUT(float, 1);
+    else if (d <= 256) ILB_KV4_INPUT(float, 2);
+    else ILB_KV4_INPUT(float, 4);
+  } else {
+    if (d <= 128) ILB_KV4_INPUT(__nv_bfloat16, 1);
+    else if (d <= 256) ILB_KV4_INPUT(__nv_bfloat16, 2);
+    else ILB_KV4_INPUT(__nv_bfloat16, 4);
+  }
 #undef ILB_KV4_INPUT
   return check_launch("qk_norm_rope_kv4");
 }

@@ -28,30 +28,40 @@ __device__ __forceinline__ int kv4_value_at(int d, int j, int G, int l) {
 }
 __device__ __forceinline__ int kv4_scale_at(int d, bool value, int j, int G) { return (value ? 17 : 16) * d + (j * (d / 32) + G) * 2; }
 
+// (x & mask) | bits, in one instruction (the compiler makes two of the expression).
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+  return y;
+}
+
 // Codes of a lane's four elements (16 bits, the first lowest) and the group's scale, from eight neighbouring lanes that hold a group.
-// ROUNDED: the elements are bfloat16 numbers.  Then x / s is a half exactly or at least 2^-12 (relatively) away from one, so a
-// product with the reciprocal, raised by 2^-20, lands on the same side as the quotient and no division is needed; a quotient of
-// 32-bit elements may be nearer to a half than a reciprocal can tell and is taken in full.
-template <bool ROUNDED>
+// BY_PRODUCT: x times the reciprocal of s, raised by 2^-20, in the quotient's place, exact where the elements are bfloat16 numbers:
+// x / s is then a half exactly or at least 2^-12 (relatively) away from one, the product is within 2^-22 of x / s (1 + 2^-20) and so lands
+// on the side that the quotient rounds to.  A quotient of 32-bit elements may be nearer to a half than a reciprocal can tell and is
+// taken in full where the definition counts to the last bit.
+template <bool BY_PRODUCT>
 __device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[4], __nv_bfloat16& scale) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);      // (ordered like the numbers, NaN above infinity)
+  uint32_t top = max(max(__float_as_uint(x[0]) & 0x7fffffffu, __float_as_uint(x[1]) & 0x7fffffffu),      // (ordered like the numbers, NaN above infinity)
+                     max(__float_as_uint(x[2]) & 0x7fffffffu, __float_as_uint(x[3]) & 0x7fffffffu));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 4));
   scale = __float2bfloat16_rn(__fmul_rn(__uint_as_float(top), 1.0f / 7.0f));
   const float s = __bfloat162float(scale);
-  if (top >= 0x7f800000u) scale = __ushort_as_bfloat16(0x7fc0);
-  else if (s < 1.17549435e-38f) scale = __ushort_as_bfloat16(0);
-  if (top >= 0x7f800000u || s < 1.17549435e-38f) return 0x8888u;
-  uint32_t codes = 0;
-  if (ROUNDED) {
-    const float inv = __fmul_rn(__frcp_rn(s), 1.0f + 0x1p-20f);
+  const bool none = top >= 0x7f800000u, flat = s < 1.17549435e-38f;
+  scale = none ? __ushort_as_bfloat16(0x7fc0) : flat ? __ushort_as_bfloat16(0) : scale;
+  uint32_t codes;
+  if (BY_PRODUCT) {
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    inv = __fmul_rn(inv, 1.0f + 0x1p-20f);
+    uint32_t c[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)      // 1.5 2^23 + 8: the sum's last bits are the rounded product plus 8
-      codes |= (__float_as_uint(__fmaf_rn(x[i], inv, 12582920.0f)) & 15u) << (4 * i);
+    for (int i = 0; i < 4; ++i) c[i] = __float_as_uint(__fmaf_rn(x[i], inv, 12582920.0f));      // 1.5 2^23 + 8: the sum's last bits are the rounded product plus 8
+    codes = and_or(c[3] << 12, 0xf000u, and_or(c[2] << 8, 0xf00u, and_or(c[1] << 4, 0xf0u, c[0] & 15u)));
   } else {
+    codes = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float y = __fdiv_rn(x[i], s), a = fabsf(y), w = truncf(a);
@@ -59,7 +69,7 @@ __device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[4], __nv_bfloa
       codes |= (uint32_t)(y < 0.f ? 8 - c : 8 + c) << (4 * i);
     }
   }
-  return codes;
+  return none || flat ? 0x8888u : codes;
 }
 
 }  // namespace ilb

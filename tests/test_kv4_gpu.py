@@ -72,6 +72,27 @@ def test_rows_are_kept_as_the_definition_says(ops, dtype, nkv, d, page):
         assert float((got != want).float().mean()) <= 1e-4
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [32, 128, 160])
+@pytest.mark.parametrize("starts,lens", [([0], [301]), ([7, 0, 250], [130, 1, 175])])
+def test_many_rows_are_kept_as_the_definition_says(ops, dtype, d, starts, lens):
+    """Steps long enough for the form that takes tokens by fours, cut anywhere, with a page that is not held."""
+    nkv, page, T = 3, 32, sum(lens)
+    table, pool = plain.make_table([a + n for a, n in zip(starts, lens)], page, 2, 1)
+    table[0, 1] = -1
+    step = plain.make_step(starts, lens, DEV)
+    k, v = random_rows(T, nkv, d, dtype, 11), random_rows(T, nkv, d, dtype, 12)
+    want = torch.zeros(plain_shape(pool, nkv, page, d), dtype=torch.uint8)
+    pos, seq = step.positions.cpu().long(), step.seq_of_token.cpu().long()
+    pages = table[seq, pos // page]
+    held = pages >= 0
+    plain.write(want, pages[held], (pos % page)[held], k[held], v[held])
+    got = torch.zeros_like(want, device=DEV)
+    ops.kv4_write(k.to(DEV), v.to(DEV), step, table.to(DEV), got)
+    wrong = float((got.cpu() != want).float().mean())
+    assert wrong == 0 if dtype == torch.bfloat16 else wrong <= 1e-4
+
+
 @pytest.mark.parametrize("odd", [1, 2, 3])
 def test_rows_on_any_element_boundary(ops, odd):
     """Rows that start where no vector load may."""
