@@ -30,6 +30,7 @@
 #include <cuda_fp16.h>
 #include <type_traits>
 #include "kv4.cuh"
+#include "packed.h"
 #include "sm100.cuh"
 
 using namespace ilb;
@@ -1036,5 +1037,8 @@ ILB_EXPORT int ilb_kv4_attention_simple(const void* q, void* out, int dtype, con
                 out_stride, sink);
   return check_launch("kv4_attention");
 }
+
+ILB_PACKED(ilb_kv4_attention_rows)
+ILB_PACKED(ilb_kv4_attention_simple)
 
 ILB_DEFINE_LAST_ERROR()

@@ -50,6 +50,7 @@
 #include <mutex>
 #include <unordered_map>
 #include "common.cuh"
+#include "packed.h"
 #include "sm100.cuh"
 
 using namespace ilb;
@@ -753,5 +754,7 @@ ILB_EXPORT int ilb_attention_prefill_half(const void* q, void* out, const void* 
     return d == 64 ? launch<64, 64, 2, false, true>(m, p, n_tiles, stream) : launch<128, 128, 2, false, true>(m, p, n_tiles, stream);
   return d == 64 ? launch<64, 64, 1, false, true>(m, p, n_tiles, stream) : launch<128, 128, 1, false, true>(m, p, n_tiles, stream);
 }
+
+ILB_PACKED(ilb_attention_prefill_half)
 
 ILB_DEFINE_LAST_ERROR()

@@ -1,6 +1,7 @@
 // Rows into the 4-bit key/value cache and back (format: kv4.cuh).
 #include <cuda_fp16.h>
 #include "kv4.cuh"
+#include "packed.h"
 
 using namespace ilb;
 
@@ -576,5 +577,10 @@ ILB_EXPORT int ilb_kv4_unpack(const void* cache, const int* block_table, int tab
 #undef ILB_KV4_UNPACK
   return check_launch("kv4_unpack");
 }
+
+ILB_PACKED(ilb_kv4_write)
+ILB_PACKED(ilb_kv4_read)
+ILB_PACKED(ilb_qk_norm_rope_kv4)
+ILB_PACKED(ilb_kv4_unpack)
 
 ILB_DEFINE_LAST_ERROR()

@@ -7,6 +7,7 @@ a library that cannot be built or loaded, raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import torch
@@ -59,8 +60,8 @@ LAUNCHES = 0          # kernels launched through this module since import
 
 _FUNCTIONS: dict = {}  # launcher name -> (function, its library)
 
-# Argument kinds of launchers whose calls pass plain numbers (p pointer, i int, q 64-bit int, f float): converted by ctypes at a
-# fraction of what wrapping every argument takes.  The others wrap theirs (`_i`, `_f`, `_ptr`).
+# Argument kinds of launchers that take their arguments as one packed record of plain numbers (packed.h; p pointer, i int, q 64-bit int,
+# f float).  The others' are wrapped one by one (`_i`, `_f`, `_ptr`).
 _SIGNATURES = {
     "ilb_kv4_write": "pqqpqqipppiiipiiip",
     "ilb_kv4_read": "ppipipiiiippiiip",
@@ -70,7 +71,6 @@ _SIGNATURES = {
     "ilb_kv4_attention_simple": "ppippppiiiifiiiiiipp",
     "ilb_kv4_attention_rows": "ppippppiiiifiiiiiiiipipqpqpp",
 }
-_KINDS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "q": ctypes.c_longlong, "f": ctypes.c_float}
 
 
 SCOPE = "other"       # the op class the next launches belong to (see `scope`)
@@ -90,14 +90,18 @@ def _call(module: str, fn: str, *args) -> None:
     entry = _FUNCTIONS.get(fn)
     if entry is None:
         lib = load_module(module)
-        f = getattr(lib, fn)
-        f.restype = ctypes.c_int
+        pack = None
         if fn in _SIGNATURES:
-            f.argtypes = [_KINDS[k] for k in _SIGNATURES[fn]]
-        entry = _FUNCTIONS[fn] = (f, lib)
+            f = getattr(lib, fn + "_packed")
+            f.argtypes = [ctypes.c_char_p]
+            pack = struct.Struct("@" + _SIGNATURES[fn].upper().replace("I", "i").replace("Q", "q").replace("F", "f")).pack
+        else:
+            f = getattr(lib, fn)
+        f.restype = ctypes.c_int
+        entry = _FUNCTIONS[fn] = (f, lib, pack)
     timer = TIMER
     begin = timer.node_begin() if timer is not None else None
-    rc = entry[0](*args)
+    rc = entry[0](*args) if entry[2] is None else entry[0](entry[2](*args))
     if rc != 0:
         raise KernelError(entry[1].ilb_last_error().decode())
     if begin is not None:
@@ -1732,9 +1736,9 @@ def qk_norm_rope_kv4(qkv: torch.Tensor, q_out: torch.Tensor, q_weight: Optional[
             or any(w is not None and w.numel() != d for w in (q_weight, k_weight)):
         raise KernelError("qk_norm_rope_kv4: projection, queries, weights, angles and step do not agree")
     _call("kv4", "ilb_qk_norm_rope_kv4", qkv.data_ptr(), qkv.stride(0), q_out.data_ptr(), nq * d, _code(qkv),
-          None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps,
-          None if rope is None else rope.data_ptr(), rotary_dim, mode, step.positions.data_ptr(), step.seq_of_token.data_ptr(), block_table.data_ptr(),
-          block_table.shape[1], page_size, num_pages, cache.data_ptr() if write else None, T, nq, nkv, d, _raw_stream(cache))
+          0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), eps,
+          0 if rope is None else rope.data_ptr(), rotary_dim, mode, step.positions.data_ptr(), step.seq_of_token.data_ptr(), block_table.data_ptr(),
+          block_table.shape[1], page_size, num_pages, cache.data_ptr() if write else 0, T, nq, nkv, d, _raw_stream(cache))
 
 
 def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, out_table: torch.Tensor, k_out: torch.Tensor,
@@ -1800,7 +1804,7 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
         return
     window, device, code = window or 0, q.device, F32 if dtype is torch.float32 else _code(q)
     at, to, held = q.data_ptr(), out.data_ptr(), cache.data_ptr()
-    sinks = None if sink is None else sink.data_ptr()
+    sinks = 0 if sink is None else sink.data_ptr()
     if d not in KV4_ROWS_HEADS or (at | to | held) % 16:
         _need(step.seq_of_token, "kv4_attention sequence indices", torch.int32)
         _call("attention_kv4", "ilb_kv4_attention_simple", at, to, code, held, positions.data_ptr(), step.seq_of_token.data_ptr(),
@@ -1838,7 +1842,7 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
         if lib.ilb_kv4_attention_rows_plan(*map(_i, key), *map(ctypes.byref, found)) != 0:
             raise KernelError(lib.ilb_last_error().decode())
         plan = _KV4_PLANS[key] = (found[0].value, found[1].value)
-    scratch = tickets = None
+    scratch = tickets = 0
     if plan[0]:
         scratch = ws.address("kv4.records", plan[0], torch.float32)
         tickets = ws.address("kv4.tickets", max(plan[1], 4096), torch.int32, True)
@@ -1858,7 +1862,7 @@ def _kv4_portions(q, out, cache, step, block_table, a: int, b: int, tiles: int, 
     if order is None or order.numel() < n * tiles:       # page s * tiles + t holds tile t of sequence s
         order = _KV4_ORDER[device] = torch.arange(max(n * tiles, 1 << 14), dtype=torch.int32, device=device)
     positions, cu_q, stream = step.positions.data_ptr(), step.cu_q.data_ptr() + 4 * a, _raw_stream(q)
-    sinks = None if sink is None else sink.data_ptr()
+    sinks = 0 if sink is None else sink.data_ptr()
     _call("kv4", "ilb_kv4_unpack", cache.data_ptr(), block_table.data_ptr() + 4 * a * block_table.shape[1], block_table.shape[1],
           step.kv_len.data_ptr() + 4 * a, positions, cu_q, window, cache.shape[2] * KV4_UNIT, cache.shape[0], n, tiles, nkv, d, k, v, info,
           q.data_ptr(), q_half, q_power, nq, sum(lens) * nq, stream)
