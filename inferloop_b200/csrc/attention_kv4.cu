@@ -51,6 +51,7 @@ struct Params {
   float* scratch; int* tickets; int* error_flag;
   int max_blocks, page_size, num_pages, window, nq, nkv, q_stride, out_stride, row_blocks, max_tokens;
   int single;                              // every sequence brings one token
+  int unit_shift;                          // log2 of the units of a page, or -1
   int n_z, slots;                          // (sequence, block of rows) pairs; CTAs at work at once, or 0: a CTA a block
   float scale_log2;
 };
@@ -192,6 +193,13 @@ inline long long most_ctas(long long blocks, long long slots) {
   return blocks < slots && slots < by_average ? by_average : blocks < slots ? slots : by_average;
 }
 
+// a / b for a >= 0, b > 0 and a quotient below 2^20: a float's quotient is at most one off.
+__device__ __forceinline__ int quotient(int a, int b) {
+  int q = (int)__fdividef((float)a, (float)b);
+  const int rest = a - q * b;
+  return q + (rest >= b ? 1 : 0) - (rest < 0 ? 1 : 0);
+}
+
 // Warps that an SM has registers for: those of few rows' state (NB = 1 up to D = 128), half as many otherwise.
 template <int D, int NB> constexpr int kSmWarps = NB == 1 && D <= 128 ? 16 : 8;
 
@@ -261,14 +269,18 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
     mine4 = block_of(z = 0);
     const int n = pairs_of(mine4);
     if (n == 0) return;
-    runs = (n + longest_run(n * p.nkv, p.nkv, p.slots, kWarps) - 1) / longest_run(n * p.nkv, p.nkv, p.slots, kWarps);
-    head = blockIdx.x / runs;
-    run = blockIdx.x % runs;
+    const int longest = longest_run(n * p.nkv, p.nkv, p.slots, kWarps);
+    runs = quotient(n + longest - 1, longest);
+    head = quotient(blockIdx.x, runs);
+    run = blockIdx.x - head * runs;
     place = head * runs;
     if (head >= p.nkv) return;
   } else {
-    int total = 0;
-    for (int z0 = lane; z0 < p.n_z; z0 += 32) total += pairs_of(block_of(z0));
+    int first[2];                                                         // (64 blocks' stay for the second pass)
+    first[0] = lane < p.n_z ? pairs_of(block_of(lane)) : 0;
+    first[1] = lane + 32 < p.n_z ? pairs_of(block_of(lane + 32)) : 0;
+    int total = first[0] + first[1];
+    for (int z0 = lane + 64; z0 < p.n_z; z0 += 32) total += pairs_of(block_of(z0));
 #pragma unroll
     for (int o = 16; o > 0; o /= 2) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (total == 0) return;
@@ -276,8 +288,8 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
     int before = 0;
     z = -1;
     for (int z0 = 0; z0 < p.n_z && z < 0; z0 += 32) {
-      const int4 b = z0 + lane < p.n_z ? block_of(z0 + lane) : make_int4(0, 0, -1, -1);
-      const int cuts = (pairs_of(b) + longest - 1) / longest;             // CTAs a head
+      const int pairs = z0 == 0 ? first[0] : z0 == 32 ? first[1] : z0 + lane < p.n_z ? pairs_of(block_of(z0 + lane)) : 0;
+      const int cuts = quotient(pairs + longest - 1, longest);            // CTAs a head
       int upto = cuts * p.nkv;
 #pragma unroll
       for (int o = 1; o < 32; o *= 2) {
@@ -290,9 +302,9 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
         z = z0 + at;
         runs = __shfl_sync(0xffffffffu, cuts, at);
         const int local = (int)blockIdx.x - before - __shfl_sync(0xffffffffu, upto, at) + runs * p.nkv;
-        mine4 = make_int4(__shfl_sync(0xffffffffu, b.x, at), __shfl_sync(0xffffffffu, b.y, at), __shfl_sync(0xffffffffu, b.z, at), __shfl_sync(0xffffffffu, b.w, at));
-        head = local / runs;
-        run = local % runs;
+        mine4 = block_of(z);
+        head = quotient(local, runs);
+        run = local - head * runs;
         place = (int)blockIdx.x - run;
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
@@ -313,12 +325,13 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
   uint32_t there_now = 0;                                                 // bit 2 i + h: it is held
   auto unit_of = [&](int i0) { return 2 * (begin + warp + (i0 + (lane >> 1)) * kWarps) + (lane & 1); };
   auto page_of = [&](int i0) {                                            // (its load may be waited for later)
-    const int u = unit_of(i0), blk = (unit0 + u) / upp;
+    const int u = unit_of(i0), blk = p.unit_shift >= 0 ? (unit0 + u) >> p.unit_shift : (unit0 + u) / upp;
     return i0 + (lane >> 1) < mine && u < n_units && blk < p.max_blocks ? table[blk] : -1;
   };
   auto look_up = [&](int i0, int page) {
     const bool is_held = page >= 0 && page < p.num_pages;
-    src_unit = is_held ? p.cache + (((size_t)page * p.nkv + head) * upp + (unit0 + unit_of(i0)) % upp) * U : nullptr;
+    const int in_page = p.unit_shift >= 0 ? (unit0 + unit_of(i0)) & (upp - 1) : (unit0 + unit_of(i0)) % upp;
+    src_unit = is_held ? p.cache + (((size_t)page * p.nkv + head) * upp + in_page) * U : nullptr;
     there_now = __ballot_sync(0xffffffffu, is_held);
   };
   uint32_t asked = 0;                                                     // two bits a pair on its way: which of its units come
@@ -344,12 +357,17 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
   };
   constexpr int kItems = (NB * NG + kWarps - 1) / kWarps;
   uint4 raw[PIECES == 1 ? NG : 1], own[PIECES == 1 ? kItems : 1];
+  auto ask_row = [&](const T* src) {
+#pragma unroll
+    for (int G32 = 0; G32 < NG; ++G32) raw[G32] = src != nullptr ? *reinterpret_cast<const uint4*>(src + G32 * 32) : make_uint4(0u, 0u, 0u, 0u);
+  };
   if constexpr (PIECES == 1) {
 #pragma unroll
     for (int j = 0; j < kItems; ++j) {
       const int item = warp + j * kWarps, nb = item / NG;
       const T* src = item < NB * NG ? row_at(nb) : nullptr;
       own[j] = src != nullptr ? *reinterpret_cast<const uint4*>(src + item % NG * 32) : make_uint4(0u, 0u, 0u, 0u);
+      if (kItems == 1) ask_row(src);
     }
   }
   if (mine > 0) {
@@ -363,10 +381,8 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
     for (int j = 0; j < kItems; ++j) {
       const int item = warp + j * kWarps, nb = item / NG;
       if (item >= NB * NG) break;
-      const T* src = row_at(nb);
+      if (kItems > 1) ask_row(row_at(nb));
       uint32_t top = 0;
-#pragma unroll
-      for (int G32 = 0; G32 < NG; ++G32) raw[G32] = src != nullptr ? *reinterpret_cast<const uint4*>(src + G32 * 32) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
       for (int G32 = 0; G32 < NG; ++G32) {
         const uint32_t w[4] = {raw[G32].x, raw[G32].y, raw[G32].z, raw[G32].w};
@@ -1005,8 +1021,11 @@ ILB_EXPORT int ilb_kv4_attention_rows(const void* q, void* out, int dtype, const
   ILB_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache | (uintptr_t)scratch) % 16 == 0 && q_stride % 8 == 0 && out_stride % 8 == 0,
               "kv4_attention: queries, output, cache and scratch must start on 16-byte boundaries");
   if (n_seqs == 0) return 0;
+  int shift = -1;
+  for (int i = 0; i < 20; ++i)
+    if (page_size / kKv4Unit == 1 << i) shift = i;
   Params p = {q, out, (const uint8_t*)cache, positions, cu_q, block_table, sink, scratch, tickets, error_flag, max_blocks, page_size, num_pages, window,
-              nq, nkv, q_stride, out_stride, pl.row_blocks, max_tokens, single, pl.n_z, pl.slots, scale * kLog2e};
+              nq, nkv, q_stride, out_stride, pl.row_blocks, max_tokens, single, shift, pl.n_z, pl.slots, scale * kLog2e};
   const dim3 grid = pl.slots > 0 ? dim3((unsigned)pl.ctas) : dim3(1, (unsigned)nkv, (unsigned)pl.n_z);
   const bool wide = rows_per_block(dtype, max_tokens * (nq / nkv), d) == 16;
   switch (d) {
