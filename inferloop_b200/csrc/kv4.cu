@@ -1,5 +1,6 @@
 // Rows into the 4-bit key/value cache and back (format: kv4.cuh).
 #include <cuda_fp16.h>
+#include <type_traits>
 #include "kv4.cuh"
 #include "packed.h"
 
@@ -37,18 +38,16 @@ __device__ __forceinline__ void store4(float* p, const float (&x)[4]) { *reinter
 
 constexpr int kThreads = 128, kMaxHeadDim = 512;
 
-// Eight lanes a group of 32 elements: maximum over them, four codes each, 16 bits of V or (two lanes together) a word of K.  A thread has
-// one place of the rows (keys or values, head, group, four elements) of TOKENS tokens in a row, all asked for before any is looked
-// at: with one token a thread the chain of loads (position, page, store) was most of the time (2,048 tokens of 8 heads of 128: 9 us, four a
-// thread 5).
-template <typename T, int TOKENS, int DIM>
+// Rows of any type, stride and head size.  Eight lanes a group of 32 elements: maximum over them, four codes each, 16 bits of V or (two
+// lanes together) a word of K.  A thread has one place of the rows (keys or values, head, group, four elements) of TOKENS tokens in a
+// row, all asked for before any is looked at: the chain of loads (position, page, store) is most of its time.
+template <typename T, int TOKENS>
 __global__ void __launch_bounds__(kThreads)
 kv4_write_kernel(const T* k, long long k_row, long long k_head, const T* v, long long v_row, long long v_head,
                  bool wide, const int* positions, const int* seq_of_token, const int* block_table,
-                 int max_blocks, int page_size, int num_pages, uint8_t* cache, int n_tokens, int nkv, int d_any) {
+                 int max_blocks, int page_size, int num_pages, uint8_t* cache, int n_tokens, int nkv, int d) {
   pdl_launch_dependents();
   pdl_wait();
-  const int d = DIM > 0 ? DIM : d_any;
   const int per_row = d / kKv4Group, at = (blockIdx.y * kThreads + threadIdx.x) >> 3;        // group of (k | v, head)
   const int l = threadIdx.x & 7, G = at % per_row, head = at / per_row % nkv, value = at / per_row / nkv;
   const long long t0 = (long long)blockIdx.x * TOKENS;
@@ -72,52 +71,19 @@ kv4_write_kernel(const T* k, long long k_row, long long k_head, const T* v, long
     place = pos % kKv4Unit;
   }
   const size_t unit_bytes = kv4_unit_bytes(d);
-  constexpr bool kTurn = TOKENS == 4 && DIM == 128;
   uint32_t codes[TOKENS];
   __nv_bfloat16 scale[TOKENS];
 #pragma unroll
   for (int i = 0; i < TOKENS; ++i) codes[i] = kv4_quantise<sizeof(T) == 2>(x[i], scale[i]);
-  if constexpr (kTurn) {
-    // A warp holds a row of each of four tokens: lane (G, l) trades its 16 bits of the four tokens for those of the four groups of token G,
-    // eight bytes of values, and of keys after a trade with its neighbour: a store of eight bytes in place of four of two.
-    const int g = lane >> 3;
-    uint32_t mine4[4];                                                    // [group] of token g
-#pragma unroll
-    for (int i = 0; i < 4; ++i) mine4[i] = 0;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {                                         // round r: the lane r groups further has this lane's token, and wants that one's
-      const int send = (g - r) & 3;
-      const uint32_t out = send == 0 ? codes[0] : send == 1 ? codes[1] : send == 2 ? codes[2] : codes[3];
-      const uint32_t in = __shfl_sync(0xffffffffu, out, ((g + r) & 3) * 8 + l);
-      const int from = (g + r) & 3;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mine4[i] = from == i ? in : mine4[i];
-    }
-    uint32_t lo = mine4[0] | mine4[1] << 16, hi = mine4[2] | mine4[3] << 16;      // values: the groups' half-words lie side by side
-    if (!value) {                                                         // keys: words of one group, halves of l and l + 1
-      const uint32_t other_lo = __shfl_xor_sync(0xffffffffu, lo, 1), other_hi = __shfl_xor_sync(0xffffffffu, hi, 1);
-      const uint32_t a = l & 1 ? other_hi : lo, b = l & 1 ? hi : other_lo;        // even lanes take groups 0 and 1, odd ones 2 and 3
-      lo = __byte_perm(a, b, 0x5410);
-      hi = __byte_perm(a, b, 0x7632);
-    }
-    const long long at_unit = __shfl_sync(0xffffffffu, where, g);
-    const int j = __shfl_sync(0xffffffffu, place, g);
-    if (at_unit >= 0 && mine) {
-      uint8_t* unit = cache + (size_t)(at_unit + (long long)head * upp) * unit_bytes;
-      *reinterpret_cast<uint2*>(unit + (value ? kv4_value_at(d, j, 0, l) : kv4_key_at(d, j, 0, l & 6) + 8 * (l & 1))) = make_uint2(lo, hi);
-    }
-  }
 #pragma unroll
   for (int i = 0; i < TOKENS; ++i) {
     const long long at_unit = __shfl_sync(0xffffffffu, where, i);
     const int j = __shfl_sync(0xffffffffu, place, i);
-    const uint32_t pair = kTurn ? 0u : codes[i] | (__shfl_down_sync(0xffffffffu, codes[i], 1) << 16);
+    const uint32_t pair = codes[i] | (__shfl_down_sync(0xffffffffu, codes[i], 1) << 16);
     if (at_unit < 0 || !mine) continue;
     uint8_t* unit = cache + (size_t)(at_unit + (long long)head * upp) * unit_bytes;
-    if constexpr (!kTurn) {
-      if (value) *reinterpret_cast<uint16_t*>(unit + kv4_value_at(d, j, G, l)) = (uint16_t)codes[i];
-      else if ((l & 1) == 0) *reinterpret_cast<uint32_t*>(unit + kv4_key_at(d, j, G, l)) = pair;
-    }
+    if (value) *reinterpret_cast<uint16_t*>(unit + kv4_value_at(d, j, G, l)) = (uint16_t)codes[i];
+    else if ((l & 1) == 0) *reinterpret_cast<uint32_t*>(unit + kv4_key_at(d, j, G, l)) = pair;
     if (l == 0) *reinterpret_cast<__nv_bfloat16*>(unit + kv4_scale_at(d, value, j, G)) = scale[i];
   }
 }
@@ -200,7 +166,7 @@ kv4_read_kernel(const uint8_t* cache, const int* block_table, int table_stride, 
 }
 
 // The input stage of a layer whose cache is held in 4 bits: per-head norm and rotation of queries and keys as in qk_norm_rope.cu (its modes),
-// in 32 bits, queries out, keys and values into the cache.  A warp a (token, head), four elements a lane and 128 of them; rotation
+// in 32 bits, queries out, keys and values into the cache; what kv4_wide_kernel does not take.  A warp a (token, head), four elements a lane and 128 of them; rotation
 // partners through shared memory.  Keys are quantised from their 32-bit values (in the
 // bfloat16 engine by the product: a quotient within 2^-20 of a half may go either way), values as kv4_write does.
 constexpr int kInputWarps = 8;
@@ -323,6 +289,170 @@ qk_norm_rope_kv4_kernel(const T* qkv, int qkv_stride, T* q_out, int q_stride, bo
     else if ((l & 1) == 0) *reinterpret_cast<uint32_t*>(unit + kv4_key_at(d, j, G, l)) = pair;
     if (l == 0) *reinterpret_cast<__nv_bfloat16*>(unit + kv4_scale_at(d, is_v, j, G)) = scale;
   }
+}
+
+// ------------------------------------------------------------------ rows of bfloat16 in vectors
+// kv4_write and the input stage for what nearly every call brings: bfloat16, heads of 64 or 128, rows on 16-byte boundaries, a rotation
+// of the whole head by halves behind the norm.  A lane has eight elements of a row's lower half and their partners of the upper, so
+// that the rotation needs no other lane, D / 16 lanes a row; a group of 32 is a word each of four lanes, of keys a word in the cache.
+// A warp has the same heads of one token in all its passes, with one look at the angles and the weights.  Its time is instructions (loads, codes, the norm):
+// 32 + 16 heads of 128, 2,048 tokens: 11.1 us for 44 MB (4.0 TB/s; the stage of a bfloat16 cache 10.6, four elements a lane and a row a warp 28),
+// 64 tokens 2.8, one 2.0.  Keys and values alone, 8 + 8 heads of 128: 1, 64, 2,048 and 8,192 tokens 1.7, 2.1, 4.3 and 12.8 us, the last 3.4 TB/s;
+// rows of four lanes' elements, four tokens a thread: 1.9, 2.1, 7.5 and 26.8.
+struct WideArgs {
+  const __nv_bfloat16 *q, *k, *v;                                         // q: null where only keys and values are written
+  long long q_row, k_row, k_head, v_row, v_head;
+  __nv_bfloat16* q_out;
+  int q_stride;
+  const float *q_weight, *k_weight;
+  float eps;
+  const float2* rope;
+  bool normed;
+  const int *positions, *seq_of_token, *block_table;
+  int max_blocks, page_size, num_pages;
+  uint8_t* cache;
+  int n_tokens, nq, nkv;
+};
+
+constexpr int kWideWarps = 8;
+
+__device__ __forceinline__ void unpack8(uint4 w, float (&x)[8]) {
+  const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(r[i] << 16); x[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u); }
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    r[i] = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+template <int D, int PASSES, bool STAGE>
+__global__ void __launch_bounds__(kWideWarps * 32)
+kv4_wide_kernel(const WideArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int LANES = D / 16, ROWS = 32 / LANES, H = PASSES * ROWS;     // lanes a row, rows a pass, heads a warp
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LANES;
+  const int t = blockIdx.x * kWideWarps + warp;
+  if (t >= a.n_tokens) return;
+  const int q_chunks = STAGE ? (a.nq + H - 1) / H : 0, kv_chunks = (a.nkv + H - 1) / H;
+  const int part = (int)blockIdx.y < q_chunks ? 0 : (int)blockIdx.y < q_chunks + kv_chunks ? 1 : 2;
+  const int head0 = ((int)blockIdx.y - (part == 0 ? 0 : part == 1 ? q_chunks : q_chunks + kv_chunks)) * H + lane / LANES, heads = part == 0 ? a.nq : a.nkv;
+  const __nv_bfloat16* src = part == 0 ? a.q + t * a.q_row : part == 1 ? a.k + t * a.k_row : a.v + t * a.v_row;
+  const long long apart = part == 0 ? D : part == 1 ? a.k_head : a.v_head;
+  uint4 raw[PASSES][2];
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const uint4* row = reinterpret_cast<const uint4*>(src + (head0 + p * ROWS) * apart) + l;
+    raw[p][0] = raw[p][1] = make_uint4(0u, 0u, 0u, 0u);
+    if (head0 + p * ROWS < heads) { raw[p][0] = row[0]; raw[p][1] = row[LANES]; }
+  }
+  uint8_t* unit = nullptr;                                                // of head 0
+  int j = 0;
+  const int upp = a.page_size / kKv4Unit;
+  if (part != 0) {
+    if (a.cache == nullptr) return;
+    const int pos = a.positions[t], u = pos / kKv4Unit, blk = u / upp;
+    const int page = pos >= 0 && blk < a.max_blocks ? a.block_table[(size_t)a.seq_of_token[t] * a.max_blocks + blk] : -1;
+    if (page < 0 || page >= a.num_pages) return;                          // never outside the pool
+    unit = a.cache + ((size_t)page * a.nkv * upp + (u - blk * upp)) * kv4_unit_bytes(D);
+    j = pos % kKv4Unit;
+  }
+  float w[2][8];                                                          // the norm's weights
+  float2 cs[8];                                                           // cosines and sines
+  if constexpr (STAGE) {
+    const float* weight = part == 0 ? a.q_weight : a.k_weight;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[0][i] = w[1][i] = 1.f;
+    if (part != 2 && weight != nullptr) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          const float4 m = *reinterpret_cast<const float4*>(weight + h * (D / 2) + 8 * l + i);
+          w[h][i] = m.x; w[h][i + 1] = m.y; w[h][i + 2] = m.z; w[h][i + 3] = m.w;
+        }
+    }
+    if (part != 2 && a.rope != nullptr) {
+      const float4* at = reinterpret_cast<const float4*>(a.rope + (size_t)t * (D / 2) + 8 * l);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { const float4 c = at[i]; cs[2 * i] = make_float2(c.x, c.y); cs[2 * i + 1] = make_float2(c.z, c.w); }
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const int head = head0 + p * ROWS;
+    float x[2][8];
+    unpack8(raw[p][0], x[0]);
+    unpack8(raw[p][1], x[1]);
+    if (STAGE && part != 2) {
+      if (a.normed) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ss = fmaf(x[i / 8][i % 8], x[i / 8][i % 8], ss);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float inv = 1.0f / sqrtf(ss / (float)D + a.eps);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i / 8][i % 8] = x[i / 8][i % 8] * inv * w[i / 8][i % 8];
+      }
+      if (a.rope != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {                                     // products and sums rounded separately, as in the layers with a wider cache
+          const float lo = x[0][i], hi = x[1][i];
+          x[0][i] = __fsub_rn(__fmul_rn(lo, cs[i].x), __fmul_rn(hi, cs[i].y));
+          x[1][i] = __fadd_rn(__fmul_rn(lo, cs[i].y), __fmul_rn(hi, cs[i].x));
+        }
+      }
+      if (part == 0) {
+        if (head < heads) {
+          uint4* to = reinterpret_cast<uint4*>(a.q_out + (size_t)t * a.q_stride + (size_t)head * D) + l;
+          to[0] = pack8(x[0]);
+          to[LANES] = pack8(x[1]);
+        }
+        continue;
+      }
+    }
+    __nv_bfloat16 scale[2];
+    const uint32_t lower = kv4_quantise8(x[0], scale[0]), upper = kv4_quantise8(x[1], scale[1]);
+    constexpr int NG = D / kKv4Group;
+    const int G = l / 4, e = l % 4;                                       // the lane's groups are G and G + NG / 2
+    uint8_t* here = unit + (size_t)head * upp * kv4_unit_bytes(D);
+    if (part == 1) {
+      if (head < heads) {
+        *reinterpret_cast<uint32_t*>(here + kv4_key_at(D, j, G, 2 * e)) = lower;
+        *reinterpret_cast<uint32_t*>(here + kv4_key_at(D, j, G + NG / 2, 2 * e)) = upper;
+      }
+    } else if constexpr (NG == 2) {                                       // half-words of the groups lie side by side
+      if (head < heads) {
+        *reinterpret_cast<uint32_t*>(here + kv4_value_at(D, j, 0, 2 * e)) = __byte_perm(lower, upper, 0x5410);
+        *reinterpret_cast<uint32_t*>(here + kv4_value_at(D, j, 0, 2 * e + 1)) = __byte_perm(lower, upper, 0x7632);
+      }
+    } else {                                                              // .. and two lanes hold them: lane G takes the half-words G of all
+      const uint32_t kept = __byte_perm(lower, upper, G == 0 ? 0x5410 : 0x7632);
+      const uint32_t got = __shfl_xor_sync(0xffffffffu, __byte_perm(lower, upper, G == 0 ? 0x7632 : 0x5410), 4);
+      const uint32_t even = G == 0 ? kept : got, odd = G == 0 ? got : kept;
+      if (head < heads)
+        *reinterpret_cast<uint2*>(here + kv4_value_at(D, j, 0, 2 * e + G)) = make_uint2(__byte_perm(even, odd, 0x5410), __byte_perm(even, odd, 0x7632));
+    }
+    if (e == 0 && head < heads) {
+      *reinterpret_cast<__nv_bfloat16*>(here + kv4_scale_at(D, part == 2, j, G)) = scale[0];
+      *reinterpret_cast<__nv_bfloat16*>(here + kv4_scale_at(D, part == 2, j, G + NG / 2)) = scale[1];
+    }
+  }
+}
+
+template <int D, bool STAGE, int PASSES>
+void launch_wide(const WideArgs& a, cudaStream_t stream) {
+  constexpr int H = PASSES * 512 / D;
+  const int chunks = (STAGE ? (a.nq + H - 1) / H : 0) + 2 * ((a.nkv + H - 1) / H);
+  ilb::launch(kv4_wide_kernel<D, PASSES, STAGE>, dim3((unsigned)((a.n_tokens + kWideWarps - 1) / kWideWarps), (unsigned)chunks), dim3(kWideWarps * 32), 0, stream, a);
 }
 
 // ------------------------------------------------------------------ operands of the prefill attention
@@ -471,21 +601,30 @@ ILB_EXPORT int ilb_kv4_write(const void* k, long long k_row, long long k_head, c
   ILB_REQUIRE((uintptr_t)cache % 16 == 0, "kv4_write: the cache must start on a 16-byte boundary");
   if (n_tokens == 0) return 0;
   const bool wide = (((uintptr_t)k | (uintptr_t)v) % (dtype == kF32 ? 16 : 8)) == 0 && ((k_row | k_head | v_row | v_head) & 3) == 0;
+  ILB_REQUIRE(nkv <= 16384, "kv4_write: too many heads for one launch");
+  if (dtype == kBF16 && (d == 64 || d == 128) && (((uintptr_t)k | (uintptr_t)v) % 16) == 0 && ((k_row | k_head | v_row | v_head) & 7) == 0) {
+    WideArgs w = {};
+    w.k = (const __nv_bfloat16*)k; w.v = (const __nv_bfloat16*)v;
+    w.k_row = k_row; w.k_head = k_head; w.v_row = v_row; w.v_head = v_head;
+    w.positions = positions; w.seq_of_token = seq_of_token; w.block_table = block_table;
+    w.max_blocks = max_blocks; w.page_size = page_size; w.num_pages = num_pages; w.cache = (uint8_t*)cache; w.n_tokens = n_tokens; w.nkv = nkv;
+    if (d == 64) launch_wide<64, false, 1>(w, stream);
+    else launch_wide<128, false, 1>(w, stream);
+    return check_launch("kv4_write");
+  }
   const long long lanes = 2LL * nkv * d / 4, rows = (lanes + kThreads - 1) / kThreads;
   ILB_REQUIRE(rows <= 65535, "kv4_write: too many heads for one launch");
-  const int tokens = n_tokens >= 256 ? 4 : 1;                             // (fewer tokens do not fill the device four at a time)
+  const int tokens = n_tokens >= 1024 ? 4 : 1;                            // (600 tokens of 8 heads of 128 in float32: 4.8 us by ones, 6.7 by fours; 2,048: 12.6 and 8.8)
   const dim3 grid((unsigned)((n_tokens + tokens - 1) / tokens), (unsigned)rows);
-#define ILB_KV4_WRITE(T, TOKENS, DIM)                                                                                                            \
-  ilb::launch(kv4_write_kernel<T, TOKENS, DIM>, grid, dim3(kThreads), 0, stream, (const T*)k, k_row, k_head, (const T*)v, v_row, v_head, wide, positions, \
+#define ILB_KV4_WRITE(T, TOKENS)                                                                                                                  \
+  ilb::launch(kv4_write_kernel<T, TOKENS>, grid, dim3(kThreads), 0, stream, (const T*)k, k_row, k_head, (const T*)v, v_row, v_head, wide, positions, \
               seq_of_token, block_table, max_blocks, page_size, num_pages, (uint8_t*)cache, n_tokens, nkv, d)
   if (dtype == kF32) {
-    if (tokens == 4 && d == 128) ILB_KV4_WRITE(float, 4, 128);
-    else if (tokens == 4) ILB_KV4_WRITE(float, 4, 0);
-    else ILB_KV4_WRITE(float, 1, 0);
+    if (tokens == 4) ILB_KV4_WRITE(float, 4);
+    else ILB_KV4_WRITE(float, 1);
   } else {
-    if (tokens == 4 && d == 128) ILB_KV4_WRITE(__nv_bfloat16, 4, 128);
-    else if (tokens == 4) ILB_KV4_WRITE(__nv_bfloat16, 4, 0);
-    else ILB_KV4_WRITE(__nv_bfloat16, 1, 0);
+    if (tokens == 4) ILB_KV4_WRITE(__nv_bfloat16, 4);
+    else ILB_KV4_WRITE(__nv_bfloat16, 1);
   }
 #undef ILB_KV4_WRITE
   return check_launch("kv4_write");
@@ -535,6 +674,18 @@ ILB_EXPORT int ilb_qk_norm_rope_kv4(const void* qkv, int qkv_stride, void* q_out
   ILB_REQUIRE(mode >= 0 && mode < 8 && qkv_stride >= (nq + 2 * nkv) * d && q_stride >= nq * d && q_stride % 4 == 0, "qk_norm_rope_kv4: unknown mode or rows too short");
   ILB_REQUIRE((((uintptr_t)cache | (uintptr_t)q_out) % 16) == 0, "qk_norm_rope_kv4: cache and queries must start on 16-byte boundaries");
   if (n_tokens == 0) return 0;
+  if (dtype == kBF16 && (d == 64 || d == 128) && (mode & (kPairsInterleaved | kNormAfterRotation)) == 0 && (rope == nullptr || rotary_dim == d) &&
+      (qkv_stride | q_stride) % 8 == 0 && (((uintptr_t)qkv | (uintptr_t)rope | (uintptr_t)q_weight | (uintptr_t)k_weight) % 16) == 0 &&
+      (q_weight == nullptr) == (k_weight == nullptr)) {
+    const __nv_bfloat16* rows = (const __nv_bfloat16*)qkv;
+    const WideArgs w = {rows, rows + (size_t)nq * d, rows + (size_t)(nq + nkv) * d, qkv_stride, qkv_stride, d, qkv_stride, d, (__nv_bfloat16*)q_out, q_stride, q_weight, k_weight,
+                        eps, (const float2*)rope, q_weight != nullptr || (mode & kNormUnweighted) != 0, positions, seq_of_token, block_table, max_blocks, page_size,
+                        num_pages, (uint8_t*)cache, n_tokens, nq, nkv};
+    // two rows a lane where there are many (48 heads of 128, us: 64 tokens 2.8 with one and 3.1 with two, 512 tokens 5.2 and 4.5, 2,048 13.5 and 11.1)
+    if (d == 64) n_tokens < 256 ? launch_wide<64, true, 1>(w, stream) : launch_wide<64, true, 2>(w, stream);
+    else n_tokens < 256 ? launch_wide<128, true, 1>(w, stream) : launch_wide<128, true, 2>(w, stream);
+    return check_launch("qk_norm_rope_kv4");
+  }
   const dim3 grid((unsigned)n_tokens, (unsigned)((nq + 2 * nkv + kInputWarps - 1) / kInputWarps));
   ILB_REQUIRE(grid.y <= 65535, "qk_norm_rope_kv4: too many heads for one launch");
   const bool wide = (uintptr_t)qkv % (dtype == kF32 ? 16 : 8) == 0 && qkv_stride % 4 == 0;

@@ -72,4 +72,24 @@ __device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[4], __nv_bfloa
   return none || flat ? 0x8888u : codes;
 }
 
+// The same of eight bfloat16 elements a lane (by the product), from four neighbouring lanes that hold a group.
+__device__ __forceinline__ uint32_t kv4_quantise8(const float (&x)[8], __nv_bfloat16& scale) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  scale = __float2bfloat16_rn(__fmul_rn(__uint_as_float(top), 1.0f / 7.0f));
+  const float s = __bfloat162float(scale);
+  const bool none = top >= 0x7f800000u, flat = s < 1.17549435e-38f;
+  scale = none ? __ushort_as_bfloat16(0x7fc0) : flat ? __ushort_as_bfloat16(0) : scale;
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  inv = __fmul_rn(inv, 1.0f + 0x1p-20f);
+  uint32_t codes = 0;
+#pragma unroll
+  for (int i = 7; i >= 0; --i) codes = codes << 4 | (__float_as_uint(__fmaf_rn(x[i], inv, 12582920.0f)) & 15u);
+  return none || flat ? 0x88888888u : codes;
+}
+
 }  // namespace ilb

@@ -141,6 +141,41 @@ def test_input_stage_keeps_what_the_write_keeps():
             assert not bool(cache.any())
 
 
+@pytest.mark.parametrize("d,nq,nkv", [(64, 9, 3), (128, 32, 8), (128, 5, 1), (64, 2, 2)])
+@pytest.mark.parametrize("starts,lens", [([30, 0], [2, 1]), ([0, 17], [260, 41])])
+@pytest.mark.parametrize("norm,turn", [(True, True), (False, True), (True, False), (False, False)])
+def test_input_stage_in_vectors_is_the_general_one(d, nq, nkv, starts, lens, norm, turn):
+    """Rows on 16-byte boundaries and off them, with one page not held.  Norms summed in another order are 2^-22 apart: queries a
+    rounding to bfloat16, values nothing, keys a code or scale whose rounding hung on it (1e-3 of the bytes at the most)."""
+    from inferloop_b200.csrc import ops
+    dev, T, page = "cuda:0", sum(lens), 32
+    gen = torch.Generator().manual_seed(6)
+    step = kv4_plain.make_step(starts, lens, dev)
+    table, pool = kv4_plain.make_table([a + n for a, n in zip(starts, lens)], page, 1, 3)
+    table[0, 0] = -1
+    table = table.to(dev)
+    width = (nq + 2 * nkv) * d
+    even = torch.randn(T, width + 8, generator=gen).to(torch.bfloat16).to(dev)
+    odd = torch.zeros(T, width + 9, dtype=torch.bfloat16, device=dev)
+    odd[:, 1:1 + width] = even[:, :width]
+    weights = [(1 + 0.1 * torch.randn(d, generator=gen)).to(dev) if norm else None for _ in range(2)]
+    angle = torch.rand(T, d // 2, generator=gen) * 6
+    rope = torch.stack([angle.cos(), angle.sin()], -1).contiguous().to(dev) if turn else None
+    found = []
+    for qkv in (even[:, :width], odd[:, 1:1 + width]):
+        q = torch.full((T, nq * d), 9.0, dtype=torch.bfloat16, device=dev)
+        cache = torch.zeros(ops.kv4_cache_shape(pool, nkv, page, d), dtype=torch.uint8, device=dev)
+        ops.qk_norm_rope_kv4(qkv, q, *weights, 1e-6, rope, d if turn else 0, step, table, cache, True, nq, nkv, d)
+        found.append((q.double(), cache))
+    (q, cache), (q_ref, ref) = found
+    assert bool(((q - q_ref).abs() <= 2.0 ** -7 * q_ref.abs() + 2.0 ** -20).all())
+    values = torch.zeros(18 * d, dtype=torch.bool, device=dev)
+    values[8 * d:16 * d] = values[17 * d:] = True
+    assert int(cache.sum()) > 0 and torch.equal(cache[..., values], ref[..., values])
+    wrong = float((cache != ref).float().mean())
+    assert wrong <= 1e-3 if norm else wrong == 0
+
+
 def test_refusals_of_the_engine(folders):
     from inferloop_b200 import Engine
     with pytest.raises(ValueError, match="auto or int4"):

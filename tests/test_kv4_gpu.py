@@ -93,6 +93,27 @@ def test_many_rows_are_kept_as_the_definition_says(ops, dtype, d, starts, lens):
     assert wrong == 0 if dtype == torch.bfloat16 else wrong <= 1e-4
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [96, 128])
+def test_rows_of_a_long_step_off_their_boundaries(ops, dtype, d):
+    starts, lens, nkv, page = [3, 0, 900], [701, 1, 445], 2, 64
+    T = sum(lens)
+    table, pool = plain.make_table([a + n for a, n in zip(starts, lens)], page, 2, 1)
+    table[2, 15] = -1
+    step = plain.make_step(starts, lens, DEV)
+    x = random_rows(T, 2 * nkv, d + 1, dtype, 13)
+    k, v = x[:, :nkv, 1:], x[:, nkv:, 1:]
+    want = torch.zeros(plain_shape(pool, nkv, page, d), dtype=torch.uint8)
+    pos, seq = step.positions.cpu().long(), step.seq_of_token.cpu().long()
+    pages = table[seq, pos // page]
+    held = pages >= 0
+    plain.write(want, pages[held], (pos % page)[held], k[held], v[held])
+    got, x = torch.zeros_like(want, device=DEV), x.to(DEV)
+    ops.kv4_write(x[:, :nkv, 1:], x[:, nkv:, 1:], step, table.to(DEV), got)
+    wrong = float((got.cpu() != want).float().mean())
+    assert wrong == 0 if dtype == torch.bfloat16 else wrong <= 1e-4
+
+
 @pytest.mark.parametrize("odd", [1, 2, 3])
 def test_rows_on_any_element_boundary(ops, odd):
     """Rows that start where no vector load may."""
