@@ -52,6 +52,7 @@ struct Params {
   int max_blocks, page_size, num_pages, window, nq, nkv, q_stride, out_stride, row_blocks, max_tokens;
   int single;                              // every sequence brings one token
   int unit_shift;                          // log2 of the units of a page, or -1
+  int group;                               // query heads of a kv head
   int n_z, slots;                          // (sequence, block of rows) pairs; CTAs at work at once, or 0: a CTA a block
   float scale_log2;
 };
@@ -179,6 +180,16 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[PIECE
   }
 }
 
+// a / b for a >= 0, b > 0: a float's quotient, off by 2^-20 of itself, and another one of what is left.
+__device__ __forceinline__ int quotient(int a, int b) {
+  const float inv = __fdividef(1.f, (float)b);
+  int q = (int)((float)a * inv), rest = a - q * b;
+  const int more = (int)((float)rest * inv);
+  q += more;
+  rest -= more * b;
+  return q + (rest >= b ? 1 : 0) - (rest < 0 ? 1 : 0);
+}
+
 // Pairs that a run has at most.  Fewer blocks than `slots`: so many that no more CTAs than slots come out, however the lengths lie.  More,
 // or nearly as many: half as much again as the slots' average, so that blocks of about one length stay whole (64 x 1,030 keys in 512 blocks:
 // 25 us, cut in two 33).  At least a pair a warp.
@@ -191,13 +202,6 @@ __device__ __forceinline__ int longest_run(int pairs, int blocks, int slots, int
 inline long long most_ctas(long long blocks, long long slots) {
   const long long by_average = blocks + (2 * slots + 2) / 3;
   return blocks < slots && slots < by_average ? by_average : blocks < slots ? slots : by_average;
-}
-
-// a / b for a >= 0, b > 0 and a quotient below 2^20: a float's quotient is at most one off.
-__device__ __forceinline__ int quotient(int a, int b) {
-  int q = (int)__fdividef((float)a, (float)b);
-  const int rest = a - q * b;
-  return q + (rest >= b ? 1 : 0) - (rest < 0 ? 1 : 0);
 }
 
 // Warps that an SM has registers for: those of few rows' state (NB = 1 up to D = 128), half as many otherwise.
@@ -243,10 +247,10 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
   __syncwarp();
   pdl_wait();
 
-  const int G = p.nq / p.nkv, upp = p.page_size / kKv4Unit;
+  const int G = p.group, upp = p.page_size / kKv4Unit;
   // A block: its sequence's first token and their number, positions of the first and the last token that has rows in it
   auto block_of = [&](int z) {
-    const int seq = z / p.row_blocks, row0 = z % p.row_blocks * kRows;
+    const int seq = p.row_blocks == 1 ? z : quotient(z, p.row_blocks), row0 = (z - seq * p.row_blocks) * kRows;
     if (p.single && p.row_blocks == 1) {                                  // (a step of single tokens: sequence s brings token s)
       const int pos = p.positions[seq];
       return make_int4(seq, 1, pos, pos);
@@ -255,8 +259,8 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
     b.y = p.cu_q[seq + 1] - b.x;
     if (b.y > p.max_tokens || row0 >= b.y * G) b.y = 0;                   // (not this launch's, or no rows)
     if (b.y > 0) {
-      b.z = p.positions[b.x + row0 / G];
-      b.w = p.positions[b.x + (min(row0 + kRows, b.y * G) - 1) / G];
+      b.z = p.positions[b.x + quotient(row0, G)];
+      b.w = p.positions[b.x + quotient(min(row0 + kRows, b.y * G) - 1, G)];
     }
     return b;
   };
@@ -311,9 +315,10 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
     }
     if (z < 0) return;
   }
-  const int n_pairs = pairs_of(mine4), begin = (int)((unsigned)n_pairs * run / runs), end = (int)((unsigned)n_pairs * (run + 1) / runs);
+  const int n_pairs = pairs_of(mine4), share = quotient(n_pairs, runs), left = n_pairs - share * runs, begin = run * share + min(run, left),
+            end = begin + share + (run < left ? 1 : 0);
   if (n_pairs == 0) return;
-  const int seq = z / p.row_blocks, row0 = z % p.row_blocks * kRows, tok0 = mine4.x, rows = mine4.y * G, n_rows = min(kRows, rows - row0);
+  const int seq = p.row_blocks == 1 ? z : quotient(z, p.row_blocks), row0 = (z - seq * p.row_blocks) * kRows, tok0 = mine4.x, rows = mine4.y * G, n_rows = min(kRows, rows - row0);
   // keys that the block's tokens see at all, and those that every one of them sees
   const int pos_a = mine4.z, pos_b = mine4.w, lo_b = first_key(pos_b, p.window);
   const int unit0 = first_key(pos_a, p.window) / kKv4Unit, n_units = pos_b / kKv4Unit + 1 - unit0;
@@ -353,7 +358,8 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
   const float sign = p.scale_log2 < 0.f ? -1.f : 1.f;                     // (a negative scale turns the query around, mult stays positive)
   auto row_at = [&](int nb) {
     const int r = row0 + nb * 8 + g;
-    return r < rows ? reinterpret_cast<const T*>(p.q) + (size_t)(tok0 + r / G) * p.q_stride + (size_t)(head * G + r % G) * D + 8 * t : nullptr;
+    const int token = quotient(r, G);
+    return r < rows ? reinterpret_cast<const T*>(p.q) + (size_t)(tok0 + token) * p.q_stride + (size_t)(head * G + r - token * G) * D + 8 * t : nullptr;
   };
   constexpr int kItems = (NB * NG + kWarps - 1) / kWarps;
   uint4 raw[PIECES == 1 ? NG : 1], own[PIECES == 1 ? kItems : 1];
@@ -433,7 +439,7 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
     }
   }
   if (threadIdx.x < kRows) {                                              // (a sequence's tokens follow one another)
-    const int r = row0 + threadIdx.x, pos = r < rows ? pos_a + r / G - row0 / G : -1;
+    const int r = row0 + threadIdx.x, pos = r < rows ? pos_a + quotient(r, G) - quotient(row0, G) : -1;
     row_sees[threadIdx.x] = r < rows ? first_key(pos, p.window) : 0;
     row_sees[kRows + threadIdx.x] = pos + 1;
   }
@@ -736,8 +742,8 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
   __syncthreads();
   auto write_row = [&](int r, int d4, float4 v, float total) {
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    const int row = row0 + r;
-    T* dst = reinterpret_cast<T*>(p.out) + (size_t)(tok0 + row / G) * p.out_stride + (size_t)(head * G + row % G) * D + 4 * d4;
+    const int row = row0 + r, token = quotient(row, G);
+    T* dst = reinterpret_cast<T*>(p.out) + (size_t)(tok0 + token) * p.out_stride + (size_t)(head * G + row - token * G) * D + 4 * d4;
     if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
     else *reinterpret_cast<float4*>(dst) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
   };
@@ -1025,7 +1031,7 @@ ILB_EXPORT int ilb_kv4_attention_rows(const void* q, void* out, int dtype, const
   for (int i = 0; i < 20; ++i)
     if (page_size / kKv4Unit == 1 << i) shift = i;
   Params p = {q, out, (const uint8_t*)cache, positions, cu_q, block_table, sink, scratch, tickets, error_flag, max_blocks, page_size, num_pages, window,
-              nq, nkv, q_stride, out_stride, pl.row_blocks, max_tokens, single, shift, pl.n_z, pl.slots, scale * kLog2e};
+              nq, nkv, q_stride, out_stride, pl.row_blocks, max_tokens, single, shift, nq / nkv, pl.n_z, pl.slots, scale * kLog2e};
   const dim3 grid = pl.slots > 0 ? dim3((unsigned)pl.ctas) : dim3(1, (unsigned)nkv, (unsigned)pl.n_z);
   const bool wide = rows_per_block(dtype, max_tokens * (nq / nkv), d) == 16;
   switch (d) {
