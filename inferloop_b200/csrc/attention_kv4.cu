@@ -41,7 +41,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // ------------------------------------------------------------------ few rows, many keys
 constexpr int kStages = 2;                  // pairs of units in a warp's ring
-constexpr int kMinPairs = 1;                // pairs a warp should have before another CTA joins
+constexpr int kMinPairs = 1;                // pairs that a warp of a run has at least
+// Pairs a warp up to which a block is left whole: joining its runs costs as much as two more pairs (8 heads of 128, us, whole and cut: 19 x 700
+// keys in float32 8.4 and 8.8, 2 x 900 9.3 and 9.7; 1 x 1,030, 33 pairs for 16 warps, 9.8 and 8.7).
+constexpr int kWholePairs = 2;
 constexpr int kSms = 148;
 constexpr int kMaxCut = 1024;               // (sequence, block of rows) pairs whose keys are cut: so many and more even out by themselves
 constexpr int kFewRecords = 8;              // records that a thread asks for all at once
@@ -274,7 +277,7 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
     const int n = pairs_of(mine4);
     if (n == 0) return;
     const int longest = longest_run(n * p.nkv, p.nkv, p.slots, kWarps);
-    runs = quotient(n + longest - 1, longest);
+    runs = n <= kWholePairs * kWarps ? 1 : quotient(n + longest - 1, longest);
     head = quotient(blockIdx.x, runs);
     run = blockIdx.x - head * runs;
     place = head * runs;
@@ -293,7 +296,7 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
     z = -1;
     for (int z0 = 0; z0 < p.n_z && z < 0; z0 += 32) {
       const int pairs = z0 == 0 ? first[0] : z0 == 32 ? first[1] : z0 + lane < p.n_z ? pairs_of(block_of(z0 + lane)) : 0;
-      const int cuts = quotient(pairs + longest - 1, longest);            // CTAs a head
+      const int cuts = pairs == 0 ? 0 : pairs <= kWholePairs * kWarps ? 1 : quotient(pairs + longest - 1, longest);            // CTAs a head
       int upto = cuts * p.nkv;
 #pragma unroll
       for (int o = 1; o < 32; o *= 2) {
@@ -789,12 +792,11 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
     __stcg(reinterpret_cast<float2*>(record + (size_t)threadIdx.x * (D + 4) + D), make_float2(row_m[threadIdx.x], row_m[kRows + threadIdx.x]));
   __syncthreads();
   if (threadIdx.x == 0) {
-    __threadfence();                                                      // (for all of the CTA's writes, which the barrier put before it)
     int* ticket = p.tickets + (size_t)z * p.nkv + head;
-    const int n = atomicAdd(ticket, 1);
+    int n;                                                                // (for all of the CTA's writes, which the barrier put before it)
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(n) : "l"(ticket) : "memory");
     flags[0] = n == runs - 1;
     if (n == runs - 1) *ticket = 0;                                       // (zero between launches)
-    __threadfence();
   }
   __syncthreads();
   if (!flags[0]) return;
