@@ -1678,7 +1678,8 @@ def kv4_scratch_bytes(tokens: int, nq: int, nkv: int, d: int) -> int:
     """Workspace that `kv4_attention` asks for at most in steps of so many tokens: the unpacked keys and values of a group of
     portions, their queries, the records of shared keys."""
     unpacked = KV4_UNPACK_TOKENS * nkv * d * 4 if attention_tc_supported(nq, nkv, d, KV4_TILE) else 0
-    return unpacked + tokens * nq * (2 * d + 4) + (512 * nkv + 4 * 148) * 8 * (d + 4) * 4
+    ctas = min(tokens, 1024) * nkv + 12 * 148            # a block of rows a sequence, or fewer sequences cut in several
+    return unpacked + tokens * nq * (2 * d + 4) + ctas * (8 if nq <= 8 * nkv else 16) * (d + 4) * 4
 
 
 def _kv4_need(what: str, cache: torch.Tensor, block_table: torch.Tensor, nkv: int, d: int) -> tuple:
@@ -1762,7 +1763,12 @@ def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tens
 
 
 KV4_ROWS_HEADS = (32, 64, 96, 128, 256)     # head sizes of the kernel of few rows (others: the simple kernel)
-KV4_PORTION_ROWS = 128      # rows (tokens x query heads of a group) from which a portion's keys and values are unpacked once for the prefill kernel
+KV4_SHORT_ROWS = 128        # rows (tokens x query heads of a group) up to which a sequence shares a launch with single tokens
+# Blocks of 16 rows an SM up to which long portions read the codes as well; more of them unpack their keys and values once for the prefill
+# kernel.  One round of the device, where the kernel of rows takes its two CTAs an SM (behind 1,030 keys, 32 / 8 heads of 128, us, codes and
+# unpacked: 64 tokens 15.6 and 23.6, 128 tokens 22.4 and 26.8, 160 tokens 40.7 and 25.3, 1,024 tokens 173 and 55).
+KV4_ROWS_ROUNDS = 2
+KV4_BLOCKS = 65535          # (sequence, block of rows) pairs of a launch
 KV4_UNPACK_TOKENS = 1 << 17 # tokens whose keys and values are unpacked at a time: sequences in groups; one with more keys reads the codes
 KV4_TILE = 128              # keys of a tile of the prefill kernel
 _KV4_ORDER: dict = {}       # 0, 1, 2, .. on each device
@@ -1783,8 +1789,8 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
                   nq: int, nkv: int, d: int, sink: Optional[torch.Tensor] = None, workspace=None) -> None:
     """Causal attention of the step's tokens over the 4-bit cache; q and out are [T, nq * d] of one type.  `window` and `sink`
     as in `attention`; a token that sees no key (its pages are not held) gets zeros.  Sequences that bring few tokens read the
-    codes themselves; longer portions' keys and values (bfloat16 queries, heads of 64 and 128) are unpacked into `workspace` (None:
-    one of the device's own) for the tensor cores' prefill kernel.  There a value that was kept as NaN reaches every token of its
+    codes themselves; longer portions' keys and values (bfloat16 queries, heads of 64 and 128; KV4_ROWS_ROUNDS) are unpacked into `workspace`
+    (None: one of the device's own) for the tensor cores' prefill kernel.  There a value that was kept as NaN reaches every token of its
     portion that lies in the same tile of 128 keys, as it does with a bfloat16 cache."""
     dtype = q.dtype
     if out.dtype is not dtype or not (q.is_cuda and out.is_cuda and q.is_contiguous() and out.is_contiguous()):
@@ -1811,31 +1817,49 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
               block_table.data_ptr(), max_blocks, page_size, num_pages, window, scale, T, nq, nkv, d, width, width, sinks, _raw_stream(q))
         return
     ws = _kv4_workspace(device) if workspace is None else workspace
-    most, sms = 1, _sm_count(device)
-    if not step.decode_only:
-        lens = step.h_q_len
-        most = longest = max(lens)
-        short = max(KV4_PORTION_ROWS // (nq // nkv), 1)
-        if longest > short and dtype is torch.bfloat16 and scale > 0 and attention_tc_supported(nq, nkv, d, KV4_TILE):
-            kv, a, most = step.h_kv_len, 0, 0
-            if max(kv) <= KV4_UNPACK_TOKENS:             # (else the rows kernel takes whatever comes: it leaves out by length alone)
-                while a < S:                             # runs of neighbouring sequences with long portions, as many as the scratch takes
-                    if lens[a] <= short:
-                        a, most = a + 1, max(most, lens[a])
-                        continue
-                    b, tiles = a, 0
-                    while b < S and lens[b] > short:
-                        n = max(tiles, -(-kv[b] // KV4_TILE))
-                        if b > a and n * KV4_TILE * (b + 1 - a) > KV4_UNPACK_TOKENS:
-                            break
-                        b, tiles = b + 1, n
-                    _kv4_portions(q, out, cache, step, block_table, a, b, tiles, window, scale, nq, nkv, d, sink, ws)
-                    a = b
-            else:
-                most = longest
-        if most == 0:
-            return
-    key = (code, S, most, nq, nkv, d, sms)
+    if step.decode_only:
+        _kv4_rows(q, out, cache, step, block_table, 0, S, 1, 1, window, scale, nq, nkv, d, sinks, code, ws)
+        return
+    lens, kv, G, sms = step.h_q_len, step.h_kv_len, nq // nkv, _sm_count(device)
+    longest = max(lens)
+    short = max(KV4_SHORT_ROWS // G, 1)
+    if longest <= short or -(-longest * G // 16) * S * nkv <= KV4_ROWS_ROUNDS * sms:
+        _kv4_rows(q, out, cache, step, block_table, 0, S, longest, 0, window, scale, nq, nkv, d, sinks, code, ws)
+        return
+    unpacks = dtype is torch.bfloat16 and scale > 0 and attention_tc_supported(nq, nkv, d, KV4_TILE)
+    a = rest = 0
+    while a < S:                                         # runs of neighbouring sequences with long portions
+        if lens[a] <= short:
+            a, rest = a + 1, max(rest, lens[a])
+            continue
+        if unpacks and kv[a] <= KV4_UNPACK_TOKENS:       # as many as the scratch takes
+            b, tiles, blocks = a, 0, 0
+            while b < S and lens[b] > short:
+                n = max(tiles, -(-kv[b] // KV4_TILE))
+                if b > a and n * KV4_TILE * (b + 1 - a) > KV4_UNPACK_TOKENS:
+                    break
+                b, tiles, blocks = b + 1, n, blocks + -(-lens[b] * G // 16) * nkv
+            if blocks > KV4_ROWS_ROUNDS * sms:
+                _kv4_portions(q, out, cache, step, block_table, a, b, tiles, window, scale, nq, nkv, d, sink, ws)
+                a = b
+                continue
+            most = max(lens[a:b])
+        else:                                            # as many as a launch takes
+            b, most = a + 1, lens[a]
+            while b < S and lens[b] > short and not (unpacks and kv[b] <= KV4_UNPACK_TOKENS) \
+                    and (b + 1 - a) * -(-max(most, lens[b]) * G // 8) <= KV4_BLOCKS:
+                b, most = b + 1, max(most, lens[b])
+        _kv4_rows(q, out, cache, step, block_table, a, b, most, 0, window, scale, nq, nkv, d, sinks, code, ws)
+        a = b
+    if rest:                                             # the others, by their length
+        _kv4_rows(q, out, cache, step, block_table, 0, S, rest, 0, window, scale, nq, nkv, d, sinks, code, ws)
+
+
+def _kv4_rows(q, out, cache, step, block_table, a: int, b: int, most: int, single: int, window: int, scale: float, nq: int, nkv: int, d: int,
+              sinks: int, code: int, ws) -> None:
+    """Sequences a .. b - 1 of the step, those of up to `most` tokens, on the kernel that reads the codes."""
+    device, width, max_blocks = q.device, nq * d, block_table.shape[1]
+    key = (code, b - a, most, nq, nkv, d, _sm_count(device))
     plan = _KV4_PLANS.get(key)
     if plan is None:
         lib, found = load_module("attention_kv4"), (ctypes.c_longlong(), ctypes.c_longlong())
@@ -1846,9 +1870,9 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
     if plan[0]:
         scratch = ws.address("kv4.records", plan[0], torch.float32)
         tickets = ws.address("kv4.tickets", max(plan[1], 4096), torch.int32, True)
-    _call("attention_kv4", "ilb_kv4_attention_rows", at, to, code, held, positions.data_ptr(), cu_q.data_ptr(), block_table.data_ptr(),
-          max_blocks, page_size, num_pages, window, scale, S, most, 1 if step.decode_only else 0, nq, nkv, d, width, width, sinks, sms, scratch, plan[0], tickets, plan[1],
-          _tc_state(device).error.data_ptr(), _raw_stream(q))
+    _call("attention_kv4", "ilb_kv4_attention_rows", q.data_ptr(), out.data_ptr(), code, cache.data_ptr(), step.positions.data_ptr(),
+          step.cu_q.data_ptr() + 4 * a, block_table.data_ptr() + 4 * a * max_blocks, max_blocks, cache.shape[2] * KV4_UNIT, cache.shape[0], window, scale,
+          b - a, most, single, nq, nkv, d, width, width, sinks, key[6], scratch, plan[0], tickets, plan[1], _tc_state(device).error.data_ptr(), _raw_stream(q))
 
 
 def _kv4_portions(q, out, cache, step, block_table, a: int, b: int, tiles: int, window: int, scale: float, nq: int, nkv: int, d: int, sink, ws) -> None:

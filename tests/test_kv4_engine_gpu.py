@@ -75,6 +75,15 @@ def test_logits_over_the_rows_that_the_cache_holds(folders, monkeypatch, name):
         assert not held
 
 
+def test_logits_with_every_long_portion_unpacked(folders, monkeypatch):
+    from inferloop_b200.csrc import ops
+    monkeypatch.setattr(ops, "KV4_ROWS_ROUNDS", 0)
+    calls, inner = [], ops._kv4_portions
+    monkeypatch.setattr(ops, "_kv4_portions", lambda *args: (calls.append(1), inner(*args)))
+    test_logits_over_the_rows_that_the_cache_holds(folders, monkeypatch, "D")
+    assert calls
+
+
 @pytest.mark.parametrize("name", ["B", "D"])
 def test_generation_and_pages_given_back(folders, kept_rows, name):
     from inferloop_b200 import Engine, SamplingParams

@@ -298,6 +298,61 @@ def test_a_far_key_that_stands_out(ops, lens):
         assert bool(((out.cpu().double() - want).abs() <= 2.0 ** -8 * (want.abs() + top)).all())
 
 
+@pytest.fixture
+def unpacked(ops, monkeypatch):
+    """Every sequence above KV4_SHORT_ROWS has its keys and values unpacked, however little fills the device."""
+    monkeypatch.setattr(ops, "KV4_ROWS_ROUNDS", 0)
+    calls, inner = [], ops._kv4_portions
+    monkeypatch.setattr(ops, "_kv4_portions", lambda *args: (calls.append(args[5:7]), inner(*args)))
+    return calls
+
+
+@pytest.mark.parametrize("nq,nkv,d", [(8, 2, 64), (32, 8, 128), (34, 2, 128), (2, 2, 128)])
+@pytest.mark.parametrize("window", [0, 20, -24])
+def test_unpacked_portions_beside_single_tokens(ops, unpacked, nq, nkv, d, window):
+    check(ops, torch.bfloat16, nq, nkv, d, 16, [60, 0, 33, 7, 100], [1, 19, 3, 170, 1], window, window == 20, 30)
+    assert unpacked
+
+
+@pytest.mark.parametrize("lens", [[3, 1, 40], [50, 33, 1]])
+def test_unpacked_what_no_token_sees_may_be_anything(ops, unpacked, lens):
+    test_what_no_token_sees_may_be_anything(ops, torch.bfloat16, lens)
+    assert unpacked
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, 2.0])
+def test_unpacked_scales_of_scores(ops, unpacked, scale):
+    check(ops, torch.bfloat16, 8, 2, 64, 16, [33, 90], [1, 140], 0, False, 70, scale=scale)
+    assert bool(unpacked) == (scale > 0)
+
+
+def test_an_unpacked_far_key_that_stands_out(ops, unpacked):
+    test_a_far_key_that_stands_out(ops, [40, 1])
+    assert unpacked
+
+
+@pytest.mark.parametrize("d", [64, 96])
+@pytest.mark.parametrize("blocks,tokens", [(1 << 16, 1 << 17), (20, 1 << 17), (1 << 16, 640), (40, 400), (1 << 16, 100)])
+def test_runs_of_long_portions(ops, unpacked, monkeypatch, d, blocks, tokens):
+    """Long portions beside short ones in groups by what a launch and the scratch take, one too long for the scratch among them."""
+    monkeypatch.setattr(ops, "KV4_BLOCKS", blocks)
+    monkeypatch.setattr(ops, "KV4_UNPACK_TOKENS", tokens)
+    starts, lens = [9, 250, 0, 7, 77, 0, 300, 5], [1, 60, 41, 3, 0, 130, 90, 2]
+    check(ops, torch.bfloat16, 8, 2, d, 16, starts, lens, 0, True, 120)
+    covered = [s for a, b in unpacked for s in range(a, b)]
+    assert covered == ([s for s in (1, 2, 5, 6) if starts[s] + lens[s] <= tokens] if d == 64 else [])
+
+
+def test_a_portion_on_either_side_of_the_rule(ops, monkeypatch):
+    calls = []
+    monkeypatch.setattr(ops, "_kv4_portions", lambda *args: calls.append(args[5:7]))
+    sms, q = ops._sm_count(torch.device(DEV)), lambda n: torch.zeros(n, 8 * 64, dtype=torch.bfloat16, device=DEV)
+    cache, table = torch.zeros(plain_shape(400, 1, 16, 64), dtype=torch.uint8, device=DEV), torch.arange(400, dtype=torch.int32, device=DEV).view(1, 400)
+    for tokens, want in ((4 * sms, []), (4 * sms + 1, [(0, 1)])):         # 16 rows a block, 8 heads a token, two blocks an SM
+        ops.kv4_attention(q(tokens), q(tokens), cache, plain.make_step([0], [tokens], DEV), table, 0, 0.125, 8, 1, 64)
+        assert calls == want
+
+
 @pytest.mark.parametrize("n,batch", [(5000, 1), (2500, 3), (9000, 2)])
 def test_many_keys(ops, n, batch):
     """Long enough for every way in which a sequence's keys are shared out; small heads keep the statement quick."""
