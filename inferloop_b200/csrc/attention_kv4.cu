@@ -45,6 +45,9 @@ constexpr int kMinPairs = 1;                // pairs that a warp of a run has at
 // Pairs a warp up to which a block is left whole: joining its runs costs as much as two more pairs (8 heads of 128, us, whole and cut: 19 x 700
 // keys in float32 8.4 and 8.8, 2 x 900 9.3 and 9.7; 1 x 1,030, 33 pairs for 16 warps, 9.8 and 8.7).
 constexpr int kWholePairs = 2;
+// The same where blocks alone fill three quarters of the device: what evens out ragged ends then costs every CTA a look at all lengths (8 heads of
+// 128, us, without this rule and with it: 64 x 1,030 keys 24.0 and 22.8, 200 x 500 41 and 36, 500 x 200 76 and 54).
+constexpr int kWholeOfMany = 16;
 constexpr int kSms = 148;
 constexpr int kMaxCut = 1024;               // (sequence, block of rows) pairs whose keys are cut: so many and more even out by themselves
 constexpr int kFewRecords = 8;              // records that a thread asks for all at once
@@ -201,10 +204,10 @@ __device__ __forceinline__ int longest_run(int pairs, int blocks, int slots, int
   const int by_count = blocks < slots ? (pairs + slots - blocks - 1) / (slots - blocks) : by_average;
   return max(min(by_average, by_count), kMinPairs * warps);
 }
-// The CTAs that come out at most.
-inline long long most_ctas(long long blocks, long long slots) {
-  const long long by_average = blocks + (2 * slots + 2) / 3;
-  return blocks < slots && slots < by_average ? by_average : blocks < slots ? slots : by_average;
+// The runs but the first ones of all blocks at most.
+inline long long most_extra(long long blocks, long long slots) {
+  const long long by_average = (2 * slots + 2) / 3;
+  return blocks < slots && by_average < slots - blocks ? slots - blocks : by_average;
 }
 
 // Warps that an SM has registers for: those of few rows' state (NB = 1 up to D = 128), half as many otherwise.
@@ -268,64 +271,120 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
     return b;
   };
   auto pairs_of = [&](int4 b) { return b.y > 0 ? (b.w / kKv4Unit + 2 - first_key(b.z, p.window) / kKv4Unit) / 2 : 0; };
-  // Which block and which run of it: every warp finds out by itself, a lane a block of every 32
-  int z = blockIdx.z, head = blockIdx.y, run = 0, runs = 1, place = 0;    // place: of the block's first record
+  // Which block and which run of it.  Run 0 of block b is CTA b's, and the others' CTAs come behind all blocks: a CTA of the first kind
+  // asks for its pages and queries before it knows how long its run is.
+  int z, head, run = 0, runs = 1, extra = 0;                              // extra: of the block's runs but the first, the first one's number among all such
+  const int blocks = p.n_z * p.nkv;
   int4 mine4;
-  if (p.slots == 0) mine4 = block_of(z);
-  else if (p.n_z == 1) {
-    mine4 = block_of(z = 0);
-    const int n = pairs_of(mine4);
-    if (n == 0) return;
-    const int longest = longest_run(n * p.nkv, p.nkv, p.slots, kWarps);
-    runs = n <= kWholePairs * kWarps ? 1 : quotient(n + longest - 1, longest);
-    head = quotient(blockIdx.x, runs);
-    run = blockIdx.x - head * runs;
-    place = head * runs;
-    if (head >= p.nkv) return;
-  } else {
-    int first[2];                                                         // (64 blocks' stay for the second pass)
-    first[0] = lane < p.n_z ? pairs_of(block_of(lane)) : 0;
-    first[1] = lane + 32 < p.n_z ? pairs_of(block_of(lane + 32)) : 0;
-    int total = first[0] + first[1];
-    for (int z0 = lane + 64; z0 < p.n_z; z0 += 32) total += pairs_of(block_of(z0));
+  int longest = 0;
+  const bool cut = p.slots > 0, first_run = cut && (int)blockIdx.x < blocks;
+  const int whole_up_to = kWarps * (4 * blocks >= 3 * p.slots ? kWholeOfMany : kWholePairs);
+  auto cuts_of = [&](int pairs) { return pairs <= whole_up_to ? 1 : quotient(pairs + longest - 1, longest); };
+  // pairs of all blocks together and the most of one, every warp by itself, 32 blocks at a time and the loads of four times as many at once
+  int total = 0, top = 0, first[4];                                       // first: of the first blocks
+  auto survey = [&](auto count) {
+    constexpr int N = decltype(count)::value;
+    for (int z0 = lane; z0 - lane < p.n_z; z0 += 32 * N) {
+      int4 b[N];
+      int row0[N];
 #pragma unroll
-    for (int o = 16; o > 0; o /= 2) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (total == 0) return;
-    const int longest = longest_run(total * p.nkv, p.n_z * p.nkv, p.slots, kWarps);
+      for (int i = 0; i < N; ++i) {
+        const int zi = min(z0 + 32 * i, p.n_z - 1), seq = p.row_blocks == 1 ? zi : quotient(zi, p.row_blocks);
+        row0[i] = (zi - seq * p.row_blocks) * kRows;
+        b[i] = make_int4(seq, seq + 1, 0, 0);
+      }
+      if (!(p.single && p.row_blocks == 1)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) b[i].z = p.cu_q[b[i].x];
+#pragma unroll
+        for (int i = 0; i < N; ++i) b[i].w = p.cu_q[b[i].y];
+#pragma unroll
+        for (int i = 0; i < N; ++i) { b[i].x = b[i].z; b[i].y = b[i].w - b[i].z > p.max_tokens || row0[i] >= (b[i].w - b[i].z) * G ? 0 : b[i].w - b[i].z; }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) b[i].y = 1;
+      }
+      // (a block without rows asks for the position of its first token or, behind the last, of the one before)
+#pragma unroll
+      for (int i = 0; i < N; ++i) b[i].w = b[i].y > 0 ? p.positions[b[i].x + (p.row_blocks == 1 ? b[i].y - 1 : quotient(min(row0[i] + kRows, b[i].y * G) - 1, G))] : -1;
+#pragma unroll
+      for (int i = 0; i < N; ++i) b[i].z = b[i].y > 0 && p.window != 0 ? p.positions[b[i].x + (p.row_blocks == 1 ? 0 : quotient(row0[i], G))] : 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int n = z0 + 32 * i < p.n_z ? pairs_of(b[i]) : 0;
+        total += n;
+        top = max(top, n);
+        if (z0 == lane) first[i] = n;
+      }
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    top = __reduce_max_sync(0xffffffffu, top);
+  };
+  auto survey_all = [&] {
+    if (p.n_z <= 32) survey(std::integral_constant<int, 1>{});
+    else survey(std::integral_constant<int, 4>{});
+  };
+  if (!cut) {
+    z = blockIdx.z;
+    head = blockIdx.y;
+    mine4 = block_of(z);
+  } else if (first_run) {
+    z = p.n_z == 1 ? 0 : quotient(blockIdx.x, p.nkv);
+    head = (int)blockIdx.x - z * p.nkv;
+    mine4 = block_of(z);
+  } else if (p.n_z == 1) {                                                // (one length for all heads)
+    mine4 = block_of(z = 0);
+    const int n = pairs_of(mine4), at = (int)blockIdx.x - blocks;
+    longest = longest_run(n * p.nkv, p.nkv, p.slots, kWarps);
+    runs = cuts_of(n);
+    if (at >= (runs - 1) * p.nkv) return;
+    head = quotient(at, runs - 1);
+    extra = head * (runs - 1);
+    run = 1 + at - extra;
+  } else {
+    survey_all();
+    if (total == 0 || top <= whole_up_to) return;
+    longest = longest_run(total * p.nkv, blocks, p.slots, kWarps);
+    if (cuts_of(top) == 1) return;
+    const int at = (int)blockIdx.x - blocks;
     int before = 0;
     z = -1;
-    for (int z0 = 0; z0 < p.n_z && z < 0; z0 += 32) {
-      const int pairs = z0 == 0 ? first[0] : z0 == 32 ? first[1] : z0 + lane < p.n_z ? pairs_of(block_of(z0 + lane)) : 0;
-      const int cuts = pairs == 0 ? 0 : pairs <= kWholePairs * kWarps ? 1 : quotient(pairs + longest - 1, longest);            // CTAs a head
-      int upto = cuts * p.nkv;
+    for (int z0 = 0; z0 < p.n_z && z < 0; z0 += 32) {                     // a lane a block of every 32
+      const int n = z0 == 0 ? first[0] : z0 == 32 ? first[1] : z0 == 64 ? first[2] : z0 == 96 ? first[3] : z0 + lane < p.n_z ? pairs_of(block_of(z0 + lane)) : 0;
+      const int more = cuts_of(n) - 1;
+      int upto = more * p.nkv;
 #pragma unroll
       for (int o = 1; o < 32; o *= 2) {
         const int v = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += v;
       }
-      const uint32_t reached = __ballot_sync(0xffffffffu, (int)blockIdx.x < before + upto);
+      const uint32_t reached = __ballot_sync(0xffffffffu, at < before + upto);
       if (reached != 0u) {
-        const int at = __ffs(reached) - 1;
-        z = z0 + at;
-        runs = __shfl_sync(0xffffffffu, cuts, at);
-        const int local = (int)blockIdx.x - before - __shfl_sync(0xffffffffu, upto, at) + runs * p.nkv;
-        mine4 = block_of(z);
-        head = quotient(local, runs);
-        run = local - head * runs;
-        place = (int)blockIdx.x - run;
+        const int by = __ffs(reached) - 1;
+        z = z0 + by;
+        const int others = __shfl_sync(0xffffffffu, more, by);
+        const int local = at - before - __shfl_sync(0xffffffffu, upto, by) + others * p.nkv;
+        head = quotient(local, others);
+        runs = others + 1;
+        run = 1 + local - head * others;
+        extra = at - run + 1;
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
     if (z < 0) return;
+    mine4 = block_of(z);
   }
-  const int n_pairs = pairs_of(mine4), share = quotient(n_pairs, runs), left = n_pairs - share * runs, begin = run * share + min(run, left),
-            end = begin + share + (run < left ? 1 : 0);
+  const int n_pairs = pairs_of(mine4);
   if (n_pairs == 0) return;
   const int seq = p.row_blocks == 1 ? z : quotient(z, p.row_blocks), row0 = (z - seq * p.row_blocks) * kRows, tok0 = mine4.x, rows = mine4.y * G, n_rows = min(kRows, rows - row0);
   // keys that the block's tokens see at all, and those that every one of them sees
   const int pos_a = mine4.z, pos_b = mine4.w, lo_b = first_key(pos_b, p.window);
   const int unit0 = first_key(pos_a, p.window) / kKv4Unit, n_units = pos_b / kKv4Unit + 1 - unit0;
-  const int mine = end - begin > warp ? (end - begin - warp + kWarps - 1) / kWarps : 0;      // pairs of this warp: begin + warp + i kWarps
+  auto begin_of = [&](int r) {                                            // the runs' lengths differ by one at the most
+    const int share = quotient(n_pairs, runs);
+    return r * share + min(r, n_pairs - share * runs);
+  };
+  const int begin = run == 0 ? 0 : begin_of(run);
 
   // ---- the stream of units: lane 2 i + h knows where unit h of the i-th of every 16 pairs lies
   const int* table = p.block_table + (size_t)seq * p.max_blocks;
@@ -334,25 +393,10 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
   auto unit_of = [&](int i0) { return 2 * (begin + warp + (i0 + (lane >> 1)) * kWarps) + (lane & 1); };
   auto page_of = [&](int i0) {                                            // (its load may be waited for later)
     const int u = unit_of(i0), blk = p.unit_shift >= 0 ? (unit0 + u) >> p.unit_shift : (unit0 + u) / upp;
-    return i0 + (lane >> 1) < mine && u < n_units && blk < p.max_blocks ? table[blk] : -1;
-  };
-  auto look_up = [&](int i0, int page) {
-    const bool is_held = page >= 0 && page < p.num_pages;
-    const int in_page = p.unit_shift >= 0 ? (unit0 + unit_of(i0)) & (upp - 1) : (unit0 + unit_of(i0)) % upp;
-    src_unit = is_held ? p.cache + (((size_t)page * p.nkv + head) * upp + in_page) * U : nullptr;
-    there_now = __ballot_sync(0xffffffffu, is_held);
-  };
-  uint32_t asked = 0;                                                     // two bits a pair on its way: which of its units come
-  auto ask = [&](int i, int s, int behind) {                              // pair i, one of the 16 looked up, into stage s, behind so many others
-    const uint32_t both = (there_now >> (2 * i & 31)) & 3u;
-    asked |= both << (2 * behind);
-    if ((lane >> 1) == (i & 15)) {                                        // the lanes that know where
-      const uint32_t bar = bar0 + 8 * s;
-      if ((lane & 1) == 0) mbar_expect_tx(bar, ((both & 1u) + (both >> 1)) * U);
-      if (src_unit != nullptr) bulk_load(ring + (2 * s + (lane & 1)) * U, src_unit, U, bar);
-    }
+    return u < n_units && blk < p.max_blocks ? table[blk] : -1;
   };
   const int first_page = page_of(0);
+
 
   // ---- queries as second operands, rows g of each block of 8, made once a CTA (a warp a group of 32 elements) and shared; with them what the
   // offsets of the keys' operands add to the groups' sums
@@ -379,6 +423,31 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
       if (kItems == 1) ask_row(src);
     }
   }
+  if (first_run && n_pairs > whole_up_to) {
+    if (p.n_z > 1) survey_all();
+    else total = n_pairs;
+    longest = longest_run(total * p.nkv, blocks, p.slots, kWarps);
+    runs = cuts_of(n_pairs);
+    if (p.n_z == 1) extra = head * (runs - 1);
+  }
+  const int end = runs == 1 ? n_pairs : begin_of(run + 1);
+  const int mine = end - begin > warp ? (end - begin - warp + kWarps - 1) / kWarps : 0;      // pairs of this warp: begin + warp + i kWarps
+  auto look_up = [&](int i0, int page) {
+    const bool is_held = i0 + (lane >> 1) < mine && page >= 0 && page < p.num_pages;
+    const int in_page = p.unit_shift >= 0 ? (unit0 + unit_of(i0)) & (upp - 1) : (unit0 + unit_of(i0)) % upp;
+    src_unit = is_held ? p.cache + (((size_t)page * p.nkv + head) * upp + in_page) * U : nullptr;
+    there_now = __ballot_sync(0xffffffffu, is_held);
+  };
+  uint32_t asked = 0;                                                     // two bits a pair on its way: which of its units come
+  auto ask = [&](int i, int s, int behind) {                              // pair i, one of the 16 looked up, into stage s, behind so many others
+    const uint32_t both = (there_now >> (2 * i & 31)) & 3u;
+    asked |= both << (2 * behind);
+    if ((lane >> 1) == (i & 15)) {                                        // the lanes that know where
+      const uint32_t bar = bar0 + 8 * s;
+      if ((lane & 1) == 0) mbar_expect_tx(bar, ((both & 1u) + (both >> 1)) * U);
+      if (src_unit != nullptr) bulk_load(ring + (2 * s + (lane & 1)) * U, src_unit, U, bar);
+    }
+  };
   if (mine > 0) {
     look_up(0, first_page);
 #pragma unroll
@@ -771,8 +840,10 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
   }
   __syncthreads();
   constexpr size_t kRecord = (size_t)kRows * (D + 4);
-  float* first_record = p.scratch + (size_t)place * kRecord;              // of the block's runs, one behind the other
-  float* record = first_record + (size_t)run * kRecord;
+  // records: run 0's at its block's number, the others' behind those of all blocks
+  float* first_record = p.scratch + (size_t)(z * p.nkv + head) * kRecord;
+  auto others_at = [&] { return p.scratch + ((ptrdiff_t)(blocks + extra) - 1) * (ptrdiff_t)kRecord; };      // (run c of them c records further)
+  float* record = run == 0 ? first_record : others_at() + run * kRecord;
   constexpr int kQuads = D / 4;
   for (int at = threadIdx.x; at < n_rows * kQuads; at += kThreads) {
     const int r = at / kQuads, d4 = at % kQuads;
@@ -793,25 +864,30 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
   __syncthreads();
   if (threadIdx.x == 0) {
     int* ticket = p.tickets + (size_t)z * p.nkv + head;
+    int* told = reinterpret_cast<int*>(first_record + D + 2);             // (behind its first row's maximum and sum)
+    if (run != 0 && p.n_z > 1) __stcg(told, extra);                                   // (every one the same: for run 0, should it be the last)
     int n;                                                                // (for all of the CTA's writes, which the barrier put before it)
     asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(n) : "l"(ticket) : "memory");
     flags[0] = n == runs - 1;
+    if (n == runs - 1) flags[1] = first_run && p.n_z > 1 ? __ldcg(told) : extra;
     if (n == runs - 1) *ticket = 0;                                       // (zero between launches)
   }
   __syncthreads();
   if (!flags[0]) return;
+  extra = flags[1];
+  const float* others = others_at();
   auto share_of = [&](float2 ml, float top) { return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2f(ml.x - top); };
   if (runs <= kFewRecords) {                                              // one wait for everything, in the order of the runs
     for (int at = threadIdx.x; at < n_rows * kQuads; at += kThreads) {
       const int r = at / kQuads, d4 = at % kQuads;
-      const float* src = first_record + (size_t)r * (D + 4);
       float2 ml[kFewRecords];
       float4 x[kFewRecords];
 #pragma unroll
       for (int c = 0; c < kFewRecords; ++c) {
         const bool there = c < runs;
-        ml[c] = there ? __ldcg(reinterpret_cast<const float2*>(src + c * kRecord + D)) : make_float2(-INFINITY, 0.f);
-        x[c] = there ? __ldcg(reinterpret_cast<const float4*>(src + c * kRecord + 4 * d4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float* src = (c == 0 ? first_record : others + c * kRecord) + (size_t)r * (D + 4);
+        ml[c] = there ? __ldcg(reinterpret_cast<const float2*>(src + D)) : make_float2(-INFINITY, 0.f);
+        x[c] = there ? __ldcg(reinterpret_cast<const float4*>(src + 4 * d4)) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
       const float sink = sink_of(r);
       float top = sink;
@@ -835,7 +911,7 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
     const float sink = sink_of(r);
     float top = sink;
     for (int c = lane; c < runs; c += 32) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(first_record + c * kRecord + (size_t)r * (D + 4) + D));
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>((c == 0 ? first_record : others + c * kRecord) + (size_t)r * (D + 4) + D));
       shares[2 * (r * runs + c)] = ml.x;
       shares[2 * (r * runs + c) + 1] = ml.y;
       top = fmaxf(top, ml.x);
@@ -854,11 +930,10 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
   __syncthreads();
   for (int at = threadIdx.x; at < n_rows * kQuads; at += kThreads) {
     const int r = at / kQuads, d4 = at % kQuads;
-    const float* src = first_record + (size_t)r * (D + 4) + 4 * d4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
     for (int c = 0; c < runs; ++c) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(src + c * kRecord));
+      const float4 x = __ldcg(reinterpret_cast<const float4*>((c == 0 ? first_record : others + c * kRecord) + (size_t)r * (D + 4) + 4 * d4));
       const float f = shares[2 * (r * runs + c)];
       v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
     }
@@ -999,7 +1074,7 @@ static int make_plan(Plan* pl, int dtype, int n_seqs, int max_tokens, int nq, in
   pl->warps = n_z * nkv > sms ? 4 : sm_warps;
   pl->slots = (sms < kSms ? sms : kSms) * (sm_warps / pl->warps);
   if (n_z >= kMaxCut || (rb > 1 && n_z * nkv >= 2 * pl->slots)) pl->slots = 0;      // (blocks of rows of one portion are of about one length)
-  pl->ctas = (int)most_ctas(n_z * nkv, pl->slots);
+  pl->ctas = (int)(n_z * nkv + (pl->slots > 0 ? most_extra(n_z * nkv, pl->slots) : 0));
   pl->scratch = pl->slots > 0 ? (long long)pl->ctas * per * (d + 4) : 0;
   pl->tickets = pl->slots > 0 ? n_z * nkv : 0;
   return 0;

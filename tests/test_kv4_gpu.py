@@ -360,6 +360,22 @@ def test_many_keys(ops, n, batch):
     check(ops, torch.bfloat16, 4, 2, 64, 64, [n - 37 * s for s in range(batch)], [2] + [1] * (batch - 1), 0, False, 91)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("batch,nkv,window", [(150, 4, 0), (150, 4, 700), (40, 2, 0), (33, 1, 0), (300, 2, 0), (9, 1, 0)])
+@pytest.mark.parametrize("more", [0, 2])
+def test_long_sequences_among_many_short_ones(ops, dtype, batch, nkv, window, more):
+    """A few sequences are cut and the others are not; `more` further tokens in some."""
+    longer = {0: 5000, batch // 2: 3100, batch - 1: 2500}
+    starts = [longer.get(s, 1 + 37 * s % 90) for s in range(batch)]
+    check(ops, dtype, 2 * nkv, nkv, 32, 32, starts, [1 + (more if s % 7 == 3 else 0) for s in range(batch)], window, False, 130)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_more_blocks_of_rows_than_a_launch_takes(ops, dtype):
+    """A long portion beside single tokens whose blocks, counted by the longest, are more than 65,535."""
+    check(ops, dtype, 64, 1, 32, 32, [40] * 7 + [0], [1] * 7 + [1200], 100, False, 140)
+
+
 def test_a_pool_past_32_bits(ops):
     """Pages whose byte offsets, and whose rows read back, need more than 32 bits."""
     nkv, d, page = 8, 128, 16
