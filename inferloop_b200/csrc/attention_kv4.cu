@@ -5,8 +5,8 @@
 //
 // Few rows against many keys (`rows_kernel`).  A row is a (token, query head of the group); 8 NB rows of a (sequence, kv head) are a block
 // of work.  A block's keys are cut into equal runs, one a CTA, none longer than the device's share (`longest_run`): a few blocks fill it, and
-// one long sequence among short ones does not hold the launch up; the CTAs find their runs from the lengths, which the device
-// knows.  In a run a warp takes two units of 16 keys at a time (one at a time took a quarter more instructions a key).  A unit
+// one long sequence among short ones does not hold the launch up; the CTAs find their runs from the lengths, which only the device
+// knows while a recorded step is replayed.  In a run a warp takes two units of 16 keys at a time (one at a time took a quarter more instructions a key).  A unit
 // is one piece of 18 D bytes of the cache: a warp keeps kStages pairs of them on their way to its own ring in shared memory by bulk
 // copies, so nothing but the merge at the end crosses from warp to warp.
 //   scores   S^T = K Q^T on m16n8k16, the 16 keys as rows, so that groups of up to 8 query heads fill the 8 columns.  In fp16, where one
@@ -26,6 +26,11 @@
 //            The accumulator of S^T is turned into the second operand by movmatrix.
 //   merge    a CTA's warps through shared memory; several CTAs' records through a scratch buffer, by the CTA that takes the last ticket, in
 //            the order of the CTAs (the result does not depend on who is last).
+// What bounds it.  Many keys: instructions.  A unit takes 297 a warp for eight rows (ALU 141, FMA 95, shared memory 21, tensor 17), and an SM
+// with 12 warps at it 111 clocks a unit, where the copy rate would be 97.  Few keys: the chain launch, position, page, first units, merge, ticket, records, 5.5 us where nothing is cut and 8.5 where runs are joined.
+// Measured, us (floor of bytes), launch after launch, bfloat16, 32 / 8 heads of 128: 1 x 1,030 keys 8.5 (0.2), 8 x 1,030 10.0 (1.3), 64 x 1,030
+// 22.8 (10.4, 3.0 TB/s), 64 x 4,102 69.6 (41.1, 3.9 TB/s), 16 x 4,000 21.4 (10.5), 64 / 8 heads 2 x 16,000 17.2 (5.6), 128 / 8 heads 64 x 1,030 36.7,
+// 32 / 8 heads of 64 14.9 (5.2); float32 19 x 700 of 8 / 2 heads of 64 7.6.
 #include <math.h>
 #include <cuda_fp16.h>
 #include <type_traits>
@@ -49,7 +54,9 @@ constexpr int kWholePairs = 2;
 // 128, us, without this rule and with it: 64 x 1,030 keys 24.0 and 22.8, 200 x 500 41 and 36, 500 x 200 76 and 54).
 constexpr int kWholeOfMany = 16;
 constexpr int kSms = 148;
-constexpr int kMaxCut = 1024;               // (sequence, block of rows) pairs whose keys are cut: so many and more even out by themselves
+// (sequence, block of rows) pairs whose keys are cut.  So many and more even out by themselves, and to survey them costs each CTA more
+// than the ragged end (8 / 2 heads, us, surveyed and not: 1,100 x 100 keys 90 and 25, 1,500 x 600 192 and 67).
+constexpr int kMaxCut = 1024;
 constexpr int kFewRecords = 8;              // records that a thread asks for all at once
 
 struct Params {
@@ -967,7 +974,9 @@ int launch_head(const Params& p, int dtype, bool wide, dim3 grid, int warps, cud
 }
 
 // ------------------------------------------------------------------ any head size
-// One block a (token, query head); a warp takes 32 keys at a time, a lane a key for the scores and every 32nd element of the values.
+// One block a (token, query head); a warp takes 32 keys at a time, a lane a key for the scores and every 32nd element of the values.  It reads a
+// kv head's codes once a query head and a lane walks a whole key by itself: loads of four bytes with nothing to hide them bound it (64 x 1,030 keys of
+// 32 / 8 heads of 160: 610 us, 1 x 70 of 8 / 1 heads of 512 33).  It is there so that every head size is served, and kept plain.
 constexpr int kSimpleWarps = 4, kMaxHead = 512;
 
 template <typename T>
@@ -1062,7 +1071,7 @@ static bool rows_head(int d) { return d == 32 || d == 64 || d == 96 || d == 128 
 struct Plan { int row_blocks, n_z, warps, slots, ctas; long long scratch, tickets; };
 
 // Blocks that fill the device by themselves get CTAs of four warps, several to an SM; fewer blocks, whose keys more CTAs share, CTAs of a
-// whole SM each, so that fewer records have to meet (2 x 16,000 keys: 31 us with four warps, 21 with 16).
+// whole SM each, so that fewer records have to meet (2 x 16,000 keys of 64 / 8 heads: 23 us with four warps, 18 with eight, 17 with 16).
 static int make_plan(Plan* pl, int dtype, int n_seqs, int max_tokens, int nq, int nkv, int d, int sms) {
   ILB_REQUIRE(n_seqs >= 0 && max_tokens > 0 && nkv > 0 && nq > 0 && nq % nkv == 0 && sms > 0 && rows_head(d), "kv4_attention: bad sizes");
   const int rows = max_tokens * (nq / nkv), per = rows_per_block(dtype, rows, d);
