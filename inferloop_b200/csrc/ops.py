@@ -1771,17 +1771,18 @@ KV4_ROWS_ROUNDS = 2
 KV4_BLOCKS = 65535          # (sequence, block of rows) pairs of a launch
 KV4_UNPACK_TOKENS = 1 << 17 # tokens whose keys and values are unpacked at a time: sequences in groups; one with more keys reads the codes
 KV4_TILE = 128              # keys of a tile of the prefill kernel
-_KV4_ORDER: dict = {}       # 0, 1, 2, .. on each device
+_KV4_ORDER: dict = {}       # 0, 1, 2, .. on each device, written on the stream that reads it
 _KV4_WORKSPACE: dict = {}
 _KV4_PLANS: dict = {}      # sizes of a launch -> (floats of scratch, tickets) that it needs
 
 
-def _kv4_workspace(device: torch.device):
-    """The scratch of callers that bring no workspace of their own: one per device."""
-    ws = _KV4_WORKSPACE.get(device)
+def _kv4_workspace(q: torch.Tensor):
+    """The scratch of callers that bring no workspace of their own: one per device and stream."""
+    key = (q.device, _raw_stream(q))
+    ws = _KV4_WORKSPACE.get(key)
     if ws is None:
         from ..parts.base import Workspace
-        ws = _KV4_WORKSPACE[device] = Workspace(device)
+        ws = _KV4_WORKSPACE[key] = Workspace(q.device)
     return ws
 
 
@@ -1790,7 +1791,7 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
     """Causal attention of the step's tokens over the 4-bit cache; q and out are [T, nq * d] of one type.  `window` and `sink`
     as in `attention`; a token that sees no key (its pages are not held) gets zeros.  Sequences that bring few tokens read the
     codes themselves; longer portions' keys and values (bfloat16 queries, heads of 64 and 128; KV4_ROWS_ROUNDS) are unpacked into `workspace`
-    (None: one of the device's own) for the tensor cores' prefill kernel.  There a value that was kept as NaN reaches every token of its
+    (None: one of the stream's own) for the tensor cores' prefill kernel.  There a value that was kept as NaN reaches every token of its
     portion that lies in the same tile of 128 keys, as it does with a bfloat16 cache."""
     dtype = q.dtype
     if out.dtype is not dtype or not (q.is_cuda and out.is_cuda and q.is_contiguous() and out.is_contiguous()):
@@ -1816,7 +1817,7 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
         _call("attention_kv4", "ilb_kv4_attention_simple", at, to, code, held, positions.data_ptr(), step.seq_of_token.data_ptr(),
               block_table.data_ptr(), max_blocks, page_size, num_pages, window, scale, T, nq, nkv, d, width, width, sinks, _raw_stream(q))
         return
-    ws = _kv4_workspace(device) if workspace is None else workspace
+    ws = _kv4_workspace(q) if workspace is None else workspace
     if step.decode_only:
         _kv4_rows(q, out, cache, step, block_table, 0, S, 1, 1, window, scale, nq, nkv, d, sinks, code, ws)
         return
@@ -1882,10 +1883,11 @@ def _kv4_portions(q, out, cache, step, block_table, a: int, b: int, tiles: int, 
     k, v = (ws.address("kv4." + w, n * tiles * nkv * KV4_TILE * d, half) for w in ("keys", "values"))
     info = ws.address("kv4.tiles", n * tiles * nkv * 4, torch.float32)
     q_half, q_power = ws.address("kv4.queries", q.numel(), half), ws.address("kv4.query_powers", q.shape[0] * nq, torch.float32)
-    order = _KV4_ORDER.get(device)
+    stream = _raw_stream(q)
+    order = _KV4_ORDER.get((device, stream))
     if order is None or order.numel() < n * tiles:       # page s * tiles + t holds tile t of sequence s
-        order = _KV4_ORDER[device] = torch.arange(max(n * tiles, 1 << 14), dtype=torch.int32, device=device)
-    positions, cu_q, stream = step.positions.data_ptr(), step.cu_q.data_ptr() + 4 * a, _raw_stream(q)
+        order = _KV4_ORDER[device, stream] = torch.arange(max(n * tiles, 1 << 14), dtype=torch.int32, device=device)
+    positions, cu_q = step.positions.data_ptr(), step.cu_q.data_ptr() + 4 * a
     sinks = 0 if sink is None else sink.data_ptr()
     _call("kv4", "ilb_kv4_unpack", cache.data_ptr(), block_table.data_ptr() + 4 * a * block_table.shape[1], block_table.shape[1],
           step.kv_len.data_ptr() + 4 * a, positions, cu_q, window, cache.shape[2] * KV4_UNIT, cache.shape[0], n, tiles, nkv, d, k, v, info,

@@ -421,6 +421,27 @@ def test_same_bits_twice_and_on_another_stream(ops, lens):
     assert all(torch.equal(o, outs[0]) for o in outs)
 
 
+@pytest.mark.parametrize("lens", [[1] * 3, [70, 60, 2]])
+def test_two_streams_at_once(ops, unpacked, lens):
+    """Calls on two streams share nothing: neither the records of shared keys nor the unpacked ones."""
+    starts = [6000, 4100, 30]
+    cache, table = filled([a + n for a, n in zip(starts, lens)], 2, 64, 32, torch.bfloat16, 97)
+    step, streams = plain.make_step(starts, lens, DEV), [torch.cuda.Stream() for _ in range(2)]
+    qs = [torch.randn(sum(lens), 8 * 64, generator=torch.Generator().manual_seed(s)).bfloat16().to(DEV) for s in (5, 6)]
+    run = lambda q, o: ops.kv4_attention(q, o, cache, step, table, 0, 0.125, 8, 2, 64)
+    alone = [torch.zeros_like(q) for q in qs]
+    for q, o in zip(qs, alone):
+        run(q, o)
+    outs = [[torch.zeros_like(q) for _ in range(20)] for q in qs]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for s, q, o in zip(streams, qs, outs):
+            with torch.cuda.stream(s):
+                run(q, o[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, a) for os, a in zip(outs, alone) for o in os)
+
+
 def test_refusals(ops):
     E = ops.KernelError
     cache = torch.zeros(4, 2, 1, 18 * 64, dtype=torch.uint8, device=DEV)
