@@ -1683,22 +1683,25 @@ def kv4_scratch_bytes(tokens: int, nq: int, nkv: int, d: int) -> int:
 
 
 def _kv4_need(what: str, cache: torch.Tensor, block_table: torch.Tensor, nkv: int, d: int) -> tuple:
-    """(pages, page size) of a 4-bit cache that holds `nkv` heads of `d`."""
+    """(pages, page size, rows and columns of the block table) of a 4-bit cache that holds `nkv` heads of `d`."""
     if cache.dtype is not torch.uint8 or block_table.dtype is not torch.int32 or not (cache.is_contiguous() and block_table.is_contiguous()
                                                                                      and cache.is_cuda and block_table.is_cuda):
         _need(cache, what + " cache", torch.uint8); _need(block_table, what + " block table", torch.int32)
-    shape = cache.shape
-    if len(shape) != 4 or shape[1] != nkv or shape[3] != 18 * d or shape[2] == 0 or d % KV4_GROUP or not 0 < d <= KV4_MAX_HEAD:
+    shape, table = cache.shape, block_table.shape
+    if len(shape) != 4 or len(table) != 2:
+        raise KernelError(f"{what}: the cache must be [pages, heads, units, bytes] and the block table [sequences, blocks]")
+    pages, heads, units, width = shape
+    if heads != nkv or width != 18 * d or units == 0 or d % KV4_GROUP or not 0 < d <= KV4_MAX_HEAD:
         raise KernelError(f"{what}: cache shape {tuple(shape)} is not [pages, {nkv}, page size / {KV4_UNIT}, {18 * d}]")
-    if block_table.dim() != 2:
-        raise KernelError(f"{what}: the block table must be [sequences, blocks]")
-    return shape[0], shape[2] * KV4_UNIT
+    return pages, units * KV4_UNIT, *table
 
 
-def _kv4_ints(what: str, *tensors: torch.Tensor) -> None:
-    for t in tensors:
-        if t.dtype is not torch.int32 or not (t.is_cuda and t.is_contiguous()):
-            _need(t, what, torch.int32)
+_INT32 = torch.int32
+
+
+def _kv4_ints(what: str, a: torch.Tensor, b: torch.Tensor) -> None:
+    if not (a.dtype is b.dtype is _INT32 and a.is_cuda and b.is_cuda and a.is_contiguous() and b.is_contiguous()):
+        _need(a, what, torch.int32); _need(b, what, torch.int32)
 
 
 def kv4_write(k: torch.Tensor, v: torch.Tensor, step, block_table: torch.Tensor, cache: torch.Tensor) -> None:
@@ -1709,16 +1712,16 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, step, block_table: torch.Tensor,
     if v.dtype is not k.dtype or not (k.is_cuda and v.is_cuda):
         _need(k, "kv4_write keys", contiguous=False); _need(v, "kv4_write values", k.dtype, contiguous=False)
     shape, ks, vs = k.shape, k.stride(), v.stride()
-    if len(shape) != 3 or v.shape != shape or (k.numel() and (ks[2] != 1 or vs[2] != 1)):
+    if len(shape) != 3 or v.shape != shape or ((ks[2] != 1 or vs[2] != 1) and k.numel()):
         raise KernelError("kv4_write: keys and values must be [tokens, heads, head size] with a head's elements side by side")
     T, nkv, d = shape
-    num_pages, page_size = _kv4_need("kv4_write", cache, block_table, nkv, d)
+    num_pages, page_size, _, max_blocks = _kv4_need("kv4_write", cache, block_table, nkv, d)
     positions, seqs = step.positions, step.seq_of_token
     _kv4_ints("kv4_write positions and sequence indices", positions, seqs)
     if positions.numel() != T or seqs.numel() != T:
         raise KernelError(f"kv4_write: {T} rows for a step of {positions.numel()} tokens")
     _call("kv4", "ilb_kv4_write", k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _code(k),
-          positions.data_ptr(), seqs.data_ptr(), block_table.data_ptr(), block_table.shape[1], page_size, num_pages, cache.data_ptr(), T, nkv, d,
+          positions.data_ptr(), seqs.data_ptr(), block_table.data_ptr(), max_blocks, page_size, num_pages, cache.data_ptr(), T, nkv, d,
           _raw_stream(cache))
 
 
@@ -1730,7 +1733,7 @@ def qk_norm_rope_kv4(qkv: torch.Tensor, q_out: torch.Tensor, q_weight: Optional[
     _need(qkv, "qkv", contiguous=False); _need(q_out, "q_out", qkv.dtype); _need(q_weight, "q_norm weight", torch.float32)
     _need(k_weight, "k_norm weight", torch.float32); _need(rope, "rope table", torch.float32)
     T = qkv.shape[0]
-    num_pages, page_size = _kv4_need("qk_norm_rope_kv4", cache, block_table, nkv, d)
+    num_pages, page_size, _, max_blocks = _kv4_need("qk_norm_rope_kv4", cache, block_table, nkv, d)
     _kv4_ints("qk_norm_rope_kv4 positions and sequence indices", step.positions, step.seq_of_token)
     if qkv.stride(1) != 1 or qkv.shape[1] < (nq + 2 * nkv) * d or tuple(q_out.shape) != (T, nq * d) or step.positions.numel() != T \
             or step.seq_of_token.numel() != T or (rope is not None and tuple(rope.shape) != (T, rotary_dim // 2, 2)) \
@@ -1739,7 +1742,7 @@ def qk_norm_rope_kv4(qkv: torch.Tensor, q_out: torch.Tensor, q_weight: Optional[
     _call("kv4", "ilb_qk_norm_rope_kv4", qkv.data_ptr(), qkv.stride(0), q_out.data_ptr(), nq * d, _code(qkv),
           0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), eps,
           0 if rope is None else rope.data_ptr(), rotary_dim, mode, step.positions.data_ptr(), step.seq_of_token.data_ptr(), block_table.data_ptr(),
-          block_table.shape[1], page_size, num_pages, cache.data_ptr() if write else 0, T, nq, nkv, d, _raw_stream(cache))
+          max_blocks, page_size, num_pages, cache.data_ptr() if write else 0, T, nq, nkv, d, _raw_stream(cache))
 
 
 def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, out_table: torch.Tensor, k_out: torch.Tensor,
@@ -1753,11 +1756,10 @@ def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tens
     if len(shape) != 4 or v_out.shape != shape:
         raise KernelError("kv4_read: outputs must be [pages, heads, page size, head size]")
     out_pages, nkv, ps, d = shape
-    num_pages, page_size = _kv4_need("kv4_read", cache, block_table, nkv, d)
+    num_pages, page_size, S, max_blocks = _kv4_need("kv4_read", cache, block_table, nkv, d)
     _kv4_ints("kv4_read output table and lengths", out_table, lengths)
-    if ps != page_size or out_table.shape != block_table.shape or lengths.numel() != block_table.shape[0]:
+    if ps != page_size or out_table.shape != block_table.shape or lengths.numel() != S:
         raise KernelError("kv4_read: output pages, output table or lengths do not match the cache and its block table")
-    S, max_blocks = block_table.shape
     _call("kv4", "ilb_kv4_read", cache.data_ptr(), block_table.data_ptr(), max_blocks, out_table.data_ptr(), max_blocks, lengths.data_ptr(), S, page_size, num_pages,
           out_pages, k_out.data_ptr(), v_out.data_ptr(), _code(k_out), nkv, d, _raw_stream(cache))
 
@@ -1796,13 +1798,14 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
     dtype = q.dtype
     if out.dtype is not dtype or not (q.is_cuda and out.is_cuda and q.is_contiguous() and out.is_contiguous()):
         _need(q, "kv4_attention q"); _need(out, "kv4_attention out", dtype)
-    num_pages, page_size = _kv4_need("kv4_attention", cache, block_table, nkv, d)
-    shape, (S, max_blocks) = q.shape, block_table.shape
+    num_pages, page_size, S, max_blocks = _kv4_need("kv4_attention", cache, block_table, nkv, d)
+    shape = q.shape
     T, width = shape if len(shape) == 2 else (-1, -1)
     positions, cu_q = step.positions, step.cu_q
     if nq <= 0 or nq % nkv or width != nq * d or out.shape != shape or positions.numel() != T or cu_q.numel() != S + 1:
         raise KernelError("kv4_attention: queries, output, step and block table do not agree")
-    _kv4_ints("kv4_attention positions, offsets and lengths", positions, cu_q, step.kv_len)
+    _kv4_ints("kv4_attention positions and offsets", positions, cu_q)
+    _kv4_ints("kv4_attention positions and lengths", positions, step.kv_len)
     if sink is not None:
         _need(sink, "kv4_attention sink", torch.float32)
         if sink.numel() != nq:
