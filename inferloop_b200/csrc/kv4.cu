@@ -519,9 +519,10 @@ void launch_wide(const WideArgs& a, cudaStream_t stream) {
 // A portion's keys and values in fp16 for tensor cores that multiply one type: code times scale has 11 significant bits, fp16's, so
 // they are exact once a tile of 128 keys is brought to fp16's range by one power of two for its keys and one for its values (what is
 // 2^-24 of the tile's largest loses bits).  Queries, a row each, likewise: bfloat16's 8 bits are exact.
-// Blocks of kUnpackThreads: first a tile of a head each, then rows of queries, a warp a row.  A block reads its scales first (the tile's power of two) and then
-// the codes: two chains of loads bound it (2,048 keys of 8 heads of 128 and 1,024 tokens' queries: 6 us for 28 MB, most of it written; the attention
-// behind it 46, as long as over a bfloat16 cache).
+// Blocks of kUnpackThreads: first a tile of a head each, then rows of queries, eight elements a lane.  A block asks for a tile's codes and
+// scales at once and finds the power of two from the latter; the chain of loads (length, page, codes) bounds it (2,048 keys of 8
+// heads of 128 and 1,024 tokens' queries: 5.5 us for 28 MB, most of it written; the attention behind it 46, as long as over a
+// bfloat16 cache).
 constexpr int kTile = 128, kUnpackThreads = 512;
 
 __device__ __forceinline__ uint32_t half_times(uint32_t code_pair, __half2 s) {        // (codes + 1024 as fp16 numbers) -> (code - 8) s
@@ -545,30 +546,32 @@ kv4_unpack_kernel(const uint8_t* cache, const int* block_table, int table_stride
                   __half* q_out, float* q_power, int nq, int tile_blocks) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int kUnits = kTile / kKv4Unit, NG = D / kKv4Group, U = kv4_unit_bytes(D);
+  constexpr int kUnits = kTile / kKv4Unit, U = kv4_unit_bytes(D);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if ((int)blockIdx.x >= tile_blocks) {                                   // ---- queries
     const int tok0 = cu_q[0], rows = (cu_q[n_seqs] - tok0) * nq;
-    const int row = ((int)blockIdx.x - tile_blocks) * (kUnpackThreads / 32) + warp;
-    if (row >= rows) return;
-    const size_t at = ((size_t)tok0 * nq + row) * D;
-    constexpr int E = D / 32;                                             // elements a lane
-    float x[E];
+    constexpr int LANES = D / 8, ROWS = kUnpackThreads / LANES;           // eight elements a lane
+    const int row = ((int)blockIdx.x - tile_blocks) * ROWS + threadIdx.x / LANES;
+    const bool there = row < rows;
+    const size_t at = ((size_t)tok0 * nq + row) * D + threadIdx.x % LANES * 8;
+    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+    if (there) w = *reinterpret_cast<const uint4*>(q + at);
+    float x[8];
+    unpack8(w, x);
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < E; i += 2) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(q + at + lane * E + i);
-      x[i] = __uint_as_float(w << 16);
-      x[i + 1] = __uint_as_float(w & 0xffff0000u);
-      top = max(top, max((w & 0x7fffu) << 16, w & 0x7fff0000u));
-    }
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
 #pragma unroll
-    for (int o = 16; o > 0; o /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int o = LANES / 2; o > 0; o /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     const int e = top >= 0x7f800000u ? 0 : max((int)(top >> 23) - 127, -126);
     const float bring = power_of_two(-e);
+    __align__(16) __half2 h[4];
 #pragma unroll
-    for (int i = 0; i < E; i += 2) *reinterpret_cast<__half2*>(q_out + at + lane * E + i) = __floats2half2_rn(x[i] * bring, x[i + 1] * bring);
-    if (lane == 0) q_power[(size_t)tok0 * nq + row] = power_of_two(e);
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[2 * i] * bring, x[2 * i + 1] * bring);
+    if (there) {
+      *reinterpret_cast<uint4*>(q_out + at) = *reinterpret_cast<const uint4*>(h);
+      if (threadIdx.x % LANES == 0) q_power[(size_t)tok0 * nq + row] = power_of_two(e);
+    }
     return;
   }
   // ---- a tile of a head
@@ -588,16 +591,28 @@ kv4_unpack_kernel(const uint8_t* cache, const int* block_table, int table_stride
   }
   __syncthreads();
   const int lo = max(first - key0, 0), hi = min(length - key0, kTile);    // rows that some token sees
-  uint32_t most[2] = {0u, 0u};
-  for (int i = threadIdx.x; i < kTile * NG; i += kUnpackThreads) {
-    const int row = i / NG, at = unit_at[row / kKv4Unit];
-    if (at < 0 || row < lo || row >= hi) continue;
-    const uint8_t* unit = cache + (size_t)at * U;
+  constexpr int kPerRow = D / 8, kItems = kTile * kPerRow / kUnpackThreads;
+  static_assert(kItems * kUnpackThreads == kTile * kPerRow, "eight elements a thread at a time");
+  uint32_t k[kItems], v[kItems], ks[kItems], vs[kItems];
 #pragma unroll
-    for (int value = 0; value < 2; ++value) {
-      const uint32_t s = *reinterpret_cast<const uint16_t*>(unit + kv4_scale_at(D, value, row % kKv4Unit, i % NG));
-      if (s < 0x7f80u) most[value] = max(most[value], s);
+  for (int n = 0; n < kItems; ++n) {
+    const int i = threadIdx.x + n * kUnpackThreads, row = i / kPerRow, e8 = i % kPerRow, j = row % kKv4Unit, G = e8 >> 2, l = 2 * (e8 & 3), at = unit_at[row / kKv4Unit];
+    k[n] = v[n] = 0x88888888u;
+    ks[n] = vs[n] = 0u;
+    if (at >= 0 && row >= lo && row < hi) {
+      const uint8_t* unit = cache + (size_t)at * U;
+      k[n] = *reinterpret_cast<const uint32_t*>(unit + kv4_key_at(D, j, G, l));
+      v[n] = (uint32_t)*reinterpret_cast<const uint16_t*>(unit + kv4_value_at(D, j, G, l)) |
+             (uint32_t)*reinterpret_cast<const uint16_t*>(unit + kv4_value_at(D, j, G, l + 1)) << 16;
+      ks[n] = *reinterpret_cast<const uint16_t*>(unit + kv4_scale_at(D, false, j, G));
+      vs[n] = *reinterpret_cast<const uint16_t*>(unit + kv4_scale_at(D, true, j, G));
     }
+  }
+  uint32_t most[2] = {0u, 0u};
+#pragma unroll
+  for (int n = 0; n < kItems; ++n) {
+    if (ks[n] < 0x7f80u) most[0] = max(most[0], ks[n]);
+    if (vs[n] < 0x7f80u) most[1] = max(most[1], vs[n]);
   }
 #pragma unroll
   for (int value = 0; value < 2; ++value) {
@@ -620,23 +635,6 @@ kv4_unpack_kernel(const uint8_t* cache, const int* block_table, int table_stride
   }
   const float bring_k = power_of_two(-e[0]), bring_v = power_of_two(-e[1]);
   const size_t out = (page * nkv + head) * kTile * D;
-  constexpr int kPerRow = D / 8, kItems = kTile * kPerRow / kUnpackThreads;
-  static_assert(kItems * kUnpackThreads == kTile * kPerRow, "eight elements a thread at a time");
-  uint32_t k[kItems], v[kItems], ks[kItems], vs[kItems];
-#pragma unroll
-  for (int n = 0; n < kItems; ++n) {
-    const int i = threadIdx.x + n * kUnpackThreads, row = i / kPerRow, e8 = i % kPerRow, j = row % kKv4Unit, G = e8 >> 2, l = 2 * (e8 & 3), at = unit_at[row / kKv4Unit];
-    k[n] = v[n] = 0x88888888u;
-    ks[n] = vs[n] = 0u;
-    if (at >= 0 && row >= lo && row < hi) {
-      const uint8_t* unit = cache + (size_t)at * U;
-      k[n] = *reinterpret_cast<const uint32_t*>(unit + kv4_key_at(D, j, G, l));
-      v[n] = (uint32_t)*reinterpret_cast<const uint16_t*>(unit + kv4_value_at(D, j, G, l)) |
-             (uint32_t)*reinterpret_cast<const uint16_t*>(unit + kv4_value_at(D, j, G, l + 1)) << 16;
-      ks[n] = *reinterpret_cast<const uint16_t*>(unit + kv4_scale_at(D, false, j, G));
-      vs[n] = *reinterpret_cast<const uint16_t*>(unit + kv4_scale_at(D, true, j, G));
-    }
-  }
 #pragma unroll
   for (int n = 0; n < kItems; ++n) {
     const size_t o = out + (size_t)(threadIdx.x + n * kUnpackThreads) * 8;
@@ -784,7 +782,7 @@ ILB_EXPORT int ilb_kv4_unpack(const void* cache, const int* block_table, int tab
   ILB_REQUIRE((d == 64 || d == 128) && n_seqs > 0 && max_tiles > 0 && nq > 0 && n_rows >= 0, "kv4_unpack: bad sizes");
   ILB_REQUIRE((((uintptr_t)cache | (uintptr_t)k | (uintptr_t)v | (uintptr_t)info | (uintptr_t)q | (uintptr_t)q_out) % 16) == 0,
               "kv4_unpack: operands must start on 16-byte boundaries");
-  const long long tiles = (long long)n_seqs * max_tiles * nkv, blocks = tiles + (n_rows + kUnpackThreads / 32 - 1) / (kUnpackThreads / 32);
+  const long long tiles = (long long)n_seqs * max_tiles * nkv, per = kUnpackThreads * 8 / d, blocks = tiles + (n_rows + per - 1) / per;
   ILB_REQUIRE(blocks <= 0x7fffffffLL, "kv4_unpack: too much for one launch");
 #define ILB_KV4_UNPACK(DIM)                                                                                                                \
   ilb::launch(kv4_unpack_kernel<DIM>, dim3((unsigned)blocks), dim3(kUnpackThreads), 0, stream, (const uint8_t*)cache, block_table, table_stride, lengths, \
