@@ -1775,16 +1775,16 @@ KV4_UNPACK_TOKENS = 1 << 17 # tokens whose keys and values are unpacked at a tim
 KV4_TILE = 128              # keys of a tile of the prefill kernel
 _KV4_ORDER: dict = {}       # 0, 1, 2, .. on each device, written on the stream that reads it
 _KV4_WORKSPACE: dict = {}
+_KV4_DEVICES: dict = {}    # device index -> (SMs, the flag of waits that ran out)
 _KV4_PLANS: dict = {}      # sizes of a launch -> (floats of scratch, tickets) that it needs
 
 
-def _kv4_workspace(q: torch.Tensor):
+def _kv4_workspace(device: torch.device, stream: int):
     """The scratch of callers that bring no workspace of their own: one per device and stream."""
-    key = (q.device, _raw_stream(q))
-    ws = _KV4_WORKSPACE.get(key)
+    ws = _KV4_WORKSPACE.get((device.index, stream))
     if ws is None:
         from ..parts.base import Workspace
-        ws = _KV4_WORKSPACE[key] = Workspace(q.device)
+        ws = _KV4_WORKSPACE[device.index, stream] = Workspace(device)
     return ws
 
 
@@ -1804,8 +1804,11 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
     positions, cu_q = step.positions, step.cu_q
     if nq <= 0 or nq % nkv or width != nq * d or out.shape != shape or positions.numel() != T or cu_q.numel() != S + 1:
         raise KernelError("kv4_attention: queries, output, step and block table do not agree")
-    _kv4_ints("kv4_attention positions and offsets", positions, cu_q)
-    _kv4_ints("kv4_attention positions and lengths", positions, step.kv_len)
+    kv_len = step.kv_len
+    if not (positions.dtype is cu_q.dtype is kv_len.dtype is _INT32 and positions.is_cuda and cu_q.is_cuda and kv_len.is_cuda
+            and positions.is_contiguous() and cu_q.is_contiguous() and kv_len.is_contiguous()):
+        for t in (positions, cu_q, kv_len):
+            _need(t, "kv4_attention positions, offsets and lengths", torch.int32)
     if sink is not None:
         _need(sink, "kv4_attention sink", torch.float32)
         if sink.numel() != nq:
@@ -1813,22 +1816,40 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
     if T == 0:
         return
     window, device, code = window or 0, q.device, F32 if dtype is torch.float32 else _code(q)
-    at, to, held = q.data_ptr(), out.data_ptr(), cache.data_ptr()
-    sinks = 0 if sink is None else sink.data_ptr()
+    at, to, held, where = q.data_ptr(), out.data_ptr(), cache.data_ptr(), positions.data_ptr()
+    sinks, stream = 0 if sink is None else sink.data_ptr(), torch._C._cuda_getCurrentRawStream(device.index)
     if d not in KV4_ROWS_HEADS or (at | to | held) % 16:
         _need(step.seq_of_token, "kv4_attention sequence indices", torch.int32)
-        _call("attention_kv4", "ilb_kv4_attention_simple", at, to, code, held, positions.data_ptr(), step.seq_of_token.data_ptr(),
-              block_table.data_ptr(), max_blocks, page_size, num_pages, window, scale, T, nq, nkv, d, width, width, sinks, _raw_stream(q))
+        _call("attention_kv4", "ilb_kv4_attention_simple", at, to, code, held, where, step.seq_of_token.data_ptr(),
+              block_table.data_ptr(), max_blocks, page_size, num_pages, window, scale, T, nq, nkv, d, width, width, sinks, stream)
         return
-    ws = _kv4_workspace(q) if workspace is None else workspace
+    known = _KV4_DEVICES.get(device.index)
+    if known is None:
+        known = _KV4_DEVICES[device.index] = _sm_count(device), _tc_state(device).error
+    sms, error = known[0], known[1].data_ptr()
+    ws, offsets, table = _kv4_workspace(device, stream) if workspace is None else workspace, cu_q.data_ptr(), block_table.data_ptr()
+
+    def rows(a: int, b: int, most: int, single: int) -> None:
+        """Sequences a .. b - 1, those of up to `most` tokens, on the kernel that reads the codes."""
+        key = (code, b - a, most, nq, nkv, d, sms)
+        plan = _KV4_PLANS.get(key)
+        if plan is None:
+            plan = _KV4_PLANS[key] = _kv4_plan(*key)
+        floats, n_tickets = plan
+        scratch = tickets = 0
+        if floats:
+            scratch, tickets = ws.address("kv4.records", floats, torch.float32), ws.address("kv4.tickets", max(n_tickets, 4096), _INT32, True)
+        _call("attention_kv4", "ilb_kv4_attention_rows", at, to, code, held, where, offsets + 4 * a, table + 4 * a * max_blocks, max_blocks, page_size,
+              num_pages, window, scale, b - a, most, single, nq, nkv, d, width, width, sinks, sms, scratch, floats, tickets, n_tickets, error, stream)
+
     if step.decode_only:
-        _kv4_rows(q, out, cache, step, block_table, 0, S, 1, 1, window, scale, nq, nkv, d, sinks, code, ws)
+        rows(0, S, 1, 1)
         return
-    lens, kv, G, sms = step.h_q_len, step.h_kv_len, nq // nkv, _sm_count(device)
+    lens, kv, G = step.h_q_len, step.h_kv_len, nq // nkv
     longest = max(lens)
     short = max(KV4_SHORT_ROWS // G, 1)
     if longest <= short or -(-longest * G // 16) * S * nkv <= KV4_ROWS_ROUNDS * sms:
-        _kv4_rows(q, out, cache, step, block_table, 0, S, longest, 0, window, scale, nq, nkv, d, sinks, code, ws)
+        rows(0, S, longest, 0)
         return
     unpacks = dtype is torch.bfloat16 and scale > 0 and attention_tc_supported(nq, nkv, d, KV4_TILE)
     a = rest = 0
@@ -1853,30 +1874,18 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
             while b < S and lens[b] > short and not (unpacks and kv[b] <= KV4_UNPACK_TOKENS) \
                     and (b + 1 - a) * -(-max(most, lens[b]) * G // 8) <= KV4_BLOCKS:
                 b, most = b + 1, max(most, lens[b])
-        _kv4_rows(q, out, cache, step, block_table, a, b, most, 0, window, scale, nq, nkv, d, sinks, code, ws)
+        rows(a, b, most, 0)
         a = b
     if rest:                                             # the others, by their length
-        _kv4_rows(q, out, cache, step, block_table, 0, S, rest, 0, window, scale, nq, nkv, d, sinks, code, ws)
+        rows(0, S, rest, 0)
 
 
-def _kv4_rows(q, out, cache, step, block_table, a: int, b: int, most: int, single: int, window: int, scale: float, nq: int, nkv: int, d: int,
-              sinks: int, code: int, ws) -> None:
-    """Sequences a .. b - 1 of the step, those of up to `most` tokens, on the kernel that reads the codes."""
-    device, width, max_blocks = q.device, nq * d, block_table.shape[1]
-    key = (code, b - a, most, nq, nkv, d, _sm_count(device))
-    plan = _KV4_PLANS.get(key)
-    if plan is None:
-        lib, found = load_module("attention_kv4"), (ctypes.c_longlong(), ctypes.c_longlong())
-        if lib.ilb_kv4_attention_rows_plan(*map(_i, key), *map(ctypes.byref, found)) != 0:
-            raise KernelError(lib.ilb_last_error().decode())
-        plan = _KV4_PLANS[key] = (found[0].value, found[1].value)
-    scratch = tickets = 0
-    if plan[0]:
-        scratch = ws.address("kv4.records", plan[0], torch.float32)
-        tickets = ws.address("kv4.tickets", max(plan[1], 4096), torch.int32, True)
-    _call("attention_kv4", "ilb_kv4_attention_rows", q.data_ptr(), out.data_ptr(), code, cache.data_ptr(), step.positions.data_ptr(),
-          step.cu_q.data_ptr() + 4 * a, block_table.data_ptr() + 4 * a * max_blocks, max_blocks, cache.shape[2] * KV4_UNIT, cache.shape[0], window, scale,
-          b - a, most, single, nq, nkv, d, width, width, sinks, key[6], scratch, plan[0], tickets, plan[1], _tc_state(device).error.data_ptr(), _raw_stream(q))
+def _kv4_plan(*sizes: int) -> tuple:
+    """(floats of scratch, tickets) that a launch of the kernel that reads the codes needs."""
+    lib, found = load_module("attention_kv4"), (ctypes.c_longlong(), ctypes.c_longlong())
+    if lib.ilb_kv4_attention_rows_plan(*map(_i, sizes), *map(ctypes.byref, found)) != 0:
+        raise KernelError(lib.ilb_last_error().decode())
+    return found[0].value, found[1].value
 
 
 def _kv4_portions(q, out, cache, step, block_table, a: int, b: int, tiles: int, window: int, scale: float, nq: int, nkv: int, d: int, sink, ws) -> None:
