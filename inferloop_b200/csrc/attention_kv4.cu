@@ -27,10 +27,11 @@
 //   merge    a CTA's warps through shared memory; several CTAs' records through a scratch buffer, by the CTA that takes the last ticket, in
 //            the order of the CTAs (the result does not depend on who is last).
 // What bounds it.  Many keys: instructions.  A unit takes 297 a warp for eight rows (ALU 141, FMA 95, shared memory 21, tensor 17), and an SM
-// with 12 warps at it 111 clocks a unit, where the copy rate would be 97.  Few keys: the chain launch, position, page, first units, merge, ticket, records, 5.5 us where nothing is cut and 8.5 where runs are joined.
-// Measured, us (floor of bytes), launch after launch, bfloat16, 32 / 8 heads of 128: 1 x 1,030 keys 8.5 (0.2), 8 x 1,030 10.0 (1.3), 64 x 1,030
-// 22.8 (10.4, 3.0 TB/s), 64 x 4,102 69.6 (41.1, 3.9 TB/s), 16 x 4,000 21.4 (10.5), 64 / 8 heads 2 x 16,000 17.2 (5.6), 128 / 8 heads 64 x 1,030 36.7,
-// 32 / 8 heads of 64 14.9 (5.2); float32 19 x 700 of 8 / 2 heads of 64 7.6.
+// with 12 warps at it 111 clocks a unit, where the copy rate would be 97.  Few keys: the chain launch, position, page, first units, merge,
+// ticket, records, 5.5 us where nothing is cut and 8.5 where runs are joined.
+// Measured, us (floor of bytes), launch after launch, bfloat16, 32 / 8 heads of 128: 1 x 1,030 keys 8.5 (0.2), 8 x 1,030 10.0 (1.3),
+// 64 x 1,030 22.8 (10.4, 3.0 TB/s), 64 x 4,102 69.6 (41.1, 3.9 TB/s), 16 x 4,000 21.4 (10.5), 64 / 8 heads 2 x 16,000 17.3 (5.6), 128 / 8 heads
+// 64 x 1,030 36.7, 32 / 8 heads of 64 14.9 (5.2); float32 19 x 700 of 8 / 2 heads of 64 7.6.
 #include <math.h>
 #include <cuda_fp16.h>
 #include <type_traits>
@@ -54,8 +55,8 @@ constexpr int kWholePairs = 2;
 // 128, us, without this rule and with it: 64 x 1,030 keys 24.0 and 22.8, 200 x 500 41 and 36, 500 x 200 76 and 54).
 constexpr int kWholeOfMany = 16;
 constexpr int kSms = 148;
-// (sequence, block of rows) pairs whose keys are cut.  So many and more even out by themselves, and to survey them costs each CTA more
-// than the ragged end (8 / 2 heads, us, surveyed and not: 1,100 x 100 keys 90 and 25, 1,500 x 600 192 and 67).
+// (sequence, block of rows) pairs whose keys are cut.  So many and more even out by themselves, and the CTAs that look for further runs
+// cost more than the ragged end (8 / 2 heads, us, with them and without: 1,100 x 100 keys 30 and 25, 1,500 x 600 73 and 67, 4,000 x 60 97 and 77).
 constexpr int kMaxCut = 1024;
 constexpr int kFewRecords = 8;              // records that a thread asks for all at once
 
@@ -383,7 +384,8 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
   }
   const int n_pairs = pairs_of(mine4);
   if (n_pairs == 0) return;
-  const int seq = p.row_blocks == 1 ? z : quotient(z, p.row_blocks), row0 = (z - seq * p.row_blocks) * kRows, tok0 = mine4.x, rows = mine4.y * G, n_rows = min(kRows, rows - row0);
+  const int seq = p.row_blocks == 1 ? z : quotient(z, p.row_blocks), row0 = (z - seq * p.row_blocks) * kRows, tok0 = mine4.x, rows = mine4.y * G,
+            n_rows = min(kRows, rows - row0);
   // keys that the block's tokens see at all, and those that every one of them sees
   const int pos_a = mine4.z, pos_b = mine4.w, lo_b = first_key(pos_b, p.window);
   const int unit0 = first_key(pos_a, p.window) / kKv4Unit, n_units = pos_b / kKv4Unit + 1 - unit0;

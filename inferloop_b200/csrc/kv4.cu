@@ -743,9 +743,9 @@ ILB_EXPORT int ilb_qk_norm_rope_kv4(const void* qkv, int qkv_stride, void* q_out
       (qkv_stride | q_stride) % 8 == 0 && (((uintptr_t)qkv | (uintptr_t)rope | (uintptr_t)q_weight | (uintptr_t)k_weight) % 16) == 0 &&
       (q_weight == nullptr) == (k_weight == nullptr)) {
     const __nv_bfloat16* rows = (const __nv_bfloat16*)qkv;
-    const WideArgs w = {rows, rows + (size_t)nq * d, rows + (size_t)(nq + nkv) * d, qkv_stride, qkv_stride, d, qkv_stride, d, (__nv_bfloat16*)q_out, q_stride, q_weight, k_weight,
-                        eps, (const float2*)rope, q_weight != nullptr || (mode & kNormUnweighted) != 0, positions, seq_of_token, block_table, max_blocks, page_size,
-                        num_pages, (uint8_t*)cache, n_tokens, nq, nkv};
+    const WideArgs w = {rows, rows + (size_t)nq * d, rows + (size_t)(nq + nkv) * d, qkv_stride, qkv_stride, d, qkv_stride, d, (__nv_bfloat16*)q_out,
+                        q_stride, q_weight, k_weight, eps, (const float2*)rope, q_weight != nullptr || (mode & kNormUnweighted) != 0, positions,
+                        seq_of_token, block_table, max_blocks, page_size, num_pages, (uint8_t*)cache, n_tokens, nq, nkv};
     // two rows a lane where there are many (48 heads of 128, us: 64 tokens 2.8 with one and 3.1 with two, 512 tokens 5.2 and 4.5, 2,048 13.5 and 11.1)
     if (d == 64) n_tokens < 256 ? launch_wide<64, true, 1>(w, stream) : launch_wide<64, true, 2>(w, stream);
     else n_tokens < 256 ? launch_wide<128, true, 1>(w, stream) : launch_wide<128, true, 2>(w, stream);
