@@ -464,7 +464,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const int row_pooled = POOL ? lo / p.pool : 0;     // pooled rows this row sees
     constexpr int kOCols = DV / 2;                     // columns of O this thread owns
     float m_used = -1e30f, l = 0.f;
-    const float row_scale = HALF && live ? p.scale_log2 * p.q_power[(size_t)(tok0 + tl) * p.nq + head] : p.scale_log2;
+    const float row_power = HALF && live ? p.q_power[(size_t)(tok0 + tl) * p.nq + head] : 1.f;
     bool ok = true;
     auto block_sync = [&]() {                           // the 256 threads of this row block
       if (q == 0) asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -476,11 +476,11 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const int see_lo = in_pool ? 0 : lo, see_hi = in_pool ? row_pooled - 1 : pos;      // what this row sees of the tile's set of keys
       const int t = s_buf(q, u);
       const uint32_t s_t = s_cols(q, u) + lane_addr;     // this row of the S buffer
-      float scale = row_scale, v_exp = 0.f, v_back = 1.f;
+      float scale = p.scale_log2, v_exp = 0.f, v_back = 1.f;
       uint32_t held = 0xfu;                               // this thread's 64 keys
       if constexpr (HALF) {
         const float4 info = p.tile_info[((size_t)seq * p.max_blocks + first_tile + u) * p.nkv + kvh];
-        scale = row_scale * info.x;
+        scale = fmaxf(scale * info.x * row_power, 1.17549435e-38f);      // (a factor that falls to 0 would make NaN of a masked key's -inf; scores that small are all alike)
         v_exp = info.y;
         v_back = info.z;
         held = (__float_as_uint(info.w) >> (4 * half)) & 0xfu;

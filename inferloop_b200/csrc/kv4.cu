@@ -563,7 +563,7 @@ kv4_unpack_kernel(const uint8_t* cache, const int* block_table, int table_stride
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
 #pragma unroll
     for (int o = LANES / 2; o > 0; o /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const int e = top >= 0x7f800000u ? 0 : max((int)(top >> 23) - 127, -126);
+    const int e = top == 0u || top >= 0x7f800000u ? 0 : max((int)(top >> 23) - 127, -126);
     const float bring = power_of_two(-e);
     __align__(16) __half2 h[4];
 #pragma unroll
