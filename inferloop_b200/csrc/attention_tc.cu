@@ -37,7 +37,10 @@
 //
 // HALF: operands in fp16 that were brought into its range by powers of two (a 4-bit cache read back exactly, kv4.cu): queries a row,
 // keys and values a tile of 128 keys.  A row's scores get its and the tile's powers back with the scale; the values' power joins the
-// exponents, so that P V comes out in one unit, and leaves the row sum again.  Keys whose page is not held are not seen.
+// exponents, so that P V comes out in one unit, and leaves the row sum again, which is held at 2^-12 of its size so that powers from
+// 2^-110 to 2^115 and a long row stay in 32-bit range.  A tile whose values are all zero must not set that unit: it comes with the lowest power, its
+// exponentials are taken against its own largest score and only its share of the row sum is brought to the others'.  Keys whose
+// page is not held are not seen.
 //
 // Reference counterparts: the query-tile prefill kernel on MMAs
 // (crates/backend/cuda-kernels/src/tile/attention/resident_attention_prefill_kernels.rs:378-469)
@@ -66,6 +69,7 @@ __host__ __device__ constexpr int stages_k(int d, int qb) { return qb == 2 ? (d 
 __host__ __device__ constexpr int stages_v(int d, int qb) { return d == 128 ? 2 : 3; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleStep = 8.0f;   // log2 units
+constexpr float kSumBits = 12.0f, kSumUnit = 0x1p-12f;   // HALF: what the row sum is held in
 
 // K-major operand (rows of 128 bytes along K, 8-row groups `group_bytes` apart), 128-byte swizzle.
 __device__ __forceinline__ uint64_t desc_k_major(uint32_t addr, uint32_t group_bytes = 1024) {
@@ -155,7 +159,8 @@ struct Params {
   const float2* turn;                             // POOL: [tokens][DV / 2] (cos, sin), or null
   int skip_single;       // sequences that bring one token are somebody else's (the decode kernel's)
   const float* sink;     // [nq] or null: a logit per query head that joins the softmax's denominator unscaled, without a value
-  // HALF: [sequence][tile][kv head] 2^e of the keys, e of the values, 2^-e of the values, a bit for every 16 keys that are held; [token][nq] 2^e of the queries
+  // HALF: [sequence][tile][kv head] 2^e of the keys, e of the values, 2^-e of the values (0: they are all zero), a bit for every 16 keys that are
+  // held; [token][nq] 2^e of the queries
   const float4* tile_info; const float* q_power;
 };
 
@@ -518,13 +523,19 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       mx = fmaxf(mx, xmax[(u & 1) * 256 + (half ^ 1) * 128 + row]);
       const bool grow = mx > m_used + kRescaleStep;
       const float m_new = grow ? mx : m_used;
+      float shift = v_exp - m_new;
+      if (HALF && v_back == 0.f) {
+        const float own = mx - v_exp;                     // (-inf where the row sees none of the tile)
+        shift = own == -INFINITY ? 0.f : -own;
+        v_back = exp2f(own - m_new);
+      }
       // exponentials and the row sum (two chains); P as bfloat16, two keys to a 32-bit word
       float sum0 = 0.f, sum1 = 0.f;
       uint32_t packed[E / 2];
 #pragma unroll
       for (int e = 0; e < E / 2; ++e) {
-        const float e0 = ex2(fmaf(v[2 * e], scale, v_exp - m_new));
-        const float e1 = ex2(fmaf(v[2 * e + 1], scale, v_exp - m_new));
+        const float e0 = ex2(fmaf(v[2 * e], scale, shift));
+        const float e1 = ex2(fmaf(v[2 * e + 1], scale, shift));
         sum0 += e0; sum1 += e1;
         if constexpr (HALF) {
           __half2 hh = __floats2half2_rn(e0, e1);
@@ -551,10 +562,13 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             tmem_store_32(o_t + half * kOCols + c0, o);
           }
         }
-        l *= corr;
+        if constexpr (HALF) {                              // (behind tiles of zeros the steps can be wider than one factor holds)
+          const float root = exp2f(0.5f * (m_used - m_new));
+          l = l * root * root;
+        } else l *= corr;
         m_used = m_new;
       }
-      l += HALF ? (sum0 + sum1) * v_back : sum0 + sum1;
+      l += HALF ? (sum0 + sum1) * kSumUnit * v_back : sum0 + sum1;
       // P takes the first KS / 2 columns of the S buffer its scores came from: this thread's
       // keys are columns (E / 2) half .. (E / 2) half + E / 2 - 1
       tmem_store_32u(s_t + half * (E / 2), packed);
@@ -569,7 +583,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     block_sync();
     l += xmax[512 + (half ^ 1) * 128 + row];
     // the sink's term, relative to the maximum the sums were taken against (both halves of a row share it)
-    if (p.sink != nullptr && live && l > 0.f) l += exp2f(p.sink[head] * kLog2e - m_used);
+    if (p.sink != nullptr && live && l > 0.f) l += exp2f(HALF ? p.sink[head] * kLog2e - m_used - kSumBits : p.sink[head] * kLog2e - m_used);
     if (ok) {
       const float inv = l > 0.f ? 1.f / l : 0.f;
       __nv_bfloat16* dst = p.out + (size_t)(tok0 + (live ? tl : 0)) * p.out_stride + (size_t)head * DV + half * kOCols;
@@ -577,6 +591,10 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       for (int c0 = 0; c0 < kOCols; c0 += 32) {
         float o[32];
         tmem_load_32(o_t + half * kOCols + c0, o);       // collective: every lane of the warp takes part
+        if constexpr (HALF) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] *= kSumUnit;
+        }
         if constexpr (POOL) {
           if (p.turn != nullptr) {                         // the pair's other member is the other thread's column
             float w[32];

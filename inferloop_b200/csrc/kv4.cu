@@ -622,16 +622,18 @@ kv4_unpack_kernel(const uint8_t* cache, const int* block_table, int table_stride
   }
   __syncthreads();
   int e[2];
+  bool flat[2];
   for (int value = 0; value < 2; ++value) {
     uint32_t m = 0;
     for (int w = 0; w < kUnpackThreads / 32; ++w) m = max(m, top[value][w]);
-    e[value] = m == 0u ? 0 : max((int)(m >> 7) - 127, -100) - 10;         // the largest scale comes to 2^10, seven times it below 2^14
+    e[value] = max((int)(m >> 7) - 127, -100) - 10;                       // the largest scale comes to 2^10, seven times it below 2^14
+    flat[value] = m == 0u;                                                // (no scale but 0, or none that is a number)
   }
   const size_t page = (size_t)seq * max_tiles + tile;
   if (threadIdx.x == 0) {
     uint32_t held = 0;
     for (int u = 0; u < kUnits; ++u) held |= unit_at[u] >= 0 ? 1u << u : 0u;
-    info[page * nkv + head] = make_float4(power_of_two(e[0]), (float)e[1], power_of_two(-e[1]), __uint_as_float(held));
+    info[page * nkv + head] = make_float4(power_of_two(e[0]), (float)e[1], flat[1] ? 0.f : power_of_two(-e[1]), __uint_as_float(held));
   }
   const float bring_k = power_of_two(-e[0]), bring_v = power_of_two(-e[1]);
   const size_t out = (page * nkv + head) * kTile * D;

@@ -62,3 +62,40 @@ def test_queries_of_nothing_and_next_to_nothing(ops, unpacked, tokens, query, ke
     q[:, d:2 * d] = 0.0
     check(ops, q.bfloat16(), cache, table, L - tokens, tokens, nq, nkv, unpacked=tokens == 90)
     assert bool(unpacked) == (tokens == 90)
+
+
+def leading(lead, tokens, nq, nkv, d, L, ahead, seed):
+    """Queries of one direction with a little noise, and keys of which those in `ahead` stand `lead` before the others in every token's logits."""
+    base = randn(nkv, d, seed=seed).double()
+    q = (base.repeat_interleave(nq // nkv, 0) + 0.1 * randn(tokens, nq, d, seed=seed + 1).double()).flatten(1).bfloat16()
+    k = 0.3 * randn(L, nkv, d, seed=seed + 2).double()
+    k[ahead] += base / (base * base).sum(1, keepdim=True) * lead * d ** 0.5
+    return q, k.bfloat16()
+
+
+@pytest.mark.parametrize("tokens", [1, 90])
+@pytest.mark.parametrize("first,last", [(0, 128), (0, 130), (128, 256), (256, 400), (399, 400), (0, 400)])
+@pytest.mark.parametrize("lead,size", [(0, 1e-3), (6, 1.0), (10, 0.02), (8, 1e-30), (5, 1e6)])
+def test_tiles_of_values_of_nothing(ops, unpacked, tokens, first, last, lead, size):
+    """A tile of 128 keys whose values are all zero weighs what its scores say and takes no precision from the others."""
+    nq, nkv, d, L = 8, 2, 64, 400
+    ahead = torch.arange(first, last)
+    q, k = leading(lead, tokens, nq, nkv, d, L, ahead, 5)
+    v = (size * randn(L, nkv, d, seed=9).double()).bfloat16()
+    v[ahead] = 0.0
+    cache, table = filled(k, v, 16, 3)
+    out = check(ops, q, cache, table, L - tokens, tokens, nq, nkv, unpacked=tokens == 90)
+    assert bool(unpacked) == (tokens == 90) and (last - first < L or not bool(out.any()))
+
+
+@pytest.mark.parametrize("tokens", [1, 90])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -100, 2.0 ** 60])
+def test_long_beginnings_without_values(ops, unpacked, tokens, size):
+    """Many tiles of zeros before the first values, which the sum of the weights has to hold; a head with a sink beside."""
+    nq, nkv, d, L = 4, 1, 128, 3000
+    q, k = leading(4, tokens, nq, nkv, d, L, torch.arange(0, 2700), 15)
+    v = (size * randn(L, nkv, d, seed=19).double()).bfloat16()
+    v[:2700] = 0.0
+    cache, table = filled(k, v, 32, 3)
+    check(ops, q, cache, table, L - tokens, tokens, nq, nkv, unpacked=tokens == 90)
+    check(ops, q, cache, table, L - tokens, tokens, nq, nkv, sink=randn(nq, seed=1), unpacked=tokens == 90)
