@@ -37,8 +37,10 @@
 //
 // HALF: operands in fp16 that were brought into its range by powers of two (a 4-bit cache read back exactly, kv4.cu): queries a row,
 // keys and values a tile of 128 keys.  A row's scores get its and the tile's powers back with the scale; the values' power joins the
-// exponents, so that P V comes out in one unit, and leaves the row sum again, which is held at 2^-12 of its size so that powers from
-// 2^-110 to 2^115 and a long row stay in 32-bit range.  A tile whose values are all zero must not set that unit: it comes with the lowest power, its
+// exponents, so that P V comes out in one unit, and leaves the row sum again, which is held at 2^-19 of its size so that powers from
+// 2^-110 to 2^115 and a long row stay in 32-bit range.  The reference point of P's exponentials lies 2^7 below the largest score: with the
+// 2^8 that it may be behind, P stays below fp16's largest number and is a normal one down to 2^-21 of the largest (a first key that takes
+// nearly all the weight and has next to no value leaves the others 2^-20 of it each; without, they came out 1.5 % off at a lead of 14 nats).  A tile whose values are all zero must not set that unit: it comes with the lowest power, its
 // exponentials are taken against its own largest score and only its share of the row sum is brought to the others'.  Keys whose
 // page is not held are not seen.
 //
@@ -69,7 +71,8 @@ __host__ __device__ constexpr int stages_k(int d, int qb) { return qb == 2 ? (d 
 __host__ __device__ constexpr int stages_v(int d, int qb) { return d == 128 ? 2 : 3; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleStep = 8.0f;   // log2 units
-constexpr float kSumBits = 12.0f, kSumUnit = 0x1p-12f;   // HALF: what the row sum is held in
+constexpr float kLift = 7.0f;          // HALF: the reference point's distance from the largest score, log2 units
+constexpr float kSumBits = 19.0f, kSumUnit = 0x1p-19f;      // HALF: what the row sum is held in (kv4_unpack puts it into the powers that take it there)
 
 // K-major operand (rows of 128 bytes along K, 8-row groups `group_bytes` apart), 128-byte swizzle.
 __device__ __forceinline__ uint64_t desc_k_major(uint32_t addr, uint32_t group_bytes = 1024) {
@@ -159,7 +162,7 @@ struct Params {
   const float2* turn;                             // POOL: [tokens][DV / 2] (cos, sin), or null
   int skip_single;       // sequences that bring one token are somebody else's (the decode kernel's)
   const float* sink;     // [nq] or null: a logit per query head that joins the softmax's denominator unscaled, without a value
-  // HALF: [sequence][tile][kv head] 2^e of the keys, e of the values, 2^-e of the values (0: they are all zero), a bit for every 16 keys that are
+  // HALF: [sequence][tile][kv head] 2^e of the keys, e of the values, 2^(-e - 19) of the values (0: they are all zero), a bit for every 16 keys that are
   // held; [token][nq] 2^e of the queries
   const float4* tile_info; const float* q_power;
 };
@@ -469,7 +472,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const int row_pooled = POOL ? lo / p.pool : 0;     // pooled rows this row sees
     constexpr int kOCols = DV / 2;                     // columns of O this thread owns
     float m_used = -1e30f, l = 0.f;
-    const float row_power = HALF && live ? p.q_power[(size_t)(tok0 + tl) * p.nq + head] : 1.f;
+    const float row_scale = HALF && live ? p.scale_log2 * p.q_power[(size_t)(tok0 + tl) * p.nq + head] : p.scale_log2;
     bool ok = true;
     auto block_sync = [&]() {                           // the 256 threads of this row block
       if (q == 0) asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -481,11 +484,11 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const int see_lo = in_pool ? 0 : lo, see_hi = in_pool ? row_pooled - 1 : pos;      // what this row sees of the tile's set of keys
       const int t = s_buf(q, u);
       const uint32_t s_t = s_cols(q, u) + lane_addr;     // this row of the S buffer
-      float scale = p.scale_log2, v_exp = 0.f, v_back = 1.f;
+      float scale = row_scale, v_exp = 0.f, v_back = 1.f;
       uint32_t held = 0xfu;                               // this thread's 64 keys
       if constexpr (HALF) {
         const float4 info = p.tile_info[((size_t)seq * p.max_blocks + first_tile + u) * p.nkv + kvh];
-        scale = fmaxf(scale * info.x * row_power, 1.17549435e-38f);      // (a factor that falls to 0 would make NaN of a masked key's -inf; scores that small are all alike)
+        scale = fmaxf(row_scale * info.x, 1.17549435e-38f);      // (a factor that falls to 0 would make NaN of a masked key's -inf; scores that small are all alike)
         v_exp = info.y;
         v_back = info.z;
         held = (__float_as_uint(info.w) >> (4 * half)) & 0xfu;
@@ -521,14 +524,10 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       // (this barrier also separates every thread's reads of S from the other half's writes of P below)
       block_sync();
       mx = fmaxf(mx, xmax[(u & 1) * 256 + (half ^ 1) * 128 + row]);
-      const bool grow = mx > m_used + kRescaleStep;
-      const float m_new = grow ? mx : m_used;
-      float shift = v_exp - m_new;
-      if (HALF && v_back == 0.f) {
-        const float own = mx - v_exp;                     // (-inf where the row sees none of the tile)
-        shift = own == -INFINITY ? 0.f : -own;
-        v_back = exp2f(own - m_new);
-      }
+      const bool grow = mx > m_used + (HALF ? kRescaleStep + kLift : kRescaleStep);
+      const float m_new = grow ? (HALF ? mx - kLift : mx) : m_used;
+      const bool no_values = HALF && v_back == 0.f;
+      const float point = no_values ? fmaxf(mx, -1e30f) : m_new, shift = v_exp - point;      // (-1e30: the row sees none of the tile)
       // exponentials and the row sum (two chains); P as bfloat16, two keys to a 32-bit word
       float sum0 = 0.f, sum1 = 0.f;
       uint32_t packed[E / 2];
@@ -568,7 +567,8 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         } else l *= corr;
         m_used = m_new;
       }
-      l += HALF ? (sum0 + sum1) * kSumUnit * v_back : sum0 + sum1;
+      if (no_values) v_back = exp2f(point - v_exp - m_new - kSumBits);
+      l += HALF ? (sum0 + sum1) * v_back : sum0 + sum1;
       // P takes the first KS / 2 columns of the S buffer its scores came from: this thread's
       // keys are columns (E / 2) half .. (E / 2) half + E / 2 - 1
       tmem_store_32u(s_t + half * (E / 2), packed);

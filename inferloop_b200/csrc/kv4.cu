@@ -623,6 +623,7 @@ kv4_unpack_kernel(const uint8_t* cache, const int* block_table, int table_stride
   __syncthreads();
   int e[2];
   bool flat[2];
+#pragma unroll
   for (int value = 0; value < 2; ++value) {
     uint32_t m = 0;
     for (int w = 0; w < kUnpackThreads / 32; ++w) m = max(m, top[value][w]);
@@ -633,7 +634,7 @@ kv4_unpack_kernel(const uint8_t* cache, const int* block_table, int table_stride
   if (threadIdx.x == 0) {
     uint32_t held = 0;
     for (int u = 0; u < kUnits; ++u) held |= unit_at[u] >= 0 ? 1u << u : 0u;
-    info[page * nkv + head] = make_float4(power_of_two(e[0]), (float)e[1], flat[1] ? 0.f : power_of_two(-e[1]), __uint_as_float(held));
+    info[page * nkv + head] = make_float4(power_of_two(e[0]), (float)e[1], flat[1] ? 0.f : power_of_two(-e[1]) * 0x1p-19f, __uint_as_float(held));
   }
   const float bring_k = power_of_two(-e[0]), bring_v = power_of_two(-e[1]);
   const size_t out = (page * nkv + head) * kTile * D;

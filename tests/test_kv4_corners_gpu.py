@@ -99,3 +99,16 @@ def test_long_beginnings_without_values(ops, unpacked, tokens, size):
     cache, table = filled(k, v, 32, 3)
     check(ops, q, cache, table, L - tokens, tokens, nq, nkv, unpacked=tokens == 90)
     check(ops, q, cache, table, L - tokens, tokens, nq, nkv, sink=randn(nq, seed=1), unpacked=tokens == 90)
+
+
+@pytest.mark.parametrize("tokens", [1, 90])
+@pytest.mark.parametrize("lead", [8, 12, 14, 16, 17])
+def test_a_first_key_that_only_takes_weight(ops, unpacked, tokens, lead):
+    """One key with nearly all the weight and next to no value: what comes out is the others', a 2^-24 of the weights each."""
+    nq, nkv, d, L = 8, 2, 64, 700
+    q, k = leading(lead, tokens, nq, nkv, d, L, torch.arange(1), 25)
+    v = randn(L, nkv, d, seed=29)
+    v[0] *= 1e-7
+    cache, table = filled(k, v.bfloat16(), 16, 3)
+    check(ops, q, cache, table, L - tokens, tokens, nq, nkv, unpacked=tokens == 90)
+    assert bool(unpacked) == (tokens == 90)
