@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       mult[nb][c] = fabsf(p.scale_log2) * (PIECES == 1 ? q_sums[kRows * NG + nb * 8 + 2 * t + c] : 1.f);
-      mult[nb][c] = fmaxf(mult[nb][c], 1e-30f);                           // (a scale of zero: no score is told from another)
+      mult[nb][c] = fmaxf(mult[nb][c], 1e-37f);                           // (a scale of zero: no score is told from another; 4 / mult is finite)
       step[nb][c] = 4.f / mult[nb][c];
       base[nb][c] = 0.f; top_score[nb][c] = -INFINITY; l[nb][c] = 0.f;
     }

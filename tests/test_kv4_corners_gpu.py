@@ -64,6 +64,16 @@ def test_queries_of_nothing_and_next_to_nothing(ops, unpacked, tokens, query, ke
     assert bool(unpacked) == (tokens == 90)
 
 
+@pytest.mark.parametrize("tokens", [1, 3, 90])
+def test_next_to_nothing_against_nearly_everything(ops, unpacked, tokens):
+    """Queries of 2^-110 over keys of 2^90 tell nothing apart either."""
+    nq, nkv, d, L = 8, 2, 64, 300
+    k, v = (randn(L, nkv, d, seed=s).bfloat16() for s in (1, 2))
+    cache, table = filled((2.0 ** 90 * k.double()).bfloat16(), v, 16, 3)
+    q = (randn(tokens, nq * d, seed=4).double() * 2.0 ** -110).bfloat16()
+    check(ops, q, cache, table, L - tokens, tokens, nq, nkv, unpacked=tokens == 90)
+
+
 def leading(lead, tokens, nq, nkv, d, L, ahead, seed):
     """Queries of one direction with a little noise, and keys of which those in `ahead` stand `lead` before the others in every token's logits."""
     base = randn(nkv, d, seed=seed).double()
