@@ -333,7 +333,7 @@ qk_norm_rope_kv4_kernel(const T* qkv, int qkv_stride, T* q_out, int q_stride, bo
   }
   if (cache == nullptr) return;
   const int pos = positions[t], blk = pos / page_size;
-  const int page = blk >= 0 && blk < max_blocks ? block_table[(size_t)seq_of_token[t] * max_blocks + blk] : -1;
+  const int page = pos >= 0 && blk < max_blocks ? block_table[(size_t)seq_of_token[t] * max_blocks + blk] : -1;
   if (page < 0 || page >= num_pages) return;                              // never write outside the pool
   const int slot = pos % page_size, j = slot % kKv4Unit, l = lane & 7;
   uint8_t* unit = cache + (((size_t)page * nkv + h) * (page_size / kKv4Unit) + slot / kKv4Unit) * kv4_unit_bytes(d);

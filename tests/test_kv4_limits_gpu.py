@@ -1,0 +1,43 @@
+"""What the 4-bit cache's operators do with tokens, tables and tensors at the edge of what they take: nothing is read or written outside them."""
+import pytest
+import torch
+
+import kv4_bounds
+import kv4_plain as plain
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from inferloop_b200.csrc import ops
+    return ops
+
+
+def randn(*shape, seed):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+
+
+@pytest.mark.parametrize("before", [1, 3, 15, 16, 17, 31, 32, 33, 1000])
+@pytest.mark.parametrize("dtype,off,mode", [(torch.bfloat16, 0, 0), (torch.bfloat16, 1, 0), (torch.bfloat16, 0, 1), (torch.float32, 0, 0)])
+def test_tokens_before_the_first_position_are_left_out(ops, before, dtype, off, mode):
+    """Rows of padding, at positions below 0, in every form of the input stage and of the write."""
+    nq, nkv, d, page = 4, 2, 64, 32
+    step = plain.make_step([5, 0], [2, 3], DEV)
+    step.positions[2:4] = -before
+    table = torch.tensor([[1, 2], [0, 3]], dtype=torch.int32, device=DEV)
+    qkv = randn(5, (nq + 2 * nkv) * d + 8, seed=1).to(dtype).to(DEV)[:, off:off + (nq + 2 * nkv) * d]
+    cache, want = (torch.zeros(6, nkv, page // 16, 18 * d, dtype=torch.uint8, device=DEV) for _ in range(2))
+    cache[:2] = want[:2] = 0xA5                     # (what lies before page 0 of the cache that the call gets)
+    q = torch.zeros(5, nq * d, dtype=dtype, device=DEV)
+    ops.qk_norm_rope_kv4(qkv, q, None, None, 1e-6, None, 0, step, table, cache[2:], True, nq, nkv, d, mode)
+    rows = qkv.unflatten(1, (-1, d)).cpu()
+    pages = [(s, p) for s, p in zip(step.seq_of_token.tolist(), step.positions.tolist())]
+    live = [i for i, (_, p) in enumerate(pages) if p >= 0]
+    host = want.cpu()[2:].clone()
+    plain.write(host, [int(table[pages[i][0], pages[i][1] // page]) for i in live], [pages[i][1] % page for i in live], rows[live, nq:nq + nkv], rows[live, nq + nkv:])
+    assert bool((cache[:2] == 0xA5).all()) and torch.equal(cache[2:].cpu(), host)
+    cache[2:] = 0
+    ops.kv4_write(qkv.unflatten(1, (-1, d))[:, nq:nq + nkv], qkv.unflatten(1, (-1, d))[:, nq + nkv:], step, table, cache[2:])
+    assert bool((cache[:2] == 0xA5).all()) and torch.equal(cache[2:].cpu(), host)
