@@ -278,7 +278,8 @@ __global__ void __launch_bounds__(kWarps * 32, kSmWarps<D, NB> / kWarps) rows_ke
     }
     return b;
   };
-  auto pairs_of = [&](int4 b) { return b.y > 0 ? (b.w / kKv4Unit + 2 - first_key(b.z, p.window) / kKv4Unit) / 2 : 0; };
+  // (a token at a position below 0 sees no key and has one pair, so that its zeros are written and the sum over blocks stays one of counts)
+  auto pairs_of = [&](int4 b) { return b.y > 0 ? max((b.w / kKv4Unit + 2 - first_key(b.z, p.window) / kKv4Unit) / 2, 1) : 0; };
   // Which block and which run of it.  Run 0 of block b is CTA b's, and the others' CTAs come behind all blocks: a CTA of the first kind
   // asks for its pages and queries before it knows how long its run is.
   int z, head, run = 0, runs = 1, extra = 0;                              // extra: of the block's runs but the first, the first one's number among all such

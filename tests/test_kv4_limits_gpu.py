@@ -41,3 +41,30 @@ def test_tokens_before_the_first_position_are_left_out(ops, before, dtype, off, 
     cache[2:] = 0
     ops.kv4_write(qkv.unflatten(1, (-1, d))[:, nq:nq + nkv], qkv.unflatten(1, (-1, d))[:, nq + nkv:], step, table, cache[2:])
     assert bool((cache[:2] == 0xA5).all()) and torch.equal(cache[2:].cpu(), host)
+
+
+def requests(kv, nkv, d, page, seed):
+    """(cache, block table) of sequences of so many keys."""
+    table, pool = plain.make_table(kv, page, 2, seed)
+    cache = torch.zeros(pool, nkv, page // 16, 18 * d, dtype=torch.uint8)
+    for s, n in enumerate(kv):
+        at = torch.arange(n)
+        plain.write(cache, table[s, at // page], at % page, *(randn(n, nkv, d, seed=seed + 2 * s + i).bfloat16() for i in (0, 1)))
+    return cache.to(DEV), table.to(DEV)
+
+
+@pytest.mark.parametrize("window", [0, 700, -512])
+@pytest.mark.parametrize("before", [1, 40, 1000000])
+def test_queries_before_the_first_position_see_nothing(ops, window, before):
+    """A row of padding beside long sequences whose keys are shared out: zeros, and the others as if it were not there, also in the calls after."""
+    nq, nkv, d, kv = 8, 8, 32, [9000, 9000, 33, 9000]
+    cache, table = requests(kv, nkv, d, 64, 7)
+    q = randn(4, nq * d, seed=8).bfloat16()
+    ref, bound = kv4_bounds.outcome(q, cache, table, [n - 1 for n in kv], [1] * 4, window, 0.2, nq, nkv)
+    step = plain.make_step([n - 1 for n in kv], [1] * 4, DEV)
+    for padded in (True, False, True):
+        step.positions[2] = -before if padded else kv[2] - 1
+        out = torch.full((4, nq * d), 5.0, dtype=torch.bfloat16, device=DEV)
+        ops.kv4_attention(q.to(DEV), out, cache, step, table, window, 0.2, nq, nkv, d)
+        rows = [0, 1, 3] if padded else [0, 1, 2, 3]
+        assert bool(((out.cpu().double() - ref).abs() <= bound)[rows].all()) and not (padded and bool(out[2].any()))
