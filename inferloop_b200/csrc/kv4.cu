@@ -583,7 +583,7 @@ kv4_unpack_kernel(const uint8_t* cache, const int* block_table, int table_stride
   if (threadIdx.x < 32) {
     const int key = key0 + (int)threadIdx.x * kKv4Unit;
     int at = -1;
-    if (threadIdx.x < kUnits && key < length) {
+    if (threadIdx.x < kUnits && key < length && key / page_size < table_stride) {
       const int page = block_table[(size_t)seq * table_stride + key / page_size];
       if (page >= 0 && page < num_pages) at = (page * nkv + head) * (page_size / kKv4Unit) + key % page_size / kKv4Unit;
     }

@@ -68,3 +68,19 @@ def test_queries_before_the_first_position_see_nothing(ops, window, before):
         ops.kv4_attention(q.to(DEV), out, cache, step, table, window, 0.2, nq, nkv, d)
         rows = [0, 1, 3] if padded else [0, 1, 2, 3]
         assert bool(((out.cpu().double() - ref).abs() <= bound)[rows].all()) and not (padded and bool(out[2].any()))
+
+
+@pytest.mark.parametrize("tokens", [1, 90])
+@pytest.mark.parametrize("columns", [40, 1])
+def test_keys_past_the_block_table_are_not_held(ops, monkeypatch, tokens, columns):
+    """A length beyond the table's columns, by the codes and with every long portion unpacked."""
+    monkeypatch.setattr(ops, "KV4_ROWS_ROUNDS", 0)
+    nq, nkv, d, L = 8, 2, 64, 1000
+    cache, table = requests([L], nkv, d, 16, 9)
+    q = randn(tokens, nq * d, seed=10).bfloat16()
+    known = table.clone()
+    known[:, columns:] = -1
+    ref, bound = kv4_bounds.outcome(q, cache, known, [L - tokens], [tokens], 0, 0.1, nq, nkv, unpacked=tokens > 1)
+    out = torch.full((tokens, nq * d), 5.0, dtype=torch.bfloat16, device=DEV)
+    ops.kv4_attention(q.to(DEV), out, cache, plain.make_step([L - tokens], [tokens], DEV), table[:, :columns].contiguous(), 0, 0.1, nq, nkv, d)
+    assert bool(((out.cpu().double() - ref).abs() <= bound).all())
