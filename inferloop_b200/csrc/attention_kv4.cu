@@ -1140,6 +1140,7 @@ ILB_EXPORT int ilb_kv4_attention_simple(const void* q, void* out, int dtype, con
   ILB_REQUIRE(d > 0 && d % kKv4Group == 0 && d <= kMaxHead, "kv4_attention: head size %d must be a multiple of 32 up to %d", d, kMaxHead);
   ILB_REQUIRE(page_size > 0 && page_size % kKv4Unit == 0 && num_pages > 0 && max_blocks > 0, "kv4_attention: bad cache geometry");
   ILB_REQUIRE(dtype == kF32 || dtype == kBF16, "kv4_attention: unknown element type");
+  ILB_REQUIRE((uintptr_t)cache % 2 == 0, "kv4_attention: the cache must start on a 2-byte boundary");      // (codes and scales are read two bytes at a time)
   if (n_tokens == 0) return 0;
   const dim3 grid((unsigned)n_tokens, (unsigned)nq);
   if (dtype == kF32)

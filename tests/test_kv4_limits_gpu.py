@@ -84,3 +84,24 @@ def test_keys_past_the_block_table_are_not_held(ops, monkeypatch, tokens, column
     out = torch.full((tokens, nq * d), 5.0, dtype=torch.bfloat16, device=DEV)
     ops.kv4_attention(q.to(DEV), out, cache, plain.make_step([L - tokens], [tokens], DEV), table[:, :columns].contiguous(), 0, 0.1, nq, nkv, d)
     assert bool(((out.cpu().double() - ref).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_cache_off_its_boundary(ops, dtype):
+    """On any even address attention is served; on an odd one it is refused, before anything runs."""
+    nq, nkv, d, kv = 4, 2, 64, [33, 70]
+    cache, table = requests(kv, nkv, d, 16, 11)
+    q, step = randn(2, nq * d, seed=12).to(dtype).to(DEV), plain.make_step([n - 1 for n in kv], [1, 1], DEV)
+    ref, bound = kv4_bounds.outcome(q, cache, table, [n - 1 for n in kv], [1, 1], 0, 0.1, nq, nkv)
+    room = torch.zeros(cache.numel() + 16, dtype=torch.uint8, device=DEV)
+    for off in (2, 8, 14, 1, 15):
+        moved = room[off:off + cache.numel()].view(cache.shape)
+        moved.copy_(cache)
+        out = torch.full_like(q, 5.0)
+        if off % 2:
+            with pytest.raises(ops.KernelError, match="2-byte boundary"):
+                ops.kv4_attention(q, out, moved, step, table, 0, 0.1, nq, nkv, d)
+            assert bool((out == 5.0).all())
+        else:
+            ops.kv4_attention(q, out, moved, step, table, 0, 0.1, nq, nkv, d)
+            assert bool(((out.cpu().double() - ref).abs() <= bound).all())
