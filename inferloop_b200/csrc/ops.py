@@ -1805,6 +1805,8 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
     if nq <= 0 or nq % nkv or width != nq * d or out.shape != shape or positions.numel() != T or cu_q.numel() != S + 1:
         raise KernelError("kv4_attention: queries, output, step and block table do not agree")
     kv_len = step.kv_len
+    if kv_len.numel() != S or (T != S if step.decode_only else len(step.h_q_len) != S or len(step.h_kv_len) != S):
+        raise KernelError(f"kv4_attention: a step of {T} tokens of {S} sequences, whose lengths or kind say otherwise")
     if not (positions.dtype is cu_q.dtype is kv_len.dtype is _INT32 and positions.is_cuda and cu_q.is_cuda and kv_len.is_cuda
             and positions.is_contiguous() and cu_q.is_contiguous() and kv_len.is_contiguous()):
         for t in (positions, cu_q, kv_len):
@@ -1820,6 +1822,8 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
     sinks, stream = 0 if sink is None else sink.data_ptr(), torch._C._cuda_getCurrentRawStream(device.index)
     if d not in KV4_ROWS_HEADS or (at | to | held) % 16:
         _need(step.seq_of_token, "kv4_attention sequence indices", torch.int32)
+        if step.seq_of_token.numel() != T:
+            raise KernelError(f"kv4_attention: {step.seq_of_token.numel()} sequence indices for {T} tokens")
         _call("attention_kv4", "ilb_kv4_attention_simple", at, to, code, held, where, step.seq_of_token.data_ptr(),
               block_table.data_ptr(), max_blocks, page_size, num_pages, window, scale, T, nq, nkv, d, width, width, sinks, stream)
         return

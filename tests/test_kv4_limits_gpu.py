@@ -105,3 +105,29 @@ def test_a_cache_off_its_boundary(ops, dtype):
         else:
             ops.kv4_attention(q, out, moved, step, table, 0, 0.1, nq, nkv, d)
             assert bool(((out.cpu().double() - ref).abs() <= bound).all())
+
+
+def test_steps_that_contradict_themselves(ops):
+    """Fewer tokens than sequences in a step of single tokens, lengths of other sequences than it has, indices of other tokens: refused on the host."""
+    nq, nkv, d = 4, 2, 64
+    cache, table = requests([40, 40, 40], nkv, d, 16, 13)
+    q = randn(3, nq * d, seed=14).bfloat16().to(DEV)
+
+    def step(lens, **changes):
+        st = plain.make_step([20] * len(lens), lens, DEV)
+        for name, value in changes.items():
+            setattr(st, name, value)
+        return st
+    call = lambda st, t, d=d, cache=cache: ops.kv4_attention(q[:t, :nq * d].contiguous(), torch.zeros(t, nq * d, dtype=q.dtype, device=DEV), cache, st, table,
+                                                              0, 0.1, nq, nkv, d)
+    call(step([1, 1, 1]), 3)
+    call(step([0, 2, 1]), 3)
+    bad = [(step([1, 1, 0], decode_only=True), 2), (step([0, 2, 1], kv_len=torch.zeros(2, dtype=torch.int32, device=DEV)), 3),
+           (step([1, 1, 1], kv_len=torch.zeros(4, dtype=torch.int32, device=DEV)), 3), (step([0, 2, 1], h_q_len=[2, 1]), 3), (step([0, 2, 1], h_kv_len=[2, 1]), 3)]
+    for st, t in bad:
+        with pytest.raises(ops.KernelError, match="say otherwise"):
+            call(st, t)
+    other = torch.zeros(3, nkv, 1, 18 * 160, dtype=torch.uint8, device=DEV)
+    with pytest.raises(ops.KernelError, match="indices"):
+        ops.kv4_attention(torch.zeros(3, nq * 160, device=DEV), torch.zeros(3, nq * 160, device=DEV), other,
+                          step([1, 1, 1], seq_of_token=torch.zeros(2, dtype=torch.int32, device=DEV)), table, 0, 0.1, nq, nkv, 160)
