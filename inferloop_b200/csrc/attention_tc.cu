@@ -314,7 +314,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       if (has_box && j < n_tiles) {
         const int key0 = (first_tile + j - pool_tiles) * kKeys;
         const int blk = key0 / p.page_size + box_page;
-        const int pg = blk < p.max_blocks ? __ldg(table + blk) : -1;
+        const int pg = blk >= p.max_blocks ? -1 : HALF ? seq * p.max_blocks + blk : __ldg(table + blk);      // (unpacked tiles lie in order)
         if (pg >= 0 && pg < p.num_pages && key0 + box_page * p.page_size <= pos_last) page = pg;
       }
       return page;
@@ -756,7 +756,7 @@ ILB_EXPORT int ilb_attention_prefill_tc(const void* q, void* out, const void* k_
 // ilb_kv4_unpack leaves them with `tile_info` [n_seqs][max_tiles][nkv][4], `q_power` [tokens][nq] and the queries q [tokens][nq d]:
 // portions of more than one token, scale > 0.
 ILB_EXPORT int ilb_attention_prefill_half(const void* q, void* out, const void* k, const void* v, const void* tile_info, const float* q_power,
-                                          const int* positions, const int* cu_q, const int* page_order, int max_tiles, int window, float scale,
+                                          const int* positions, const int* cu_q, int max_tiles, int window, float scale,
                                           int n_tokens, int n_seqs, int n_tiles, int row_blocks, int nq, int nkv, int d, const float* sink,
                                           int* error_flag, cudaStream_t stream) {
   ILB_REQUIRE(row_blocks == 1 || row_blocks == 2, "attention (tensor cores): %d row blocks per CTA (1 or 2)", row_blocks);
@@ -766,7 +766,7 @@ ILB_EXPORT int ilb_attention_prefill_half(const void* q, void* out, const void* 
   ILB_REQUIRE((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)tile_info) % 16) == 0, "attention (tensor cores): misaligned operands");
   Maps m;
   if (make_maps(&m, q, k, v, n_tokens, nq * d, nq, nkv, d, d, kKeys, n_seqs * max_tiles)) return -1;
-  Params p{(__nv_bfloat16*)out, positions, cu_q, page_order, error_flag, max_tiles, n_seqs, nq, nkv, window, nq * d, kKeys, n_seqs * max_tiles,
+  Params p{(__nv_bfloat16*)out, positions, cu_q, nullptr, error_flag, max_tiles, n_seqs, nq, nkv, window, nq * d, kKeys, n_seqs * max_tiles,
            scale * kLog2e, nullptr, 0, 0, nullptr, 0, sink, (const float4*)tile_info, q_power};
   if (row_blocks == 2)
     return d == 64 ? launch<64, 64, 2, false, true>(m, p, n_tiles, stream) : launch<128, 128, 2, false, true>(m, p, n_tiles, stream);

@@ -67,7 +67,7 @@ _SIGNATURES = {
     "ilb_kv4_read": "ppipipiiiippiiip",
     "ilb_qk_norm_rope_kv4": "pipi" + "ippfpii" + "pppiii" + "piiiip",
     "ilb_kv4_unpack": "ppippp" + "iiiiiii" + "pppppp" + "iqp",
-    "ilb_attention_prefill_half": "ppppppppp" + "iifiiiiiii" + "ppp",
+    "ilb_attention_prefill_half": "pppppppp" + "iifiiiiiii" + "ppp",
     "ilb_kv4_attention_simple": "ppippppiiiifiiiiiipp",
     "ilb_kv4_attention_rows": "ppippppiiiifiiiiiiiipipqpqpp",
 }
@@ -1773,7 +1773,6 @@ KV4_ROWS_ROUNDS = 2
 KV4_BLOCKS = 65535          # (sequence, block of rows) pairs of a launch
 KV4_UNPACK_TOKENS = 1 << 17 # tokens whose keys and values are unpacked at a time: sequences in groups; one with more keys reads the codes
 KV4_TILE = 128              # keys of a tile of the prefill kernel
-_KV4_ORDER: dict = {}       # 0, 1, 2, .. on each device, written on the stream that reads it
 _KV4_WORKSPACE: dict = {}
 _KV4_DEVICES: dict = {}    # device index -> (SMs, the flag of waits that ran out)
 _KV4_PLANS: dict = {}      # sizes of a launch -> (floats of scratch, tickets) that it needs
@@ -1894,15 +1893,12 @@ def _kv4_plan(*sizes: int) -> tuple:
 
 def _kv4_portions(q, out, cache, step, block_table, a: int, b: int, tiles: int, window: int, scale: float, nq: int, nkv: int, d: int, sink, ws) -> None:
     """Sequences a .. b - 1 of the step on the prefill kernel: what they see is unpacked, `tiles` tiles of 128 keys a sequence."""
-    n, device, lens = b - a, q.device, step.h_q_len[a:b]
+    n, lens = b - a, step.h_q_len[a:b]
     half = torch.float16
     k, v = (ws.address("kv4." + w, n * tiles * nkv * KV4_TILE * d, half) for w in ("keys", "values"))
     info = ws.address("kv4.tiles", n * tiles * nkv * 4, torch.float32)
     q_half, q_power = ws.address("kv4.queries", q.numel(), half), ws.address("kv4.query_powers", q.shape[0] * nq, torch.float32)
     stream = _raw_stream(q)
-    order = _KV4_ORDER.get((device, stream))
-    if order is None or order.numel() < n * tiles:       # page s * tiles + t holds tile t of sequence s
-        order = _KV4_ORDER[device, stream] = torch.arange(max(n * tiles, 1 << 14), dtype=torch.int32, device=device)
     positions, cu_q = step.positions.data_ptr(), step.cu_q.data_ptr() + 4 * a
     sinks = 0 if sink is None else sink.data_ptr()
     _call("kv4", "ilb_kv4_unpack", cache.data_ptr(), block_table.data_ptr() + 4 * a * block_table.shape[1], block_table.shape[1],
@@ -1910,8 +1906,8 @@ def _kv4_portions(q, out, cache, step, block_table, a: int, b: int, tiles: int, 
           q.data_ptr(), q_half, q_power, nq, sum(lens) * nq, stream)
     per_block = 128 // (nq // nkv)
     one, two = sum(-(-x // per_block) for x in lens), sum(-(-x // (2 * per_block)) for x in lens)
-    blocks = TC_ATTENTION_ROW_BLOCKS or tc_row_blocks(one * nkv, two * nkv, _sm_count(device), all(kv >= 2 * x for x, kv in zip(lens, step.h_kv_len[a:b])))
-    _call("attention_tc", "ilb_attention_prefill_half", q_half, out.data_ptr(), k, v, info, q_power, positions, cu_q, order.data_ptr(), tiles, window,
+    blocks = TC_ATTENTION_ROW_BLOCKS or tc_row_blocks(one * nkv, two * nkv, _sm_count(q.device), all(kv >= 2 * x for x, kv in zip(lens, step.h_kv_len[a:b])))
+    _call("attention_tc", "ilb_attention_prefill_half", q_half, out.data_ptr(), k, v, info, q_power, positions, cu_q, tiles, window,
           scale, q.shape[0], n, two if blocks == 2 else one, blocks, nq, nkv, d, sinks, _tc_state(device).error.data_ptr(), stream)
 
 
