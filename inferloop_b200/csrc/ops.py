@@ -1908,7 +1908,7 @@ def _kv4_portions(q, out, cache, step, block_table, a: int, b: int, tiles: int, 
     one, two = sum(-(-x // per_block) for x in lens), sum(-(-x // (2 * per_block)) for x in lens)
     blocks = TC_ATTENTION_ROW_BLOCKS or tc_row_blocks(one * nkv, two * nkv, _sm_count(q.device), all(kv >= 2 * x for x, kv in zip(lens, step.h_kv_len[a:b])))
     _call("attention_tc", "ilb_attention_prefill_half", q_half, out.data_ptr(), k, v, info, q_power, positions, cu_q, tiles, window,
-          scale, q.shape[0], n, two if blocks == 2 else one, blocks, nq, nkv, d, sinks, _tc_state(device).error.data_ptr(), stream)
+          scale, q.shape[0], n, two if blocks == 2 else one, blocks, nq, nkv, d, sinks, _tc_state(q.device).error.data_ptr(), stream)
 
 
 DECODE_FUSED_ENABLED = True     # tests switch it off to run q/k norm + rotation + cache write as a launch of its own
