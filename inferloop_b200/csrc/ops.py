@@ -1774,17 +1774,36 @@ KV4_BLOCKS = 65535          # (sequence, block of rows) pairs of a launch
 KV4_UNPACK_TOKENS = 1 << 17 # tokens whose keys and values are unpacked at a time: sequences in groups; one with more keys reads the codes
 KV4_TILE = 128              # keys of a tile of the prefill kernel
 _KV4_WORKSPACE: dict = {}
+_KV4_RECORDS: dict = {}
 _KV4_DEVICES: dict = {}    # device index -> (SMs, the flag of waits that ran out)
 _KV4_PLANS: dict = {}      # sizes of a launch -> (floats of scratch, tickets) that it needs
 
 
+_recording = torch._C._cuda_isCurrentStreamCapturing
+
+
 def _kv4_workspace(device: torch.device, stream: int):
-    """The scratch of callers that bring no workspace of their own: one per device and stream."""
+    """The scratch of portions of callers that bring no workspace of their own: one per device and stream, and, while a graph is recorded, one
+    of this call alone.  The graph's memory pool keeps that one's buffers, so that no recording reads what a later call replaces."""
+    from ..parts.base import Workspace
+    if _recording():
+        return Workspace(device)
     ws = _KV4_WORKSPACE.get((device.index, stream))
     if ws is None:
-        from ..parts.base import Workspace
         ws = _KV4_WORKSPACE[device.index, stream] = Workspace(device)
     return ws
+
+
+def _kv4_records(device: torch.device, stream: int, floats: int, n_tickets: int) -> tuple:
+    """The same for shared keys: (floats, tickets, where they lie, the buffers).  A recording sets its tickets to zero itself: those of
+    another one are not zero before that one is replayed."""
+    old = (0, 4096) if _recording() else _KV4_RECORDS.get((device.index, stream), (0, 4096))
+    floats, n_tickets = max(floats, old[0]), max(n_tickets, old[1])
+    held = torch.empty(floats, dtype=torch.float32, device=device), torch.zeros(n_tickets, dtype=_INT32, device=device)
+    found = floats, n_tickets, held[0].data_ptr(), held[1].data_ptr(), held
+    if not _recording():
+        _KV4_RECORDS[device.index, stream] = found
+    return found
 
 
 def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step, block_table: torch.Tensor, window: int, scale: float,
@@ -1792,8 +1811,8 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
     """Causal attention of the step's tokens over the 4-bit cache; q and out are [T, nq * d] of one type.  `window` and `sink`
     as in `attention`; a token that sees no key (its pages are not held) gets zeros.  Sequences that bring few tokens read the
     codes themselves; longer portions' keys and values (bfloat16 queries, heads of 64 and 128; KV4_ROWS_ROUNDS) are unpacked into `workspace`
-    (None: one of the stream's own) for the tensor cores' prefill kernel.  There a value that was kept as NaN reaches every token of its
-    portion that lies in the same tile of 128 keys, as it does with a bfloat16 cache."""
+    (None: one of the stream's own, or of the graph that is being recorded) for the tensor cores' prefill kernel.  There a value that was
+    kept as NaN reaches every token of its portion that lies in the same tile of 128 keys, as it does with a bfloat16 cache."""
     dtype = q.dtype
     if out.dtype is not dtype or not (q.is_cuda and out.is_cuda and q.is_contiguous() and out.is_contiguous()):
         _need(q, "kv4_attention q"); _need(out, "kv4_attention out", dtype)
@@ -1804,7 +1823,8 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
     if nq <= 0 or nq % nkv or width != nq * d or out.shape != shape or positions.numel() != T or cu_q.numel() != S + 1:
         raise KernelError("kv4_attention: queries, output, step and block table do not agree")
     kv_len = step.kv_len
-    if kv_len.numel() != S or (T != S if step.decode_only else len(step.h_q_len) != S or len(step.h_kv_len) != S):
+    singles = step.decode_only
+    if kv_len.numel() != S or (T != S if singles else len(step.h_q_len) != S or len(step.h_kv_len) != S):
         raise KernelError(f"kv4_attention: a step of {T} tokens of {S} sequences, whose lengths or kind say otherwise")
     if not (positions.dtype is cu_q.dtype is kv_len.dtype is _INT32 and positions.is_cuda and cu_q.is_cuda and kv_len.is_cuda
             and positions.is_contiguous() and cu_q.is_contiguous() and kv_len.is_contiguous()):
@@ -1818,7 +1838,8 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
         return
     window, device, code = window or 0, q.device, F32 if dtype is torch.float32 else _code(q)
     at, to, held, where = q.data_ptr(), out.data_ptr(), cache.data_ptr(), positions.data_ptr()
-    sinks, stream = 0 if sink is None else sink.data_ptr(), torch._C._cuda_getCurrentRawStream(device.index)
+    index = device.index
+    sinks, stream = 0 if sink is None else sink.data_ptr(), torch._C._cuda_getCurrentRawStream(index)
     if d not in KV4_ROWS_HEADS or (at | to | held) % 16:
         _need(step.seq_of_token, "kv4_attention sequence indices", torch.int32)
         if step.seq_of_token.numel() != T:
@@ -1826,11 +1847,11 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
         _call("attention_kv4", "ilb_kv4_attention_simple", at, to, code, held, where, step.seq_of_token.data_ptr(),
               block_table.data_ptr(), max_blocks, page_size, num_pages, window, scale, T, nq, nkv, d, width, width, sinks, stream)
         return
-    known = _KV4_DEVICES.get(device.index)
+    known = _KV4_DEVICES.get(index)
     if known is None:
-        known = _KV4_DEVICES[device.index] = _sm_count(device), _tc_state(device).error
+        known = _KV4_DEVICES[index] = _sm_count(device), _tc_state(device).error
     sms, error = known[0], known[1].data_ptr()
-    ws, offsets, table = _kv4_workspace(device, stream) if workspace is None else workspace, cu_q.data_ptr(), block_table.data_ptr()
+    offsets, table = cu_q.data_ptr(), block_table.data_ptr()
 
     def rows(a: int, b: int, most: int, single: int) -> None:
         """Sequences a .. b - 1, those of up to `most` tokens, on the kernel that reads the codes."""
@@ -1841,11 +1862,18 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
         floats, n_tickets = plan
         scratch = tickets = 0
         if floats:
-            scratch, tickets = ws.address("kv4.records", floats, torch.float32), ws.address("kv4.tickets", max(n_tickets, 4096), _INT32, True)
+            if workspace is not None:
+                scratch, tickets = (workspace.address("kv4.records", floats, torch.float32),
+                                    workspace.address("kv4.tickets", max(n_tickets, 4096), _INT32, True))
+            else:
+                found = None if _recording() else _KV4_RECORDS.get((index, stream))
+                if found is None or found[0] < floats or found[1] < n_tickets:
+                    found = _kv4_records(device, stream, floats, n_tickets)
+                scratch, tickets = found[2], found[3]
         _call("attention_kv4", "ilb_kv4_attention_rows", at, to, code, held, where, offsets + 4 * a, table + 4 * a * max_blocks, max_blocks, page_size,
               num_pages, window, scale, b - a, most, single, nq, nkv, d, width, width, sinks, sms, scratch, floats, tickets, n_tickets, error, stream)
 
-    if step.decode_only:
+    if singles:
         rows(0, S, 1, 1)
         return
     lens, kv, G = step.h_q_len, step.h_kv_len, nq // nkv
@@ -1868,7 +1896,8 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
                     break
                 b, tiles, blocks = b + 1, n, blocks + -(-lens[b] * G // 16) * nkv
             if blocks > KV4_ROWS_ROUNDS * sms:
-                _kv4_portions(q, out, cache, step, block_table, a, b, tiles, window, scale, nq, nkv, d, sink, ws)
+                _kv4_portions(q, out, cache, step, block_table, a, b, tiles, window, scale, nq, nkv, d, sink,
+                              _kv4_workspace(device, stream) if workspace is None else workspace)
                 a = b
                 continue
             most = max(lens[a:b])
