@@ -1674,6 +1674,12 @@ def kv4_cache_shape(pages: int, nkv: int, page_size: int, d: int) -> tuple:
     return (int(pages), int(nkv), page_size // KV4_UNIT, 18 * d)
 
 
+def kv4_unpack_room(longest: Optional[int]) -> int:
+    """Tokens whose keys and values a model's workspace takes unpacked, where a request has up to `longest` of them (None: not known)."""
+    most = KV4_UNPACK_TOKENS if longest is None else KV4_ROOM_REQUESTS * -(-longest // KV4_TILE) * KV4_TILE
+    return min(most, KV4_UNPACK_TOKENS)
+
+
 def kv4_scratch_bytes(tokens: int, nq: int, nkv: int, d: int) -> int:
     """Workspace that `kv4_attention` asks for at most in steps of so many tokens: the unpacked keys and values of a group of
     portions, their queries, the records of shared keys."""
@@ -1773,6 +1779,7 @@ KV4_ROWS_ROUNDS = 2
 KV4_BLOCKS = 65535          # (sequence, block of rows) pairs of a launch
 KV4_UNPACK_TOKENS = 1 << 17 # tokens whose keys and values are unpacked at a time: sequences in groups; one with more keys reads the codes
 KV4_TILE = 128              # keys of a tile of the prefill kernel
+KV4_ROOM_REQUESTS = 8       # portions of requests of full length that a model's scratch takes at a time
 _KV4_WORKSPACE: dict = {}
 _KV4_RECORDS: dict = {}
 _KV4_DEVICES: dict = {}    # device index -> (SMs, the flag of waits that ran out)
@@ -1807,12 +1814,14 @@ def _kv4_records(device: torch.device, stream: int, floats: int, n_tickets: int)
 
 
 def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step, block_table: torch.Tensor, window: int, scale: float,
-                  nq: int, nkv: int, d: int, sink: Optional[torch.Tensor] = None, workspace=None) -> None:
+                  nq: int, nkv: int, d: int, sink: Optional[torch.Tensor] = None, workspace=None, unpack_room: int = 0) -> None:
     """Causal attention of the step's tokens over the 4-bit cache; q and out are [T, nq * d] of one type.  `window` and `sink`
     as in `attention`; a token that sees no key (its pages are not held) gets zeros.  Sequences that bring few tokens read the
     codes themselves; longer portions' keys and values (bfloat16 queries, heads of 64 and 128; KV4_ROWS_ROUNDS) are unpacked into `workspace`
     (None: one of the stream's own, or of the graph that is being recorded) for the tensor cores' prefill kernel.  There a value that was
-    kept as NaN reaches every token of its portion that lies in the same tile of 128 keys, as it does with a bfloat16 cache."""
+    kept as NaN reaches every token of its portion that lies in the same tile of 128 keys, as it does with a bfloat16 cache.
+    `unpack_room`: tokens (`kv4_unpack_room`) that the workspace takes unpacked from the first portion on, so that it does not follow
+    the context."""
     dtype = q.dtype
     if out.dtype is not dtype or not (q.is_cuda and out.is_cuda and q.is_contiguous() and out.is_contiguous()):
         _need(q, "kv4_attention q"); _need(out, "kv4_attention out", dtype)
@@ -1897,7 +1906,7 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
                 b, tiles, blocks = b + 1, n, blocks + -(-lens[b] * G // 16) * nkv
             if blocks > KV4_ROWS_ROUNDS * sms:
                 _kv4_portions(q, out, cache, step, block_table, a, b, tiles, window, scale, nq, nkv, d, sink,
-                              _kv4_workspace(device, stream) if workspace is None else workspace)
+                              _kv4_workspace(device, stream) if workspace is None else workspace, unpack_room)
                 a = b
                 continue
             most = max(lens[a:b])
@@ -1920,13 +1929,15 @@ def _kv4_plan(*sizes: int) -> tuple:
     return found[0].value, found[1].value
 
 
-def _kv4_portions(q, out, cache, step, block_table, a: int, b: int, tiles: int, window: int, scale: float, nq: int, nkv: int, d: int, sink, ws) -> None:
+def _kv4_portions(q, out, cache, step, block_table, a: int, b: int, tiles: int, window: int, scale: float, nq: int, nkv: int, d: int, sink, ws,
+                  unpack_room: int) -> None:
     """Sequences a .. b - 1 of the step on the prefill kernel: what they see is unpacked, `tiles` tiles of 128 keys a sequence."""
-    n, lens = b - a, step.h_q_len[a:b]
-    half = torch.float16
-    k, v = (ws.address("kv4." + w, n * tiles * nkv * KV4_TILE * d, half) for w in ("keys", "values"))
-    info = ws.address("kv4.tiles", n * tiles * nkv * 4, torch.float32)
-    q_half, q_power = ws.address("kv4.queries", q.numel(), half), ws.address("kv4.query_powers", q.shape[0] * nq, torch.float32)
+    n, lens, half, recording = b - a, step.h_q_len[a:b], torch.float16, _recording()
+    held, room = n * tiles * nkv, -(-unpack_room // KV4_TILE) * nkv          # (tiles of a head)
+    k, v = (ws.unrecorded("kv4." + w, held * KV4_TILE * d, half, room * KV4_TILE * d, recording) for w in ("keys", "values"))
+    info = ws.unrecorded("kv4.tiles", held * 4, torch.float32, room * 4, recording)
+    q_half = ws.unrecorded("kv4.queries", q.numel(), half, 0, recording)
+    q_power = ws.unrecorded("kv4.query_powers", q.shape[0] * nq, torch.float32, 0, recording)
     stream = _raw_stream(q)
     positions, cu_q = step.positions.data_ptr(), step.cu_q.data_ptr() + 4 * a
     sinks = 0 if sink is None else sink.data_ptr()

@@ -219,7 +219,7 @@ class ModelRunner:
         self.dtype = dtype
         self.device = device
         self.kv_cache = kv_cache
-        self.ctx = BuildContext(dtype=dtype, device=device, workspace=Workspace(device), kv_bits=parse_kv_cache(kv_cache))
+        self.ctx = BuildContext(dtype=dtype, device=device, workspace=Workspace(device), longest=spec.max_positions, kv_bits=parse_kv_cache(kv_cache))
         self.model = DecoderModel(spec, self.ctx)
         if self.ctx.kv_bits is not None:
             wide = sorted({n.paged for n in self.model.cache_needs() if n.paged is not None and n.paged.bits is None}, key=repr)

@@ -296,7 +296,8 @@ class GQAttention(Mixer):
             ops.qk_norm_rope_kv4(qkv, q, self.q_norm, self.k_norm, self.qk_norm_eps, rope, self.rotary_dim, step, table, cache.kv4, cache.writable,
                                  self.nq, self.nkv, self.d, self.mode)
             ops.scope("attention.attention")
-            ops.kv4_attention(q, o, cache.kv4, step, table, self.seen, self.scale, self.nq, self.nkv, self.d, sink=self.sink, workspace=ws)
+            ops.kv4_attention(q, o, cache.kv4, step, table, self.seen, self.scale, self.nq, self.nkv, self.d, sink=self.sink, workspace=ws,
+                              unpack_room=ops.kv4_unpack_room(self.ctx.longest))
             self._finish(o, qkv, gate_col0, residual, out)
             return
         v_first = None

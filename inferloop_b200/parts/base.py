@@ -38,7 +38,8 @@ class Workspace:
     def __init__(self, device: Optional[torch.device]) -> None:
         self.device = device
         self._buffers: Dict[Tuple[str, torch.dtype], torch.Tensor] = {}
-        self.generation = 0   # bumped whenever a buffer is reallocated
+        self._unrecorded: set = set()      # buffers of `unrecorded` that no recorded step has asked for
+        self.generation = 0   # bumped whenever a buffer that a recorded step may read is reallocated
 
     def buffer(self, tag: str, shape: Sequence[int], dtype: torch.dtype) -> torch.Tensor:
         n = 1
@@ -74,6 +75,25 @@ class Workspace:
             buf = (self.zeroed if zero else self.buffer)(tag, (elements,), dtype)
         return buf.data_ptr()
 
+    def unrecorded(self, tag: str, elements: int, dtype: torch.dtype, room: int = 0, recording: bool = False) -> int:
+        """Like :meth:`address`, for a buffer of steps that are not recorded: it holds `room` elements from the start and grows by doubling
+        behind that, and `generation` stays, so that recorded steps are not recorded again, unless one was asked for with `recording`
+        set.  The buffer is handed out under its tag here alone."""
+        key = (tag, dtype)
+        buf = self._buffers.get(key)
+        if buf is None and not recording:
+            self._unrecorded.add(key)
+        elif recording:
+            self._unrecorded.discard(key)
+        if buf is None or buf.numel() < elements:
+            wanted = max(elements, room, 1) if buf is None or buf.numel() < room else max(elements, 2 * buf.numel())
+            del buf
+            self._buffers.pop(key, None)      # (its memory may be part of what comes: work already on its way is in stream order)
+            buf = self._buffers[key] = torch.empty(wanted, dtype=dtype, device=self.device)
+            if key not in self._unrecorded:
+                self.generation += 1
+        return buf.data_ptr()
+
     def nbytes(self) -> int:
         return sum(b.numel() * b.element_size() for b in self._buffers.values())
 
@@ -84,6 +104,7 @@ class BuildContext:
     device: Optional[torch.device]           # None while only declaring weights
     workspace: Workspace
     cache_dtype: Optional[torch.dtype] = None
+    longest: Optional[int] = None            # tokens that a request has at most (None: not known)
     kv_bits: Optional[int] = None            # 4: keys and values are kept in 4 bits (csrc/kv4.cuh); None: in the cache's dtype
 
     def __post_init__(self) -> None:
