@@ -1680,12 +1680,15 @@ def kv4_unpack_room(longest: Optional[int]) -> int:
     return min(most, KV4_UNPACK_TOKENS)
 
 
-def kv4_scratch_bytes(tokens: int, nq: int, nkv: int, d: int) -> int:
-    """Workspace that `kv4_attention` asks for at most in steps of so many tokens: the unpacked keys and values of a group of
-    portions, their queries, the records of shared keys."""
-    unpacked = KV4_UNPACK_TOKENS * nkv * d * 4 if attention_tc_supported(nq, nkv, d, KV4_TILE) else 0
+def kv4_scratch_bytes(tokens: int, nq: int, nkv: int, d: int, dtype: torch.dtype, longest: Optional[int] = None) -> int:
+    """Workspace that a model of requests of up to `longest` tokens asks for in steps of so many: where portions are unpacked, room for
+    keys and values with their tiles' facts, and the queries; the records of shared keys."""
+    unpacked = 0
+    if dtype is torch.bfloat16 and attention_tc_supported(nq, nkv, d, KV4_TILE):
+        room = kv4_unpack_room(longest)
+        unpacked = room * nkv * 4 * d + room // KV4_TILE * nkv * 16 + tokens * nq * (2 * d + 4)
     ctas = min(tokens, 1024) * nkv + 12 * 148            # a block of rows a sequence, or fewer sequences cut in several
-    return unpacked + tokens * nq * (2 * d + 4) + ctas * (8 if nq <= 8 * nkv else 16) * (d + 4) * 4
+    return unpacked + ctas * (8 if nq <= 8 * nkv else 16) * (d + 4) * 4
 
 
 def _kv4_need(what: str, cache: torch.Tensor, block_table: torch.Tensor, nkv: int, d: int) -> tuple:

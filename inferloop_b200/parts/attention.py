@@ -249,7 +249,7 @@ class GQAttention(Mixer):
         size = torch.empty((), dtype=self.ctx.dtype).element_size()
         width = (self.nq + self.nkv) * self.d + self.v_cols + self.gate_rows
         kept = self.nkv * self.dv if self.value_mix else 0
-        four = ops.kv4_scratch_bytes(tokens, self.nq, self.nkv, self.d) if self.kv_bits == 4 else 0
+        four = ops.kv4_scratch_bytes(tokens, self.nq, self.nkv, self.d, self.ctx.dtype, self.ctx.longest) if self.kv_bits == 4 else 0
         return four + tokens * ((width + self.nq * (self.d + self.dv) + kept) * size + self.rotary_dim * 4)
 
     # ------------------------------------------------------------------ run

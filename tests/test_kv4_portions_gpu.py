@@ -31,3 +31,5 @@ def test_recorded_steps_outlive_a_long_prompt(monkeypatch):
         assert bool(torch.isfinite(step("a", [t])).all())
     assert r.graphs.replays == replays + 3 and all(r.graphs._recorded[k] is rec for k, rec in recorded.items())
     ops.check_device_errors()
+    asked = sum(b.numel() * b.element_size() for (tag, _), b in r.ctx.workspace._buffers.items() if tag.startswith("kv4."))
+    assert asked <= ops.kv4_scratch_bytes(chunk, cfg["num_attention_heads"], cfg["num_key_value_heads"], cfg["head_dim"], torch.bfloat16, 17000)
