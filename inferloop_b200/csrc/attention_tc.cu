@@ -304,6 +304,10 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 
     bool ok = true;
     auto lookup = [&](int j) {                            // page of this lane's box of tile j
+      if constexpr (HALF) {                               // a page a tile, in order
+        const int t = first_tile + j;
+        return t < p.max_blocks && t * kKeys <= pos_last ? seq * p.max_blocks + t : p.num_pages;
+      }
       if (POOL && j < pool_tiles) {
         const int blk = j * pages_per_tile + box_page;
         int pg = -1;
@@ -314,7 +318,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       if (has_box && j < n_tiles) {
         const int key0 = (first_tile + j - pool_tiles) * kKeys;
         const int blk = key0 / p.page_size + box_page;
-        const int pg = blk >= p.max_blocks ? -1 : HALF ? seq * p.max_blocks + blk : __ldg(table + blk);      // (unpacked tiles lie in order)
+        const int pg = blk < p.max_blocks ? __ldg(table + blk) : -1;
         if (pg >= 0 && pg < p.num_pages && key0 + box_page * p.page_size <= pos_last) page = pg;
       }
       return page;
@@ -567,7 +571,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         } else l *= corr;
         m_used = m_new;
       }
-      if (no_values) v_back = exp2f(point - v_exp - m_new - kSumBits);
+      if (no_values) v_back = ex2(point - v_exp - m_new - kSumBits);
       l += HALF ? (sum0 + sum1) * v_back : sum0 + sum1;
       // P takes the first KS / 2 columns of the S buffer its scores came from: this thread's
       // keys are columns (E / 2) half .. (E / 2) half + E / 2 - 1

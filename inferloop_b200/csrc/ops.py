@@ -1795,12 +1795,13 @@ _recording = torch._C._cuda_isCurrentStreamCapturing
 def _kv4_workspace(device: torch.device, stream: int):
     """The scratch of portions of callers that bring no workspace of their own: one per device and stream, and, while a graph is recorded, one
     of this call alone.  The graph's memory pool keeps that one's buffers, so that no recording reads what a later call replaces."""
-    from ..parts.base import Workspace
-    if _recording():
-        return Workspace(device)
-    ws = _KV4_WORKSPACE.get((device.index, stream))
+    recording = _recording()
+    ws = None if recording else _KV4_WORKSPACE.get((device.index, stream))
     if ws is None:
-        ws = _KV4_WORKSPACE[device.index, stream] = Workspace(device)
+        from ..parts.base import Workspace
+        ws = Workspace(device)
+        if not recording:
+            _KV4_WORKSPACE[device.index, stream] = ws
     return ws
 
 

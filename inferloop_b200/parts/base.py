@@ -81,10 +81,10 @@ class Workspace:
         set.  The buffer is handed out under its tag here alone."""
         key = (tag, dtype)
         buf = self._buffers.get(key)
-        if buf is None and not recording:
-            self._unrecorded.add(key)
-        elif recording:
+        if recording:
             self._unrecorded.discard(key)
+        elif buf is None:
+            self._unrecorded.add(key)
         if buf is None or buf.numel() < elements:
             wanted = max(elements, room, 1) if buf is None or buf.numel() < room else max(elements, 2 * buf.numel())
             del buf
