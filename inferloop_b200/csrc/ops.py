@@ -1833,7 +1833,7 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, step,
     shape = q.shape
     T, width = shape if len(shape) == 2 else (-1, -1)
     positions, cu_q = step.positions, step.cu_q
-    if nq <= 0 or nq % nkv or width != nq * d or out.shape != shape or positions.numel() != T or cu_q.numel() != S + 1:
+    if nq <= 0 or nkv <= 0 or nq % nkv or width != nq * d or out.shape != shape or positions.numel() != T or cu_q.numel() != S + 1:
         raise KernelError("kv4_attention: queries, output, step and block table do not agree")
     kv_len = step.kv_len
     singles = step.decode_only

@@ -127,6 +127,8 @@ def test_steps_that_contradict_themselves(ops):
     for st, t in bad:
         with pytest.raises(ops.KernelError, match="say otherwise"):
             call(st, t)
+    with pytest.raises(ops.KernelError, match="do not agree"):           # no heads at all
+        ops.kv4_attention(q, torch.zeros_like(q), cache[:, :0].contiguous(), step([1, 1, 1]), table, 0, 0.1, nq, 0, d)
     other = torch.zeros(3, nkv, 1, 18 * 160, dtype=torch.uint8, device=DEV)
     with pytest.raises(ops.KernelError, match="indices"):
         ops.kv4_attention(torch.zeros(3, nq * 160, device=DEV), torch.zeros(3, nq * 160, device=DEV), other,
