@@ -13,9 +13,11 @@
 //            AND-OR in place makes an exact number of a code c + 8: 1024 + c + 8 from the last bits of the mantissa, 64 + c + 8 from the
 //            four before them.  The sums of a group of 32 elements start at minus what the offsets 1032 and 72 will add (a bare subtraction
 //            per operand would cost as much as making it), and are then scaled by the group's scale in 32 bits.  A bfloat16 query is exact
-//            in fp16 once its row is brought to [1, 2) by a power of two (what is 2^-16 of the row's largest loses bits that the
-//            sum does not hold).  32-bit queries go in as three bfloat16 pieces, and there the operands are c itself: the
-//            offsets' cancellation would cost 10 of the sum's 24 bits.
+//            in fp16 once its row is brought to [1, 2) by a power of two (what is 2^-16 of the row's largest loses bits, 2^-25
+//            of the largest at most: less than the sum holds unless that element's keys are 2^12 times the others').  The offsets'
+//            cancellation leaves the sum some 14 bits of the group's largest key times |q|, where the query's own rounding left 8.  32-bit
+//            queries go in as three bfloat16 pieces, and there the operands are c itself: the cancellation would cost 10 of the
+//            sum's 24 bits.
 //   softmax  32-bit, base 2.  The reference point of a row's exponentials is not raised before a score exceeds it by 4 (in powers of
 //            two), a vote of the warp: the sums stay far from overflow and the maximum's exchange between lanes is rare.
 //   values   O^T += V^T P^T in fp16: the codes of two neighbouring tokens lie in one word each, so AND-OR (1024 + c + 8) and a

@@ -521,8 +521,8 @@ void launch_wide(const WideArgs& a, cudaStream_t stream) {
 // 2^-24 of the tile's largest loses bits).  Queries, a row each, likewise: bfloat16's 8 bits are exact.
 // Blocks of kUnpackThreads: first a tile of a head each, then rows of queries, eight elements a lane.  A block asks for a tile's codes and
 // scales at once and finds the power of two from the latter; the chain of loads (length, page, codes) bounds it (2,048 keys of 8
-// heads of 128 and 1,024 tokens' queries: 5.5 us for 28 MB, most of it written; the attention behind it 46, as long as over a
-// bfloat16 cache).
+// heads of 128 and 1,024 tokens' queries: 7.5 us for 28 MB, most of it written; the attention behind it 44.8, as long as over
+// a bfloat16 cache).
 constexpr int kTile = 128, kUnpackThreads = 512;
 
 __device__ __forceinline__ uint32_t half_times(uint32_t code_pair, __half2 s) {        // (codes + 1024 as fp16 numbers) -> (code - 8) s

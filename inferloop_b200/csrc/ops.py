@@ -1776,8 +1776,12 @@ def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tens
 KV4_ROWS_HEADS = (32, 64, 96, 128, 256)     # head sizes of the kernel of few rows (others: the simple kernel)
 KV4_SHORT_ROWS = 128        # rows (tokens x query heads of a group) up to which a sequence shares a launch with single tokens
 # Blocks of 16 rows an SM up to which long portions read the codes as well; more of them unpack their keys and values once for the prefill
-# kernel.  One round of the device, where the kernel of rows takes its two CTAs an SM (behind 1,030 keys, 32 / 8 heads of 128, us, codes and
-# unpacked: 64 tokens 15.6 and 23.6, 128 tokens 22.4 and 26.8, 160 tokens 40.7 and 25.3, 1,024 tokens 173 and 55).
+# kernel.  One round of the device, where the kernel of rows takes its two CTAs an SM: both ways cost by the key, the unpacking once and the codes
+# once a round, so that the number of keys moves the border little (us, codes and unpacked, behind 0, 1,030, 8,192 and 32,000 keys; 32 / 8
+# heads of 128, 64 tokens (128 blocks): 8 and 11, 14 and 24, 58 and 104, 200 and 396; 160 tokens (320): 16 and 13, 37 and 26, 176 and 107, 622 and 397;
+# 64 / 8 heads, 64 tokens (256): 8 and 11, 20 and 25, 103 and 105, 373 and 395; 160 tokens (640): 23 and 13, 57 and 26, 267 and 108, 976 and 399;
+# 16 / 4 heads of 64, 160 tokens (160): 8 and 11, 26 and 22 (the one that the rule misses), 74 and 96, 231 and 334;
+# 512 tokens (512): 17 and 14, 33 and 27, 145 and 98, 504 and 339).
 KV4_ROWS_ROUNDS = 2
 KV4_BLOCKS = 65535          # (sequence, block of rows) pairs of a launch
 KV4_UNPACK_TOKENS = 1 << 17 # tokens whose keys and values are unpacked at a time: sequences in groups; one with more keys reads the codes

@@ -48,7 +48,8 @@ output (a mixer that runs beside another one), applied in 32-bit to what the out
 
 A cache in 4 bits (`BuildContext.kv_bits`): keys and values are quantised as the input stage writes them and attention reads the codes
 (csrc/kv4.cuh), for layers with keys and values of one head size (a multiple of 32), per-head norms or none, a plain softmax, with a
-window, aligned chunks or neither, sinks and gates.
+window, aligned chunks or neither, sinks and gates.  (No architecture here reaches its chunks and sinks: the one with chunks norms whole
+rows, the one with sinks reshapes its scores, and both are refused.  They are there for descriptions of a caller's own.)
 """
 from __future__ import annotations
 
