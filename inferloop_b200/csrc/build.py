@@ -50,6 +50,7 @@ MODULES: Dict[str, List[str]] = {
     "mlstm": [],
     "kv4": [],
     "attention_kv4": [],
+    "beam": [],
 }
 
 _LOCK = threading.Lock()

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+from dataclasses import dataclass
 from typing import Optional
 
 import torch
@@ -70,6 +71,7 @@ _SIGNATURES = {
     "ilb_attention_prefill_half": "pppppppp" + "iifiiiiiii" + "ppp",
     "ilb_kv4_attention_simple": "ppippppiiiifiiiiiipp",
     "ilb_kv4_attention_rows": "ppippppiiiifiiiiiiiipipqpqpp",
+    "ilb_beam_select": "piq" + "ppppp" + "iiii" + "ppp",
 }
 
 
@@ -106,6 +108,37 @@ def _call(module: str, fn: str, *args) -> None:
         raise KernelError(entry[1].ilb_last_error().decode())
     if begin is not None:
         timer.node_end(SCOPE, fn, begin)
+
+
+def _same_device(what: str, *tensors) -> None:
+    """Raise unless the tensors (None is passed over) lie on one device."""
+    where = None
+    for t in tensors:
+        if t is None:
+            continue
+        if where is None:
+            where = t.device
+        elif t.device != where:
+            raise KernelError(f"{what}: tensors on {where} and {t.device}")
+
+
+class _on_device:
+    """The tensors' device as the current one while a kernel is launched (a launch goes to the current device, whatever its stream); nothing is
+    asked of the driver where it is current already."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, index: int) -> None:
+        self.index = index
+
+    def __enter__(self) -> None:
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc) -> None:
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
 
 
 def _i(v) -> ctypes.c_int:
@@ -1230,6 +1263,284 @@ def sample_temperature(logits: torch.Tensor, temperature: torch.Tensor, uniform:
     _call("sampling", "ilb_sample_temperature", _ptr(logits), _ptr(temperature), _ptr(uniform), _ptr(top_k), _ptr(top_p),
           _ptr(min_p), _ptr(seen), _ptr(gen), _ptr(rep), _ptr(pres), _ptr(out), _ptr(bad), _i(rows), _i(vocab),
           _i(logits.stride(0)), _stream(logits))
+
+
+# --------------------------------------------------------------------------- beam search
+BEAM_MAX = 32              # beams of a request
+BEAM_MAX_BEST = 64         # candidates that a request's beams are asked for
+BEAM_MAX_ROWS = 1024       # rows (requests times beams) of a reordering
+BEAM_MAX_GROUPS = 8        # page groups of a reordering or of a step
+_BEAM_SCRATCH: dict = {}   # (device index, stream) -> the scratch of selections there
+_BEAM_PLANS: dict = {}     # sizes of a selection -> (8-byte words of keys, sums) that it needs
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, parents: torch.Tensor, tokens: torch.Tensor, out_scores: torch.Tensor,
+                bad: Optional[torch.Tensor] = None) -> None:
+    """The best continuations of every request's beams: row r * W + w of `logits` [R * W, vocab] (float32 or bfloat16, rows of any stride) belongs
+    to beam w of request r, whose score is scores[r, w] (float32).  parents, tokens and out_scores [R, k] get the k best (beam, token) by
+    score + log softmax(logits), best first; equal ones by the higher logit, then the lower beam, then the lower token.  A logit of -inf is
+    no candidate, nor is anything of a beam whose score is not finite; a row with NaN or +inf brings nothing and is flagged in
+    `bad` [R * W].  Where fewer than k are found the rest is beam -1, token -1, score -inf."""
+    _need(logits, "beam_select logits", contiguous=False)
+    for t, w, dt in ((scores, "scores", torch.float32), (parents, "parents", torch.int32), (tokens, "tokens", torch.int32),
+                     (out_scores, "new scores", torch.float32), (bad, "flags", torch.int32)):
+        _need(t, "beam_select " + w, dt)
+    if logits.dim() != 2 or scores.dim() != 2 or parents.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise KernelError("beam_select: logits must be [rows, vocabulary] with a row's elements side by side, scores [requests, beams], "
+                          "parents [requests, candidates]")
+    (rows, vocab), (R, W), k = logits.shape, scores.shape, parents.shape[1]
+    if rows != R * W or parents.shape[0] != R or tokens.shape != parents.shape or out_scores.shape != parents.shape \
+            or (bad is not None and bad.numel() != rows):
+        raise KernelError("beam_select: logits, scores and outputs do not agree")
+    if not (0 < W <= BEAM_MAX and 0 < k <= BEAM_MAX_BEST and vocab > 0):
+        raise KernelError(f"beam_select: up to {BEAM_MAX} beams and {BEAM_MAX_BEST} candidates, found {W} and {k} over a vocabulary of {vocab}")
+    _same_device("beam_select", logits, scores, parents, tokens, out_scores, bad)
+    if R == 0:
+        return
+    stride = logits.stride(0) if rows > 1 else vocab
+    if stride < vocab:
+        raise KernelError("beam_select: rows of logits overlap")
+    code, index, stream = _code(logits), logits.device.index, _raw_stream(logits)
+    key = (code, rows, W, vocab, k, index)
+    plan = _BEAM_PLANS.get(key)
+    if plan is None:
+        lib, found = load_module("beam"), (ctypes.c_longlong(), ctypes.c_longlong())
+        if lib.ilb_beam_select_plan(_i(code), _i(rows), _i(vocab), _i(k), *map(ctypes.byref, found)) != 0:
+            raise KernelError(lib.ilb_last_error().decode())
+        plan = _BEAM_PLANS[key] = (found[0].value, found[1].value)
+    need = 8 * (plan[0] + plan[1])
+    # (one scratch per device and stream; a graph that is being recorded gets its own, which its memory pool keeps)
+    held = None if _recording() else _BEAM_SCRATCH.get((index, stream))
+    if held is None or held.numel() < need:
+        held = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        if not _recording():
+            _BEAM_SCRATCH[index, stream] = held
+    at = held.data_ptr()
+    with _on_device(index):
+        _call("beam", "ilb_beam_select", logits.data_ptr(), code, stride, scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), out_scores.data_ptr(),
+              0 if bad is None else bad.data_ptr(), R, W, vocab, k, at, at + 8 * plan[0], stream)
+
+
+@dataclass
+class BeamTrack:
+    """What a search of R requests with W beams keeps on the device while it runs, and what it finds: `finished` hypotheses sorted best
+    first, each the beam that it came from (before its last step), that step and its last token.  `past_parents` and `past_tokens`
+    [steps, R, W] are the beams after every step, for walking a hypothesis back."""
+    scores: torch.Tensor               # [R, W] float32: the beams that go on
+    parents: torch.Tensor              # [R, W] int32: the beams that they continue (-1: none)
+    tokens: torch.Tensor               # [R, W] int32
+    past_parents: torch.Tensor         # [steps, R, W] int32
+    past_tokens: torch.Tensor          # [steps, R, W] int32
+    done_scores: torch.Tensor          # [R, W] float32: sum of log probabilities / generated tokens ^ length penalty
+    done_steps: torch.Tensor           # [R, W] int32
+    done_parents: torch.Tensor         # [R, W] int32
+    done_tokens: torch.Tensor          # [R, W] int32
+    done_count: torch.Tensor           # [R] int32
+    done: torch.Tensor                 # [R] int32: nothing that is still to come can better the finished ones
+
+    @staticmethod
+    def make(requests: int, beams: int, steps: int, device) -> "BeamTrack":
+        full = lambda *shape: torch.full(shape, -1, dtype=torch.int32, device=device)  # noqa: E731
+        low = lambda: torch.full((requests, beams), float("-inf"), device=device)  # noqa: E731
+        scores = low()
+        scores[:, 0] = 0.0                     # before the first step only the first beam is there
+        return BeamTrack(scores, full(requests, beams), full(requests, beams), full(steps, requests, beams), full(steps, requests, beams), low(),
+                         full(requests, beams), full(requests, beams), full(requests, beams),
+                         torch.zeros(requests, dtype=torch.int32, device=device), torch.zeros(requests, dtype=torch.int32, device=device))
+
+
+def beam_keep(parents: torch.Tensor, tokens: torch.Tensor, scores: torch.Tensor, stops: Optional[torch.Tensor], track: BeamTrack, step: int,
+              last: int, length_penalty: float = 1.0, early_stopping: bool = False) -> None:
+    """Candidates of `beam_select` [R, k] -> the beams that go on (`track.scores`, `parents`, `tokens` and row `step` of the past) and the finished
+    ones.  A candidate whose token is one of `stops` [n] int32 is finished if fewer than W candidates are above it; the first W others go on,
+    and with the step that makes the `last`-th token they are finished too.  A request is done when W have finished and (not `early_stopping`)
+    its best candidate's score over the length so far is not above the worst of them, or when no beam is left; what it finds
+    after that is not kept."""
+    _need(parents, "beam_keep parents", torch.int32); _need(tokens, "beam_keep tokens", torch.int32); _need(scores, "beam_keep scores", torch.float32)
+    _need(stops, "beam_keep stop tokens", torch.int32)
+    for name in ("scores", "parents", "tokens", "past_parents", "past_tokens", "done_scores", "done_steps", "done_parents", "done_tokens", "done_count",
+                 "done"):
+        _need(getattr(track, name), "beam_keep " + name, torch.float32 if name.endswith("scores") else torch.int32)
+    (R, W), (_, k) = track.scores.shape, parents.shape
+    steps = track.past_parents.shape[0]
+    if parents.shape[0] != R or tokens.shape != parents.shape or scores.shape != parents.shape or track.past_tokens.shape != track.past_parents.shape \
+            or tuple(track.past_parents.shape[1:]) != (R, W) or track.done_count.numel() != R or track.done.numel() != R \
+            or any(t.shape != track.scores.shape for t in (track.parents, track.tokens, track.done_scores, track.done_steps, track.done_parents,
+                                                           track.done_tokens)):
+        raise KernelError("beam_keep: candidates and what is kept do not agree")
+    if not (0 <= step < min(int(last), steps)) or not 0 < W <= BEAM_MAX or not 0 < k <= BEAM_MAX_BEST:
+        raise KernelError(f"beam_keep: step {step} of {last}, {steps} kept, {W} beams, {k} candidates")
+    _same_device("beam_keep", parents, tokens, scores, stops, track.scores, track.past_parents, track.done)
+    with _on_device(parents.device.index):
+        _call("beam", "ilb_beam_keep", _ptr(parents), _ptr(tokens), _ptr(scores), _i(k), _ptr(stops), _i(0 if stops is None else stops.numel()),
+              _ptr(track.parents), _ptr(track.tokens), _ptr(track.scores), _ptr(track.past_parents[step]), _ptr(track.past_tokens[step]), _i(step),
+              _i(last), _f(length_penalty), _i(1 if early_stopping else 0), _ptr(track.done_scores), _ptr(track.done_steps), _ptr(track.done_parents),
+              _ptr(track.done_tokens), _ptr(track.done_count), _ptr(track.done), _i(R), _i(W), _stream(parents))
+
+
+class BeamState:
+    """What moves with the beams, described once: `groups` = [(storages, page size, tokens a row stands for)], a storage being [..., pages, heads,
+    rows, row] (a group in 4 bits: uint8 [..., pages, heads, units of 16 rows, bytes]), and `slots`, tensors [slots, ...] of state
+    per sequence.  The tensors are kept, and moved where they lie."""
+
+    def __init__(self, groups, slots=(), device=None) -> None:
+        self.tensors = [x for storages, _, _ in groups for x in storages] + list(slots)
+        self.device = torch.device(device) if device is not None else self.tensors[0].device
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        records, first, at = [], [], 0
+        self.sizes = []
+        if len(groups) > BEAM_MAX_GROUPS:
+            raise KernelError(f"beam state: up to {BEAM_MAX_GROUPS} page groups, found {len(groups)}")
+        for g, (storages, page_size, stride) in enumerate(groups):
+            pages = None
+            if page_size <= 0 or stride <= 0 or not storages:
+                raise KernelError("beam state: a page group needs storage, a page size and a stride")
+            for x in storages:
+                self._check(x)
+                if x.dim() < 4 or x.shape[-2] == 0 or page_size % x.shape[-2] or (pages is not None and x.shape[-4] != pages):
+                    raise KernelError(f"beam state: {tuple(x.shape)} is not [..., pages, heads, rows, row] of pages of {page_size}")
+                pages = x.shape[-4]
+                unit, row = page_size // x.shape[-2], x.shape[-1] * x.element_size()
+                part, heads = x.shape[-2] * row, x.shape[-3]
+                outer = x.numel() // max(pages * heads * x.shape[-2] * x.shape[-1], 1)
+                if x.numel() == 0 or unit * row >= 1 << 31:
+                    raise KernelError(f"beam state: storage of shape {tuple(x.shape)} is empty or its rows too long")
+                records.append(struct.pack("@Pqqqqiiiiii", x.data_ptr(), pages * heads * part, heads * part, part, part, outer, heads, g, unit, row, 0))
+                first.append(at)
+                at += outer * heads
+            self.sizes.append((int(pages), int(page_size), int(stride)))
+        self.num_slots = None
+        for x in slots:
+            self._check(x)
+            if x.dim() < 1 or x.shape[0] == 0 or (self.num_slots is not None and x.shape[0] != self.num_slots):
+                raise KernelError(f"beam state: {tuple(x.shape)} is not [slots, ...]")
+            self.num_slots = x.shape[0]
+            size = x.numel() // x.shape[0] * x.element_size()
+            if size == 0:
+                continue
+            parts = -(-size // 4096)
+            records.append(struct.pack("@Pqqqqiiiiii", x.data_ptr(), 0, size, 4096, size, 1, parts, -1, 0, 0, 0))
+            first.append(at)
+            at += parts
+        if at >= 1 << 31:
+            raise KernelError("beam state: too many parts")
+        self.parts, self.n = at, len(records)
+        self.records = torch.frombuffer(bytearray(b"".join(records) or bytes(64)), dtype=torch.uint8).to(self.device)
+        self.first = torch.tensor(first or [0], dtype=torch.int32).to(self.device)
+
+    def _check(self, x: torch.Tensor) -> None:
+        _need(x, "beam state")
+        if x.device != self.device:
+            raise KernelError(f"beam state: a tensor is on {x.device}, the state on {self.device}")
+
+
+def beam_reorder(state: BeamState, parents: torch.Tensor, kv_len: torch.Tensor, tables, slots: Optional[torch.Tensor] = None) -> None:
+    """Beam w of request r continues beam parents[r, w] (int32 [R, W]; -1: none, its rows are worth nothing).  Row r * W + w of every group's block table
+    (`tables`, [R * W, blocks] int32 in the order of the state's groups) follows its parent's over the kv_len[r * W] tokens that the
+    request's beams all have, and `slots` [R * W] (the rows' state slots) with them.  Full pages are shared from there on.  A page that is not full is
+    a row's own, as its slot is: a parent's first child takes those over, every other child takes the ones of a beam without children, in the order
+    of both, and the parent's rows and state are copied there.  Before the call the last, partly filled pages of a request's rows and
+    their slots must be different ones."""
+    _need(parents, "beam_reorder parents", torch.int32); _need(kv_len, "beam_reorder lengths", torch.int32); _need(slots, "beam_reorder slots", torch.int32)
+    if parents.dim() != 2:
+        raise KernelError("beam_reorder: parents must be [requests, beams]")
+    R, W = parents.shape
+    rows = R * W
+    tables = list(tables)
+    if len(tables) != len(state.sizes):
+        raise KernelError(f"beam_reorder: {len(tables)} block tables for {len(state.sizes)} page groups")
+    for t in tables:
+        _need(t, "beam_reorder block table", torch.int32)
+        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] == 0:
+            raise KernelError(f"beam_reorder: a block table {tuple(t.shape)} for {rows} rows")
+    if kv_len.numel() != rows or (slots is not None and slots.numel() != rows) or (slots is None and state.num_slots is not None):
+        raise KernelError("beam_reorder: lengths or slots do not match the rows")
+    if not 0 < W <= BEAM_MAX or rows > BEAM_MAX_ROWS:
+        raise KernelError(f"beam_reorder: up to {BEAM_MAX} beams and {BEAM_MAX_ROWS} rows, found {W} and {rows}")
+    _same_device("beam_reorder", state.records, parents, kv_len, slots, *tables)
+    if R == 0:
+        return
+    n = len(tables)
+    where = (ctypes.c_longlong * max(n, 1))(*[t.data_ptr() for t in tables])
+    sizes = (ctypes.c_int * max(4 * n, 1))(*[x for t, (pages, page_size, stride) in zip(tables, state.sizes) for x in (t.shape[1], page_size, stride, pages)])
+    with _on_device(parents.device.index):
+        _call("beam", "ilb_beam_reorder", _ptr(parents), _ptr(kv_len), _ptr(slots), _ptr(state.records), _ptr(state.first), _i(state.n), _i(state.parts),
+              _i(state.num_slots or 0), where, sizes, _i(n), _i(R), _i(W), _i(_sm_count(parents.device)), _stream(parents))
+
+
+@dataclass
+class StepPages:
+    """Where a page group's new pages go and come from: block table [S, blocks], the pages that may be taken (`free`), how many of them are taken
+    already (`used` [1], all int32), and where the number goes (`used_out`, by default `used` itself)."""
+    table: torch.Tensor
+    free: torch.Tensor
+    used: torch.Tensor
+    page_size: int
+    stride: int = 1                    # tokens that a row of a page stands for
+    used_out: Optional[torch.Tensor] = None
+
+
+def step_build(new: torch.Tensor, cached: torch.Tensor, kv_len: torch.Tensor, positions: torch.Tensor, seq_of_token: torch.Tensor, cu_q: torch.Tensor,
+               pages, refused: torch.Tensor, slot_map: Optional[torch.Tensor] = None) -> None:
+    """A step's arrays on the device, from the tokens that each sequence brings and has (`new`, `cached` [S]): offsets cu_q [S + 1], lengths
+    kv_len [S] (may be `cached` itself), per token its position and sequence, and, group by group of `pages` (StepPages), the pages that the new
+    rows need, taken from the front of the free list in the order of sequences and blocks and entered in the block tables.  `slot_map` [T] int64: each
+    token's row among all rows of the first group's pages (page * page size + place; -1 where no page is held).  All or nothing: where
+    a length is negative or too long, tokens, pages or columns do not suffice, nothing is written but a bit in `refused` [1] (1 tokens, 2 pages,
+    4 columns, 8 lengths).  Entries behind the last token stay as they are."""
+    for t, w in ((new, "new tokens"), (cached, "cached tokens"), (kv_len, "lengths"), (positions, "positions"), (seq_of_token, "sequence indices"),
+                 (cu_q, "offsets"), (refused, "refusal flag")):
+        _need(t, "step_build " + w, torch.int32)
+    _need(slot_map, "step_build slot map", torch.int64)
+    S, T, pages = new.numel(), positions.numel(), list(pages)
+    if cached.numel() != S or kv_len.numel() != S or cu_q.numel() != S + 1 or seq_of_token.numel() != T or refused.numel() != 1 \
+            or (slot_map is not None and slot_map.numel() != T):
+        raise KernelError("step_build: arrays do not agree")
+    if len(pages) > BEAM_MAX_GROUPS or (slot_map is not None and (not pages or pages[0].stride != 1)):
+        raise KernelError(f"step_build: up to {BEAM_MAX_GROUPS} page groups, and a slot map of a group with a row per token")
+    _same_device("step_build", new, cached, kv_len, positions, seq_of_token, cu_q, refused, slot_map)
+    held = []
+    for g in pages:
+        out = g.used if g.used_out is None else g.used_out
+        for t, w in ((g.table, "block table"), (g.free, "free list"), (g.used, "pages taken"), (out, "pages taken")):
+            _need(t, "step_build " + w, torch.int32)
+        if g.table.dim() != 2 or g.table.shape[0] != S or (g.table.shape[1] == 0 and S) or g.used.numel() != 1 or out.numel() != 1 or g.page_size <= 0 \
+                or g.stride <= 0:
+            raise KernelError("step_build: a page group's arrays do not agree")
+        _same_device("step_build", new, g.table, g.free, g.used, out)
+        held += [g.table.data_ptr(), g.free.data_ptr(), g.used.data_ptr(), out.data_ptr(), g.table.shape[1], g.free.numel(), g.page_size, g.stride]
+    if S == 0:
+        return
+    with _on_device(new.device.index):
+        _call("beam", "ilb_step_build", _ptr(new), _ptr(cached), _ptr(kv_len), _ptr(positions), _ptr(seq_of_token), _ptr(cu_q), _ptr(slot_map),
+              _ptr(refused), _i(S), _i(T), (ctypes.c_longlong * max(len(held), 1))(*held), _i(len(pages)), _stream(new))
+
+
+def attention_beams(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, step, block_table: torch.Tensor, beams: int,
+                    window: int, scale: float, nq: int, nkv: int, d: int, sink: Optional[torch.Tensor] = None, workspace=None) -> None:
+    """`attention` of a step of single tokens whose rows are beams: rows r * beams .. (r + 1) * beams - 1 (the last request may have fewer) belong to one
+    request and share the pages that their block tables share.  q and out are [rows, nq * d] of the cache's type, float32 or bfloat16;
+    `window` and `sink` as in `attention`; a token that sees no key (its pages are not held) gets zeros.  `workspace`: where the scratch
+    of shared keys lies (None: scratch of the stream's own, or of the graph that is being recorded)."""
+    _need(q, "attention_beams q"); _need(out, "attention_beams out", q.dtype); _need(k_cache, "attention_beams keys", q.dtype)
+    _need(v_cache, "attention_beams values", q.dtype); _need(block_table, "attention_beams block table", torch.int32)
+    _need(step.positions, "attention_beams positions", torch.int32); _need(sink, "attention_beams sink", torch.float32)
+    rows = step.positions.numel()
+    if nq <= 0 or nkv <= 0 or nq % nkv or d <= 0 or q.dim() != 2 or tuple(q.shape) != (rows, nq * d) or out.shape != q.shape or block_table.dim() != 2 \
+            or block_table.shape[0] != rows or k_cache.dim() != 4 or k_cache.shape[1] != nkv or k_cache.shape[3] != d or v_cache.shape != k_cache.shape:
+        raise KernelError("attention_beams: queries, output, cache, block table and step do not agree")
+    if not 0 < beams <= BEAM_MAX:
+        raise KernelError(f"attention_beams: up to {BEAM_MAX} beams, found {beams}")
+    if sink is not None and sink.numel() != nq:
+        raise KernelError("attention_beams: one sink logit per query head")
+    _same_device("attention_beams", q, out, k_cache, v_cache, block_table, step.positions, sink)
+    if rows == 0:
+        return
+    if block_table.shape[1] == 0 or k_cache.shape[0] == 0 or k_cache.shape[2] == 0:
+        raise KernelError("attention_beams: the cache or the block table is empty")
+    with _on_device(q.device.index):
+        paged_attention_simple(q, out, k_cache, v_cache, step.positions, step.seq_of_token, block_table, window, scale, nq, nkv, d, d, sink)
 
 
 # --------------------------------------------------------------------------- tensor-core GEMM
