@@ -57,6 +57,7 @@ paged_attention_simple_kernel(const TQ* __restrict__ q, TQ* __restrict__ out,
   auto locate = [&](int j, const TC*& kr, const TC*& vr) {
     const bool pooled = j < n_pooled;
     const int row = pooled ? j : lo + j - n_pooled;
+    if (row / page_size >= max_blocks) return false;             // (behind the table)
     const int page = (pooled ? ptable : table)[row / page_size];
     if (page < 0 || page >= (pooled ? p_num_pages : num_pages)) return false;
     const size_t at = ((size_t)page * nkv + kvh) * page_size + row % page_size;

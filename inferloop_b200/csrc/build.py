@@ -51,6 +51,7 @@ MODULES: Dict[str, List[str]] = {
     "kv4": [],
     "attention_kv4": [],
     "beam": [],
+    "attention_beams": [],
 }
 
 _LOCK = threading.Lock()

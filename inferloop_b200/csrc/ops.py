@@ -71,6 +71,7 @@ _SIGNATURES = {
     "ilb_attention_prefill_half": "pppppppp" + "iifiiiiiii" + "ppp",
     "ilb_kv4_attention_simple": "ppippppiiiifiiiiiipp",
     "ilb_kv4_attention_rows": "ppippppiiiifiiiiiiiipipqpqpp",
+    "ilb_attention_beams": "ppi" + "pppp" + "iiii" + "f" + "iiiii" + "qq" + "pip",
     "ilb_beam_select": "piq" + "ppppp" + "iiii" + "ppp",
 }
 
@@ -1517,16 +1518,24 @@ def step_build(new: torch.Tensor, cached: torch.Tensor, kv_len: torch.Tensor, po
               _ptr(refused), _i(S), _i(T), (ctypes.c_longlong * max(len(held), 1))(*held), _i(len(pages)), _stream(new))
 
 
+def attention_beams_supported(dtype: torch.dtype, cache_dtype: torch.dtype, nq: int, nkv: int, d: int, page_size: int) -> bool:
+    """Geometries whose shared pages are read once; others go through the exact kernel, a row at a time."""
+    return (dtype == cache_dtype and dtype in (torch.bfloat16, torch.float32) and nkv > 0 and nq % nkv == 0 and d in (32, 64, 96, 128)
+            and page_size > 0 and page_size % 16 == 0 and nq // nkv <= (32 if dtype == torch.float32 else 64) and nkv * BEAM_MAX <= 65535)
+
+
 def attention_beams(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, step, block_table: torch.Tensor, beams: int,
-                    window: int, scale: float, nq: int, nkv: int, d: int, sink: Optional[torch.Tensor] = None, workspace=None) -> None:
+                    window: int, scale: float, nq: int, nkv: int, d: int, sink: Optional[torch.Tensor] = None) -> None:
     """`attention` of a step of single tokens whose rows are beams: rows r * beams .. (r + 1) * beams - 1 (the last request may have fewer) belong to one
-    request and share the pages that their block tables share.  q and out are [rows, nq * d] of the cache's type, float32 or bfloat16;
-    `window` and `sink` as in `attention`; a token that sees no key (its pages are not held) gets zeros.  `workspace`: where the scratch
-    of shared keys lies (None: scratch of the stream's own, or of the graph that is being recorded)."""
+    request, and a page that several of their block tables hold is read once for all of them.  q and out are [rows, nq * d] of the cache's
+    type, float32 or bfloat16; `window` and `sink` as in `attention`; a token that sees no key (its pages are not held) gets zeros.  A value meets only
+    the rows that see its key, whatever it is.  (`step`: its positions; sequence indices where the exact kernel takes the call; max_kv_len, if
+    it has one, only decides how the keys are split.)"""
     _need(q, "attention_beams q"); _need(out, "attention_beams out", q.dtype); _need(k_cache, "attention_beams keys", q.dtype)
     _need(v_cache, "attention_beams values", q.dtype); _need(block_table, "attention_beams block table", torch.int32)
-    _need(step.positions, "attention_beams positions", torch.int32); _need(sink, "attention_beams sink", torch.float32)
-    rows = step.positions.numel()
+    positions = step.positions
+    _need(positions, "attention_beams positions", torch.int32); _need(sink, "attention_beams sink", torch.float32)
+    rows, code = positions.numel(), _code(q)
     if nq <= 0 or nkv <= 0 or nq % nkv or d <= 0 or q.dim() != 2 or tuple(q.shape) != (rows, nq * d) or out.shape != q.shape or block_table.dim() != 2 \
             or block_table.shape[0] != rows or k_cache.dim() != 4 or k_cache.shape[1] != nkv or k_cache.shape[3] != d or v_cache.shape != k_cache.shape:
         raise KernelError("attention_beams: queries, output, cache, block table and step do not agree")
@@ -1534,13 +1543,26 @@ def attention_beams(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v
         raise KernelError(f"attention_beams: up to {BEAM_MAX} beams, found {beams}")
     if sink is not None and sink.numel() != nq:
         raise KernelError("attention_beams: one sink logit per query head")
-    _same_device("attention_beams", q, out, k_cache, v_cache, block_table, step.positions, sink)
+    _same_device("attention_beams", q, out, k_cache, v_cache, block_table, positions, sink)
     if rows == 0:
         return
-    if block_table.shape[1] == 0 or k_cache.shape[0] == 0 or k_cache.shape[2] == 0:
+    pages, _, page_size, _ = k_cache.shape
+    blocks, window, index = block_table.shape[1], window or 0, q.device.index
+    if blocks == 0 or pages == 0 or page_size == 0:
         raise KernelError("attention_beams: the cache or the block table is empty")
-    with _on_device(q.device.index):
-        paged_attention_simple(q, out, k_cache, v_cache, step.positions, step.seq_of_token, block_table, window, scale, nq, nkv, d, d, sink)
+    with _on_device(index):
+        if not attention_beams_supported(q.dtype, k_cache.dtype, nq, nkv, d, page_size) or (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+            _need(step.seq_of_token, "attention_beams sequence indices", torch.int32)
+            if step.seq_of_token.numel() != rows:
+                raise KernelError(f"attention_beams: {step.seq_of_token.numel()} sequence indices for {rows} rows")
+            paged_attention_simple(q, out, k_cache, v_cache, positions, step.seq_of_token, block_table, window, scale, nq, nkv, d, d, sink)
+            return
+        longest = min(getattr(step, "max_kv_len", None) or blocks * page_size, blocks * page_size)
+        if window:
+            longest = min(longest, abs(window) + page_size)
+        _call("attention_beams", "ilb_attention_beams", q.data_ptr(), out.data_ptr(), code, k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(),
+              block_table.data_ptr(), blocks, page_size, pages, window, scale, rows, beams, nq, nkv, d, nq * d, nq * d,
+              0 if sink is None else sink.data_ptr(), longest, _raw_stream(q))
 
 
 # --------------------------------------------------------------------------- tensor-core GEMM

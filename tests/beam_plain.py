@@ -153,7 +153,7 @@ def attention(q, k_cache, v_cache, positions, table, window, scale, nq, nkv, sin
         if pos < 0:
             continue
         lo = max(0, pos + 1 - window) if window > 0 else pos - pos % -window if window < 0 else 0
-        at = torch.arange(lo, min(pos + 1, table.shape[1] * page))
+        at = torch.arange(lo, max(lo, min(pos + 1, table.shape[1] * page)))
         ids = table[i, at // page].long()
         at, ids = at[(ids >= 0) & (ids < k_cache.shape[0])], ids[(ids >= 0) & (ids < k_cache.shape[0])]
         k, v = k_cache[ids, :, at % page], v_cache[ids, :, at % page]
