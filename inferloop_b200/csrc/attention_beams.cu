@@ -6,15 +6,18 @@
 //   units    a warp looks at a column of the block tables for each of its groups of lanes, a lane a beam: lanes with equal pages find each
 //            other (match), and the first of them enters (page, beams that hold it, column) in the list.  Nothing need be known about who descends
 //            from whom.  A unit is 16 keys of a page.
-//   split    a cluster of S = 1..16 CTAs shares a (request, kv head); column c goes to CTA c % S, so that the columns that beams do not share
-//            (the latest ones) are dealt out evenly.  S is the most that leaves all CTAs of the launch resident at once.
-//   loads    cp.async into a ring of tiles of four units, K and V, swizzled in 16-byte pieces for ldmatrix: a unit of a head is one
-//            contiguous block of memory.
-//   bfloat16 mma.sync m16n8k16: RB blocks of 16 rows a warp, WR warps side by side over the rows and 4 / WR over a tile's units; online softmax in
-//            32 bits.  Up to 64 rows a CTA; more rows are cut into chunks of whole beams.
+//   split    a cluster of S = 1..16 CTAs with GROUPS rings each shares a (request, kv head); column c goes to CTA c % S, there to the rings in
+//            turn, so that the columns that beams do not share (the latest ones) are dealt out evenly.  Every warp lists its ring's units for
+//            itself, and until the join nobody waits for another ring.  S is the most that leaves all CTAs of the launch resident at once.
+//   loads    cp.async into rings of units, K and V, swizzled in 16-byte pieces for ldmatrix: a unit of a head is one contiguous block of
+//            memory.  A ring belongs to a team of WR warps that share its keys and have 16 rows each; only they wait for one another.
+//   bfloat16 mma.sync m16n8k16.  A warp has a long chain of short steps for every unit (fragments, products, maxima, exponentials, products), so the next
+//            unit's scores are asked for before this one's softmax, and the running maximum is only raised, the sums rescaled, when a score
+//            exceeds it by 2^8: weights stay below 256, and most units need no exchange between lanes.  Sums in 32 bits.
 //   float32  fused multiply-adds, a lane a key for the scores and columns for the values; rows of the matrix dealt out to the warps.
-//   join     the warps' records (maximum, sum, O) meet in shared memory, the CTAs' in the cluster's: row i is added up by CTA i % S in the
-//            order of the ranks.  No scratch buffer, no tickets, no atomics.
+//   join     the rings' records (maximum, sum, O) of a row meet in shared memory; the CTA's record of row i is sent to CTA i % S of the cluster,
+//            which adds up its rows in the order of the ranks.  The cluster's first barrier is passed at the start and only waited for before the
+//            records are sent, the second stands between sending and adding.  No scratch buffer, no tickets, no atomics.
 // A value that is masked for a row is never multiplied into it, whatever it is: a unit that some row does not see in full is looked at for
 // infinities and NaN, and added by hand if it has any.
 #include <math.h>
@@ -27,15 +30,11 @@
 using namespace ilb;
 using std::max;
 using std::min;
-
 namespace {
 
 constexpr int kMaxBeams = 32;
 constexpr int kUnit = 16;              // keys
-constexpr int kTile = 4;               // units of a tile
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
-constexpr int kListOfWarp = 128;       // units that a warp lists at a time
+constexpr int kList = 64;              // pages that a ring lists at a time
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Params {
@@ -43,18 +42,21 @@ struct Params {
   const int* positions; const int* table; const float* sink;
   long long q_stride, out_stride;
   int rows, beams, beams_of_chunk, chunks, max_blocks, page_size, num_pages, window, nq, nkv, split;
-  float scale_log2;
+  float scale_log2;                    // bfloat16: of the absolute value; the sign is in the queries
+  uint32_t flip, keep;                 // of queries' bits: signs, all (a scale of 0: none)
 };
 
-struct Units {
-  int page[kWarps * kListOfWarp];
-  unsigned beams[kWarps * kListOfWarp];
-  int column[kWarps * kListOfWarp];
-  int count[kWarps], more[kWarps];
-};
+// A page that is listed: where its rows of the kv head lie (bytes from the cache's start), its first key, the beams that hold it.
+struct Listed { long long at; int key0; unsigned beams; };
 
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// 2^x with the hardware's instruction (2 steps of 32 bits); results below 2^-126 are 0.
+__device__ __forceinline__ float power_of_two(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -65,6 +67,9 @@ struct Job {
   int kvh, group;                      // kv head, query heads of it
   int lo_col, hi_col;                  // columns that some beam sees keys of
   int key_lo, key_hi;                  // keys that some beam sees
+  int all_lo, all_hi;                  // keys that every beam sees
+  unsigned all_beams;                  // their bits
+  int lo, hi;                          // the keys of the lane's beam
 };
 
 // The keys [lo, hi) that row `row` sees.
@@ -82,80 +87,101 @@ __device__ __forceinline__ Job make_job(const Params& p) {
   j.group = p.nq / p.nkv;
   const int first = chunk * p.beams_of_chunk;
   j.first_row = request * p.beams + first;
-  j.beams = min(min(p.beams_of_chunk, p.beams - first), p.rows - j.first_row);
-  if (j.beams < 0) j.beams = 0;
-  const int lane = threadIdx.x & 31;
-  int lo = 0x7fffffff, hi = 0;
-  if (lane < j.beams) {
-    keys_of(p, j.first_row + lane, &lo, &hi);
-    if (hi <= lo) lo = 0x7fffffff, hi = 0;
-  }
-  j.key_lo = __reduce_min_sync(0xffffffffu, lo);
-  j.key_hi = __reduce_max_sync(0xffffffffu, hi);
-  if (j.key_hi <= j.key_lo) j.key_lo = j.key_hi = 0;
-  j.lo_col = j.key_lo / p.page_size;
-  j.hi_col = (j.key_hi + p.page_size - 1) / p.page_size;
+  j.beams = max(min(min(p.beams_of_chunk, p.beams - first), p.rows - j.first_row), 0);
+  j.all_beams = j.beams == 32 ? 0xffffffffu : (1u << j.beams) - 1;
   return j;
 }
 
-// Lists the units of this CTA's next columns; `next` is the warp's turn (its `turn`-th group of columns), kept from call to call.  Returns how many
-// there are in all; the block is synchronised before and after.
-__device__ __forceinline__ int list_units(const Params& p, const Job& j, Units& u, int rank, int& next, bool* more) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// The keys that its beams see: found when their positions have come.
+__device__ __forceinline__ void find_keys(const Params& p, Job& j) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0x7fffffff, hi = 0, all_lo = 0, all_hi = 0x7fffffff;
+  j.lo = j.hi = 0;
+  if (lane < j.beams) {
+    keys_of(p, j.first_row + lane, &j.lo, &j.hi);
+    all_lo = j.lo;
+    all_hi = j.hi;
+    if (j.hi > j.lo) lo = j.lo, hi = j.hi;
+  }
+  j.key_lo = __reduce_min_sync(0xffffffffu, lo);
+  j.key_hi = __reduce_max_sync(0xffffffffu, hi);
+  j.all_lo = __reduce_max_sync(0xffffffffu, all_lo);
+  j.all_hi = __reduce_min_sync(0xffffffffu, all_hi);
+  if (j.key_hi <= j.key_lo) j.key_lo = j.key_hi = 0;
+  j.lo_col = j.key_lo / p.page_size;
+  j.hi_col = (j.key_hi + p.page_size - 1) / p.page_size;
+}
+
+// A CTA's columns: rank + split * i.  A turn of a warp looks at 32 / (beams, rounded up to a power of two) of them at once, a lane a beam; the
+// pages of the first turns are asked for ahead of everything else, should the first column be the table's (with a window it is not known yet).
+constexpr int kTurns = 4;              // turns whose pages are on their way at a time
+struct Turn { int columns, c, w, rank, next; int page[kTurns]; };
+__device__ __forceinline__ void ask_pages(const Params& p, const Job& j, Turn& x, int lo_col, int hi_col) {
+#pragma unroll
+  for (int n = 0; n < kTurns; ++n) {
+    const int column = lo_col + x.rank + p.split * ((x.next + n) * x.columns + x.c);
+    x.page[n] = -1;
+    if (x.w < j.beams && column < hi_col) x.page[n] = p.table[(long long)(j.first_row + x.w) * p.max_blocks + column];
+  }
+}
+__device__ __forceinline__ Turn first_turn(const Params& p, const Job& j, int rank) {
+  const int lane = threadIdx.x & 31;
   int wide = 1;
   while (wide < j.beams) wide *= 2;
-  const int columns = 32 / wide, c = lane / wide, w = lane - c * wide;
-  const int mine = (j.hi_col - j.lo_col - rank + p.split - 1) / p.split;       // columns of this CTA: lo_col + rank + split * i
-  const int turns = j.hi_col - j.lo_col > rank ? (mine + columns - 1) / columns : 0;
+  Turn x;
+  x.columns = 32 / wide;
+  x.c = lane / wide;
+  x.w = lane - x.c * wide;
+  x.rank = rank;
+  x.next = 0;
+  if (p.window == 0) ask_pages(p, j, x, 0, p.max_blocks);
+  return x;
+}
+__device__ __forceinline__ bool more_columns(const Params& p, const Job& j, const Turn& x) {
+  return j.lo_col + x.rank + p.split * (x.next * x.columns) < j.hi_col;
+}
+
+// Lists the pages of the CTA's next columns in `list` (the warp's own; all warps of a CTA make the same list) and returns how many there are.
+__device__ __forceinline__ int list_units(const Params& p, const Job& j, Turn& x, Listed* list, int row_bytes) {
+  const int lane = threadIdx.x & 31, wide = 32 / x.columns;
   int n = 0;
-  __syncthreads();
-  for (; next * kWarps + warp < turns && n + 32 <= kListOfWarp; ++next) {
-    const int i = (next * kWarps + warp) * columns + c, column = j.lo_col + rank + p.split * i;
-    int page = -1;
-    if (w < j.beams && i < mine) page = p.table[(long long)(j.first_row + w) * p.max_blocks + column];
-    const bool held = page >= 0 && page < p.num_pages;
-    const unsigned same = __match_any_sync(0xffffffffu, held ? (unsigned long long)c << 32 | (unsigned)page : ~0ull);
-    const bool first = held && lane == __ffs((int)same) - 1;
-    const unsigned listed = __ballot_sync(0xffffffffu, first);
-    if (first) {
-      const int at = warp * kListOfWarp + n + __popc(listed & ((1u << lane) - 1));
-      u.page[at] = page;
-      u.beams[at] = same >> (c * wide);
-      u.column[at] = column;
+  __syncwarp();
+  bool room = true;
+  while (room && more_columns(p, j, x)) {
+    if (x.next != 0 || p.window != 0) ask_pages(p, j, x, j.lo_col, j.hi_col);
+#pragma unroll
+    for (int turn = 0; turn < kTurns; ++turn) {
+      if (!room || !more_columns(p, j, x)) break;
+      const int column = j.lo_col + x.rank + p.split * (x.next * x.columns + x.c), page = x.page[turn];
+      const bool held = page >= 0 && page < p.num_pages && column < j.hi_col;
+      const unsigned same = __match_any_sync(0xffffffffu, held ? (unsigned long long)x.c << 32 | (unsigned)page : ~0ull);
+      const bool first = held && lane == __ffs((int)same) - 1;
+      const unsigned listed = __ballot_sync(0xffffffffu, first);
+      if (first)
+        list[n + __popc(listed & ((1u << lane) - 1))] =
+            Listed{((long long)page * p.nkv + j.kvh) * p.page_size * row_bytes, column * p.page_size, same >> (x.c * wide)};
+      n += __popc(listed);
+      ++x.next;
+      room = n + 32 <= kList;
     }
-    n += __popc(listed);
   }
-  if (lane == 0) { u.count[warp] = n; u.more[warp] = next * kWarps + warp < turns; }
-  __syncthreads();
-  int total = 0;
-  bool again = false;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) { total += u.count[i]; again |= u.more[i] != 0; }
-  *more = again;
-  return total;
+  __syncwarp();
+  return n;
 }
 
-// Where unit i of the lists is.
-__device__ __forceinline__ int unit_at(const Units& u, int i) {
-  int warp = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps - 1; ++w)
-    if (warp == w && i >= u.count[w]) { i -= u.count[w]; warp = w + 1; }
-  return warp * kListOfWarp + i;
-}
-
-// A unit of the running list: first key, beams, where its rows lie (row of the cache that its first key is), or no unit.
-struct Unit { int key0; unsigned beams; long long row; };
-__device__ __forceinline__ Unit unit_of(const Params& p, const Job& j, const Units& u, int i, int total, int parts) {
-  Unit x{0, 0, 0};
-  if (i < total * parts) {
-    const int which = i / parts, part = i - which * parts, at = unit_at(u, which);
-    const int key0 = u.column[at] * p.page_size + part * kUnit;
-    if (key0 < j.key_hi && key0 + kUnit > j.key_lo) {
-      x.key0 = key0;
-      x.beams = u.beams[at];
-      x.row = ((long long)u.page[at] * p.nkv + j.kvh) * p.page_size + part * kUnit;
-    }
+// Unit i of the list (page i / parts, its 16 keys i % parts); beams 0: there is no such unit, or nobody sees it.
+__device__ __forceinline__ Listed unit_of(const Job& j, const Listed* list, int i, int total, int parts, int unit_bytes) {
+  Listed x{0, 0, 0};
+  if (parts == 1) {
+    if (i < total) x = list[i];
+    return x;
+  }
+  const int which = i / parts, part = i - which * parts;
+  if (which < total) {
+    x = list[which];
+    x.at += (long long)part * unit_bytes;
+    x.key0 += part * kUnit;
+    if (x.key0 >= j.key_hi || x.key0 + kUnit <= j.key_lo) x.beams = 0;
   }
   return x;
 }
@@ -167,103 +193,145 @@ __device__ __forceinline__ uint32_t piece_at(uint32_t base, int row, int piece) 
   else return base + row * BYTES + ((piece ^ ((row >> 1) & 3)) << 4);
 }
 
-// The records of the CTA's rows (in its shared memory: O [ROWS][D], then (maximum, sum) [ROWS]) -> the rows' outputs; with a cluster, row i by CTA
-// i % split.  The maxima are in units of log2.
-template <typename T, int D, int ROWS>
-__device__ __forceinline__ void write_rows(const Params& p, const Job& j, const float* o, const float2* ml, int rank) {
+// ------------------------------------------------------------------ the join
+// Records of rows in shared memory, D + kPad floats apart (the pad spreads the rows over the banks).
+constexpr int kPad = 8;
+constexpr int kSpare = 4;              // rows of an inbox beyond the CTA's: the rows are rounded up to a multiple of the split
+template <int E>
+__device__ __forceinline__ void get(float (&x)[E], const float* from) {
+  if constexpr (E == 4) {
+    const float4 y = *reinterpret_cast<const float4*>(from);
+    x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = from[e];
+  }
+}
+
+// `records` [GROUPS][ROWS][D + kPad] with `ml` [GROUPS][ROWS] = (maximum in units of log2, sum), what each ring made of each row -> the rows' outputs.  `inbox`
+// [ROWS / split][split][D + kPad] with inbox_ml: what the CTAs of the cluster send about the rows that this one owns.
+template <typename T, int D, int ROWS, int GROUPS, int WARPS>
+__device__ __forceinline__ void join(const Params& p, const Job& j, const float* records, const float2* ml, float* inbox, float2* inbox_ml, int rank) {
+  constexpr int E = D / 32;            // columns E lane .. E lane + E - 1
   const int live = j.beams * j.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (p.split > 1) cluster_sync_all();
-  else __syncthreads();
-  for (int i = rank + p.split * warp; i < live; i += p.split * kWarps) {
+  auto finish = [&](int i, const float (&acc)[E], float top, float l) {
     const int w = i / j.group, head = j.kvh * j.group + i - w * j.group;
-    // lane c: the maximum and sum of CTA c
-    float mc = -INFINITY, lc = 0.f;
-    if (lane < p.split) {
-      const uint32_t at = smem_u32(&ml[i]);
-      mc = p.split > 1 ? ld_peer_f32(at, lane) : ml[i].x;
-      lc = p.split > 1 ? ld_peer_f32(at + 4, lane) : ml[i].y;
+    float scale = 1.f;
+    if (p.sink != nullptr) {
+      const float sink = p.sink[head] * kLog2e, all = fmaxf(top, sink), base = all == -INFINITY ? 0.f : all;
+      scale = exp2f(top - base);
+      l = l * scale + exp2f(sink - base);
     }
-    const float sink = p.sink != nullptr ? p.sink[head] * kLog2e : -INFINITY;
-    const float top = fmaxf(warp_max(mc), sink), base = top == -INFINITY ? 0.f : top;
-    const float f = mc == -INFINITY && lc == 0.f ? 0.f : exp2f(mc - base);     // (0: nothing seen there)
-    const float l = warp_sum(lc * f) + exp2f(sink - base);
-    float acc[D / 32];
-#pragma unroll
-    for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
-    const float* row = o + i * D + lane;
-    if (p.split == 1) {
-#pragma unroll
-      for (int e = 0; e < D / 32; ++e) acc[e] = __shfl_sync(0xffffffffu, f, 0) * row[e * 32];
-    } else {
-      for (int c = 0; c < p.split; c += 2) {
-        float x[2][D / 32];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < D / 32; ++e) x[h][e] = ld_peer_f32(smem_u32(row + e * 32), c + h);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float fc = __shfl_sync(0xffffffffu, f, c + h);
-#pragma unroll
-          for (int e = 0; e < D / 32; ++e) acc[e] += fc * x[h][e];
-        }
-      }
-    }
-    T* to = (T*)p.out + (long long)(j.first_row + w) * p.out_stride + (long long)head * D;
+    T* to = (T*)p.out + (long long)(j.first_row + w) * p.out_stride + (long long)head * D + E * lane;
     // a sum of 0 is a row that sees nothing
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) to[e * 32 + lane] = from_float<T>(l == 0.f ? 0.f : acc[e] / l);
+    for (int e = 0; e < E; ++e) to[e] = from_float<T>(l == 0.f ? 0.f : acc[e] * scale / l);
+  };
+  if (p.split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // every CTA of the cluster has begun
+  // (rows of a warp together: a chain of loads and exponentials as long as one row's)
+  constexpr int TOGETHER = ROWS / WARPS < 4 ? ROWS / WARPS : 4;
+  for (int i0 = warp; i0 < live; i0 += WARPS * TOGETHER) {
+    float acc[TOGETHER][E], top[TOGETHER], l[TOGETHER];
+#pragma unroll
+    for (int n = 0; n < TOGETHER; ++n) {
+      const int i = min(i0 + n * WARPS, ROWS - 1);
+      float f[GROUPS];
+      top[n] = -INFINITY;
+      l[n] = 0.f;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) top[n] = fmaxf(top[n], ml[g * ROWS + i].x);
+      const float base = top[n] == -INFINITY ? 0.f : top[n];
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        f[g] = exp2f(ml[g * ROWS + i].x - base);
+        l[n] += ml[g * ROWS + i].y * (top[n] == -INFINITY ? 1.f : f[g]);
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[n][e] = 0.f;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        float x[E];
+        get<E>(x, records + ((size_t)g * ROWS + i) * (D + kPad) + E * lane);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[n][e] += f[g] * x[e];
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < TOGETHER; ++n) {
+      const int i = i0 + n * WARPS;
+      if (i >= live) break;
+      if (p.split == 1) { finish(i, acc[n], top[n], l[n]); continue; }
+      const int turn = i / p.split, owner = i - turn * p.split, place = turn * p.split + rank;
+      const uint32_t to = peer_addr(smem_u32(inbox + (size_t)place * (D + kPad) + E * lane), owner);
+      if constexpr (E == 4) {
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(acc[n][0]), "f"(acc[n][1]), "f"(acc[n][2]), "f"(acc[n][3]) : "memory");
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4 * e), "f"(acc[n][e]) : "memory");
+      }
+      if (lane == 0)
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(peer_addr(smem_u32(inbox_ml + place), owner)), "f"(top[n]), "f"(l[n]) : "memory");
+    }
   }
-  if (p.split > 1) cluster_sync_all();                   // nobody leaves while a peer may still read its records
+  if (p.split == 1) return;
+  cluster_sync_all();
+  for (int n = warp, i = rank + p.split * warp; i < live; n += WARPS, i += p.split * WARPS) {
+    // lane c: the maximum and sum of CTA c
+    const float2 mine = lane < p.split ? inbox_ml[n * p.split + lane] : make_float2(-INFINITY, 0.f);
+    const float top = warp_max(mine.x), base = top == -INFINITY ? 0.f : top;
+    const float f = exp2f(mine.x - base), l = warp_sum(top == -INFINITY ? mine.y : mine.y * f);
+    float acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < p.split; c += 2) {               // (two records on their way at a time)
+      float x[2][E];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) get<E>(x[h], inbox + (size_t)(n * p.split + min(c + h, p.split - 1)) * (D + kPad) + E * lane);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (c + h >= p.split) break;
+        const float fc = __shfl_sync(0xffffffffu, f, c + h);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += fc * x[h][e];
+      }
+    }
+    finish(i, acc, top, l);
+  }
 }
 
 // ------------------------------------------------------------------ bfloat16
-template <int D>
-constexpr int kTileBf16 = kTile * kUnit * D * 2 * 2;
+// WR warps of RB blocks of 16 rows a ring, GROUPS rings of STAGES units.
+template <int D, int RB, int WR, int GROUPS, int STAGES>
+struct Shape {
+  static constexpr int BYTES = D * 2, PIECES = BYTES / 16, ROWS = 16 * RB * WR, WARPS = GROUPS * WR, THREADS = 32 * WARPS;
+  static constexpr int UNIT_BYTES = kUnit * BYTES, STAGE_BYTES = 2 * UNIT_BYTES, RING_BYTES = STAGES * STAGE_BYTES;
+  static constexpr int RECORDS = GROUPS * ROWS * (D + kPad) * 4, INBOX = (ROWS + kSpare) * (D + kPad) * 4;
+  static constexpr int RINGS = GROUPS * RING_BYTES > RECORDS ? GROUPS * RING_BYTES : RECORDS, SMEM = RINGS + INBOX + 256;
+};
+constexpr float kHeadroom = 8.f;       // log2 of what a weight may be
 
-template <int D, int RB, int WR, int STAGES>
-constexpr size_t smem_bf16() {
-  constexpr int ROWS = 16 * RB * WR, WK = kWarps / WR;
-  constexpr size_t ring = (size_t)STAGES * kTileBf16<D>, join = (size_t)WK * ROWS * D * 4;
-  return (ring > join ? ring : join) + 128;
-}
-
-template <int D, int RB, int WR, int STAGES>
-__global__ void __launch_bounds__(kThreads)
+template <int D, int RB, int WR, int GROUPS, int STAGES, int CTAS>
+__global__ void __launch_bounds__(32 * WR * GROUPS, CTAS)
 attention_beams_kernel(Params p) {
-  constexpr int BYTES = D * 2, PIECES = BYTES / 16, ROWS = 16 * RB * WR, WK = kWarps / WR;
-  constexpr uint32_t kUnitBytes = kUnit * BYTES, kTileBytes = kTileBf16<D>;
+  using S = Shape<D, RB, WR, GROUPS, STAGES>;
+  constexpr int BYTES = S::BYTES, PIECES = S::PIECES, ROWS = S::ROWS, TEAM = 32 * WR;
   extern __shared__ char s_raw[];
-  __shared__ Units s_units;
-  __shared__ float2 s_ml[WK * ROWS];
+  __shared__ Listed s_lists[S::WARPS][kList];
+  __shared__ float2 s_ml[GROUPS * ROWS], s_inbox_ml[ROWS + kSpare];
+  if (p.split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   pdl_launch_dependents();
   pdl_wait();
-  char* ring = (char*)(((uintptr_t)s_raw + 127) & ~(uintptr_t)127);
-  const uint32_t ring_at = smem_u32(ring);
+  char* ring = (char*)(((uintptr_t)s_raw + 255) & ~(uintptr_t)255);
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rank = p.split > 1 ? (int)cluster_rank() : 0;
-  const int rg = warp / WK, kg = warp - rg * WK, g = lane >> 2, tq = lane & 3;
-  const Job j = make_job(p);
+  // (a ring's warps take their rows in another order than its neighbour's: the fewer last ones fall to schedulers in turn)
+  const int group = warp / WR, rg = (warp - group * WR + group) % WR, in_team = rg * 32 + lane, g = lane >> 2, tq = lane & 3;
+  const uint32_t ring_at = smem_u32(ring) + group * S::RING_BYTES;
+  Job j = make_job(p);
+  Turn turn = first_turn(p, j, rank);
+  Listed* list = s_lists[warp];
   const int live = j.beams * j.group, parts = p.page_size / kUnit;
-  // the warp's rows: queries as fragments, beams and keys that they see
-  uint32_t q[RB][D / 16][4];
-  int lo[RB][2], hi[RB][2], beam[RB][2];
-#pragma unroll
-  for (int b = 0; b < RB; ++b)
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int i = (rg * RB + b) * 16 + g + 8 * r;
-      const bool there = i < live;
-      const int w = there ? i / j.group : 0;
-      beam[b][r] = there ? w : -1;
-      lo[b][r] = hi[b][r] = 0;
-      if (there) keys_of(p, j.first_row + w, &lo[b][r], &hi[b][r]);
-      const __nv_bfloat16* row = (const __nv_bfloat16*)p.q + (long long)(j.first_row + w) * p.q_stride + (long long)(j.kvh * j.group + i - w * j.group) * D;
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        q[b][kk][r] = there ? *reinterpret_cast<const uint32_t*>(row + kk * 16 + 2 * tq) : 0u;
-        q[b][kk][2 + r] = there ? *reinterpret_cast<const uint32_t*>(row + kk * 16 + 2 * tq + 8) : 0u;
-      }
-    }
+  find_keys(p, j);
   float o[RB][D / 8][4], m[RB][2], l[RB][2];
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
@@ -274,182 +342,253 @@ attention_beams_kernel(Params p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[b][i][e] = 0.f;
   }
+  auto meet = [&] {                                      // the warps of a ring
+    if constexpr (WR == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(TEAM) : "memory");
+  };
+  // where a lane's pieces lie in a unit (a stage starts on a multiple of 256 bytes, so that the swizzle is an exclusive or of the address): those that
+  // it copies, keys' and values' fragments
+  constexpr int CHUNKS = D / 16;       // of 32 pieces of 16 bytes
+  const uint32_t copy_at = piece_at<BYTES>(0u, (rg * 32 + lane) / PIECES, (rg * 32 + lane) % PIECES), key_at = piece_at<BYTES>(0u, lane & 7, lane >> 3);
+  const uint32_t value_at = S::UNIT_BYTES + piece_at<BYTES>(0u, (lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
+  uint32_t q[RB][D / 16][4];
+  int lo[RB][2], hi[RB][2];
+  unsigned beam[RB][2];
+  bool asked = false;
+  const bool idle = rg * RB * 16 >= live;                // none of the warp's rows is there: it only helps to copy
 
-  int next = 0;
-  bool more = true;
-  while (more) {
-    const int total = list_units(p, j, s_units, rank, next, &more);
-    const int tiles = (total * parts + kTile - 1) / kTile;
-    auto load = [&](int tile) {                          // warp w brings unit w of the tile
-      if (tile < tiles) {
-        const Unit u = unit_of(p, j, s_units, tile * kTile + warp, total, parts);
-        if (u.beams != 0) {
-          const uint32_t ks = ring_at + (tile % STAGES) * kTileBytes + warp * kUnitBytes, vs = ks + kTile * kUnitBytes;
-          const char* k = (const char*)p.k + u.row * BYTES;
-          const char* v = (const char*)p.v + u.row * BYTES;
+  while (more_columns(p, j, turn)) {
+    const int total = list_units(p, j, turn, list, BYTES), steps = (total * parts + GROUPS - 1) / GROUPS;
+    auto unit = [&](int step) { return unit_of(j, list, step * GROUPS + group, total, parts, S::UNIT_BYTES); };
+    auto load = [&](int step, int stage) {
+      const Listed u = unit(step);
+      if (u.beams != 0) {
+        // 32 pieces at a time, dealt out to the warps
+        const uint32_t ks = ring_at + stage * S::STAGE_BYTES + copy_at;
+        const char* k = (const char*)p.k + u.at + in_team * 16;
+        const char* v = (const char*)p.v + u.at + in_team * 16;
 #pragma unroll
-          for (int i = 0; i < kUnit * PIECES / 32; ++i) {
-            const int c = i * 32 + lane, row = c / PIECES, piece = c - row * PIECES;
-            cp_async_16(piece_at<BYTES>(ks, row, piece), k + c * 16);
-            cp_async_16(piece_at<BYTES>(vs, row, piece), v + c * 16);
-          }
+        for (int i = 0; i < (CHUNKS + WR - 1) / WR; ++i) {
+          if (CHUNKS % WR != 0 && i * WR + rg >= CHUNKS) break;
+          uint32_t to;
+          if constexpr (D == 96) to = ring_at + stage * S::STAGE_BYTES + piece_at<BYTES>(0u, ((i * WR + rg) * 32 + lane) / PIECES, ((i * WR + rg) * 32 + lane) % PIECES);
+          else to = (ks ^ (D == 128 ? ((i * WR) & 3) << 5 : D == 64 ? ((i * WR) & 1) << 6 : 0)) + i * WR * 512;
+          cp_async_16(to, k + i * WR * 512);
+          cp_async_16(to + S::UNIT_BYTES, v + i * WR * 512);
         }
       }
       cp_async_commit();
     };
+    auto scores = [&](float (&s)[RB][2][4], uint32_t ks) {
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) load(s);
-    for (int tile = 0; tile < tiles; ++tile) {
-      cp_async_wait<STAGES - 2>();
-      __syncthreads();
-      load(tile + STAGES - 1);
+      for (int b = 0; b < RB; ++b)
 #pragma unroll
-      for (int n = 0; n < kTile / WK; ++n) {
-        const int in_tile = n * WK + kg;
-        const Unit u = unit_of(p, j, s_units, tile * kTile + in_tile, total, parts);
-        if (u.beams == 0) continue;
-        const uint32_t ks = ring_at + (tile % STAGES) * kTileBytes + in_tile * kUnitBytes, vs = ks + kTile * kUnitBytes;
-        bool sees[RB], whole[RB];                        // some row of the block sees some of the unit; every row sees all of it
+        for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
-        for (int b = 0; b < RB; ++b) {
-          bool any = false, all = true;
+          for (int e = 0; e < 4; ++e) s[b][nb][e] = 0.f;
+      ks += key_at;
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            if (beam[b][r] < 0) continue;
-            const bool held = (u.beams >> beam[b][r]) & 1;
-            any |= held && u.key0 < hi[b][r] && u.key0 + kUnit > lo[b][r];
-            all &= held && u.key0 >= lo[b][r] && u.key0 + kUnit <= hi[b][r];
+      for (int kk = 0; kk < D / 16; kk += 2) {
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) {
+          uint32_t r0, r1, r2, r3;
+          ldmatrix_x4((BYTES % 128 == 0 ? ks ^ (kk * 32) : ks + kk * 32) + nb * 8 * BYTES, r0, r1, r2, r3);
+#pragma unroll
+          for (int b = 0; b < RB; ++b) {
+            mma_16816(s[b][nb], q[b][kk], r0, r1);
+            mma_16816(s[b][nb], q[b][kk + 1], r2, r3);
           }
-          sees[b] = __any_sync(0xffffffffu, any);
-          whole[b] = __all_sync(0xffffffffu, all);
         }
-        bool any_sees = false;
+      }
+    };
+    auto values = [&](int nd, uint32_t vs, uint32_t (&v)[4]) {
+      ldmatrix_x4_trans(BYTES % 128 == 0 ? vs ^ (nd * 32) : (vs ^ ((nd & 1) * 32)) + (nd >> 1) * 64, v[0], v[1], v[2], v[3]);
+    };
+    meet();                                              // (the ring is free: the last list's steps are done)
 #pragma unroll
-        for (int b = 0; b < RB; ++b) any_sees |= sees[b];
-        if (!any_sees) continue;
-        float s[RB][2][4];
+    for (int s = 0; s < STAGES - 1; ++s) load(s, s);
+    if (!asked) {
+      // the warp's rows, while the first keys are on their way: queries as fragments, beams (as bits) and keys that they see
+      asked = true;
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          // (a row that is not there reads the last one's queries: what becomes of it is nobody's)
+          const int i = (rg * RB + b) * 16 + g + 8 * r, at = min(i, live - 1), w = at / j.group;
+          const uint32_t* row = reinterpret_cast<const uint32_t*>((const __nv_bfloat16*)p.q + (long long)(j.first_row + w) * p.q_stride
+                                                                  + (long long)(j.kvh * j.group + at - w * j.group) * D) + tq;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            q[b][kk][r] = row[kk * 8];
+            q[b][kk][2 + r] = row[kk * 8 + 4];
+          }
+          beam[b][r] = i < live ? 1u << w : 0u;
+          lo[b][r] = __shfl_sync(0xffffffffu, j.lo, w);
+          hi[b][r] = __shfl_sync(0xffffffffu, j.hi, w);
+        }
+      if (p.flip != 0u || p.keep != 0xffffffffu) {
 #pragma unroll
         for (int b = 0; b < RB; ++b)
 #pragma unroll
-          for (int nb = 0; nb < 2; ++nb)
+          for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[b][nb][e] = 0.f;
+            for (int e = 0; e < 4; ++e) q[b][kk][e] = (q[b][kk][e] & p.keep) ^ p.flip;
+      }
+    }
+    // with one block of rows the next unit's scores are asked for a step ahead, with two each covers the other's waits
+    constexpr int AHEAD = RB == 1 ? 1 : 0;
+    Listed u{0, 0, 0};
+    float s[RB][2][4];
+    if constexpr (AHEAD) {
+      cp_async_wait<STAGES - 2>();
+      meet();
+      u = unit(0);
+      scores(s, ring_at);                                // (of a unit that is not there: nothing is made of them)
+    }
+    int stage = 0;
+    for (int step = 0; step < steps; ++step) {
+      cp_async_wait<STAGES - 2 - AHEAD>();
+      meet();
+      const int before = stage == 0 ? STAGES - 1 : stage - 1, after = stage + 1 == STAGES ? 0 : stage + 1;
+      load(step + STAGES - 1, before);
+      Listed u_next{0, 0, 0};
+      float s_next[RB][2][4];
+      if constexpr (AHEAD) {
+        u_next = unit(step + 1);
+        if (u_next.beams != 0 && !idle) scores(s_next, ring_at + after * S::STAGE_BYTES);
+      } else {
+        u = unit(step);
+      }
+      const uint32_t vs = ring_at + stage * S::STAGE_BYTES + value_at;
+      bool sees = !idle, whole = true;                   // some row of the warp sees some of the unit; every row sees all of it
+      if (u.beams != j.all_beams || u.key0 < j.all_lo || u.key0 + kUnit > j.all_hi) {
+        bool any = false;
+        whole = false;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; kk += 2) {
+        for (int b = 0; b < RB; ++b)
 #pragma unroll
-          for (int nb = 0; nb < 2; ++nb) {
-            uint32_t r0, r1, r2, r3;
-            ldmatrix_x4(piece_at<BYTES>(ks, nb * 8 + (lane & 7), kk * 2 + (lane >> 3)), r0, r1, r2, r3);
+          for (int r = 0; r < 2; ++r) any |= (u.beams & beam[b][r]) != 0 && u.key0 < hi[b][r] && u.key0 + kUnit > lo[b][r];
+        sees = __any_sync(0xffffffffu, any);
+      }
+      if (sees) {
+        if constexpr (!AHEAD) scores(s, ring_at + stage * S::STAGE_BYTES);
+        bool odd = false;                                // an infinity or NaN among the values, and a row that must not meet it
+        if (!whole) {
+          uint32_t zero = 0u;
 #pragma unroll
-            for (int b = 0; b < RB; ++b) {
-              mma_16816(s[b][nb], q[b][kk], r0, r1);
-              mma_16816(s[b][nb], q[b][kk + 1], r2, r3);
-            }
+          for (int nd = 0; nd < D / 16; ++nd) {
+            uint32_t v[4];
+            values(nd, vs, v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(zero) : "r"(v[e]), "r"(0u));
           }
+          odd = __any_sync(0xffffffffu, zero != 0u);
+#pragma unroll
+          for (int b = 0; b < RB; ++b)
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int key = u.key0 + nb * 8 + 2 * tq + (e & 1), r = e >> 1;
+                if (!((u.beams & beam[b][r]) != 0 && key >= lo[b][r] && key < hi[b][r])) s[b][nb][e] = -INFINITY;
+              }
+        }
+        float mx[RB][2];
+        bool rises = false;
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            mx[b][r] = fmaxf(fmaxf(s[b][0][2 * r], s[b][0][2 * r + 1]), fmaxf(s[b][1][2 * r], s[b][1][2 * r + 1]));
+            rises |= mx[b][r] * p.scale_log2 > m[b][r] + kHeadroom;
+          }
+        if (__any_sync(0xffffffffu, rises)) {
+#pragma unroll
+          for (int b = 0; b < RB; ++b)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              float x = mx[b][r];
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+              const float m_new = fmaxf(m[b][r], x == -INFINITY ? -INFINITY : x * p.scale_log2);
+              const float corr = m_new == -INFINITY ? 1.f : power_of_two(m[b][r] - m_new);
+              m[b][r] = m_new;
+              l[b][r] *= corr;
+#pragma unroll
+              for (int i = 0; i < D / 8; ++i) { o[b][i][2 * r] *= corr; o[b][i][2 * r + 1] *= corr; }
+            }
         }
         uint32_t a[RB][4];
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
-          float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-          for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int key = u.key0 + nb * 8 + 2 * tq + (e & 1), r = e >> 1;
-              const bool ok = whole[b] || (beam[b][r] >= 0 && ((u.beams >> beam[b][r]) & 1) && key >= lo[b][r] && key < hi[b][r]);
-              s[b][nb][e] = ok ? s[b][nb][e] * p.scale_log2 : -INFINITY;
-              mx[r] = fmaxf(mx[r], s[b][nb][e]);
-            }
-          float corr[2], base[2], sum[2] = {0.f, 0.f};
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-            const float m_new = fmaxf(m[b][r], mx[r]);
-            base[r] = m_new == -INFINITY ? 0.f : m_new;
-            corr[r] = exp2f(m[b][r] - base[r]);
-            m[b][r] = m_new;
-          }
+            const float base = m[b][r] == -INFINITY ? 0.f : m[b][r];
 #pragma unroll
-          for (int nb = 0; nb < 2; ++nb)
+            for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              s[b][nb][e] = exp2f(s[b][nb][e] - base[e >> 1]);
-              sum[e >> 1] += s[b][nb][e];
-            }
-#pragma unroll
-          for (int r = 0; r < 2; ++r) l[b][r] = l[b][r] * corr[r] + sum[r];
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            o[b][i][0] *= corr[0]; o[b][i][1] *= corr[0];
-            o[b][i][2] *= corr[1]; o[b][i][3] *= corr[1];
+              for (int e = 2 * r; e < 2 * r + 2; ++e) s[b][nb][e] = power_of_two(fmaf(s[b][nb][e], p.scale_log2, -base));
+            l[b][r] += (s[b][0][2 * r] + s[b][0][2 * r + 1]) + (s[b][1][2 * r] + s[b][1][2 * r + 1]);
           }
           a[b][0] = pack_bf16(s[b][0][0], s[b][0][1]);
           a[b][1] = pack_bf16(s[b][0][2], s[b][0][3]);
           a[b][2] = pack_bf16(s[b][1][0], s[b][1][1]);
           a[b][3] = pack_bf16(s[b][1][2], s[b][1][3]);
         }
-        bool all_whole = true;
-#pragma unroll
-        for (int b = 0; b < RB; ++b) all_whole &= whole[b];
-        bool odd = false;                                // an infinity or NaN among the values, and a row that must not meet it
-        if (!all_whole) {
-#pragma unroll
-          for (int i = 0; i < kUnit * PIECES / 32; ++i) {
-            const int c = i * 32 + lane, row = c / PIECES;
-            uint32_t x[4];
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                         : "r"(piece_at<BYTES>(vs, row, c - row * PIECES)));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) odd |= (x[e] & 0x7f80u) == 0x7f80u || (x[e] & 0x7f800000u) == 0x7f800000u;
-          }
-          odd = __any_sync(0xffffffffu, odd);
-        }
         if (!odd) {
 #pragma unroll
           for (int nd = 0; nd < D / 16; ++nd) {
-            uint32_t r0, r1, r2, r3;
-            ldmatrix_x4_trans(piece_at<BYTES>(vs, (lane & 7) + ((lane >> 3) & 1) * 8, nd * 2 + (lane >> 4)), r0, r1, r2, r3);
+            uint32_t v[4];
+            values(nd, vs, v);
 #pragma unroll
             for (int b = 0; b < RB; ++b) {
-              if (!sees[b]) continue;
-              mma_16816(o[b][2 * nd], a[b], r0, r1);
-              mma_16816(o[b][2 * nd + 1], a[b], r2, r3);
+              mma_16816(o[b][2 * nd], a[b], v[0], v[1]);
+              mma_16816(o[b][2 * nd + 1], a[b], v[2], v[3]);
             }
           }
         } else {
 #pragma unroll 1
           for (int key = 0; key < kUnit; ++key) {
-            const int from = (lane & ~3) | ((key & 7) >> 1);
+            const int from = (lane & ~3) | ((key & 7) >> 1), at = u.key0 + key;
 #pragma unroll
             for (int b = 0; b < RB; ++b) {
               // (the fragment's words: rows g and g + 8 of keys 0 .. 7, then of keys 8 .. 15)
-              const uint32_t w0 = __shfl_sync(0xffffffffu, key < 8 ? a[b][0] : a[b][2], from), w1 = __shfl_sync(0xffffffffu, key < 8 ? a[b][1] : a[b][3], from);
+              const uint32_t w0 = __shfl_sync(0xffffffffu, key < 8 ? a[b][0] : a[b][2], from);
+              const uint32_t w1 = __shfl_sync(0xffffffffu, key < 8 ? a[b][1] : a[b][3], from);
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
-                const int at = u.key0 + key;
-                if (beam[b][r] < 0 || !((u.beams >> beam[b][r]) & 1) || at < lo[b][r] || at >= hi[b][r]) continue;
+                if ((u.beams & beam[b][r]) == 0 || at < lo[b][r] || at >= hi[b][r]) continue;
                 const uint32_t word = r ? w1 : w0;
                 const float weight = __uint_as_float((key & 1) ? word & 0xffff0000u : word << 16);
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) {
-                  uint32_t x;
-                  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(piece_at<BYTES>(vs, key, i) + tq * 4));
-                  o[b][i][2 * r] += weight * __uint_as_float(x << 16);
-                  o[b][i][2 * r + 1] += weight * __uint_as_float(x & 0xffff0000u);
+                  uint32_t y;
+                  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(y) : "r"(piece_at<BYTES>(vs - value_at + S::UNIT_BYTES, key, i) + tq * 4));
+                  o[b][i][2 * r] += weight * __uint_as_float(y << 16);
+                  o[b][i][2 * r + 1] += weight * __uint_as_float(y & 0xffff0000u);
                 }
               }
             }
           }
         }
       }
+      if constexpr (AHEAD) {
+        u = u_next;
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+          for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[b][nb][e] = s_next[b][nb][e];
+      }
+      stage = after;
     }
     cp_async_wait<0>();
   }
 
-  // the warps that share rows: one record a row
   __syncthreads();
-  float* records = (float*)ring;                         // [WK][ROWS][D]
+  float* records = (float*)ring;                         // [GROUPS][ROWS][D + kPad]
 #pragma unroll
   for (int b = 0; b < RB; ++b)
 #pragma unroll
@@ -458,49 +597,27 @@ attention_beams_kernel(Params p) {
       float sum = l[b][r];
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      if (tq == 0) s_ml[kg * ROWS + i] = make_float2(m[b][r], sum);
+      if (tq == 0) s_ml[group * ROWS + i] = make_float2(m[b][r], sum);
 #pragma unroll
       for (int d = 0; d < D / 8; ++d)
-        *reinterpret_cast<float2*>(records + ((size_t)kg * ROWS + i) * D + d * 8 + 2 * tq) = make_float2(o[b][d][2 * r], o[b][d][2 * r + 1]);
+        *reinterpret_cast<float2*>(records + ((size_t)group * ROWS + i) * (D + kPad) + d * 8 + 2 * tq) = make_float2(o[b][d][2 * r], o[b][d][2 * r + 1]);
     }
   __syncthreads();
-  if constexpr (WK > 1) {
-    for (int x = t; x < ROWS * D / 4; x += kThreads) {
-      const int i = x / (D / 4), c = x - i * (D / 4);
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < WK; ++w) top = fmaxf(top, s_ml[w * ROWS + i].x);
-      const float base = top == -INFINITY ? 0.f : top;
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < WK; ++w) {
-        const float f = exp2f(s_ml[w * ROWS + i].x - base);
-        const float4 y = *reinterpret_cast<const float4*>(records + ((size_t)w * ROWS + i) * D + c * 4);
-        sum.x += f * y.x; sum.y += f * y.y; sum.z += f * y.z; sum.w += f * y.w;
-      }
-      *reinterpret_cast<float4*>(records + (size_t)i * D + c * 4) = sum;
-    }
-    __syncthreads();
-    if (t < ROWS) {
-      float top = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < WK; ++w) top = fmaxf(top, s_ml[w * ROWS + t].x);
-      const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-      for (int w = 0; w < WK; ++w) sum += s_ml[w * ROWS + t].y * exp2f(s_ml[w * ROWS + t].x - base);
-      s_ml[t] = make_float2(top, sum);
-    }
-  }
-  write_rows<__nv_bfloat16, D, ROWS>(p, j, records, s_ml, rank);
+  join<__nv_bfloat16, D, ROWS, GROUPS, S::WARPS>(p, j, records, s_ml, (float*)(ring + S::RINGS), s_inbox_ml, rank);
 }
 
 // ------------------------------------------------------------------ float32
 constexpr int kExactTile = 2;          // units: a key a lane
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
 template <int D>
 constexpr int kTileF32 = kExactTile * kUnit * (D + 4 + D) * 4;      // (keys' rows are four longer: lanes read them side by side)
 
 template <int D, int RPW, int STAGES>
-constexpr size_t smem_f32() { return (size_t)STAGES * kTileF32<D> + (size_t)kWarps * RPW * D * 4 * 2; }
+constexpr size_t smem_f32() {                            // ring (then records), queries, inbox
+  constexpr size_t ring = (size_t)STAGES * kTileF32<D>, records = (size_t)kWarps * RPW * (D + kPad) * 4;
+  static_assert(ring >= records, "the records take the ring's place");
+  return ring + (size_t)kWarps * RPW * D * 4 + (size_t)(kWarps * RPW + kSpare) * (D + kPad) * 4;
+}
 
 template <int D, int RPW, int STAGES>
 __global__ void __launch_bounds__(kThreads)
@@ -508,16 +625,21 @@ attention_beams_exact_kernel(Params p) {
   constexpr int ROWS = kWarps * RPW, PIECES = D / 4;
   constexpr uint32_t kTileBytes = kTileF32<D>, kRow = (D + 4) * 4, kValues = kExactTile * kUnit * kRow;
   extern __shared__ __align__(16) char s_raw[];
-  __shared__ Units s_units;
-  __shared__ float2 s_ml[ROWS];
+  __shared__ Listed s_lists[kWarps][kList];
+  __shared__ float2 s_ml[ROWS], s_inbox_ml[ROWS + kSpare];
+  if (p.split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   pdl_launch_dependents();
   pdl_wait();
   char* ring = s_raw;
   float* s_q = (float*)(s_raw + STAGES * kTileBytes);    // [ROWS][D]
-  float* records = s_q + ROWS * D;                       // [ROWS][D]
+  float* records = (float*)s_raw;                        // [ROWS][D + kPad], when the ring is done with
+  float* inbox = s_q + ROWS * D;
   const uint32_t ring_at = smem_u32(ring);
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rank = p.split > 1 ? (int)cluster_rank() : 0;
-  const Job j = make_job(p);
+  Job j = make_job(p);
+  Turn turn = first_turn(p, j, rank);
+  Listed* list = s_lists[warp];
+  find_keys(p, j);
   const int live = j.beams * j.group, parts = p.page_size / kUnit;
   for (int x = t; x < ROWS * PIECES; x += kThreads) {
     const int i = x / PIECES, c = x - i * PIECES, w = i / j.group;
@@ -539,18 +661,17 @@ attention_beams_exact_kernel(Params p) {
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) o[k][e] = 0.f;
   }
-  int next = 0;
-  bool more = true;
-  while (more) {
-    const int total = list_units(p, j, s_units, rank, next, &more);
+  while (more_columns(p, j, turn)) {
+    const int total = list_units(p, j, turn, list, D * 4);
+    __syncthreads();                                     // (the ring is free)
     const int tiles = (total * parts + kExactTile - 1) / kExactTile;
     auto load = [&](int tile) {                          // a warp a unit's keys or values
       if (tile < tiles) {
         const int which = warp >> 1;
-        const Unit u = unit_of(p, j, s_units, tile * kExactTile + which, total, parts);
+        const Listed u = unit_of(j, list, tile * kExactTile + which, total, parts, kUnit * D * 4);
         if (u.beams != 0) {
           const uint32_t at = ring_at + (tile % STAGES) * kTileBytes;
-          const char* from = (const char*)((warp & 1) ? p.v : p.k) + u.row * (D * 4);
+          const char* from = (const char*)((warp & 1) ? p.v : p.k) + u.at;
           const uint32_t to = (warp & 1) ? at + kValues + which * kUnit * D * 4 : at + which * kUnit * kRow, row_bytes = (warp & 1) ? D * 4 : kRow;
 #pragma unroll
           for (int i = 0; i < kUnit * PIECES / 32; ++i) {
@@ -567,7 +688,7 @@ attention_beams_exact_kernel(Params p) {
       cp_async_wait<STAGES - 2>();
       __syncthreads();
       load(tile + STAGES - 1);
-      const Unit u = unit_of(p, j, s_units, tile * kExactTile + (lane >> 4), total, parts);
+      const Listed u = unit_of(j, list, tile * kExactTile + (lane >> 4), total, parts, kUnit * D * 4);
       const int key = u.key0 + (lane & 15);
       unsigned seen[RPW], any = 0, every = 0xffffffffu;
 #pragma unroll
@@ -637,46 +758,49 @@ attention_beams_exact_kernel(Params p) {
     }
     cp_async_wait<0>();
   }
+  __syncthreads();
 #pragma unroll
   for (int k = 0; k < RPW; ++k) {
     const int i = k * kWarps + warp;
     const float sum = warp_sum(l[k]);
     if (lane == 0) s_ml[i] = make_float2(m[k], sum);
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) records[i * D + e * 32 + lane] = o[k][e];
+    for (int e = 0; e < D / 32; ++e) records[i * (D + kPad) + e * 32 + lane] = o[k][e];
   }
-  write_rows<float, D, ROWS>(p, j, records, s_ml, rank);
+  __syncthreads();
+  join<float, D, ROWS, 1, kWarps>(p, j, records, s_ml, inbox, s_inbox_ml, rank);
 }
 
 // ------------------------------------------------------------------ launches
 // Clusters of `split` CTAs of a kernel that the current device holds at once (found once per device and split).
+constexpr int kMaxSplit = 16;
 struct Room {
   OncePerDevice attributes;
-  std::atomic<int> clusters[OncePerDevice::kMax][5];     // 0: not asked yet, else the number + 1
+  std::atomic<int> clusters[OncePerDevice::kMax][kMaxSplit + 1];     // 0: not asked yet, else the number + 1
   template <typename K>
-  int of(K* kernel, size_t smem, int log_split) {
+  int of(K* kernel, int threads, size_t smem, int split) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= OncePerDevice::kMax) dev = 0;
-    int n = clusters[dev][log_split].load(std::memory_order_relaxed);
+    int n = clusters[dev][split].load(std::memory_order_relaxed);
     if (n) return n - 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(1 << log_split, 64, 8);
-    cfg.blockDim = dim3(kThreads);
+    cfg.gridDim = dim3(split, 64, 8);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1u << log_split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.x = (unsigned)split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int found = 0;
     if (cudaOccupancyMaxActiveClusters(&found, kernel, &cfg) != cudaSuccess) { cudaGetLastError(); found = 0; }
-    clusters[dev][log_split].store(found + 1, std::memory_order_relaxed);
+    clusters[dev][split].store(found + 1, std::memory_order_relaxed);
     return found;
   }
 };
 
 template <typename K>
-int run(K* kernel, size_t smem, Room& room, int rows_of_cta, Params& p, int longest, cudaStream_t stream) {
+int run(K* kernel, int threads, size_t smem, int units_at_once, Room& room, int rows_of_cta, Params& p, int longest, cudaStream_t stream) {
   const cudaError_t e = room.attributes.run([&] {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -684,35 +808,46 @@ int run(K* kernel, size_t smem, Room& room, int rows_of_cta, Params& p, int long
   });
   if (e != cudaSuccess) return check_launch("attention_beams");
   const int group = p.nq / p.nkv, requests = (p.rows + p.beams - 1) / p.beams;
-  p.beams_of_chunk = min(p.beams, max(1, rows_of_cta / group));
-  p.chunks = (p.beams + p.beams_of_chunk - 1) / p.beams_of_chunk;
+  const int most = max(1, rows_of_cta / group);
+  p.chunks = (p.beams + most - 1) / most;
+  p.beams_of_chunk = (p.beams + p.chunks - 1) / p.chunks;
   const long long jobs = (long long)requests * p.nkv * p.chunks;
-  // the widest clusters that are all resident at once, down to a tile a CTA
-  int log_split = 4;
+  // the widest clusters that are all resident at once, down to one step a CTA, and whose inboxes hold the rows
   const int units = (longest + kUnit - 1) / kUnit;
-  while (log_split > 0 && ((kTile << log_split) > units + kTile || room.of(kernel, smem, log_split) < jobs)) --log_split;
-  p.split = 1 << log_split;
-  launch_cluster(kernel, dim3(p.split, (unsigned)(p.nkv * p.chunks), (unsigned)requests), dim3(kThreads), smem, stream, p.split, p);
+  int split = min(kMaxSplit, max(1, (units + units_at_once - 1) / units_at_once));
+  while (split > 1 && ((rows_of_cta + split - 1) / split * split > rows_of_cta + kSpare || room.of(kernel, threads, smem, split) < jobs)) --split;
+  p.split = split;
+  launch_cluster(kernel, dim3(p.split, (unsigned)(p.nkv * p.chunks), (unsigned)requests), dim3(threads), smem, stream, p.split, p);
   return check_launch("attention_beams");
 }
 
+template <int D, int RB, int WR, int GROUPS, int STAGES, int CTAS>
+int run_shape(Params& p, int longest, cudaStream_t stream) {
+  using S = Shape<D, RB, WR, GROUPS, STAGES>;
+  static Room room;
+  return run(attention_beams_kernel<D, RB, WR, GROUPS, STAGES, CTAS>, S::THREADS, S::SMEM, GROUPS, room, S::ROWS, p, longest, stream);
+}
+
+// Shapes, us at 32 / 8 heads of 128: 16 rows (16 x 4 beams, 1,100 keys) 4 rings of 3 stages, two CTAs to an SM 16.6, 3 of 4 18.6, 6 of 4 in one CTA 18.2; 32 rows
+// (16 x 8) two warps of 16 rows, 4 rings, one CTA 27, 3 rings in each of two CTAs 40, one warp of two blocks 38; 64 rows (6 x 8, 40 / 8 heads, 6,000 keys) two
+// warps of two blocks, 2 rings in each of two CTAs 69, 4 in one 89, four warps of one block 90.
 template <int D>
 int run_bf16(Params& p, int longest, cudaStream_t stream) {
-  constexpr int STAGES = D >= 96 ? 3 : 4;
-  static Room room[3];
   const int rows = min(p.beams, p.rows) * (p.nq / p.nkv);
-  if (rows <= 16) return run(attention_beams_kernel<D, 1, 1, STAGES>, smem_bf16<D, 1, 1, STAGES>(), room[0], 16, p, longest, stream);
-  if (rows <= 32) return run(attention_beams_kernel<D, 1, 2, STAGES>, smem_bf16<D, 1, 2, STAGES>(), room[1], 32, p, longest, stream);
-  return run(attention_beams_kernel<D, 2, 2, STAGES>, smem_bf16<D, 2, 2, STAGES>(), room[2], 64, p, longest, stream);
+  if (rows <= 16) return run_shape<D, 1, 1, 4, 3, 2>(p, longest, stream);
+  if (rows <= 32) return run_shape<D, 1, 2, 4, 3, 1>(p, longest, stream);
+  return run_shape<D, 2, 2, 2, 4, 2>(p, longest, stream);
+}
+
+template <int D, int RPW>
+int run_exact(Params& p, int longest, cudaStream_t stream) {
+  static Room room;
+  return run(attention_beams_exact_kernel<D, RPW, 3>, kThreads, smem_f32<D, RPW, 3>(), kExactTile, room, kWarps * RPW, p, longest, stream);
 }
 
 template <int D>
 int run_f32(Params& p, int longest, cudaStream_t stream) {
-  constexpr int STAGES = 3;
-  static Room room[2];
-  const int rows = min(p.beams, p.rows) * (p.nq / p.nkv);
-  if (rows <= 16) return run(attention_beams_exact_kernel<D, 4, STAGES>, smem_f32<D, 4, STAGES>(), room[0], 16, p, longest, stream);
-  return run(attention_beams_exact_kernel<D, 8, STAGES>, smem_f32<D, 8, STAGES>(), room[1], 32, p, longest, stream);
+  return min(p.beams, p.rows) * (p.nq / p.nkv) <= 16 ? run_exact<D, 4>(p, longest, stream) : run_exact<D, 8>(p, longest, stream);
 }
 
 }  // namespace
@@ -733,8 +868,10 @@ ILB_EXPORT int ilb_attention_beams(const void* q, void* out, int dtype, const vo
   ILB_REQUIRE(requests <= 65535 && (long long)nkv * beams <= 65535, "attention_beams: too many requests or heads");
   if (rows == 0) return 0;
   Params p{q, out, k, v, positions, table, sink, q_stride, out_stride, rows, beams, 0, 0, max_blocks, page_size, num_pages, window, nq, nkv, 1,
-           scale * kLog2e};
+           scale * kLog2e, 0u, 0xffffffffu};
   if (dtype == kBF16) {
+    if (scale < 0.f) { p.flip = 0x80008000u; p.scale_log2 = -p.scale_log2; }
+    if (scale == 0.f) { p.keep = 0u; p.scale_log2 = 1.f; }
     switch (d) {
       case 32: return run_bf16<32>(p, longest, stream);
       case 64: return run_bf16<64>(p, longest, stream);
