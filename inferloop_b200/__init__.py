@@ -14,10 +14,13 @@ def __getattr__(name):
     if name in ("Engine", "TokenOutput"):
         from .engine import engine as _e
         return getattr(_e, name)
+    if name == "BeamHypothesis":
+        from .engine import beams as _b
+        return _b.BeamHypothesis
     if name in ("ModelRunner", "StepEntry"):
         from . import engine as _pkg
         return getattr(_pkg, name)
     raise AttributeError(name)
 
 
-__all__ = ["Engine", "SamplingParams", "ModelRunner", "StepEntry", "TokenOutput"]
+__all__ = ["Engine", "SamplingParams", "ModelRunner", "StepEntry", "TokenOutput", "BeamHypothesis"]

@@ -167,6 +167,7 @@ class CacheManager:
                         self._slot_state[(owner, need.name)] = torch.zeros(
                             (max_requests,) + tuple(need.shape), dtype=need.dtype, device=device)
         self._live: Dict[Hashable, int] = {}        # request -> its number in the ledger
+        self._beam_state = None
 
     def __del__(self) -> None:
         h = getattr(self, "_h", None)
@@ -326,6 +327,14 @@ class CacheManager:
         """The state per request that belongs to no layer: name -> [slots, *shape]."""
         return {need.name: self._slot_state[(MODEL_OWNER, need.name)]
                 for need in self._slot_needs.get(MODEL_OWNER, ()) if (MODEL_OWNER, need.name) in self._slot_state}
+
+    def beam_state(self):
+        """Every page group's storage and all state per slot, as what moves when beams continue their parents."""
+        if self._beam_state is None:
+            from ..csrc.ops import BeamState
+            groups = [([x for x in (g.storage, g.storage_v) if x is not None], g.page_size, g.need.stride) for g in self.groups]
+            self._beam_state = BeamState(groups, list(self._slot_state.values()), self.device)
+        return self._beam_state
 
     # ------------------------------------------------------------------ facts
     def free_pages(self) -> Dict[int, int]:

@@ -63,6 +63,10 @@ def build_parser() -> argparse.ArgumentParser:
     gen.add_argument("--repetition-penalty", type=float, default=None)
     gen.add_argument("--seed", type=int, default=None)
     gen.add_argument("--eos-token", type=int, default=None)
+    gen.add_argument("--beams", type=int, default=None, metavar="N",
+                     help="search with N beams: prints the N best continuations with their scores (no sampling options)")
+    gen.add_argument("--length-penalty", type=float, default=1.0, help="with --beams: scores are divided by tokens ^ this")
+    gen.add_argument("--early-stopping", action="store_true", help="with --beams: end as soon as N continuations have finished")
     _add_engine_options(gen)
     ins = sub.add_parser("inspect-model", help="print the typed configuration")
     ins.add_argument("model_path", metavar="MODEL_PATH")
@@ -153,6 +157,15 @@ def cmd_run(args) -> int:
 
 def cmd_generate(args) -> int:
     tokens = [int(t) for t in args.tokens.replace(" ", "").split(",") if t]
+    if args.beams is not None:
+        given = [k for k in ("temperature", "top_k", "top_p", "min_p", "presence_penalty", "repetition_penalty", "seed") if getattr(args, k) is not None]
+        if given:
+            raise ValueError(f"--beams takes no sampling options, found {', '.join('--' + k.replace('_', '-') for k in given)}")
+        engine = _engine(args, args.model_path)
+        found = engine.beam_search([tokens], args.beams, args.max_new_tokens, args.length_penalty, args.early_stopping,
+                                   None if args.eos_token is None else [args.eos_token])[0]
+        print(json.dumps({"beams": [{"tokens": h.tokens, "score": h.score, "reason": h.finish_reason} for h in found]}))
+        return 0
     engine = _engine(args, args.model_path)
     params = _sampling(engine, {k: getattr(args, k) for k in (
         "temperature", "top_k", "top_p", "min_p", "presence_penalty", "repetition_penalty", "seed", "eos_token")})

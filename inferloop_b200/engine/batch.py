@@ -68,6 +68,7 @@ class StepContext:
     max_q_len: int = 0
     max_kv_len: int = 0
     decode_only: bool = False
+    beams: int = 0                 # rows r * beams .. (r + 1) * beams - 1 are the beams of one request and share pages (0: no beams)
     position_tables: Dict[object, torch.Tensor] = field(default_factory=dict)
     memo: Dict[str, object] = field(default_factory=dict)    # what one part of a step leaves for the next one to run
 

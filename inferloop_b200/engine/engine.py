@@ -375,6 +375,32 @@ class Engine:
             self.check_device()
         return [list(self.requests[i].generated) for i in ids]
 
+    def beam_search(self, prompts: Sequence[Sequence[int]], beams: int = 4, max_new_tokens: int = 16, length_penalty: float = 1.0,
+                    early_stopping: bool = False, eos_tokens: Optional[Sequence[int]] = None):
+        """The best continuations of every prompt that a search with `beams` beams finds: for each prompt a list of `BeamHypothesis`, best first (as many
+        as beams, or fewer where the vocabulary or the length has no more).  A hypothesis is finished by a token of `eos_tokens` (None: the
+        model's stop tokens) or by its length, and ranked by the sum of its log probabilities / (tokens ^ length_penalty).  A
+        request's search ends when as many have finished as it has beams and its best beam's score over its length so far is no
+        better than the worst of them, or, with `early_stopping`, as soon as they have finished.  Requests that are already being served
+        keep their pages; the search runs on what is free."""
+        from .beams import BeamSearch
+        defaults = self.generation_defaults.base
+        if eos_tokens is None:
+            eos_tokens = [t for t in (defaults.eos_token, *defaults.eos_tokens) if t is not None]
+        if self.max_output_tokens is not None:
+            max_new_tokens = min(max_new_tokens, int(self.max_output_tokens))
+        vocab = self.runner.spec.vocab_size
+        toks = [[int(t) for t in p] for p in prompts]
+        for p in toks:
+            if not p:
+                raise ValueError("a prompt needs at least one token")
+            for t in p:
+                if not 0 <= t < vocab:
+                    raise ValueError(f"token {t} is outside the vocabulary of {vocab}")
+            if len(p) + int(max_new_tokens) > self.max_model_len:
+                raise ValueError(f"{len(p)} tokens and {max_new_tokens} new ones exceed the model's limit of {self.max_model_len}")
+        return BeamSearch(self, beams, max_new_tokens, eos_tokens, length_penalty, early_stopping).run(toks)
+
     def result(self, request_id: Hashable) -> Request:
         return self.requests[request_id]
 

@@ -127,6 +127,11 @@ class DecodeGraphs:
         r = self.runner
         ints = torch.zeros(StepStager.layout(self._shapes(bucket)), dtype=torch.int32, device=r.device)
         ctx = self._prepare(entries, bucket, ints)
+        return self._record_step(key, ctx, ints, bucket, with_argmax)
+
+    def _record_step(self, key: tuple, ctx: StepContext, ints: torch.Tensor, bucket: int, with_argmax: bool) -> _Recorded:
+        """Run the step `ctx`, whose arrays lie in `ints`, and record it."""
+        r = self.runner
         pair = torch.zeros((2, bucket), dtype=torch.int32, device=r.device) if with_argmax else None
         # Once eagerly: builds kernels, sizes every scratch buffer, and does this step's work.
         logits = r.model.forward(ctx, r.cache)
@@ -291,6 +296,48 @@ class DecodeGraphs:
         rec.graph.replay()
         self.replays += 1
         return Drawn(rec.pair, n)
+
+    # ------------------------------------------------------------------ steps of beams
+    def beam_step(self, rows: int, beams: int, longest: int) -> tuple:
+        """(key, the recorded step or None, the context and integer arrays to fill in) of steps of `rows` rows, `beams` to a request, the longest of
+        which reaches `longest` tokens: what they read of the batch lies at one place for as long as the step is recorded."""
+        bucket = bucket_for(rows)
+        if bucket is None:
+            raise ValueError(f"{rows} rows exceed the largest decode bucket {BUCKETS[-1]}")
+        if not self.whole or self.runner.spec.token_extras:
+            raise ValueError("beams need a model whose whole step is recorded as one graph and that takes no inputs per token "
+                             "beside ids and positions")
+        key = ("beams", bucket, beams, longest >= ops.DECODE_LONG_CONTEXT)
+        rec = self._recorded.get(key)
+        if rec is not None and rec.workspace_generation != self.runner.ctx.workspace.generation:
+            del self._recorded[key]
+            rec = None
+        if rec is not None:
+            rec.ctx.position_tables.clear()
+            return key, rec, rec.ctx, rec.ints
+        shapes = self._shapes(bucket)
+        ints = torch.zeros(StepStager.layout(shapes), dtype=torch.int32, device=self.runner.device)
+        views, at = [], 0
+        for shape in shapes:
+            n = 1
+            for d in shape:
+                n *= int(d)
+            views.append(ints[at:at + n].view(*shape))
+            at += (n + 3) // 4 * 4
+        tokens, positions, seq_of_token, cu_q, kv_len, slots, logit_rows = views[:7]
+        ctx = StepContext(n_tokens=bucket, n_seqs=bucket, n_logit_rows=bucket, tokens=tokens, positions=positions, seq_of_token=seq_of_token, cu_q=cu_q,
+                          kv_len=kv_len, slots=slots, logit_rows=logit_rows, block_tables={g: views[7 + g] for g in range(len(self.runner.cache.groups))},
+                          h_q_start=[0] * rows, h_q_len=[1] * rows, h_kv_len=[longest] * rows, h_slots=[0] * rows, max_q_len=1, max_kv_len=longest,
+                          decode_only=True, beams=beams)
+        return key, None, ctx, ints
+
+    def run_beams(self, key: tuple, rec: Optional[_Recorded], ctx: StepContext, ints: torch.Tensor) -> _Recorded:
+        """Run a step of `beam_step` on the arrays as they are: replayed, or the first time kernel by kernel and recorded."""
+        if rec is None:
+            return self._record_step(key, ctx, ints, ctx.n_seqs, False)
+        rec.graph.replay()
+        self.replays += 1
+        return rec
 
     def recorded(self, n: int, with_argmax: bool) -> Optional[_Recorded]:
         """The graph recorded for this many sequences (the short-context one if both exist)."""

@@ -305,7 +305,8 @@ class GQAttention(Mixer):
         if self.value_mix is not None:
             # the step's tokens' values of the first layer that mixes: kept by it, read by the later ones
             v_first = ws.buffer(f"attn.v_first/{self.nkv}x{self.dv}", (T, self.nkv * self.dv), dt)
-        if (self.dv == self.d and step.decode_only and cache.k is not None and (cache.writable or self.value_mix is None)
+        shared = self._beams_share(step, cache, dt)
+        if (not shared and self.dv == self.d and step.decode_only and cache.k is not None and (cache.writable or self.value_mix is None)
                 and not self.shaped and not self.has_sink
                 and ops.attention_decode_fused_supported(
                     dt, cache.k.dtype, self.nq, self.nkv, self.d, cache.page_size, self.rotary_dim, rope is not None,
@@ -333,7 +334,9 @@ class GQAttention(Mixer):
             v_lambda=self.v_lambda if self.value_mix == "mixed" else None, v_keep=self.value_mix == "first")
         o = ws.buffer("attn.o", (T, self.nq * self.dv), dt)
         ops.scope("attention.attention")
-        if self.shaped:
+        if shared:
+            ops.attention_beams(q, o, cache.k, cache.v, step, table, step.beams, self.seen, self.scale, self.nq, self.nkv, self.d, sink=self.sink)
+        elif self.shaped:
             ops.attention_mixed_heads(q, o, cache.k, cache.v, step, table, self.seen, self.scale, self.nq, self.nkv,
                                       self.d, self.dv, sink=self.sink, head_mix=self.mix, dist_r1=self.r1, dist_r2=self.r2,
                                       softcap=self.softcap, temp_coef=self.temp_coef, temp_every=self.temp_every,
@@ -342,6 +345,11 @@ class GQAttention(Mixer):
             ops.attention(q, o, cache.k, cache.v, step, table, self.seen, self.scale,
                           self.nq, self.nkv, self.d, workspace=ws, decode_chunk=self.decode_chunk, dv=self.dv, sink=self.sink)
         self._finish(o, qkv, gate_col0, residual, out)
+
+    def _beams_share(self, step, cache, dtype) -> bool:
+        """Whether the step's rows are beams whose shared pages are read once."""
+        return (step.beams > 1 and not self.shaped and self.dv == self.d and cache.k is not None
+                and ops.attention_beams_supported(dtype, cache.k.dtype, self.nq, self.nkv, self.d, cache.page_size))
 
     def _forward_rows(self, qkv, rope, table, step, cache, gate_col0, residual, out) -> None:
         """The layer with norms over whole rows: input stage, means of the blocks this step completes, attention, the
@@ -368,8 +376,11 @@ class GQAttention(Mixer):
             ops.pool_means(cache.k, cache.v, pooled, step, table)
         o = ws.buffer("attn.o", (T, self.nq * self.dv), dt)
         ops.scope("attention.attention")
-        ops.attention(q, o, cache.k, cache.v, step, table, self.seen, self.scale, self.nq, self.nkv, self.d, workspace=ws,
-                      decode_chunk=self.decode_chunk, dv=self.dv, pooled=pooled, turn=v_rope)
+        if pooled is None and v_rope is None and self._beams_share(step, cache, dt):
+            ops.attention_beams(q, o, cache.k, cache.v, step, table, step.beams, self.seen, self.scale, self.nq, self.nkv, self.d)
+        else:
+            ops.attention(q, o, cache.k, cache.v, step, table, self.seen, self.scale, self.nq, self.nkv, self.d, workspace=ws,
+                          decode_chunk=self.decode_chunk, dv=self.dv, pooled=pooled, turn=v_rope)
         self._finish(o, qkv, gate_col0, residual, out)
 
     def _finish(self, o: torch.Tensor, qkv: torch.Tensor, gate_col0: int, residual: torch.Tensor, out: Optional[torch.Tensor]) -> None:
