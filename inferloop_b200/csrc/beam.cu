@@ -4,19 +4,17 @@
 // beam_select: the k best continuations (beam w, token v) of every request by
 //   s = (score[w] - lse_w) + x[w, v],   lse_w = log sum_v exp x[w, v],
 // in 64 bits, best first; equal ones by the higher logit, then the lower w V + v (the logits are exact, so that nothing but the scores' own
-// rounding decides between tokens that a beam's score swallows).  Two launches.  The first reads every logit once: a CTA takes a run of a
-// row into registers, leaves its maximum and sum of exponentials, and the run's k best.  No sort of the run is needed for those: the k-th
-// largest of the threads' maxima is a border that at least k elements reach, and only the k threads whose maxima reach it can hold such
-// elements, so that what is left to rank is bounded by k times the elements of a thread and is about 1.5 k in practice.  The second
-// launch, a CTA a request, joins the runs of its rows in the same way.
+// rounding decides between tokens that a beam's score swallows).  Two launches.  The first reads every logit once and leaves of each segment of 64
+// that a thread took its maximum and its sum of exponentials: no list, no sort, no barrier, so that it runs at the rate of the memory.  The second, a
+// CTA a request, adds up the sums, finds a border that at least k candidates reach (the k-th largest of the best four threads' maxima of every warp),
+// and reads again only the segments whose maxima reach it: about 2 k of them.
 // Bound: the logits' bytes.
 //
 // beam_keep: which of the candidates go on as beams and which are finished, one warp a request.
 //
 // beam_reorder: child w continues beam p = parents[w].  Its first child takes over a beam's last page and slot; the others take those of
 // the beams without children and have the rows copied there.  Sources have children and targets have none, so no copy reads what
-// another writes and one pass does.  Every CTA works the places out for itself (256 parents are 1 KB), which spares a launch and scratch; the
-// tables change in a second launch, after the copies have read them.  Bound: the copied bytes, read and written.
+// another writes and one pass does.  Bound: the copied bytes, read and written.
 //
 // step_build: positions, sequence indices, offsets, lengths and block tables of a step from the tokens that each sequence has and brings.
 #include <math.h>
@@ -31,9 +29,6 @@ namespace {
 
 constexpr int kMaxBeams = 32;
 constexpr int kMaxBest = 64;           // candidates a request
-constexpr int kRunThreads = 256;
-constexpr u64 kNone = 0;               // below every candidate's key
-
 // Unsigned order of the values; -0 and +0 are one value (the caller adds +0).
 __device__ __forceinline__ unsigned ordered(float v) {
   const unsigned u = __float_as_uint(v);
@@ -44,282 +39,299 @@ __device__ __forceinline__ u64 ordered(double v) {
   const u64 u = (u64)__double_as_longlong(v);
   return (u >> 63) ? ~u : (u | (1ull << 63));
 }
-__device__ __forceinline__ u64 make_key(float v, unsigned index) { return ((u64)ordered(v) << 32) | (unsigned)~index; }
+__device__ __forceinline__ double unordered(u64 k) { return __longlong_as_double((long long)((k >> 63) ? (k ^ (1ull << 63)) : ~k)); }
 
-// ------------------------------------------------------------------ beam_select: runs of a row
-// keys [rows][runs][k] sorted, kNone behind the last; sums [rows][runs] = (maximum, sum of exp(x - maximum)); a maximum of NaN marks a run
-// with NaN or +inf in it.
-template <typename T, int ITEMS>
-__global__ void __launch_bounds__(kRunThreads)
-beam_runs_kernel(const T* __restrict__ logits, long long stride, int vocab, int k, u64* __restrict__ keys, float2* __restrict__ sums) {
-  pdl_launch_dependents();
-  pdl_wait();
-  __shared__ u64 s_max[kRunThreads];
-  __shared__ float s_m[kRunThreads / 32], s_sum[kRunThreads / 32];
-  __shared__ u64 s_border;
-  __shared__ int s_count, s_bad;
-  extern __shared__ u64 s_cand[];                       // [k * ITEMS]
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const int run = blockIdx.x, runs = gridDim.x, row = blockIdx.y;
-  const T* x = logits + (long long)row * stride;
-  const int first = run * (ITEMS * kRunThreads);
-  if (t == 0) { s_border = kNone; s_count = 0; s_bad = 0; }
-  float v[ITEMS];
+// ------------------------------------------------------------------ beam_select: maxima and sums of segments
+constexpr int kSegment = 64;           // logits of a thread
+constexpr int kTile = 32 * kSegment;   // of a warp
+constexpr int kSegmentThreads = 256;
+
+// Token of element i of a lane's segment in its tile: whole vectors of 16 bytes side by side over the warp where the row lies on a 16-byte
+// boundary, else single values.
+template <typename T>
+__device__ __forceinline__ int place_in_tile(int lane, int i, bool vectors) {
   constexpr int VEC = 16 / (int)sizeof(T);
-  const bool whole = first + ITEMS * kRunThreads <= vocab && ((uintptr_t)(x + first) & 15) == 0;
-#pragma unroll
-  for (int j = 0; j < ITEMS / VEC; ++j) {
-    const int at = first + (j * kRunThreads + t) * VEC;
-    if (whole) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(x + at);
-      const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j * VEC + i] = to_float(e[i]) + 0.f;
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j * VEC + i] = at + i < vocab ? to_float(x[at + i]) + 0.f : -INFINITY;
-    }
-  }
-  auto index = [&](int i) { return (unsigned)(first + ((i / VEC) * kRunThreads + t) * VEC + i % VEC); };
-  float m = -INFINITY;
-  int best = -1;
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    bad |= !(v[i] < INFINITY);
-    if (v[i] > m) { m = v[i]; best = i; }               // (a thread's indices rise with i: the first of equals is the lowest)
-  }
-  const float base = m == -INFINITY ? 0.f : m;
-  float sum = 0.f;                     // in pairs: a sum of 32 takes five roundings
-  {
-    float part[5];
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      float e = exp2f((v[i] - base) * 1.4426950408889634f);
-#pragma unroll
-      for (int level = 0; level < 5; ++level) {
-        if (!((i >> level) & 1)) { part[level] = e; break; }
-        e += part[level];
-      }
-      if (i == ITEMS - 1) sum = e;
-    }
-  }
-  u64 mine = kNone;
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i) if (i == best) mine = make_key(m, index(i));
-  // the warp's maximum and sum
-  const float wm = warp_max(m);
-  const float ws = warp_sum(m == -INFINITY ? 0.f : sum * expf(m - wm));
-  if (lane == 0) { s_m[warp] = wm; s_sum[warp] = ws; }
-  // the threads' maxima, sorted within the warp, largest first
-  u64 sorted = mine;
-#pragma unroll
-  for (int size = 2; size <= 32; size *= 2) {
-#pragma unroll
-    for (int d = size / 2; d > 0; d /= 2) {
-      const u64 other = __shfl_xor_sync(0xffffffffu, sorted, d);
-      const bool keep_large = ((lane & d) == 0) == ((lane & size) == 0);
-      sorted = keep_large ? (sorted > other ? sorted : other) : (sorted < other ? sorted : other);
-    }
-  }
-  s_max[t] = sorted;
-  __syncthreads();
-  if (bad) s_bad = 1;
-  // the border: the maximum with k - 1 larger ones (kNone if there are fewer than k)
-  if (sorted != kNone) {
-    int larger = lane;
-#pragma unroll
-    for (int o = 1; o < kRunThreads / 32; ++o) {
-      const u64* other = s_max + ((warp + o) & (kRunThreads / 32 - 1)) * 32;
-      int at = 0;                                       // how many of the other warp's are larger
-#pragma unroll
-      for (int step = 16; step > 0; step /= 2) if (other[at + step - 1] > sorted) at += step;
-      if (at == 31 && other[31] > sorted) at = 32;
-      larger += at;
-    }
-    if (larger == k - 1) s_border = sorted;
-  }
-  __syncthreads();
-  const u64 border = s_border;
-  if (mine != kNone && mine >= border) {
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      if (v[i] > -INFINITY) {
-        const u64 key = make_key(v[i], index(i));
-        if (key >= border) s_cand[atomicAdd(&s_count, 1)] = key;
-      }
-    }
-  }
-  __syncthreads();
-  // (their order in the list depends on the threads' timing, their ranks do not)
-  const int n = s_count;
-  u64* out = keys + ((long long)row * runs + run) * k;
-  for (int c = t; c < n; c += kRunThreads) {
-    const u64 key = s_cand[c];
-    int rank = 0;
-    for (int o = 0; o < n && rank < k; ++o) rank += s_cand[o] > key;
-    if (rank < k) out[rank] = key;
-  }
-  for (int c = n + t; c < k; c += kRunThreads) out[c] = kNone;
-  if (t == 0) {
-    float M = -INFINITY;
-    for (int w = 0; w < kRunThreads / 32; ++w) M = fmaxf(M, s_m[w]);
-    float S = 0.f;
-    if (M != -INFINITY)
-      for (int w = 0; w < kRunThreads / 32; ++w) S += s_sum[w] * expf(s_m[w] - M);
-    sums[(long long)row * runs + run] = make_float2(s_bad ? NAN : M, S);
-  }
+  return vectors ? ((i / VEC) * 32 + lane) * VEC + i % VEC : i * 32 + lane;
 }
 
-// ------------------------------------------------------------------ beam_select: the runs of a request's rows joined
+// sums [rows][tiles * 32] = (maximum, sum of exp(x - maximum)) of every segment; a sum of NaN marks NaN or +inf among its logits.
+template <typename T>
+__global__ void __launch_bounds__(kSegmentThreads)
+beam_segments_kernel(const T* __restrict__ logits, long long stride, int rows, int vocab, int tiles, float2* __restrict__ sums) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const int lane = threadIdx.x & 31;
+  const long long tile = (long long)blockIdx.x * (kSegmentThreads / 32) + (threadIdx.x >> 5);
+  if (tile >= (long long)rows * tiles) return;
+  const int row = (int)(tile / tiles), first = (int)(tile - (long long)row * tiles) * kTile;
+  const T* x = logits + (long long)row * stride + first;
+  const bool vectors = ((uintptr_t)(logits + (long long)row * stride) & 15) == 0;
+  float v[kSegment];
+  if (vectors && first + kTile <= vocab) {
+    uint4 raw[kSegment / VEC];
+#pragma unroll
+    for (int j = 0; j < kSegment / VEC; ++j) raw[j] = *reinterpret_cast<const uint4*>(x + (j * 32 + lane) * VEC);
+#pragma unroll
+    for (int j = 0; j < kSegment / VEC; ++j) {
+      const T* e = reinterpret_cast<const T*>(&raw[j]);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[j * VEC + i] = to_float(e[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kSegment; ++i) {
+      const int at = place_in_tile<T>(lane, i, vectors);
+      v[i] = first + at < vocab ? to_float(x[at]) : -INFINITY;
+    }
+  }
+  float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < kSegment; ++i) part[i & 3] = fmaxf(part[i & 3], v[i]);
+  const float m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) + 0.f, base = m == -INFINITY ? 0.f : m;
+  // the sum in pairs: 64 terms take six roundings (an infinity less itself, and NaN, make it NaN)
+#pragma unroll
+  for (int i = 0; i < kSegment; ++i) {
+    const float t = (v[i] - base) * 1.4426950408889634f;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v[i]) : "f"(t));
+  }
+#pragma unroll
+  for (int n = 1; n < kSegment; n *= 2)
+#pragma unroll
+    for (int i = 0; i < kSegment; i += 2 * n) v[i] += v[i + n];
+  sums[tile * 32 + lane] = make_float2(m, v[0]);
+}
+
+// ------------------------------------------------------------------ beam_select: the rows of a request joined
 struct Ranked { u64 score, tie; };      // the score's order, then (logit's order, ~(w V + v))
 __device__ __forceinline__ bool above(const Ranked& a, const Ranked& b) { return a.score > b.score || (a.score == b.score && a.tie > b.tie); }
 
-constexpr int kJoinThreads = 256;
-constexpr int kMaxRuns = 512;
-
 // The first launch's sums of exponentials are of 32 bits.  A term at distance d below the maximum is off by (2^-23 + 2^-26) d (difference,
-// product, the constant's last bits) and 2^-22 (each of three exponentials), a sum by 18 roundings and the scaling by 2: with sum p d <= ln(vocab) that is
-// 4.1e-6 for up to 4 M tokens, and two beams are in order for sure when their scores differ by twice as much.  Where candidates of two beams that
+// product, the constant's last bits) and 2^-22 (each of two exponentials), a segment's sum by 6 roundings (further sums are of 64 bits): with
+// sum p d <= ln(vocab) that is 3e-6 for up to 4 M tokens, and two beams are in order for sure when their scores differ by twice as much.  Where candidates of two beams that
 // matter come closer, those beams' sums are taken once more, in 64 bits: about one step of one request in a thousand.
-constexpr double kUncertain = 8.2e-6;
+constexpr double kUncertain = 6e-6;
+constexpr int kJoinThreads = 1024, kJoinWarps = kJoinThreads / 32;
+constexpr int kListed = 1024;          // segments, and candidates, that are looked at in one go
+constexpr int kBestOfWarp = 4;
+constexpr int kMaxVocab = 1 << 22;
 
-__device__ __forceinline__ double score_of(const Ranked& e) {
-  const u64 u = e.score;
-  return __longlong_as_double((long long)((u >> 63) ? (u ^ (1ull << 63)) : ~u));
+// The sum over the block of a 64-bit value, the same for every thread.
+__device__ double block_sum(double v, double* part) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double all = part[threadIdx.x & 31];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+  return all;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads)
-beam_join_kernel(const T* __restrict__ logits, long long stride, const u64* __restrict__ keys, const float2* __restrict__ sums,
-                 const float* __restrict__ scores, int beams, int runs, int vocab, int k, int* __restrict__ parents, int* __restrict__ tokens,
-                 float* __restrict__ out_scores, int* __restrict__ bad) {
+beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* __restrict__ sums, const float* __restrict__ scores, int beams, int tiles,
+                 int vocab, int k, int* __restrict__ parents, int* __restrict__ tokens, float* __restrict__ out_scores, int* __restrict__ bad) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ double s_base[kMaxBeams];                  // score - lse, or NaN: the beam brings no candidates
-  __shared__ double s_top[kMaxBeams];                   // a row's maximum
-  __shared__ double s_part[kJoinThreads / 32];
-  __shared__ Ranked s_border;
-  __shared__ int s_count, s_reaching, s_reach[kMaxBest];
-  __shared__ unsigned s_close;                          // beams whose order is not certain
-  extern __shared__ Ranked s_list[];                    // heads of the lists, then candidates: [max(beams * runs, k * k)]
+  __shared__ double s_base[kMaxBeams], s_top[kMaxBeams], s_part[kJoinWarps];      // score - lse or NaN (the beam brings no candidates), maximum
+  __shared__ float s_m[kJoinWarps];
+  __shared__ double s_sum[kJoinWarps];
+  __shared__ u64 s_best[kBestOfWarp * kJoinWarps];
+  __shared__ double s_border;
+  __shared__ int s_segments, s_count, s_list[kListed];
+  __shared__ unsigned s_live, s_close, s_bad;
+  __shared__ Ranked s_cand[kListed];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, r = blockIdx.x;
-  for (int w = warp; w < beams; w += kJoinThreads / 32) {
-    const long long row = (long long)r * beams + w;
-    double m = -INFINITY;
-    bool broken = false;
-    for (int c = lane; c < runs; c += 32) {
-      const float x = sums[row * runs + c].x;
-      broken |= isnan(x);
-      m = fmax(m, (double)x);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-    broken = __any_sync(0xffffffffu, broken);
-    double s = 0.0;
-    for (int c = lane; c < runs; c += 32) {
-      const float2 p = sums[row * runs + c];
-      if (p.x > -INFINITY) s += (double)p.y * exp((double)p.x - m);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) {
-      const double base = (double)scores[row] - (m + log(s));
-      s_base[w] = broken || !isfinite(base) ? (double)NAN : base;
-      s_top[w] = m;
-      if (bad != nullptr) bad[row] = broken ? 1 : 0;
+  const int segments = tiles * 32;
+  const float2* request = sums + (long long)r * beams * segments;
+  if (warp == 0) {
+    const bool alive = lane < beams && isfinite(scores[(long long)r * beams + lane]);
+    const unsigned live = __ballot_sync(0xffffffffu, alive);
+    if (lane == 0) { s_live = live; s_segments = 0; s_count = 0; s_close = 0; s_bad = 0; }
+    if (lane < beams) s_base[lane] = (double)NAN;
+  }
+  __syncthreads();
+  // the warps are dealt out to the beams that are alive: so many side by side, rounded up to a power of two
+  const unsigned live = s_live;
+  const int lives = __popc(live);
+  int wide = 1;
+  while (wide < lives) wide *= 2;
+  const int turn = warp & (wide - 1), share = warp / wide, shares = kJoinWarps / wide;
+  const int w = turn < lives ? (int)__fns(live, 0, turn + 1) : -1;
+  const float2* mine = request + (long long)(w < 0 ? 0 : w) * segments;
+  // a row's maximum (the thread's best segment on the way), then its sum
+  float m = -INFINITY;
+  if (w >= 0)
+    for (int s = share * 32 + lane; s < segments; s += shares * 32) m = fmaxf(m, mine[s].x);
+  const float top = warp_max(m);
+  double sum = 0.0;
+  if (w >= 0) {
+    for (int s = share * 32 + lane; s < segments; s += shares * 32) {
+      const float2 p = mine[s];
+      sum += p.x == -INFINITY ? (double)p.y : (double)p.y * (double)expf(p.x - top);
     }
   }
-  const int lists = beams * runs;
-  auto entry = [&](int list, int i) {
-    const int w = list / runs;
-    const u64 key = keys[((long long)r * lists + list) * k + i];
-    const double base = s_base[w];
-    if (key == kNone || isnan(base)) return Ranked{0, 0};
-    const unsigned flat = (unsigned)w * (unsigned)vocab + ~(unsigned)key;
-    return Ranked{ordered(base + (double)unordered((unsigned)(key >> 32)) + 0.0), (key & 0xffffffff00000000ull) | (unsigned)~flat};
-  };
-  auto beam_of = [&](const Ranked& e) { return (int)(~(unsigned)e.tie / (unsigned)vocab); };
-  const long long out = (long long)r * k;
-  int n = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    if (t == 0) { s_count = 0; s_reaching = 0; s_close = 0; s_border = Ranked{0, 0}; }
-    __syncthreads();
-    for (int l = t; l < lists; l += kJoinThreads) s_list[l] = entry(l, 0);
-    __syncthreads();
-    // the border: the head with k - 1 larger ones; at most k lists reach it (all of them where fewer than k bring anything)
-    for (int l = t; l < lists; l += kJoinThreads) {
-      const Ranked mine = s_list[l];
-      if (mine.tie == 0) continue;
-      int larger = 0;
-      for (int o = 0; o < lists && larger < k; ++o) larger += above(s_list[o], mine);
-      if (larger == k - 1) s_border = mine;
-    }
-    __syncthreads();
-    const Ranked border = s_border;
-    const double near = border.tie != 0 ? score_of(border) - kUncertain : 0.0;
-    const int border_beam = border.tie != 0 ? beam_of(border) : 0;
-    unsigned close = 0;
-    // (what is left out, but less than kUncertain below the border)
-    auto left_out = [&](const Ranked& e) {
-      if (score_of(e) >= near) {
-        const int w = beam_of(e);
-        if (w != border_beam) close |= 1u << w | 1u << border_beam;
-      }
-    };
-    for (int l = t; l < lists; l += kJoinThreads) {
-      const Ranked e = s_list[l];
-      if (e.tie == 0) continue;
-      if (above(border, e)) left_out(e);
-      else s_reach[atomicAdd(&s_reaching, 1)] = l;
-    }
-    __syncthreads();
-    const int reaching = s_reaching;
-    for (int i = t; i < reaching * k; i += kJoinThreads) {
-      const Ranked e = entry(s_reach[i / k], i % k);
-      if (e.tie == 0) continue;
-      if (above(border, e)) left_out(e);
-      else s_list[atomicAdd(&s_count, 1)] = e;
-    }
-    __syncthreads();
-    n = s_count;
-    for (int c = t; c < n; c += kJoinThreads) {
-      const Ranked e = s_list[c];
-      const double mine = score_of(e);
-      const int w = beam_of(e);
-      int rank = 0;
-      for (int o = 0; o < n; ++o) {
-        const Ranked x = s_list[o];
-        rank += above(x, e);
-        if (pass == 0 && fabs(score_of(x) - mine) <= kUncertain && beam_of(x) != w) close |= 1u << w | 1u << beam_of(x);
-      }
-      if (rank >= k) continue;
-      const unsigned flat = ~(unsigned)e.tie;
-      parents[out + rank] = w;
-      tokens[out + rank] = (int)(flat - (unsigned)w * (unsigned)vocab);
-      out_scores[out + rank] = (float)mine;
-    }
-    if (pass == 1) break;
-    if (close) atomicOr(&s_close, close);
-    __syncthreads();
-    const unsigned again = s_close;
-    if (again == 0) break;
-    for (int w = 0; w < beams; ++w) {
-      if (!(again >> w & 1)) continue;
-      const T* x = logits + ((long long)r * beams + w) * stride;
-      const double top = s_top[w];
-      double s = 0.0;
-      for (int i = t; i < vocab; i += kJoinThreads) s += exp((double)to_float(x[i]) - top);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0) s_part[warp] = s;
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) { s_m[warp] = top; s_sum[warp] = sum; }
+  if (bad != nullptr && lives < beams) {
+    for (int dead = 0; dead < beams; ++dead) {           // (of those that are not alive only whether the row is broken is asked)
+      if (live >> dead & 1) continue;
+      bool broken = false;
+      for (int s = t; s < segments; s += kJoinThreads) broken |= isnan(request[(long long)dead * segments + s].y);
+      if (broken) atomicOr(&s_bad, 1u << dead);
+    }
+  }
+  __syncthreads();
+  if (t < lives) {
+    const int beam = (int)__fns(live, 0, t + 1);
+    double all_top = -INFINITY, all = 0.0;
+    for (int i = t; i < kJoinWarps; i += wide) all_top = fmax(all_top, (double)s_m[i]);
+    for (int i = t; i < kJoinWarps; i += wide) all += s_m[i] > -INFINITY ? s_sum[i] * exp((double)s_m[i] - all_top) : s_sum[i];
+    const double base = (double)scores[(long long)r * beams + beam] - (all_top + log(all));
+    s_base[beam] = !isfinite(base) ? (double)NAN : base;
+    s_top[beam] = all_top;
+    if (isnan(all)) atomicOr(&s_bad, 1u << beam);
+  }
+  __syncthreads();
+  if (bad != nullptr && t < beams) bad[(long long)r * beams + t] = s_bad >> t & 1;
+  // the border: of every warp its threads' four best maxima, of those the k-th largest (at least half of the 32 warps have a beam, unless all are dead)
+  {
+    u64 best = w >= 0 && m > -INFINITY && !isnan(s_base[w]) ? ordered(s_base[w] + (double)m + 0.0) : 0;
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2) {
+#pragma unroll
+      for (int d = size / 2; d > 0; d /= 2) {
+        const u64 other = __shfl_xor_sync(0xffffffffu, best, d);
+        const bool larger = ((lane & d) == 0) == ((lane & size) == 0);
+        best = larger ? (best > other ? best : other) : (best < other ? best : other);
+      }
+    }
+    if (lane < kBestOfWarp) s_best[warp * kBestOfWarp + lane] = best;
+  }
+  __syncthreads();
+  if (t < kBestOfWarp * kJoinWarps) {
+    const u64 key = s_best[t];
+    int larger = 0;
+    for (int i = 0; i < kBestOfWarp * kJoinWarps; ++i) larger += s_best[i] > key || (s_best[i] == key && i < t);
+    if (larger == k - 1) s_border = key == 0 ? -INFINITY : unordered(key);
+  }
+  __syncthreads();
+  // segments, then logits, that reach it or come closer than the sums are certain
+  const double border = s_border - kUncertain;
+  if (w >= 0 && !isnan(s_base[w]) && m > -INFINITY && s_base[w] + (double)m >= border) {
+    for (int s = share * 32 + lane; s < segments; s += shares * 32) {
+      const float x = mine[s].x;
+      if (x > -INFINITY && s_base[w] + (double)x >= border) {
+        const int at = atomicAdd(&s_segments, 1);
+        if (at < kListed) s_list[at] = w * segments + s;
+      }
+    }
+  }
+  __syncthreads();
+  const int listed = s_segments;
+  auto rank_of = [&](float x, int beam, int token) {
+    const unsigned flat = (unsigned)beam * (unsigned)vocab + (unsigned)token;
+    return Ranked{ordered(s_base[beam] + (double)x + 0.0), ((u64)ordered(x) << 32) | (unsigned)~flat};
+  };
+  if (listed <= kListed) {
+    for (int i = warp; i < listed; i += kJoinWarps) {
+      const int beam = s_list[i] / segments, s = s_list[i] - beam * segments, tile = s >> 5;
+      const T* row = logits + ((long long)r * beams + beam) * stride;
+      const bool vectors = ((uintptr_t)row & 15) == 0;
+#pragma unroll
+      for (int e = lane; e < kSegment; e += 32) {
+        const int token = tile * kTile + place_in_tile<T>(s & 31, e, vectors);
+        const float x = token < vocab ? to_float(row[token]) + 0.f : -INFINITY;
+        if (x > -INFINITY && s_base[beam] + (double)x >= border) {
+          const int at = atomicAdd(&s_count, 1);
+          if (at < kListed) s_cand[at] = rank_of(x, beam, token);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const long long out = (long long)r * k;
+  auto put = [&](int rank, const Ranked& e) {
+    const unsigned flat = ~(unsigned)e.tie;
+    const int beam = (int)(flat / (unsigned)vocab);
+    parents[out + rank] = beam;
+    tokens[out + rank] = (int)(flat - (unsigned)beam * (unsigned)vocab);
+    out_scores[out + rank] = (float)unordered(e.score);
+  };
+  // the beam's sum once more, in 64 bits (all threads)
+  auto again = [&](int beam) {
+    const T* x = logits + ((long long)r * beams + beam) * stride;
+    const double top = s_top[beam];
+    double s = 0.0;
+    for (int i = t; i < vocab; i += kJoinThreads) s += exp((double)to_float(x[i]) - top);
+    s = block_sum(s, s_part);
+    if (t == 0) s_base[beam] = (double)scores[(long long)r * beams + beam] - (top + log(s));
+  };
+  int n = s_count;
+  if (listed <= kListed && n <= kListed) {
+    for (int pass = 0; pass < 2; ++pass) {
+      // (the list's order depends on the threads' timing, the ranks do not)
+      unsigned close = 0;
+      for (int c = t; c < n; c += kJoinThreads) {
+        const Ranked e = s_cand[c];
+        const double score = unordered(e.score);
+        const int beam = (int)(~(unsigned)e.tie / (unsigned)vocab);
+        int rank = 0;
+        unsigned near = 0;
+        for (int i = 0; i < n; ++i) {
+          const Ranked x = s_cand[i];
+          rank += above(x, e);
+          if (pass == 0 && fabs(unordered(x.score) - score) <= kUncertain) near |= 1u << (~(unsigned)x.tie / (unsigned)vocab);
+        }
+        if (rank < k) put(rank, e);
+        if (rank <= k && (near & ~(1u << beam))) close |= near | 1u << beam;       // (of the k-th and the one behind it, both know)
+      }
+      if (pass == 1) break;
+      if (close) atomicOr(&s_close, close);
       __syncthreads();
-      if (t == 0) {
-        double all = 0.0;
-        for (int i = 0; i < kJoinThreads / 32; ++i) all += s_part[i];
-        s_base[w] = (double)scores[(long long)r * beams + w] - (top + log(all));
+      const unsigned unsure = s_close;
+      if (unsure == 0) break;
+      for (int beam = 0; beam < beams; ++beam) if (unsure >> beam & 1) again(beam);
+      __syncthreads();
+      for (int c = t; c < n; c += kJoinThreads) {
+        const unsigned flat = ~(unsigned)s_cand[c].tie, beam = flat / (unsigned)vocab;
+        s_cand[c] = rank_of(unordered((unsigned)(s_cand[c].tie >> 32)), (int)beam, (int)(flat - beam * (unsigned)vocab));
       }
       __syncthreads();
+    }
+  } else {
+    // More candidates than the lists hold (thousands of equal logits): one after the other, each the best below the one before.
+    for (int beam = 0; beam < beams; ++beam)
+      if (!isnan(s_base[beam])) again(beam);             // (uniform: s_base is the same for all)
+    __syncthreads();
+    Ranked last{~0ull, ~0ull};
+    for (n = 0; n < k; ++n) {
+      Ranked best{0, 0};
+      for (int beam = 0; beam < beams; ++beam) {
+        if (isnan(s_base[beam])) continue;
+        const T* row = logits + ((long long)r * beams + beam) * stride;
+        for (int token = t; token < vocab; token += kJoinThreads) {
+          const float x = to_float(row[token]) + 0.f;
+          if (!(x > -INFINITY)) continue;
+          const Ranked e = rank_of(x, beam, token);
+          if (above(last, e) && above(e, best)) best = e;
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const Ranked x{__shfl_xor_sync(0xffffffffu, best.score, o), __shfl_xor_sync(0xffffffffu, best.tie, o)};
+        if (above(x, best)) best = x;
+      }
+      __syncthreads();
+      if (lane == 0) s_cand[warp] = best;
+      __syncthreads();
+      for (int i = 0; i < kJoinWarps; ++i) if (above(s_cand[i], best)) best = s_cand[i];
+      if (best.tie == 0) break;
+      if (t == 0) put(n, best);
+      last = best;
     }
   }
   for (int c = n + t; c < k; c += kJoinThreads) {
@@ -329,52 +341,27 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const u64* __re
   }
 }
 
-int items_of(int rows, int vocab, int dtype) {
-  (void)rows; (void)vocab; (void)dtype;
-  return 32;
-}
-
 }  // namespace
 
-// Sizes of the scratch that ilb_beam_select needs: 8-byte words of `keys`, elements of `sums`.
-ILB_EXPORT int ilb_beam_select_plan(int dtype, int rows, int vocab, int k, long long* words, long long* elements) {
-  ILB_REQUIRE(rows >= 0 && vocab > 0 && k > 0 && k <= kMaxBest, "beam_select: bad sizes (up to %d candidates)", kMaxBest);
-  const int run = items_of(rows, vocab, dtype) * kRunThreads, runs = (vocab + run - 1) / run;
-  *words = (long long)rows * runs * k;
-  *elements = (long long)rows * runs;
-  return 0;
-}
+// Elements (of 8 bytes) of the scratch that ilb_beam_select needs.
+ILB_EXPORT long long ilb_beam_select_scratch(long long rows, int vocab) { return rows * ((vocab + kTile - 1) / kTile) * 32; }
 
 ILB_EXPORT int ilb_beam_select(const void* logits, int dtype, long long stride, const float* scores, int* parents, int* tokens, float* out_scores,
-                               int* bad, int requests, int beams, int vocab, int k, void* keys, void* sums, cudaStream_t stream) {
-  ILB_REQUIRE(requests >= 0 && beams > 0 && beams <= kMaxBeams && vocab > 0 && k > 0 && k <= kMaxBest && stride >= vocab,
-              "beam_select: bad sizes (up to %d beams and %d candidates)", kMaxBeams, kMaxBest);
-  const long long rows = (long long)requests * beams;
-  ILB_REQUIRE(rows <= 65535 && (long long)beams * vocab < (1ll << 32), "beam_select: up to 65535 rows, beams times vocabulary below 2^32");
+                               int* bad, int requests, int beams, int vocab, int k, void* sums, cudaStream_t stream) {
+  ILB_REQUIRE(requests >= 0 && beams > 0 && beams <= kMaxBeams && vocab > 0 && vocab <= kMaxVocab && k > 0 && k <= kMaxBest && stride >= vocab,
+              "beam_select: bad sizes (up to %d beams, %d candidates and a vocabulary of %d)", kMaxBeams, kMaxBest, kMaxVocab);
   ILB_REQUIRE(dtype == kF32 || dtype == kBF16, "beam_select: unknown element type %d", dtype);
+  const int tiles = (vocab + kTile - 1) / kTile;
+  const long long rows = (long long)requests * beams, blocks = (rows * tiles + kSegmentThreads / 32 - 1) / (kSegmentThreads / 32);
+  ILB_REQUIRE(rows < (1 << 24) && blocks < (1ll << 31), "beam_select: too many rows");
   if (requests == 0) return 0;
-  const int items = items_of((int)rows, vocab, dtype), run = items * kRunThreads, runs = (vocab + run - 1) / run;
-  ILB_REQUIRE(runs <= kMaxRuns, "beam_select: a vocabulary of up to %d", kMaxRuns * run);
-  const size_t smem = (size_t)k * items * sizeof(u64);
-  const dim3 grid(runs, (unsigned)rows);
-  if (dtype == kF32)
-    launch(beam_runs_kernel<float, 32>, grid, dim3(kRunThreads), smem, stream, (const float*)logits, stride, vocab, k, (u64*)keys, (float2*)sums);
-  else
-    launch(beam_runs_kernel<__nv_bfloat16, 32>, grid, dim3(kRunThreads), smem, stream, (const __nv_bfloat16*)logits, stride, vocab, k, (u64*)keys,
-           (float2*)sums);
-  int rc = check_launch("beam_select");
-  if (rc) return rc;
-  const int lists = beams * runs, room = lists > k * k ? lists : k * k;
-  const size_t join = (size_t)room * sizeof(Ranked);
-  ILB_REQUIRE(join <= 200 * 1024, "beam_select: %d beams of %d runs do not fit a CTA's memory", beams, runs);
-  auto joined = [&](auto* kernel, auto* x, OncePerDevice& once) {
-    if (once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024); }) != cudaSuccess) return;
-    launch(kernel, dim3((unsigned)requests), dim3(kJoinThreads), join, stream, x, stride, (const u64*)keys, (const float2*)sums, scores, beams, runs, vocab,
-           k, parents, tokens, out_scores, bad);
+  auto both = [&](auto* x, auto* segments, auto* join) {
+    launch(segments, dim3((unsigned)blocks), dim3(kSegmentThreads), 0, stream, x, stride, (int)rows, vocab, tiles, (float2*)sums);
+    launch(join, dim3((unsigned)requests), dim3(kJoinThreads), 0, stream, x, stride, (const float2*)sums, scores, beams, tiles, vocab, k, parents, tokens,
+           out_scores, bad);
   };
-  static OncePerDevice once[2];
-  if (dtype == kF32) joined(beam_join_kernel<float>, (const float*)logits, once[0]);
-  else joined(beam_join_kernel<__nv_bfloat16>, (const __nv_bfloat16*)logits, once[1]);
+  if (dtype == kF32) both((const float*)logits, beam_segments_kernel<float>, beam_join_kernel<float>);
+  else both((const __nv_bfloat16*)logits, beam_segments_kernel<__nv_bfloat16>, beam_join_kernel<__nv_bfloat16>);
   return check_launch("beam_select");
 }
 ILB_PACKED(ilb_beam_select)
@@ -488,6 +475,7 @@ ILB_EXPORT int ilb_beam_keep(const int* parents, const int* tokens, const float*
   launch(beam_keep_kernel, dim3((unsigned)requests), dim3(32), 0, stream, p);
   return check_launch("beam_keep");
 }
+ILB_PACKED(ilb_beam_keep)
 
 // ------------------------------------------------------------------ beam_reorder
 namespace {
@@ -512,105 +500,166 @@ struct Groups {
   int n;
 };
 
-// Child w of row group r: whose place it takes (a beam of the request), and whose rows are copied there (-1: nobody's).
-__device__ __forceinline__ void places_of(const int* parents, int beams, int w, int* place, int* source) {
-  auto parent = [&](int i) { const int p = parents[i]; return p >= 0 && p < beams ? p : -1; };
-  auto is_first = [&](int i) {
-    const int p = parent(i);
-    if (p < 0) return false;
-    for (int j = 0; j < i; ++j) if (parent(j) == p) return false;
-    return true;
-  };
-  if (is_first(w)) { *place = parent(w); *source = -1; return; }
-  int turn = 0;                        // children before w that look for a place as well
-  for (int j = 0; j < w; ++j) turn += !is_first(j);
-  int b = 0;
-  for (; b < beams; ++b) {             // the turn-th beam without children
-    bool has = false;
-    for (int j = 0; j < beams; ++j) has |= parent(j) == b;
-    if (!has && turn-- == 0) break;
-  }
-  *place = b;
-  *source = parent(w);
+// Where a child goes, a lane a child of one request: whose place it takes (a beam of the request) and whose rows are copied there (-1: nobody's).  An
+// entry of `parents` outside the beams counts as -1.
+__device__ __forceinline__ void places_of(int parent, int beams, int lane, int* place, int* source) {
+  const bool there = lane < beams, has = there && parent >= 0 && parent < beams;
+  const unsigned same = __match_any_sync(0xffffffffu, has ? parent : -1 - lane);
+  const bool first = has && lane == __ffs((int)same) - 1;
+  const unsigned taken = __reduce_or_sync(0xffffffffu, first ? 1u << parent : 0u), looking = __ballot_sync(0xffffffffu, there && !first);
+  const unsigned free = ~taken & (beams == 32 ? 0xffffffffu : (1u << beams) - 1);
+  const int turn = __popc(looking & ((1u << lane) - 1));
+  *place = first ? parent : there ? (int)__fns(free, 0, turn + 1) : 0;           // (as many are free as look for a place)
+  *source = has && !first ? parent : -1;
 }
 
-// Whether every entry of `parents` makes sense is not looked at here: one outside the beams counts as -1.
-__device__ void work_out_places(const int* parents, int rows, int beams, short* place, short* source, int* s_parents) {
-  for (int i = threadIdx.x; i < rows; i += blockDim.x) s_parents[i] = parents[i];
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows; i += blockDim.x) {
-    int a, b;
-    places_of(s_parents + i / beams * beams, beams, i % beams, &a, &b);
-    place[i] = (short)a;
-    source[i] = (short)b;
-  }
-  __syncthreads();
-}
-
+// `bytes` bytes from a to b by one warp, eight vectors a lane on their way.
 template <typename V>
-__device__ __forceinline__ void copy_part(char* to, const char* from, long long bytes, int lane) {
+__device__ __forceinline__ void copy_part(char* to, const char* from, int bytes, int lane) {
   const V* a = reinterpret_cast<const V*>(from);
   V* b = reinterpret_cast<V*>(to);
-  const int n = (int)(bytes / (long long)sizeof(V));
-  int i = lane;
-  for (; i + 96 < n; i += 128) {
-    const V x0 = a[i], x1 = a[i + 32], x2 = a[i + 64], x3 = a[i + 96];
-    b[i] = x0; b[i + 32] = x1; b[i + 64] = x2; b[i + 96] = x3;
+  const int n = bytes / (int)sizeof(V);
+  for (int i0 = lane; i0 < n; i0 += 256) {
+    V x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) if (i0 + 32 * j < n) x[j] = a[i0 + 32 * j];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) if (i0 + 32 * j < n) b[i0 + 32 * j] = x[j];
   }
-  for (; i < n; i += 32) b[i] = a[i];
 }
 
-__global__ void __launch_bounds__(256)
-beam_copy_kernel(const int* __restrict__ parents, const int* __restrict__ kv_len, const int* __restrict__ slots, const Moved* __restrict__ moved,
-                 const int* __restrict__ first_part, int n_moved, int parts_of_copy, int num_slots, Groups groups, int rows, int beams) {
+// One launch.  Every CTA works the places out and reads the last pages and slots of all rows that copy (a few KB) before it does anything else, and
+// takes a ticket; the one that takes the last ticket replaces those entries, which nobody reads any more.  The other columns belong to full pages:
+// no copy reads them, a CTA a request moves them.  Warps take runs of neighbouring parts, so that they look up places and storage once a run.
+// `turns` [1]: zero between launches.
+constexpr int kCopyThreads = 256, kCopyWarps = kCopyThreads / 32;
+struct Copy { int from, to, fill; };    // of a row that copies: pages, filled rows (of a group), or slots
+__global__ void __launch_bounds__(kCopyThreads)
+beam_reorder_kernel(const int* __restrict__ parents, const int* __restrict__ kv_len, int* slots, const Moved* __restrict__ moved,
+                    const int* __restrict__ first_part, int n_moved, int parts_of_copy, int num_slots, Groups groups, int rows, int beams, int* turns) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ int s_parents[kMaxRows];
-  __shared__ short s_place[kMaxRows], s_source[kMaxRows], s_rows[kMaxRows];
-  __shared__ int s_copies;
-  work_out_places(parents, rows, beams, s_place, s_source, s_parents);
-  if (threadIdx.x < 32) {              // the rows that copy, in order
-    int n = 0;
-    for (int i0 = 0; i0 < rows; i0 += 32) {
-      const int i = i0 + (int)threadIdx.x;
-      const bool copies = i < rows && s_source[i] >= 0;
-      const unsigned mask = __ballot_sync(0xffffffffu, copies);
-      if (copies) s_rows[n + __popc(mask & ((1u << threadIdx.x) - 1))] = (short)i;
-      n += __popc(mask);
-    }
-    if (threadIdx.x == 0) s_copies = n;
+  extern __shared__ int s_mem[];
+  const int requests = rows / beams, kinds = groups.n + 1;
+  short* s_place = (short*)s_mem;                                    // [rows]
+  short* s_source = s_place + rows;                                  // [rows]
+  int* s_len = (int*)(s_source + rows);                              // [requests]
+  Copy* s_copy = (Copy*)(s_len + requests);                          // [rows][kinds]: groups, then slots
+  __shared__ int s_before[kCopyWarps + 1], s_last;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  // requests in runs a warp, so that the rows that copy are numbered in order
+  const int each = (requests + kCopyWarps - 1) / kCopyWarps, r0 = min(warp * each, requests), r1 = min(r0 + each, requests);
+  int n = 0;
+  for (int r = r0; r < r1; ++r) {
+    int place, source;
+    places_of(lane < beams ? parents[r * beams + lane] : -1, beams, lane, &place, &source);
+    if (lane < beams) { s_place[r * beams + lane] = (short)place; s_source[r * beams + lane] = (short)source; }
+    if (lane == 0) s_len[r] = kv_len[r * beams];
+    n += __popc(__ballot_sync(0xffffffffu, source >= 0));
+  }
+  if (lane == 0) s_before[warp + 1] = n;
+  __syncthreads();
+  if (t == 0) {
+    s_before[0] = 0;
+    for (int i = 0; i < kCopyWarps; ++i) s_before[i + 1] += s_before[i];
   }
   __syncthreads();
-  const int lane = threadIdx.x & 31;
-  const long long total = (long long)s_copies * parts_of_copy, step = (long long)gridDim.x * (blockDim.x / 32);
-  for (long long u = (long long)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); u < total; u += step) {
-    const int copy = (int)(u / parts_of_copy), part = (int)(u - (long long)copy * parts_of_copy);
-    const int i = s_rows[copy], first = i / beams * beams, from_row = first + s_source[i], to_row = first + s_place[i];
-    int lo = 0, hi = n_moved - 1;      // the storage that this part belongs to
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (first_part[mid] <= part) lo = mid; else hi = mid - 1;
+  const int copies = s_before[kCopyWarps];
+  n = s_before[warp];
+  for (int r = r0; r < r1; ++r) {
+    const int source = lane < beams ? s_source[r * beams + lane] : -1, place = lane < beams ? s_place[r * beams + lane] : 0;
+    const unsigned mask = __ballot_sync(0xffffffffu, source >= 0);
+    if (source >= 0) {
+      Copy* c = s_copy + (size_t)(n + __popc(mask & ((1u << lane) - 1))) * kinds;
+      const int from_row = r * beams + source, to_row = r * beams + place, len = s_len[r];
+      for (int g = 0; g < groups.n; ++g) {
+        const int have = len / groups.stride[g], block = have / groups.page_size[g], fill = have - block * groups.page_size[g];
+        Copy x{-1, -1, 0};
+        if (fill > 0 && block < groups.width[g]) {
+          x.from = groups.table[g][(long long)from_row * groups.width[g] + block];
+          x.to = groups.table[g][(long long)to_row * groups.width[g] + block];
+          // (a page that is not held: nothing moves)
+          if (x.from >= 0 && x.to >= 0 && x.from < groups.pages[g] && x.to < groups.pages[g]) x.fill = fill;
+        }
+        c[g] = x;
+      }
+      Copy x{-1, -1, 0};
+      if (slots != nullptr) {
+        x.from = slots[from_row];
+        x.to = slots[to_row];
+        x.fill = x.from >= 0 && x.to >= 0 && x.from < num_slots && x.to < num_slots;
+      }
+      c[groups.n] = x;
     }
-    const Moved m = moved[lo];
-    const int at = part - first_part[lo], plane = at / m.parts, piece = at - plane * m.parts;
-    long long from, to, bytes;
-    if (m.group >= 0) {
-      const int g = m.group, have = kv_len[first] / groups.stride[g], fill = have % groups.page_size[g], block = have / groups.page_size[g];
-      if (have < 0 || fill <= 0 || block >= groups.width[g]) continue;
-      from = groups.table[g][(long long)from_row * groups.width[g] + block];
-      to = groups.table[g][(long long)to_row * groups.width[g] + block];
-      if (from < 0 || to < 0 || from >= groups.pages[g] || to >= groups.pages[g]) continue;      // not held
-      bytes = (long long)((fill + m.unit_rows - 1) / m.unit_rows) * m.unit_bytes;
-    } else {
-      from = slots[from_row];
-      to = slots[to_row];
-      if (from < 0 || to < 0 || from >= num_slots || to >= num_slots) continue;
-      bytes = m.bytes - (long long)piece * kPart;
-      if (bytes > kPart) bytes = kPart;
+    n += __popc(mask);
+  }
+  __syncthreads();
+  if (t == 0) s_last = atomicAdd(turns, 1) == (int)gridDim.x - 1;
+  // full pages: columns before the last one of a request's rows
+  for (int r = blockIdx.x; r < requests; r += gridDim.x) {
+    for (int g = 0; g < groups.n; ++g) {
+      const int width = groups.width[g], columns = min(width, s_len[r] / groups.stride[g] / groups.page_size[g]);
+      int* table = groups.table[g] + (long long)r * beams * width;
+      for (int c = t; c < columns; c += kCopyThreads) {              // (a thread a column: nothing is read after it was replaced)
+        int old[kMaxBeams];
+#pragma unroll
+        for (int w = 0; w < kMaxBeams; ++w) { if (w >= beams) break; old[w] = table[(long long)w * width + c]; }
+        for (int w = 0; w < beams; ++w) {
+          const int p = parents[r * beams + w];
+          if (p < 0 || p >= beams || p == w) continue;
+          int x = old[0];
+#pragma unroll
+          for (int i = 1; i < kMaxBeams; ++i) if (i == p) x = old[i];
+          table[(long long)w * width + c] = x;
+        }
+      }
     }
+  }
+  __syncthreads();
+  if (s_last) {
+    // the last pages and the slots of all rows, read before any is replaced: a warp a request
+    if (t == 0) *turns = 0;
+    for (int r = warp; r < requests; r += kCopyWarps) {
+      const int row = r * beams + lane, from_row = r * beams + (lane < beams ? s_place[row] : 0);
+      for (int g = 0; g < groups.n; ++g) {
+        const int have = s_len[r] / groups.stride[g], block = have / groups.page_size[g];
+        if (have <= 0 || have == block * groups.page_size[g] || block >= groups.width[g]) continue;
+        const int x = groups.table[g][(long long)from_row * groups.width[g] + block];
+        __syncwarp();
+        if (lane < beams) groups.table[g][(long long)row * groups.width[g] + block] = x;
+      }
+      if (slots != nullptr) {
+        const int x = slots[from_row];
+        __syncwarp();
+        if (lane < beams) slots[row] = x;
+      }
+    }
+  }
+  // the copies
+  const long long total = (long long)copies * parts_of_copy, warps = (long long)gridDim.x * kCopyWarps;
+  const long long run = (total + warps - 1) / warps, at0 = ((long long)blockIdx.x * kCopyWarps + warp) * run, at1 = min(at0 + run, total);
+  if (at0 >= at1) return;
+  int copy = (int)(at0 / parts_of_copy), part = (int)(at0 - (long long)copy * parts_of_copy), which = 0, end = 0;
+  Moved m{};
+  for (long long u = at0; u < at1; ++u, ++part) {
+    if (part == parts_of_copy) { ++copy; part = 0; }
+    if (u == at0 || part == 0 || part == end) {                      // another storage
+      int lo = 0, hi = n_moved - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (first_part[mid] <= part) lo = mid; else hi = mid - 1;
+      }
+      which = lo;
+      m = moved[which];
+      end = which + 1 < n_moved ? first_part[which + 1] : parts_of_copy;
+    }
+    const Copy c = s_copy[(size_t)copy * kinds + (m.group >= 0 ? m.group : groups.n)];
+    if (c.fill == 0) continue;
+    const int at = part - first_part[which], plane = at / m.parts, piece = at - plane * m.parts;
+    const int bytes = m.group >= 0 ? (c.fill + m.unit_rows - 1) / m.unit_rows * m.unit_bytes : (int)min((long long)kPart, m.bytes - (long long)piece * kPart);
     char* base = m.base + plane * m.outer_stride + piece * m.part_stride;
-    const char* a = base + from * m.place_stride;
-    char* b = base + to * m.place_stride;
+    const char* a = base + c.from * m.place_stride;
+    char* b = base + c.to * m.place_stride;
     const uintptr_t odd = (uintptr_t)a | (uintptr_t)b | (uintptr_t)bytes;
     if ((odd & 15) == 0) copy_part<uint4>(b, a, bytes, lane);
     else if ((odd & 3) == 0) copy_part<unsigned>(b, a, bytes, lane);
@@ -618,47 +667,15 @@ beam_copy_kernel(const int* __restrict__ parents, const int* __restrict__ kv_len
   }
 }
 
-// The tables and slots follow: a CTA a request; a thread moves a column of a table at a time, so nothing is read after it was replaced.
-constexpr int kTableThreads = 128;
-__global__ void __launch_bounds__(kTableThreads)
-beam_tables_kernel(const int* __restrict__ parents, const int* __restrict__ kv_len, int* __restrict__ slots, Groups groups, int beams) {
-  pdl_launch_dependents();
-  pdl_wait();
-  __shared__ int s_parents[kMaxBeams];
-  __shared__ short s_place[kMaxBeams], s_source[kMaxBeams];
-  __shared__ int s_column[kMaxBeams][kTableThreads];
-  const int first = blockIdx.x * beams, t = threadIdx.x;
-  work_out_places(parents + first, beams, beams, s_place, s_source, s_parents);
-  const int len = kv_len[first];
-  for (int g = 0; g < groups.n; ++g) {
-    const int have = len / groups.stride[g], ps = groups.page_size[g], fill = have % ps, last = have / ps;
-    const int used = min(groups.width[g], have / ps + (fill > 0));
-    int* table = groups.table[g] + (long long)first * groups.width[g];
-    for (int c = t; c < used; c += kTableThreads) {
-      for (int w = 0; w < beams; ++w) s_column[w][t] = table[(long long)w * groups.width[g] + c];
-      for (int w = 0; w < beams; ++w) {
-        const int p = s_parents[w];
-        const int from = c == last && fill > 0 ? s_place[w] : p >= 0 && p < beams ? p : w;
-        if (from != w) table[(long long)w * groups.width[g] + c] = s_column[from][t];
-      }
-    }
-  }
-  if (slots != nullptr && t < 32) {
-    const int mine = t < beams ? slots[first + s_place[t]] : 0;
-    __syncwarp();
-    if (t < beams) slots[first + t] = mine;
-  }
-}
-
 }  // namespace
 
 ILB_EXPORT int ilb_beam_reorder(const int* parents, const int* kv_len, int* slots, const void* moved, const int* first_part, int n_moved,
-                                int parts_of_copy, int num_slots, const long long* tables, const int* sizes, int n_groups, int requests, int beams,
-                                int sms, cudaStream_t stream) {
+                                int parts_of_copy, int num_slots, const long long* tables, const int* sizes, int n_groups, int* turns, int requests,
+                                int beams, int sms, cudaStream_t stream) {
   const long long rows = (long long)requests * beams;
   ILB_REQUIRE(requests >= 0 && beams > 0 && beams <= kMaxBeams && rows <= kMaxRows && n_groups >= 0 && n_groups <= kMaxGroups && n_moved >= 0,
               "beam_reorder: bad sizes (up to %d beams, %d rows and %d page groups)", kMaxBeams, kMaxRows, kMaxGroups);
-  if (requests == 0) return 0;
+  if (requests == 0 || beams == 1) return 0;                         // (a single beam goes on where it is)
   Groups g{};
   g.n = n_groups;
   for (int i = 0; i < n_groups; ++i) {
@@ -669,15 +686,16 @@ ILB_EXPORT int ilb_beam_reorder(const int* parents, const int* kv_len, int* slot
     g.pages[i] = sizes[4 * i + 3];
     ILB_REQUIRE(g.width[i] > 0 && g.page_size[i] > 0 && g.stride[i] > 0 && g.pages[i] > 0, "beam_reorder: bad sizes of page group %d", i);
   }
-  if (n_moved > 0 && beams > 1) {
-    launch(beam_copy_kernel, dim3(2 * sms), dim3(256), 0, stream, parents, kv_len, (const int*)slots, (const Moved*)moved, first_part, n_moved,
-           parts_of_copy, num_slots, g, (int)rows, beams);
-    const int rc = check_launch("beam_reorder");
-    if (rc) return rc;
-  }
-  launch(beam_tables_kernel, dim3((unsigned)requests), dim3(kTableThreads), 0, stream, parents, kv_len, slots, g, beams);
+  static OncePerDevice once;
+  constexpr int kMostShared = kMaxRows * 4 + kMaxRows * 4 + kMaxRows * (kMaxGroups + 1) * (int)sizeof(Copy);
+  if (once.run([] { return cudaFuncSetAttribute(beam_reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared); }) != cudaSuccess)
+    return check_launch("beam_reorder");
+  const size_t smem = rows * 4 + (size_t)requests * 4 + rows * (n_groups + 1) * sizeof(Copy);
+  launch(beam_reorder_kernel, dim3(2 * sms), dim3(kCopyThreads), smem, stream, parents, kv_len, slots, (const Moved*)moved, first_part, n_moved,
+         parts_of_copy, num_slots, g, (int)rows, beams, turns);
   return check_launch("beam_reorder");
 }
+ILB_PACKED(ilb_beam_reorder)
 
 // ------------------------------------------------------------------ step_build
 namespace {
@@ -685,128 +703,134 @@ namespace {
 constexpr int kBuildThreads = 1024;
 constexpr int kMaxSequences = 8192;
 constexpr int kMaxTokens = 1 << 17;    // (their sum over all sequences stays below 2^31)
+constexpr int kBuildTokens = 2048;     // tokens of a CTA, up to a cluster of eight
 
+struct PageSource {
+  int* table; const int* free_list; const int* used; int* used_out;
+  int width, n_free, page_size, stride, page_shift, stride_shift;    // shifts: -1 where the number is no power of two
+};
 struct Build {
   const int* fresh; const int* cached;                               // [S] tokens brought, tokens in the cache before
   int* kv_len; int* positions; int* seq_of_token; int* cu_q;         // [S], [T], [T], [S + 1]
   long long* slot_map;                                               // [T] or null: of group 0
   int* refused;
-  int n_seqs, room;                                                  // room: elements of positions
-  int n_groups;
-  int* table[kMaxGroups]; const int* free_list[kMaxGroups]; const int* used[kMaxGroups]; int* used_out[kMaxGroups];
-  int width[kMaxGroups], n_free[kMaxGroups], page_size[kMaxGroups], stride[kMaxGroups];
+  int n_seqs, room, n_groups, ctas;                                  // room: elements of positions
+  PageSource pages[kMaxGroups];
 };
 enum Refusal : int { kTooManyTokens = 1, kNoPages = 2, kTableFull = 4, kBadLength = 8 };
 
-__device__ __forceinline__ int blocks_of(int tokens, int stride, int page_size) { return (tokens / stride + page_size - 1) / page_size; }
+__device__ __forceinline__ int over(int x, int by, int shift) { return shift >= 0 ? x >> shift : x / by; }
+__device__ __forceinline__ int blocks_of(int tokens, const PageSource& g) { return over(over(tokens, g.stride, g.stride_shift) + g.page_size - 1, g.page_size, g.page_shift); }
 
-// Exclusive sums of v[0 .. n) in place (shared memory), the total in *total; the whole block takes part.
-__device__ void scan_in_place(int* v, int n, int* warps, int* total) {
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, each = (n + kBuildThreads - 1) / kBuildThreads;
-  int mine = 0;
-  for (int i = 0; i < each; ++i) { const int at = t * each + i; if (at < n) mine += v[at]; }
-  int sum = mine;
+// Sums of v over the threads before this one; *total: of all threads.  `warps` [32] of shared memory is the caller's until the next barrier.
+__device__ __forceinline__ int sum_before(int v, int* warps, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int sum = v;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) { const int x = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += x; }
-  __syncthreads();
   if (lane == 31) warps[warp] = sum;
   __syncthreads();
-  if (warp == 0) {
-    int x = warps[lane];
+  int all = warps[lane];
 #pragma unroll
-    for (int o = 1; o < 32; o *= 2) { const int y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
-    warps[lane] = x;
-  }
-  __syncthreads();
-  int before = sum - mine + (warp > 0 ? warps[warp - 1] : 0);
-  for (int i = 0; i < each; ++i) {
-    const int at = t * each + i;
-    if (at < n) { const int x = v[at]; v[at] = before; before += x; }
-  }
-  if (t == kBuildThreads - 1) *total = warps[31];
-  __syncthreads();
+  for (int o = 1; o < 32; o *= 2) { const int x = __shfl_up_sync(0xffffffffu, all, o); if (lane >= o) all += x; }
+  *total = __shfl_sync(0xffffffffu, all, 31);
+  const int before = __shfl_sync(0xffffffffu, all, warp - 1 < 0 ? 0 : warp - 1);
+  return sum - v + (warp > 0 ? before : 0);
 }
 
-__global__ void __launch_bounds__(kBuildThreads) step_build_kernel(Build p) {
+// Every CTA of the cluster (or the only one) works out where each sequence's tokens and pages start; the first writes what there is once a sequence, each its
+// share of the tokens.  Nothing is written before all have read what they need, so that lengths and counters may be replaced in place.
+__global__ void __launch_bounds__(kBuildThreads) step_build_kernel(const __grid_constant__ Build p) {
   pdl_launch_dependents();
   pdl_wait();
   extern __shared__ int s_mem[];
-  const int S = p.n_seqs, t = threadIdx.x;
+  const int S = p.n_seqs, t = threadIdx.x, rank = p.ctas > 1 ? (int)cluster_rank() : 0;
   int* s_start = s_mem;                                              // [S] first token of a sequence
   int* s_cached = s_mem + S;                                         // [S]
-  int* s_pages = s_mem + 2 * S;                                      // [S] of a group: pages taken before the sequence's
-  __shared__ int s_warps[32], s_total, s_need[kMaxGroups], s_refused;
+  int* s_first = s_mem + 2 * S;                                      // [n_groups][S] a group's pages taken before the sequence's
+  __shared__ int s_warps[2][32], s_refused;
   if (t == 0) s_refused = 0;
   __syncthreads();
-  int wrong = 0;
-  for (int s = t; s < S; s += kBuildThreads) {
-    const int n = p.fresh[s], c = p.cached[s];
-    if (n < 0 || c < 0 || (long long)n + c > 0x7fffffffll) wrong |= kBadLength;
-    if (n > p.room) wrong |= kTooManyTokens;
-    s_start[s] = n;
-    s_cached[s] = c;
-    for (int g = 0; g < p.n_groups; ++g)
-      if (!(wrong & kBadLength) && blocks_of(c + n, p.stride[g], p.page_size[g]) > p.width[g]) wrong |= kTableFull;
+  int wrong = 0, carry = 0, taken[kMaxGroups], turn = 0, total;
+#pragma unroll
+  for (int g = 0; g < kMaxGroups; ++g) taken[g] = 0;
+  for (int s0 = 0; s0 < S; s0 += kBuildThreads) {
+    const int s = s0 + t;
+    int n = 0, c = 0;
+    if (s < S) { n = p.fresh[s]; c = p.cached[s]; }
+    if (n < 0 || c < 0 || (long long)n + c > 0x7fffffffll - (1 << 20)) { wrong |= kBadLength; n = c = 0; }
+    if (n > p.room) { wrong |= kTooManyTokens; n = 0; }              // (so that no sum overflows)
+    const int before = carry + sum_before(n, s_warps[turn], &total);
+    turn ^= 1;
+    carry += total;
+    if (s < S) { s_start[s] = before; s_cached[s] = c; }
+#pragma unroll
+    for (int g = 0; g < kMaxGroups; ++g) {
+      if (g >= p.n_groups) break;
+      const int want = blocks_of(c + n, p.pages[g]);
+      if (want > p.pages[g].width) wrong |= kTableFull;
+      const int first = taken[g] + sum_before(s < S ? want - blocks_of(c, p.pages[g]) : 0, s_warps[turn], &total);
+      turn ^= 1;
+      taken[g] += total;
+      if (s < S) s_first[g * S + s] = first;
+    }
+  }
+  if (carry > p.room) wrong |= kTooManyTokens;
+#pragma unroll
+  for (int g = 0; g < kMaxGroups; ++g) {
+    if (g >= p.n_groups) break;
+    const int used = *p.pages[g].used;
+    if (used < 0 || used > p.pages[g].n_free || taken[g] > p.pages[g].n_free - used) wrong |= kNoPages;
+    taken[g] += used;                                                // (behind the step)
   }
   if (wrong) atomicOr(&s_refused, wrong);
   __syncthreads();
-  if (s_refused) {                     // (sums of what was refused could overflow)
-    if (t == 0) atomicOr(p.refused, s_refused);
+  const bool refused = s_refused != 0;
+  auto start_of = [&](int s) { return s < S ? s_start[s] : carry; };
+  // new pages: read here (the counters are replaced below), written by the first CTA
+  if (!refused && rank == 0) {
+    for (int g = 0; g < p.n_groups; ++g) {
+      const PageSource& x = p.pages[g];
+      const int used = *x.used;
+      for (int s = t >> 5; s < S; s += kBuildThreads / 32) {
+        const int c = s_cached[s], had = blocks_of(c, x), want = blocks_of(c + start_of(s + 1) - s_start[s], x), first = s_first[g * S + s];
+        for (int b = had + (t & 31); b < want; b += 32) x.table[(long long)s * x.width + b] = x.free_list[used + first + b - had];
+      }
+    }
+  }
+  const int used0 = p.n_groups > 0 ? *p.pages[0].used : 0;
+  if (p.ctas > 1) cluster_sync_all();
+  else __syncthreads();
+  if (refused) {
+    if (t == 0 && rank == 0) atomicOr(p.refused, s_refused);
     return;
   }
-  scan_in_place(s_start, S, s_warps, &s_total);
-  const int total = s_total;
-  __syncthreads();
-  auto brought = [&](int s) { return (s + 1 < S ? s_start[s + 1] : total) - s_start[s]; };
-  if (t == 0 && total > p.room) s_refused = kTooManyTokens;
-  for (int g = 0; g < p.n_groups; ++g) {
-    for (int s = t; s < S; s += kBuildThreads)
-      s_pages[s] = blocks_of(s_cached[s] + brought(s), p.stride[g], p.page_size[g]) - blocks_of(s_cached[s], p.stride[g], p.page_size[g]);
-    __syncthreads();
-    scan_in_place(s_pages, S, s_warps, &s_need[g]);
+  if (rank == 0) {
+    for (int s = t; s < S; s += kBuildThreads) {
+      p.kv_len[s] = s_cached[s] + start_of(s + 1) - s_start[s];
+      p.cu_q[s] = s_start[s];
+    }
     if (t == 0) {
-      const int used = *p.used[g];
-      if (used < 0 || used > p.n_free[g] || s_need[g] > p.n_free[g] - used) s_refused |= kNoPages;
+      p.cu_q[S] = carry;
+#pragma unroll
+      for (int g = 0; g < kMaxGroups; ++g) if (g < p.n_groups) *p.pages[g].used_out = taken[g];
     }
-    __syncthreads();
   }
-  if (s_refused) {
-    if (t == 0) atomicOr(p.refused, s_refused);
-    return;
-  }
-  for (int g = 0; g < p.n_groups; ++g) {
-    if (p.n_groups > 1) {              // (the last group's sums are there)
-      for (int s = t; s < S; s += kBuildThreads)
-        s_pages[s] = blocks_of(s_cached[s] + brought(s), p.stride[g], p.page_size[g]) - blocks_of(s_cached[s], p.stride[g], p.page_size[g]);
-      __syncthreads();
-      scan_in_place(s_pages, S, s_warps, &s_total);
-    }
-    const int used = *p.used[g];
-    for (int s = t >> 5; s < S; s += kBuildThreads / 32) {
-      const int had = blocks_of(s_cached[s], p.stride[g], p.page_size[g]), want = blocks_of(s_cached[s] + brought(s), p.stride[g], p.page_size[g]);
-      for (int b = had + (t & 31); b < want; b += 32) p.table[g][(long long)s * p.width[g] + b] = p.free_list[g][used + s_pages[s] + b - had];
-    }
-    __syncthreads();
-    if (t == 0) *p.used_out[g] = used + s_need[g];
-  }
-  __syncthreads();                     // (the slot map reads the tables that this CTA wrote)
-  for (int s = t; s < S; s += kBuildThreads) {
-    p.kv_len[s] = s_cached[s] + brought(s);
-    p.cu_q[s] = s_start[s];
-  }
-  if (t == 0) p.cu_q[S] = total;
-  for (int i = t; i < total; i += kBuildThreads) {
+  for (int i = rank * kBuildThreads + t; i < carry; i += p.ctas * kBuildThreads) {
     int lo = 0, hi = S - 1;            // the last sequence that starts at or before the token
+    if (carry == S && s_start[i] == i && start_of(i + 1) == i + 1) lo = hi = i;      // (the i-th token is sequence i's only one, as in a decode step)
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
       if (s_start[mid] <= i) lo = mid; else hi = mid - 1;
     }
-    const int pos = s_cached[lo] + i - s_start[lo];
+    const int c = s_cached[lo], pos = c + i - s_start[lo];
     p.positions[i] = pos;
     p.seq_of_token[i] = lo;
     if (p.slot_map != nullptr) {
-      const int page = p.table[0][(long long)lo * p.width[0] + pos / p.page_size[0]];
-      p.slot_map[i] = page < 0 ? -1 : (long long)page * p.page_size[0] + pos % p.page_size[0];
+      const PageSource& x = p.pages[0];
+      const int block = over(pos, x.page_size, x.page_shift), had = blocks_of(c, x);
+      const int page = block < had ? x.table[(long long)lo * x.width + block] : x.free_list[used0 + s_first[lo] + block - had];
+      p.slot_map[i] = page < 0 ? -1 : (long long)page * x.page_size + pos - block * x.page_size;
     }
   }
 }
@@ -819,25 +843,26 @@ ILB_EXPORT int ilb_step_build(const int* fresh, const int* cached, int* kv_len, 
   ILB_REQUIRE(n_seqs >= 0 && n_seqs <= kMaxSequences && room >= 0 && room <= kMaxTokens && n_groups >= 0 && n_groups <= kMaxGroups,
               "step_build: bad sizes (up to %d sequences, %d tokens and %d page groups)", kMaxSequences, kMaxTokens, kMaxGroups);
   if (n_seqs == 0) return 0;
-  Build p{fresh, cached, kv_len, positions, seq_of_token, cu_q, slot_map, refused, n_seqs, room, n_groups};
+  Build p{fresh, cached, kv_len, positions, seq_of_token, cu_q, slot_map, refused, n_seqs, room, n_groups, 1};
+  auto shift_of = [](int x) { int n = 0; while ((1 << n) < x) ++n; return (1 << n) == x ? n : -1; };
   for (int g = 0; g < n_groups; ++g) {
     const long long* x = pages + 8 * g;
-    p.table[g] = (int*)(uintptr_t)x[0];
-    p.free_list[g] = (const int*)(uintptr_t)x[1];
-    p.used[g] = (const int*)(uintptr_t)x[2];
-    p.used_out[g] = (int*)(uintptr_t)x[3];
-    p.width[g] = (int)x[4];
-    p.n_free[g] = (int)x[5];
-    p.page_size[g] = (int)x[6];
-    p.stride[g] = (int)x[7];
-    ILB_REQUIRE(p.width[g] > 0 && p.n_free[g] >= 0 && p.page_size[g] > 0 && p.stride[g] > 0, "step_build: bad sizes of page group %d", g);
+    PageSource& to = p.pages[g];
+    ILB_REQUIRE(x[4] > 0 && x[4] < (1 << 30) && x[5] >= 0 && x[5] < (1ll << 31) && x[6] > 0 && x[6] <= (1 << 20) && x[7] > 0 && x[7] <= (1 << 20),
+                "step_build: bad sizes of page group %d", g);
+    to = PageSource{(int*)(uintptr_t)x[0], (const int*)(uintptr_t)x[1], (const int*)(uintptr_t)x[2], (int*)(uintptr_t)x[3], (int)x[4], (int)x[5], (int)x[6],
+                    (int)x[7], shift_of((int)x[6]), shift_of((int)x[7])};
   }
-  ILB_REQUIRE(slot_map == nullptr || (n_groups > 0 && p.stride[0] == 1), "step_build: a slot map needs a group with a row per token");
+  ILB_REQUIRE(slot_map == nullptr || (n_groups > 0 && p.pages[0].stride == 1), "step_build: a slot map needs a group with a row per token");
+  const size_t smem = (size_t)n_seqs * 4 * (2 + n_groups);
+  ILB_REQUIRE(smem <= 220 * 1024, "step_build: %d sequences with %d page groups do not fit a CTA's memory", n_seqs, n_groups);
   static OncePerDevice once;
-  if (once.run([] { return cudaFuncSetAttribute(step_build_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * kMaxSequences * 4); }) != cudaSuccess)
+  if (once.run([] { return cudaFuncSetAttribute(step_build_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024); }) != cudaSuccess)
     return check_launch("step_build");
-  launch(step_build_kernel, dim3(1), dim3(kBuildThreads), (size_t)n_seqs * 12, stream, p);
+  while (p.ctas < 8 && room > p.ctas * kBuildTokens) p.ctas *= 2;
+  launch_cluster(step_build_kernel, dim3(p.ctas), dim3(kBuildThreads), smem, stream, p.ctas, p);
   return check_launch("step_build");
 }
+ILB_PACKED(ilb_step_build)
 
 ILB_DEFINE_LAST_ERROR()

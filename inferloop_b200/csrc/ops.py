@@ -72,7 +72,10 @@ _SIGNATURES = {
     "ilb_kv4_attention_simple": "ppippppiiiifiiiiiipp",
     "ilb_kv4_attention_rows": "ppippppiiiifiiiiiiiipipqpqpp",
     "ilb_attention_beams": "ppi" + "pppp" + "iiii" + "f" + "iiiii" + "qq" + "pip",
-    "ilb_beam_select": "piq" + "ppppp" + "iiii" + "ppp",
+    "ilb_beam_keep": "pppi" + "pi" + "ppppp" + "iifi" + "pppppp" + "iip",
+    "ilb_beam_reorder": "ppp" + "ppiii" + "ppip" + "iiip",
+    "ilb_step_build": "pppppppp" + "iipip",
+    "ilb_beam_select": "piq" + "ppppp" + "iiii" + "pp",
 }
 
 
@@ -123,23 +126,24 @@ def _same_device(what: str, *tensors) -> None:
             raise KernelError(f"{what}: tensors on {where} and {t.device}")
 
 
-class _on_device:
-    """The tensors' device as the current one while a kernel is launched (a launch goes to the current device, whatever its stream); nothing is
-    asked of the driver where it is current already."""
+_current_device = torch._C._cuda_getDevice
 
-    __slots__ = ("index", "before")
 
-    def __init__(self, index: int) -> None:
-        self.index = index
+def _call_on(index: int, module: str, fn: str, *args) -> None:
+    """`_call` with the tensors' device as the current one (a launch goes to the current device, whatever its stream)."""
+    if _current_device() == index:
+        _call(module, fn, *args)
+        return
+    with torch.cuda.device(index):
+        _call(module, fn, *args)
 
-    def __enter__(self) -> None:
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
 
-    def __exit__(self, *exc) -> None:
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+def _ready(index: int, dtype: torch.dtype, *tensors) -> bool:
+    """Whether all tensors are contiguous ones of `dtype` on the CUDA device `index`."""
+    for t in tensors:
+        if t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():
+            return False
+    return True
 
 
 def _i(v) -> ctypes.c_int:
@@ -1272,7 +1276,6 @@ BEAM_MAX_BEST = 64         # candidates that a request's beams are asked for
 BEAM_MAX_ROWS = 1024       # rows (requests times beams) of a reordering
 BEAM_MAX_GROUPS = 8        # page groups of a reordering or of a step
 _BEAM_SCRATCH: dict = {}   # (device index, stream) -> the scratch of selections there
-_BEAM_PLANS: dict = {}     # sizes of a selection -> (8-byte words of keys, sums) that it needs
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, parents: torch.Tensor, tokens: torch.Tensor, out_scores: torch.Tensor,
@@ -1282,10 +1285,14 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, parents: torch.Tenso
     score + log softmax(logits), best first; equal ones by the higher logit, then the lower beam, then the lower token.  A logit of -inf is
     no candidate, nor is anything of a beam whose score is not finite; a row with NaN or +inf brings nothing and is flagged in
     `bad` [R * W].  Where fewer than k are found the rest is beam -1, token -1, score -inf."""
-    _need(logits, "beam_select logits", contiguous=False)
-    for t, w, dt in ((scores, "scores", torch.float32), (parents, "parents", torch.int32), (tokens, "tokens", torch.int32),
-                     (out_scores, "new scores", torch.float32), (bad, "flags", torch.int32)):
-        _need(t, "beam_select " + w, dt)
+    index = logits.get_device()
+    if index < 0 or not (_ready(index, _INT32, parents, tokens) and _ready(index, torch.float32, scores, out_scores)) \
+            or (bad is not None and not _ready(index, _INT32, bad)):
+        _need(logits, "beam_select logits", contiguous=False)
+        for t, w, dt in ((scores, "scores", torch.float32), (parents, "parents", torch.int32), (tokens, "tokens", torch.int32),
+                         (out_scores, "new scores", torch.float32), (bad, "flags", torch.int32)):
+            _need(t, "beam_select " + w, dt)
+        _same_device("beam_select", logits, scores, parents, tokens, out_scores, bad)
     if logits.dim() != 2 or scores.dim() != 2 or parents.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise KernelError("beam_select: logits must be [rows, vocabulary] with a row's elements side by side, scores [requests, beams], "
                           "parents [requests, candidates]")
@@ -1295,31 +1302,21 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, parents: torch.Tenso
         raise KernelError("beam_select: logits, scores and outputs do not agree")
     if not (0 < W <= BEAM_MAX and 0 < k <= BEAM_MAX_BEST and vocab > 0):
         raise KernelError(f"beam_select: up to {BEAM_MAX} beams and {BEAM_MAX_BEST} candidates, found {W} and {k} over a vocabulary of {vocab}")
-    _same_device("beam_select", logits, scores, parents, tokens, out_scores, bad)
     if R == 0:
         return
     stride = logits.stride(0) if rows > 1 else vocab
     if stride < vocab:
         raise KernelError("beam_select: rows of logits overlap")
-    code, index, stream = _code(logits), logits.device.index, _raw_stream(logits)
-    key = (code, rows, W, vocab, k, index)
-    plan = _BEAM_PLANS.get(key)
-    if plan is None:
-        lib, found = load_module("beam"), (ctypes.c_longlong(), ctypes.c_longlong())
-        if lib.ilb_beam_select_plan(_i(code), _i(rows), _i(vocab), _i(k), *map(ctypes.byref, found)) != 0:
-            raise KernelError(lib.ilb_last_error().decode())
-        plan = _BEAM_PLANS[key] = (found[0].value, found[1].value)
-    need = 8 * (plan[0] + plan[1])
+    code, stream = _code(logits), torch._C._cuda_getCurrentRawStream(index)
+    need = rows * -(-vocab // 2048) * 32 * 8             # (maximum and sum of every segment of 64 logits)
     # (one scratch per device and stream; a graph that is being recorded gets its own, which its memory pool keeps)
     held = None if _recording() else _BEAM_SCRATCH.get((index, stream))
     if held is None or held.numel() < need:
         held = torch.empty(need, dtype=torch.uint8, device=logits.device)
         if not _recording():
             _BEAM_SCRATCH[index, stream] = held
-    at = held.data_ptr()
-    with _on_device(index):
-        _call("beam", "ilb_beam_select", logits.data_ptr(), code, stride, scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), out_scores.data_ptr(),
-              0 if bad is None else bad.data_ptr(), R, W, vocab, k, at, at + 8 * plan[0], stream)
+    _call_on(index, "beam", "ilb_beam_select", logits.data_ptr(), code, stride, scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+             out_scores.data_ptr(), 0 if bad is None else bad.data_ptr(), R, W, vocab, k, held.data_ptr(), stream)
 
 
 @dataclass
@@ -1371,12 +1368,15 @@ def beam_keep(parents: torch.Tensor, tokens: torch.Tensor, scores: torch.Tensor,
         raise KernelError("beam_keep: candidates and what is kept do not agree")
     if not (0 <= step < min(int(last), steps)) or not 0 < W <= BEAM_MAX or not 0 < k <= BEAM_MAX_BEST:
         raise KernelError(f"beam_keep: step {step} of {last}, {steps} kept, {W} beams, {k} candidates")
-    _same_device("beam_keep", parents, tokens, scores, stops, track.scores, track.past_parents, track.done)
-    with _on_device(parents.device.index):
-        _call("beam", "ilb_beam_keep", _ptr(parents), _ptr(tokens), _ptr(scores), _i(k), _ptr(stops), _i(0 if stops is None else stops.numel()),
-              _ptr(track.parents), _ptr(track.tokens), _ptr(track.scores), _ptr(track.past_parents[step]), _ptr(track.past_tokens[step]), _i(step),
-              _i(last), _f(length_penalty), _i(1 if early_stopping else 0), _ptr(track.done_scores), _ptr(track.done_steps), _ptr(track.done_parents),
-              _ptr(track.done_tokens), _ptr(track.done_count), _ptr(track.done), _i(R), _i(W), _stream(parents))
+    _same_device("beam_keep", parents, tokens, scores, stops, track.scores, track.parents, track.tokens, track.past_parents, track.past_tokens,
+                 track.done_scores, track.done_steps, track.done_parents, track.done_tokens, track.done_count, track.done)
+    index = parents.get_device()
+    at = [t.data_ptr() for t in (track.parents, track.tokens, track.scores, track.past_parents, track.past_tokens, track.done_scores, track.done_steps,
+                                 track.done_parents, track.done_tokens, track.done_count, track.done)]
+    past = 4 * step * R * W
+    _call_on(index, "beam", "ilb_beam_keep", parents.data_ptr(), tokens.data_ptr(), scores.data_ptr(), k, 0 if stops is None else stops.data_ptr(),
+             0 if stops is None else stops.numel(), *at[:3], at[3] + past, at[4] + past, step, int(last), length_penalty, 1 if early_stopping else 0, *at[5:],
+             R, W, torch._C._cuda_getCurrentRawStream(index))
 
 
 class BeamState:
@@ -1429,6 +1429,8 @@ class BeamState:
         self.parts, self.n = at, len(records)
         self.records = torch.frombuffer(bytearray(b"".join(records) or bytes(64)), dtype=torch.uint8).to(self.device)
         self.first = torch.tensor(first or [0], dtype=torch.int32).to(self.device)
+        self.turns = torch.zeros(1, dtype=torch.int32, device=self.device)        # tickets of a launch, zero between launches
+        self.index, self.sms = self.device.index, _sm_count(self.device)
 
     def _check(self, x: torch.Tensor) -> None:
         _need(x, "beam state")
@@ -1443,31 +1445,34 @@ def beam_reorder(state: BeamState, parents: torch.Tensor, kv_len: torch.Tensor, 
     a row's own, as its slot is: a parent's first child takes those over, every other child takes the ones of a beam without children, in the order
     of both, and the parent's rows and state are copied there.  Before the call the last, partly filled pages of a request's rows and
     their slots must be different ones."""
-    _need(parents, "beam_reorder parents", torch.int32); _need(kv_len, "beam_reorder lengths", torch.int32); _need(slots, "beam_reorder slots", torch.int32)
+    index, tables = state.index, list(tables)
+    if not _ready(index, _INT32, parents, kv_len, *tables) or (slots is not None and not _ready(index, _INT32, slots)):
+        for t, w in ((parents, "parents"), (kv_len, "lengths"), (slots, "slots"), *((t, "block table") for t in tables)):
+            _need(t, "beam_reorder " + w, torch.int32)
+        _same_device("beam_reorder", state.records, parents, kv_len, slots, *tables)
     if parents.dim() != 2:
         raise KernelError("beam_reorder: parents must be [requests, beams]")
     R, W = parents.shape
-    rows = R * W
-    tables = list(tables)
-    if len(tables) != len(state.sizes):
-        raise KernelError(f"beam_reorder: {len(tables)} block tables for {len(state.sizes)} page groups")
-    for t in tables:
-        _need(t, "beam_reorder block table", torch.int32)
-        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] == 0:
-            raise KernelError(f"beam_reorder: a block table {tuple(t.shape)} for {rows} rows")
+    rows, n = R * W, len(tables)
+    if n != len(state.sizes):
+        raise KernelError(f"beam_reorder: {n} block tables for {len(state.sizes)} page groups")
+    where, sizes = [], []
+    for t, (pages, page_size, stride) in zip(tables, state.sizes):
+        shape = t.shape
+        if len(shape) != 2 or shape[0] != rows or shape[1] == 0:
+            raise KernelError(f"beam_reorder: a block table {tuple(shape)} for {rows} rows")
+        where.append(t.data_ptr())
+        sizes += (shape[1], page_size, stride, pages)
     if kv_len.numel() != rows or (slots is not None and slots.numel() != rows) or (slots is None and state.num_slots is not None):
         raise KernelError("beam_reorder: lengths or slots do not match the rows")
     if not 0 < W <= BEAM_MAX or rows > BEAM_MAX_ROWS:
         raise KernelError(f"beam_reorder: up to {BEAM_MAX} beams and {BEAM_MAX_ROWS} rows, found {W} and {rows}")
-    _same_device("beam_reorder", state.records, parents, kv_len, slots, *tables)
     if R == 0:
         return
-    n = len(tables)
-    where = (ctypes.c_longlong * max(n, 1))(*[t.data_ptr() for t in tables])
-    sizes = (ctypes.c_int * max(4 * n, 1))(*[x for t, (pages, page_size, stride) in zip(tables, state.sizes) for x in (t.shape[1], page_size, stride, pages)])
-    with _on_device(parents.device.index):
-        _call("beam", "ilb_beam_reorder", _ptr(parents), _ptr(kv_len), _ptr(slots), _ptr(state.records), _ptr(state.first), _i(state.n), _i(state.parts),
-              _i(state.num_slots or 0), where, sizes, _i(n), _i(R), _i(W), _i(_sm_count(parents.device)), _stream(parents))
+    where, sizes = (ctypes.c_longlong * max(n, 1))(*where), (ctypes.c_int * max(4 * n, 1))(*sizes)
+    _call_on(index, "beam", "ilb_beam_reorder", parents.data_ptr(), kv_len.data_ptr(), 0 if slots is None else slots.data_ptr(), state.records.data_ptr(),
+             state.first.data_ptr(), state.n, state.parts, state.num_slots or 0, ctypes.addressof(where), ctypes.addressof(sizes), n,
+             state.turns.data_ptr(), R, W, state.sms, torch._C._cuda_getCurrentRawStream(index))
 
 
 @dataclass
@@ -1490,32 +1495,37 @@ def step_build(new: torch.Tensor, cached: torch.Tensor, kv_len: torch.Tensor, po
     token's row among all rows of the first group's pages (page * page size + place; -1 where no page is held).  All or nothing: where
     a length is negative or too long, tokens, pages or columns do not suffice, nothing is written but a bit in `refused` [1] (1 tokens, 2 pages,
     4 columns, 8 lengths).  Entries behind the last token stay as they are."""
-    for t, w in ((new, "new tokens"), (cached, "cached tokens"), (kv_len, "lengths"), (positions, "positions"), (seq_of_token, "sequence indices"),
-                 (cu_q, "offsets"), (refused, "refusal flag")):
-        _need(t, "step_build " + w, torch.int32)
-    _need(slot_map, "step_build slot map", torch.int64)
+    index = new.get_device()
+    if index < 0 or not _ready(index, _INT32, new, cached, kv_len, positions, seq_of_token, cu_q, refused) \
+            or (slot_map is not None and not _ready(index, torch.int64, slot_map)):
+        for t, w in ((new, "new tokens"), (cached, "cached tokens"), (kv_len, "lengths"), (positions, "positions"), (seq_of_token, "sequence indices"),
+                     (cu_q, "offsets"), (refused, "refusal flag")):
+            _need(t, "step_build " + w, torch.int32)
+        _need(slot_map, "step_build slot map", torch.int64)
+        _same_device("step_build", new, cached, kv_len, positions, seq_of_token, cu_q, refused, slot_map)
     S, T, pages = new.numel(), positions.numel(), list(pages)
     if cached.numel() != S or kv_len.numel() != S or cu_q.numel() != S + 1 or seq_of_token.numel() != T or refused.numel() != 1 \
             or (slot_map is not None and slot_map.numel() != T):
         raise KernelError("step_build: arrays do not agree")
     if len(pages) > BEAM_MAX_GROUPS or (slot_map is not None and (not pages or pages[0].stride != 1)):
         raise KernelError(f"step_build: up to {BEAM_MAX_GROUPS} page groups, and a slot map of a group with a row per token")
-    _same_device("step_build", new, cached, kv_len, positions, seq_of_token, cu_q, refused, slot_map)
     held = []
     for g in pages:
         out = g.used if g.used_out is None else g.used_out
-        for t, w in ((g.table, "block table"), (g.free, "free list"), (g.used, "pages taken"), (out, "pages taken")):
-            _need(t, "step_build " + w, torch.int32)
+        if not _ready(index, _INT32, g.table, g.free, g.used, out):
+            for t, w in ((g.table, "block table"), (g.free, "free list"), (g.used, "pages taken"), (out, "pages taken")):
+                _need(t, "step_build " + w, torch.int32)
+            _same_device("step_build", new, g.table, g.free, g.used, out)
         if g.table.dim() != 2 or g.table.shape[0] != S or (g.table.shape[1] == 0 and S) or g.used.numel() != 1 or out.numel() != 1 or g.page_size <= 0 \
                 or g.stride <= 0:
             raise KernelError("step_build: a page group's arrays do not agree")
-        _same_device("step_build", new, g.table, g.free, g.used, out)
         held += [g.table.data_ptr(), g.free.data_ptr(), g.used.data_ptr(), out.data_ptr(), g.table.shape[1], g.free.numel(), g.page_size, g.stride]
     if S == 0:
         return
-    with _on_device(new.device.index):
-        _call("beam", "ilb_step_build", _ptr(new), _ptr(cached), _ptr(kv_len), _ptr(positions), _ptr(seq_of_token), _ptr(cu_q), _ptr(slot_map),
-              _ptr(refused), _i(S), _i(T), (ctypes.c_longlong * max(len(held), 1))(*held), _i(len(pages)), _stream(new))
+    held = (ctypes.c_longlong * max(len(held), 1))(*held)
+    _call_on(index, "beam", "ilb_step_build", new.data_ptr(), cached.data_ptr(), kv_len.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(),
+             cu_q.data_ptr(), 0 if slot_map is None else slot_map.data_ptr(), refused.data_ptr(), S, T, ctypes.addressof(held), len(pages),
+             torch._C._cuda_getCurrentRawStream(index))
 
 
 def attention_beams_supported(dtype: torch.dtype, cache_dtype: torch.dtype, nq: int, nkv: int, d: int, page_size: int) -> bool:
@@ -1531,10 +1541,13 @@ def attention_beams(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v
     type, float32 or bfloat16; `window` and `sink` as in `attention`; a token that sees no key (its pages are not held) gets zeros.  A value meets only
     the rows that see its key, whatever it is.  (`step`: its positions; sequence indices where the exact kernel takes the call; max_kv_len, if
     it has one, only decides how the keys are split.)"""
-    _need(q, "attention_beams q"); _need(out, "attention_beams out", q.dtype); _need(k_cache, "attention_beams keys", q.dtype)
-    _need(v_cache, "attention_beams values", q.dtype); _need(block_table, "attention_beams block table", torch.int32)
-    positions = step.positions
-    _need(positions, "attention_beams positions", torch.int32); _need(sink, "attention_beams sink", torch.float32)
+    positions, dtype, index = step.positions, q.dtype, q.get_device()
+    if index < 0 or not (_ready(index, dtype, q, out, k_cache, v_cache) and _ready(index, _INT32, block_table, positions)) \
+            or (sink is not None and not _ready(index, torch.float32, sink)):
+        _need(q, "attention_beams q"); _need(out, "attention_beams out", dtype); _need(k_cache, "attention_beams keys", dtype)
+        _need(v_cache, "attention_beams values", dtype); _need(block_table, "attention_beams block table", torch.int32)
+        _need(positions, "attention_beams positions", torch.int32); _need(sink, "attention_beams sink", torch.float32)
+        _same_device("attention_beams", q, out, k_cache, v_cache, block_table, positions, sink)
     rows, code = positions.numel(), _code(q)
     if nq <= 0 or nkv <= 0 or nq % nkv or d <= 0 or q.dim() != 2 or tuple(q.shape) != (rows, nq * d) or out.shape != q.shape or block_table.dim() != 2 \
             or block_table.shape[0] != rows or k_cache.dim() != 4 or k_cache.shape[1] != nkv or k_cache.shape[3] != d or v_cache.shape != k_cache.shape:
@@ -1543,26 +1556,25 @@ def attention_beams(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v
         raise KernelError(f"attention_beams: up to {BEAM_MAX} beams, found {beams}")
     if sink is not None and sink.numel() != nq:
         raise KernelError("attention_beams: one sink logit per query head")
-    _same_device("attention_beams", q, out, k_cache, v_cache, block_table, positions, sink)
     if rows == 0:
         return
     pages, _, page_size, _ = k_cache.shape
-    blocks, window, index = block_table.shape[1], window or 0, q.device.index
+    blocks, window = block_table.shape[1], window or 0
     if blocks == 0 or pages == 0 or page_size == 0:
         raise KernelError("attention_beams: the cache or the block table is empty")
-    with _on_device(index):
-        if not attention_beams_supported(q.dtype, k_cache.dtype, nq, nkv, d, page_size) or (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16:
-            _need(step.seq_of_token, "attention_beams sequence indices", torch.int32)
-            if step.seq_of_token.numel() != rows:
-                raise KernelError(f"attention_beams: {step.seq_of_token.numel()} sequence indices for {rows} rows")
+    if not attention_beams_supported(dtype, k_cache.dtype, nq, nkv, d, page_size) or (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+        _need(step.seq_of_token, "attention_beams sequence indices", torch.int32)
+        if step.seq_of_token.numel() != rows:
+            raise KernelError(f"attention_beams: {step.seq_of_token.numel()} sequence indices for {rows} rows")
+        with torch.cuda.device(index):
             paged_attention_simple(q, out, k_cache, v_cache, positions, step.seq_of_token, block_table, window, scale, nq, nkv, d, d, sink)
-            return
-        longest = min(getattr(step, "max_kv_len", None) or blocks * page_size, blocks * page_size)
-        if window:
-            longest = min(longest, abs(window) + page_size)
-        _call("attention_beams", "ilb_attention_beams", q.data_ptr(), out.data_ptr(), code, k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(),
-              block_table.data_ptr(), blocks, page_size, pages, window, scale, rows, beams, nq, nkv, d, nq * d, nq * d,
-              0 if sink is None else sink.data_ptr(), longest, _raw_stream(q))
+        return
+    longest = min(getattr(step, "max_kv_len", None) or blocks * page_size, blocks * page_size)
+    if window:
+        longest = min(longest, abs(window) + page_size)
+    _call_on(index, "attention_beams", "ilb_attention_beams", q.data_ptr(), out.data_ptr(), code, k_cache.data_ptr(), v_cache.data_ptr(),
+             positions.data_ptr(), block_table.data_ptr(), blocks, page_size, pages, window, scale, rows, beams, nq, nkv, d, nq * d, nq * d,
+             0 if sink is None else sink.data_ptr(), longest, torch._C._cuda_getCurrentRawStream(index))
 
 
 # --------------------------------------------------------------------------- tensor-core GEMM

@@ -308,7 +308,8 @@ def run_build(ops, new, cached, geometry, extra_tokens=0, in_place=False, spare=
 @pytest.mark.parametrize("new,cached,geometry", [
     ([1], [0], [(16, 1)]), ([1], [15], [(16, 1)]), ([1], [16], [(16, 1)]), ([0], [3], [(16, 1)]), ([0, 0], [0, 0], [(16, 1)]),
     ([5, 0, 1, 40, 0], [16, 7, 31, 0, 0], [(16, 1)]), ([1] * 33, list(range(33)), [(16, 1), (16, 16)]), ([3, 2000, 1], [5, 100, 4000], [(64, 1), (16, 4), (32, 1)]),
-    ([7, 1], [2, 2], []), ([2048] * 5, [0] * 5, [(128, 1)]), ([1] * 257, [i % 19 for i in range(257)], [(1, 1)]), ([9, 9], [3, 3], [(16, 3)])])
+    ([7, 1], [2, 2], []), ([2048] * 5, [0] * 5, [(128, 1)]), ([1] * 257, [i % 19 for i in range(257)], [(1, 1)]), ([9, 9], [3, 3], [(16, 3)]),
+    ([1, 0, 2, 1], [4, 4, 4, 4], [(16, 1)]), ([0, 0, 3], [15, 16, 17], [(16, 1), (24, 5)])])
 def test_build(ops, new, cached, geometry):
     run_build(ops, new, cached, geometry)
     run_build(ops, new, cached, geometry, extra_tokens=5, in_place=True, spare=0, width_more=0)
