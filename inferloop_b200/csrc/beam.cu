@@ -107,13 +107,14 @@ struct Ranked { u64 score, tie; };      // the score's order, then (logit's orde
 __device__ __forceinline__ bool above(const Ranked& a, const Ranked& b) { return a.score > b.score || (a.score == b.score && a.tie > b.tie); }
 
 // The first launch's sums of exponentials are of 32 bits.  A term at distance d below the maximum is off by (2^-23 + 2^-26) d (difference,
-// product, the constant's last bits) and 2^-22 (each of two exponentials), a segment's sum by 6 roundings (further sums are of 64 bits): with
-// sum p d <= ln(vocab) that is 3e-6 for up to 4 M tokens, and two beams are in order for sure when their scores differ by twice as much.  Where candidates of two beams that
+// product, the constant's last bits) and 2^-22 (each of three exponentials), a segment's sum by 6 roundings, that of ten segments by 11 more (further
+// sums are of 64 bits): with sum p d <= ln(vocab) that is 3.9e-6 for up to 4 M tokens, and two beams are in order for sure when their scores differ by twice as much.  Where candidates of two beams that
 // matter come closer, those beams' sums are taken once more, in 64 bits: about one step of one request in a thousand.
-constexpr double kUncertain = 6e-6;
+constexpr double kUncertain = 8e-6;
 constexpr int kJoinThreads = 1024, kJoinWarps = kJoinThreads / 32;
 constexpr int kListed = 1024;          // segments, and candidates, that are looked at in one go
 constexpr int kBestOfWarp = 4;
+constexpr int kHeld = 10;              // segments that a thread keeps (all of them at four beams of 151,936 tokens)
 constexpr int kMaxVocab = 1 << 22;
 
 // The sum over the block of a 64-bit value, the same for every thread.
@@ -138,7 +139,8 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
   __shared__ double s_base[kMaxBeams], s_top[kMaxBeams], s_part[kJoinWarps];      // score - lse or NaN (the beam brings no candidates), maximum
   __shared__ float s_m[kJoinWarps];
   __shared__ double s_sum[kJoinWarps];
-  __shared__ u64 s_best[kBestOfWarp * kJoinWarps];
+  __shared__ unsigned s_best[kBestOfWarp * kJoinWarps];
+  __shared__ signed char s_order[kMaxBeams];             // the beams that are alive
   __shared__ double s_border;
   __shared__ int s_segments, s_count, s_list[kListed];
   __shared__ unsigned s_live, s_close, s_bad;
@@ -151,6 +153,7 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
     const unsigned live = __ballot_sync(0xffffffffu, alive);
     if (lane == 0) { s_live = live; s_segments = 0; s_count = 0; s_close = 0; s_bad = 0; }
     if (lane < beams) s_base[lane] = (double)NAN;
+    if (alive) s_order[__popc(live & ((1u << lane) - 1))] = (signed char)lane;
   }
   __syncthreads();
   // the warps are dealt out to the beams that are alive: so many side by side, rounded up to a power of two
@@ -158,20 +161,30 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
   const int lives = __popc(live);
   int wide = 1;
   while (wide < lives) wide *= 2;
-  const int turn = warp & (wide - 1), share = warp / wide, shares = kJoinWarps / wide;
-  const int w = turn < lives ? (int)__fns(live, 0, turn + 1) : -1;
+  const int log_wide = __ffs(wide) - 1, turn = warp & (wide - 1), share = warp >> log_wide, shares = kJoinWarps >> log_wide;
+  const int w = turn < lives ? s_order[turn] : -1;
   const float2* mine = request + (long long)(w < 0 ? 0 : w) * segments;
-  // a row's maximum (the thread's best segment on the way), then its sum
+  // a row's maximum (the thread's best segment on the way), then its sum; the thread's first segments stay in registers
+  float2 held[kHeld];
+  const int s0 = w >= 0 ? share * 32 + lane : segments, step = shares * 32;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) held[i] = s0 + i * step < segments ? mine[s0 + i * step] : make_float2(-INFINITY, 0.f);
   float m = -INFINITY;
-  if (w >= 0)
-    for (int s = share * 32 + lane; s < segments; s += shares * 32) m = fmaxf(m, mine[s].x);
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) m = fmaxf(m, held[i].x);
+#pragma unroll 8
+  for (int s = s0 + kHeld * step; s < segments; s += step) m = fmaxf(m, mine[s].x);
   const float top = warp_max(m);
-  double sum = 0.0;
-  if (w >= 0) {
-    for (int s = share * 32 + lane; s < segments; s += shares * 32) {
-      const float2 p = mine[s];
-      sum += p.x == -INFINITY ? (double)p.y : (double)p.y * (double)expf(p.x - top);
-    }
+  auto term = [&](const float2& p) { return p.x == -INFINITY ? p.y : p.y * expf(p.x - top); };
+  float ten = 0.f;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) ten += term(held[i]);
+  double sum = (double)ten;
+  for (int s = s0 + kHeld * step; s < segments; s += 8 * step) {
+    float eight = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) eight += s + i * step < segments ? term(mine[s + i * step]) : 0.f;
+    sum += (double)eight;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -185,50 +198,62 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
     }
   }
   __syncthreads();
-  if (t < lives) {
-    const int beam = (int)__fns(live, 0, t + 1);
-    double all_top = -INFINITY, all = 0.0;
-    for (int i = t; i < kJoinWarps; i += wide) all_top = fmax(all_top, (double)s_m[i]);
-    for (int i = t; i < kJoinWarps; i += wide) all += s_m[i] > -INFINITY ? s_sum[i] * exp((double)s_m[i] - all_top) : s_sum[i];
-    const double base = (double)scores[(long long)r * beams + beam] - (all_top + log(all));
-    s_base[beam] = !isfinite(base) ? (double)NAN : base;
-    s_top[beam] = all_top;
-    if (isnan(all)) atomicOr(&s_bad, 1u << beam);
+  if (warp < lives) {                  // a warp a beam: lane i has warp i's part of it
+    const int beam = s_order[warp];
+    const bool part = (lane & (wide - 1)) == warp;
+    const float all_top = warp_max(part ? s_m[lane] : -INFINITY);
+    double all = !part ? 0.0 : s_m[lane] > -INFINITY ? s_sum[lane] * (double)expf(s_m[lane] - all_top) : s_sum[lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if (lane == 0) {
+      const double base = (double)scores[(long long)r * beams + beam] - ((double)all_top + log(all));
+      s_base[beam] = !isfinite(base) ? (double)NAN : base;
+      s_top[beam] = (double)all_top;
+      if (isnan(all)) atomicOr(&s_bad, 1u << beam);
+    }
   }
   __syncthreads();
   if (bad != nullptr && t < beams) bad[(long long)r * beams + t] = s_bad >> t & 1;
   // the border: of every warp its threads' four best maxima, of those the k-th largest (at least half of the 32 warps have a beam, unless all are dead)
+  // In 32 bits, rounded down, so that what reaches the border in 64 bits is no fewer.
   {
-    u64 best = w >= 0 && m > -INFINITY && !isnan(s_base[w]) ? ordered(s_base[w] + (double)m + 0.0) : 0;
+    unsigned best = w >= 0 && m > -INFINITY && !isnan(s_base[w]) ? ordered(__double2float_rd(s_base[w] + (double)m)) : 0u;
 #pragma unroll
-    for (int size = 2; size <= 32; size *= 2) {
-#pragma unroll
-      for (int d = size / 2; d > 0; d /= 2) {
-        const u64 other = __shfl_xor_sync(0xffffffffu, best, d);
-        const bool larger = ((lane & d) == 0) == ((lane & size) == 0);
-        best = larger ? (best > other ? best : other) : (best < other ? best : other);
-      }
+    for (int i = 0; i < kBestOfWarp; ++i) {
+      const unsigned most = __reduce_max_sync(0xffffffffu, best);
+      if (lane == __ffs((int)__ballot_sync(0xffffffffu, best == most)) - 1) best = 0u;
+      if (lane == i) s_best[warp * kBestOfWarp + i] = most;
     }
-    if (lane < kBestOfWarp) s_best[warp * kBestOfWarp + lane] = best;
   }
   __syncthreads();
-  if (t < kBestOfWarp * kJoinWarps) {
-    const u64 key = s_best[t];
+  {                                    // eight threads a key
+    constexpr int keys = kBestOfWarp * kJoinWarps, threads = kJoinThreads / keys;
+    const int at = t / threads, first = t % threads;
+    const unsigned key = s_best[at];
     int larger = 0;
-    for (int i = 0; i < kBestOfWarp * kJoinWarps; ++i) larger += s_best[i] > key || (s_best[i] == key && i < t);
-    if (larger == k - 1) s_border = key == 0 ? -INFINITY : unordered(key);
+#pragma unroll
+    for (int i = 0; i < keys / threads; ++i) {
+      const int o = i * threads + first;
+      larger += s_best[o] > key || (s_best[o] == key && o < at);
+    }
+#pragma unroll
+    for (int o = threads / 2; o > 0; o >>= 1) larger += __shfl_xor_sync(0xffffffffu, larger, o);
+    if (larger == k - 1 && first == 0) s_border = key == 0u ? -INFINITY : (double)unordered(key);
   }
   __syncthreads();
   // segments, then logits, that reach it or come closer than the sums are certain
   const double border = s_border - kUncertain;
   if (w >= 0 && !isnan(s_base[w]) && m > -INFINITY && s_base[w] + (double)m >= border) {
-    for (int s = share * 32 + lane; s < segments; s += shares * 32) {
-      const float x = mine[s].x;
+    auto list = [&](float x, int s) {
       if (x > -INFINITY && s_base[w] + (double)x >= border) {
         const int at = atomicAdd(&s_segments, 1);
         if (at < kListed) s_list[at] = w * segments + s;
       }
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) list(held[i].x, s0 + i * step);
+#pragma unroll 8
+    for (int s = s0 + kHeld * step; s < segments; s += step) list(mine[s].x, s);
   }
   __syncthreads();
   const int listed = s_segments;
@@ -273,24 +298,26 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
   int n = s_count;
   if (listed <= kListed && n <= kListed) {
     for (int pass = 0; pass < 2; ++pass) {
-      // (the list's order depends on the threads' timing, the ranks do not)
+      // a warp a candidate (the list's order depends on the threads' timing, the ranks do not)
       unsigned close = 0;
-      for (int c = t; c < n; c += kJoinThreads) {
+      for (int c = warp; c < n; c += kJoinWarps) {
         const Ranked e = s_cand[c];
         const double score = unordered(e.score);
         const int beam = (int)(~(unsigned)e.tie / (unsigned)vocab);
         int rank = 0;
         unsigned near = 0;
-        for (int i = 0; i < n; ++i) {
+        for (int i = lane; i < n; i += 32) {
           const Ranked x = s_cand[i];
           rank += above(x, e);
           if (pass == 0 && fabs(unordered(x.score) - score) <= kUncertain) near |= 1u << (~(unsigned)x.tie / (unsigned)vocab);
         }
-        if (rank < k) put(rank, e);
+        rank = __reduce_add_sync(0xffffffffu, rank);
+        near = __reduce_or_sync(0xffffffffu, near);
+        if (rank < k && lane == 0) put(rank, e);
         if (rank <= k && (near & ~(1u << beam))) close |= near | 1u << beam;       // (of the k-th and the one behind it, both know)
       }
       if (pass == 1) break;
-      if (close) atomicOr(&s_close, close);
+      if (close && lane == 0) atomicOr(&s_close, close);
       __syncthreads();
       const unsigned unsure = s_close;
       if (unsure == 0) break;
