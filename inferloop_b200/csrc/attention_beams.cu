@@ -608,7 +608,7 @@ attention_beams_kernel(Params p) {
 
 // ------------------------------------------------------------------ float32
 constexpr int kExactTile = 2;          // units: a key a lane
-constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
 template <int D>
 constexpr int kTileF32 = kExactTile * kUnit * (D + 4 + D) * 4;      // (keys' rows are four longer: lanes read them side by side)
 
@@ -665,17 +665,18 @@ attention_beams_exact_kernel(Params p) {
     const int total = list_units(p, j, turn, list, D * 4);
     __syncthreads();                                     // (the ring is free)
     const int tiles = (total * parts + kExactTile - 1) / kExactTile;
-    auto load = [&](int tile) {                          // a warp a unit's keys or values
+    auto load = [&](int tile) {                          // a warp half of a unit's keys or values
       if (tile < tiles) {
-        const int which = warp >> 1;
+        const int which = warp >> 2, half = warp & 1;
         const Listed u = unit_of(j, list, tile * kExactTile + which, total, parts, kUnit * D * 4);
         if (u.beams != 0) {
+          const bool values = (warp & 2) != 0;
           const uint32_t at = ring_at + (tile % STAGES) * kTileBytes;
-          const char* from = (const char*)((warp & 1) ? p.v : p.k) + u.at;
-          const uint32_t to = (warp & 1) ? at + kValues + which * kUnit * D * 4 : at + which * kUnit * kRow, row_bytes = (warp & 1) ? D * 4 : kRow;
+          const char* from = (const char*)(values ? p.v : p.k) + u.at;
+          const uint32_t to = values ? at + kValues + which * kUnit * D * 4 : at + which * kUnit * kRow, row_bytes = values ? D * 4 : kRow;
 #pragma unroll
-          for (int i = 0; i < kUnit * PIECES / 32; ++i) {
-            const int c = i * 32 + lane, row = c / PIECES;
+          for (int i = 0; i < kUnit * PIECES / 64; ++i) {
+            const int c = (i * 2 + half) * 32 + lane, row = c / PIECES;
             cp_async_16(to + row * row_bytes + (c - row * PIECES) * 16, from + c * 16);
           }
         }
@@ -703,7 +704,7 @@ attention_beams_exact_kernel(Params p) {
       float s[RPW];
 #pragma unroll
       for (int k = 0; k < RPW; ++k) s[k] = 0.f;
-#pragma unroll 4
+#pragma unroll 8
       for (int d = 0; d < D; d += 4) {
         const float4 x = *reinterpret_cast<const float4*>(kr + d);
 #pragma unroll
@@ -726,32 +727,39 @@ attention_beams_exact_kernel(Params p) {
 #pragma unroll
         for (int e = 0; e < D / 32; ++e) o[k][e] *= corr;
       }
-      if (every == 0xffffffffu) {
-#pragma unroll 4
-        for (int n = 0; n < 32; ++n) {
-          float v[D / 32];
+      // (a unit that nobody sees, or that is not there, is passed over)
+      const int n0 = (any & 0xffffu) != 0 ? 0 : kUnit, n1 = (any >> kUnit) != 0 ? 2 * kUnit : kUnit;
+      float before[RPW][D / 32], odd = 0.f;              // odd: no number once an infinity or NaN was among the values
 #pragma unroll
-          for (int e = 0; e < D / 32; ++e) v[e] = vr[n * D + e * 32];
+      for (int k = 0; k < RPW; ++k)
 #pragma unroll
-          for (int k = 0; k < RPW; ++k) {
-            const float w = __shfl_sync(0xffffffffu, s[k], n);
+        for (int e = 0; e < D / 32; ++e) before[k][e] = o[k][e];
+#pragma unroll 8
+      for (int n = n0; n < n1; ++n) {
+        float v[D / 32];
 #pragma unroll
-            for (int e = 0; e < D / 32; ++e) o[k][e] = fmaf(w, v[e], o[k][e]);
-          }
+        for (int e = 0; e < D / 32; ++e) { v[e] = vr[n * D + e * 32]; odd = fmaf(v[e], 0.f, odd); }
+#pragma unroll
+        for (int k = 0; k < RPW; ++k) {
+          const float weight = __shfl_sync(0xffffffffu, s[k], n);
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) o[k][e] = fmaf(weight, v[e], o[k][e]);
         }
-      } else {                                           // a value meets only the rows that see it
-#pragma unroll 2
-        for (int n = 0; n < 32; ++n) {
-          if (!((any >> n) & 1)) continue;
-          float v[D / 32];
+      }
+      if (every != 0xffffffffu && __any_sync(0xffffffffu, odd != 0.f)) {
+        // once more: a value meets only the rows that see it
 #pragma unroll
-          for (int e = 0; e < D / 32; ++e) v[e] = vr[n * D + e * 32];
+        for (int k = 0; k < RPW; ++k)
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) o[k][e] = before[k][e];
+#pragma unroll 1
+        for (int n = n0; n < n1; ++n) {
 #pragma unroll
           for (int k = 0; k < RPW; ++k) {
-            const float w = __shfl_sync(0xffffffffu, s[k], n);
+            const float weight = __shfl_sync(0xffffffffu, s[k], n);
             if (!((seen[k] >> n) & 1)) continue;
 #pragma unroll
-            for (int e = 0; e < D / 32; ++e) o[k][e] = fmaf(w, v[e], o[k][e]);
+            for (int e = 0; e < D / 32; ++e) o[k][e] = fmaf(weight, vr[n * D + e * 32], o[k][e]);
           }
         }
       }
@@ -847,7 +855,7 @@ int run_exact(Params& p, int longest, cudaStream_t stream) {
 
 template <int D>
 int run_f32(Params& p, int longest, cudaStream_t stream) {
-  return min(p.beams, p.rows) * (p.nq / p.nkv) <= 16 ? run_exact<D, 4>(p, longest, stream) : run_exact<D, 8>(p, longest, stream);
+  return min(p.beams, p.rows) * (p.nq / p.nkv) <= 16 ? run_exact<D, 2>(p, longest, stream) : run_exact<D, 4>(p, longest, stream);
 }
 
 }  // namespace
