@@ -24,27 +24,14 @@
 #include <algorithm>
 #include <atomic>
 #include "common.cuh"
+#include "attention_beams.cuh"
 #include "packed.h"
 #include "sm100.cuh"
 
 using namespace ilb;
-using std::max;
-using std::min;
 namespace {
 
-constexpr int kMaxBeams = 32;
-constexpr int kUnit = 16;              // keys
 constexpr int kList = 64;              // pages that a ring lists at a time
-constexpr float kLog2e = 1.4426950408889634f;
-
-struct Params {
-  const void* q; void* out; const void* k; const void* v;
-  const int* positions; const int* table; const float* sink;
-  long long q_stride, out_stride;
-  int rows, beams, beams_of_chunk, chunks, max_blocks, page_size, num_pages, window, nq, nkv, split;
-  float scale_log2;                    // bfloat16: of the absolute value; the sign is in the queries
-  uint32_t flip, keep;                 // of queries' bits: signs, all (a scale of 0: none)
-};
 
 // A page that is listed: where its rows of the kv head lie (bytes from the cache's start), its first key, the beams that hold it.
 struct Listed { long long at; int key0; unsigned beams; };
@@ -61,108 +48,55 @@ __device__ __forceinline__ float power_of_two(float x) {
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// What a CTA works on, the same for both kinds of arithmetic.
-struct Job {
-  int first_row, beams;                // of this chunk: row of its first beam, beams
-  int kvh, group;                      // kv head, query heads of it
-  int lo_col, hi_col;                  // columns that some beam sees keys of
-  int key_lo, key_hi;                  // keys that some beam sees
-  int all_lo, all_hi;                  // keys that every beam sees
-  unsigned all_beams;                  // their bits
-  int lo, hi;                          // the keys of the lane's beam
-};
-
-// The keys [lo, hi) that row `row` sees.
-__device__ __forceinline__ void keys_of(const Params& p, int row, int* lo, int* hi) {
-  const int pos = p.positions[row];
-  const long long room = (long long)p.max_blocks * p.page_size;
-  *hi = pos < 0 ? 0 : (int)min((long long)pos + 1, room);
-  *lo = pos < 0 ? 0 : first_key(pos, p.window);
-}
-
-__device__ __forceinline__ Job make_job(const Params& p) {
-  Job j;
-  const int chunk = blockIdx.y / p.nkv, request = blockIdx.z;
-  j.kvh = blockIdx.y - chunk * p.nkv;
-  j.group = p.nq / p.nkv;
-  const int first = chunk * p.beams_of_chunk;
-  j.first_row = request * p.beams + first;
-  j.beams = max(min(min(p.beams_of_chunk, p.beams - first), p.rows - j.first_row), 0);
-  j.all_beams = j.beams == 32 ? 0xffffffffu : (1u << j.beams) - 1;
-  return j;
-}
-
-// The keys that its beams see: found when their positions have come.
-__device__ __forceinline__ void find_keys(const Params& p, Job& j) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0x7fffffff, hi = 0, all_lo = 0, all_hi = 0x7fffffff;
-  j.lo = j.hi = 0;
-  if (lane < j.beams) {
-    keys_of(p, j.first_row + lane, &j.lo, &j.hi);
-    all_lo = j.lo;
-    all_hi = j.hi;
-    if (j.hi > j.lo) lo = j.lo, hi = j.hi;
-  }
-  j.key_lo = __reduce_min_sync(0xffffffffu, lo);
-  j.key_hi = __reduce_max_sync(0xffffffffu, hi);
-  j.all_lo = __reduce_max_sync(0xffffffffu, all_lo);
-  j.all_hi = __reduce_min_sync(0xffffffffu, all_hi);
-  if (j.key_hi <= j.key_lo) j.key_lo = j.key_hi = 0;
-  j.lo_col = j.key_lo / p.page_size;
-  j.hi_col = (j.key_hi + p.page_size - 1) / p.page_size;
-}
-
-// A CTA's columns: rank + split * i.  A turn of a warp looks at 32 / (beams, rounded up to a power of two) of them at once, a lane a beam; the
-// pages of the first turns are asked for ahead of everything else, should the first column be the table's (with a window it is not known yet).
-constexpr int kTurns = 4;              // turns whose pages are on their way at a time
-struct Turn { int columns, c, w, rank, next; int page[kTurns]; };
+// The pages of the next columns: asked for four turns at a time, those of the first turns ahead of everything else, should the first column be the table's
+// (with a window it is not known yet).
+constexpr int kTurns = 4;
+struct Turn { Lanes lanes; int rank, next, base; bool asked; int page[kTurns]; };
 __device__ __forceinline__ void ask_pages(const Params& p, const Job& j, Turn& x, int lo_col, int hi_col) {
 #pragma unroll
   for (int n = 0; n < kTurns; ++n) {
-    const int column = lo_col + x.rank + p.split * ((x.next + n) * x.columns + x.c);
+    const int column = lo_col + x.rank + p.split * ((x.base + n) * x.lanes.columns + x.lanes.c);
     x.page[n] = -1;
-    if (x.w < j.beams && column < hi_col) x.page[n] = p.table[(long long)(j.first_row + x.w) * p.max_blocks + column];
+    if (x.lanes.w < j.beams && column < hi_col) x.page[n] = p.table[(long long)(j.first_row + x.lanes.w) * p.max_blocks + column];
   }
 }
 __device__ __forceinline__ Turn first_turn(const Params& p, const Job& j, int rank) {
-  const int lane = threadIdx.x & 31;
-  int wide = 1;
-  while (wide < j.beams) wide *= 2;
   Turn x;
-  x.columns = 32 / wide;
-  x.c = lane / wide;
-  x.w = lane - x.c * wide;
+  x.lanes = make_lanes(j);
   x.rank = rank;
-  x.next = 0;
-  if (p.window == 0) ask_pages(p, j, x, 0, p.max_blocks);
+  x.next = x.base = 0;
+  x.asked = p.window == 0;
+  if (x.asked) ask_pages(p, j, x, 0, p.max_blocks);
   return x;
 }
 __device__ __forceinline__ bool more_columns(const Params& p, const Job& j, const Turn& x) {
-  return j.lo_col + x.rank + p.split * (x.next * x.columns) < j.hi_col;
+  return j.lo_col + x.rank + p.split * (x.next * x.lanes.columns) < j.hi_col;
 }
 
 // Lists the pages of the CTA's next columns in `list` (the warp's own; all warps of a CTA make the same list) and returns how many there are.
 __device__ __forceinline__ int list_units(const Params& p, const Job& j, Turn& x, Listed* list, int row_bytes) {
-  const int lane = threadIdx.x & 31, wide = 32 / x.columns;
+  const int lane = threadIdx.x & 31;
   int n = 0;
   __syncwarp();
-  bool room = true;
-  while (room && more_columns(p, j, x)) {
-    if (x.next != 0 || p.window != 0) ask_pages(p, j, x, j.lo_col, j.hi_col);
+  if (!x.asked) {
+    ask_pages(p, j, x, j.lo_col, j.hi_col);
+    x.asked = true;
+  }
+  while (n + 32 <= kList && more_columns(p, j, x)) {
 #pragma unroll
     for (int turn = 0; turn < kTurns; ++turn) {
-      if (!room || !more_columns(p, j, x)) break;
-      const int column = j.lo_col + x.rank + p.split * (x.next * x.columns + x.c), page = x.page[turn];
-      const bool held = page >= 0 && page < p.num_pages && column < j.hi_col;
-      const unsigned same = __match_any_sync(0xffffffffu, held ? (unsigned long long)x.c << 32 | (unsigned)page : ~0ull);
-      const bool first = held && lane == __ffs((int)same) - 1;
+      if (x.base + turn != x.next || n + 32 > kList || !more_columns(p, j, x)) continue;
+      const int column = j.lo_col + x.rank + p.split * (x.next * x.lanes.columns + x.lanes.c), page = x.page[turn];
+      bool first;
+      const unsigned beams = beams_of_page(x.lanes, page < p.num_pages && column < j.hi_col ? page : -1, &first);
       const unsigned listed = __ballot_sync(0xffffffffu, first);
-      if (first)
-        list[n + __popc(listed & ((1u << lane) - 1))] =
-            Listed{((long long)page * p.nkv + j.kvh) * p.page_size * row_bytes, column * p.page_size, same >> (x.c * wide)};
+      if (first) list[n + __popc(listed & ((1u << lane) - 1))] = Listed{((long long)page * p.nkv + j.kvh) * p.page_size * row_bytes, column * p.page_size, beams};
       n += __popc(listed);
       ++x.next;
-      room = n + 32 <= kList;
+    }
+    if (x.next == x.base + kTurns) {
+      x.base += kTurns;
+      ask_pages(p, j, x, j.lo_col, j.hi_col);
     }
   }
   __syncwarp();

@@ -52,6 +52,7 @@ MODULES: Dict[str, List[str]] = {
     "attention_kv4": [],
     "beam": [],
     "attention_beams": [],
+    "attention_beams_tc": [],
 }
 
 _LOCK = threading.Lock()

@@ -71,6 +71,7 @@ _SIGNATURES = {
     "ilb_attention_prefill_half": "pppppppp" + "iifiiiiiii" + "ppp",
     "ilb_kv4_attention_simple": "ppippppiiiifiiiiiipp",
     "ilb_kv4_attention_rows": "ppippppiiiifiiiiiiiipipqpqpp",
+    "ilb_attention_beams_tc": "pppp" + "pp" + "iiii" + "f" + "iiiii" + "qq" + "pipp",
     "ilb_attention_beams": "ppi" + "pppp" + "iiii" + "f" + "iiiii" + "qq" + "pip",
     "ilb_beam_keep": "pppi" + "pi" + "ppppp" + "iifi" + "pppppp" + "iip",
     "ilb_beam_reorder": "ppp" + "ppiii" + "ppip" + "iiip",
@@ -1528,6 +1529,9 @@ def step_build(new: torch.Tensor, cached: torch.Tensor, kv_len: torch.Tensor, po
              torch._C._cuda_getCurrentRawStream(index))
 
 
+BEAMS_TC_ROWS = 33         # rows (beams of a request times query heads of a kv head) from which shared pages go to the tcgen05 kernel
+
+
 def attention_beams_supported(dtype: torch.dtype, cache_dtype: torch.dtype, nq: int, nkv: int, d: int, page_size: int) -> bool:
     """Geometries whose shared pages are read once; others go through the exact kernel, a row at a time."""
     return (dtype == cache_dtype and dtype in (torch.bfloat16, torch.float32) and nkv > 0 and nq % nkv == 0 and d in (32, 64, 96, 128)
@@ -1572,6 +1576,13 @@ def attention_beams(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v
     longest = min(getattr(step, "max_kv_len", None) or blocks * page_size, blocks * page_size)
     if window:
         longest = min(longest, abs(window) + page_size)
+    if min(beams, rows) * (nq // nkv) >= BEAMS_TC_ROWS and dtype is torch.bfloat16 and d in (64, 128) and scale > 0 and page_size <= 128:
+        with torch.cuda.device(index):
+            error = _tc_state(q.device).error
+        _call_on(index, "attention_beams_tc", "ilb_attention_beams_tc", q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                 positions.data_ptr(), block_table.data_ptr(), blocks, page_size, pages, window, scale, rows, beams, nq, nkv, d, nq * d, nq * d,
+                 0 if sink is None else sink.data_ptr(), longest, error.data_ptr(), torch._C._cuda_getCurrentRawStream(index))
+        return
     _call_on(index, "attention_beams", "ilb_attention_beams", q.data_ptr(), out.data_ptr(), code, k_cache.data_ptr(), v_cache.data_ptr(),
              positions.data_ptr(), block_table.data_ptr(), blocks, page_size, pages, window, scale, rows, beams, nq, nkv, d, nq * d, nq * d,
              0 if sink is None else sink.data_ptr(), longest, torch._C._cuda_getCurrentRawStream(index))

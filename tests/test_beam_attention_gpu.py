@@ -12,10 +12,13 @@ DEV = "cuda:0"
 BF, F32 = torch.bfloat16, torch.float32
 
 
-@pytest.fixture(scope="module")
-def ops():
+@pytest.fixture(params=["few rows", "tcgen05"])
+def ops(request, monkeypatch):
+    """Every case through the kernels of few rows, and again with all that the tcgen05 kernel takes sent there."""
     from inferloop_b200.csrc import ops
-    return ops
+    monkeypatch.setattr(ops, "BEAMS_TC_ROWS", 1 if request.param == "tcgen05" else 10 ** 9)
+    yield ops
+    ops.check_device_errors()
 
 
 def case(R, W, lens, nkv, d, page, seed, rows=None, dtype=BF, shared=0.7, spare=2):
