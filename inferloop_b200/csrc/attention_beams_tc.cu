@@ -35,7 +35,7 @@ constexpr int kKeys = 128;             // of a tile
 constexpr int kTileUnits = kKeys / kUnit;
 constexpr int kStagesK = 3, kStagesV = 2;
 constexpr int kListed = 8 + 32 * 8;    // units: less than a tile's, and those of a turn's 32 pages
-constexpr int kAsked = 32;             // turns that pages are asked for ahead
+constexpr int kAsked = 16;             // turns that pages are asked for ahead
 constexpr int kInfos = 8;
 constexpr int kThreads = 256, kWarps = 8;
 constexpr int kPad = 8;                // floats between the records of two rows
@@ -47,6 +47,7 @@ __device__ __forceinline__ float power_of_two(float x) {
   return y;
 }
 
+__device__ __forceinline__ void tensormap_prefetch(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -66,6 +67,11 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   constexpr int kChunks = D / 64;
   constexpr uint32_t kSlice = kRows * 128, kTileBytes = kChunks * kSlice, kGroup = kChunks * 1024, kUnitBytes = 2 * kGroup;
   constexpr uint32_t kTmemCols = 512;
+  if (threadIdx.x == 32) {
+    tensormap_prefetch(&map_q);
+    tensormap_prefetch(&map_k);
+    tensormap_prefetch(&map_v);
+  }
   pdl_launch_dependents();
   pdl_wait();
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -111,7 +117,7 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     cp_async_commit();
   };
   if (warp == 6 && p.window == 0) {                      // (with a window the first column is not known yet)
-#pragma unroll 1
+#pragma unroll 4
     for (int turn = 0; turn < kAsked; ++turn) ask(turn, 0, p.max_blocks);
   }
   find_keys(p, j);
@@ -130,7 +136,7 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     // ---------------------------------------------------------------- units
     const int outside = p.num_pages * p.nkv;
     if (p.window != 0) {
-#pragma unroll 1
+#pragma unroll 4
       for (int turn = 0; turn < kAsked; ++turn) ask(turn, j.lo_col, j.hi_col);
     }
     int units = 0, taken = 0, turn = 0;                  // units in the list, of them taken by tiles
@@ -300,12 +306,10 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 #pragma unroll
           for (int n = 0; n < kTileUnits; ++n) {
             const int2 x = unit[n];
-            const bool held = ((unsigned)x.y & bit) != 0;
-            const int a = held ? lo - x.x : kUnit, b = hi - x.x;      // of the unit's keys it sees a .. b - 1
-            if (a > 0 || b < kUnit) {
+            const int a = min(max(lo - x.x, 0), kUnit), b = min(max(hi - x.x, 0), kUnit);      // of the unit's keys it sees a .. b - 1, if it holds it
+            const unsigned sees = ((unsigned)x.y & bit) != 0 ? (1u << b) - (1u << min(a, b)) : 0u;
 #pragma unroll
-              for (int c = 0; c < kUnit; ++c) if (c < a || c >= b) v[n * kUnit + c] = -INFINITY;
-            }
+            for (int c = 0; c < kUnit; ++c) v[n * kUnit + c] = (sees >> c & 1) != 0 ? v[n * kUnit + c] : -INFINITY;
           }
         }
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -353,16 +357,16 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           uint8_t* tile = smem + (v_s - base) + sv * kTileBytes;
           const int rows = 32 * active, mine = quad * 32 + lane;
           unsigned* odd = s_odd[u & 1];
-          uint32_t zero = 0u;                            // no zero any more once a value was no number
+          uint32_t zeros[4] = {};                        // no zero any more once a value was no number
 #pragma unroll 8
           for (int x = mine; x < (int)kTileBytes / 16; x += rows) {
             const uint4 y = *reinterpret_cast<const uint4*>(tile + x * 16);
-            asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(zero) : "r"(y.x), "r"(0u));
-            asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(zero) : "r"(y.y), "r"(0u));
-            asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(zero) : "r"(y.z), "r"(0u));
-            asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(zero) : "r"(y.w), "r"(0u));
+            asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(zeros[0]) : "r"(y.x), "r"(0u));
+            asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(zeros[1]) : "r"(y.y), "r"(0u));
+            asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(zeros[2]) : "r"(y.z), "r"(0u));
+            asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(zeros[3]) : "r"(y.w), "r"(0u));
           }
-          if (zero != 0u) {
+          if (((zeros[0] | zeros[1] | zeros[2] | zeros[3]) & 0x7fff7fffu) != 0u) {      // (a sum of zeros may carry a sign)
             for (int x = mine; x < (int)kTileBytes / 16; x += rows) {
               const uint4 y = *reinterpret_cast<const uint4*>(tile + x * 16);
               const uint32_t word[4] = {y.x, y.y, y.z, y.w};
@@ -490,9 +494,10 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       if (n == 1 && i0 + p.split * kWarps >= live) break;
       const int w = rows[n] / j.group, head = j.kvh * j.group + rows[n] - w * j.group;
       __nv_bfloat16* to = (__nv_bfloat16*)p.out + (long long)(j.first_row + w) * p.out_stride + (long long)head * D + E * lane;
-      // a sum of 0 is a row that sees nothing
+      // (a sum of 0 is a row that sees nothing; the product with a rounded inverse is off by 1.5 ulp of 32 bits, the rounding to bfloat16 by 2^15)
+      const float inverse = l[n] == 0.f ? 0.f : 1.f / l[n];
 #pragma unroll
-      for (int e = 0; e < E; ++e) to[e] = __float2bfloat16_rn(l[n] == 0.f ? 0.f : acc[n][e] / l[n]);
+      for (int e = 0; e < E; ++e) to[e] = __float2bfloat16_rn(acc[n][e] * inverse);
     }
   }
   if (p.split > 1) cluster_sync_all();                   // nobody leaves while a peer may still read its records
