@@ -31,9 +31,9 @@ using namespace ilb;
 namespace {
 
 constexpr int kRows = 128;             // MMA M
-constexpr int kKeys = 128;             // of a tile
+constexpr int kKeys = 64;              // of a tile
 constexpr int kTileUnits = kKeys / kUnit;
-constexpr int kStagesK = 3, kStagesV = 2;
+constexpr int kMaxPage = 128;          // tokens
 constexpr int kListed = 8 + 32 * 8;    // units: less than a tile's, and those of a turn's 32 pages
 constexpr int kAsked = 16;             // turns that pages are asked for ahead
 constexpr int kInfos = 8;
@@ -57,22 +57,24 @@ template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile(
 // What a tile is made of: first key and beams of its units, where they lie in the cache; state 0: there is no tile (the walk is over), 1: some row does not see all of it, 2: all do.
 struct Info { int2 unit[kTileUnits], box[kTileUnits]; int state, pad[3]; };
 
-template <int D>
-constexpr int smem_bytes() { return kRows * D * 2 * (1 + kStagesK + kStagesV) + 1024 + 512; }
+template <int D> constexpr int kStages = D == 64 ? 4 : 2;      // tiles of K, and of V: two CTAs share an SM's memory
+template <int D> constexpr int smem_bytes() { return kRows * D * 2 + kKeys * D * 2 * 2 * kStages<D> + 1024 + 512; }
+// Two CTAs to an SM, with 256 of its 512 columns of tensor memory each, and never a third next to kernels of the like (gemm_few.cuh says why).
+static_assert(3 * (smem_bytes<64>() + 1024) > 228 * 1024 && 2 * (smem_bytes<128>() + 10 * 1024) <= 228 * 1024, "two CTAs to an SM");
 
 template <int D>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 2)
 attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                           const Params p, int* error_flag) {
   constexpr int kChunks = D / 64;
-  constexpr uint32_t kSlice = kRows * 128, kTileBytes = kChunks * kSlice, kGroup = kChunks * 1024, kUnitBytes = 2 * kGroup;
-  constexpr uint32_t kTmemCols = 512;
+  constexpr uint32_t kSlice = kRows * 128, kQueryBytes = kChunks * kSlice, kTileBytes = kKeys * D * 2, kGroup = kChunks * 1024, kUnitBytes = 2 * kGroup;
+  constexpr int kStagesK = kStages<D>, kStagesV = kStages<D>;
+  constexpr uint32_t kTmemCols = 256;                    // two S tiles, O
   if (threadIdx.x == 32) {
     tensormap_prefetch(&map_q);
     tensormap_prefetch(&map_k);
     tensormap_prefetch(&map_v);
   }
-  pdl_launch_dependents();
   pdl_wait();
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ int4 s_list[kListed];                       // page x kv head, group of 8 keys in the page, first key, beams
@@ -82,7 +84,7 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   __shared__ unsigned s_odd[2][kKeys / 32];              // keys of an even and an odd tile whose values hold an infinity or NaN
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t q_s = base, k_s = q_s + kTileBytes, v_s = k_s + kStagesK * kTileBytes, end_s = v_s + kStagesV * kTileBytes;
+  const uint32_t q_s = base, k_s = q_s + kQueryBytes, v_s = k_s + kStagesK * kTileBytes, end_s = v_s + kStagesV * kTileBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (end_s - base));
   const uint32_t bar0 = smem_u32(bars);
   const uint32_t q_full = bar0, k_full = bar0 + 8, k_empty = k_full + 8 * kStagesK, v_full = k_empty + 8 * kStagesK, v_empty = v_full + 8 * kStagesV,
@@ -108,6 +110,8 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(kTmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    // Only now may the next kernel start: a matrix product takes its tensor memory before it waits for this kernel, and tcgen05.alloc waits without a limit.
+    pdl_launch_dependents();
   }
   // The block tables' entries of turn `turn` (warp 6): behind the boxes of five tiles an answer takes long, so they are asked for kAsked turns ahead.
   const Lanes lanes = make_lanes(j);
@@ -124,7 +128,7 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0), tmem_s = tmem_base, tmem_o = tmem_base + 256;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0), tmem_s = tmem_base, tmem_o = tmem_base + 2 * kKeys;
   bool ok = true;
   // the state of tile n, when it is known (0 too if the wait ran out: `there` is false then)
   auto state_of = [&](int n, bool* there) {
@@ -321,7 +325,7 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         const float m_new = grows ? mx : m, shift = m_new == -INFINITY ? 0.f : -m_new;
         float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {                    // P over the scores: 64 keys are 32 columns
+        for (int h = 0; h < kKeys / 64; ++h) {           // P over the scores: 64 keys are 32 columns
           uint32_t packed[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
@@ -517,6 +521,10 @@ int encode(CUtensorMap* out, const void* ptr, int rank, const cuuint64_t* dims, 
 constexpr int kMaxSplit = 16;
 std::atomic<int> g_clusters[2][OncePerDevice::kMax][kMaxSplit + 1];      // by head size and device: clusters of so many CTAs that fit at once, and one
 
+// An empty kernel of the same shape is asked about: the occupancy query counts one CTA to an SM for any kernel that allocates tensor memory.
+__global__ void __launch_bounds__(kThreads, 2) beams_shape_kernel() {}
+constexpr int kFixed = 9 * 1024;       // static shared memory of the kernel, at most
+
 template <int D>
 int clusters_at_once(int split) {
   int dev = 0;
@@ -527,25 +535,33 @@ int clusters_at_once(int split) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(split, 64, 8);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem_bytes<D>();
+  cfg.dynamicSmemBytes = smem_bytes<D>() + kFixed;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int found = 0;
-  if (cudaOccupancyMaxActiveClusters(&found, attention_beams_tc_kernel<D>, &cfg) != cudaSuccess) { cudaGetLastError(); found = 0; }
+  if (cudaOccupancyMaxActiveClusters(&found, beams_shape_kernel, &cfg) != cudaSuccess) { cudaGetLastError(); found = 0; }
   known.store(found + 1, std::memory_order_relaxed);
   return found;
+}
+
+template <typename Kernel>
+cudaError_t configure(Kernel kernel, int smem) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  // two CTAs share an SM only with the largest shared-memory carve-out
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  return e;
 }
 
 template <int D>
 int run(Params& p, int longest, int* error_flag, cudaStream_t stream) {
   static OncePerDevice once;
   const cudaError_t set = once.run([] {
-    cudaError_t e = cudaFuncSetAttribute(attention_beams_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<D>());
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_beams_tc_kernel<D>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    return e;
+    cudaError_t e = configure(attention_beams_tc_kernel<D>, smem_bytes<D>());
+    return e == cudaSuccess ? configure(beams_shape_kernel, smem_bytes<128>() + kFixed) : e;
   });
   if (set != cudaSuccess) return check_launch("attention_beams");
   const int group = p.nq / p.nkv, requests = (p.rows + p.beams - 1) / p.beams, most = kRows / group;
@@ -580,7 +596,7 @@ ILB_EXPORT int ilb_attention_beams_tc(const void* q, void* out, const void* k, c
                                       const float* sink, int longest, int* error_flag, cudaStream_t stream) {
   ILB_REQUIRE(rows >= 0 && beams > 0 && beams <= kMaxBeams && nq > 0 && nkv > 0 && nq % nkv == 0 && nq / nkv <= kRows && max_blocks > 0 && num_pages > 0,
               "attention_beams: bad sizes (up to %d beams)", kMaxBeams);
-  ILB_REQUIRE(page_size >= kUnit && page_size % kUnit == 0 && page_size <= kKeys && (d == 64 || d == 128) && scale > 0.f,
+  ILB_REQUIRE(page_size >= kUnit && page_size % kUnit == 0 && page_size <= kMaxPage && (d == 64 || d == 128) && scale > 0.f,
               "attention_beams: pages of 16 to 128 tokens, heads of 64 or 128 and a scale above 0, found %d, %d and %g", page_size, d, (double)scale);
   ILB_REQUIRE(q_stride >= (long long)nq * d && out_stride >= (long long)nq * d && q_stride % 8 == 0, "attention_beams: strides too small or odd");
   ILB_REQUIRE(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 == 0, "attention_beams: queries and cache must lie on 16-byte boundaries");
