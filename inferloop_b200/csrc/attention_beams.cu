@@ -2,9 +2,10 @@
 // and a page that several beams hold is read once for all of them: for request r, kv head h and query rows i = (beam w, head g of the group)
 //   o_i = sum_j p_ij v_j,  p_i = softmax over the keys j of row w's table of  scale q_i k_j
 // with the rows of all beams as one matrix against each distinct page, and the rows whose beam does not hold it masked.
+// Requests with many rows and much to read go to the tensor cores' tcgen05 kernel (attention_beams_tc.cu) instead; ops.py has the rule.
 //
 //   units    a warp looks at a column of the block tables for each of its groups of lanes, a lane a beam: lanes with equal pages find each
-//            other (match), and the first of them enters (page, beams that hold it, column) in the list.  Nothing need be known about who descends
+//            other (by shuffles), and the first of them enters (page, beams that hold it, column) in the list.  Nothing need be known about who descends
 //            from whom.  A unit is 16 keys of a page.
 //   split    a cluster of S = 1..16 CTAs with GROUPS rings each shares a (request, kv head); column c goes to CTA c % S, there to the rings in
 //            turn, so that the columns that beams do not share (the latest ones) are dealt out evenly.  Every warp lists its ring's units for

@@ -1,19 +1,22 @@
 // Attention of one new token of every beam over shared pages (attention_beams.cu says what and why) on the tcgen05 tensor cores, for requests whose beams and query
-// heads make more rows than two warps' products take: up to 128 rows (beam, query head of the group) of one request and kv head as the M of an MMA.
+// heads make many rows: up to 128 rows (beam, query head of the group) of one request and kv head as the M of an MMA.
 //
-//   tile     128 keys = 8 units of 16 keys of a page, whichever pages the beams hold between them; each unit comes by one TMA box for K and one for V, in the
+//   tile     64 keys = 4 units of 16 keys of a page, whichever pages the beams hold between them; each unit comes by one TMA box for K and one for V, in the
 //            operands' layout ([group of 8 keys][64-wide slice of the head][8 keys][64], 128-byte swizzle).  Units that are missing at the end are asked for
 //            outside the tensor, which TMA fills with zeros.
-//   warp 6   finds the units and leaves what a tile is made of in a ring of 8 for the others, an end mark behind the last tile.
-//   warps 0, 7  issue the boxes of K and of V: rings of 3 K tiles and 2 V tiles.  (One warp for all three took 4,000 clocks a tile: 850 a turn of
-//            the block tables, 770 and 600 for eight boxes.)
-//   warp 1   allocates tensor memory (two S tiles of 128 columns, O of D) and issues S = Q K^T two tiles ahead and O += P V.
+//   warp 6   finds the units, the block tables asked for 16 turns ahead, and leaves what a tile is made of in a ring of 8 for the others, an end mark
+//            behind the last tile.
+//   warps 0, 7  issue the boxes of K and of V into rings of 2 tiles each (heads of 64: 4).  (One warp for all three took 4,000 clocks for 128 keys: 850 a turn
+//            of the block tables, 770 and 600 for eight boxes.)
+//   warp 1   allocates tensor memory (two S tiles of 64 columns, O of D) and issues S = Q K^T two tiles ahead and O += P V.
 //   warps 2-5  a thread a row (= tensor-memory lane): masks what its beam does not hold or see, exponentials, P as packed bfloat16 over the
 //            scores; O is rescaled only when a maximum has grown by more than 2^8.  Warps without rows leave at once.
 //   split    clusters of S CTAs share a (request, kv head) by columns of the block tables, as in attention_beams.cu; at the end every CTA leaves its rows'
 //            records (maximum, sum, O) in its shared memory and row i is added up by CTA i % S.
-// Bound: the cache's bytes (a tile's products take 1,550 clocks of the tensor core and its exponentials 1,024 of the special-function unit, its bytes
-// 2,800 at an SM's share of the memory).
+// Two CTAs to an SM: a tile of one row's chain (wait for S, load, exponentials, wait for O: 1,700 clocks) leaves the tensor cores and the memory idle, and a
+// second CTA fills that.  6 x 8 beams of 6000 keys, 40 rows, 48 jobs: 41.8 us, 3.6 TB/s (55 % of the measured copy rate); one CTA to an SM with tiles of 128 keys
+// took 47.1 (clusters of three did not all fit then).  8 x 16 of 1000: 26.0 us.
+// Bound: the same chain, at clusters' sizes that leave some SMs without work (240 CTAs of 296), and 10,000 clocks before the first tile and after the last.
 // A value that is masked for a row never reaches it: where a tile is not seen whole by all rows its values are looked at, and infinities and NaN
 // are added by hand to the rows that see them and taken out of the tile before the product.
 // Every mbarrier wait is bounded; on expiry a flag is raised and the CTA still walks through the cluster's barriers.  No multicast.
@@ -54,13 +57,15 @@ __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// What a tile is made of: first key and beams of its units, where they lie in the cache; state 0: there is no tile (the walk is over), 1: some row does not see all of it, 2: all do.
+// What a tile is made of: first key and beams of its units, where they lie in the cache; state 0: there is no tile (the walk is over), 1: some row does not see
+// all of it, 2: all do.
 struct Info { int2 unit[kTileUnits], box[kTileUnits]; int state, pad[3]; };
 
 template <int D> constexpr int kStages = D == 64 ? 4 : 2;      // tiles of K, and of V: two CTAs share an SM's memory
 template <int D> constexpr int smem_bytes() { return kRows * D * 2 + kKeys * D * 2 * 2 * kStages<D> + 1024 + 512; }
+constexpr int kFixed = 9 * 1024;       // static shared memory, at most
 // Two CTAs to an SM, with 256 of its 512 columns of tensor memory each, and never a third next to kernels of the like (gemm_few.cuh says why).
-static_assert(3 * (smem_bytes<64>() + 1024) > 228 * 1024 && 2 * (smem_bytes<128>() + 10 * 1024) <= 228 * 1024, "two CTAs to an SM");
+static_assert(3 * (smem_bytes<64>() + 1024) > 228 * 1024 && 2 * (smem_bytes<128>() + kFixed + 1024) <= 228 * 1024, "two CTAs to an SM");
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -518,24 +523,23 @@ int encode(CUtensorMap* out, const void* ptr, int rank, const cuuint64_t* dims, 
   return 0;
 }
 
-constexpr int kMaxSplit = 16;
-std::atomic<int> g_clusters[2][OncePerDevice::kMax][kMaxSplit + 1];      // by head size and device: clusters of so many CTAs that fit at once, and one
-
-// An empty kernel of the same shape is asked about: the occupancy query counts one CTA to an SM for any kernel that allocates tensor memory.
+// Clusters of `split` CTAs that the device holds at once with one CTA to an SM (ask = kAskOne) or two.  An empty kernel of the same shape is asked about: the
+// occupancy query counts one CTA to an SM for any kernel that allocates tensor memory.
 __global__ void __launch_bounds__(kThreads, 2) beams_shape_kernel() {}
-constexpr int kFixed = 9 * 1024;       // static shared memory of the kernel, at most
+constexpr int kMaxSplit = 16;
+constexpr int kAskOne = 120 * 1024, kAskTwo = smem_bytes<128>() + kFixed;
+std::atomic<int> g_clusters[2][OncePerDevice::kMax][kMaxSplit + 1];      // by CTAs to an SM and device: their number and one
 
-template <int D>
-int clusters_at_once(int split) {
+int clusters_at_once(int ctas, int split) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= OncePerDevice::kMax) dev = 0;
-  std::atomic<int>& known = g_clusters[D == 128][dev][split];
+  std::atomic<int>& known = g_clusters[ctas - 1][dev][split];
   const int n = known.load(std::memory_order_relaxed);
   if (n) return n - 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(split, 64, 8);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem_bytes<D>() + kFixed;
+  cfg.dynamicSmemBytes = ctas == 1 ? kAskOne : kAskTwo;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
@@ -545,6 +549,19 @@ int clusters_at_once(int split) {
   if (cudaOccupancyMaxActiveClusters(&found, beams_shape_kernel, &cfg) != cudaSuccess) { cudaGetLastError(); found = 0; }
   known.store(found + 1, std::memory_order_relaxed);
   return found;
+}
+
+// CTAs that share a (request, kv head): as many as one to an SM allows; where that is fewer than three, as many as two to an SM allow, less a twelfth (56
+// clusters of 5, which the query grants, took a second round: 34.4 us where 4 take 29.0).  Measured with one to an SM / two: 6 x 8 beams of 6000 keys,
+// 48 jobs, 59.6 (2 CTAs) / 41.8 us (5); 8 x 16 of 1000, 64 jobs, 30.7 (2) / 26.1 (4); but 5 x 8 of 1000, 40 jobs, 18.9 (3) / 21.1 (6); 4 x 16 of
+// 2000, 32 jobs, 28.0 (4) / 33.6 (8); 1 x 10 of 8000, 8 jobs, 37.2 (10) / 41.9 (16).
+int split_of(long long jobs, int tiles) {
+  const int most = min(kMaxSplit, max(tiles, 1));
+  int one = most, two = most;
+  while (one > 1 && clusters_at_once(1, one) < jobs) --one;
+  if (one >= min(3, most)) return one;
+  while (two > 1 && clusters_at_once(2, two) * 11 / 12 < jobs) --two;
+  return max(one, two);
 }
 
 template <typename Kernel>
@@ -561,7 +578,7 @@ int run(Params& p, int longest, int* error_flag, cudaStream_t stream) {
   static OncePerDevice once;
   const cudaError_t set = once.run([] {
     cudaError_t e = configure(attention_beams_tc_kernel<D>, smem_bytes<D>());
-    return e == cudaSuccess ? configure(beams_shape_kernel, smem_bytes<128>() + kFixed) : e;
+    return e == cudaSuccess ? configure(beams_shape_kernel, kAskOne) : e;
   });
   if (set != cudaSuccess) return check_launch("attention_beams");
   const int group = p.nq / p.nkv, requests = (p.rows + p.beams - 1) / p.beams, most = kRows / group;
@@ -569,8 +586,7 @@ int run(Params& p, int longest, int* error_flag, cudaStream_t stream) {
   p.beams_of_chunk = (p.beams + p.chunks - 1) / p.chunks;
   const long long jobs = (long long)requests * p.nkv * p.chunks;
   const int tiles = (longest + kKeys - 1) / kKeys;
-  p.split = min(kMaxSplit, max(tiles, 1));
-  while (p.split > 1 && clusters_at_once<D>(p.split) < jobs) --p.split;
+  p.split = split_of(jobs, tiles);
   CUtensorMap q, k, v;
   {   // queries as (d, heads, rows): a box is one slice of the rows of a chunk
     const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)p.nq, (cuuint64_t)p.rows}, strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)p.q_stride * 2};

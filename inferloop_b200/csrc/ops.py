@@ -1529,7 +1529,20 @@ def step_build(new: torch.Tensor, cached: torch.Tensor, kv_len: torch.Tensor, po
              torch._C._cuda_getCurrentRawStream(index))
 
 
-BEAMS_TC_ROWS = 33         # rows (beams of a request times query heads of a kv head) from which shared pages go to the tcgen05 kernel
+# Which kernel reads shared pages of bfloat16, by the rows (beams of a request times query heads of a kv head) and the keys of all requests and kv heads.
+# Measured with few rows' kernel / the tcgen05 kernel: 40 rows, 6 x 8 kv heads of 6000 keys 71.5 / 41.8 us, 3 x 8 of 200 17.2 / 14.3, 36 rows, 8 of 500
+# 11.7 / 12.1; 128 rows, 16 of 4000 40.4 / 36.7, 16 of 500 27.2 / 32.1; 20 rows, 64 kv heads of 3000 36.9 / 27.1, 256 of 500 33.8 / 24.2, but 128 of 500
+# 17.8 / 18.8 and 32 of 3000 20.0 / 24.6; 16 rows, 512 of 1030 60.8 / 65.4, 64 of 4000 29.7 / 30.9.
+BEAMS_TC_ROWS, BEAMS_TC_FEW, BEAMS_TC_KEYS = 33, 17, 100_000
+# Keys and values that a layer's beams read, each by itself, from which reading shared pages once pays for a launch more and a longer start than those of
+# attention_decode_fused.  Steps of 16 layers with groups of 2 / 4 / 5 / 8 query heads, what sharing gains a layer in us: 8 x 4 beams of 1,230 keys
+# (161 MB) 7.4 / 6.5 / 3.1 / 2.9; 16 x 4 of 630 (165 MB) 6.2 / 4.4 / 1.7 / 2.0; 4 x 4 of 2,030 (133 MB) -0.8 / -1.4 / 2.7 / 2.5; 8 x 8 of 330
+# (87 MB) -0.2 / -1.9 / -8.5 / -8.4; 4 x 4 of 630 (41 MB) -6.2 / -6.9 / -3.0 / -3.4; 1 x 4 of 130 (2 MB) -4.2 / -3.9 / -3.5 / -4.9.
+# Against attention_decode_tma, which is a launch of its own too, it pays from a twelfth of that: us with shared pages / each by itself, 8 kv heads, 1 x 4 beams
+# of 640 keys (10 MB) 7.6 / 10.3, 4 x 4 of 2,040 (134 MB) 12.5 / 23.3, 1 x 4 of 140 (2 MB) 8.0 / 6.7; 2 kv heads of 8 query heads, 4 x 4 of 640 (10 MB)
+# 9.0 / 9.0, 1 x 4 of 2,040 (8 MB) 9.6 / 8.7, 16 x 4 of 640 (42 MB) 10.3 / 10.6, but 8 x 8 of 340 (22 MB, 64 rows) 16.6 / 8.5.  In 32 bits no kernel of
+# single tokens splits a sequence, and 1 x 4 of 640 take 10.8 / 209.
+BEAMS_SHARE_BYTES = 120_000_000
 
 
 def attention_beams_supported(dtype: torch.dtype, cache_dtype: torch.dtype, nq: int, nkv: int, d: int, page_size: int) -> bool:
@@ -1576,7 +1589,9 @@ def attention_beams(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v
     longest = min(getattr(step, "max_kv_len", None) or blocks * page_size, blocks * page_size)
     if window:
         longest = min(longest, abs(window) + page_size)
-    if min(beams, rows) * (nq // nkv) >= BEAMS_TC_ROWS and dtype is torch.bfloat16 and d in (64, 128) and scale > 0 and page_size <= 128:
+    per_head = min(beams, rows) * (nq // nkv)
+    if dtype is torch.bfloat16 and (per_head >= BEAMS_TC_ROWS or (per_head >= BEAMS_TC_FEW and -(-rows // beams) * nkv * longest >= BEAMS_TC_KEYS)) \
+            and d in (64, 128) and scale > 0 and page_size <= 128:
         with torch.cuda.device(index):
             error = _tc_state(q.device).error
         _call_on(index, "attention_beams_tc", "ilb_attention_beams_tc", q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),

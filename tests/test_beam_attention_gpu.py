@@ -17,6 +17,7 @@ def ops(request, monkeypatch):
     """Every case through the kernels of few rows, and again with all that the tcgen05 kernel takes sent there."""
     from inferloop_b200.csrc import ops
     monkeypatch.setattr(ops, "BEAMS_TC_ROWS", 1 if request.param == "tcgen05" else 10 ** 9)
+    monkeypatch.setattr(ops, "BEAMS_TC_FEW", 10 ** 9)
     yield ops
     ops.check_device_errors()
 
