@@ -307,7 +307,10 @@ class DecodeGraphs:
         if not self.whole or self.runner.spec.token_extras:
             raise ValueError("beams need a model whose whole step is recorded as one graph and that takes no inputs per token "
                              "beside ids and positions")
-        key = ("beams", bucket, beams, longest >= ops.DECODE_LONG_CONTEXT)
+        # (which kernels run, and how they split the keys, goes by the longest context, in eighths of a power of two)
+        grain = max(1 << max(longest.bit_length() - 3, 0), 64)
+        longest = max(longest, min(-(-longest // grain) * grain, self.runner.spec.max_positions))
+        key = ("beams", bucket, beams, longest)
         rec = self._recorded.get(key)
         if rec is not None and rec.workspace_generation != self.runner.ctx.workspace.generation:
             del self._recorded[key]

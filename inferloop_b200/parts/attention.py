@@ -305,12 +305,13 @@ class GQAttention(Mixer):
         if self.value_mix is not None:
             # the step's tokens' values of the first layer that mixes: kept by it, read by the later ones
             v_first = ws.buffer(f"attn.v_first/{self.nkv}x{self.dv}", (T, self.nkv * self.dv), dt)
-        shared = self._beams_share(step, cache, dt)
-        if (not shared and self.dv == self.d and step.decode_only and cache.k is not None and (cache.writable or self.value_mix is None)
-                and not self.shaped and not self.has_sink
-                and ops.attention_decode_fused_supported(
-                    dt, cache.k.dtype, self.nq, self.nkv, self.d, cache.page_size, self.rotary_dim, rope is not None,
-                    interleaved=bool(self.mode & ops.ROPE_INTERLEAVED))):
+        fused = (self.dv == self.d and step.decode_only and cache.k is not None and (cache.writable or self.value_mix is None)
+                 and not self.shaped and not self.has_sink
+                 and ops.attention_decode_fused_supported(
+                     dt, cache.k.dtype, self.nq, self.nkv, self.d, cache.page_size, self.rotary_dim, rope is not None,
+                     interleaved=bool(self.mode & ops.ROPE_INTERLEAVED)))
+        shared = self._beams_share(step, cache, dt, fused)
+        if fused and not shared:
             # one token per sequence: norm, rotation and the cache write of the new key and
             # value happen inside the attention kernel
             o = ws.buffer("attn.o", (T, self.nq * self.d), dt)
@@ -346,10 +347,15 @@ class GQAttention(Mixer):
                           self.nq, self.nkv, self.d, workspace=ws, decode_chunk=self.decode_chunk, dv=self.dv, sink=self.sink)
         self._finish(o, qkv, gate_col0, residual, out)
 
-    def _beams_share(self, step, cache, dtype) -> bool:
-        """Whether the step's rows are beams whose shared pages are read once."""
-        return (step.beams > 1 and not self.shaped and self.dv == self.d and cache.k is not None
-                and ops.attention_beams_supported(dtype, cache.k.dtype, self.nq, self.nkv, self.d, cache.page_size))
+    def _beams_share(self, step, cache, dtype, fused: bool = False) -> bool:
+        """Whether the step's rows are beams whose shared pages are read once (fused: else one launch would norm, rotate, cache and
+        attend, each beam by itself)."""
+        if (step.beams <= 1 or self.shaped or self.dv != self.d or cache.k is None
+                or not ops.attention_beams_supported(dtype, cache.k.dtype, self.nq, self.nkv, self.d, cache.page_size)):
+            return False
+        keys = min(step.max_kv_len, abs(self.seen)) if self.seen else step.max_kv_len
+        read = step.n_tokens * keys * self.nkv * 2 * self.d * cache.k.element_size()
+        return dtype is torch.float32 or read >= (ops.BEAMS_SHARE_BYTES if fused else ops.BEAMS_SHARE_BYTES // 12)
 
     def _forward_rows(self, qkv, rope, table, step, cache, gate_col0, residual, out) -> None:
         """The layer with norms over whole rows: input stage, means of the blocks this step completes, attention, the

@@ -185,3 +185,26 @@ def test_states_follow_the_beams(tmp_path_factory, family, case):
     if tried == 0:
         with pytest.raises(ValueError, match="recorded as one graph"):
             engine.beam_search([[1, 2]], 2, 2)
+
+
+@pytest.mark.parametrize("tc_rows", [1, 10 ** 9])
+@pytest.mark.parametrize("name", ["D", "F", "E"])
+def test_bfloat16_scores_with_shared_pages(folders, monkeypatch, name, tc_rows):
+    """The same where pages are read once for all beams however little that is, by either kernel."""
+    from inferloop_b200.csrc import ops
+    monkeypatch.setattr(ops, "BEAMS_SHARE_BYTES", 0)
+    monkeypatch.setattr(ops, "BEAMS_TC_ROWS", tc_rows)
+    test_bfloat16_scores(folders, name, {})
+    ops.check_device_errors()
+
+
+def test_a_short_search_leaves_a_long_one_as_it_is(folders):
+    vocab = CONFIGS["D"][0]["vocab_size"]
+    prompts = [random_tokens(n, vocab, 80 + n) for n in (700, 650)]
+
+    def long(engine):
+        return [[(h.tokens, h.score) for h in x] for x in engine.beam_search(prompts, 4, 8, eos_tokens=[])]
+    first = long(engine_for(folders["D"], dtype="bfloat16"))
+    engine = engine_for(folders["D"], dtype="bfloat16")
+    engine.beam_search([p[:20] for p in prompts], 4, 8, eos_tokens=[])
+    assert long(engine) == first
