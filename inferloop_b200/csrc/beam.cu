@@ -107,9 +107,10 @@ struct Ranked { u64 score, tie; };      // the score's order, then (logit's orde
 __device__ __forceinline__ bool above(const Ranked& a, const Ranked& b) { return a.score > b.score || (a.score == b.score && a.tie > b.tie); }
 
 // The first launch's sums of exponentials are of 32 bits.  A term at distance d below the maximum is off by (2^-23 + 2^-26) d (difference,
-// product, the constant's last bits) and 2^-22 (each of three exponentials), a segment's sum by 6 roundings, that of ten segments by 11 more (further
-// sums are of 64 bits): with sum p d <= ln(vocab) that is 3.9e-6 for up to 4 M tokens, and two beams are in order for sure when their scores differ by twice as much.  Where candidates of two beams that
-// matter come closer, those beams' sums are taken once more, in 64 bits: about one step of one request in a thousand.
+// product, the constant's last bits) and 2^-22 (each of three exponentials), a segment's sum by 6 roundings, that of ten segments by 11 more
+// (further sums are of 64 bits): with sum p d <= ln(vocab) that is 3.9e-6 for up to 4 M tokens, and two beams are in order for sure when their
+// scores differ by twice as much.  Where candidates of two beams that matter come closer, those beams' sums are taken once more, in 64 bits:
+// about one step of one request in a thousand.
 constexpr double kUncertain = 8e-6;
 constexpr int kJoinThreads = 1024, kJoinWarps = kJoinThreads / 32;
 constexpr int kListed = 1024;          // segments, and candidates, that are looked at in one go
@@ -137,7 +138,7 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
   pdl_launch_dependents();
   pdl_wait();
   __shared__ double s_base[kMaxBeams], s_top[kMaxBeams], s_part[kJoinWarps];      // score - lse or NaN (the beam brings no candidates), maximum
-  __shared__ float s_m[kJoinWarps];
+  __shared__ float s_m[kJoinWarps], s_score[kMaxBeams];  // (scores are read once: the new ones may be written over them)
   __shared__ double s_sum[kJoinWarps];
   __shared__ unsigned s_best[kBestOfWarp * kJoinWarps];
   __shared__ signed char s_order[kMaxBeams];             // the beams that are alive
@@ -149,7 +150,9 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
   const int segments = tiles * 32;
   const float2* request = sums + (long long)r * beams * segments;
   if (warp == 0) {
-    const bool alive = lane < beams && isfinite(scores[(long long)r * beams + lane]);
+    const float score = lane < beams ? scores[(long long)r * beams + lane] : NAN;
+    const bool alive = isfinite(score);
+    s_score[lane] = score;
     const unsigned live = __ballot_sync(0xffffffffu, alive);
     if (lane == 0) { s_live = live; s_segments = 0; s_count = 0; s_close = 0; s_bad = 0; }
     if (lane < beams) s_base[lane] = (double)NAN;
@@ -206,7 +209,7 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
     if (lane == 0) {
-      const double base = (double)scores[(long long)r * beams + beam] - ((double)all_top + log(all));
+      const double base = (double)s_score[beam] - ((double)all_top + log(all));
       s_base[beam] = !isfinite(base) ? (double)NAN : base;
       s_top[beam] = (double)all_top;
       if (isnan(all)) atomicOr(&s_bad, 1u << beam);
@@ -293,7 +296,7 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
     double s = 0.0;
     for (int i = t; i < vocab; i += kJoinThreads) s += exp((double)to_float(x[i]) - top);
     s = block_sum(s, s_part);
-    if (t == 0) s_base[beam] = (double)scores[(long long)r * beams + beam] - (top + log(s));
+    if (t == 0) s_base[beam] = (double)s_score[beam] - (top + log(s));
   };
   int n = s_count;
   if (listed <= kListed && n <= kListed) {
@@ -572,6 +575,7 @@ beam_reorder_kernel(const int* __restrict__ parents, const int* __restrict__ kv_
   short* s_source = s_place + rows;                                  // [rows]
   int* s_len = (int*)(s_source + rows);                              // [requests]
   Copy* s_copy = (Copy*)(s_len + requests);                          // [rows][kinds]: groups, then slots
+  int* old = (int*)(s_copy + (size_t)rows * kinds) + threadIdx.x;    // [beams][kCopyThreads]: a thread's column
   __shared__ int s_before[kCopyWarps + 1], s_last;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   // requests in runs a warp, so that the rows that copy are numbered in order
@@ -628,16 +632,11 @@ beam_reorder_kernel(const int* __restrict__ parents, const int* __restrict__ kv_
       const int width = groups.width[g], columns = min(width, s_len[r] / groups.stride[g] / groups.page_size[g]);
       int* table = groups.table[g] + (long long)r * beams * width;
       for (int c = t; c < columns; c += kCopyThreads) {              // (a thread a column: nothing is read after it was replaced)
-        int old[kMaxBeams];
-#pragma unroll
-        for (int w = 0; w < kMaxBeams; ++w) { if (w >= beams) break; old[w] = table[(long long)w * width + c]; }
+#pragma unroll 8
+        for (int w = 0; w < beams; ++w) old[w * kCopyThreads] = table[(long long)w * width + c];
         for (int w = 0; w < beams; ++w) {
           const int p = parents[r * beams + w];
-          if (p < 0 || p >= beams || p == w) continue;
-          int x = old[0];
-#pragma unroll
-          for (int i = 1; i < kMaxBeams; ++i) if (i == p) x = old[i];
-          table[(long long)w * width + c] = x;
+          if (p >= 0 && p < beams && p != w) table[(long long)w * width + c] = old[p * kCopyThreads];
         }
       }
     }
@@ -714,10 +713,10 @@ ILB_EXPORT int ilb_beam_reorder(const int* parents, const int* kv_len, int* slot
     ILB_REQUIRE(g.width[i] > 0 && g.page_size[i] > 0 && g.stride[i] > 0 && g.pages[i] > 0, "beam_reorder: bad sizes of page group %d", i);
   }
   static OncePerDevice once;
-  constexpr int kMostShared = kMaxRows * 4 + kMaxRows * 4 + kMaxRows * (kMaxGroups + 1) * (int)sizeof(Copy);
+  constexpr int kMostShared = kMaxRows * 4 + kMaxRows * 4 + kMaxRows * (kMaxGroups + 1) * (int)sizeof(Copy) + kMaxBeams * kCopyThreads * 4;
   if (once.run([] { return cudaFuncSetAttribute(beam_reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared); }) != cudaSuccess)
     return check_launch("beam_reorder");
-  const size_t smem = rows * 4 + (size_t)requests * 4 + rows * (n_groups + 1) * sizeof(Copy);
+  const size_t smem = rows * 4 + (size_t)requests * 4 + rows * (n_groups + 1) * sizeof(Copy) + (size_t)beams * kCopyThreads * 4;
   launch(beam_reorder_kernel, dim3(2 * sms), dim3(kCopyThreads), smem, stream, parents, kv_len, slots, (const Moved*)moved, first_part, n_moved,
          parts_of_copy, num_slots, g, (int)rows, beams, turns);
   return check_launch("beam_reorder");

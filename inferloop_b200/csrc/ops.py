@@ -1285,7 +1285,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, parents: torch.Tenso
     to beam w of request r, whose score is scores[r, w] (float32).  parents, tokens and out_scores [R, k] get the k best (beam, token) by
     score + log softmax(logits), best first; equal ones by the higher logit, then the lower beam, then the lower token.  A logit of -inf is
     no candidate, nor is anything of a beam whose score is not finite; a row with NaN or +inf brings nothing and is flagged in
-    `bad` [R * W].  Where fewer than k are found the rest is beam -1, token -1, score -inf."""
+    `bad` [R * W].  Where fewer than k are found the rest is beam -1, token -1, score -inf.  out_scores may be `scores` itself."""
     index = logits.get_device()
     if index < 0 or not (_ready(index, _INT32, parents, tokens) and _ready(index, torch.float32, scores, out_scores)) \
             or (bad is not None and not _ready(index, _INT32, bad)):
@@ -1383,7 +1383,7 @@ def beam_keep(parents: torch.Tensor, tokens: torch.Tensor, scores: torch.Tensor,
 class BeamState:
     """What moves with the beams, described once: `groups` = [(storages, page size, tokens a row stands for)], a storage being [..., pages, heads,
     rows, row] (a group in 4 bits: uint8 [..., pages, heads, units of 16 rows, bytes]), and `slots`, tensors [slots, ...] of state
-    per sequence.  The tensors are kept, and moved where they lie."""
+    per sequence.  The tensors are kept, and moved where they lie; reorderings of one state go one after the other, not on two streams at once."""
 
     def __init__(self, groups, slots=(), device=None) -> None:
         self.tensors = [x for storages, _, _ in groups for x in storages] + list(slots)

@@ -231,3 +231,22 @@ def test_refusals(ops):
         a = {**good, **change}
         with pytest.raises(ops.KernelError):
             ops.attention_beams(a["q"], a["out"], a["k"], a["v"], a["step"], a["table"], a["beams"], 0, 0.125, a["nq"], a["nkv"], a["d"], sink=a["sink"])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_a_cache_of_more_than_32_bits(ops, dtype):
+    """The pages at the end of a pool of more than 2^32 bytes give the bits that they give in a pool of their own."""
+    nq, nkv, d, W, page = 16, 8, 128, 4, 16
+    k, v, table, positions = case(2, W, [300, 77], nkv, d, page, 11, dtype=dtype)
+    own, pool = k.shape[0], (1 << 32) // (nkv * page * d * k.element_size()) + 50
+    q, step = queries(2 * W, nq, d, dtype, 7).to(DEV), make_step(positions)
+    outs = []
+    for moved in (0, pool - own):
+        caches = []
+        for x in (k, v):
+            big = torch.empty((moved + own, *x.shape[1:]), dtype=dtype, device=DEV)
+            big[moved:] = x.to(DEV)
+            caches.append(big)
+        outs.append(torch.zeros_like(q))
+        ops.attention_beams(q, outs[-1], *caches, step, torch.where(table < 0, table, table + moved).to(DEV), W, 0, d ** -0.5, nq, nkv, d)
+    assert outs[0].abs().sum() > 0 and torch.equal(outs[0], outs[1])

@@ -114,6 +114,18 @@ def test_select_strides_and_alignment(ops):
     assert got[0][0].tolist() == found[0][0] and got[1][0].tolist() == found[0][1] and (got[3] == 77).all()
 
 
+def test_select_scores_in_place(ops):
+    """The new scores may be written over the old ones, also where the beams come so close that their sums are taken again."""
+    near = randn(1, 40000, seed=5)
+    rows = torch.cat([near, near.flip(1), 3 * randn(1, 40000, seed=6), near.roll(7, 1)])
+    for logits, R in ((rows, 1), (3 * randn(12, 9001, seed=7), 3)):
+        scores = -torch.arange(logits.shape[0], dtype=torch.float32).remainder(2).view(R, 4) / 64
+        parents, tokens, out, bad = select(ops, logits, scores, 4)
+        x, again = scores.to(DEV), [torch.zeros((R, 4), dtype=torch.int32, device=DEV) for _ in range(2)]
+        ops.beam_select(logits.to(DEV), x, *again, x)
+        assert torch.equal(x.cpu(), out) and torch.equal(again[0].cpu(), parents) and torch.equal(again[1].cpu(), tokens)
+
+
 def test_select_two_streams_and_graph(ops):
     """Two selections on two streams at once, and a recorded one beside them, each with scratch of its own."""
     R, W, V, k = 2, 4, 60000, 8
@@ -258,6 +270,18 @@ def test_reorder_storages(ops, groups):
 def test_reorder_every_child_of_one_and_none(ops):
     for parents in ([[2, 2, 2, 2]], [[0, 1, 2, 3]], [[3, 2, 1, 0]], [[-1, -1, -1, -1]], [[1, -1, 1, 0]], [[0, 0, -1, -1]]):
         run_reorder(ops, *reorder_case(1, 1, 4, [21], [((2, 2), 2, 16, 64, BF, 1, 1)], [((9,), F32)], torch.tensor(parents, dtype=torch.int32)))
+
+
+def test_reorder_in_a_pool_of_more_than_32_bits(ops):
+    pages = (1 << 32) // (8 * 16 * 128 * 2) + 9
+    x = torch.empty((1, pages, 8, 16, 128), dtype=BF, device=DEV)
+    x[:, -8:] = randn(1, 8, 8, 16, 128, seed=9).to(BF).to(DEV)
+    was, table = x[:, -8:].clone(), torch.tensor([[pages - 8 + i] for i in range(8)], dtype=torch.int32, device=DEV)
+    state = ops.BeamState([([x], 16, 1)], [], DEV)
+    ops.beam_reorder(state, i32([[1, 1, 3, 3], [2, 0, 0, 0]]), i32([11] * 4 + [16 * 1 - 1] * 4), [table], None)
+    for row, (source, fill) in enumerate(((1, 11), (1, 11), (3, 11), (3, 11), (6, 15), (4, 15), (4, 15), (4, 15))):
+        assert torch.equal(x[0, int(table[row, 0]), :, :fill], was[0, source, :, :fill])
+    assert sorted(table.flatten().tolist()) == list(range(pages - 8, pages))
 
 
 def test_reorder_pages_that_are_not_held(ops):
