@@ -113,8 +113,9 @@ __device__ __forceinline__ bool above(const Ranked& a, const Ranked& b) { return
 // about one step of one request in a thousand.
 constexpr double kUncertain = 8e-6;
 constexpr int kJoinThreads = 1024, kJoinWarps = kJoinThreads / 32;
-constexpr int kListed = 1024;          // segments, and candidates, that are looked at in one go
-constexpr int kBestOfWarp = 4;
+constexpr int kListed = 1024;          // segments, and candidates, that the lists hold
+constexpr int kKeyed = 128;            // segments whose logits fit eight registers a thread
+constexpr int kKeys = 128;             // warps' best maxima that the border is found from
 constexpr int kHeld = 10;              // segments that a thread keeps (all of them at four beams of 151,936 tokens)
 constexpr int kMaxVocab = 1 << 22;
 
@@ -140,15 +141,17 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
   __shared__ double s_base[kMaxBeams], s_top[kMaxBeams], s_part[kJoinWarps];      // score - lse or NaN (the beam brings no candidates), maximum
   __shared__ float s_m[kJoinWarps], s_score[kMaxBeams];  // (scores are read once: the new ones may be written over them)
   __shared__ double s_sum[kJoinWarps];
-  __shared__ unsigned s_best[kBestOfWarp * kJoinWarps];
+  __shared__ unsigned s_best[kKeys];
   __shared__ signed char s_order[kMaxBeams];             // the beams that are alive
   __shared__ double s_border;
-  __shared__ int s_segments, s_count, s_list[kListed];
+  __shared__ int s_segments, s_count, s_list[kListed], s_reached[32];
   __shared__ unsigned s_live, s_close, s_bad;
   __shared__ Ranked s_cand[kListed];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, r = blockIdx.x;
   const int segments = tiles * 32;
   const float2* request = sums + (long long)r * beams * segments;
+  if (t < kKeys) s_best[t] = 0u;
+  if (t < 32) s_reached[t] = 0;
   if (warp == 0) {
     const float score = lane < beams ? scores[(long long)r * beams + lane] : NAN;
     const bool alive = isfinite(score);
@@ -217,20 +220,20 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
   }
   __syncthreads();
   if (bad != nullptr && t < beams) bad[(long long)r * beams + t] = s_bad >> t & 1;
-  // the border: of every warp its threads' four best maxima, of those the k-th largest (at least half of the 32 warps have a beam, unless all are dead)
+  // The border: of every warp that has segments its threads' best maxima, as many as make 128 keys (four where all have some), and of those the k-th largest.
   // In 32 bits, rounded down, so that what reaches the border in 64 bits is no fewer.
-  {
-    unsigned best = w >= 0 && m > -INFINITY && !isnan(s_base[w]) ? ordered(__double2float_rd(s_base[w] + (double)m)) : 0u;
-#pragma unroll
-    for (int i = 0; i < kBestOfWarp; ++i) {
+  if (w >= 0 && share < tiles) {
+    const int with = lives * min(shares, tiles), each = min(kKeys / with, 32);
+    unsigned best = m > -INFINITY && !isnan(s_base[w]) ? ordered(__double2float_rd(s_base[w] + (double)m)) : 0u;
+    for (int i = 0; i < each; ++i) {
       const unsigned most = __reduce_max_sync(0xffffffffu, best);
       if (lane == __ffs((int)__ballot_sync(0xffffffffu, best == most)) - 1) best = 0u;
-      if (lane == i) s_best[warp * kBestOfWarp + i] = most;
+      if (lane == 0) s_best[(share * lives + turn) * each + i] = most;
     }
   }
   __syncthreads();
   {                                    // eight threads a key
-    constexpr int keys = kBestOfWarp * kJoinWarps, threads = kJoinThreads / keys;
+    constexpr int keys = kKeys, threads = kJoinThreads / keys;
     const int at = t / threads, first = t % threads;
     const unsigned key = s_best[at];
     int larger = 0;
@@ -245,26 +248,27 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
   }
   __syncthreads();
   // segments, then logits, that reach it or come closer than the sums are certain
-  const double border = s_border - kUncertain;
-  if (w >= 0 && !isnan(s_base[w]) && m > -INFINITY && s_base[w] + (double)m >= border) {
-    auto list = [&](float x, int s) {
-      if (x > -INFINITY && s_base[w] + (double)x >= border) {
-        const int at = atomicAdd(&s_segments, 1);
-        if (at < kListed) s_list[at] = w * segments + s;
-      }
-    };
+  auto list_segments = [&](double border) {
+    if (w >= 0 && !isnan(s_base[w]) && m > -INFINITY && s_base[w] + (double)m >= border) {
+      auto list = [&](float x, int s) {
+        if (x > -INFINITY && s_base[w] + (double)x >= border) {
+          const int at = atomicAdd(&s_segments, 1);
+          if (at < kListed) s_list[at] = w * segments + s;
+        }
+      };
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) list(held[i].x, s0 + i * step);
+      for (int i = 0; i < kHeld; ++i) list(held[i].x, s0 + i * step);
 #pragma unroll 8
-    for (int s = s0 + kHeld * step; s < segments; s += step) list(mine[s].x, s);
-  }
-  __syncthreads();
-  const int listed = s_segments;
+      for (int s = s0 + kHeld * step; s < segments; s += step) list(mine[s].x, s);
+    }
+    __syncthreads();
+    return s_segments;
+  };
   auto rank_of = [&](float x, int beam, int token) {
     const unsigned flat = (unsigned)beam * (unsigned)vocab + (unsigned)token;
     return Ranked{ordered(s_base[beam] + (double)x + 0.0), ((u64)ordered(x) << 32) | (unsigned)~flat};
   };
-  if (listed <= kListed) {
+  auto collect = [&](int listed, double border) {          // the listed segments' logits, two a lane
     for (int i = warp; i < listed; i += kJoinWarps) {
       const int beam = s_list[i] / segments, s = s_list[i] - beam * segments, tile = s >> 5;
       const T* row = logits + ((long long)r * beams + beam) * stride;
@@ -279,8 +283,72 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
         }
       }
     }
+    __syncthreads();
+    return s_count;
+  };
+  // A border of 32 bits that k to 2 k of what `count` counts reach, or else the largest that at least k do: count(b) is how many of the thread's reach b
+  // (ordered).
+  auto best_border = [&](auto&& count) {
+    unsigned reached = 0u;
+    for (int bit = 31; bit >= 0; --bit) {
+      const unsigned key = reached | 1u << bit;
+      const int n = __reduce_add_sync(0xffffffffu, count(key));
+      if (lane == 0 && n) atomicAdd(&s_reached[bit], n);
+      __syncthreads();
+      const int all = s_reached[bit];
+      if (all >= k) reached = key;
+      if (all >= k && all <= 2 * k) break;               // (near enough)
+    }
+    __syncthreads();
+    if (t < 32) s_reached[t] = 0;
+    if (t == 0) { s_segments = 0; s_count = 0; }
+    __syncthreads();
+    return reached == 0u ? -INFINITY : (double)unordered(reached);
+  };
+  // Where beams' scores lie far apart, few warps have the best logits, the first border is low and much would be listed: then the k-th largest of all
+  // segments' maxima is the border, and that of all listed logits where these are few segments with many logits each.  (A logit reaches b if it is no less
+  // than b - base, rounded up twice: never one too many.)  10 x 12 beams of 58,754 tokens with scores over 40 nats: 6.9 ms one after the other (see
+  // below), 30 us so.
+  double border = s_border - kUncertain;
+  int listed = list_segments(border);
+  if (listed > 2 * k + 32) {
+    border = best_border([&](unsigned b) {
+      const float least = w < 0 || isnan(s_base[w]) ? NAN : __double2float_ru(__dsub_ru((double)unordered(b), s_base[w]));
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) n += held[i].x > -INFINITY && held[i].x >= least;
+#pragma unroll 8
+      for (int s = s0 + kHeld * step; s < segments; s += step) n += mine[s].x > -INFINITY && mine[s].x >= least;
+      return n;
+    }) - kUncertain;
+    listed = list_segments(border);
   }
-  __syncthreads();
+  int n = 0;
+  if (listed <= kListed) {
+    n = collect(listed, border);
+    if (n > 4 * k + 32 && listed <= kKeyed) {
+      unsigned key[kKeyed * kSegment / kJoinThreads];
+#pragma unroll
+      for (int i = 0; i < kKeyed * kSegment / kJoinThreads; ++i) {
+        const int at = i * kJoinThreads + t, which = at / kSegment;
+        key[i] = 0u;
+        if (which < listed) {
+          const int beam = s_list[which] / segments, s = s_list[which] - beam * segments;
+          const T* row = logits + ((long long)r * beams + beam) * stride;
+          const int token = (s >> 5) * kTile + place_in_tile<T>(s & 31, at % kSegment, ((uintptr_t)row & 15) == 0);
+          const float x = token < vocab ? to_float(row[token]) : -INFINITY;
+          if (x > -INFINITY) key[i] = ordered(__double2float_rd(s_base[beam] + (double)x));
+        }
+      }
+      border = best_border([&](unsigned b) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kKeyed * kSegment / kJoinThreads; ++i) n += key[i] >= b;
+        return n;
+      }) - kUncertain;
+      n = collect(listed, border);
+    }
+  }
   const long long out = (long long)r * k;
   auto put = [&](int rank, const Ranked& e) {
     const unsigned flat = ~(unsigned)e.tie;
@@ -298,7 +366,6 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
     s = block_sum(s, s_part);
     if (t == 0) s_base[beam] = (double)s_score[beam] - (top + log(s));
   };
-  int n = s_count;
   if (listed <= kListed && n <= kListed) {
     for (int pass = 0; pass < 2; ++pass) {
       // a warp a candidate (the list's order depends on the threads' timing, the ranks do not)

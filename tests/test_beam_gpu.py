@@ -126,6 +126,21 @@ def test_select_scores_in_place(ops):
         assert torch.equal(x.cpu(), out) and torch.equal(again[0].cpu(), parents) and torch.equal(again[1].cpu(), tokens)
 
 
+@pytest.mark.parametrize("R,W,V,k", [(3, 1, 2048, 64), (1, 3, 700, 64), (40, 2, 33000, 4), (150, 2, 6000, 8), (1, 32, 70000, 64), (9, 6, 50000, 12)])
+def test_select_sizes_between(ops, R, W, V, k):
+    logits = 3 * randn(R * W, V, seed=V)
+    check_select(ops, logits, -5 * torch.rand(R, W, generator=torch.Generator().manual_seed(4)), k)
+
+
+@pytest.mark.parametrize("R,W,V,k,gap", [(2, 12, 58754, 24, 4.0), (1, 16, 13900, 32, 9.0), (3, 8, 9573, 24, 30.0), (1, 32, 40000, 64, 50.0), (2, 2, 2048, 64, 100.0),
+                                         (1, 2, 5000, 64, 100.0), (1, 32, 700, 64, 1.0), (1, 3, 151936, 64, 20.0), (2, 16, 1073, 48, 5.0)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_select_scores_far_apart(ops, R, W, V, k, gap, dtype):
+    """One or a few beams bring all that is found; with bfloat16 logits, many equal ones."""
+    scores = torch.stack([-gap * torch.randperm(W, generator=torch.Generator().manual_seed(r)).float() for r in range(R)])
+    check_select(ops, (2 * randn(R * W, V, seed=V + W)).to(dtype), scores, k)
+
+
 def test_select_two_streams_and_graph(ops):
     """Two selections on two streams at once, and a recorded one beside them, each with scratch of its own."""
     R, W, V, k = 2, 4, 60000, 8
