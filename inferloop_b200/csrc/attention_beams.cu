@@ -4,11 +4,11 @@
 // with the rows of all beams as one matrix against each distinct page, and the rows whose beam does not hold it masked.
 // Requests with many rows and much to read go to the tensor cores' tcgen05 kernel (attention_beams_tc.cu) instead; ops.py has the rule.
 //
-//   units    a warp looks at a column of the block tables for each of its groups of lanes, a lane a beam: lanes with equal pages find each
-//            other (by shuffles), and the first of them enters (page, beams that hold it, column) in the list.  Nothing need be known about who descends
-//            from whom.  A unit is 16 keys of a page.
-//   split    a cluster of S = 1..16 CTAs with GROUPS rings each shares a (request, kv head); column c goes to CTA c % S, there to the rings in
-//            turn, so that the columns that beams do not share (the latest ones) are dealt out evenly.  Every warp lists its ring's units for
+//   units    a warp looks at the pages of 16 keys (a strip) for each of its groups of lanes, a lane a beam: lanes with equal pages find each
+//            other (by shuffles), and the first of them enters (page, beams that hold it, keys) in the list: a unit.  Nothing need be known
+//            about who descends from whom.
+//   split    a cluster of S = 1..16 CTAs with GROUPS rings each shares a (request, kv head); strip c goes to CTA c % S, there to the rings in
+//            turn, so that the keys that beams do not share (the latest ones) are dealt out evenly.  Every warp lists its ring's units for
 //            itself, and until the join nobody waits for another ring.  S is the most that leaves all CTAs of the launch resident at once.
 //   loads    cp.async into rings of units, K and V, swizzled in 16-byte pieces for ldmatrix: a unit of a head is one contiguous block of
 //            memory.  A ring belongs to a team of WR warps that share its keys and have 16 rows each; only they wait for one another.
@@ -49,16 +49,16 @@ __device__ __forceinline__ float power_of_two(float x) {
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// The pages of the next columns: asked for four turns at a time, those of the first turns ahead of everything else, should the first column be the table's
+// The pages of the next strips: asked for four turns at a time, those of the first turns ahead of everything else, should the first strip be the table's
 // (with a window it is not known yet).
 constexpr int kTurns = 4;
 struct Turn { Lanes lanes; int rank, next, base; bool asked; int page[kTurns]; };
-__device__ __forceinline__ void ask_pages(const Params& p, const Job& j, Turn& x, int lo_col, int hi_col) {
+__device__ __forceinline__ void ask_pages(const Params& p, const Job& j, Turn& x, int lo_strip, int hi_strip) {
 #pragma unroll
   for (int n = 0; n < kTurns; ++n) {
-    const int column = lo_col + x.rank + p.split * ((x.base + n) * x.lanes.columns + x.lanes.c);
+    const int strip = strip_of(p, x.lanes, lo_strip, x.rank, x.base + n);
     x.page[n] = -1;
-    if (x.lanes.w < j.beams && column < hi_col) x.page[n] = p.table[(long long)(j.first_row + x.lanes.w) * p.max_blocks + column];
+    if (x.lanes.w < j.beams && strip < hi_strip) x.page[n] = p.table[(long long)(j.first_row + x.lanes.w) * p.max_blocks + block_of(p, strip)];
   }
 }
 __device__ __forceinline__ Turn first_turn(const Params& p, const Job& j, int rank) {
@@ -67,57 +67,51 @@ __device__ __forceinline__ Turn first_turn(const Params& p, const Job& j, int ra
   x.rank = rank;
   x.next = x.base = 0;
   x.asked = p.window == 0;
-  if (x.asked) ask_pages(p, j, x, 0, p.max_blocks);
+  if (x.asked) ask_pages(p, j, x, 0, p.strips);
   return x;
 }
-__device__ __forceinline__ bool more_columns(const Params& p, const Job& j, const Turn& x) {
-  return j.lo_col + x.rank + p.split * (x.next * x.lanes.columns) < j.hi_col;
+__device__ __forceinline__ bool more_strips(const Params& p, const Job& j, const Turn& x) {
+  return j.lo_strip + x.rank + p.split * (x.next * x.lanes.columns) < j.hi_strip;
 }
 
-// Lists the pages of the CTA's next columns in `list` (the warp's own; all warps of a CTA make the same list) and returns how many there are.
+// Lists the units of the CTA's next strips in `list` (the warp's own; all warps of a CTA make the same list) and returns how many there are.
 __device__ __forceinline__ int list_units(const Params& p, const Job& j, Turn& x, Listed* list, int row_bytes) {
   const int lane = threadIdx.x & 31;
   int n = 0;
   __syncwarp();
   if (!x.asked) {
-    ask_pages(p, j, x, j.lo_col, j.hi_col);
+    ask_pages(p, j, x, j.lo_strip, j.hi_strip);
     x.asked = true;
   }
-  while (n + 32 <= kList && more_columns(p, j, x)) {
+  while (n + 32 <= kList && more_strips(p, j, x)) {
 #pragma unroll
     for (int turn = 0; turn < kTurns; ++turn) {
-      if (x.base + turn != x.next || n + 32 > kList || !more_columns(p, j, x)) continue;
-      const int column = j.lo_col + x.rank + p.split * (x.next * x.lanes.columns + x.lanes.c), page = x.page[turn];
+      if (x.base + turn != x.next || n + 32 > kList || !more_strips(p, j, x)) continue;
+      const int strip = strip_of(p, x.lanes, j.lo_strip, x.rank, x.next), page = x.page[turn];
       bool first;
-      const unsigned beams = beams_of_page(x.lanes, page < p.num_pages && column < j.hi_col ? page : -1, &first);
+      const unsigned beams = beams_of_page(x.lanes, page < p.num_pages && strip < j.hi_strip ? page : -1, &first);
       const unsigned listed = __ballot_sync(0xffffffffu, first);
-      if (first) list[n + __popc(listed & ((1u << lane) - 1))] = Listed{((long long)page * p.nkv + j.kvh) * p.page_size * row_bytes, column * p.page_size, beams};
+      if (first) {
+        const int part = strip - block_of(p, strip) * p.parts;
+        list[n + __popc(listed & ((1u << lane) - 1))] =
+            Listed{(((long long)page * p.nkv + j.kvh) * p.page_size + part * kUnit) * row_bytes, strip * kUnit, beams};
+      }
       n += __popc(listed);
       ++x.next;
     }
     if (x.next == x.base + kTurns) {
       x.base += kTurns;
-      ask_pages(p, j, x, j.lo_col, j.hi_col);
+      ask_pages(p, j, x, j.lo_strip, j.hi_strip);
     }
   }
   __syncwarp();
   return n;
 }
 
-// Unit i of the list (page i / parts, its 16 keys i % parts); beams 0: there is no such unit, or nobody sees it.
-__device__ __forceinline__ Listed unit_of(const Job& j, const Listed* list, int i, int total, int parts, int unit_bytes) {
+// Unit i of the list; beams 0: there is no such unit.
+__device__ __forceinline__ Listed unit_of(const Listed* list, int i, int total) {
   Listed x{0, 0, 0};
-  if (parts == 1) {
-    if (i < total) x = list[i];
-    return x;
-  }
-  const int which = i / parts, part = i - which * parts;
-  if (which < total) {
-    x = list[which];
-    x.at += (long long)part * unit_bytes;
-    x.key0 += part * kUnit;
-    if (x.key0 >= j.key_hi || x.key0 + kUnit <= j.key_lo) x.beams = 0;
-  }
+  if (i < total) x = list[i];
   return x;
 }
 
@@ -265,7 +259,7 @@ attention_beams_kernel(Params p) {
   Job j = make_job(p);
   Turn turn = first_turn(p, j, rank);
   Listed* list = s_lists[warp];
-  const int live = j.beams * j.group, parts = p.page_size / kUnit;
+  const int live = j.beams * j.group;
   find_keys(p, j);
   float o[RB][D / 8][4], m[RB][2], l[RB][2];
 #pragma unroll
@@ -292,9 +286,9 @@ attention_beams_kernel(Params p) {
   bool asked = false;
   const bool idle = rg * RB * 16 >= live;                // none of the warp's rows is there: it only helps to copy
 
-  while (more_columns(p, j, turn)) {
-    const int total = list_units(p, j, turn, list, BYTES), steps = (total * parts + GROUPS - 1) / GROUPS;
-    auto unit = [&](int step) { return unit_of(j, list, step * GROUPS + group, total, parts, S::UNIT_BYTES); };
+  while (more_strips(p, j, turn)) {
+    const int total = list_units(p, j, turn, list, BYTES), steps = (total + GROUPS - 1) / GROUPS;
+    auto unit = [&](int step) { return unit_of(list, step * GROUPS + group, total); };
     auto load = [&](int step, int stage) {
       const Listed u = unit(step);
       if (u.beams != 0) {
@@ -575,7 +569,7 @@ attention_beams_exact_kernel(Params p) {
   Turn turn = first_turn(p, j, rank);
   Listed* list = s_lists[warp];
   find_keys(p, j);
-  const int live = j.beams * j.group, parts = p.page_size / kUnit;
+  const int live = j.beams * j.group;
   for (int x = t; x < ROWS * PIECES; x += kThreads) {
     const int i = x / PIECES, c = x - i * PIECES, w = i / j.group;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -596,14 +590,14 @@ attention_beams_exact_kernel(Params p) {
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) o[k][e] = 0.f;
   }
-  while (more_columns(p, j, turn)) {
+  while (more_strips(p, j, turn)) {
     const int total = list_units(p, j, turn, list, D * 4);
     __syncthreads();                                     // (the ring is free)
-    const int tiles = (total * parts + kExactTile - 1) / kExactTile;
+    const int tiles = (total + kExactTile - 1) / kExactTile;
     auto load = [&](int tile) {                          // a warp half of a unit's keys or values
       if (tile < tiles) {
         const int which = warp >> 2, half = warp & 1;
-        const Listed u = unit_of(j, list, tile * kExactTile + which, total, parts, kUnit * D * 4);
+        const Listed u = unit_of(list, tile * kExactTile + which, total);
         if (u.beams != 0) {
           const bool values = (warp & 2) != 0;
           const uint32_t at = ring_at + (tile % STAGES) * kTileBytes;
@@ -624,7 +618,7 @@ attention_beams_exact_kernel(Params p) {
       cp_async_wait<STAGES - 2>();
       __syncthreads();
       load(tile + STAGES - 1);
-      const Listed u = unit_of(j, list, tile * kExactTile + (lane >> 4), total, parts, kUnit * D * 4);
+      const Listed u = unit_of(list, tile * kExactTile + (lane >> 4), total);
       const int key = u.key0 + (lane & 15);
       unsigned seen[RPW], any = 0, every = 0xffffffffu;
 #pragma unroll
@@ -811,7 +805,7 @@ ILB_EXPORT int ilb_attention_beams(const void* q, void* out, int dtype, const vo
   ILB_REQUIRE(requests <= 65535 && (long long)nkv * beams <= 65535, "attention_beams: too many requests or heads");
   if (rows == 0) return 0;
   Params p{q, out, k, v, positions, table, sink, q_stride, out_stride, rows, beams, 0, 0, max_blocks, page_size, num_pages, window, nq, nkv, 1,
-           scale * kLog2e, 0u, 0xffffffffu};
+           page_size / kUnit, shift_of(page_size / kUnit), strips_of(max_blocks, page_size), scale * kLog2e, 0u, 0xffffffffu};
   if (dtype == kBF16) {
     if (scale < 0.f) { p.flip = 0x80008000u; p.scale_log2 = -p.scale_log2; }
     if (scale == 0.f) { p.keep = 0u; p.scale_log2 = 1.f; }

@@ -14,15 +14,27 @@ struct Params {
   const int* positions; const int* table; const float* sink;
   long long q_stride, out_stride;
   int rows, beams, beams_of_chunk, chunks, max_blocks, page_size, num_pages, window, nq, nkv, split;
+  int parts, parts_shift, strips;      // strips of 16 keys: of a page (shift: -1 where that is no power of two), of a block table
   float scale_log2;                    // bfloat16: of the absolute value; the sign is in the queries
   uint32_t flip, keep;                 // of queries' bits: signs, all (a scale of 0: none)
 };
+
+inline int strips_of(int max_blocks, int page_size) {     // (positions are of 31 bits)
+  const long long n = (long long)max_blocks * (page_size / kUnit);
+  return n < (1 << 27) ? (int)n : 1 << 27;
+}
+
+inline int shift_of(int x) {
+  int n = 0;
+  while ((1 << n) < x) ++n;
+  return (1 << n) == x ? n : -1;
+}
 
 // What a CTA works on, the same for both kinds of arithmetic.
 struct Job {
   int first_row, beams;                // of this chunk: row of its first beam, beams
   int kvh, group;                      // kv head, query heads of it
-  int lo_col, hi_col;                  // columns that some beam sees keys of
+  int lo_strip, hi_strip;              // strips that some beam sees keys of
   int key_lo, key_hi;                  // keys that some beam sees
   int all_lo, all_hi;                  // keys that every beam sees
   unsigned all_beams;                  // their bits
@@ -65,12 +77,13 @@ __device__ __forceinline__ void find_keys(const Params& p, Job& j) {
   j.all_lo = __reduce_max_sync(0xffffffffu, all_lo);
   j.all_hi = __reduce_min_sync(0xffffffffu, all_hi);
   if (j.key_hi <= j.key_lo) j.key_lo = j.key_hi = 0;
-  j.lo_col = j.key_lo / p.page_size;
-  j.hi_col = (j.key_hi + p.page_size - 1) / p.page_size;
+  j.lo_strip = j.key_lo / kUnit;
+  j.hi_strip = (j.key_hi - 1 + kUnit) / kUnit;           // (0 where key_hi is)
 }
 
-// A CTA's columns: rank + split * i.  A turn of a warp looks at `columns` = 32 / (beams, rounded up to a power of two) of them at once, a lane a beam.
-struct Lanes { int columns, wide, c, w; };       // columns of a turn, lanes of a column, the lane's column and beam
+// The keys are dealt out in strips of 16, whatever the pages' size (beams that hold a large page each would else leave all of it to one CTA).  A CTA's strips:
+// rank + split * i.  A turn of a warp looks at `columns` = 32 / (beams, rounded up to a power of two) of them at once, a lane a beam.
+struct Lanes { int columns, wide, c, w; };       // strips of a turn, lanes of a strip, the lane's strip and beam
 __device__ __forceinline__ Lanes make_lanes(const Job& j) {
   Lanes x;
   x.wide = 1;
@@ -80,7 +93,7 @@ __device__ __forceinline__ Lanes make_lanes(const Job& j) {
   x.w = (threadIdx.x & 31) - x.c * x.wide;
   return x;
 }
-// Which beams hold the lane's page (-1: none), and whether the lane is the first of them: every beam's page of the column, by shuffles that do not wait for
+// Which beams hold the lane's page (-1: none), and whether the lane is the first of them: every beam's page of the strip, by shuffles that do not wait for
 // one another.
 __device__ __forceinline__ unsigned beams_of_page(const Lanes& x, int page, bool* first) {
   unsigned same = 0;
@@ -95,6 +108,15 @@ __device__ __forceinline__ unsigned beams_of_page(const Lanes& x, int page, bool
   }
   *first = page >= 0 && x.w == __ffs((int)same) - 1;
   return same;
+}
+
+// The lane's strip of turn `turn`, and where its page stands in the beam's row of the block tables.
+__device__ __forceinline__ int strip_of(const Params& p, const Lanes& x, int lo_strip, int rank, int turn) {
+  return lo_strip + rank + p.split * (turn * x.columns + x.c);
+}
+__device__ __forceinline__ int block_of(const Params& p, int strip) {
+  if (p.parts_shift >= 0) return strip >> p.parts_shift;
+  return strip / p.parts;
 }
 
 }  // namespace ilb

@@ -11,7 +11,7 @@
 //   warp 1   allocates tensor memory (two S tiles of 64 columns, O of D) and issues S = Q K^T two tiles ahead and O += P V.
 //   warps 2-5  a thread a row (= tensor-memory lane): masks what its beam does not hold or see, exponentials, P as packed bfloat16 over the
 //            scores; O is rescaled only when a maximum has grown by more than 2^8.  Warps without rows leave at once.
-//   split    clusters of S CTAs share a (request, kv head) by columns of the block tables, as in attention_beams.cu; at the end every CTA leaves its rows'
+//   split    clusters of S CTAs share a (request, kv head) by strips of 16 keys, as in attention_beams.cu; at the end every CTA leaves its rows'
 //            records (maximum, sum, O) in its shared memory and row i is added up by CTA i % S.
 // Two CTAs to an SM: a tile of one row's chain (wait for S, load, exponentials, wait for O: 1,700 clocks) leaves the tensor cores and the memory idle, and a
 // second CTA fills that.  6 x 8 beams of 6000 keys, 40 rows, 48 jobs: 41.8 us, 3.6 TB/s (55 % of the measured copy rate); one CTA to an SM with tiles of 128 keys
@@ -37,7 +37,7 @@ constexpr int kRows = 128;             // MMA M
 constexpr int kKeys = 64;              // of a tile
 constexpr int kTileUnits = kKeys / kUnit;
 constexpr int kMaxPage = 128;          // tokens
-constexpr int kListed = 8 + 32 * 8;    // units: less than a tile's, and those of a turn's 32 pages
+constexpr int kListed = kTileUnits + 32;       // units: less than a tile's, and a turn's
 constexpr int kAsked = 16;             // turns that pages are asked for ahead
 constexpr int kInfos = 8;
 constexpr int kThreads = 256, kWarps = 8;
@@ -100,7 +100,7 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + kBars);
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, rank = p.split > 1 ? (int)cluster_rank() : 0;
   Job j = make_job(p);
-  const int live = j.beams * j.group, parts = p.page_size / kUnit, active = (live + 31) / 32;      // softmax warps with rows
+  const int live = j.beams * j.group, active = (live + 31) / 32;      // softmax warps with rows
   if (t == 0) {
     mbar_init(q_full, 1);
     for (int s = 0; s < kStagesK; ++s) { mbar_init(k_full + 8 * s, 1); mbar_init(k_empty + 8 * s, 1); }
@@ -120,14 +120,15 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   }
   // The block tables' entries of turn `turn` (warp 6): behind the boxes of five tiles an answer takes long, so they are asked for kAsked turns ahead.
   const Lanes lanes = make_lanes(j);
-  auto ask = [&](int turn, int lo_col, int hi_col) {
-    const int column = lo_col + rank + p.split * (turn * lanes.columns + lanes.c);
-    if (lanes.w < j.beams && column < hi_col) cp_async_4(smem_u32(&s_page[turn % kAsked][lane]), p.table + (long long)(j.first_row + lanes.w) * p.max_blocks + column);
+  auto ask = [&](int turn, int lo_strip, int hi_strip) {
+    const int strip = strip_of(p, lanes, lo_strip, rank, turn);
+    if (lanes.w < j.beams && strip < hi_strip)
+      cp_async_4(smem_u32(&s_page[turn % kAsked][lane]), p.table + (long long)(j.first_row + lanes.w) * p.max_blocks + block_of(p, strip));
     cp_async_commit();
   };
-  if (warp == 6 && p.window == 0) {                      // (with a window the first column is not known yet)
+  if (warp == 6 && p.window == 0) {                      // (with a window the first strip is not known yet)
 #pragma unroll 4
-    for (int turn = 0; turn < kAsked; ++turn) ask(turn, 0, p.max_blocks);
+    for (int turn = 0; turn < kAsked; ++turn) ask(turn, 0, p.strips);
   }
   find_keys(p, j);
   tcgen05_fence_before();
@@ -146,12 +147,12 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     const int outside = p.num_pages * p.nkv;
     if (p.window != 0) {
 #pragma unroll 4
-      for (int turn = 0; turn < kAsked; ++turn) ask(turn, j.lo_col, j.hi_col);
+      for (int turn = 0; turn < kAsked; ++turn) ask(turn, j.lo_strip, j.hi_strip);
     }
     int units = 0, taken = 0, turn = 0;                  // units in the list, of them taken by tiles
-    auto more_columns = [&] { return j.lo_col + rank + p.split * (turn * lanes.columns) < j.hi_col; };
+    auto more_strips = [&] { return j.lo_strip + rank + p.split * (turn * lanes.columns) < j.hi_strip; };
     for (int tile = 0;; ++tile) {
-      if (units - taken < kTileUnits && more_columns()) {  // what is left goes to the front, and more behind it
+      if (units - taken < kTileUnits && more_strips()) {  // what is left goes to the front, and more behind it
         const int left = units - taken;
         const int4 kept = lane < left ? s_list[taken + lane] : make_int4(0, 0, 0, 0);
         __syncwarp();
@@ -159,25 +160,20 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         units = left;
         taken = 0;
 #pragma unroll 1
-        for (; units < kTileUnits && more_columns(); ++turn) {
+        for (; units < kTileUnits && more_strips(); ++turn) {
           cp_async_wait<kAsked - 1>();
-          const int column = j.lo_col + rank + p.split * (turn * lanes.columns + lanes.c);
+          const int strip = strip_of(p, lanes, j.lo_strip, rank, turn);
           int page = -1;
-          if (lanes.w < j.beams && column < j.hi_col) page = *(volatile int*)&s_page[turn % kAsked][lane];
+          if (lanes.w < j.beams && strip < j.hi_strip) page = *(volatile int*)&s_page[turn % kAsked][lane];
           bool first;
           const unsigned beams = beams_of_page(lanes, page < p.num_pages ? page : -1, &first);
           const unsigned listed = __ballot_sync(0xffffffffu, first);
-          ask(turn + kAsked, j.lo_col, j.hi_col);
+          ask(turn + kAsked, j.lo_strip, j.hi_strip);
           if (first) {
-            const int at = units + parts * __popc(listed & ((1u << lane) - 1));
-#pragma unroll 1
-            for (int part = 0; part < parts; ++part) {
-              const int key0 = column * p.page_size + part * kUnit;
-              const bool seen = key0 < j.key_hi && key0 + kUnit > j.key_lo;
-              s_list[at + part] = make_int4(seen ? page * p.nkv + j.kvh : outside, 2 * part, key0, (int)(seen ? beams : 0u));
-            }
+            const int part = strip - block_of(p, strip) * p.parts;
+            s_list[units + __popc(listed & ((1u << lane) - 1))] = make_int4(page * p.nkv + j.kvh, 2 * part, strip * kUnit, (int)beams);
           }
-          units += parts * __popc(listed);
+          units += __popc(listed);
         }
         __syncwarp();
       }
@@ -619,8 +615,8 @@ ILB_EXPORT int ilb_attention_beams_tc(const void* q, void* out, const void* k, c
   const int requests = (rows + beams - 1) / beams;
   ILB_REQUIRE(requests <= 65535 && (long long)nkv * beams <= 65535 && (long long)num_pages * nkv < (1ll << 31) - 1, "attention_beams: too many requests, heads or pages");
   if (rows == 0) return 0;
-  Params p{q, out, k, v, positions, table, sink, q_stride, out_stride, rows, beams, 0, 0, max_blocks, page_size, num_pages, window, nq, nkv, 1, scale * kLog2e,
-           0u, 0xffffffffu};
+  Params p{q, out, k, v, positions, table, sink, q_stride, out_stride, rows, beams, 0, 0, max_blocks, page_size, num_pages, window, nq, nkv, 1, page_size / kUnit,
+           shift_of(page_size / kUnit), strips_of(max_blocks, page_size), scale * kLog2e, 0u, 0xffffffffu};
   return d == 64 ? run<64>(p, longest, error_flag, stream) : run<128>(p, longest, error_flag, stream);
 }
 ILB_PACKED(ilb_attention_beams_tc)

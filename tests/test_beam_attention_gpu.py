@@ -250,3 +250,13 @@ def test_a_cache_of_more_than_32_bits(ops, dtype):
         outs.append(torch.zeros_like(q))
         ops.attention_beams(q, outs[-1], *caches, step, torch.where(table < 0, table, table + moved).to(DEV), W, 0, d ** -0.5, nq, nkv, d)
     assert outs[0].abs().sum() > 0 and torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("page,shared", [(48, 0.7), (112, 0.5), (128, 0.0), (80, 0.0)])
+def test_large_and_odd_pages(ops, dtype, page, shared):
+    """Pages of 3, 7, 8 and 5 strips; beams that hold a page each."""
+    nq, nkv, d, W = 8, 1, 64, 8
+    k, v, table, positions = case(2, W, [301, 47], nkv, d, page, page, dtype=dtype, shared=shared)
+    check(ops, queries(2 * W, nq, d, dtype, 9), k, v, table, positions, W, 0, d ** -0.5, nq, nkv)
+    check(ops, queries(2 * W, nq, d, dtype, 9), k, v, table, positions, W, 70, d ** -0.5, nq, nkv)
