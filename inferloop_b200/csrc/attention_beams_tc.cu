@@ -14,7 +14,7 @@
 //   split    clusters of S CTAs share a (request, kv head) by strips of 16 keys, as in attention_beams.cu; at the end every CTA leaves its rows'
 //            records (maximum, sum, O) in its shared memory and row i is added up by CTA i % S.
 // Two CTAs to an SM: a tile of one row's chain (wait for S, load, exponentials, wait for O: 1,700 clocks) leaves the tensor cores and the memory idle, and a
-// second CTA fills that.  6 x 8 beams of 6000 keys, 40 rows, 48 jobs: 41.8 us, 3.6 TB/s (55 % of the measured copy rate); one CTA to an SM with tiles of 128 keys
+// second CTA fills that.  6 x 8 beams of 6000 keys, 40 rows, 48 jobs: 42.9 us, 3.5 TB/s (53 % of the measured copy rate; 5.4 TB/s in the loop); one CTA to an SM with tiles of 128 keys
 // took 47.1 (clusters of three did not all fit then).  8 x 16 of 1000: 26.0 us.
 // Bound: the same chain, at clusters' sizes that leave some SMs without work (240 CTAs of 296), and 10,000 clocks before the first tile and after the last.
 // A value that is masked for a row never reaches it: where a tile is not seen whole by all rows its values are looked at, and infinities and NaN
@@ -549,7 +549,7 @@ int clusters_at_once(int ctas, int split) {
 
 // CTAs that share a (request, kv head): as many as one to an SM allows; where that is fewer than three, as many as two to an SM allow, less a twelfth (56
 // clusters of 5, which the query grants, took a second round: 34.4 us where 4 take 29.0).  Measured with one to an SM / two: 6 x 8 beams of 6000 keys,
-// 48 jobs, 59.6 (2 CTAs) / 41.8 us (5); 8 x 16 of 1000, 64 jobs, 30.7 (2) / 26.1 (4); but 5 x 8 of 1000, 40 jobs, 18.9 (3) / 21.1 (6); 4 x 16 of
+// 48 jobs, 59.6 (2 CTAs) / 42.9 us (5); 8 x 16 of 1000, 64 jobs, 30.7 (2) / 26.1 (4); but 5 x 8 of 1000, 40 jobs, 18.9 (3) / 21.1 (6); 4 x 16 of
 // 2000, 32 jobs, 28.0 (4) / 33.6 (8); 1 x 10 of 8000, 8 jobs, 37.2 (10) / 41.9 (16).
 int split_of(long long jobs, int tiles) {
   const int most = min(kMaxSplit, max(tiles, 1));

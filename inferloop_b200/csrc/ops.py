@@ -1530,7 +1530,7 @@ def step_build(new: torch.Tensor, cached: torch.Tensor, kv_len: torch.Tensor, po
 
 
 # Which kernel reads shared pages of bfloat16, by the rows (beams of a request times query heads of a kv head) and the keys of all requests and kv heads.
-# Measured with few rows' kernel / the tcgen05 kernel: 40 rows, 6 x 8 kv heads of 6000 keys 71.5 / 41.8 us, 3 x 8 of 200 17.2 / 14.3, 36 rows, 8 of 500
+# Measured with few rows' kernel / the tcgen05 kernel: 40 rows, 6 x 8 kv heads of 6000 keys 71.5 / 42.9 us, 3 x 8 of 200 17.2 / 14.3, 36 rows, 8 of 500
 # 11.7 / 12.1; 128 rows, 16 of 4000 40.4 / 36.7, 16 of 500 27.2 / 32.1; 20 rows, 64 kv heads of 3000 36.9 / 27.1, 256 of 500 33.8 / 24.2, but 128 of 500
 # 17.8 / 18.8 and 32 of 3000 20.0 / 24.6; 16 rows, 512 of 1030 60.8 / 65.4, 64 of 4000 29.7 / 30.9.
 BEAMS_TC_ROWS, BEAMS_TC_FEW, BEAMS_TC_KEYS = 33, 17, 100_000
