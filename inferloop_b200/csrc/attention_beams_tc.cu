@@ -23,6 +23,7 @@
 #include <cuda.h>
 #include <math.h>
 #include <atomic>
+#include <type_traits>
 #include "common.cuh"
 #include "attention_beams.cuh"
 #include "packed.h"
@@ -40,6 +41,7 @@ constexpr int kMaxPage = 128;          // tokens
 constexpr int kListed = kTileUnits + 32;       // units: less than a tile's, and a turn's
 constexpr int kAsked = 16;             // turns that pages are asked for ahead
 constexpr int kInfos = 8;
+constexpr int kMaxSplit = 16;
 constexpr int kThreads = 256, kWarps = 8;
 constexpr int kPad = 8;                // floats between the records of two rows
 constexpr float kRescaleStep = 8.f;    // log2
@@ -80,12 +82,13 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     tensormap_prefetch(&map_k);
     tensormap_prefetch(&map_v);
   }
+  if (p.split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   pdl_wait();
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ int4 s_list[kListed];                       // page x kv head, group of 8 keys in the page, first key, beams
   __shared__ int s_page[kAsked][32];                     // block-table entries on their way: turn, lane
   __shared__ Info s_info[kInfos];
-  __shared__ float2 s_ml[kRows];
+  __shared__ float2 s_ml[kRows + kMaxSplit];             // maxima and sums that the cluster's CTAs have of this one's rows: [row / split][CTA]
   __shared__ unsigned s_odd[2][kKeys / 32];              // keys of an even and an odd tile whose values hold an infinity or NaN
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
@@ -141,6 +144,8 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     *there = mbar_wait(info_full + 8 * (n % kInfos), (n / kInfos) & 1);
     return *there ? *(volatile int*)&s_info[n % kInfos].state : 0;
   };
+
+  auto all_begun = [&] { if (p.split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); };      // every CTA of the cluster
 
   if (warp == 6) {
     // ---------------------------------------------------------------- units
@@ -437,8 +442,17 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         for (int c = 0; c < 32; c += 4) *reinterpret_cast<float4*>(record + c0 + c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
       }
     }
-    s_ml[row] = make_float2(m, l);
+    all_begun();
+    if (row < live) {                                    // to the CTA that adds the row up
+      const float2* to = &s_ml[row / p.split * p.split + rank];
+      if (p.split > 1) {
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(peer_addr(smem_u32(to), row % p.split)), "f"(m), "f"(l) : "memory");
+      } else {
+        s_ml[row] = make_float2(m, l);
+      }
+    }
   }
+  if (warp < 2 || warp > 5 || (warp & 3) >= active) all_begun();
   if (!ok && lane == 0 && error_flag != nullptr) *error_flag = 1;
   tcgen05_fence_before();
   __syncthreads();
@@ -449,37 +463,34 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   // row i by CTA i % split, from its peers' memory
   constexpr int E = D / 32;            // columns E lane .. E lane + E - 1
   if (p.split > 1) cluster_sync_all();
-  // (lane c has the maximum and sum of CTA c; rows of a warp two at a time, eight peers' parts of each on their way)
-  for (int i0 = rank + p.split * warp; i0 < live; i0 += 2 * p.split * kWarps) {
-    float acc[2][E], f[2], l[2];
-    const int rows[2] = {i0, min(i0 + p.split * kWarps, live - 1)};
+  // (lane c has the maximum and sum of CTA c; rows of a warp two at a time where there are two, eight peers' parts of each on their way)
+  auto add_up = [&](int i0, auto count) {
+    constexpr int N = decltype(count)::value;
+    float acc[N][E], f[N], l[N];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const uint32_t ml_at = smem_u32(&s_ml[rows[n]]);
-      float mc = -INFINITY, lc = 0.f;
-      if (lane < p.split) {
-        mc = p.split > 1 ? ld_peer_f32(ml_at, lane) : s_ml[rows[n]].x;
-        lc = p.split > 1 ? ld_peer_f32(ml_at + 4, lane) : s_ml[rows[n]].y;
-      }
-      const float sink = p.sink != nullptr ? p.sink[j.kvh * j.group + rows[n] % j.group] * kLog2e : -INFINITY;
-      const float top = fmaxf(warp_max(mc), sink), shift = top == -INFINITY ? 0.f : top;
-      f[n] = exp2f(mc - shift);
-      l[n] = warp_sum(mc == -INFINITY ? lc : lc * f[n]) + exp2f(sink - shift);
+    for (int n = 0; n < N; ++n) {
+      const int i = i0 + n * p.split * kWarps;
+      const float2 ml = lane < p.split ? s_ml[i / p.split * p.split + lane] : make_float2(-INFINITY, 0.f);
+      const float sink = p.sink != nullptr ? p.sink[j.kvh * j.group + i % j.group] * kLog2e : -INFINITY;
+      const float top = fmaxf(warp_max(ml.x), sink), shift = top == -INFINITY ? 0.f : top;
+      f[n] = exp2f(ml.x - shift);
+      l[n] = warp_sum(ml.x == -INFINITY ? ml.y : ml.y * f[n]) + exp2f(sink - shift);
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[n][e] = 0.f;
     }
     for (int c0 = 0; c0 < p.split; c0 += 8) {
-      float x[2][8][E];
+      float x[N][8][E];
 #pragma unroll
       for (int h = 0; h < 8; ++h) {
         if (c0 + h >= p.split) break;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const uint32_t at = base + (uint32_t)(rows[n] * (D + kPad) + E * lane) * 4, peer = p.split > 1 ? peer_addr(at, c0 + h) : at;
-#pragma unroll
-          for (int e = 0; e < E; e += 2) {
-            if (p.split > 1) asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x[n][h][e]), "=f"(x[n][h][e + 1]) : "r"(peer + 4 * e) : "memory");
-            else asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(x[n][h][e]), "=f"(x[n][h][e + 1]) : "r"(peer + 4 * e) : "memory");
+        for (int n = 0; n < N; ++n) {
+          const uint32_t at = base + (uint32_t)((i0 + n * p.split * kWarps) * (D + kPad) + E * lane) * 4, from = p.split > 1 ? peer_addr(at, c0 + h) : at;
+          if constexpr (E == 4) {
+            const float4 y = ld_peer_v4(from);           // (an address of the CTA's own memory is one of the cluster's too)
+            x[n][h][0] = y.x; x[n][h][1] = y.y; x[n][h][2] = y.z; x[n][h][3] = y.w;
+          } else {
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x[n][h][0]), "=f"(x[n][h][1]) : "r"(from) : "memory");
           }
         }
       }
@@ -487,7 +498,7 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       for (int h = 0; h < 8; ++h) {
         if (c0 + h >= p.split) break;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int n = 0; n < N; ++n) {
           const float fc = __shfl_sync(0xffffffffu, f[n], c0 + h);
 #pragma unroll
           for (int e = 0; e < E; ++e) acc[n][e] += fc * x[n][h][e];
@@ -495,15 +506,18 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       }
     }
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      if (n == 1 && i0 + p.split * kWarps >= live) break;
-      const int w = rows[n] / j.group, head = j.kvh * j.group + rows[n] - w * j.group;
+    for (int n = 0; n < N; ++n) {
+      const int i = i0 + n * p.split * kWarps, w = i / j.group, head = j.kvh * j.group + i - w * j.group;
       __nv_bfloat16* to = (__nv_bfloat16*)p.out + (long long)(j.first_row + w) * p.out_stride + (long long)head * D + E * lane;
       // (a sum of 0 is a row that sees nothing; the product with a rounded inverse is off by 1.5 ulp of 32 bits, the rounding to bfloat16 by 2^15)
       const float inverse = l[n] == 0.f ? 0.f : 1.f / l[n];
 #pragma unroll
       for (int e = 0; e < E; ++e) to[e] = __float2bfloat16_rn(acc[n][e] * inverse);
     }
+  };
+  for (int i0 = rank + p.split * warp; i0 < live; i0 += 2 * p.split * kWarps) {
+    if (i0 + p.split * kWarps < live) add_up(i0, std::integral_constant<int, 2>());
+    else add_up(i0, std::integral_constant<int, 1>());
   }
   if (p.split > 1) cluster_sync_all();                   // nobody leaves while a peer may still read its records
 }
@@ -522,7 +536,6 @@ int encode(CUtensorMap* out, const void* ptr, int rank, const cuuint64_t* dims, 
 // Clusters of `split` CTAs that the device holds at once with one CTA to an SM (ask = kAskOne) or two.  An empty kernel of the same shape is asked about: the
 // occupancy query counts one CTA to an SM for any kernel that allocates tensor memory.
 __global__ void __launch_bounds__(kThreads, 2) beams_shape_kernel() {}
-constexpr int kMaxSplit = 16;
 constexpr int kAskOne = 120 * 1024, kAskTwo = smem_bytes<128>() + kFixed;
 std::atomic<int> g_clusters[2][OncePerDevice::kMax][kMaxSplit + 1];      // by CTAs to an SM and device: their number and one
 
