@@ -485,12 +485,15 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         if (c0 + h >= p.split) break;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-          const uint32_t at = base + (uint32_t)((i0 + n * p.split * kWarps) * (D + kPad) + E * lane) * 4, from = p.split > 1 ? peer_addr(at, c0 + h) : at;
-          if constexpr (E == 4) {
-            const float4 y = ld_peer_v4(from);           // (an address of the CTA's own memory is one of the cluster's too)
+          const uint32_t at = (uint32_t)((i0 + n * p.split * kWarps) * (D + kPad) + E * lane) * 4;
+          if (c0 + h == rank) {                          // its own
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[n][h][e] = *reinterpret_cast<const float*>(smem + at + 4 * e);
+          } else if constexpr (E == 4) {
+            const float4 y = ld_peer_v4(peer_addr(base + at, c0 + h));
             x[n][h][0] = y.x; x[n][h][1] = y.y; x[n][h][2] = y.z; x[n][h][3] = y.w;
           } else {
-            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x[n][h][0]), "=f"(x[n][h][1]) : "r"(from) : "memory");
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x[n][h][0]), "=f"(x[n][h][1]) : "r"(peer_addr(base + at, c0 + h)) : "memory");
           }
         }
       }
