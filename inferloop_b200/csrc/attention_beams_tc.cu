@@ -11,12 +11,13 @@
 //   warp 1   allocates tensor memory (two S tiles of 64 columns, O of D) and issues S = Q K^T two tiles ahead and O += P V.
 //   warps 2-5  a thread a row (= tensor-memory lane): masks what its beam does not hold or see, exponentials, P as packed bfloat16 over the
 //            scores; O is rescaled only when a maximum has grown by more than 2^8.  Warps without rows leave at once.
-//   split    clusters of S CTAs share a (request, kv head) by strips of 16 keys, as in attention_beams.cu; at the end every CTA leaves its rows'
-//            records (maximum, sum, O) in its shared memory and row i is added up by CTA i % S.
-// Two CTAs to an SM: a tile of one row's chain (wait for S, load, exponentials, wait for O: 1,700 clocks) leaves the tensor cores and the memory idle, and a
-// second CTA fills that.  6 x 8 beams of 6000 keys, 40 rows, 48 jobs: 42.9 us, 3.5 TB/s (53 % of the measured copy rate; 5.4 TB/s in the loop); one CTA to an SM with tiles of 128 keys
-// took 47.1 (clusters of three did not all fit then).  8 x 16 of 1000: 26.0 us.
-// Bound: the same chain, at clusters' sizes that leave some SMs without work (240 CTAs of 296), and 10,000 clocks before the first tile and after the last.
+//   split    clusters of S CTAs share a (request, kv head) by strips of 16 keys, as in attention_beams.cu; at the end every CTA leaves O of
+//            its rows in its shared memory, sends their maxima and sums to the rows' owners, and row i is added up by CTA i % S.
+// Two CTAs to an SM: a tile's chain (wait for S, load, exponentials, wait for O: 1,700 clocks) leaves the tensor cores and the memory idle, and a second CTA fills
+// that (one, with tiles of 128 keys, took 47.1 where two took 41.8).  6 x 8 beams of 6000 keys, 40 rows, 48 jobs: 37.7 us, 4.0 TB/s (61 % of the measured copy
+// rate; 5.4 TB/s in the loop).  8 x 16 of 1000: 24.4 us.
+// Bound: memory in the loop; 7,500 clocks before the first tile's scores and about as many behind the last, and SMs without work where jobs and splits do not fill
+// them (240 CTAs of 296 here).
 // A value that is masked for a row never reaches it: where a tile is not seen whole by all rows its values are looked at, and infinities and NaN
 // are added by hand to the rows that see them and taken out of the tile before the product.
 // Every mbarrier wait is bounded; on expiry a flag is raised and the CTA still walks through the cluster's barriers.  No multicast.
@@ -536,22 +537,22 @@ int encode(CUtensorMap* out, const void* ptr, int rank, const cuuint64_t* dims, 
   return 0;
 }
 
-// Clusters of `split` CTAs that the device holds at once with one CTA to an SM (ask = kAskOne) or two.  An empty kernel of the same shape is asked about: the
-// occupancy query counts one CTA to an SM for any kernel that allocates tensor memory.
+// Clusters of `split` CTAs that the device holds at once, two CTAs to an SM.  An empty kernel of the same shape is asked about: the occupancy query counts one
+// CTA to an SM for any kernel that allocates tensor memory.
 __global__ void __launch_bounds__(kThreads, 2) beams_shape_kernel() {}
-constexpr int kAskOne = 120 * 1024, kAskTwo = smem_bytes<128>() + kFixed;
-std::atomic<int> g_clusters[2][OncePerDevice::kMax][kMaxSplit + 1];      // by CTAs to an SM and device: their number and one
+constexpr int kAsk = smem_bytes<128>() + kFixed;
+std::atomic<int> g_clusters[OncePerDevice::kMax][kMaxSplit + 1];         // by device: their number and one
 
-int clusters_at_once(int ctas, int split) {
+int clusters_at_once(int split) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= OncePerDevice::kMax) dev = 0;
-  std::atomic<int>& known = g_clusters[ctas - 1][dev][split];
+  std::atomic<int>& known = g_clusters[dev][split];
   const int n = known.load(std::memory_order_relaxed);
   if (n) return n - 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(split, 64, 8);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = ctas == 1 ? kAskOne : kAskTwo;
+  cfg.dynamicSmemBytes = kAsk;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
@@ -563,17 +564,13 @@ int clusters_at_once(int ctas, int split) {
   return found;
 }
 
-// CTAs that share a (request, kv head): as many as one to an SM allows; where that is fewer than three, as many as two to an SM allow, less a twelfth (56
-// clusters of 5, which the query grants, took a second round: 34.4 us where 4 take 29.0).  Measured with one to an SM / two: 6 x 8 beams of 6000 keys,
-// 48 jobs, 59.6 (2 CTAs) / 42.9 us (5); 8 x 16 of 1000, 64 jobs, 30.7 (2) / 26.1 (4); but 5 x 8 of 1000, 40 jobs, 18.9 (3) / 21.1 (6); 4 x 16 of
-// 2000, 32 jobs, 28.0 (4) / 33.6 (8); 1 x 10 of 8000, 8 jobs, 37.2 (10) / 41.9 (16).
+// CTAs that share a (request, kv head): as many as run at once, less a twelfth (56 clusters of 5, which the query grants, take a second round: 29.8 us where 4 take
+// 27.9).  Fewer were never faster, us at 1, 2, 3, ... CTAs: 6 x 8 beams of 6000 keys, 48 jobs, 106, 61, 51, 43, 37.8; 5 x 8 of 1000, 40 jobs, 34, 23, 19.0,
+// 18.6, 16.7, 16.4; 4 x 16 of 2000, 32 jobs, 67, 40, 32, 27.7, 26.0, 24.8, (8) 24.1; 1 x 10 of 8000, 8 jobs, (10) 31.9, (16) 30.3.
 int split_of(long long jobs, int tiles) {
-  const int most = min(kMaxSplit, max(tiles, 1));
-  int one = most, two = most;
-  while (one > 1 && clusters_at_once(1, one) < jobs) --one;
-  if (one >= min(3, most)) return one;
-  while (two > 1 && clusters_at_once(2, two) * 11 / 12 < jobs) --two;
-  return max(one, two);
+  int split = min(kMaxSplit, max(tiles, 1));
+  while (split > 1 && clusters_at_once(split) * 11 / 12 < jobs) --split;
+  return split;
 }
 
 template <typename Kernel>
@@ -590,7 +587,7 @@ int run(Params& p, int longest, int* error_flag, cudaStream_t stream) {
   static OncePerDevice once;
   const cudaError_t set = once.run([] {
     cudaError_t e = configure(attention_beams_tc_kernel<D>, smem_bytes<D>());
-    return e == cudaSuccess ? configure(beams_shape_kernel, kAskOne) : e;
+    return e == cudaSuccess ? configure(beams_shape_kernel, kAsk) : e;
   });
   if (set != cudaSuccess) return check_launch("attention_beams");
   const int group = p.nq / p.nkv, requests = (p.rows + p.beams - 1) / p.beams, most = kRows / group;

@@ -1530,10 +1530,10 @@ def step_build(new: torch.Tensor, cached: torch.Tensor, kv_len: torch.Tensor, po
 
 
 # Which kernel reads shared pages of bfloat16, by the rows (beams of a request times query heads of a kv head) and the keys of all requests and kv heads.
-# Measured with few rows' kernel / the tcgen05 kernel: 40 rows, 6 x 8 kv heads of 6000 keys 71.5 / 42.9 us, 3 x 8 of 200 17.2 / 14.3, 36 rows, 8 of 500
-# 11.7 / 12.1; 128 rows, 16 of 4000 40.4 / 36.7, 16 of 500 27.2 / 32.1; 20 rows, 64 kv heads of 3000 36.9 / 27.1, 256 of 500 33.8 / 24.2, but 128 of 500
-# 17.8 / 18.8 and 32 of 3000 20.0 / 24.6; 16 rows, 512 of 1030 60.8 / 65.4, 64 of 4000 29.7 / 30.9.
-BEAMS_TC_ROWS, BEAMS_TC_FEW, BEAMS_TC_KEYS = 33, 17, 100_000
+# Measured with few rows' kernel / the tcgen05 kernel: 40 rows, 6 x 8 kv heads of 6000 keys 71.5 / 37.7 us, 3 x 8 of 200 17.0 / 13.2, 36 rows, 8 of 500
+# 11.6 / 9.5; 128 rows, 16 of 4000 40.0 / 31.2, 16 of 500 27.2 / 30.2; 20 rows, 64 kv heads of 3000 36.9 / 25.9, 256 of 500 33.8 / 25.7, 32 of 3000
+# 20.4 / 18.9, but 128 of 500 18.0 / 19.5 and 8 of 3000 13.4 / 14.8; 16 rows, 512 of 1030 61.1 / 67.2, 64 of 4000 30.0 / 29.6.
+BEAMS_TC_ROWS, BEAMS_TC_FEW, BEAMS_TC_KEYS = 33, 17, 90_000
 # Keys and values that a layer's beams read, each by itself, from which reading shared pages once pays for a launch more and a longer start than those of
 # attention_decode_fused.  Steps of 16 layers with groups of 2 / 4 / 5 / 8 query heads, what sharing gains a layer in us: 8 x 4 beams of 1,230 keys
 # (161 MB) 7.4 / 6.5 / 3.1 / 2.9; 16 x 4 of 630 (165 MB) 6.2 / 4.4 / 1.7 / 2.0; 4 x 4 of 2,030 (133 MB) -0.8 / -1.4 / 2.7 / 2.5; 8 x 8 of 330
