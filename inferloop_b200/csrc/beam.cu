@@ -116,7 +116,8 @@ __device__ __forceinline__ bool above(const Ranked& a, const Ranked& b) { return
 // about one step of one request in a thousand.
 constexpr double kUncertain = 8e-6;
 constexpr int kJoinThreads = 1024, kJoinWarps = kJoinThreads / 32;
-constexpr int kListed = 1024;          // segments, and candidates, that the lists hold
+constexpr int kListed = 1024;          // candidates that the list holds, and segments whose logits are looked at
+constexpr int kFound = 4096;           // segments that their list holds
 constexpr int kKeyed = 128;            // segments whose logits fit eight registers a thread
 constexpr int kKeys = 128;             // warps' best maxima that the border is found from
 constexpr int kHeld = 10;              // segments that a thread keeps (all of them at four beams of 151,936 tokens)
@@ -147,7 +148,7 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
   __shared__ unsigned s_best[kKeys];
   __shared__ signed char s_order[kMaxBeams];             // the beams that are alive
   __shared__ double s_border;
-  __shared__ int s_segments, s_count, s_list[kListed], s_reached[32];
+  __shared__ int s_segments, s_count, s_list[kFound], s_reached[32];
   __shared__ unsigned s_live, s_close, s_bad;
   __shared__ Ranked s_cand[kListed];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, r = blockIdx.x;
@@ -256,7 +257,7 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
       auto list = [&](float x, int s) {
         if (x > -INFINITY && s_base[w] + (double)x >= border) {
           const int at = atomicAdd(&s_segments, 1);
-          if (at < kListed) s_list[at] = w * segments + s;
+          if (at < kFound) s_list[at] = w * segments + s;
         }
       };
 #pragma unroll
@@ -309,21 +310,36 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
     return reached == 0u ? -INFINITY : (double)unordered(reached);
   };
   // Where beams' scores lie far apart, few warps have the best logits, the first border is low and much would be listed: then the k-th largest of all
-  // segments' maxima is the border, and that of all listed logits where these are few segments with many logits each.  (A logit reaches b if it is no less
-  // than b - base, rounded up twice: never one too many.)  10 x 12 beams of 58,754 tokens with scores over 40 nats: 6.9 ms one after the other (see
+  // segments' maxima is the border, and that of all listed logits where these are few segments with many logits each.  (Of segments that are too many for
+  // the list a maximum reaches b if it is no less than b - base, rounded up twice: never one too many.)  10 x 12 beams of 58,754 tokens with scores over 40 nats: 6.9 ms one after the other (see
   // below), 30 us so.
   double border = s_border - kUncertain;
   int listed = list_segments(border);
   if (listed > 2 * k + 32) {
-    border = best_border([&](unsigned b) {
-      const float least = w < 0 || isnan(s_base[w]) ? NAN : __double2float_ru(__dsub_ru((double)unordered(b), s_base[w]));
-      int n = 0;
+    if (listed <= kFound) {
+      unsigned key[kFound / kJoinThreads];
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) n += held[i].x > -INFINITY && held[i].x >= least;
+      for (int i = 0; i < kFound / kJoinThreads; ++i) {
+        const int at = i * kJoinThreads + t;
+        key[i] = at < listed ? ordered(__double2float_rd(s_base[s_list[at] / segments] + (double)request[s_list[at]].x)) : 0u;
+      }
+      border = best_border([&](unsigned b) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kFound / kJoinThreads; ++i) n += key[i] >= b;
+        return n;
+      }) - kUncertain;
+    } else {
+      border = best_border([&](unsigned b) {
+        const float least = w < 0 || isnan(s_base[w]) ? NAN : __double2float_ru(__dsub_ru((double)unordered(b), s_base[w]));
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) n += held[i].x > -INFINITY && held[i].x >= least;
 #pragma unroll 8
-      for (int s = s0 + kHeld * step; s < segments; s += step) n += mine[s].x > -INFINITY && mine[s].x >= least;
-      return n;
-    }) - kUncertain;
+        for (int s = s0 + kHeld * step; s < segments; s += step) n += mine[s].x > -INFINITY && mine[s].x >= least;
+        return n;
+      }) - kUncertain;
+    }
     listed = list_segments(border);
   }
   int n = 0;
