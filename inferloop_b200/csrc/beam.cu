@@ -8,8 +8,8 @@
 // that a thread took its maximum and its sum of exponentials: no list, no sort, no barrier, so that it runs at the rate of the memory.  The second, a
 // CTA a request, adds up the sums, finds a border that at least k candidates reach (the k-th largest of the best threads' maxima of every warp, or, where
 // that lets much through, of all segments), and reads again only the segments whose maxima reach it: about 2 k of them.
-// Bound: the logits' bytes.  64 x 4 rows of 151,936 float32 logits: the first launch 28.6 us, 5.4 TB/s (0.83 of the measured copy rate), both 34.2; 1 x 4 rows: 9.7,
-// the chain of loads, sums and barriers of the two (4 and 5 us).
+// Bound: the logits' bytes.  64 x 4 rows of 151,936 float32 logits: the first launch 28.6 us, 5.4 TB/s (0.83 of the measured copy rate), both 34.0, of bfloat16
+// 24.2 (instructions); 1 x 4 rows: 10.2, the chain of loads, sums and barriers of the two (4 and 5 us).
 //
 // beam_keep: which of the candidates go on as beams and which are finished, one warp a request (a few reads in a row, then as many writes).
 //
@@ -49,12 +49,33 @@ constexpr int kSegment = 64;           // logits of a thread
 constexpr int kTile = 32 * kSegment;   // of a warp
 constexpr int kSegmentThreads = 256;
 
-// Token of element i of a lane's segment in its tile: whole vectors of 16 bytes side by side over the warp where the row lies on a 16-byte
-// boundary, else single values.
+// Tiles of a row, wherever it begins.
+__host__ __device__ constexpr int tiles_of(int vocab) { return (vocab + 7 + kTile - 1) / kTile; }
+
+// A row is looked at in vectors of 16 bytes from the 16-byte boundary at or before its start, `lead` elements before it.
 template <typename T>
-__device__ __forceinline__ int place_in_tile(int lane, int i, bool vectors) {
+__device__ __forceinline__ int lead_of(const T* row) { return (int)(((uintptr_t)row & 15) / sizeof(T)); }
+// Where element i of a lane's segment lies in its tile: whole vectors side by side over the warp.
+template <typename T>
+__device__ __forceinline__ int place_in_tile(int lane, int i) {
   constexpr int VEC = 16 / (int)sizeof(T);
-  return vectors ? ((i / VEC) * 32 + lane) * VEC + i % VEC : i * 32 + lane;
+  return ((i / VEC) * 32 + lane) * VEC + i % VEC;
+}
+__device__ __forceinline__ float power_of_two(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Maximum and sum of exp(x - maximum) of 64 logits: sums of eight in turn, then in pairs (eleven roundings).  An infinity less itself, and NaN, make the sum NaN.
+__device__ __forceinline__ float2 sum_of(const float (&v)[kSegment]) {
+  float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sum[8] = {};
+#pragma unroll
+  for (int i = 0; i < kSegment; ++i) part[i & 3] = fmaxf(part[i & 3], v[i]);
+  const float m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) + 0.f, base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int i = 0; i < kSegment; ++i) sum[i & 7] += power_of_two((v[i] - base) * 1.4426950408889634f);
+  return make_float2(m, ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7])));
 }
 
 // sums [rows][tiles * 32] = (maximum, sum of exp(x - maximum)) of every segment; a sum of NaN marks NaN or +inf among its logits.
@@ -63,46 +84,38 @@ __global__ void __launch_bounds__(kSegmentThreads)
 beam_segments_kernel(const T* __restrict__ logits, long long stride, int rows, int vocab, int tiles, float2* __restrict__ sums) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int VEC = 16 / (int)sizeof(T);
+  constexpr int VEC = 16 / (int)sizeof(T), VECTORS = kSegment / VEC;
   const int lane = threadIdx.x & 31;
   const long long tile = (long long)blockIdx.x * (kSegmentThreads / 32) + (threadIdx.x >> 5);
   if (tile >= (long long)rows * tiles) return;
-  const int row = (int)(tile / tiles), first = (int)(tile - (long long)row * tiles) * kTile;
-  const T* x = logits + (long long)row * stride + first;
-  const bool vectors = ((uintptr_t)(logits + (long long)row * stride) & 15) == 0;
+  const int row = (int)(tile / tiles);
+  const T* x = logits + (long long)row * stride;
+  const int lead = lead_of(x), first = (int)(tile - (long long)row * tiles) * kTile - lead;      // token of the tile's first place
+  uint4 raw[VECTORS];
+  if (first >= 0 && first + kTile <= vocab) {
+#pragma unroll
+    for (int j = 0; j < VECTORS; ++j) raw[j] = *reinterpret_cast<const uint4*>(x + first + (j * 32 + lane) * VEC);
+  } else {                             // the row's ends: -inf beyond them
+#pragma unroll
+    for (int j = 0; j < VECTORS; ++j) {
+      const int at = first + (j * 32 + lane) * VEC;
+      if (at >= 0 && at + VEC <= vocab) {
+        raw[j] = *reinterpret_cast<const uint4*>(x + at);
+      } else {
+        T* e = reinterpret_cast<T*>(&raw[j]);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) e[i] = at + i >= 0 && at + i < vocab ? x[at + i] : from_float<T>(-INFINITY);
+      }
+    }
+  }
   float v[kSegment];
-  if (vectors && first + kTile <= vocab) {
-    uint4 raw[kSegment / VEC];
 #pragma unroll
-    for (int j = 0; j < kSegment / VEC; ++j) raw[j] = *reinterpret_cast<const uint4*>(x + (j * 32 + lane) * VEC);
+  for (int j = 0; j < VECTORS; ++j) {
+    const T* e = reinterpret_cast<const T*>(&raw[j]);
 #pragma unroll
-    for (int j = 0; j < kSegment / VEC; ++j) {
-      const T* e = reinterpret_cast<const T*>(&raw[j]);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j * VEC + i] = to_float(e[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kSegment; ++i) {
-      const int at = place_in_tile<T>(lane, i, vectors);
-      v[i] = first + at < vocab ? to_float(x[at]) : -INFINITY;
-    }
+    for (int i = 0; i < VEC; ++i) v[j * VEC + i] = to_float(e[i]);
   }
-  float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-  for (int i = 0; i < kSegment; ++i) part[i & 3] = fmaxf(part[i & 3], v[i]);
-  const float m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) + 0.f, base = m == -INFINITY ? 0.f : m;
-  // the sum in pairs: 64 terms take six roundings (an infinity less itself, and NaN, make it NaN)
-#pragma unroll
-  for (int i = 0; i < kSegment; ++i) {
-    const float t = (v[i] - base) * 1.4426950408889634f;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v[i]) : "f"(t));
-  }
-#pragma unroll
-  for (int n = 1; n < kSegment; n *= 2)
-#pragma unroll
-    for (int i = 0; i < kSegment; i += 2 * n) v[i] += v[i + n];
-  sums[tile * 32 + lane] = make_float2(m, v[0]);
+  sums[tile * 32 + lane] = sum_of(v);
 }
 
 // ------------------------------------------------------------------ beam_select: the rows of a request joined
@@ -110,11 +123,11 @@ struct Ranked { u64 score, tie; };      // the score's order, then (logit's orde
 __device__ __forceinline__ bool above(const Ranked& a, const Ranked& b) { return a.score > b.score || (a.score == b.score && a.tie > b.tie); }
 
 // The first launch's sums of exponentials are of 32 bits.  A term at distance d below the maximum is off by (2^-23 + 2^-26) d (difference,
-// product, the constant's last bits) and 2^-22 (each of three exponentials), a segment's sum by 6 roundings, that of ten segments by 11 more
-// (further sums are of 64 bits): with sum p d <= ln(vocab) that is 3.9e-6 for up to 4 M tokens, and two beams are in order for sure when their
+// product, the constant's last bits) and 2^-22 (each of three exponentials), a segment's sum by 11 roundings, that of ten segments by 11 more
+// (further sums are of 64 bits): with sum p d <= ln(vocab) that is 4.1e-6 for up to 4 M tokens, and two beams are in order for sure when their
 // scores differ by twice as much.  Where candidates of two beams that matter come closer, those beams' sums are taken once more, in 64 bits:
 // about one step of one request in a thousand.
-constexpr double kUncertain = 8e-6;
+constexpr double kUncertain = 9e-6;
 constexpr int kJoinThreads = 1024, kJoinWarps = kJoinThreads / 32;
 constexpr int kListed = 1024;          // candidates that the list holds, and segments whose logits are looked at
 constexpr int kFound = 4096;           // segments that their list holds
@@ -276,11 +289,11 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
     for (int i = warp; i < listed; i += kJoinWarps) {
       const int beam = s_list[i] / segments, s = s_list[i] - beam * segments, tile = s >> 5;
       const T* row = logits + ((long long)r * beams + beam) * stride;
-      const bool vectors = ((uintptr_t)row & 15) == 0;
+      const int first = tile * kTile - lead_of(row);
 #pragma unroll
       for (int e = lane; e < kSegment; e += 32) {
-        const int token = tile * kTile + place_in_tile<T>(s & 31, e, vectors);
-        const float x = token < vocab ? to_float(row[token]) + 0.f : -INFINITY;
+        const int token = first + place_in_tile<T>(s & 31, e);
+        const float x = token >= 0 && token < vocab ? to_float(row[token]) + 0.f : -INFINITY;
         if (x > -INFINITY && s_base[beam] + (double)x >= border) {
           const int at = atomicAdd(&s_count, 1);
           if (at < kListed) s_cand[at] = rank_of(x, beam, token);
@@ -312,7 +325,7 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
   // Where beams' scores lie far apart, few warps have the best logits, the first border is low and much would be listed: then the k-th largest of all
   // segments' maxima is the border, and that of all listed logits where these are few segments with many logits each.  (Of segments that are too many for
   // the list a maximum reaches b if it is no less than b - base, rounded up twice: never one too many.)  10 x 12 beams of 58,754 tokens with scores over 40 nats: 6.9 ms one after the other (see
-  // below), 30 us so.
+  // below), 22 us so.
   double border = s_border - kUncertain;
   int listed = list_segments(border);
   if (listed > 2 * k + 32) {
@@ -354,8 +367,8 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
         if (which < listed) {
           const int beam = s_list[which] / segments, s = s_list[which] - beam * segments;
           const T* row = logits + ((long long)r * beams + beam) * stride;
-          const int token = (s >> 5) * kTile + place_in_tile<T>(s & 31, at % kSegment, ((uintptr_t)row & 15) == 0);
-          const float x = token < vocab ? to_float(row[token]) : -INFINITY;
+          const int token = (s >> 5) * kTile - lead_of(row) + place_in_tile<T>(s & 31, at % kSegment);
+          const float x = token >= 0 && token < vocab ? to_float(row[token]) : -INFINITY;
           if (x > -INFINITY) key[i] = ordered(__double2float_rd(s_base[beam] + (double)x));
         }
       }
@@ -460,14 +473,14 @@ beam_join_kernel(const T* __restrict__ logits, long long stride, const float2* _
 }  // namespace
 
 // Elements (of 8 bytes) of the scratch that ilb_beam_select needs.
-ILB_EXPORT long long ilb_beam_select_scratch(long long rows, int vocab) { return rows * ((vocab + kTile - 1) / kTile) * 32; }
+ILB_EXPORT long long ilb_beam_select_scratch(long long rows, int vocab) { return rows * tiles_of(vocab) * 32; }
 
 ILB_EXPORT int ilb_beam_select(const void* logits, int dtype, long long stride, const float* scores, int* parents, int* tokens, float* out_scores,
                                int* bad, int requests, int beams, int vocab, int k, void* sums, cudaStream_t stream) {
   ILB_REQUIRE(requests >= 0 && beams > 0 && beams <= kMaxBeams && vocab > 0 && vocab <= kMaxVocab && k > 0 && k <= kMaxBest && stride >= vocab,
               "beam_select: bad sizes (up to %d beams, %d candidates and a vocabulary of %d)", kMaxBeams, kMaxBest, kMaxVocab);
   ILB_REQUIRE(dtype == kF32 || dtype == kBF16, "beam_select: unknown element type %d", dtype);
-  const int tiles = (vocab + kTile - 1) / kTile;
+  const int tiles = tiles_of(vocab);
   const long long rows = (long long)requests * beams, blocks = (rows * tiles + kSegmentThreads / 32 - 1) / (kSegmentThreads / 32);
   ILB_REQUIRE(rows < (1 << 24) && blocks < (1ll << 31), "beam_select: too many rows");
   if (requests == 0) return 0;

@@ -1309,7 +1309,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, parents: torch.Tenso
     if stride < vocab:
         raise KernelError("beam_select: rows of logits overlap")
     code, stream = _code(logits), torch._C._cuda_getCurrentRawStream(index)
-    need = rows * -(-vocab // 2048) * 32 * 8             # (maximum and sum of every segment of 64 logits)
+    need = rows * -(-(vocab + 7) // 2048) * 32 * 8       # (maximum and sum of every segment of 64 logits, wherever a row begins)
     # (one scratch per device and stream; a graph that is being recorded gets its own, which its memory pool keeps)
     held = None if _recording() else _BEAM_SCRATCH.get((index, stream))
     if held is None or held.numel() < need:

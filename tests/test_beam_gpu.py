@@ -422,3 +422,21 @@ def test_refusals(ops):
     for args in ((*c, None, track, 3, 3), (*c, None, track, 2, 2), (z(1, 8), *c[1:], None, track, 0, 3), (c[0], c[1], c[1], None, track, 0, 3)):
         with pytest.raises(ops.KernelError):
             ops.beam_keep(*args)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [2041, 2048, 2049, 4089, 6144, 1])
+def test_select_rows_that_begin_anywhere(ops, dtype, V):
+    """Rows at every place of a 16-byte vector, the best tokens at their ends."""
+    for offset in range(0, 9, 1 if V == 2041 else 4):
+        base = torch.full((6, V + 16), 50.0)                # (what lies beside a row is larger than all of it)
+        base[:, offset:offset + V] = 2 * randn(6, V, seed=V + offset)
+        for w in range(6):
+            base[w, offset] += 4.0 + w / 16
+            base[w, offset + V - 1] += 4.5 + w / 32
+        x = base.to(dtype).to(DEV)[:, offset:offset + V]
+        parents, tokens, out, bad = select(ops, x, torch.zeros(2, 3), 5)
+        found, flags = plain.select(x.cpu(), torch.zeros(2, 3), 5)
+        for r, (p, t, s) in enumerate(found):
+            assert parents[r].tolist() == p and tokens[r].tolist() == t and not bad.any()
+            assert all(a == b or abs(a - b) <= 2e-5 + 2 ** -23 * abs(b) for a, b in zip(out[r].tolist(), s))
