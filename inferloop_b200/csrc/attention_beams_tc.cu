@@ -430,9 +430,10 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         tcgen05_fence_before();
         mbar_arrive(p_full + 8 * (u & 1));
     }
-    if (ok && u > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done, (u - 1) & 1));
+    // The row's record takes the place of queries and keys: once the last product has read them, or, in a CTA without a tile (its request is shorter than the
+    // launch's longest), once the queries, which nothing else there waits for, have come.
+    if (ok) ok = __all_sync(0xffffffffu, u > 0 ? mbar_wait(o_done, (u - 1) & 1) : mbar_wait(q_full, 0));
     tcgen05_fence_after();
-    // the row's record, where queries and keys were
     float* record = reinterpret_cast<float*>(smem) + (size_t)row * (D + kPad);
 #pragma unroll 1
     for (int c0 = 0; c0 < D; c0 += 32) {
