@@ -14,8 +14,10 @@
 //            memory.  A ring belongs to a team of WR warps that share its keys and have 16 rows each; only they wait for one another.
 //   bfloat16 mma.sync m16n8k16.  A warp has a long chain of short steps for every unit (fragments, products, maxima, exponentials, products), so the next
 //            unit's scores are asked for before this one's softmax, and the running maximum is only raised, the sums rescaled, when a score
-//            exceeds it by 2^8: weights stay below 256, and most units need no exchange between lanes.  Sums in 32 bits.
+//            exceeds it by 2^8, and most units need no exchange between lanes.  Weights are rounded to bfloat16 for the second product, as its operand
+//            must be (half a step, 2^-8, of each); the sums that divide it are of the unrounded ones, in 32 bits.
 //   float32  fused multiply-adds, a lane a key for the scores and columns for the values; rows of the matrix dealt out to the warps.
+//   range    weights are 2^-16 at most (kLift, kLeast), so that no sum of finite values passes the type's largest on the way to a mean that does not.
 //   join     the rings' records (maximum, sum, O) of a row meet in shared memory; the CTA's record of row i is sent to CTA i % S of the cluster,
 //            which adds up its rows in the order of the ranks.  The cluster's first barrier is passed at the start and only waited for before the
 //            records are sent, the second stands between sending and adding.  No scratch buffer, no tickets, no atomics.
@@ -137,8 +139,9 @@ __device__ __forceinline__ void get(float (&x)[E], const float* from) {
   }
 }
 
-// `records` [GROUPS][ROWS][D + kPad] with `ml` [GROUPS][ROWS] = (maximum in units of log2, sum), what each ring made of each row -> the rows' outputs.  `inbox`
+// `records` [GROUPS][ROWS][D + kPad] with `ml` [GROUPS][ROWS] = (reference in units of log2, sum), what each ring made of each row -> the rows' outputs.  `inbox`
 // [ROWS / split][split][D + kPad] with inbox_ml: what the CTAs of the cluster send about the rows that this one owns.
+constexpr float kUnitF32 = 0x1p-16f;   // float32: what the largest weight is (a factor, which costs no rounding where a reference off the maximum would)
 template <typename T, int D, int ROWS, int GROUPS, int WARPS>
 __device__ __forceinline__ void join(const Params& p, const Job& j, const float* records, const float2* ml, float* inbox, float2* inbox_ml, int rank) {
   constexpr int E = D / 32;            // columns E lane .. E lane + E - 1
@@ -149,7 +152,7 @@ __device__ __forceinline__ void join(const Params& p, const Job& j, const float*
     if (p.sink != nullptr) {
       const float sink = p.sink[head] * kLog2e, all = fmaxf(top, sink), base = all == -INFINITY ? 0.f : all;
       scale = exp2f(top - base);
-      l = l * scale + exp2f(sink - base);
+      l = l * scale + exp2f(sink - base) * (sizeof(T) == 4 ? kUnitF32 : 1.f);
     }
     T* to = (T*)p.out + (long long)(j.first_row + w) * p.out_stride + (long long)head * D + E * lane;
     // a sum of 0 is a row that sees nothing
@@ -238,8 +241,6 @@ struct Shape {
   static constexpr int RECORDS = GROUPS * ROWS * (D + kPad) * 4, INBOX = (ROWS + kSpare) * (D + kPad) * 4;
   static constexpr int RINGS = GROUPS * RING_BYTES > RECORDS ? GROUPS * RING_BYTES : RECORDS, SMEM = RINGS + INBOX + 256;
 };
-constexpr float kHeadroom = 8.f;       // log2 of what a weight may be
-
 template <int D, int RB, int WR, int GROUPS, int STAGES, int CTAS>
 __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS)
 attention_beams_kernel(Params p) {
@@ -430,7 +431,7 @@ attention_beams_kernel(Params p) {
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             mx[b][r] = fmaxf(fmaxf(s[b][0][2 * r], s[b][0][2 * r + 1]), fmaxf(s[b][1][2 * r], s[b][1][2 * r + 1]));
-            rises |= mx[b][r] * p.scale_log2 > m[b][r] + kHeadroom;
+            rises |= mx[b][r] * p.scale_log2 > m[b][r] - kLeast;
           }
         if (__any_sync(0xffffffffu, rises)) {
 #pragma unroll
@@ -440,7 +441,7 @@ attention_beams_kernel(Params p) {
               float x = mx[b][r];
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-              const float m_new = fmaxf(m[b][r], x == -INFINITY ? -INFINITY : x * p.scale_log2);
+              const float m_new = fmaxf(m[b][r], x == -INFINITY ? -INFINITY : x * p.scale_log2 + kLift);
               const float corr = m_new == -INFINITY ? 1.f : power_of_two(m[b][r] - m_new);
               m[b][r] = m_new;
               l[b][r] *= corr;
@@ -652,7 +653,7 @@ attention_beams_exact_kernel(Params p) {
         s[k] = (seen[k] >> lane) & 1 ? s[k] * p.scale_log2 : -INFINITY;
         const float m_new = fmaxf(m[k], warp_max(s[k])), base = m_new == -INFINITY ? 0.f : m_new;
         const float corr = exp2f(m[k] - base);
-        s[k] = exp2f(s[k] - base);
+        s[k] = exp2f(s[k] - base) * kUnitF32;
         l[k] = l[k] * corr + s[k];
         m[k] = m_new;
 #pragma unroll

@@ -8,6 +8,10 @@ namespace ilb {
 constexpr int kMaxBeams = 32;
 constexpr int kUnit = 16;              // keys
 constexpr float kLog2e = 1.4426950408889634f;
+// Log2 of the weights.  A weight is 2^(score - reference); the reference lies kLift above the largest score when it was last raised, and is raised when a
+// score comes closer than kLeast to it.  So no weight is above 2^-16, and sums of up to 65,536 finite values stay finite as their mean does; the largest weight is
+// 2^-24 at least, and what lies 2^102 below it is 0.
+constexpr float kLift = 24.f, kLeast = 16.f;
 
 struct Params {
   const void* q; void* out; const void* k; const void* v;

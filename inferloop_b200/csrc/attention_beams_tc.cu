@@ -9,8 +9,8 @@
 //   warps 0, 7  issue the boxes of K and of V into rings of 2 tiles each (heads of 64: 4).  (One warp for all three took 4,000 clocks for 128 keys: 850 a turn
 //            of the block tables, 770 and 600 for eight boxes.)
 //   warp 1   allocates tensor memory (two S tiles of 64 columns, O of D) and issues S = Q K^T two tiles ahead and O += P V.
-//   warps 2-5  a thread a row (= tensor-memory lane): masks what its beam does not hold or see, exponentials, P as packed bfloat16 over the
-//            scores; O is rescaled only when a maximum has grown by more than 2^8.  Warps without rows leave at once.
+//   warps 2-5  a thread a row (= tensor-memory lane): masks what its beam does not hold or see, exponentials, P as packed bfloat16 (the operand's type: half a
+//            step, 2^-8, of each weight; the sums that divide are of the unrounded ones) over the scores; O is rescaled only when a maximum has grown by more than 2^8.  Warps without rows leave at once.
 //   split    clusters of S CTAs share a (request, kv head) by strips of 16 keys, as in attention_beams.cu; at the end every CTA leaves O of
 //            its rows in its shared memory, sends their maxima and sums to the rows' owners, and row i is added up by CTA i % S.
 // Two CTAs to an SM: a tile's chain (wait for S, load, exponentials, wait for O: 1,700 clocks) leaves the tensor cores and the memory idle, and a second CTA fills
@@ -45,7 +45,6 @@ constexpr int kInfos = 8;
 constexpr int kMaxSplit = 16;
 constexpr int kThreads = 256, kWarps = 8;
 constexpr int kPad = 8;                // floats between the records of two rows
-constexpr float kRescaleStep = 8.f;    // log2
 
 __device__ __forceinline__ float power_of_two(float x) {
   float y;
@@ -328,8 +327,8 @@ attention_beams_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         for (int c = 0; c < kKeys; ++c) m4[c & 3] = fmaxf(m4[c & 3], v[c]);
         float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         mx = mx == -INFINITY ? -INFINITY : mx * p.scale_log2;
-        const bool grows = mx > m + kRescaleStep;        // (the first key that is seen: from -inf)
-        const float m_new = grows ? mx : m, shift = m_new == -INFINITY ? 0.f : -m_new;
+        const bool grows = mx > m - kLeast;              // (the first key that is seen: from -inf)
+        const float m_new = grows ? mx + kLift : m, shift = m_new == -INFINITY ? 0.f : -m_new;
         float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
         for (int h = 0; h < kKeys / 64; ++h) {           // P over the scores: 64 keys are 32 columns

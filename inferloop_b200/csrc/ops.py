@@ -1556,8 +1556,8 @@ def attention_beams(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v
     """`attention` of a step of single tokens whose rows are beams: rows r * beams .. (r + 1) * beams - 1 (the last request may have fewer) belong to one
     request, and a page that several of their block tables hold is read once for all of them.  q and out are [rows, nq * d] of the cache's
     type, float32 or bfloat16; `window` and `sink` as in `attention`; a token that sees no key (its pages are not held) gets zeros.  A value meets only
-    the rows that see its key, whatever it is.  (`step`: its positions; sequence indices where the exact kernel takes the call; max_kv_len, if
-    it has one, only decides how the keys are split.)"""
+    the rows that see its key, whatever it is, and where shared pages are read once, up to 65,536 finite ones do not overflow on the way to their mean.  (`step`:
+    its positions; sequence indices where the exact kernel takes the call; max_kv_len, if it has one, only decides how the keys are split.)"""
     positions, dtype, index = step.positions, q.dtype, q.get_device()
     if index < 0 or not (_ready(index, dtype, q, out, k_cache, v_cache) and _ready(index, _INT32, block_table, positions)) \
             or (sink is not None and not _ready(index, torch.float32, sink)):
