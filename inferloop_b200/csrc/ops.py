@@ -8,6 +8,8 @@ from __future__ import annotations
 
 import ctypes
 import struct
+import threading
+from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import Optional
 
@@ -1277,6 +1279,7 @@ BEAM_MAX_BEST = 64         # candidates that a request's beams are asked for
 BEAM_MAX_ROWS = 1024       # rows (requests times beams) of a reordering
 BEAM_MAX_GROUPS = 8        # page groups of a reordering or of a step
 _BEAM_SCRATCH: dict = {}   # (device index, stream) -> the scratch of selections there
+_BEAM_SCRATCH_TURN = threading.Lock()      # held from a selection's look at it to the last of its two launches
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, parents: torch.Tensor, tokens: torch.Tensor, out_scores: torch.Tensor,
@@ -1310,14 +1313,17 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, parents: torch.Tenso
         raise KernelError("beam_select: rows of logits overlap")
     code, stream = _code(logits), torch._C._cuda_getCurrentRawStream(index)
     need = rows * -(-(vocab + 7) // 2048) * 32 * 8       # (maximum and sum of every segment of 64 logits, wherever a row begins)
-    # (one scratch per device and stream; a graph that is being recorded gets its own, which its memory pool keeps)
-    held = None if _recording() else _BEAM_SCRATCH.get((index, stream))
-    if held is None or held.numel() < need:
-        held = torch.empty(need, dtype=torch.uint8, device=logits.device)
-        if not _recording():
-            _BEAM_SCRATCH[index, stream] = held
-    _call_on(index, "beam", "ilb_beam_select", logits.data_ptr(), code, stride, scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
-             out_scores.data_ptr(), 0 if bad is None else bad.data_ptr(), R, W, vocab, k, held.data_ptr(), stream)
+    # (one scratch per device and stream; a graph that is being recorded gets its own, which its memory pool keeps.  The foreign call lets other threads
+    # run, and its second launch reads what its first left: another thread's selection on the stream comes before both or behind both)
+    recording = _recording()
+    with nullcontext() if recording else _BEAM_SCRATCH_TURN:
+        held = None if recording else _BEAM_SCRATCH.get((index, stream))
+        if held is None or held.numel() < need:
+            held = torch.empty(need, dtype=torch.uint8, device=logits.device)
+            if not recording:
+                _BEAM_SCRATCH[index, stream] = held
+        _call_on(index, "beam", "ilb_beam_select", logits.data_ptr(), code, stride, scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+                 out_scores.data_ptr(), 0 if bad is None else bad.data_ptr(), R, W, vocab, k, held.data_ptr(), stream)
 
 
 @dataclass
