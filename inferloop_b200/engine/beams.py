@@ -188,7 +188,7 @@ class BeamSearch:
         track = ops.BeamTrack.make(R, W, self.last, device)
         track.tokens = ctx.tokens[:n].view(R, W)              # the tokens that go on are the next step's
         cand = [torch.empty((R, k), dtype=t, device=device) for t in (torch.int32, torch.int32, torch.float32)]
-        bad, any_bad = (torch.zeros(n, dtype=torch.int32, device=device) for _ in range(2))
+        bad, any_bad, alive = (torch.zeros(n, dtype=torch.int32, device=device) for _ in range(3))
         refused = torch.zeros(1, dtype=torch.int32, device=device)
         stops = torch.tensor(self.stops, dtype=torch.int32, device=device) if self.stops else None
         seen, looked = torch.zeros(R, dtype=torch.int32).pin_memory(), None
@@ -203,7 +203,9 @@ class BeamSearch:
                 r_.tokens_run += n
                 ops.scope("beam search")
                 ops.beam_select(rec.logits[:n], track.scores, *cand, bad)
-                any_bad.bitwise_or_(bad)
+                # (a beam that has no tokens keeps its row, whose pages hold anything)
+                torch.gt(track.scores.view(-1), float("-inf"), out=alive)
+                any_bad.addcmul_(bad, alive)
             ops.beam_keep(*cand, stops, track, step, self.last, self.penalty, self.early)
             if step + 1 == self.last:
                 break
