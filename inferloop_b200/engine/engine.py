@@ -380,9 +380,9 @@ class Engine:
         """The best continuations of every prompt that a search with `beams` beams finds: for each prompt a list of `BeamHypothesis`, best first (as many
         as beams, or fewer where the vocabulary or the length has no more).  A hypothesis is finished by a token of `eos_tokens` (None: the
         model's stop tokens) or by its length, and ranked by the sum of its log probabilities / (tokens ^ length_penalty).  A
-        request's search ends when as many have finished as it has beams and its best beam's score over its length so far is no
-        better than the worst of them, or, with `early_stopping`, as soon as they have finished.  Requests that are already being served
-        keep their pages; the search runs on what is free."""
+        request's search ends when as many have finished as it has beams and the score of the step's best continuation (one that a stop token has
+        just ended counts too) over its length is no better than the worst of them, or, with `early_stopping`, as soon as they have
+        finished.  Requests that are already being served keep their pages; the search runs on what is free."""
         from .beams import BeamSearch
         defaults = self.generation_defaults.base
         if eos_tokens is None:

@@ -27,3 +27,23 @@ def test_more_beams_than_tokens(tmp_path, beams, vocab):
     else:
         compare(engine, (9, 16, 21), beams, 5)
     assert all(torch.isfinite(torch.tensor([h.score for h in x])).all() for x in engine.beam_search([[0] * 3, [0] * 20], beams, 4, eos_tokens=[]))
+
+
+def test_the_best_continuation_decides_whether_a_search_ends():
+    """Two beams.  Once two have finished the search goes on while the step's best continuation is better than the worst of them, also where a stop token ends
+    just that continuation and the best beam is worse than both."""
+    from inferloop_b200.csrc import ops
+    dev = "cuda:0"
+    i32 = lambda x: torch.tensor([x], dtype=torch.int32, device=dev)  # noqa: E731
+    stops = torch.tensor([7], dtype=torch.int32, device=dev)
+
+    def keep(track, step, tokens, scores):
+        ops.beam_keep(i32([0, 0, 1, 1]), i32(tokens), torch.tensor([scores], device=dev), stops, track, step, 9, 0.0, False)
+        return int(track.done), track.done_scores[0].tolist(), track.scores[0].tolist()
+    a = ops.BeamTrack.make(1, 2, 9, dev)
+    assert keep(a, 0, [1, 7, 2, 3], [-2.0, -3.0, -4.0, -5.0]) == (0, [-3.0, float("-inf")], [-2.0, -4.0])
+    assert keep(a, 1, [7, 1, 2, 3], [-2.5, -3.5, -4.0, -5.0]) == (0, [-2.5, -3.0], [-3.5, -4.0])
+    assert keep(a, 2, [1, 7, 2, 3], [-4.0, -4.5, -5.0, -6.0]) == (1, [-2.5, -3.0], [-4.0, -5.0])
+    b = ops.BeamTrack.make(1, 2, 9, dev)
+    assert keep(b, 0, [7, 1, 2, 3], [-1.0, -2.0, -3.0, -4.0]) == (0, [-1.0, float("-inf")], [-2.0, -3.0])
+    assert keep(b, 1, [7, 1, 2, 3], [-2.5, -3.5, -4.0, -5.0]) == (1, [-1.0, -2.5], [-3.5, -4.0])      # (no better than the worst, which it is)
