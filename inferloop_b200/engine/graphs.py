@@ -33,6 +33,7 @@ from ..csrc import ops
 from .batch import Drawn, StepContext, StepEntry, StepStager
 
 BUCKETS = (1, 2, 4, 8, 16, 24, 32, 48, 64, 96, 128, 192, 256)
+BEAM_STEPS_KEPT = 16       # recorded steps of beams: there is one for every (rows, beams, longest context in eighths of a power of two) that is searched
 
 
 def bucket_for(n: int) -> Optional[int]:
@@ -316,8 +317,10 @@ class DecodeGraphs:
             del self._recorded[key]
             rec = None
         if rec is not None:
+            self._recorded[key] = self._recorded.pop(key)            # (the last in turn is the latest used)
             rec.ctx.position_tables.clear()
             return key, rec, rec.ctx, rec.ints
+        self._let_go_of_beam_steps(BEAM_STEPS_KEPT - 1)
         shapes = self._shapes(bucket)
         ints = torch.zeros(StepStager.layout(shapes), dtype=torch.int32, device=self.runner.device)
         views, at = [], 0
@@ -333,6 +336,18 @@ class DecodeGraphs:
                           h_q_start=[0] * rows, h_q_len=[1] * rows, h_kv_len=[longest] * rows, h_slots=[0] * rows, max_q_len=1, max_kv_len=longest,
                           decode_only=True, beams=beams)
         return key, None, ctx, ints
+
+    def _let_go_of_beam_steps(self, keep: int) -> None:
+        """Keep the `keep` latest used of the recorded steps of beams, and none whose scratch has moved: each holds a graph and its arrays on the device."""
+        kept = [k for k in self._recorded if k[0] == "beams"]
+        current = self.runner.ctx.workspace.generation
+        gone = [k for k in kept if self._recorded[k].workspace_generation != current]
+        kept = [k for k in kept if k not in gone]
+        gone += kept[:max(len(kept) - keep, 0)]
+        if gone:
+            torch.cuda.current_stream(self.runner.device).synchronize()       # (a replay may still be on its way)
+            for k in gone:
+                del self._recorded[k]
 
     def run_beams(self, key: tuple, rec: Optional[_Recorded], ctx: StepContext, ints: torch.Tensor) -> _Recorded:
         """Run a step of `beam_step` on the arrays as they are: replayed, or the first time kernel by kernel and recorded."""
