@@ -149,6 +149,14 @@ def _ready(index: int, dtype: torch.dtype, *tensors) -> bool:
     return True
 
 
+def _apart(what: str, *places) -> None:
+    """Raise where two of the places (address, bytes) that a call writes have bytes in common."""
+    places = sorted(places)
+    for (a, n), (b, _) in zip(places, places[1:]):
+        if b < a + n:
+            raise KernelError(f"{what} share memory")
+
+
 def _i(v) -> ctypes.c_int:
     return ctypes.c_int(int(v))
 
@@ -1451,7 +1459,7 @@ def beam_reorder(state: BeamState, parents: torch.Tensor, kv_len: torch.Tensor, 
     request's beams all have, and `slots` [R * W] (the rows' state slots) with them.  Full pages are shared from there on.  A page that is not full is
     a row's own, as its slot is: a parent's first child takes those over, every other child takes the ones of a beam without children, in the order
     of both, and the parent's rows and state are copied there.  Before the call the last, partly filled pages of a request's rows and
-    their slots must be different ones."""
+    their slots must be different ones; groups have a table each."""
     index, tables = state.index, list(tables)
     if not _ready(index, _INT32, parents, kv_len, *tables) or (slots is not None and not _ready(index, _INT32, slots)):
         for t, w in ((parents, "parents"), (kv_len, "lengths"), (slots, "slots"), *((t, "block table") for t in tables)):
@@ -1470,6 +1478,8 @@ def beam_reorder(state: BeamState, parents: torch.Tensor, kv_len: torch.Tensor, 
             raise KernelError(f"beam_reorder: a block table {tuple(shape)} for {rows} rows")
         where.append(t.data_ptr())
         sizes += (shape[1], page_size, stride, pages)
+    if n > 1:
+        _apart("beam_reorder: two groups' block tables", *((a, 4 * rows * w) for a, w in zip(where, sizes[::4])))
     if kv_len.numel() != rows or (slots is not None and slots.numel() != rows) or (slots is None and state.num_slots is not None):
         raise KernelError("beam_reorder: lengths or slots do not match the rows")
     if not 0 < W <= BEAM_MAX or rows > BEAM_MAX_ROWS:
@@ -1501,7 +1511,7 @@ def step_build(new: torch.Tensor, cached: torch.Tensor, kv_len: torch.Tensor, po
     rows need, taken from the front of the free list in the order of sequences and blocks and entered in the block tables.  `slot_map` [T] int64: each
     token's row among all rows of the first group's pages (page * page size + place; -1 where no page is held).  All or nothing: where
     a length is negative or too long, tokens, pages or columns do not suffice, nothing is written but a bit in `refused` [1] (1 tokens, 2 pages,
-    4 columns, 8 lengths).  Entries behind the last token stay as they are."""
+    4 columns, 8 lengths).  Entries behind the last token stay as they are.  Groups have a table and a count of taken pages each."""
     index = new.get_device()
     if index < 0 or not _ready(index, _INT32, new, cached, kv_len, positions, seq_of_token, cu_q, refused) \
             or (slot_map is not None and not _ready(index, torch.int64, slot_map)):
@@ -1527,6 +1537,11 @@ def step_build(new: torch.Tensor, cached: torch.Tensor, kv_len: torch.Tensor, po
                 or g.stride <= 0:
             raise KernelError("step_build: a page group's arrays do not agree")
         held += [g.table.data_ptr(), g.free.data_ptr(), g.used.data_ptr(), out.data_ptr(), g.table.shape[1], g.free.numel(), g.page_size, g.stride]
+    if len(pages) > 1:
+        _apart("step_build: two page groups' block tables", *((a, 4 * S * w) for a, w in zip(held[::8], held[4::8])))
+        for i, out in enumerate(held[3::8]):
+            if any(out in (held[8 * j + 2], held[8 * j + 3]) for j in range(len(pages)) if j != i):
+                raise KernelError("step_build: two page groups count the pages that they take in one place")
     if S == 0:
         return
     held = (ctypes.c_longlong * max(len(held), 1))(*held)
