@@ -7,6 +7,7 @@ a library that cannot be built or loaded, raises.
 from __future__ import annotations
 
 import ctypes
+import math
 import struct
 import threading
 from contextlib import nullcontext
@@ -1286,6 +1287,7 @@ BEAM_MAX = 32              # beams of a request
 BEAM_MAX_BEST = 64         # candidates that a request's beams are asked for
 BEAM_MAX_ROWS = 1024       # rows (requests times beams) of a reordering
 BEAM_MAX_GROUPS = 8        # page groups of a reordering or of a step
+BEAM_MAX_POWER = 100.0     # log2 of tokens ^ length penalty (or its inverse): beyond, scores over it are no normal numbers of 32 bits
 _BEAM_SCRATCH: dict = {}   # (device index, stream) -> the scratch of selections there
 _BEAM_SCRATCH_TURN = threading.Lock()      # held from a selection's look at it to the last of its two launches
 
@@ -1362,6 +1364,12 @@ class BeamTrack:
                          torch.zeros(requests, dtype=torch.int32, device=device), torch.zeros(requests, dtype=torch.int32, device=device))
 
 
+def beam_penalty_served(length_penalty: float, last: int) -> bool:
+    """Whether scores over up to `last` tokens ^ length_penalty can be told apart in 32 bits."""
+    most = abs(float(length_penalty))
+    return most <= 3e38 and most * math.log2(max(int(last), 1)) <= BEAM_MAX_POWER
+
+
 def beam_keep(parents: torch.Tensor, tokens: torch.Tensor, scores: torch.Tensor, stops: Optional[torch.Tensor], track: BeamTrack, step: int,
               last: int, length_penalty: float = 1.0, early_stopping: bool = False) -> None:
     """Candidates of `beam_select` [R, k] -> the beams that go on (`track.scores`, `parents`, `tokens` and row `step` of the past) and the finished
@@ -1383,6 +1391,8 @@ def beam_keep(parents: torch.Tensor, tokens: torch.Tensor, scores: torch.Tensor,
         raise KernelError("beam_keep: candidates and what is kept do not agree")
     if not (0 <= step < min(int(last), steps)) or not 0 < W <= BEAM_MAX or not 0 < k <= BEAM_MAX_BEST:
         raise KernelError(f"beam_keep: step {step} of {last}, {steps} kept, {W} beams, {k} candidates")
+    if not beam_penalty_served(length_penalty, last):
+        raise KernelError(f"beam_keep: {last} tokens to the power of {length_penalty} (up to 2 ^ {BEAM_MAX_POWER:g}, or its inverse)")
     _same_device("beam_keep", parents, tokens, scores, stops, track.scores, track.parents, track.tokens, track.past_parents, track.past_tokens,
                  track.done_scores, track.done_steps, track.done_parents, track.done_tokens, track.done_count, track.done)
     index = parents.get_device()

@@ -55,6 +55,8 @@ class BeamSearch:
             raise ValueError("max_new_tokens must be positive")
         if not np.isfinite(self.penalty):
             raise ValueError("the length penalty must be a number")
+        if not ops.beam_penalty_served(self.penalty, self.last):
+            raise ValueError(f"{self.last} tokens to the power of {self.penalty}: up to 2 ^ {ops.BEAM_MAX_POWER:g}, or its inverse, is served")
         if graphs is None or not graphs.whole or self.runner.spec.token_extras:
             raise ValueError("beam search needs a model whose whole step is recorded as one graph and that takes no inputs per token beside ids "
                              "and positions")

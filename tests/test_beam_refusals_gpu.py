@@ -42,3 +42,18 @@ def test_one_count_of_pages_for_two_groups(ops):
         with pytest.raises(ops.KernelError, match="in one place"):
             ops.step_build(a, a, a, z(4), z(4), z(5), pages, z(1))
     ops.step_build(a, a, a, z(4), z(4), z(5), [page(one, two), page(one, z(1))], z(1))         # (the same number read twice)
+
+
+@pytest.mark.parametrize("last,penalty,served", [(2, 100.0, True), (2, -100.0, True), (2, 101.0, False), (16, 25.5, False), (16, -25.5, False), (4, float("nan"), False),
+                                                 (4, float("inf"), False), (1, 1e30, True), (1, float("nan"), False), (1, 1e300, False), (3, 1e300, False)])
+def test_length_penalties(ops, last, penalty, served):
+    """A power that 32 bits do not hold made all scores zero, infinite or NaN."""
+    track = ops.BeamTrack.make(1, 2, last, DEV)
+    args = (z(1, 2), torch.tensor([[1, 2]], dtype=torch.int32, device=DEV), torch.tensor([[-1.0, -1.5]], device=DEV), None, track, last - 1, last, penalty)
+    if not served:
+        with pytest.raises(ops.KernelError, match="power"):
+            ops.beam_keep(*args)
+        return
+    ops.beam_keep(*args)
+    want = torch.tensor([-1.0, -1.5], dtype=torch.float64) / float(last) ** penalty
+    assert bool(((track.done_scores[0].cpu().double() - want).abs() <= 2.0 ** -21 * want.abs()).all())
