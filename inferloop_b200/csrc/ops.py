@@ -1430,7 +1430,7 @@ class BeamState:
                 unit, row = page_size // x.shape[-2], x.shape[-1] * x.element_size()
                 part, heads = x.shape[-2] * row, x.shape[-3]
                 outer = x.numel() // max(pages * heads * x.shape[-2] * x.shape[-1], 1)
-                if x.numel() == 0 or unit * row >= 1 << 31:
+                if x.numel() == 0 or part > (1 << 31) - 4096:       # (a copy counts its bytes, and a step beyond them, in 32 bits)
                     raise KernelError(f"beam state: storage of shape {tuple(x.shape)} is empty or its rows too long")
                 records.append(struct.pack("@Pqqqqiiiiii", x.data_ptr(), pages * heads * part, heads * part, part, part, outer, heads, g, unit, row, 0))
                 first.append(at)

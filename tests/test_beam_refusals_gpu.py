@@ -57,3 +57,16 @@ def test_length_penalties(ops, last, penalty, served):
     ops.beam_keep(*args)
     want = torch.tensor([-1.0, -1.5], dtype=torch.float64) / float(last) ** penalty
     assert bool(((track.done_scores[0].cpu().double() - want).abs() <= 2.0 ** -21 * want.abs()).all())
+
+
+def test_heads_of_a_page_of_two_gigabytes(ops):
+    """A copy counts the bytes of a page's head in 32 bits: just below 2^31 it moves them, at 2^31 the storage is refused."""
+    rows = 1 << 16
+    with pytest.raises(ops.KernelError, match="too long"):
+        ops.BeamState([([torch.empty((2, 1, rows, 1 << 15), dtype=torch.uint8, device=DEV)], rows, 1)])
+    x = torch.zeros((2, 1, rows, (1 << 15) - 16), dtype=torch.uint8, device=DEV)
+    x[0, 0, :, -1] = torch.arange(rows, device=DEV).to(torch.uint8)
+    table = torch.tensor([[0], [1]], dtype=torch.int32, device=DEV)
+    state = ops.BeamState([([x], rows, 1)])
+    ops.beam_reorder(state, z(1, 2), torch.full((2,), rows - 1, dtype=torch.int32, device=DEV), [table])
+    assert torch.equal(x[1, 0, :-1], x[0, 0, :-1]) and int(x[1, 0, -1].sum()) == 0
