@@ -969,7 +969,6 @@ ILB_EXPORT int ilb_step_build(const int* fresh, const int* cached, int* kv_len, 
                               int* refused, int n_seqs, int room, const long long* pages, int n_groups, cudaStream_t stream) {
   ILB_REQUIRE(n_seqs >= 0 && n_seqs <= kMaxSequences && room >= 0 && room <= kMaxTokens && n_groups >= 0 && n_groups <= kMaxGroups,
               "step_build: bad sizes (up to %d sequences, %d tokens and %d page groups)", kMaxSequences, kMaxTokens, kMaxGroups);
-  if (n_seqs == 0) return 0;
   Build p{fresh, cached, kv_len, positions, seq_of_token, cu_q, slot_map, refused, n_seqs, room, n_groups, 1};
   auto shift_of = [](int x) { int n = 0; while ((1 << n) < x) ++n; return (1 << n) == x ? n : -1; };
   for (int g = 0; g < n_groups; ++g) {

@@ -1546,14 +1546,12 @@ def step_build(new: torch.Tensor, cached: torch.Tensor, kv_len: torch.Tensor, po
         if g.table.dim() != 2 or g.table.shape[0] != S or (g.table.shape[1] == 0 and S) or g.used.numel() != 1 or out.numel() != 1 or g.page_size <= 0 \
                 or g.stride <= 0:
             raise KernelError("step_build: a page group's arrays do not agree")
-        held += [g.table.data_ptr(), g.free.data_ptr(), g.used.data_ptr(), out.data_ptr(), g.table.shape[1], g.free.numel(), g.page_size, g.stride]
+        held += [g.table.data_ptr(), g.free.data_ptr(), g.used.data_ptr(), out.data_ptr(), max(g.table.shape[1], 1), g.free.numel(), g.page_size, g.stride]
     if len(pages) > 1:
         _apart("step_build: two page groups' block tables", *((a, 4 * S * w) for a, w in zip(held[::8], held[4::8])))
         for i, out in enumerate(held[3::8]):
             if any(out in (held[8 * j + 2], held[8 * j + 3]) for j in range(len(pages)) if j != i):
                 raise KernelError("step_build: two page groups count the pages that they take in one place")
-    if S == 0:
-        return
     held = (ctypes.c_longlong * max(len(held), 1))(*held)
     _call_on(index, "beam", "ilb_step_build", new.data_ptr(), cached.data_ptr(), kv_len.data_ptr(), positions.data_ptr(), seq_of_token.data_ptr(),
              cu_q.data_ptr(), 0 if slot_map is None else slot_map.data_ptr(), refused.data_ptr(), S, T, ctypes.addressof(held), len(pages),
