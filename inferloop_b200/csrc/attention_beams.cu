@@ -537,7 +537,7 @@ attention_beams_kernel(Params p) {
 }
 
 // ------------------------------------------------------------------ float32
-// Bound: latency where keys are few (3 x 4 beams of 700 keys, window 500, 11.0 us: positions, tables, units, the cluster's barriers), else fused multiply-adds and
+// Bound: latency where keys are few (3 x 4 beams of 700 keys, window 500, 9.9 us: positions, tables, units, the cluster's barriers), else fused multiply-adds and
 // the loads from shared memory that feed them (8 x 4 of 1,240 keys 63 us, 20 times its bytes' time; a kernel that reads each beam's own takes 877).
 constexpr int kExactTile = 2;          // units: a key a lane
 constexpr int kWarps = 8, kThreads = 32 * kWarps;

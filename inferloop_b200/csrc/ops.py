@@ -1571,6 +1571,8 @@ BEAMS_TC_ROWS, BEAMS_TC_FEW, BEAMS_TC_KEYS = 33, 17, 90_000
 # of 640 keys (10 MB) 7.6 / 10.3, 4 x 4 of 2,040 (134 MB) 12.5 / 23.3, 1 x 4 of 140 (2 MB) 8.0 / 6.7; 2 kv heads of 8 query heads, 4 x 4 of 640 (10 MB)
 # 9.0 / 9.0, 1 x 4 of 2,040 (8 MB) 9.6 / 8.7, 16 x 4 of 640 (42 MB) 10.3 / 10.6, but 8 x 8 of 340 (22 MB, 64 rows) 16.6 / 8.5.  In 32 bits no kernel of
 # single tokens splits a sequence, and 1 x 4 of 640 take 10.8 / 209.
+# Bytes alone do not tell these cases apart: by this border 4 x 4 of 2,030 with groups of 2 and 4 and, beside attention_decode_tma, 8 x 8 of 340 share pages and
+# lose by it, as 16 kv heads of 500 keys with 128 rows lose 3 us by the border of rows above.
 BEAMS_SHARE_BYTES = 120_000_000
 
 
