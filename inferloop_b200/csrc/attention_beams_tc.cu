@@ -10,7 +10,8 @@
 //            of the block tables, 770 and 600 for eight boxes.)
 //   warp 1   allocates tensor memory (two S tiles of 64 columns, O of D) and issues S = Q K^T two tiles ahead and O += P V.
 //   warps 2-5  a thread a row (= tensor-memory lane): masks what its beam does not hold or see, exponentials, P as packed bfloat16 (the operand's type: half a
-//            step, 2^-8, of each weight; the sums that divide are of the unrounded ones) over the scores; O is rescaled only when a maximum has grown by more than 2^8.  Warps without rows leave at once.
+//            step, 2^-8, of each weight; the sums that divide are of the unrounded ones) over the scores; O is rescaled only when a maximum has grown by more
+//            than 2^8.  Warps without rows leave at once.
 //   split    clusters of S CTAs share a (request, kv head) by strips of 16 keys, as in attention_beams.cu; at the end every CTA leaves O of
 //            its rows in its shared memory, sends their maxima and sums to the rows' owners, and row i is added up by CTA i % S.
 // Two CTAs to an SM: a tile's chain (wait for S, load, exponentials, wait for O: 1,700 clocks) leaves the tensor cores and the memory idle, and a second CTA fills
